@@ -105,6 +105,16 @@ _SIGS = {
     "hyq_attention_kv16": ([_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _i64, _vp, _i64, _vp, _vp, _vp], C.c_int),
     "hyq_attention_seqs_kv16": ([_vp, _vp, _vp, C.c_int, C.c_int, C.c_int, _i64, _vp, _i64, _i64, _vp, _vp, _vp],
                                 C.c_int),
+    "hyq_paged_rope_append": ([_vp, _vp, _vp, _i64, C.c_int, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, C.c_float,
+                               C.c_int, _vp, _i64, _vp], C.c_int),
+    "hyq_paged_attention_workspace_bytes": ([C.c_int, C.c_int, C.POINTER(C.c_size_t)], C.c_int),
+    "hyq_paged_attention": ([_vp, _vp, _vp, _i64, C.c_int, _vp, _i64, _vp, _vp], C.c_int),
+    "hyq_pages_workspace_bytes": ([_i64, C.POINTER(C.c_size_t)], C.c_int),
+    "hyq_pages_reserve": ([_vp, _vp, _vp, _i64, _vp, _vp, _vp], C.c_int),
+    "hyq_pages_free": ([_vp, _vp, _i64, _vp], C.c_int),
+    "hyq_pages_fork": ([_vp, _vp, _vp, _vp, _i64, _vp, _vp], C.c_int),
+    "hyq_pages_compact": ([_vp, _vp, _vp, _vp], C.c_int),
+    "hyq_sample": ([_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], C.c_int),
     "hyq_gguf_open": ([C.c_char_p, C.c_int, C.POINTER(C.c_void_p)], C.c_int),
     "hyq_gguf_close": ([_vp], None),
     "hyq_gguf_profile": ([_vp], C.c_int),

@@ -1,0 +1,80 @@
+// Device view of a paged KV cache and of a batch of new tokens, shared by the
+// append and attention kernels over it.
+#pragma once
+
+#include <cuda_fp16.h>
+#include <cuda_runtime.h>
+
+#include <cstdint>
+
+#include "hyq_common.cuh"
+
+namespace hyq {
+namespace paged {
+
+constexpr int kMaxDim = 256;
+constexpr int kMaxGroup = 16;  // query heads per kv head
+
+// hyq_paged_kv + hyq_paged_batch (include/hyq.h), as the kernels take them.
+struct Cache {
+  void* k;
+  void* v;
+  int kv_heads, dim, page_size;
+  int pages;
+  int64_t page_stride, head_stride, row_stride;  // elements
+  const int32_t* table;                          // [slots, width]
+  int slots, width;
+  const int32_t* slot;       // [seqs] or null
+  const int32_t* row_start;  // [seqs + 1]
+  const int32_t* pos;        // [seqs]
+  int seqs, tokens;
+  unsigned* status;
+};
+
+// One sequence's new tokens.
+struct Seq {
+  int row0;             // first row of the activations
+  int n;                // new tokens (0: none, or a bad sequence)
+  int pos;              // position of the first one
+  const int32_t* pages; // its table row
+};
+
+// Sequence s, checked: rows inside the activations, positions inside the
+// table row.  A bad one comes back empty and raises DEV_BAD_ARGS.
+__device__ __forceinline__ Seq load_seq(const Cache& c, int s) {
+  Seq q;
+  q.row0 = c.row_start[s];
+  const int end = c.row_start[s + 1];
+  q.pos = c.pos[s];
+  const int slot = c.slot ? c.slot[s] : s;
+  q.n = end - q.row0;
+  const bool ok = q.row0 >= 0 && q.n >= 0 && end <= c.tokens && q.pos >= 0 && slot >= 0 && slot < c.slots &&
+                  (int64_t)q.pos + q.n <= (int64_t)c.width * c.page_size;
+  if (!ok) {
+    atomicOr(c.status, DEV_BAD_ARGS);
+    q.n = 0;
+  }
+  q.pages = c.table + (ok ? (int64_t)slot * c.width : 0);
+  return q;
+}
+
+// The sequence that row t belongs to (row_start ascending), or -1.
+__device__ __forceinline__ int seq_of_row(const Cache& c, int t) {
+  int lo = 0, hi = c.seqs;  // the last s with row_start[s] <= t
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (c.row_start[mid] <= t) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo < c.seqs && c.row_start[lo] <= t ? lo : -1;
+}
+
+// Page of a table entry, or -1 with DEV_BAD_ARGS when it is no page of the pool.
+__device__ __forceinline__ int checked_page(const Cache& c, int page) {
+  if (page >= 0 && page < c.pages) return page;
+  atomicOr(c.status, DEV_BAD_ARGS);
+  return -1;
+}
+
+}  // namespace paged
+}  // namespace hyq

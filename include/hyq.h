@@ -426,6 +426,139 @@ int hyq_add_rms_norm(float* hidden, const float* delta, const float* w, int64_t 
 int hyq_argmax(const float* x, int64_t n, int32_t* token, int32_t* pos, int pos_step, void* workspace,
                void* stream);
 
+/* --- Paged KV cache --------------------------------------------------------
+ * No counterpart in the reference, whose Session keeps one contiguous f32
+ * cache (model.rs:116-120, KvCache::append model.rs:650-667).  A layer's keys
+ * and values live in pools of pages of `page_size` positions; a sequence is a
+ * row of the page table: entry j names the page that holds its positions
+ * j * page_size .. (j + 1) * page_size - 1.  The same table serves every
+ * layer.  All indexes are device int32, so that a step can be captured in a
+ * CUDA graph and replayed while the sequences grow.
+ *
+ * hyq_paged_kv: one layer's pools.  Value (page, kv head, row, d) is at
+ *   page * page_stride + head * head_stride + row * row_stride + d elements
+ *   of k and of v (so [pages, kv_heads, page_size, head_dim] and [pages,
+ *   page_size, kv_heads, head_dim] are both described by their strides).
+ *   dtype HYQ_KV_F32 or HYQ_KV_F16 (IEEE binary16).
+ * hyq_paged_batch: the new tokens of a call.  Rows row_start[s] ..
+ *   row_start[s + 1] - 1 of the activations are the new tokens of sequence s
+ *   (none is allowed), at positions pos[s], pos[s] + 1, ...; its table row is
+ *   slot[s], or s when slot is NULL.  `tokens` is the number of rows of the
+ *   activations (rows outside every sequence are left alone), max_new bounds
+ *   any sequence's new tokens and max_len any pos[s] + new tokens.
+ * A sequence whose table row, pages or positions are out of range is skipped
+ * and raises HYQ_DEV_BAD_ARGS (see hyq_device_status). */
+#define HYQ_KV_F32 0
+#define HYQ_KV_F16 1
+
+typedef struct hyq_paged_kv {
+  void *k, *v;
+  int dtype, kv_heads, head_dim, page_size;
+  int64_t pages, page_stride, head_stride, row_stride; /* strides in elements */
+  const int32_t* table;                                /* [slots, table_width] */
+  int64_t slots, table_width;
+} hyq_paged_kv;
+
+typedef struct hyq_paged_batch {
+  const int32_t *slot, *row_start, *pos; /* [seqs] or NULL, [seqs + 1], [seqs] */
+  int64_t seqs, tokens, max_new, max_len;
+} hyq_paged_batch;
+
+/* RoPE and the per-head RMSNorm of the new tokens' queries and keys
+ * (rope_with_cache model.rs:874-913, the q/k norm model.rs:425-446; norm_first
+ * as hyq_rope_qk), and the append of keys and values to the pages, in one
+ * launch.  q [tokens, heads, head_dim], k and v [tokens, kv_heads, head_dim]
+ * with rows q_stride, k_stride and v_stride floats apart (so the three may be
+ * columns of one product); the rotated queries go to q_out (rows out_stride
+ * apart; q itself is allowed), k and v are left unchanged.  Norm weights may
+ * be NULL.  Same arithmetic as hyq_rope_qk, bit for bit.  head_dim is even
+ * and at most 256; positions at or past `positions` (the rows of the rotary
+ * tables) are refused like positions past the table. */
+int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                          int heads, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                          const float* cos_tab, const float* sin_tab, int64_t positions, const float* q_norm,
+                          const float* k_norm, float eps, int norm_first, float* q_out, int64_t out_stride,
+                          void* stream);
+
+/* Causal grouped-query attention of the new tokens over the pages
+ * (attention_into, model.rs:949-1021): the token at position p of sequence s
+ * sees the sequence's positions 0 ..= p, whose keys and values must be in the
+ * pages already.  out [tokens, heads, head_dim], rows out_stride floats apart.
+ * f32 accuracy over either cache type.  Values past a token's position (page
+ * tails, later tokens of its chunk) never reach its output, whatever they
+ * hold.  head_dim at most 256, at most 16 query heads per kv head.
+ * workspace: hyq_paged_attention_workspace_bytes bytes (independent of the
+ * batch), 16-byte aligned, zero before the first call (every call leaves its
+ * counters zero again); calls that share one must not overlap in time. */
+int hyq_paged_attention_workspace_bytes(int heads, int head_dim, size_t* bytes);
+int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                        int heads, float* out, int64_t out_stride, void* workspace, void* stream);
+
+/* --- Pages of a cache: reserve, free, fork, compact ------------------------
+ * Device-side bookkeeping of the table above, and the page copies it needs
+ * (no counterpart in the reference).  hyq_pages: the table [slots,
+ * table_width] (unused entries -1), length [slots] (positions held), refs
+ * [pages] (sequences that hold a page; 0: free) and `shortage` (one int).
+ * hyq_page_pool: the memory a page copy moves: plane i (e.g. one layer's keys
+ * or values) holds page p at base + i * plane_stride + p * page_stride,
+ * page_bytes long (all in bytes; multiples of 16, base 16-byte aligned).
+ * Slots are device int32 and must be distinct within a call, at most 1024 per
+ * call.  New pages are the lowest-numbered free ones, in the order of the
+ * call, so every result is reproducible.
+ *   reserve  sequence slot[i] grows by extra[i] positions; pos[i] (may be
+ *            NULL) receives its length before.
+ *   free     gives the sequence's pages back; its length becomes 0.
+ *   fork     sequence dst[i] becomes a copy of src[i]: full pages are shared
+ *            (refs + 1), the partial last page is copied to a page of its own.
+ *            dst's old pages are given back first; no dst may be a src.
+ *   compact  moves the live pages numbered past the live count into the free
+ *            pages below it, in ascending order, and renames them in the
+ *            table: afterwards the live pages are 0 .. live - 1.
+ * When reserve or fork would need more pages than are free, nothing grows
+ * (fork: the dsts end up empty) and *shortage receives the number missing;
+ * otherwise it receives 0.  A bad slot, an overlong table row or a repeated
+ * slot leaves everything as it was and raises HYQ_DEV_BAD_ARGS.
+ * workspace: hyq_pages_workspace_bytes bytes, 16-byte aligned, no initial
+ * value needed. */
+typedef struct hyq_pages {
+  int32_t *table, *length, *refs, *shortage;
+  int64_t slots, table_width, pages;
+  int page_size;
+} hyq_pages;
+
+typedef struct hyq_page_pool {
+  void* base;
+  int64_t planes, plane_stride, page_stride, page_bytes;
+} hyq_page_pool;
+
+int hyq_pages_workspace_bytes(int64_t pages, size_t* bytes);
+int hyq_pages_reserve(const hyq_pages* p, const int32_t* slot, const int32_t* extra, int64_t n, int32_t* pos,
+                      void* workspace, void* stream);
+int hyq_pages_free(const hyq_pages* p, const int32_t* slot, int64_t n, void* stream);
+int hyq_pages_fork(const hyq_pages* p, const hyq_page_pool* pool, const int32_t* src, const int32_t* dst, int64_t n,
+                   void* workspace, void* stream);
+int hyq_pages_compact(const hyq_pages* p, const hyq_page_pool* pool, void* workspace, void* stream);
+
+/* --- Sampling (Sampler, generation.rs: temperature, top-k, top-p) ----------
+ * One token of each of `rows` rows of n logits (rows `stride` floats apart)
+ * from given uniform numbers u [rows] in [0, 1).  Per row: temperature (<= 0:
+ * greedy, the first index of the largest logit), top_k (<= 0: off), top_p
+ * (>= 1: off) and min_p (<= 0: off), each a device array of `rows` values or
+ * NULL (temperature 1, filters off).  With m the largest logit and
+ *   w_i = floor(2^40 * exp((l_i - m) * (1 / temperature)))
+ * the tokens in descending order of logit, ties by index, are cut to the
+ * first top_k, then to those whose predecessors weigh less than top_p times
+ * the rest's total, then to those with exp(..) >= min_p; the token is the
+ * first index at which the kept weights, summed in index order, exceed u times
+ * their total.  Weights and sums are whole numbers and u and top_p count in
+ * steps of 2^-24, so the token does not depend on the order of summation.
+ * prob (may be NULL): the token's share of the kept weights.  NaN logits
+ * count as -inf; a row without a logit above -inf gives token 0, prob 0;
+ * logits of +inf share the whole weight. */
+int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, const float* temperature,
+               const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
+               float* prob, void* stream);
+
 /* --- GGUF v3 model files (gguf.rs:50-210) --------------------------------
  * hyq_gguf_open maps the file read-only and checks it as the reference does
  * (header bounds, metadata types, alignment, tensor table, Tencent legacy
