@@ -100,15 +100,6 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 // Attention
 // ---------------------------------------------------------------------------
 
-struct AttendArgs {
-  Cache c;
-  const float* q;
-  int64_t q_stride;
-  int heads;
-  float* out;
-  int64_t out_stride;
-};
-
 template <bool KV16>
 __device__ __forceinline__ float load_kv(const void* base, int64_t i) {
   if constexpr (KV16) return __half2float(static_cast<const __half*>(base)[i]);
@@ -253,7 +244,7 @@ int make_cache(const hyq_paged_kv* kv, const hyq_paged_batch* b, int heads, cons
                     hyq::paged::kMaxDim, hyq::paged::kMaxGroup);
   if (kv->row_stride < kv->head_dim || kv->head_stride < kv->head_dim || kv->page_stride < kv->head_dim)
     return api_fail(HYQ_E_SHAPE, "%s: strides of the cache overlap", name);
-  if (b->seqs < 0 || b->seqs > INT32_MAX || b->tokens < 0 || b->tokens > INT32_MAX || b->max_new < 0 ||
+  if (b->seqs < 0 || b->seqs > hyq::paged::kMaxSeqs || b->tokens < 0 || b->tokens > INT32_MAX || b->max_new < 0 ||
       b->max_len < b->max_new || b->max_len > kv->table_width * kv->page_size)
     return api_fail(HYQ_E_SHAPE, "%s: shape of the batch", name);
   if (!b->slot && b->seqs > kv->slots)
@@ -334,7 +325,7 @@ int hyq_paged_attention_workspace_bytes(int heads, int head_dim, size_t* bytes) 
   if (!bytes) return api_fail(HYQ_E_INVALID, "paged_attention_workspace_bytes: null pointer");
   if (heads <= 0 || head_dim <= 0 || head_dim > hyq::paged::kMaxDim)
     return api_fail(HYQ_E_SHAPE, "paged_attention_workspace_bytes: shape");
-  *bytes = 16;
+  *bytes = hyq::paged::mma_workspace_bytes(head_dim);
   return HYQ_OK;
 }
 
@@ -355,9 +346,11 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
   a.heads = heads;
   a.out = out;
   a.out_stride = out_stride;
+  a.ws = workspace;
   const cudaStream_t st = (cudaStream_t)stream;
-  return done(kv->dtype == HYQ_KV_F16 ? hyq::paged::launch_attend<true>(a, st) : hyq::paged::launch_attend<false>(a, st),
-              name);
+  const bool kv16 = kv->dtype == HYQ_KV_F16;
+  if (hyq::paged::mma_supported(a, kv16)) return done(hyq::paged::launch_mma(a, kv16, batch->max_new, st), name);
+  return done(kv16 ? hyq::paged::launch_attend<true>(a, st) : hyq::paged::launch_attend<false>(a, st), name);
 }
 
 }  // extern "C"

@@ -76,5 +76,25 @@ __device__ __forceinline__ int checked_page(const Cache& c, int page) {
   return -1;
 }
 
+// hyq_paged_attention's activations and output.
+struct AttendArgs {
+  Cache c;
+  const float* q;
+  int64_t q_stride;
+  int heads;
+  float* out;
+  int64_t out_stride;
+  void* ws;
+};
+
+// Largest number of sequences of a call (the kernels keep a prefix sum over
+// them in shared memory).
+constexpr int kMaxSeqs = 4096;
+
+// hyq_paged_mma.cu: head sizes 64 and 128 over 16-byte aligned rows.
+bool mma_supported(const AttendArgs& a, bool kv16);
+size_t mma_workspace_bytes(int dim);
+cudaError_t launch_mma(const AttendArgs& a, bool kv16, int64_t max_new, cudaStream_t st);
+
 }  // namespace paged
 }  // namespace hyq

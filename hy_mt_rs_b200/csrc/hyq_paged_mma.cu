@@ -1,0 +1,773 @@
+// Attention over pages on the warp-level tensor instructions, head sizes 64
+// and 128: the kernel for few new tokens (the cache is read once, bound by
+// memory) and the one for chunks (16 rows of a chunk per warp).
+//
+// Both keep f32 accuracy with split operands.  Over an f16 cache K and V are
+// exact, and the scaled queries and the weights are hi + lo, both f16 (22
+// bits): two products each.  Over an f32 cache every operand is hi + lo in
+// tf32 (hi rounded, lo cut: 22 bits, the full f32 range) and
+// lo.lo is left out: three products each.  The tensor cores cut their sums
+// instead of rounding them, which over a long context adds up (8e-6 at 1,100
+// positions), so each block's output is added to the running one in f32
+// arithmetic.  Weights are 2^(x - m): the scores carry log2(e) through the
+// queries.
+#include "hyq_kernels.h"
+#include "hyq_paged.cuh"
+
+namespace hyq {
+namespace paged {
+namespace {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = 32 * kWarps;
+constexpr int kRows = 16;            // query rows of a warp: (token, head) pairs
+constexpr int kCtasPerSm = 2;
+constexpr int kMaxCtas = 148 * kCtasPerSm;
+// Weights are kept 2^10 times their size, so that their lo halves stay normal
+// f16 numbers down to 2^-24 of the largest.
+constexpr float kBias = 10.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+
+// A warp's block of positions: POS rows of K, then of V, in 16-byte chunks
+// whose low three index bits are xored with the row (reads by ldmatrix and by
+// words then fall into distinct banks).  8 KB for head size 128.
+template <int DIM, bool KV16>
+struct Geo {
+  static constexpr int pos = KV16 ? 16 : 8;
+  static constexpr int row_bytes = DIM * (KV16 ? 2 : 4);
+  static constexpr int chunks = row_bytes / 16;
+  static constexpr int block = 2 * pos * row_bytes;
+  static constexpr int stages = 24576 / block;        // 3 (head size 128), 6 (64)
+  static constexpr int tile = kWarps * pos;           // positions of a CTA's step
+  static constexpr int copies = pos * chunks / 32;    // 16-byte copies per lane, K or V
+  static constexpr int smem = kWarps * stages * block;
+};
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+__device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t (&r)[4], uint32_t a) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(a)
+               : "memory");
+}
+__device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_tf32(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm("mma.sync.aligned.m16n8k8.row.col.f32.tf32.tf32.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+      : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+
+// 16-byte asynchronous copy, zeros instead when `bytes` is 0.
+__device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
+}
+
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+__device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
+  hi = pack_f16(a, b);
+  const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+  lo = pack_f16(a - f.x, b - f.y);
+}
+__device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) {
+  hi = (__float_as_uint(x) + 0x1000u) & 0xffffe000u;  // rounded to 10 mantissa bits; lo's 11 bits or so remain
+  lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
+}
+
+// What a warp holds of its 16 rows: the queries as the left operand of the
+// score products, the running maximum and sum, and the output.  Lane l holds
+// rows l / 4 and l / 4 + 8.
+template <int DIM, bool KV16>
+struct Rows {
+  uint32_t qh[KV16 ? DIM / 16 : 1][4];  // f16: hi and lo fragments
+  uint32_t ql[KV16 ? DIM / 16 : 1][4];
+  float qf[KV16 ? 1 : DIM / 8][4];      // f32: split where they are used
+  float factor[2];                      // 2^e taken out of a row's queries (f16)
+  int sees[2];                          // last position each row sees
+  float o[DIM / 8][4];
+  float m[2], l[2];
+
+  // Rows r0 .. r0 + 15 of the sequence's n * group (token, head) rows; rows
+  // past them are zero.
+  __device__ __forceinline__ void load(const AttendArgs& a, const Seq& s, int kvh, int group, int r0) {
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;  // log2(e) / sqrt(DIM)
+    const float* q[2];
+    bool in[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = r0 + (lane >> 2) + 8 * i, tok = r / group;
+      in[i] = tok < s.n;
+      sees[i] = s.pos + min(tok, s.n - 1);
+      q[i] = a.q + (int64_t)(s.row0 + (in[i] ? tok : 0)) * a.q_stride + (int64_t)(kvh * group + (in[i] ? r - tok * group : 0)) * DIM;
+      factor[i] = 1.0f;
+    }
+    if constexpr (KV16) {
+      // the row's largest value to [1, 2): an exact power of two, put back in
+      // the scores, so that no query overflows f16
+      float x[DIM / 16][2][4];
+      float top[2] = {0.f, 0.f};
+#pragma unroll
+      for (int k = 0; k < DIM / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int j = 0; j < 4; ++j) {
+            const float v = in[i] ? q[i][16 * k + 2 * t + (j & 1) + 8 * (j >> 1)] * scale : 0.f;
+            x[k][i][j] = v;
+            top[i] = fmaxf(top[i], fabsf(v));
+          }
+      float down[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+        // exponent bits of the largest value, kept where both powers are normal
+        const int e = min(max((int)(__float_as_uint(top[i]) >> 23), 1), 253);
+        factor[i] = __uint_as_float((uint32_t)e << 23);
+        down[i] = __uint_as_float((uint32_t)(254 - e) << 23);
+      }
+#pragma unroll
+      for (int k = 0; k < DIM / 16; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          split_f16(x[k][i][0] * down[i], x[k][i][1] * down[i], qh[k][i], ql[k][i]);
+          split_f16(x[k][i][2] * down[i], x[k][i][3] * down[i], qh[k][2 + i], ql[k][2 + i]);
+        }
+    } else {
+#pragma unroll
+      for (int k = 0; k < DIM / 8; ++k)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          qf[k][i] = in[i] ? q[i][8 * k + t] * scale : 0.f;
+          qf[k][2 + i] = in[i] ? q[i][8 * k + t + 4] * scale : 0.f;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      m[i] = -INFINITY;
+      l[i] = 0.f;
+    }
+#pragma unroll
+    for (int d = 0; d < DIM / 8; ++d)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) o[d][j] = 0.f;
+  }
+
+  // One block of positions p0 .. p0 + POS - 1 (K at k_s, V behind it); with
+  // `masked`, positions a row does not see are left out.
+  __device__ __forceinline__ void step(uint32_t k_s, int p0, bool masked) {
+    using G = Geo<DIM, KV16>;
+    const int lane = threadIdx.x & 31, t = lane & 3;
+    const uint32_t v_s = k_s + G::pos * G::row_bytes;
+    constexpr int NT = G::pos / 8;  // score tiles of 8 positions
+    float s[NT][4];
+    if constexpr (KV16) {
+      float lo[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = lo[n][j] = 0.f;
+      }
+#pragma unroll
+      for (int k = 0; k < DIM / 32; ++k)
+#pragma unroll
+        for (int n = 0; n < NT; ++n) {
+          const int row = 8 * n + (lane & 7), c = 4 * k + (lane >> 3);
+          uint32_t b[4];
+          ldsm4(b, k_s + row * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4));
+          mma_f16(s[n], qh[2 * k], b[0], b[1]);
+          mma_f16(lo[n], ql[2 * k], b[0], b[1]);
+          mma_f16(s[n], qh[2 * k + 1], b[2], b[3]);
+          mma_f16(lo[n], ql[2 * k + 1], b[2], b[3]);
+        }
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = (s[n][j] + lo[n][j]) * factor[j >> 1];
+    } else {
+      float lo[4] = {0.f, 0.f, 0.f, 0.f}, lo2[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[0][j] = 0.f;
+#pragma unroll
+      for (int k = 0; k < DIM / 16; ++k) {
+        const int row = lane & 7, c = 4 * k + (lane >> 3);
+        uint32_t b[4];
+        ldsm4(b, k_s + row * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4));
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          uint32_t qh_[4], ql_[4], bh[2], bl[2];
+#pragma unroll
+          for (int j = 0; j < 4; ++j) split_tf32(qf[2 * k + h][j], qh_[j], ql_[j]);
+#pragma unroll
+          for (int j = 0; j < 2; ++j) split_tf32(__uint_as_float(b[2 * h + j]), bh[j], bl[j]);
+          mma_tf32(s[0], qh_, bh[0], bh[1]);
+          mma_tf32(lo, qh_, bl[0], bl[1]);
+          mma_tf32(lo2, ql_, bh[0], bh[1]);
+        }
+      }
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[0][j] += lo[j] + lo2[j];
+    }
+    if (masked) {
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (p0 + 8 * n + 2 * t + (j & 1) > sees[j >> 1]) s[n][j] = -INFINITY;
+    }
+    float top[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      top[i] = fmaxf(s[0][2 * i], s[0][2 * i + 1]);
+#pragma unroll
+      for (int n = 1; n < NT; ++n) top[i] = fmaxf(top[i], fmaxf(s[n][2 * i], s[n][2 * i + 1]));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
+      top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
+    }
+    float down[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float now = fmaxf(m[i], top[i]);
+      down[i] = now == -INFINITY ? 1.0f : ex2(m[i] - now);
+      m[i] = now;
+      l[i] *= down[i];
+    }
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const float base = (m[i] == -INFINITY ? 0.f : m[i]) - kBias;
+#pragma unroll
+      for (int n = 0; n < NT; ++n)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          s[n][2 * i + j] = ex2(s[n][2 * i + j] - base);
+          l[i] += s[n][2 * i + j];
+        }
+    }
+    if constexpr (KV16) {
+      uint32_t ph[4], pl[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) split_f16(s[j >> 1][2 * (j & 1)], s[j >> 1][2 * (j & 1) + 1], ph[j], pl[j]);
+#pragma unroll
+      for (int d = 0; d < DIM / 16; ++d) {
+        const int mat = lane >> 3, row = 8 * (mat & 1) + (lane & 7), c = 2 * d + (mat >> 1);
+        uint32_t b[4];
+        ldsm4_t(b, v_s + row * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4));
+        float x[2][4] = {};
+        mma_f16(x[0], ph, b[0], b[1]);
+        mma_f16(x[1], ph, b[2], b[3]);
+        mma_f16(x[0], pl, b[0], b[1]);
+        mma_f16(x[1], pl, b[2], b[3]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          o[2 * d][j] = fmaf(o[2 * d][j], down[j >> 1], x[0][j]);
+          o[2 * d + 1][j] = fmaf(o[2 * d + 1][j], down[j >> 1], x[1][j]);
+        }
+      }
+    } else {
+      // the product's inner index t stands for position 2 t, t + 4 for 2 t + 1:
+      // the scores' own layout
+      uint32_t ph[4], pl[4];
+      split_tf32(s[0][0], ph[0], pl[0]);
+      split_tf32(s[0][2], ph[1], pl[1]);
+      split_tf32(s[0][1], ph[2], pl[2]);
+      split_tf32(s[0][3], ph[3], pl[3]);
+#pragma unroll
+      for (int d = 0; d < DIM / 8; ++d) {
+        uint32_t bh[2], bl[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          const int row = 2 * t + j, c = 2 * d + (lane >> 4);
+          float y;
+          asm volatile("ld.shared.f32 %0, [%1];"
+                       : "=f"(y)
+                       : "r"(v_s + row * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4) + ((lane >> 2) & 3) * 4)
+                       : "memory");
+          split_tf32(y, bh[j], bl[j]);
+        }
+        float x[4] = {};
+        mma_tf32(x, ph, bh[0], bh[1]);
+        mma_tf32(x, ph, bl[0], bl[1]);
+        mma_tf32(x, pl, bh[0], bh[1]);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[d][j] = fmaf(o[d][j], down[j >> 1], x[j]);
+      }
+    }
+  }
+};
+
+// The copies of a warp's block of positions into its stage.
+template <int DIM, bool KV16>
+struct Feed {
+  using G = Geo<DIM, KV16>;
+  const AttendArgs& a;
+  const Seq& s;
+  int kvh, len, shift;
+
+  // page of this lane's row (lane % POS) of the block at p0; -1: no row
+  __device__ __forceinline__ int page(int p0) const {
+    const int p = p0 + (threadIdx.x & 31) % G::pos;
+    return p < len ? s.pages[shift >= 0 ? p >> shift : p / a.c.page_size] : -1;
+  }
+  __device__ __forceinline__ void copy(uint32_t dst, int p0, int page) const {
+    const int lane = threadIdx.x & 31, p = p0 + lane % G::pos;
+    int64_t at = 0;
+    int ok = 0;
+    if (p < len) {
+      if (page >= 0 && page < a.c.pages) {
+        const int row = shift >= 0 ? p & ((1 << shift) - 1) : p % a.c.page_size;
+        at = (int64_t)page * a.c.page_stride + (int64_t)kvh * a.c.head_stride + (int64_t)row * a.c.row_stride;
+        ok = 16;
+      } else {
+        atomicOr(a.c.status, DEV_BAD_ARGS);
+      }
+    }
+    constexpr int esize = KV16 ? 2 : 4;
+    const char* k = static_cast<const char*>(a.c.k);
+    const char* v = static_cast<const char*>(a.c.v);
+#pragma unroll
+    for (int i = 0; i < G::copies; ++i) {
+      const int x = i * 32 + lane, row = x / G::chunks, c = x % G::chunks;
+      const int64_t off = __shfl_sync(0xffffffffu, at, row) * esize + 16 * c;
+      const int n = __shfl_sync(0xffffffffu, ok, row);
+      const uint32_t to = dst + row * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4);
+      copy16(to, k + (n ? off : 0), n);
+      copy16(to + G::pos * G::row_bytes, v + (n ? off : 0), n);
+    }
+  }
+  // Non-finite values of V at positions past `first` (the first new token's
+  // own) become zero in shared memory: a row that does not see them would
+  // multiply them by a weight of zero.  The rows that see them add them back
+  // at the end (unseen()).  Returns whether this lane found any.
+  __device__ __forceinline__ bool clean(uint32_t dst, int p0, int first) const {
+    if (p0 + G::pos - 1 <= first) return false;
+    const int lane = threadIdx.x & 31;
+    bool found = false;
+#pragma unroll 1
+    for (int i = 0; i < G::copies; ++i) {
+      const int x = i * 32 + lane, row = x / G::chunks, c = x % G::chunks;
+      if (p0 + row <= first) continue;
+      const uint32_t at = dst + (G::pos + row) * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4);
+      uint32_t w[4];
+      asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at) : "memory");
+      bool bad = false;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if constexpr (KV16) {
+          if ((w[j] & 0x7c00u) == 0x7c00u) w[j] &= 0xffff0000u, bad = true;
+          if ((w[j] & 0x7c000000u) == 0x7c000000u) w[j] &= 0xffffu, bad = true;
+        } else {
+          if ((w[j] & 0x7f800000u) == 0x7f800000u) w[j] = 0, bad = true;
+        }
+      }
+      found = found || bad;
+      if (bad)
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(at), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]) : "memory");
+    }
+    __syncwarp();
+    return found;
+  }
+};
+
+// The non-finite values that clean() took out past token `first`'s position,
+// for a row at token `tok` of the sequence: their sum (0 when there are none).
+template <bool KV16>
+__device__ __noinline__ float unseen(const AttendArgs& a, const Seq& s, int kvh, int first, int tok, int d) {
+  float x = 0.f;
+  for (int p = s.pos + first + 1; p <= s.pos + tok; ++p) {
+    const int page = s.pages[p / a.c.page_size];
+    if (page < 0 || page >= a.c.pages) continue;
+    const int64_t at = (int64_t)page * a.c.page_stride + (int64_t)kvh * a.c.head_stride +
+                       (int64_t)(p % a.c.page_size) * a.c.row_stride + d;
+    const float v = KV16 ? __half2float(static_cast<const __half*>(a.c.v)[at]) : static_cast<const float*>(a.c.v)[at];
+    if (!isfinite(v)) x += v;
+  }
+  return x;
+}
+
+// ---------------------------------------------------------------------------
+// Few new tokens: at most 16 (token, head) rows per kv head
+// ---------------------------------------------------------------------------
+
+// Workspace: one counter per CTA, then two partial results per CTA: 16 rows of
+// DIM outputs, then the rows' (maximum, sum).
+constexpr size_t kCounterBytes = (kMaxCtas * sizeof(unsigned) + 255) / 256 * 256;
+__host__ __device__ constexpr int partial_floats(int dim) { return kRows * (dim + 2); }
+
+// The (sequence, kv head) segments' tiles form one line, cut into equal
+// ranges, one per CTA: any mix of lengths loads every SM alike and the whole
+// cache is read once.  A segment inside one CTA's range is finished there;
+// one that spans CTAs leaves partial results, and the last CTA to get there
+// adds them in the order of the CTAs (the result does not depend on which one
+// that is).  Within a tile each warp takes its own POS positions for all 16
+// rows, through its own ring of asynchronous copies; the warps meet at the
+// end of a segment.
+template <int DIM, bool KV16>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_constant__ AttendArgs a, int shift) {
+  using G = Geo<DIM, KV16>;
+  grid_dependency_wait();
+  allow_dependents_launch();
+  extern __shared__ __align__(1024) char smem[];
+  int* first_s = reinterpret_cast<int*>(smem + G::smem);  // [seqs + 1] tiles (of one kv head) before each sequence
+  __shared__ float ml_s[kWarps][kRows][2];
+  __shared__ int warp_s[kWarps];
+  __shared__ int last_s;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.heads / a.c.kv_heads, seqs = a.c.seqs, kvh_n = a.c.kv_heads;
+  // prefix sum of the sequences' tiles; sequences with more rows are the
+  // chunk kernel's
+  int carry = 0;
+  for (int s0 = 0; s0 < seqs; s0 += kThreads) {
+    const int i = s0 + (int)threadIdx.x;
+    int tiles = 0;
+    if (i < seqs) {
+      const Seq s = load_seq(a.c, i);
+      if (s.n > 0 && s.n * group <= kRows) tiles = (s.pos + s.n + G::tile - 1) / G::tile;
+    }
+    int x = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) warp_s[warp] = x;
+    __syncthreads();
+    int before = carry;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += warp_s[w];
+      carry += warp_s[w];
+    }
+    if (i < seqs) first_s[i] = before + x - tiles;
+    __syncthreads();
+  }
+  if (threadIdx.x == 0) first_s[seqs] = carry;
+  __syncthreads();
+  const int64_t work = (int64_t)carry * kvh_n;
+  const int ctas = (int)min((int64_t)gridDim.x, work), cta = blockIdx.x;
+  if (cta >= ctas) return;
+  int64_t at = work * cta / ctas;
+  const int64_t end = work * (cta + 1) / ctas;
+  const int64_t begin = at;
+  int si = 0;
+  {
+    int lo = 0, hi = seqs - 1;  // the last sequence whose segments start at or before `at`
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((int64_t)first_s[mid] * kvh_n <= at) lo = mid;
+      else hi = mid - 1;
+    }
+    si = lo;
+  }
+  float* parts = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
+  unsigned* counters = static_cast<unsigned*>(a.ws);
+  Rows<DIM, KV16> rows;
+  const uint32_t ring = smem_addr(smem) + warp * G::stages * G::block;
+  while (at < end) {
+    while ((int64_t)first_s[si + 1] * kvh_n <= at) ++si;  // past empty sequences
+    const int tiles = first_s[si + 1] - first_s[si];
+    const int64_t s_at = (int64_t)first_s[si] * kvh_n;
+    const int kvh = (int)((at - s_at) / tiles);
+    const int64_t seg0 = s_at + (int64_t)kvh * tiles, seg1 = seg0 + tiles;
+    const int j0 = (int)(at - seg0), j1 = (int)(min(end, seg1) - seg0);
+    const Seq s = load_seq(a.c, si);
+    const Feed<DIM, KV16> feed{a, s, kvh, s.pos + s.n, shift};
+    const int step = G::tile, off = warp * G::pos;
+    // fill the ring, then one block per turn
+    int page = feed.page(j0 * step + off);
+#pragma unroll
+    for (int i = 0; i < G::stages - 1; ++i) {
+      const int now = page;
+      page = feed.page((j0 + i + 1) * step + off);
+      if (j0 + i < j1) feed.copy(ring + i * G::block, (j0 + i) * step + off, now);
+      cp_async_commit();
+    }
+    rows.load(a, s, kvh, group, 0);
+    int stage = 0;
+    for (int j = j0; j < j1; ++j) {
+      const int ahead = j + G::stages - 1, now = page;
+      page = feed.page((ahead + 1) * step + off);
+      int put = stage + G::stages - 1;
+      if (put >= G::stages) put -= G::stages;
+      __syncwarp();
+      if (ahead < j1) feed.copy(ring + put * G::block, ahead * step + off, now);
+      cp_async_commit();
+      cp_async_wait<G::stages - 1>();
+      __syncwarp();
+      const int p0 = j * step + off;
+      const bool masked = p0 + G::pos - 1 > s.pos;
+      if (masked) feed.clean(ring + stage * G::block, p0, s.pos);
+      rows.step(ring + stage * G::block, p0, masked);
+      if (++stage == G::stages) stage = 0;
+    }
+    // the warps' results: maximum and sum of each row, then the outputs
+    // scaled to the common maximum, in the rings' memory
+    cp_async_wait<0>();
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      float l = rows.l[i];
+      l += __shfl_xor_sync(0xffffffffu, l, 1);
+      l += __shfl_xor_sync(0xffffffffu, l, 2);
+      if ((lane & 3) == 0) {
+        ml_s[warp][(lane >> 2) + 8 * i][0] = rows.m[i];
+        ml_s[warp][(lane >> 2) + 8 * i][1] = l;
+      }
+    }
+    __syncthreads();
+    constexpr int pitch = DIM + 4;
+    float* o_s = reinterpret_cast<float*>(smem);  // [warp][16][pitch]
+    static_assert(kWarps * kRows * pitch * 4 <= G::smem, "the rings hold the warps' outputs");
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int r = (lane >> 2) + 8 * i;
+      float top = ml_s[0][r][0];
+#pragma unroll
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, ml_s[w][r][0]);
+      const float down = rows.m[i] == -INFINITY ? 0.f : ex2(rows.m[i] - top);
+      float* to = o_s + (warp * kRows + r) * pitch + 2 * (lane & 3);
+#pragma unroll
+      for (int d = 0; d < DIM / 8; ++d)
+        *reinterpret_cast<float2*>(to + 8 * d) = make_float2(rows.o[d][2 * i] * down, rows.o[d][2 * i + 1] * down);
+    }
+    __syncthreads();
+    const int live = s.n * group;
+    const bool whole = j0 == 0 && j1 == tiles;
+    float* part = parts + (size_t)(2 * cta + (at != begin)) * partial_floats(DIM);
+    for (int x = threadIdx.x; x < live * DIM; x += kThreads) {
+      const int r = x / DIM, d = x % DIM;
+      float sum = 0.f, top = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        sum += o_s[(w * kRows + r) * pitch + d];
+        top = fmaxf(top, ml_s[w][r][0]);
+      }
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w)
+        l += ml_s[w][r][0] == -INFINITY ? 0.f : ml_s[w][r][1] * ex2(ml_s[w][r][0] - top);
+      if (whole) {
+        const int tok = r / group;
+        float y = sum / l;
+        if (s.n > 1) y += unseen<KV16>(a, s, kvh, 0, tok, d);
+        a.out[(int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + d] = y;
+      } else {
+        part[x] = sum;
+        if (d == 0) {
+          part[kRows * DIM + 2 * r] = top;
+          part[kRows * DIM + 2 * r + 1] = l;
+        }
+      }
+    }
+    if (!whole) {
+      // the CTAs that share the segment: cf holds its first tile, cl its last
+      int cf = (int)(seg0 * ctas / work);
+      while (work * (cf + 1) / ctas <= seg0) ++cf;
+      while (cf > 0 && work * cf / ctas > seg0) --cf;
+      int cl = (int)((seg1 - 1) * ctas / work);
+      while (work * (cl + 1) / ctas <= seg1 - 1) ++cl;
+      while (cl > 0 && work * cl / ctas > seg1 - 1) --cl;
+      __threadfence();
+      __syncthreads();
+      if (threadIdx.x == 0) last_s = atomicAdd(&counters[cf], 1u) == (unsigned)(cl - cf);
+      __syncthreads();
+      if (last_s) {
+        __threadfence();
+        for (int x = threadIdx.x; x < live * DIM; x += kThreads) {
+          const int r = x / DIM, d = x % DIM;
+          float top = -INFINITY;
+          for (int c = cf; c <= cl; ++c) {
+            const float* p = parts + (size_t)(2 * c + (work * c / ctas < seg0)) * partial_floats(DIM);
+            top = fmaxf(top, __ldcg(p + kRows * DIM + 2 * r));
+          }
+          float sum = 0.f, l = 0.f;
+          for (int c = cf; c <= cl; ++c) {
+            const float* p = parts + (size_t)(2 * c + (work * c / ctas < seg0)) * partial_floats(DIM);
+            const float pm = __ldcg(p + kRows * DIM + 2 * r);
+            const float f = pm == -INFINITY ? 0.f : ex2(pm - top);
+            sum = fmaf(f, __ldcg(p + x), sum);
+            l = fmaf(f, __ldcg(p + kRows * DIM + 2 * r + 1), l);
+          }
+          const int tok = r / group;
+          float y = sum / l;
+          if (s.n > 1) y += unseen<KV16>(a, s, kvh, 0, tok, d);
+          a.out[(int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + d] = y;
+        }
+        if (threadIdx.x == 0) counters[cf] = 0;
+      }
+    }
+    at = seg0 + j1;
+    __syncthreads();  // the rings are free again
+  }
+}
+
+// ---------------------------------------------------------------------------
+// Chunks: 16 rows of a sequence's (token, head) rows per warp
+// ---------------------------------------------------------------------------
+
+constexpr int kChunkRows = kWarps * kRows;
+
+// Grid (row tiles, kv heads): tile x belongs to the sequence whose tiles
+// (64 rows each) contain it.  The four warps share every tile of positions.
+template <int DIM, bool KV16>
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __grid_constant__ AttendArgs a, int shift) {
+  using G = Geo<DIM, KV16>;
+  grid_dependency_wait();
+  allow_dependents_launch();
+  extern __shared__ __align__(1024) char smem[];
+  __shared__ int found_s[2];
+  __shared__ int dirty_s;  // clean() took something out
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int group = a.heads / a.c.kv_heads, kvh = blockIdx.y;
+  if (threadIdx.x == 0) {
+    found_s[0] = -1;
+    dirty_s = 0;
+  }
+  __syncthreads();
+  if (warp == 0) {
+    int carry = 0;
+    const int want = gridDim.x - 1 - blockIdx.x;  // the last (longest) tiles first
+    for (int s0 = 0; s0 < a.c.seqs && carry <= want; s0 += 32) {
+      int tiles = 0;
+      if (s0 + lane < a.c.seqs) {
+        const Seq s = load_seq(a.c, s0 + lane);
+        if (s.n * group > kRows) tiles = (s.n * group + kChunkRows - 1) / kChunkRows;
+      }
+      int x = tiles;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(0xffffffffu, x, o);
+        if (lane >= o) x += y;
+      }
+      const int before = carry + x - tiles;
+      if (before <= want && want < before + tiles) {
+        found_s[0] = s0 + lane;
+        found_s[1] = want - before;
+      }
+      carry += __shfl_sync(0xffffffffu, x, 31);
+    }
+  }
+  __syncthreads();
+  if (found_s[0] < 0) return;
+  const Seq s = load_seq(a.c, found_s[0]);
+  const int r0 = found_s[1] * kChunkRows + warp * kRows;
+  // positions the tile's last row sees
+  const int last_tok = min(s.n - 1, (found_s[1] * kChunkRows + kChunkRows - 1) / group);
+  const int len = s.pos + last_tok + 1, tiles = (len + G::tile - 1) / G::tile;
+  const int first_tok = min(s.n - 1, found_s[1] * kChunkRows / group);
+  const Feed<DIM, KV16> feed{a, s, kvh, len, shift};
+  const uint32_t ring = smem_addr(smem);
+  constexpr int stage_bytes = kWarps * G::block;
+  const int off = warp * G::pos;
+  int page = feed.page(off);
+#pragma unroll
+  for (int i = 0; i < G::stages - 1; ++i) {
+    const int now = page;
+    page = feed.page((i + 1) * G::tile + off);
+    if (i < tiles) feed.copy(ring + i * stage_bytes + warp * G::block, i * G::tile + off, now);
+    cp_async_commit();
+  }
+  Rows<DIM, KV16> rows;
+  rows.load(a, s, kvh, group, r0);
+  const bool any = r0 < s.n * group;
+  int stage = 0;
+  for (int j = 0; j < tiles; ++j) {
+    cp_async_wait<G::stages - 2>();
+    __syncwarp();
+    if ((j + 1) * G::tile - 1 > s.pos + first_tok &&
+        feed.clean(ring + stage * stage_bytes + warp * G::block, j * G::tile + off, s.pos + first_tok))
+      dirty_s = 1;
+    __syncthreads();  // tile j has landed; tile j - 1 has been read
+    const int ahead = j + G::stages - 1, now = page;
+    page = feed.page((ahead + 1) * G::tile + off);
+    int put = stage + G::stages - 1;
+    if (put >= G::stages) put -= G::stages;
+    if (ahead < tiles) feed.copy(ring + put * stage_bytes + warp * G::block, ahead * G::tile + off, now);
+    cp_async_commit();
+    if (any) {
+#pragma unroll 1
+      for (int b = 0; b < kWarps; ++b) {
+        const int p0 = j * G::tile + b * G::pos;
+        if (p0 >= len) break;
+        rows.step(ring + stage * stage_bytes + b * G::block, p0, p0 + G::pos - 1 > s.pos + first_tok);
+      }
+    }
+    if (++stage == G::stages) stage = 0;
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  if (!any) return;
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    float l = rows.l[i];
+    l += __shfl_xor_sync(0xffffffffu, l, 1);
+    l += __shfl_xor_sync(0xffffffffu, l, 2);
+    const int r = r0 + (lane >> 2) + 8 * i, tok = r / group;
+    if (tok >= s.n) continue;
+    float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + 2 * (lane & 3);
+#pragma unroll
+    for (int d = 0; d < DIM / 8; ++d) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        float y = rows.o[d][2 * i + j] / l;
+        if (dirty_s) y += unseen<KV16>(a, s, kvh, first_tok, tok, 8 * d + 2 * (lane & 3) + j);
+        to[8 * d + j] = y;
+      }
+    }
+  }
+}
+
+template <int DIM, bool KV16>
+cudaError_t launch(const AttendArgs& a, int64_t max_new, cudaStream_t st) {
+  using G = Geo<DIM, KV16>;
+  int shift = -1;
+  if ((a.c.page_size & (a.c.page_size - 1)) == 0) shift = __builtin_ctz((unsigned)a.c.page_size);
+  const int group = a.heads / a.c.kv_heads;
+  cudaError_t e;
+  if (max_new * group > kRows) {
+    const int64_t tiles = ((int64_t)a.c.tokens * group + kChunkRows - 1) / kChunkRows + a.c.seqs;
+    auto k = chunk_kernel<DIM, KV16>;
+    if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem)) != cudaSuccess) return e;
+    if ((e = launch_ex(k, dim3((unsigned)tiles, (unsigned)a.c.kv_heads), dim3(kThreads), G::smem, st, a, shift)) != cudaSuccess)
+      return e;
+  }
+  // (one token per sequence is the fewest there can be: the rows of a
+  // sequence fit one tile of 16 unless every sequence has a chunk)
+  auto k = few_kernel<DIM, KV16>;
+  const int smem = G::smem + (kMaxSeqs + 1) * 4;
+  if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+  return launch_ex(k, dim3(kMaxCtas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4, st, a, shift);
+}
+
+}  // namespace
+
+bool mma_supported(const AttendArgs& a, bool kv16) {
+  const int64_t strides = (a.c.page_stride | a.c.head_stride | a.c.row_stride) * (kv16 ? 2 : 4);
+  return (a.c.dim == 64 || a.c.dim == 128) && strides % 16 == 0 &&
+         (reinterpret_cast<uintptr_t>(a.c.k) | reinterpret_cast<uintptr_t>(a.c.v)) % 16 == 0;
+}
+
+size_t mma_workspace_bytes(int dim) { return kCounterBytes + 2 * (size_t)kMaxCtas * partial_floats(dim) * sizeof(float); }
+
+cudaError_t launch_mma(const AttendArgs& a, bool kv16, int64_t max_new, cudaStream_t st) {
+  if (a.c.dim == 128) return kv16 ? launch<128, true>(a, max_new, st) : launch<128, false>(a, max_new, st);
+  return kv16 ? launch<64, true>(a, max_new, st) : launch<64, false>(a, max_new, st);
+}
+
+}  // namespace paged
+}  // namespace hyq

@@ -61,7 +61,467 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
   return v;
 }
 
-// One CTA per row; every pass reads the row again.
+// ---------------------------------------------------------------------------
+// Rows held in registers by a cluster of CTAs
+// ---------------------------------------------------------------------------
+//
+// The row is read from memory once: each thread keeps E logits.  What the
+// CTAs of a row tell one another goes through distributed shared memory, one
+// cluster barrier per exchange:
+//   1. the largest logit (with its index: the greedy token) and the smallest;
+//   2. with top-k or top-p, a histogram of z = (max - logit) / temperature
+//      over at most 28 (past it a weight is 0: e^-28 < 2^-40) in 512 equal
+//      bins, counts and masses; every CTA adds up all of them and finds the
+//      bin in which the k-th logit, or the top_p of the mass, falls;
+//   3. that bin's few logits, listed in every CTA, which ranks them by value
+//      and index: the last one kept is the cut.  A bin with more than kList
+//      (ties, a wide row) is divided again by the bits of the key, then by
+//      index, until it fits;
+//   4. each CTA's kept mass: the one that holds the draw walks its part.
+namespace cluster {
+
+constexpr int kT = 512;                // threads of a CTA
+constexpr int kW = kT / 32;
+constexpr int kBins = 512;
+static_assert(kBins == kT, "one bin per thread");
+constexpr int kList = 1024;
+constexpr int kMaxCluster = 16;
+constexpr float kSpan = 28.0f;
+
+__device__ __forceinline__ unsigned ctarank() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ unsigned nctas() {
+  unsigned r;
+  asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
+  return r;
+}
+__device__ __forceinline__ void barrier() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// The same shared address in CTA `rank`.
+__device__ __forceinline__ uint32_t remote(const void* p, unsigned rank) {
+  uint32_t a;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(a) : "r"(smem_addr(p)), "r"(rank));
+  return a;
+}
+__device__ __forceinline__ void put64(uint32_t a, u64 v) {
+  asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
+}
+__device__ __forceinline__ unsigned get32(uint32_t a) {
+  unsigned v;
+  asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
+  return v;
+}
+
+struct Shared {
+  // counts, and the masses in parts of 14 bits (sums of 16,384 stay below
+  // 2^32; shared 32-bit atomics are native, 64-bit ones are not)
+  unsigned hist[4][kBins];
+  u64 list[kList];              // ~key << 32 | index: ascending = kept first
+  u64 max_of[kMaxCluster];      // key << 32 | ~index
+  u64 min_of[kMaxCluster];
+  u64 mass_of[kMaxCluster];
+  u64 warp_a[kW], warp_b[kW];
+  unsigned fill;                // this CTA's entries in the list
+  unsigned bin;
+  u64 above_n, above_w, in_n;
+  u64 cut;
+};
+
+template <int E>
+struct Row {
+  float x[E];
+  int base;   // index of x[4 j + k]: base + 128 j + 4 lane + k
+  int n;
+
+  __device__ __forceinline__ int index(int i) const { return base + 128 * (i >> 2) + 4 * (threadIdx.x & 31) + (i & 3); }
+};
+
+struct Scale {
+  unsigned max_key;
+  float max, inverse, bins;
+  __device__ __forceinline__ float e(float x) const {
+    return x == max ? 1.0f : expf(__fmul_rn(__fsub_rn(x, max), inverse));
+  }
+  // monotone in the logit; kBins and more: no weight
+  __device__ __forceinline__ unsigned bin(float x) const {
+    if (x == max) return 0;
+    return (unsigned)fminf(__fmul_rn(__fmul_rn(__fsub_rn(max, x), inverse), bins), 4.0f * kBins);
+  }
+};
+
+// Order of the tokens: larger logits first, ties by index.
+__device__ __forceinline__ u64 order_of(float x, int index) { return ((u64)~key_of(x) << 32) | (unsigned)index; }
+
+// Which part of a bin is meant: a z bin, then (level > 0) leading bits of the
+// order, 9 at a time.
+struct Part {
+  unsigned zbin;
+  u64 prefix, mask;
+  int shift;     // of the next 9 bits; 64: by z
+};
+
+__device__ __forceinline__ unsigned sub_bin(const Scale& sc, const Part& p, float x, u64 order) {
+  const unsigned z = sc.bin(x);
+  if (p.shift == 64) return z;
+  if (z != p.zbin || (order & p.mask) != p.prefix) return kBins;
+  return (unsigned)(order >> p.shift) & (kBins - 1);
+}
+
+// Exclusive sums over the CTA's bins of two values, one bin per thread.
+__device__ __forceinline__ void scan2(Shared& sh, u64 a, u64 b, u64& before_a, u64& before_b) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 x = a, y = b;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 p = __shfl_up_sync(0xffffffffu, x, o), q = __shfl_up_sync(0xffffffffu, y, o);
+    if (lane >= o) {
+      x += p;
+      y += q;
+    }
+  }
+  __syncthreads();
+  if (lane == 31) {
+    sh.warp_a[warp] = x;
+    sh.warp_b[warp] = y;
+  }
+  __syncthreads();
+  before_a = x - a;
+  before_b = y - b;
+  for (int w = 0; w < warp; ++w) {
+    before_a += sh.warp_a[w];
+    before_b += sh.warp_b[w];
+  }
+}
+
+// The cut: the last token kept when the kept ones are cut either to the first
+// `want` (BY_MASS false) or to those whose predecessors weigh less than
+// `want`.  Tokens past `limit` (an earlier cut) do not count.  Returns the
+// order of the last one kept, and the mass of all kept in `mass`; ~0 when the
+// whole row weighs or counts less.
+template <int E, bool BY_MASS>
+__device__ u64 find_cut(Shared& sh, const Row<E>& row, const Scale& sc, u64 limit, u64 want, u64& mass) {
+  const unsigned rank = ctarank(), ctas = nctas();
+  u64 above_n = 0, above_w = 0;  // tokens before the part, their mass
+  Part part{0, 0, 0, 64};
+  for (int level = 0; level < 10; ++level) {
+    for (int i = threadIdx.x; i < 4 * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
+    if (threadIdx.x == 0) {
+      sh.fill = 0;
+      sh.bin = kBins;
+    }
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < E; ++i) {
+      const int at = row.index(i);
+      if (at < row.n) {
+        const u64 order = order_of(row.x[i], at);
+        const unsigned b = sub_bin(sc, part, row.x[i], order);
+        if (b < kBins && order <= limit) {
+          const u64 w = weight_of(sc.e(row.x[i]));
+          atomicAdd(&sh.hist[0][b], 1u);
+          atomicAdd(&sh.hist[1][b], (unsigned)(w & 0x3fff));
+          atomicAdd(&sh.hist[2][b], (unsigned)(w >> 14 & 0x3fff));
+          atomicAdd(&sh.hist[3][b], (unsigned)(w >> 28));
+        }
+      }
+    }
+    barrier();
+    u64 count = 0, weight = 0, lower = 0;  // of this thread's bin; entries of the CTAs before this one
+    for (unsigned c = 0; c < ctas; ++c) {
+      const uint32_t h = remote(&sh.hist[0][threadIdx.x], c);
+      const unsigned k = get32(h);
+      if (c < rank) lower += k;
+      count += k;
+      weight += (u64)get32(h + 4 * kBins) + ((u64)get32(h + 8 * kBins) << 14) + ((u64)get32(h + 12 * kBins) << 28);
+    }
+    u64 before_n, before_w;
+    scan2(sh, count, weight, before_n, before_w);
+    before_n += above_n;
+    before_w += above_w;
+    const bool here = BY_MASS ? before_w < want && before_w + weight >= want : before_n < want && before_n + count >= want;
+    if (here) {
+      sh.bin = threadIdx.x;
+      sh.above_n = before_n;
+      sh.above_w = before_w;
+      sh.in_n = count;
+      sh.fill = (unsigned)min(lower, (u64)kList);
+    }
+    if (threadIdx.x == kT - 1) sh.cut = before_w + weight;
+    __syncthreads();
+    const unsigned b = sh.bin;
+    if (b == kBins) {  // only at the first level: the row has less than that
+      mass = sh.cut;
+      return ~0ull;
+    }
+    above_n = sh.above_n;
+    above_w = sh.above_w;
+    const u64 inside = sh.in_n;
+    if (inside <= kList) {
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < E; ++i) {
+        const int at = row.index(i);
+        if (at < row.n) {
+          const u64 order = order_of(row.x[i], at);
+          if (order <= limit && sub_bin(sc, part, row.x[i], order) == b) {
+            const unsigned slot = atomicAdd(&sh.fill, 1u);
+            for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order);
+          }
+        }
+      }
+      barrier();
+      // rank and mass before each of the part's tokens
+      const int m = (int)inside;
+      u64 total = 0, last = 0;
+      for (int t = threadIdx.x; t < m; t += kT) {
+        const u64 mine = sh.list[t];
+        u64 before = above_w;
+        u64 place = above_n;
+        for (int j = 0; j < m; ++j) {
+          const u64 other = sh.list[j];
+          if (other < mine) {
+            ++place;
+            if (BY_MASS) before += weight_of(sc.e(value_of(~(unsigned)(other >> 32))));
+          }
+        }
+        if (BY_MASS ? before < want : place < want) {
+          total += weight_of(sc.e(value_of(~(unsigned)(mine >> 32))));
+          last = max(last, mine);
+        }
+      }
+      total = warp_sum_u64(total);
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) {
+        sh.warp_a[threadIdx.x >> 5] = total;
+        sh.warp_b[threadIdx.x >> 5] = last;
+      }
+      __syncthreads();
+      mass = above_w;
+      for (int w = 0; w < kW; ++w) {
+        mass += sh.warp_a[w];
+        last = max(last, sh.warp_b[w]);
+      }
+      __syncthreads();
+      return last;
+    }
+    barrier();  // the histograms are read; divide the part
+    if (part.shift == 64) {
+      part.zbin = b;
+      part.shift = 55;
+    } else {
+      part.prefix |= (u64)b << part.shift;
+      part.mask |= (u64)(kBins - 1) << part.shift;
+      part.shift = part.shift >= 9 ? part.shift - 9 : 0;
+    }
+  }
+  return ~0ull;
+}
+
+template <int E>
+__global__ void __launch_bounds__(kT, 2) sample_cluster_kernel(const __grid_constant__ Args a) {
+  grid_dependency_wait();
+  allow_dependents_launch();
+  __shared__ Shared sh;
+  const unsigned rank = ctarank(), ctas = nctas();
+  const int r = blockIdx.x / ctas, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const float* x = a.logits + r * a.stride;
+  Row<E> row;
+  row.n = a.n;
+  row.base = ((int)rank * kW + warp) * 32 * E;
+  u64 top = 0, low = ~0ull;
+  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
+#pragma unroll
+  for (int j = 0; j < E / 4; ++j) {
+    const int at = row.index(4 * j);
+    if (vec && at + 4 <= a.n) {
+      const float4 v = __ldcs(reinterpret_cast<const float4*>(x + at));
+      row.x[4 * j] = v.x;
+      row.x[4 * j + 1] = v.y;
+      row.x[4 * j + 2] = v.z;
+      row.x[4 * j + 3] = v.w;
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) row.x[4 * j + k] = at + k < a.n ? __ldcs(x + at + k) : -INFINITY;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    if (isnan(row.x[i])) row.x[i] = -INFINITY;
+    if (row.x[i] == 0.0f) row.x[i] = 0.0f;  // -0 as +0
+    const int at = row.index(i);
+    if (at < a.n) {
+      const u64 k = (u64)key_of(row.x[i]) << 32;
+      top = max(top, k | (unsigned)~at);
+      low = min(low, k);
+    }
+  }
+#pragma unroll
+  for (int o = 16; o > 0; o >>= 1) {
+    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+    low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+  }
+  if (lane == 0) {
+    sh.warp_a[warp] = top;
+    sh.warp_b[warp] = low;
+  }
+  // every CTA of the cluster runs before its shared memory is written to
+  barrier();
+  if (threadIdx.x < ctas) {
+    for (int w = 0; w < kW; ++w) {
+      top = max(top, sh.warp_a[w]);
+      low = min(low, sh.warp_b[w]);
+    }
+    put64(remote(&sh.max_of[rank], threadIdx.x), top);
+    put64(remote(&sh.min_of[rank], threadIdx.x), low);
+  }
+  barrier();
+  top = 0;
+  low = ~0ull;
+  for (unsigned c = 0; c < ctas; ++c) {
+    top = max(top, sh.max_of[c]);
+    low = min(low, sh.min_of[c]);
+  }
+  Scale sc;
+  sc.max_key = (unsigned)(top >> 32);
+  sc.max = value_of(sc.max_key);
+  const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+  if (sc.max == -INFINITY || !(temperature > 0.0f)) {
+    if (rank == 0 && threadIdx.x == 0) {
+      a.token[r] = sc.max == -INFINITY ? 0 : (int)~(unsigned)top;
+      if (a.prob) a.prob[r] = sc.max == -INFINITY ? 0.0f : 1.0f;
+    }
+    return;
+  }
+  sc.inverse = __fdiv_rn(1.0f, temperature);
+  const float span = (sc.max - value_of((unsigned)(low >> 32))) * sc.inverse;
+  sc.bins = (kBins - 1) / fminf(fmaxf(span, 1e-20f), kSpan);
+  const int k = a.top_k ? a.top_k[r] : 0;
+  const float p = a.top_p ? a.top_p[r] : 1.0f;
+  const float floor_e = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
+  u64 cut = ~0ull, mass = 0;
+  if (k > 0 && k < a.n) cut = find_cut<E, false>(sh, row, sc, cut, (u64)k, mass);
+  if (p < 1.0f) {
+    if (cut == ~0ull) {
+      // nothing cut so far: the whole row's mass
+      u64 m = 0;
+#pragma unroll
+      for (int i = 0; i < E; ++i)
+        if (row.index(i) < a.n) m += weight_of(sc.e(row.x[i]));
+      m = warp_sum_u64(m);
+      __syncthreads();
+      if (lane == 0) sh.warp_a[warp] = m;
+      __syncthreads();
+      if (threadIdx.x < ctas) {
+        m = 0;
+        for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
+        put64(remote(&sh.mass_of[rank], threadIdx.x), m);
+      }
+      barrier();
+      mass = 0;
+      for (unsigned c = 0; c < ctas; ++c) mass += sh.mass_of[c];
+    }
+    const u64 share = (u64)ceilf(__fmul_rn(fmaxf(p, 0.0f), 16777216.0f));
+    const u64 want = max(scaled(mass, share, (1u << kGrid) - 1), 1ull);
+    u64 ignored;
+    barrier();  // mass_of and the histograms may be written again
+    cut = min(cut, find_cut<E, true>(sh, row, sc, cut, want, ignored));
+  }
+  // kept mass of each thread, warp and CTA
+  u64 mine = 0;
+#pragma unroll
+  for (int i = 0; i < E; ++i) {
+    const int at = row.index(i);
+    if (at < a.n && order_of(row.x[i], at) <= cut) {
+      const float e = sc.e(row.x[i]);
+      if (e >= floor_e) mine += weight_of(e);
+    }
+  }
+  const u64 warp_mass = warp_sum_u64(mine);
+  __syncthreads();
+  if (lane == 0) sh.warp_a[warp] = warp_mass;
+  barrier();  // mass_of may be written again
+  if (threadIdx.x < ctas) {
+    u64 m = 0;
+    for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
+    put64(remote(&sh.mass_of[rank], threadIdx.x), m);
+  }
+  barrier();
+  u64 total = 0, run = 0;
+  for (unsigned c = 0; c < ctas; ++c) {
+    if (c == rank) run = total;
+    total += sh.mass_of[c];
+  }
+  const float uf = fminf(fmaxf(a.u[r], 0.0f), 1.0f);
+  const u64 ui = min((u64)__fmul_rn(uf, 16777216.0f), (u64)(1u << kGrid) - 1);
+  const u64 aim = scaled(total, ui, 0);
+  for (int w = 0; w < warp; ++w) run += sh.warp_a[w];
+  if (aim < run || aim >= run + warp_mass) return;
+  // this warp holds the token: index order is group by group of 128
+#pragma unroll
+  for (int j = 0; j < E / 4; ++j) {
+    u64 w[4], s = 0;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int at = row.index(4 * j + q);
+      w[q] = 0;
+      if (at < a.n && order_of(row.x[4 * j + q], at) <= cut) {
+        const float e = sc.e(row.x[4 * j + q]);
+        if (e >= floor_e) w[q] = weight_of(e);
+      }
+      s += w[q];
+    }
+    u64 upto = s;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
+      if (lane >= o) upto += y;
+    }
+    u64 at_mass = run + upto - s;
+    if (aim >= at_mass && aim < at_mass + s) {
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        if (aim >= at_mass && aim < at_mass + w[q]) {
+          a.token[r] = row.index(4 * j + q);
+          if (a.prob) a.prob[r] = __fdiv_rn((float)w[q], (float)total);
+        }
+        at_mass += w[q];
+      }
+    }
+    run += __shfl_sync(0xffffffffu, upto, 31);
+  }
+}
+
+template <int E>
+cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
+  auto k = sample_cluster_kernel<E>;
+  cudaError_t e = cudaSuccess;
+  if (ctas > 8 && (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = (unsigned)ctas;
+  attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+  attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[1].val.programmaticStreamSerializationAllowed = 1;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(rows * ctas));
+  cfg.blockDim = dim3(kT);
+  cfg.stream = st;
+  cfg.attrs = attr;
+  cfg.numAttrs = launch_overlap() ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, a);
+}
+
+}  // namespace cluster
+
+// ---------------------------------------------------------------------------
+// Rows past what a cluster holds: one CTA per row, every pass reads it again
+// ---------------------------------------------------------------------------
 __global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ Args a) {
   grid_dependency_wait();
   allow_dependents_launch();
@@ -274,8 +734,15 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
     if (reinterpret_cast<uintptr_t>(p) % 4)
       return hyq::api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
   const hyq::sample::Args a{logits, stride, (int)n, temperature, top_k, top_p, min_p, u, token, prob};
-  const cudaError_t e = hyq::launch_ex(hyq::sample::sample_kernel, dim3((unsigned)rows), dim3(hyq::sample::kThreads), 0,
-                                       (cudaStream_t)stream, a);
+  const cudaStream_t st = (cudaStream_t)stream;
+  namespace sc = hyq::sample::cluster;
+  cudaError_t e;
+  if (n <= sc::kT * 8)
+    e = sc::launch<8>(a, rows, 1, st);
+  else if (n <= (int64_t)sc::kT * 32 * sc::kMaxCluster && rows <= INT32_MAX / sc::kMaxCluster)
+    e = sc::launch<32>(a, rows, (int)((n + sc::kT * 32 - 1) / (sc::kT * 32)), st);
+  else
+    e = hyq::launch_ex(hyq::sample::sample_kernel, dim3((unsigned)rows), dim3(hyq::sample::kThreads), 0, st, a);
   return e == cudaSuccess ? HYQ_OK : hyq::api_fail(HYQ_E_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
