@@ -37,8 +37,104 @@ __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
   else static_cast<float*>(base)[i] = x;
 }
 
-// One CTA per row of the activations, a warp per head at a time, the head in
-// shared memory: any even head size.  Sums in the order of dot_x86.
+// One CTA per row of the activations, 16 lanes per head: lane l holds values
+// l, l + 16, ... of its head, so that the sum of squares runs in dot_x86's
+// order (one accumulator a lane, then the lane sum) and the two values of a
+// rotated pair meet in one thread: no value leaves its registers between the
+// load and the store.  Each group takes BATCH heads at a time, their loads in
+// flight together.
+template <int DIM, bool KV16>
+__global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int EL = DIM / 16, BATCH = 3;
+  grid_dependency_wait();
+  allow_dependents_launch();
+  const int t = blockIdx.x, l = threadIdx.x & 15, part = threadIdx.x >> 4;
+  const int units = a.heads + 2 * a.c.kv_heads;
+  auto source = [&](int u) {
+    return u < a.heads                    ? a.q + t * a.q_stride + u * DIM
+           : u < a.heads + a.c.kv_heads ? a.k + t * a.k_stride + (u - a.heads) * DIM
+                                          : a.v + t * a.v_stride + (u - a.heads - a.c.kv_heads) * DIM;
+  };
+  float x[BATCH][EL];
+  auto load = [&](int u0) {
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int u = u0 + 16 * b;
+      const float* src = source(u < units ? u : 0);
+#pragma unroll
+      for (int i = 0; i < EL; ++i) x[b][i] = u < units ? src[l + 16 * i] : 0.f;
+    }
+  };
+  load(part);  // these do not wait for the tables
+  float wq[EL], wk[EL];
+#pragma unroll
+  for (int i = 0; i < EL; ++i) {
+    wq[i] = a.q_norm ? a.q_norm[l + 16 * i] : 1.f;
+    wk[i] = a.k_norm ? a.k_norm[l + 16 * i] : 1.f;
+  }
+  const int s = seq_of_row(a.c, t);
+  if (s < 0) return;
+  const Seq sq = load_seq(a.c, s);
+  if (t - sq.row0 >= sq.n) return;
+  const int pos = sq.pos + (t - sq.row0);
+  const int page = checked_page(a.c, sq.pages[pos / a.c.page_size]);
+  if (page < 0 || pos >= a.positions) {
+    if (threadIdx.x == 0) atomicOr(a.c.status, DEV_BAD_ARGS);
+    return;
+  }
+  float cs[EL / 2], sn[EL / 2];
+#pragma unroll
+  for (int i = 0; i < EL / 2; ++i) {
+    cs[i] = a.cos_tab[(int64_t)pos * (DIM / 2) + l + 16 * i];
+    sn[i] = a.sin_tab[(int64_t)pos * (DIM / 2) + l + 16 * i];
+  }
+  const int64_t row = (int64_t)page * a.c.page_stride + (int64_t)(pos % a.c.page_size) * a.c.row_stride;
+  for (int u0 = part; u0 - part < units; u0 += 16 * BATCH) {
+    if (u0 != part) load(u0);
+#pragma unroll
+    for (int b = 0; b < BATCH; ++b) {
+      const int u = u0 + 16 * b;
+      if (u - part >= units) break;  // the same for the whole CTA
+      const bool rotated = u < a.heads + a.c.kv_heads, is_q = u < a.heads;
+      const float* w = is_q ? a.q_norm : a.k_norm;
+      auto norm = [&]() {
+        float acc = 0.f;
+#pragma unroll
+        for (int i = 0; i < EL; ++i) acc = fmaf(x[b][i], x[b][i], acc);
+        const float d = x86_lane_sum(acc, 0xffffffffu);
+        const float scale = __fdiv_rn(1.0f, __fsqrt_rn(__fadd_rn(__fdiv_rn(d, (float)DIM), a.eps)));
+        if (w && rotated) {
+#pragma unroll
+          for (int i = 0; i < EL; ++i) x[b][i] = __fmul_rn(__fmul_rn(x[b][i], scale), is_q ? wq[i] : wk[i]);
+        }
+      };
+      if (a.norm_first) norm();
+      if (rotated) {
+#pragma unroll
+        for (int i = 0; i < EL / 2; ++i) {
+          const float x0 = x[b][i], x1 = x[b][i + EL / 2];
+          x[b][i] = __fsub_rn(__fmul_rn(x0, cs[i]), __fmul_rn(x1, sn[i]));
+          x[b][i + EL / 2] = __fadd_rn(__fmul_rn(x0, sn[i]), __fmul_rn(x1, cs[i]));
+        }
+      }
+      if (!a.norm_first) norm();
+      if (u >= units) continue;
+      if (is_q) {
+        float* to = a.q_out + t * a.out_stride + u * DIM + l;
+#pragma unroll
+        for (int i = 0; i < EL; ++i) to[16 * i] = x[b][i];
+      } else {
+        const int kh = (u - a.heads) % a.c.kv_heads;
+        const int64_t to = row + kh * a.c.head_stride + l;
+#pragma unroll
+        for (int i = 0; i < EL; ++i) store_kv<KV16>(rotated ? a.c.k : a.c.v, to + 16 * i, x[b][i]);
+      }
+    }
+  }
+}
+
+// Any other even head size: a warp per head at a time, the head in
+// shared memory; sums in the order of dot_x86.
 template <bool KV16>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a) {
   grid_dependency_wait();
@@ -317,7 +413,11 @@ int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, 
   a.norm_first = norm_first;
   a.q_out = q_out;
   a.out_stride = out_stride;
-  auto kern = kv->dtype == HYQ_KV_F16 ? hyq::paged::append_kernel<true> : hyq::paged::append_kernel<false>;
+  using namespace hyq::paged;
+  const bool kv16 = kv->dtype == HYQ_KV_F16;
+  auto kern = kv->head_dim == 128  ? (kv16 ? append_rows_kernel<128, true> : append_rows_kernel<128, false>)
+              : kv->head_dim == 64 ? (kv16 ? append_rows_kernel<64, true> : append_rows_kernel<64, false>)
+                                   : (kv16 ? append_kernel<true> : append_kernel<false>);
   return done(hyq::launch_ex(kern, dim3((unsigned)batch->tokens), dim3(256), 0, (cudaStream_t)stream, a), name);
 }
 

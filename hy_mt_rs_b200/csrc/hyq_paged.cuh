@@ -58,15 +58,22 @@ __device__ __forceinline__ Seq load_seq(const Cache& c, int s) {
   return q;
 }
 
-// The sequence that row t belongs to (row_start ascending), or -1.
+// The sequence that row t belongs to (row_start ascending), or -1; by a whole
+// warp, 32 entries per round of loads.
 __device__ __forceinline__ int seq_of_row(const Cache& c, int t) {
-  int lo = 0, hi = c.seqs;  // the last s with row_start[s] <= t
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (c.row_start[mid] <= t) lo = mid;
-    else hi = mid - 1;
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = c.seqs + 1;  // the last entry <= t is among lo .. lo + n - 1, if any
+  while (n > 0) {
+    const int step = (n + 31) / 32, i = lo + lane * step;
+    const bool in = i < lo + n && c.row_start[i] <= t;
+    const int hits = __popc(__ballot_sync(0xffffffffu, in));  // a prefix of the lanes
+    if (hits == 0) return -1;
+    const int next = lo + (hits - 1) * step;
+    if (step == 1) return next < c.seqs ? next : -1;
+    n = min(step, lo + n - next);
+    lo = next;
   }
-  return lo < c.seqs && c.row_start[lo] <= t ? lo : -1;
+  return -1;
 }
 
 // Page of a table entry, or -1 with DEV_BAD_ARGS when it is no page of the pool.

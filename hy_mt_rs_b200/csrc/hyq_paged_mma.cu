@@ -533,7 +533,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     __syncthreads();
     constexpr int pitch = DIM + 4;
     float* o_s = reinterpret_cast<float*>(smem);  // [warp][16][pitch]
-    static_assert(kWarps * kRows * pitch * 4 <= G::smem, "the rings hold the warps' outputs");
+    static_assert(kWarps * kRows * pitch * 4 <= G::smem && kRows * kMaxCtas * 4 <= G::smem,
+                  "the rings hold the warps' outputs and a combination's weights");
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = (lane >> 2) + 8 * i;
@@ -588,25 +589,46 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
       __syncthreads();
       if (last_s) {
         __threadfence();
-        for (int x = threadIdx.x; x < live * DIM; x += kThreads) {
-          const int r = x / DIM, d = x % DIM;
-          float top = -INFINITY;
-          for (int c = cf; c <= cl; ++c) {
-            const float* p = parts + (size_t)(2 * c + (work * c / ctas < seg0)) * partial_floats(DIM);
-            top = fmaxf(top, __ldcg(p + kRows * DIM + 2 * r));
+        // partials cf .. cl, in order; only cf's may be its CTA's second
+        const int n = cl - cf + 1;
+        const float* p0 = parts + (size_t)(2 * cf + (work * cf / ctas < seg0)) * partial_floats(DIM);
+        const float* p1 = parts + (size_t)(2 * cf) * partial_floats(DIM);
+        auto part_at = [&](int i) { return i ? p1 + (size_t)(2 * i) * partial_floats(DIM) : p0; };
+        // each row's weight of each partial, a warp per row, in the rings' memory
+        float* f_s = reinterpret_cast<float*>(smem);  // [row][n]
+        for (int r = warp; r < live; r += kWarps) {
+          float top = -INFINITY, l = 0.f;
+          for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(part_at(i) + kRows * DIM + 2 * r));
+#pragma unroll
+          for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+          for (int i = lane; i < n; i += 32) {
+            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_at(i) + kRows * DIM + 2 * r));
+            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+            f_s[r * n + i] = f;
+            l = fmaf(f, ml.y, l);
           }
-          float sum = 0.f, l = 0.f;
-          for (int c = cf; c <= cl; ++c) {
-            const float* p = parts + (size_t)(2 * c + (work * c / ctas < seg0)) * partial_floats(DIM);
-            const float pm = __ldcg(p + kRows * DIM + 2 * r);
-            const float f = pm == -INFINITY ? 0.f : ex2(pm - top);
-            sum = fmaf(f, __ldcg(p + x), sum);
-            l = fmaf(f, __ldcg(p + kRows * DIM + 2 * r + 1), l);
+          l = warp_sum(l);
+          if (lane == 0) ml_s[0][r][1] = 1.0f / l;
+        }
+        __syncthreads();
+        for (int x = threadIdx.x; x < live * (DIM / 4); x += kThreads) {
+          const int r = x / (DIM / 4), d = 4 * (x % (DIM / 4));
+          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 8
+          for (int i = 0; i < n; ++i) {
+            const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(i) + r * DIM + d));
+            const float f = f_s[r * n + i];
+            sum.x = fmaf(f, v.x, sum.x);
+            sum.y = fmaf(f, v.y, sum.y);
+            sum.z = fmaf(f, v.z, sum.z);
+            sum.w = fmaf(f, v.w, sum.w);
           }
           const int tok = r / group;
-          float y = sum / l;
-          if (s.n > 1) y += unseen<KV16>(a, s, kvh, 0, tok, d);
-          a.out[(int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + d] = y;
+          float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + d;
+          const float inv = ml_s[0][r][1];
+          const float y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+#pragma unroll
+          for (int k = 0; k < 4; ++k) to[k] = s.n > 1 ? y[k] + unseen<KV16>(a, s, kvh, 0, tok, d + k) : y[k];
         }
         if (threadIdx.x == 0) counters[cf] = 0;
       }

@@ -4,7 +4,9 @@
 // token.
 #include <cuda_runtime.h>
 
+#include <algorithm>
 #include <cstdint>
+#include <cstdlib>
 
 #include "../../include/hyq.h"
 #include "hyq_common.cuh"
@@ -62,17 +64,17 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 }
 
 // ---------------------------------------------------------------------------
-// Rows held in registers by a cluster of CTAs
+// Rows held in shared memory by a cluster of CTAs
 // ---------------------------------------------------------------------------
 //
-// The row is read from memory once: each thread keeps E logits.  What the
-// CTAs of a row tell one another goes through distributed shared memory, one
-// cluster barrier per exchange:
+// The row is read from memory once, a slice per CTA.  What the CTAs of a row
+// tell one another goes through distributed shared memory, one cluster
+// barrier per exchange:
 //   1. the largest logit (with its index: the greedy token) and the smallest;
 //   2. with top-k or top-p, a histogram of z = (max - logit) / temperature
 //      over at most 28 (past it a weight is 0: e^-28 < 2^-40) in 512 equal
-//      bins, counts and masses; every CTA adds up all of them and finds the
-//      bin in which the k-th logit, or the top_p of the mass, falls;
+//      bins; every CTA adds up all of them and finds the bin in which the
+//      k-th logit, or the top_p of the mass, falls;
 //   3. that bin's few logits, listed in every CTA, which ranks them by value
 //      and index: the last one kept is the cut.  A bin with more than kList
 //      (ties, a wide row) is divided again by the bits of the key, then by
@@ -82,10 +84,12 @@ namespace cluster {
 
 constexpr int kT = 512;                // threads of a CTA
 constexpr int kW = kT / 32;
+constexpr int kUnit = kT * 4;          // a slice is whole groups of 128 per warp
 constexpr int kBins = 512;
 static_assert(kBins == kT, "one bin per thread");
 constexpr int kList = 1024;
 constexpr int kMaxCluster = 16;
+constexpr int kMaxSlice = 24 * kUnit;  // floats: 192 KB
 constexpr float kSpan = 28.0f;
 
 __device__ __forceinline__ unsigned ctarank() {
@@ -117,31 +121,43 @@ __device__ __forceinline__ unsigned get32(uint32_t a) {
 }
 
 struct Shared {
-  // counts, and the masses in parts of 14 bits (sums of 16,384 stay below
-  // 2^32; shared 32-bit atomics are native, 64-bit ones are not)
+  // counts, and the masses in parts of 14, 14 and 13 bits (a slice's sums stay
+  // below 2^32; shared 32-bit atomics are native, 64-bit ones are not)
   unsigned hist[4][kBins];
-  u64 list[kList];              // ~key << 32 | index: ascending = kept first
+  u64 list[kList];              // the order of a part's tokens
   u64 max_of[kMaxCluster];      // key << 32 | ~index
   u64 min_of[kMaxCluster];
   u64 mass_of[kMaxCluster];
   u64 warp_a[kW], warp_b[kW];
-  unsigned fill;                // this CTA's entries in the list
+  unsigned fill;                // entries of the list so far
   unsigned bin;
   u64 above_n, above_w, in_n;
-  u64 cut;
 };
+static_assert((u64)kMaxSlice << 14 < 1ull << 32, "sums of 14-bit parts");
 
-template <int E>
-struct Row {
-  float x[E];
-  int base;   // index of x[4 j + k]: base + 128 j + 4 lane + k
-  int n;
-
-  __device__ __forceinline__ int index(int i) const { return base + 128 * (i >> 2) + 4 * (threadIdx.x & 31) + (i & 3); }
+// This thread's logits: four at a time, index() + 0 .. 3, in the order of the
+// row within a warp.
+struct Slice {
+  const float* x;  // shared, the warp's part
+  int first;       // index in the row of this thread's first four
+  int n, groups;
+  __device__ __forceinline__ float4 at(int j) const { return reinterpret_cast<const float4*>(x)[32 * j + (threadIdx.x & 31)]; }
+  __device__ __forceinline__ int index(int j) const { return first + 128 * j; }
+  // f(logit, index) for each
+  template <typename F>
+  __device__ __forceinline__ void each(F f) const {
+    for (int j = 0; j < groups; ++j) {
+      const int i = index(j);
+      const float4 v = at(j);
+      if (i < n) f(v.x, i);
+      if (i + 1 < n) f(v.y, i + 1);
+      if (i + 2 < n) f(v.z, i + 2);
+      if (i + 3 < n) f(v.w, i + 3);
+    }
+  }
 };
 
 struct Scale {
-  unsigned max_key;
   float max, inverse, bins;
   __device__ __forceinline__ float e(float x) const {
     return x == max ? 1.0f : expf(__fmul_rn(__fsub_rn(x, max), inverse));
@@ -156,17 +172,18 @@ struct Scale {
 // Order of the tokens: larger logits first, ties by index.
 __device__ __forceinline__ u64 order_of(float x, int index) { return ((u64)~key_of(x) << 32) | (unsigned)index; }
 
-// Which part of a bin is meant: a z bin, then (level > 0) leading bits of the
-// order, 9 at a time.
+// Which part of the row is divided next: all of it by z, or a z bin and leading
+// bits of the order, 9 at a time.
 struct Part {
   unsigned zbin;
   u64 prefix, mask;
-  int shift;     // of the next 9 bits; 64: by z
+  int shift;  // of the next 9 bits; 64: by z
 };
 
-__device__ __forceinline__ unsigned sub_bin(const Scale& sc, const Part& p, float x, u64 order) {
+__device__ __forceinline__ unsigned sub_bin(const Scale& sc, const Part& p, float x, int index) {
   const unsigned z = sc.bin(x);
   if (p.shift == 64) return z;
+  const u64 order = order_of(x, index);
   if (z != p.zbin || (order & p.mask) != p.prefix) return kBins;
   return (unsigned)(order >> p.shift) & (kBins - 1);
 }
@@ -197,116 +214,86 @@ __device__ __forceinline__ void scan2(Shared& sh, u64 a, u64 b, u64& before_a, u
   }
 }
 
-// The cut: the last token kept when the kept ones are cut either to the first
-// `want` (BY_MASS false) or to those whose predecessors weigh less than
-// `want`.  Tokens past `limit` (an earlier cut) do not count.  Returns the
-// order of the last one kept, and the mass of all kept in `mass`; ~0 when the
-// whole row weighs or counts less.
-template <int E, bool BY_MASS>
-__device__ u64 find_cut(Shared& sh, const Row<E>& row, const Scale& sc, u64 limit, u64 want, u64& mass) {
+// The cut: the last token kept when the tokens up to `limit` (an earlier cut)
+// are cut either to the first `want` (BY_MASS false) or to those whose
+// predecessors weigh less than `want`.  Returns its order; `limit` when they
+// count or weigh less.
+template <bool BY_MASS>
+__device__ u64 find_cut(Shared& sh, const Slice& row, const Scale& sc, u64 limit, u64 want) {
   const unsigned rank = ctarank(), ctas = nctas();
   u64 above_n = 0, above_w = 0;  // tokens before the part, their mass
   Part part{0, 0, 0, 64};
+  // (8 levels divide a 64-bit order to single tokens; the bound is for safety)
   for (int level = 0; level < 10; ++level) {
-    for (int i = threadIdx.x; i < 4 * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
-    if (threadIdx.x == 0) {
-      sh.fill = 0;
-      sh.bin = kBins;
-    }
+    for (int i = threadIdx.x; i < (BY_MASS ? 4 : 1) * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
+    if (threadIdx.x == 0) sh.bin = kBins;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < E; ++i) {
-      const int at = row.index(i);
-      if (at < row.n) {
-        const u64 order = order_of(row.x[i], at);
-        const unsigned b = sub_bin(sc, part, row.x[i], order);
-        if (b < kBins && order <= limit) {
-          const u64 w = weight_of(sc.e(row.x[i]));
-          atomicAdd(&sh.hist[0][b], 1u);
-          atomicAdd(&sh.hist[1][b], (unsigned)(w & 0x3fff));
-          atomicAdd(&sh.hist[2][b], (unsigned)(w >> 14 & 0x3fff));
-          atomicAdd(&sh.hist[3][b], (unsigned)(w >> 28));
-        }
+    row.each([&](float x, int i) {
+      const unsigned b = sub_bin(sc, part, x, i);
+      if (b >= kBins || order_of(x, i) > limit) return;
+      if constexpr (BY_MASS) {
+        const u64 w = weight_of(sc.e(x));
+        if (w == 0) return;
+        atomicAdd(&sh.hist[1][b], (unsigned)(w & 0x3fff));
+        atomicAdd(&sh.hist[2][b], (unsigned)(w >> 14 & 0x3fff));
+        atomicAdd(&sh.hist[3][b], (unsigned)(w >> 28));
       }
-    }
+      atomicAdd(&sh.hist[0][b], 1u);
+    });
     barrier();
-    u64 count = 0, weight = 0, lower = 0;  // of this thread's bin; entries of the CTAs before this one
+    u64 count = 0, weight = 0, lower = 0;  // of this thread's bin; its tokens in the CTAs before this one
+#pragma unroll 4
     for (unsigned c = 0; c < ctas; ++c) {
       const uint32_t h = remote(&sh.hist[0][threadIdx.x], c);
       const unsigned k = get32(h);
       if (c < rank) lower += k;
       count += k;
-      weight += (u64)get32(h + 4 * kBins) + ((u64)get32(h + 8 * kBins) << 14) + ((u64)get32(h + 12 * kBins) << 28);
+      if constexpr (BY_MASS)
+        weight += (u64)get32(h + 4 * kBins) + ((u64)get32(h + 8 * kBins) << 14) + ((u64)get32(h + 12 * kBins) << 28);
     }
     u64 before_n, before_w;
     scan2(sh, count, weight, before_n, before_w);
     before_n += above_n;
     before_w += above_w;
-    const bool here = BY_MASS ? before_w < want && before_w + weight >= want : before_n < want && before_n + count >= want;
-    if (here) {
+    if (BY_MASS ? before_w < want && before_w + weight >= want : before_n < want && before_n + count >= want) {
       sh.bin = threadIdx.x;
       sh.above_n = before_n;
       sh.above_w = before_w;
       sh.in_n = count;
       sh.fill = (unsigned)min(lower, (u64)kList);
     }
-    if (threadIdx.x == kT - 1) sh.cut = before_w + weight;
     __syncthreads();
     const unsigned b = sh.bin;
-    if (b == kBins) {  // only at the first level: the row has less than that
-      mass = sh.cut;
-      return ~0ull;
-    }
+    if (b == kBins) return limit;  // (at the first level only)
     above_n = sh.above_n;
     above_w = sh.above_w;
-    const u64 inside = sh.in_n;
-    if (inside <= kList) {
-      __syncthreads();
-#pragma unroll
-      for (int i = 0; i < E; ++i) {
-        const int at = row.index(i);
-        if (at < row.n) {
-          const u64 order = order_of(row.x[i], at);
-          if (order <= limit && sub_bin(sc, part, row.x[i], order) == b) {
-            const unsigned slot = atomicAdd(&sh.fill, 1u);
-            for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order);
-          }
-        }
-      }
+    const int m = (int)min(sh.in_n, (u64)kList + 1);
+    if (m <= kList) {
+      row.each([&](float x, int i) {
+        if (sub_bin(sc, part, x, i) != b) return;
+        const u64 order = order_of(x, i);
+        if (order > limit || (BY_MASS && weight_of(sc.e(x)) == 0)) return;
+        const unsigned slot = atomicAdd(&sh.fill, 1u);
+        if (slot < kList)
+          for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order);
+      });
       barrier();
-      // rank and mass before each of the part's tokens
-      const int m = (int)inside;
-      u64 total = 0, last = 0;
+      // place of each of the part's tokens, or the mass before it
+      u64 last = 0;
       for (int t = threadIdx.x; t < m; t += kT) {
         const u64 mine = sh.list[t];
-        u64 before = above_w;
-        u64 place = above_n;
+        u64 before = BY_MASS ? above_w : above_n;
         for (int j = 0; j < m; ++j) {
           const u64 other = sh.list[j];
-          if (other < mine) {
-            ++place;
-            if (BY_MASS) before += weight_of(sc.e(value_of(~(unsigned)(other >> 32))));
-          }
+          if (other < mine) before += BY_MASS ? weight_of(sc.e(value_of(~(unsigned)(other >> 32)))) : 1;
         }
-        if (BY_MASS ? before < want : place < want) {
-          total += weight_of(sc.e(value_of(~(unsigned)(mine >> 32))));
-          last = max(last, mine);
-        }
+        if (before < want) last = max(last, mine);
       }
-      total = warp_sum_u64(total);
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+      if ((threadIdx.x & 31) == 0) sh.warp_a[threadIdx.x >> 5] = last;
       __syncthreads();
-      if ((threadIdx.x & 31) == 0) {
-        sh.warp_a[threadIdx.x >> 5] = total;
-        sh.warp_b[threadIdx.x >> 5] = last;
-      }
-      __syncthreads();
-      mass = above_w;
-      for (int w = 0; w < kW; ++w) {
-        mass += sh.warp_a[w];
-        last = max(last, sh.warp_b[w]);
-      }
+      for (int w = 0; w < kW; ++w) last = max(last, sh.warp_a[w]);
       __syncthreads();
       return last;
     }
@@ -320,46 +307,75 @@ __device__ u64 find_cut(Shared& sh, const Row<E>& row, const Scale& sc, u64 limi
       part.shift = part.shift >= 9 ? part.shift - 9 : 0;
     }
   }
-  return ~0ull;
+  return limit;
 }
 
-template <int E>
-__global__ void __launch_bounds__(kT, 2) sample_cluster_kernel(const __grid_constant__ Args a) {
+// Mass of the tokens up to `cut` with e >= floor: of this thread's warp and of
+// the warps and CTAs before it; returns the row's.
+__device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice& row, const Scale& sc, u64 cut, float floor_e,
+                                         u64& before, u64& mine) {
+  const unsigned rank = ctarank(), ctas = nctas();
+  const int warp = threadIdx.x >> 5;
+  u64 m = 0;
+  row.each([&](float x, int i) {
+    if (order_of(x, i) > cut) return;
+    const float e = sc.e(x);
+    if (e >= floor_e) m += weight_of(e);
+  });
+  mine = warp_sum_u64(m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.warp_a[warp] = mine;
+  __syncthreads();
+  if (threadIdx.x < ctas) {
+    m = 0;
+    for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
+    put64(remote(&sh.mass_of[rank], threadIdx.x), m);
+  }
+  barrier();
+  u64 total = 0;
+  before = 0;
+  for (unsigned c = 0; c < ctas; ++c) {
+    if (c == rank) before = total;
+    total += sh.mass_of[c];
+  }
+  for (int w = 0; w < warp; ++w) before += sh.warp_a[w];
+  return total;
+}
+
+__global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constant__ Args a, int slice) {
   grid_dependency_wait();
   allow_dependents_launch();
   __shared__ Shared sh;
+  extern __shared__ __align__(16) float x_s[];
   const unsigned rank = ctarank(), ctas = nctas();
   const int r = blockIdx.x / ctas, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float* x = a.logits + r * a.stride;
-  Row<E> row;
-  row.n = a.n;
-  row.base = ((int)rank * kW + warp) * 32 * E;
+  const int share = slice / kW;  // of a warp
+  float* mine_s = x_s + warp * share;
+  const Slice row{mine_s, (int)rank * slice + warp * share + 4 * lane, a.n, share / 128};
   u64 top = 0, low = ~0ull;
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-#pragma unroll
-  for (int j = 0; j < E / 4; ++j) {
-    const int at = row.index(4 * j);
-    if (vec && at + 4 <= a.n) {
-      const float4 v = __ldcs(reinterpret_cast<const float4*>(x + at));
-      row.x[4 * j] = v.x;
-      row.x[4 * j + 1] = v.y;
-      row.x[4 * j + 2] = v.z;
-      row.x[4 * j + 3] = v.w;
+#pragma unroll 4
+  for (int j = 0; j < row.groups; ++j) {
+    const int i = row.index(j);
+    float v[4];
+    if (vec && i + 4 <= a.n) {
+      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
+      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
     } else {
 #pragma unroll
-      for (int k = 0; k < 4; ++k) row.x[4 * j + k] = at + k < a.n ? __ldcs(x + at + k) : -INFINITY;
+      for (int k = 0; k < 4; ++k) v[k] = i + k < a.n ? __ldcs(x + i + k) : -INFINITY;
     }
-  }
 #pragma unroll
-  for (int i = 0; i < E; ++i) {
-    if (isnan(row.x[i])) row.x[i] = -INFINITY;
-    if (row.x[i] == 0.0f) row.x[i] = 0.0f;  // -0 as +0
-    const int at = row.index(i);
-    if (at < a.n) {
-      const u64 k = (u64)key_of(row.x[i]) << 32;
-      top = max(top, k | (unsigned)~at);
-      low = min(low, k);
+    for (int k = 0; k < 4; ++k) {
+      if (isnan(v[k])) v[k] = -INFINITY;
+      if (i + k < a.n) {
+        const u64 key = (u64)key_of(v[k]) << 32;
+        top = max(top, key | (unsigned)~(i + k));
+        low = min(low, key);
+      }
     }
+    reinterpret_cast<float4*>(mine_s)[32 * j + lane] = make_float4(v[0], v[1], v[2], v[3]);
   }
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
@@ -370,8 +386,7 @@ __global__ void __launch_bounds__(kT, 2) sample_cluster_kernel(const __grid_cons
     sh.warp_a[warp] = top;
     sh.warp_b[warp] = low;
   }
-  // every CTA of the cluster runs before its shared memory is written to
-  barrier();
+  barrier();  // every CTA of the cluster runs before its shared memory is written to
   if (threadIdx.x < ctas) {
     for (int w = 0; w < kW; ++w) {
       top = max(top, sh.warp_a[w]);
@@ -388,8 +403,7 @@ __global__ void __launch_bounds__(kT, 2) sample_cluster_kernel(const __grid_cons
     low = min(low, sh.min_of[c]);
   }
   Scale sc;
-  sc.max_key = (unsigned)(top >> 32);
-  sc.max = value_of(sc.max_key);
+  sc.max = value_of((unsigned)(top >> 32));
   const float temperature = a.temperature ? a.temperature[r] : 1.0f;
   if (sc.max == -INFINITY || !(temperature > 0.0f)) {
     if (rank == 0 && threadIdx.x == 0) {
@@ -404,74 +418,30 @@ __global__ void __launch_bounds__(kT, 2) sample_cluster_kernel(const __grid_cons
   const int k = a.top_k ? a.top_k[r] : 0;
   const float p = a.top_p ? a.top_p[r] : 1.0f;
   const float floor_e = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
-  u64 cut = ~0ull, mass = 0;
-  if (k > 0 && k < a.n) cut = find_cut<E, false>(sh, row, sc, cut, (u64)k, mass);
+  u64 cut = ~0ull, before, mine;
+  if (k > 0 && k < a.n) cut = find_cut<false>(sh, row, sc, cut, (u64)k);
   if (p < 1.0f) {
-    if (cut == ~0ull) {
-      // nothing cut so far: the whole row's mass
-      u64 m = 0;
-#pragma unroll
-      for (int i = 0; i < E; ++i)
-        if (row.index(i) < a.n) m += weight_of(sc.e(row.x[i]));
-      m = warp_sum_u64(m);
-      __syncthreads();
-      if (lane == 0) sh.warp_a[warp] = m;
-      __syncthreads();
-      if (threadIdx.x < ctas) {
-        m = 0;
-        for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
-        put64(remote(&sh.mass_of[rank], threadIdx.x), m);
-      }
-      barrier();
-      mass = 0;
-      for (unsigned c = 0; c < ctas; ++c) mass += sh.mass_of[c];
-    }
-    const u64 share = (u64)ceilf(__fmul_rn(fmaxf(p, 0.0f), 16777216.0f));
-    const u64 want = max(scaled(mass, share, (1u << kGrid) - 1), 1ull);
-    u64 ignored;
-    barrier();  // mass_of and the histograms may be written again
-    cut = min(cut, find_cut<E, true>(sh, row, sc, cut, want, ignored));
+    const u64 mass = mass_upto(sh, row, sc, cut, 0.0f, before, mine);
+    const u64 share_p = (u64)ceilf(__fmul_rn(fmaxf(p, 0.0f), 16777216.0f));
+    cut = find_cut<true>(sh, row, sc, cut, max(scaled(mass, share_p, (1u << kGrid) - 1), 1ull));
   }
-  // kept mass of each thread, warp and CTA
-  u64 mine = 0;
-#pragma unroll
-  for (int i = 0; i < E; ++i) {
-    const int at = row.index(i);
-    if (at < a.n && order_of(row.x[i], at) <= cut) {
-      const float e = sc.e(row.x[i]);
-      if (e >= floor_e) mine += weight_of(e);
-    }
-  }
-  const u64 warp_mass = warp_sum_u64(mine);
-  __syncthreads();
-  if (lane == 0) sh.warp_a[warp] = warp_mass;
-  barrier();  // mass_of may be written again
-  if (threadIdx.x < ctas) {
-    u64 m = 0;
-    for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
-    put64(remote(&sh.mass_of[rank], threadIdx.x), m);
-  }
-  barrier();
-  u64 total = 0, run = 0;
-  for (unsigned c = 0; c < ctas; ++c) {
-    if (c == rank) run = total;
-    total += sh.mass_of[c];
-  }
+  const u64 total = mass_upto(sh, row, sc, cut, floor_e, before, mine);
   const float uf = fminf(fmaxf(a.u[r], 0.0f), 1.0f);
   const u64 ui = min((u64)__fmul_rn(uf, 16777216.0f), (u64)(1u << kGrid) - 1);
   const u64 aim = scaled(total, ui, 0);
-  for (int w = 0; w < warp; ++w) run += sh.warp_a[w];
-  if (aim < run || aim >= run + warp_mass) return;
+  if (aim < before || aim >= before + mine) return;
   // this warp holds the token: index order is group by group of 128
-#pragma unroll
-  for (int j = 0; j < E / 4; ++j) {
+  u64 run = before;
+  for (int j = 0; j < row.groups; ++j) {
+    const float4 f = row.at(j);
+    const float v[4] = {f.x, f.y, f.z, f.w};
     u64 w[4], s = 0;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
-      const int at = row.index(4 * j + q);
+      const int i = row.index(j) + q;
       w[q] = 0;
-      if (at < a.n && order_of(row.x[4 * j + q], at) <= cut) {
-        const float e = sc.e(row.x[4 * j + q]);
+      if (i < a.n && order_of(v[q], i) <= cut) {
+        const float e = sc.e(v[q]);
         if (e >= floor_e) w[q] = weight_of(e);
       }
       s += w[q];
@@ -482,25 +452,27 @@ __global__ void __launch_bounds__(kT, 2) sample_cluster_kernel(const __grid_cons
       const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
       if (lane >= o) upto += y;
     }
-    u64 at_mass = run + upto - s;
-    if (aim >= at_mass && aim < at_mass + s) {
+    u64 at = run + upto - s;
+    if (aim >= at && aim < at + s) {
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        if (aim >= at_mass && aim < at_mass + w[q]) {
-          a.token[r] = row.index(4 * j + q);
+        if (aim >= at && aim < at + w[q]) {
+          a.token[r] = row.index(j) + q;
           if (a.prob) a.prob[r] = __fdiv_rn((float)w[q], (float)total);
         }
-        at_mass += w[q];
+        at += w[q];
       }
     }
     run += __shfl_sync(0xffffffffu, upto, 31);
+    if (aim < run) return;
   }
 }
 
-template <int E>
 cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
-  auto k = sample_cluster_kernel<E>;
-  cudaError_t e = cudaSuccess;
+  auto k = sample_cluster_kernel;
+  const int slice = ((a.n + ctas - 1) / ctas + kUnit - 1) / kUnit * kUnit;
+  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * (int)sizeof(float));
+  if (e != cudaSuccess) return e;
   if (ctas > 8 && (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
@@ -511,10 +483,11 @@ cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(kT);
+  cfg.dynamicSmemBytes = slice * sizeof(float);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = launch_overlap() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, k, a);
+  return cudaLaunchKernelEx(&cfg, k, a, slice);
 }
 
 }  // namespace cluster
@@ -737,10 +710,11 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
   const cudaStream_t st = (cudaStream_t)stream;
   namespace sc = hyq::sample::cluster;
   cudaError_t e;
-  if (n <= sc::kT * 8)
-    e = sc::launch<8>(a, rows, 1, st);
-  else if (n <= (int64_t)sc::kT * 32 * sc::kMaxCluster && rows <= INT32_MAX / sc::kMaxCluster)
-    e = sc::launch<32>(a, rows, (int)((n + sc::kT * 32 - 1) / (sc::kT * 32)), st);
+  static const char* tune = getenv("HYQ_TUNE_C");
+  const int want = tune ? atoi(tune) : 8;
+  const int ctas = (int)std::max<int64_t>(std::min<int64_t>(want, (n + sc::kUnit - 1) / sc::kUnit), (n + sc::kMaxSlice - 1) / sc::kMaxSlice);
+  if (ctas <= sc::kMaxCluster && rows <= INT32_MAX / sc::kMaxCluster)
+    e = sc::launch(a, rows, ctas, st);
   else
     e = hyq::launch_ex(hyq::sample::sample_kernel, dim3((unsigned)rows), dim3(hyq::sample::kThreads), 0, st, a);
   return e == cudaSuccess ? HYQ_OK : hyq::api_fail(HYQ_E_CUDA, "%s: %s", name, cudaGetErrorString(e));
