@@ -70,16 +70,18 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 // The row is read from memory once, a slice per CTA.  What the CTAs of a row
 // tell one another goes through distributed shared memory, one cluster
 // barrier per exchange:
-//   1. the largest logit (with its index: the greedy token) and the smallest;
+//   1. the largest and the smallest logit;
 //   2. with top-k or top-p, a histogram of z = (max - logit) / temperature
 //      over at most 28 (past it a weight is 0: e^-28 < 2^-40) in 512 equal
 //      bins; every CTA adds up all of them and finds the bin in which the
 //      k-th logit, or the top_p of the mass, falls;
-//   3. that bin's few logits, listed in every CTA, which ranks them by value
-//      and index: the last one kept is the cut.  A bin with more than kList
-//      (ties, a wide row) is divided again by the bits of the key, then by
-//      index, until it fits;
-//   4. each CTA's kept mass: the one that holds the draw walks its part.
+//   3. the tokens up to that bin, usually a few hundred at most, go to the
+//      first CTA of the cluster, which sorts them and finishes the row alone.
+// Where they are more than kList (a wide nucleus, ties), the exact cut is
+// found over the whole cluster instead: the bin's own tokens, listed in every
+// CTA, are ranked by value and index; a bin with too many is divided again by
+// the bits of the key, then by index.  Then each CTA adds up its kept mass,
+// and the one that holds the draw walks its part.
 namespace cluster {
 
 constexpr int kT = 512;                // threads of a CTA
@@ -87,7 +89,8 @@ constexpr int kW = kT / 32;
 constexpr int kUnit = kT * 4;          // a slice is whole groups of 128 per warp
 constexpr int kBins = 512;
 static_assert(kBins == kT, "one bin per thread");
-constexpr int kList = 1024;
+constexpr int kList = 2048;            // tokens the first CTA sorts
+constexpr int kRanked = 1024;          // tokens ranked pair by pair
 constexpr int kMaxCluster = 16;
 constexpr int kMaxSlice = 24 * kUnit;  // floats: 192 KB
 constexpr float kSpan = 28.0f;
@@ -114,6 +117,9 @@ __device__ __forceinline__ uint32_t remote(const void* p, unsigned rank) {
 __device__ __forceinline__ void put64(uint32_t a, u64 v) {
   asm volatile("st.shared::cluster.u64 [%0], %1;" ::"r"(a), "l"(v) : "memory");
 }
+__device__ __forceinline__ void put32(uint32_t a, unsigned v) {
+  asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
+}
 __device__ __forceinline__ unsigned get32(uint32_t a) {
   unsigned v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -125,14 +131,15 @@ struct Shared {
   // below 2^32; shared 32-bit atomics are native, 64-bit ones are not)
   unsigned hist[4][kBins];
   u64 list[kList];              // the order of a part's tokens
-  u64 max_of[kMaxCluster];      // key << 32 | ~index
-  u64 min_of[kMaxCluster];
+  float max_of[kMaxCluster], min_of[kMaxCluster];
+  unsigned first_of[kMaxCluster];
   u64 mass_of[kMaxCluster];
   u64 warp_a[kW], warp_b[kW];
   unsigned fill;                // entries of the list so far
   unsigned bin;
   u64 above_n, above_w, in_n;
 };
+static_assert(2 * kUnit * sizeof(float) >= kList * sizeof(u64), "the masses of a sorted list");
 static_assert((u64)kMaxSlice << 14 < 1ull << 32, "sums of 14-bit parts");
 
 // This thread's logits: four at a time, index() + 0 .. 3, in the order of the
@@ -162,10 +169,11 @@ struct Scale {
   __device__ __forceinline__ float e(float x) const {
     return x == max ? 1.0f : expf(__fmul_rn(__fsub_rn(x, max), inverse));
   }
-  // monotone in the logit; kBins and more: no weight
+  // (max - x) / temperature in bins, to the nearest whole number (the sum with
+  // 2^23 rounds it into the low bits): monotone in the logit; kBins and more:
+  // no weight.  `bins` carries the 1 / temperature.
   __device__ __forceinline__ unsigned bin(float x) const {
-    if (x == max) return 0;
-    return (unsigned)fminf(__fmul_rn(__fmul_rn(__fsub_rn(max, x), inverse), bins), 4.0f * kBins);
+    return __float_as_uint(fminf(__fmul_rn(__fsub_rn(max, x), bins), 4.0f * kBins) + 8388608.0f) & 0x7fffffu;
   }
 };
 
@@ -260,21 +268,21 @@ __device__ u64 find_cut(Shared& sh, const Slice& row, const Scale& sc, u64 limit
       sh.above_n = before_n;
       sh.above_w = before_w;
       sh.in_n = count;
-      sh.fill = (unsigned)min(lower, (u64)kList);
+      sh.fill = (unsigned)min(lower, (u64)kRanked);
     }
     __syncthreads();
     const unsigned b = sh.bin;
     if (b == kBins) return limit;  // (at the first level only)
     above_n = sh.above_n;
     above_w = sh.above_w;
-    const int m = (int)min(sh.in_n, (u64)kList + 1);
-    if (m <= kList) {
+    const int m = (int)min(sh.in_n, (u64)kRanked + 1);
+    if (m <= kRanked) {
       row.each([&](float x, int i) {
         if (sub_bin(sc, part, x, i) != b) return;
         const u64 order = order_of(x, i);
         if (order > limit || (BY_MASS && weight_of(sc.e(x)) == 0)) return;
         const unsigned slot = atomicAdd(&sh.fill, 1u);
-        if (slot < kList)
+        if (slot < kRanked)
           for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order);
       });
       barrier();
@@ -342,6 +350,134 @@ __device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice& row, const Sca
   return total;
 }
 
+// Exclusive sum over the CTA of one value per thread; `total` of all.
+__device__ __forceinline__ u64 scan1(Shared& sh, u64 a, u64& total) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  u64 x = a;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const u64 p = __shfl_up_sync(0xffffffffu, x, o);
+    if (lane >= o) x += p;
+  }
+  __syncthreads();
+  if (lane == 31) sh.warp_a[warp] = x;
+  __syncthreads();
+  u64 before = x - a;
+  total = 0;
+#pragma unroll
+  for (int w = 0; w < kW; ++w) {
+    if (w == warp) before += total;
+    total += sh.warp_a[w];
+  }
+  return before;
+}
+
+// Bitonic sort of list[0 .. n), n a power of two from 64 to kList, ascending,
+// by the CTA.  A warp's pairs at distances up to 32 stay inside its own 64
+// entries (per 512 threads' turn), so only the longer ones meet at a barrier.
+__device__ __forceinline__ void sort_list(u64* list, int n) {
+  for (int size = 2; size <= n; size <<= 1)
+    for (int dist = size >> 1; dist > 0; dist >>= 1) {
+      if (dist >= 32) __syncthreads();
+      else __syncwarp();
+      for (int t = threadIdx.x; t < n / 2; t += kT) {
+        const int i = 2 * t - (t & (dist - 1)), j = i + dist;
+        const u64 a = list[i], b = list[j];
+        if ((a > b) == ((i & size) == 0)) {
+          list[i] = b;
+          list[j] = a;
+        }
+      }
+      if (dist >= 32) __syncthreads();
+    }
+  __syncthreads();
+}
+
+// The rest of a row by one CTA: list[0 .. m) holds the order of every token
+// that can be kept.  `k`: keep at most that many; `want`: then those whose
+// predecessors weigh less (0: not yet known, top_p of what k keeps).
+__device__ void finish(Shared& sh, u64* mass_s, const Scale& sc, const Args& a, int r, int m, int k, u64 want,
+                       bool by_mass, u64 share_p, float floor_e) {
+  int n = 64;
+  while (n < m) n <<= 1;
+  for (int t = m + threadIdx.x; t < n; t += kT) sh.list[t] = ~0ull;
+  __syncthreads();
+  sort_list(sh.list, n);
+  // consecutive tokens per thread
+  const int per = (n + kT - 1) / kT, t0 = threadIdx.x * per;
+  constexpr int kPer = kList / kT;
+  u64 w[kPer], mine = 0;
+  float e[kPer];
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const int t = t0 + q;
+    const bool in = q < per && t < m && t < k;
+    e[q] = in ? sc.e(value_of(~(unsigned)(sh.list[t] >> 32))) : -1.0f;
+    w[q] = in ? weight_of(e[q]) : 0;
+    mine += w[q];
+  }
+  u64 total;
+  u64 before = scan1(sh, mine, total);
+  if (by_mass && want == 0) want = max(scaled(total, share_p, (1u << kGrid) - 1), 1ull);
+  mine = 0;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const u64 v = w[q];
+    if (e[q] < floor_e || (by_mass && before >= want)) w[q] = 0;
+    before += v;
+    mine += w[q];
+  }
+  __syncthreads();
+  // the kept ones in the order of their indexes
+#pragma unroll
+  for (int q = 0; q < kPer; ++q)
+    if (q < per && t0 + q < n) {
+      mass_s[t0 + q] = w[q];
+      sh.list[t0 + q] = w[q] ? (sh.list[t0 + q] << 32) | (unsigned)(t0 + q) : ~0ull;
+    }
+  scan1(sh, mine, total);
+  sort_list(sh.list, n);
+  const float uf = fminf(fmaxf(a.u[r], 0.0f), 1.0f);
+  const u64 ui = min((u64)__fmul_rn(uf, 16777216.0f), (u64)(1u << kGrid) - 1);
+  const u64 aim = scaled(total, ui, 0);
+  mine = 0;
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const u64 entry = q < per && t0 + q < n ? sh.list[t0 + q] : ~0ull;
+    w[q] = entry == ~0ull ? 0 : mass_s[(unsigned)entry];
+    mine += w[q];
+  }
+  u64 ignored;
+  before = scan1(sh, mine, ignored);
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    if (aim >= before && aim < before + w[q]) {
+      a.token[r] = (int)(sh.list[t0 + q] >> 32);
+      if (a.prob) a.prob[r] = __fdiv_rn((float)w[q], (float)total);
+    }
+    before += w[q];
+  }
+}
+
+// The bin up to which the first k logits of the row lie, at least: the k-th
+// largest of the threads' own maxima (this CTA alone holds k logits there).
+__device__ __forceinline__ unsigned local_bound(Shared& sh, const Scale& sc, float thread_max, int k) {
+  sh.hist[0][threadIdx.x] = 0;
+  if (threadIdx.x == 0) sh.bin = kBins - 1;
+  __syncthreads();
+  const unsigned b = sc.bin(thread_max);
+  if (b < kBins) atomicAdd(&sh.hist[0][b], 1u);
+  __syncthreads();
+  const u64 count = sh.hist[0][threadIdx.x];
+  u64 total;
+  const u64 before = scan1(sh, count, total);
+  if (before < (u64)k && before + count >= (u64)k) sh.bin = threadIdx.x;
+  __syncthreads();
+  const unsigned bound = sh.bin;
+  __syncthreads();
+  return bound;
+}
+
 __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constant__ Args a, int slice) {
   grid_dependency_wait();
   allow_dependents_launch();
@@ -353,7 +489,7 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
   const int share = slice / kW;  // of a warp
   float* mine_s = x_s + warp * share;
   const Slice row{mine_s, (int)rank * slice + warp * share + 4 * lane, a.n, share / 128};
-  u64 top = 0, low = ~0ull;
+  float top = -INFINITY, low = INFINITY;
   const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
 #pragma unroll 4
   for (int j = 0; j < row.groups; ++j) {
@@ -369,60 +505,170 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (isnan(v[k])) v[k] = -INFINITY;
-      if (i + k < a.n) {
-        const u64 key = (u64)key_of(v[k]) << 32;
-        top = max(top, key | (unsigned)~(i + k));
-        low = min(low, key);
-      }
+      top = fmaxf(top, v[k]);
+      if (i + k < a.n) low = fminf(low, v[k]);
     }
     reinterpret_cast<float4*>(mine_s)[32 * j + lane] = make_float4(v[0], v[1], v[2], v[3]);
   }
+  const float thread_max = top;
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) {
-    top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
-    low = min(low, __shfl_xor_sync(0xffffffffu, low, o));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    low = fminf(low, __shfl_xor_sync(0xffffffffu, low, o));
   }
+  float* warp_max = reinterpret_cast<float*>(sh.warp_a);
+  float* warp_min = reinterpret_cast<float*>(sh.warp_b);
   if (lane == 0) {
-    sh.warp_a[warp] = top;
-    sh.warp_b[warp] = low;
+    warp_max[warp] = top;
+    warp_min[warp] = low;
   }
   barrier();  // every CTA of the cluster runs before its shared memory is written to
   if (threadIdx.x < ctas) {
     for (int w = 0; w < kW; ++w) {
-      top = max(top, sh.warp_a[w]);
-      low = min(low, sh.warp_b[w]);
+      top = fmaxf(top, warp_max[w]);
+      low = fminf(low, warp_min[w]);
     }
-    put64(remote(&sh.max_of[rank], threadIdx.x), top);
-    put64(remote(&sh.min_of[rank], threadIdx.x), low);
+    put32(remote(&sh.max_of[rank], threadIdx.x), __float_as_uint(top));
+    put32(remote(&sh.min_of[rank], threadIdx.x), __float_as_uint(low));
   }
   barrier();
-  top = 0;
-  low = ~0ull;
+  top = -INFINITY;
+  low = INFINITY;
   for (unsigned c = 0; c < ctas; ++c) {
-    top = max(top, sh.max_of[c]);
-    low = min(low, sh.min_of[c]);
+    top = fmaxf(top, sh.max_of[c]);
+    low = fminf(low, sh.min_of[c]);
   }
-  Scale sc;
-  sc.max = value_of((unsigned)(top >> 32));
   const float temperature = a.temperature ? a.temperature[r] : 1.0f;
-  if (sc.max == -INFINITY || !(temperature > 0.0f)) {
+  if (top == -INFINITY) {
     if (rank == 0 && threadIdx.x == 0) {
-      a.token[r] = sc.max == -INFINITY ? 0 : (int)~(unsigned)top;
-      if (a.prob) a.prob[r] = sc.max == -INFINITY ? 0.0f : 1.0f;
+      a.token[r] = 0;
+      if (a.prob) a.prob[r] = 0.0f;
     }
     return;
   }
+  if (!(temperature > 0.0f)) {  // greedy: the first index of the largest
+    unsigned first = 0xffffffffu;
+    if (thread_max == top)
+      row.each([&](float v, int i) {
+        if (v == top) first = min(first, (unsigned)i);
+      });
+    first = __reduce_min_sync(0xffffffffu, first);
+    if (threadIdx.x == 0) sh.fill = 0xffffffffu;
+    __syncthreads();
+    if (lane == 0) atomicMin(&sh.fill, first);
+    __syncthreads();
+    if (threadIdx.x == 0) put32(remote(&sh.first_of[rank], 0), sh.fill);
+    barrier();
+    if (rank == 0 && threadIdx.x == 0) {
+      for (unsigned c = 0; c < ctas; ++c) first = min(first, sh.first_of[c]);
+      a.token[r] = (int)first;
+      if (a.prob) a.prob[r] = 1.0f;
+    }
+    return;
+  }
+  float own_max = thread_max;
+  if (top == INFINITY) {  // +inf logits share the weight: the others weigh nothing
+    for (int j = 0; j < row.groups; ++j) {
+      float4& v = reinterpret_cast<float4*>(mine_s)[32 * j + lane];
+      v.x = v.x == INFINITY ? 0.0f : -INFINITY;
+      v.y = v.y == INFINITY ? 0.0f : -INFINITY;
+      v.z = v.z == INFINITY ? 0.0f : -INFINITY;
+      v.w = v.w == INFINITY ? 0.0f : -INFINITY;
+    }
+    own_max = thread_max == INFINITY ? 0.0f : -INFINITY;
+    top = 0.0f;
+    low = -INFINITY;
+    __syncthreads();
+  }
+  Scale sc;
+  sc.max = top;
   sc.inverse = __fdiv_rn(1.0f, temperature);
-  const float span = (sc.max - value_of((unsigned)(low >> 32))) * sc.inverse;
-  sc.bins = (kBins - 1) / fminf(fmaxf(span, 1e-20f), kSpan);
+  const float span = (top - low) * sc.inverse;
+  sc.bins = fminf((kBins - 1) / fminf(fmaxf(span, 1e-20f), kSpan) * sc.inverse, 1e38f);
   const int k = a.top_k ? a.top_k[r] : 0;
   const float p = a.top_p ? a.top_p[r] : 1.0f;
   const float floor_e = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
+  const bool by_count = k > 0 && k < a.n, by_mass = p < 1.0f;
+  const u64 share_p = by_mass ? (u64)ceilf(__fmul_rn(fmaxf(p, 0.0f), 16777216.0f)) : 0;
+  if (by_count || by_mass) {
+    const bool weigh = !by_count;  // the bin is chosen by mass
+    const unsigned bound = by_count && k <= kT / 2 ? local_bound(sh, sc, own_max, k) : kBins - 1;
+    for (int i = threadIdx.x; i < (weigh ? 4 : 1) * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
+    if (threadIdx.x == 0) {
+      sh.bin = kBins;
+      sh.fill = 0;
+    }
+    __syncthreads();
+    if (weigh) {
+      row.each([&](float v, int) {
+        const unsigned b = sc.bin(v);
+        if (b >= kBins) return;
+        const u64 w = weight_of(sc.e(v));
+        if (w == 0) return;
+        atomicAdd(&sh.hist[0][b], 1u);
+        atomicAdd(&sh.hist[1][b], (unsigned)(w & 0x3fff));
+        atomicAdd(&sh.hist[2][b], (unsigned)(w >> 14 & 0x3fff));
+        atomicAdd(&sh.hist[3][b], (unsigned)(w >> 28));
+      });
+    } else {
+      row.each([&](float v, int) {
+        const unsigned b = sc.bin(v);
+        if (b <= bound) atomicAdd(&sh.hist[0][b], 1u);
+      });
+    }
+    barrier();
+    u64 count = 0, weight = 0;
+    unsigned lower = 0;
+#pragma unroll 4
+    for (unsigned c = 0; c < ctas; ++c) {
+      const uint32_t h = remote(&sh.hist[0][threadIdx.x], c);
+      const unsigned in = get32(h);
+      if (c < rank) lower += in;
+      count += in;
+      if (weigh)
+        weight += (u64)get32(h + 4 * kBins) + ((u64)get32(h + 8 * kBins) << 14) + ((u64)get32(h + 12 * kBins) << 28);
+    }
+    u64 before_n, before_w;
+    scan2(sh, count, weight, before_n, before_w);
+    u64 want = 0, all = 0;
+    if (weigh) {
+      for (int w = 0; w < kW; ++w) all += sh.warp_b[w];
+      want = max(scaled(all, share_p, (1u << kGrid) - 1), 1ull);
+    }
+    if (weigh ? before_w < want && before_w + weight >= want : before_n < (u64)k && before_n + count >= (u64)k) {
+      sh.bin = threadIdx.x;
+      sh.in_n = before_n + count;
+    }
+    __syncthreads();
+    // a row with fewer than k weighty tokens: all of them
+    unsigned b = sh.bin;
+    u64 listed = b < kBins ? sh.in_n : 0;
+    if (b == kBins) {
+      b = kBins - 1;
+      for (int w = 0; w < kW; ++w) listed += sh.warp_a[w];
+    }
+    if (listed <= kList) {
+      // this CTA's place in the list: the tokens of the CTAs before it
+      unsigned mine = threadIdx.x <= b ? lower : 0;
+      mine = __reduce_add_sync(0xffffffffu, mine);
+      if (lane == 0 && mine) atomicAdd(&sh.fill, mine);
+      __syncthreads();
+      row.each([&](float v, int i) {
+        if (sc.bin(v) > b || (weigh && weight_of(sc.e(v)) == 0)) return;
+        const unsigned slot = atomicAdd(&sh.fill, 1u);
+        if (slot < kList) put64(remote(&sh.list[slot], 0), order_of(v, i));
+      });
+      barrier();
+      if (rank == 0)
+        finish(sh, reinterpret_cast<u64*>(x_s), sc, a, r, (int)listed, by_count ? k : a.n, want, by_mass, share_p, floor_e);
+      return;
+    }
+    barrier();  // the histograms are read
+  }
   u64 cut = ~0ull, before, mine;
-  if (k > 0 && k < a.n) cut = find_cut<false>(sh, row, sc, cut, (u64)k);
-  if (p < 1.0f) {
+  if (by_count) cut = find_cut<false>(sh, row, sc, cut, (u64)k);
+  if (by_mass) {
     const u64 mass = mass_upto(sh, row, sc, cut, 0.0f, before, mine);
-    const u64 share_p = (u64)ceilf(__fmul_rn(fmaxf(p, 0.0f), 16777216.0f));
     cut = find_cut<true>(sh, row, sc, cut, max(scaled(mass, share_p, (1u << kGrid) - 1), 1ull));
   }
   const u64 total = mass_upto(sh, row, sc, cut, floor_e, before, mine);
@@ -470,7 +716,8 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
 
 cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
   auto k = sample_cluster_kernel;
-  const int slice = ((a.n + ctas - 1) / ctas + kUnit - 1) / kUnit * kUnit;
+  // (at least two units: the first CTA keeps kList masses there)
+  const int slice = std::max(((a.n + ctas - 1) / ctas + kUnit - 1) / kUnit * kUnit, 2 * kUnit);
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * (int)sizeof(float));
   if (e != cudaSuccess) return e;
   if (ctas > 8 && (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
