@@ -17,10 +17,8 @@ namespace sample {
 
 using u64 = unsigned long long;
 
-constexpr int kThreads = 1024;
-constexpr int kWarps = kThreads / 32;
 constexpr int kGrid = 24;              // u and top_p in steps of 2^-24
-constexpr float kOne = 1099511627776.0f;  // 2^40: the weight of the largest logit
+constexpr int kWeightBits = 40;        // the largest logit weighs 2^40
 
 struct Args {
   const float* logits;
@@ -45,12 +43,14 @@ __device__ __forceinline__ float value_of(unsigned key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
-// exp((x - max) / temperature) of a key, at most 1 (exactly 1 at the maximum,
-// an infinite one included)
-__device__ __forceinline__ float exp_of(unsigned key, unsigned max_key, float max, float inverse) {
-  return key == max_key ? 1.0f : expf(__fmul_rn(__fsub_rn(value_of(key), max), inverse));
+// floor(2^40 e) of 0 <= e <= 1 by its bits (a conversion to 64 bits runs at a
+// fraction of the rate)
+__device__ __forceinline__ u64 weight_of(float e) {
+  const unsigned b = __float_as_uint(e);
+  const int up = (int)(b >> 23) - (127 - kWeightBits + 23);
+  const unsigned m = (b & 0x7fffffu) | 0x800000u;
+  return up >= 0 ? (u64)m << up : up > -24 ? (u64)(m >> -up) : 0;
 }
-__device__ __forceinline__ u64 weight_of(float e) { return (u64)__fmul_rn(e, kOne); }
 
 // floor(a * m / 2^24) for m <= 2^24 (a below 2^64 / 2^24 in the low part only)
 __device__ __forceinline__ u64 scaled(u64 a, u64 m, u64 round) {
@@ -63,13 +63,13 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
   return v;
 }
 
-// ---------------------------------------------------------------------------
-// Rows held in shared memory by a cluster of CTAs
-// ---------------------------------------------------------------------------
-//
-// The row is read from memory once, a slice per CTA.  What the CTAs of a row
-// tell one another goes through distributed shared memory, one cluster
-// barrier per exchange:
+// A row is worked on by a cluster of CTAs, a slice each.  With few rows the
+// slices are staged in shared memory (the row is read from memory once and
+// the passes below read it from there); with many, or a row too long for
+// that, one CTA takes a whole row and reads it again from L2 in each pass, so
+// that every SM has rows of its own and nothing waits for another CTA.  What
+// the CTAs of a row tell one another goes through distributed shared memory,
+// one cluster barrier per exchange:
 //   1. the largest and the smallest logit;
 //   2. with top-k or top-p, a histogram of z = (max - logit) / temperature
 //      over at most 28 (past it a weight is 0: e^-28 < 2^-40) in 512 equal
@@ -79,10 +79,9 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 //      first CTA of the cluster, which sorts them and finishes the row alone.
 // Where they are more than kList (a wide nucleus, ties), the exact cut is
 // found over the whole cluster instead: the bin's own tokens, listed in every
-// CTA, are ranked by value and index; a bin with too many is divided again by
+// CTA, are sorted by value and index; a bin with too many is divided again by
 // the bits of the key, then by index.  Then each CTA adds up its kept mass,
 // and the one that holds the draw walks its part.
-namespace cluster {
 
 constexpr int kT = 512;                // threads of a CTA
 constexpr int kW = kT / 32;
@@ -90,7 +89,6 @@ constexpr int kUnit = kT * 4;          // a slice is whole groups of 128 per war
 constexpr int kBins = 512;
 static_assert(kBins == kT, "one bin per thread");
 constexpr int kList = 2048;            // tokens the first CTA sorts
-constexpr int kRanked = 1024;          // tokens ranked pair by pair
 constexpr int kMaxCluster = 16;
 constexpr int kMaxSlice = 24 * kUnit;  // floats: 192 KB
 constexpr float kSpan = 28.0f;
@@ -136,39 +134,87 @@ struct Shared {
   u64 mass_of[kMaxCluster];
   u64 warp_a[kW], warp_b[kW];
   unsigned fill;                // entries of the list so far
-  unsigned bin;
+  unsigned bin, lower_in;
   u64 above_n, above_w, in_n;
 };
 static_assert(2 * kUnit * sizeof(float) >= kList * sizeof(u64), "the masses of a sorted list");
-static_assert((u64)kMaxSlice << 14 < 1ull << 32, "sums of 14-bit parts");
+// Logits of a slice up to which the sums of 14-bit parts stay below 2^32;
+// past it (one CTA, a longer row) the masses are 64-bit atomics.
+constexpr int kPartMax = 1 << 18;
 
 // This thread's logits: four at a time, index() + 0 .. 3, in the order of the
-// row within a warp.
+// row within a warp; -inf past the row's end (no weight, past every bin).  NaN
+// stays: it fails every comparison, falls past the bins and weighs nothing.
+// With `infinite` (the row has a +inf), +inf reads as 0 and the rest as -inf,
+// so that the infinite ones share the weight.
+template <bool STAGED>
 struct Slice {
-  const float* x;  // shared, the warp's part
+  const float* x;  // STAGED: shared, the warp's part; else the row
   int first;       // index in the row of this thread's first four
   int n, groups;
-  __device__ __forceinline__ float4 at(int j) const { return reinterpret_cast<const float4*>(x)[32 * j + (threadIdx.x & 31)]; }
+  bool vec, infinite;
   __device__ __forceinline__ int index(int j) const { return first + 128 * j; }
-  // f(logit, index) for each
+  __device__ __forceinline__ float4 from_memory(const float* row, int j) const {
+    const int i = index(j);
+    if (vec && i + 4 <= n) return __ldg(reinterpret_cast<const float4*>(row + i));
+    float4 v;
+    v.x = i < n ? __ldg(row + i) : -INFINITY;
+    v.y = i + 1 < n ? __ldg(row + i + 1) : -INFINITY;
+    v.z = i + 2 < n ? __ldg(row + i + 2) : -INFINITY;
+    v.w = i + 3 < n ? __ldg(row + i + 3) : -INFINITY;
+    return v;
+  }
+  __device__ __forceinline__ float4 at(int j) const {
+    float4 v;
+    if constexpr (STAGED) v = reinterpret_cast<const float4*>(x)[32 * j + (threadIdx.x & 31)];
+    else v = from_memory(x, j);
+    if (infinite) {
+      v.x = v.x == INFINITY ? 0.0f : -INFINITY;
+      v.y = v.y == INFINITY ? 0.0f : -INFINITY;
+      v.z = v.z == INFINITY ? 0.0f : -INFINITY;
+      v.w = v.w == INFINITY ? 0.0f : -INFINITY;
+    }
+    return v;
+  }
+  // f(four logits, index of the first), with several loads in flight
   template <typename F>
-  __device__ __forceinline__ void each(F f) const {
-    for (int j = 0; j < groups; ++j) {
-      const int i = index(j);
-      const float4 v = at(j);
-      if (i < n) f(v.x, i);
-      if (i + 1 < n) f(v.y, i + 1);
-      if (i + 2 < n) f(v.z, i + 2);
-      if (i + 3 < n) f(v.w, i + 3);
+  __device__ __forceinline__ void groups_of_4(F f) const {
+    constexpr int AHEAD = STAGED ? 2 : 4;
+    for (int j0 = 0; j0 < groups; j0 += AHEAD) {
+      float4 v[AHEAD];
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) v[q] = j0 + q < groups ? at(j0 + q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+#pragma unroll
+      for (int q = 0; q < AHEAD; ++q) f(v[q], index(j0 + q));
     }
   }
+  // f(logit, index) for those of the groups that reach `least`
+  template <typename F>
+  __device__ __forceinline__ void each_from(float least, F f) const {
+    groups_of_4([&](float4 v, int i) {
+      if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least) {
+#pragma unroll 1
+        for (int k = 0; k < 4; ++k) f(k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w, i + k);
+      }
+    });
+  }
+};
+
+// The tokens kept so far: those up to logit x, and of that logit up to index i.
+struct Cut {
+  float x;
+  int i;
+  __device__ __forceinline__ bool keeps(float v, int at) const { return v > x || (v == x && at <= i); }
+  __device__ __forceinline__ bool all() const { return x == -INFINITY && i == INT32_MAX; }
 };
 
 struct Scale {
   float max, inverse, bins;
   __device__ __forceinline__ float e(float x) const {
-    return x == max ? 1.0f : expf(__fmul_rn(__fsub_rn(x, max), inverse));
+    return fmaxf(expf(__fmul_rn(__fsub_rn(x, max), inverse)), 0.0f);  // (0 for NaN)
   }
+  // a logit below which every bin is past `b` (two bins of slack for rounding)
+  __device__ __forceinline__ float least(unsigned b) const { return max - (float)(b + 2) / bins * 1.0001f; }
   // (max - x) / temperature in bins, to the nearest whole number (the sum with
   // 2^23 rounds it into the low bits): monotone in the logit; kBins and more:
   // no weight.  `bins` carries the 1 / temperature.
@@ -222,134 +268,6 @@ __device__ __forceinline__ void scan2(Shared& sh, u64 a, u64 b, u64& before_a, u
   }
 }
 
-// The cut: the last token kept when the tokens up to `limit` (an earlier cut)
-// are cut either to the first `want` (BY_MASS false) or to those whose
-// predecessors weigh less than `want`.  Returns its order; `limit` when they
-// count or weigh less.
-template <bool BY_MASS>
-__device__ u64 find_cut(Shared& sh, const Slice& row, const Scale& sc, u64 limit, u64 want) {
-  const unsigned rank = ctarank(), ctas = nctas();
-  u64 above_n = 0, above_w = 0;  // tokens before the part, their mass
-  Part part{0, 0, 0, 64};
-  // (8 levels divide a 64-bit order to single tokens; the bound is for safety)
-  for (int level = 0; level < 10; ++level) {
-    for (int i = threadIdx.x; i < (BY_MASS ? 4 : 1) * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
-    if (threadIdx.x == 0) sh.bin = kBins;
-    __syncthreads();
-    row.each([&](float x, int i) {
-      const unsigned b = sub_bin(sc, part, x, i);
-      if (b >= kBins || order_of(x, i) > limit) return;
-      if constexpr (BY_MASS) {
-        const u64 w = weight_of(sc.e(x));
-        if (w == 0) return;
-        atomicAdd(&sh.hist[1][b], (unsigned)(w & 0x3fff));
-        atomicAdd(&sh.hist[2][b], (unsigned)(w >> 14 & 0x3fff));
-        atomicAdd(&sh.hist[3][b], (unsigned)(w >> 28));
-      }
-      atomicAdd(&sh.hist[0][b], 1u);
-    });
-    barrier();
-    u64 count = 0, weight = 0, lower = 0;  // of this thread's bin; its tokens in the CTAs before this one
-#pragma unroll 4
-    for (unsigned c = 0; c < ctas; ++c) {
-      const uint32_t h = remote(&sh.hist[0][threadIdx.x], c);
-      const unsigned k = get32(h);
-      if (c < rank) lower += k;
-      count += k;
-      if constexpr (BY_MASS)
-        weight += (u64)get32(h + 4 * kBins) + ((u64)get32(h + 8 * kBins) << 14) + ((u64)get32(h + 12 * kBins) << 28);
-    }
-    u64 before_n, before_w;
-    scan2(sh, count, weight, before_n, before_w);
-    before_n += above_n;
-    before_w += above_w;
-    if (BY_MASS ? before_w < want && before_w + weight >= want : before_n < want && before_n + count >= want) {
-      sh.bin = threadIdx.x;
-      sh.above_n = before_n;
-      sh.above_w = before_w;
-      sh.in_n = count;
-      sh.fill = (unsigned)min(lower, (u64)kRanked);
-    }
-    __syncthreads();
-    const unsigned b = sh.bin;
-    if (b == kBins) return limit;  // (at the first level only)
-    above_n = sh.above_n;
-    above_w = sh.above_w;
-    const int m = (int)min(sh.in_n, (u64)kRanked + 1);
-    if (m <= kRanked) {
-      row.each([&](float x, int i) {
-        if (sub_bin(sc, part, x, i) != b) return;
-        const u64 order = order_of(x, i);
-        if (order > limit || (BY_MASS && weight_of(sc.e(x)) == 0)) return;
-        const unsigned slot = atomicAdd(&sh.fill, 1u);
-        if (slot < kRanked)
-          for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order);
-      });
-      barrier();
-      // place of each of the part's tokens, or the mass before it
-      u64 last = 0;
-      for (int t = threadIdx.x; t < m; t += kT) {
-        const u64 mine = sh.list[t];
-        u64 before = BY_MASS ? above_w : above_n;
-        for (int j = 0; j < m; ++j) {
-          const u64 other = sh.list[j];
-          if (other < mine) before += BY_MASS ? weight_of(sc.e(value_of(~(unsigned)(other >> 32)))) : 1;
-        }
-        if (before < want) last = max(last, mine);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
-      if ((threadIdx.x & 31) == 0) sh.warp_a[threadIdx.x >> 5] = last;
-      __syncthreads();
-      for (int w = 0; w < kW; ++w) last = max(last, sh.warp_a[w]);
-      __syncthreads();
-      return last;
-    }
-    barrier();  // the histograms are read; divide the part
-    if (part.shift == 64) {
-      part.zbin = b;
-      part.shift = 55;
-    } else {
-      part.prefix |= (u64)b << part.shift;
-      part.mask |= (u64)(kBins - 1) << part.shift;
-      part.shift = part.shift >= 9 ? part.shift - 9 : 0;
-    }
-  }
-  return limit;
-}
-
-// Mass of the tokens up to `cut` with e >= floor: of this thread's warp and of
-// the warps and CTAs before it; returns the row's.
-__device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice& row, const Scale& sc, u64 cut, float floor_e,
-                                         u64& before, u64& mine) {
-  const unsigned rank = ctarank(), ctas = nctas();
-  const int warp = threadIdx.x >> 5;
-  u64 m = 0;
-  row.each([&](float x, int i) {
-    if (order_of(x, i) > cut) return;
-    const float e = sc.e(x);
-    if (e >= floor_e) m += weight_of(e);
-  });
-  mine = warp_sum_u64(m);
-  __syncthreads();
-  if ((threadIdx.x & 31) == 0) sh.warp_a[warp] = mine;
-  __syncthreads();
-  if (threadIdx.x < ctas) {
-    m = 0;
-    for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
-    put64(remote(&sh.mass_of[rank], threadIdx.x), m);
-  }
-  barrier();
-  u64 total = 0;
-  before = 0;
-  for (unsigned c = 0; c < ctas; ++c) {
-    if (c == rank) before = total;
-    total += sh.mass_of[c];
-  }
-  for (int w = 0; w < warp; ++w) before += sh.warp_a[w];
-  return total;
-}
-
 // Exclusive sum over the CTA of one value per thread; `total` of all.
 __device__ __forceinline__ u64 scan1(Shared& sh, u64 a, u64& total) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -373,8 +291,8 @@ __device__ __forceinline__ u64 scan1(Shared& sh, u64 a, u64& total) {
 }
 
 // Bitonic sort of list[0 .. n), n a power of two from 64 to kList, ascending,
-// by the CTA.  A warp's pairs at distances up to 32 stay inside its own 64
-// entries (per 512 threads' turn), so only the longer ones meet at a barrier.
+// by the CTA.  A warp's pairs at distances below 32 stay inside its own 64
+// entries (per turn of 512 threads), so only the longer ones meet at a barrier.
 __device__ __forceinline__ void sort_list(u64* list, int n) {
   for (int size = 2; size <= n; size <<= 1)
     for (int dist = size >> 1; dist > 0; dist >>= 1) {
@@ -392,20 +310,221 @@ __device__ __forceinline__ void sort_list(u64* list, int n) {
     }
   __syncthreads();
 }
+// Sorts the m entries of the list; returns the power of two they are padded to.
+__device__ __forceinline__ int sort_tokens(Shared& sh, int m) {
+  int n = 64;
+  while (n < m) n <<= 1;
+  for (int t = m + threadIdx.x; t < n; t += kT) sh.list[t] = ~0ull;
+  __syncthreads();
+  sort_list(sh.list, n);
+  return n;
+}
+
+constexpr int kPer = kList / kT;  // tokens of a sorted list per thread
+
+// Where a cut falls: bin `b` of a part, the tokens and the mass before it, its
+// own tokens, and this CTA's place among them (of the bin, of all up to it).
+struct Found {
+  unsigned b;
+  u64 above_n, above_w, in_n, want;
+  unsigned lower_in, lower_upto;
+};
+
+// Finds the bin of `part` in which token number `want`, or (BY_MASS) the
+// `want`-th unit of mass, falls, among the tokens up to `limit`; with BY_MASS
+// and want 0, want is `share` of the part's mass.  b = kBins: there are fewer.
+// Bins past `bound` are known not to matter.
+template <bool BY_MASS, bool STAGED>
+__device__ Found locate(Shared& sh, const Slice<STAGED>& row, const Scale& sc, const Part& part, Cut limit, u64 want,
+                        u64 share, u64 above_n, u64 above_w, unsigned bound) {
+  const unsigned rank = ctarank(), ctas = nctas();
+  for (int i = threadIdx.x; i < (BY_MASS ? 4 : 1) * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
+  if (threadIdx.x == 0) {
+    sh.bin = kBins;
+    sh.fill = 0;
+  }
+  __syncthreads();
+  const bool all = part.shift == 64 && limit.all();
+  row.each_from(sc.least(bound), [&](float x, int i) {
+    const unsigned b = all ? sc.bin(x) : sub_bin(sc, part, x, i);
+    if (b > bound || (!all && !limit.keeps(x, i))) return;
+    if constexpr (BY_MASS) {
+      const u64 w = weight_of(sc.e(x));
+      if (w == 0) return;
+      if (row.groups * (128 * kW) <= kPartMax) {
+        atomicAdd(&sh.hist[1][b], (unsigned)(w & 0x3fff));
+        atomicAdd(&sh.hist[2][b], (unsigned)(w >> 14 & 0x3fff));
+        atomicAdd(&sh.hist[3][b], (unsigned)(w >> 28));
+      } else {
+        atomicAdd(reinterpret_cast<u64*>(&sh.hist[2][0]) + b, w);
+      }
+    }
+    atomicAdd(&sh.hist[0][b], 1u);
+  });
+  barrier();
+  u64 count = 0, weight = 0;
+  unsigned lower = 0;  // tokens of this thread's bin in the CTAs before this one
+#pragma unroll 4
+  for (unsigned c = 0; c < ctas; ++c) {
+    const uint32_t h = remote(&sh.hist[0][threadIdx.x], c);
+    const unsigned in = get32(h);
+    if (c < rank) lower += in;
+    count += in;
+    if constexpr (BY_MASS) {
+      if (row.groups * (128 * kW) <= kPartMax)
+        weight += (u64)get32(h + 4 * kBins) + ((u64)get32(h + 8 * kBins) << 14) + ((u64)get32(h + 12 * kBins) << 28);
+      else
+        weight += reinterpret_cast<const u64*>(&sh.hist[2][0])[threadIdx.x];  // (a cluster of one)
+    }
+  }
+  u64 before_n, before_w;
+  scan2(sh, count, weight, before_n, before_w);
+  if (BY_MASS && want == 0) {
+    u64 mass = 0;
+    for (int w = 0; w < kW; ++w) mass += sh.warp_b[w];
+    want = max(scaled(mass, share, (1u << kGrid) - 1), 1ull);
+  }
+  before_n += above_n;
+  before_w += above_w;
+  if (BY_MASS ? before_w < want && before_w + weight >= want : before_n < want && before_n + count >= want) {
+    sh.bin = threadIdx.x;
+    sh.above_n = before_n;
+    sh.above_w = before_w;
+    sh.in_n = count;
+    sh.lower_in = lower;
+  }
+  __syncthreads();
+  Found f;
+  f.b = sh.bin;
+  f.want = want;
+  if (f.b == kBins) {
+    f.above_n = above_n;
+    for (int w = 0; w < kW; ++w) f.above_n += sh.warp_a[w];
+    f.above_w = f.in_n = 0;
+    f.lower_in = 0;
+  } else {
+    f.above_n = sh.above_n;
+    f.above_w = sh.above_w;
+    f.in_n = sh.in_n;
+    f.lower_in = sh.lower_in;
+  }
+  unsigned mine = threadIdx.x < f.b ? lower : 0;
+  mine = __reduce_add_sync(0xffffffffu, mine);
+  if ((threadIdx.x & 31) == 0 && mine) atomicAdd(&sh.fill, mine);
+  __syncthreads();
+  f.lower_upto = sh.fill + f.lower_in;
+  __syncthreads();
+  return f;
+}
+
+// The exact cut inside a bin that locate() found.
+template <bool BY_MASS, bool STAGED>
+__device__ Cut resolve(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Found f, Cut limit) {
+  const unsigned ctas = nctas();
+  Part part{0, 0, 0, 64};
+  // (8 levels divide a 64-bit order to single tokens; the bound is for safety)
+  for (int level = 0; level < 10 && f.b < kBins; ++level) {
+    if (f.in_n <= kList) {
+      const int m = (int)f.in_n;
+      if (threadIdx.x == 0) sh.fill = f.lower_in;
+      __syncthreads();
+      row.each_from(sc.least(part.shift == 64 ? f.b : part.zbin), [&](float x, int i) {
+        if (sub_bin(sc, part, x, i) != f.b) return;
+        if (!limit.keeps(x, i) || (BY_MASS && weight_of(sc.e(x)) == 0)) return;
+        const u64 order = order_of(x, i);
+        const unsigned slot = atomicAdd(&sh.fill, 1u);
+        if (slot < kList)
+          for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order);
+      });
+      barrier();
+      const int n = sort_tokens(sh, m), per = (n + kT - 1) / kT, t0 = threadIdx.x * per;
+      u64 w[kPer], mine = 0, total, last = 0;
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        const bool in = q < per && t0 + q < m;
+        w[q] = !in ? 0 : BY_MASS ? weight_of(sc.e(value_of(~(unsigned)(sh.list[t0 + q] >> 32)))) : 1;
+        mine += w[q];
+      }
+      u64 before = scan1(sh, mine, total) + (BY_MASS ? f.above_w : f.above_n);
+#pragma unroll
+      for (int q = 0; q < kPer; ++q) {
+        if (w[q] && before < f.want) last = sh.list[t0 + q];  // ascending
+        before += w[q];
+      }
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) last = max(last, __shfl_xor_sync(0xffffffffu, last, o));
+      __syncthreads();
+      if ((threadIdx.x & 31) == 0) sh.warp_a[threadIdx.x >> 5] = last;
+      __syncthreads();
+      for (int v = 0; v < kW; ++v) last = max(last, sh.warp_a[v]);
+      __syncthreads();
+      return Cut{value_of(~(unsigned)(last >> 32)), (int)(unsigned)last};
+    }
+    barrier();  // the histograms are read; divide the bin
+    if (part.shift == 64) {
+      part.zbin = f.b;
+      part.shift = 55;
+    } else {
+      part.prefix |= (u64)f.b << part.shift;
+      part.mask |= (u64)(kBins - 1) << part.shift;
+      part.shift = part.shift >= 9 ? part.shift - 9 : 0;
+    }
+    f = locate<BY_MASS>(sh, row, sc, part, limit, f.want, 0, f.above_n, f.above_w, kBins - 1);
+  }
+  return limit;  // fewer, or lighter, than what is wanted: all
+}
+
+// Mass of the tokens up to `cut` with e >= floor: of this thread's warp and of
+// the warps and CTAs before it; returns the row's.
+template <bool STAGED>
+__device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Cut cut, float floor_e,
+                                         u64& before, u64& mine) {
+  const unsigned rank = ctarank(), ctas = nctas();
+  const int warp = threadIdx.x >> 5;
+  u64 m = 0;
+  const bool all = cut.all();
+  if (all) {
+    row.groups_of_4([&](float4 v, int) {
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const float e = sc.e(k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w);
+        m += e >= floor_e ? weight_of(e) : 0;
+      }
+    });
+  } else {
+    row.each_from(cut.x, [&](float x, int i) {
+      if (!cut.keeps(x, i)) return;
+      const float e = sc.e(x);
+      if (e >= floor_e) m += weight_of(e);
+    });
+  }
+  mine = warp_sum_u64(m);
+  __syncthreads();
+  if ((threadIdx.x & 31) == 0) sh.warp_a[warp] = mine;
+  __syncthreads();
+  if (threadIdx.x < ctas) {
+    m = 0;
+    for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
+    put64(remote(&sh.mass_of[rank], threadIdx.x), m);
+  }
+  barrier();
+  u64 total = 0;
+  before = 0;
+  for (unsigned c = 0; c < ctas; ++c) {
+    if (c == rank) before = total;
+    total += sh.mass_of[c];
+  }
+  for (int w = 0; w < warp; ++w) before += sh.warp_a[w];
+  return total;
+}
 
 // The rest of a row by one CTA: list[0 .. m) holds the order of every token
 // that can be kept.  `k`: keep at most that many; `want`: then those whose
 // predecessors weigh less (0: not yet known, top_p of what k keeps).
 __device__ void finish(Shared& sh, u64* mass_s, const Scale& sc, const Args& a, int r, int m, int k, u64 want,
                        bool by_mass, u64 share_p, float floor_e) {
-  int n = 64;
-  while (n < m) n <<= 1;
-  for (int t = m + threadIdx.x; t < n; t += kT) sh.list[t] = ~0ull;
-  __syncthreads();
-  sort_list(sh.list, n);
   // consecutive tokens per thread
-  const int per = (n + kT - 1) / kT, t0 = threadIdx.x * per;
-  constexpr int kPer = kList / kT;
+  const int n = sort_tokens(sh, m), per = (n + kT - 1) / kT, t0 = threadIdx.x * per;
   u64 w[kPer], mine = 0;
   float e[kPer];
 #pragma unroll
@@ -478,7 +597,10 @@ __device__ __forceinline__ unsigned local_bound(Shared& sh, const Scale& sc, flo
   return bound;
 }
 
-__global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constant__ Args a, int slice) {
+// STAGED: a cluster per row, the slices in shared memory (after the sorted
+// list's masses).  Otherwise one CTA per row.
+template <bool STAGED>
+__global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ Args a, int slice) {
   grid_dependency_wait();
   allow_dependents_launch();
   __shared__ Shared sh;
@@ -488,27 +610,34 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
   const float* x = a.logits + r * a.stride;
   const int share = slice / kW;  // of a warp
   float* mine_s = x_s + warp * share;
-  const Slice row{mine_s, (int)rank * slice + warp * share + 4 * lane, a.n, share / 128};
+  Slice<STAGED> row{STAGED ? mine_s : x, (int)rank * slice + warp * share + 4 * lane, a.n, share / 128,
+                    (reinterpret_cast<uintptr_t>(x) & 15) == 0, false};
   float top = -INFINITY, low = INFINITY;
-  const bool vec = (reinterpret_cast<uintptr_t>(x) & 15) == 0;
-#pragma unroll 4
-  for (int j = 0; j < row.groups; ++j) {
-    const int i = row.index(j);
-    float v[4];
-    if (vec && i + 4 <= a.n) {
-      const float4 f = __ldcs(reinterpret_cast<const float4*>(x + i));
-      v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-    } else {
+  int top_group = 0;  // where this thread first saw its largest
+  for (int j0 = 0; j0 < row.groups; j0 += 4) {
+    float4 v[4];
 #pragma unroll
-      for (int k = 0; k < 4; ++k) v[k] = i + k < a.n ? __ldcs(x + i + k) : -INFINITY;
-    }
+    for (int q = 0; q < 4; ++q)
+      if (j0 + q < row.groups) v[q] = row.from_memory(x, j0 + q);
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (isnan(v[k])) v[k] = -INFINITY;
-      top = fmaxf(top, v[k]);
-      if (i + k < a.n) low = fminf(low, v[k]);
+    for (int q = 0; q < 4; ++q) {
+      const int j = j0 + q, i = row.index(j);
+      if (j >= row.groups) break;
+      const float4 f = v[q];
+      const float most = fmaxf(fmaxf(f.x, f.y), fmaxf(f.z, f.w));
+      if (most > top) {
+        top = most;
+        top_group = j;
+      }
+      if (i + 4 <= a.n) {
+        low = fminf(fminf(fminf(low, f.x), fminf(f.y, f.z)), f.w);
+      } else {
+        if (i < a.n) low = fminf(low, f.x);
+        if (i + 1 < a.n) low = fminf(low, f.y);
+        if (i + 2 < a.n) low = fminf(low, f.z);
+      }
+      if constexpr (STAGED) reinterpret_cast<float4*>(mine_s)[32 * j + lane] = f;
     }
-    reinterpret_cast<float4*>(mine_s)[32 * j + lane] = make_float4(v[0], v[1], v[2], v[3]);
   }
   const float thread_max = top;
 #pragma unroll
@@ -548,10 +677,11 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
   }
   if (!(temperature > 0.0f)) {  // greedy: the first index of the largest
     unsigned first = 0xffffffffu;
-    if (thread_max == top)
-      row.each([&](float v, int i) {
-        if (v == top) first = min(first, (unsigned)i);
-      });
+    if (thread_max == top) {
+      const float4 v = row.at(top_group);
+      const int at = v.x == top ? 0 : v.y == top ? 1 : v.z == top ? 2 : 3;
+      first = (unsigned)(row.index(top_group) + at);
+    }
     first = __reduce_min_sync(0xffffffffu, first);
     if (threadIdx.x == 0) sh.fill = 0xffffffffu;
     __syncthreads();
@@ -568,21 +698,14 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
   }
   float own_max = thread_max;
   if (top == INFINITY) {  // +inf logits share the weight: the others weigh nothing
-    for (int j = 0; j < row.groups; ++j) {
-      float4& v = reinterpret_cast<float4*>(mine_s)[32 * j + lane];
-      v.x = v.x == INFINITY ? 0.0f : -INFINITY;
-      v.y = v.y == INFINITY ? 0.0f : -INFINITY;
-      v.z = v.z == INFINITY ? 0.0f : -INFINITY;
-      v.w = v.w == INFINITY ? 0.0f : -INFINITY;
-    }
+    row.infinite = true;
     own_max = thread_max == INFINITY ? 0.0f : -INFINITY;
     top = 0.0f;
     low = -INFINITY;
-    __syncthreads();
   }
   Scale sc;
   sc.max = top;
-  sc.inverse = __fdiv_rn(1.0f, temperature);
+  sc.inverse = fminf(__fdiv_rn(1.0f, temperature), 3e38f);
   const float span = (top - low) * sc.inverse;
   sc.bins = fminf((kBins - 1) / fminf(fmaxf(span, 1e-20f), kSpan) * sc.inverse, 1e38f);
   const int k = a.top_k ? a.top_k[r] : 0;
@@ -590,86 +713,39 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
   const float floor_e = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
   const bool by_count = k > 0 && k < a.n, by_mass = p < 1.0f;
   const u64 share_p = by_mass ? (u64)ceilf(__fmul_rn(fmaxf(p, 0.0f), 16777216.0f)) : 0;
+  Cut cut{-INFINITY, INT32_MAX};
+  u64 before, mine;
   if (by_count || by_mass) {
-    const bool weigh = !by_count;  // the bin is chosen by mass
+    const Part whole{0, 0, 0, 64};
     const unsigned bound = by_count && k <= kT / 2 ? local_bound(sh, sc, own_max, k) : kBins - 1;
-    for (int i = threadIdx.x; i < (weigh ? 4 : 1) * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
-    if (threadIdx.x == 0) {
-      sh.bin = kBins;
-      sh.fill = 0;
-    }
-    __syncthreads();
-    if (weigh) {
-      row.each([&](float v, int) {
-        const unsigned b = sc.bin(v);
-        if (b >= kBins) return;
-        const u64 w = weight_of(sc.e(v));
-        if (w == 0) return;
-        atomicAdd(&sh.hist[0][b], 1u);
-        atomicAdd(&sh.hist[1][b], (unsigned)(w & 0x3fff));
-        atomicAdd(&sh.hist[2][b], (unsigned)(w >> 14 & 0x3fff));
-        atomicAdd(&sh.hist[3][b], (unsigned)(w >> 28));
-      });
-    } else {
-      row.each([&](float v, int) {
-        const unsigned b = sc.bin(v);
-        if (b <= bound) atomicAdd(&sh.hist[0][b], 1u);
-      });
-    }
-    barrier();
-    u64 count = 0, weight = 0;
-    unsigned lower = 0;
-#pragma unroll 4
-    for (unsigned c = 0; c < ctas; ++c) {
-      const uint32_t h = remote(&sh.hist[0][threadIdx.x], c);
-      const unsigned in = get32(h);
-      if (c < rank) lower += in;
-      count += in;
-      if (weigh)
-        weight += (u64)get32(h + 4 * kBins) + ((u64)get32(h + 8 * kBins) << 14) + ((u64)get32(h + 12 * kBins) << 28);
-    }
-    u64 before_n, before_w;
-    scan2(sh, count, weight, before_n, before_w);
-    u64 want = 0, all = 0;
-    if (weigh) {
-      for (int w = 0; w < kW; ++w) all += sh.warp_b[w];
-      want = max(scaled(all, share_p, (1u << kGrid) - 1), 1ull);
-    }
-    if (weigh ? before_w < want && before_w + weight >= want : before_n < (u64)k && before_n + count >= (u64)k) {
-      sh.bin = threadIdx.x;
-      sh.in_n = before_n + count;
-    }
-    __syncthreads();
-    // a row with fewer than k weighty tokens: all of them
-    unsigned b = sh.bin;
-    u64 listed = b < kBins ? sh.in_n : 0;
-    if (b == kBins) {
-      b = kBins - 1;
-      for (int w = 0; w < kW; ++w) listed += sh.warp_a[w];
-    }
-    if (listed <= kList) {
-      // this CTA's place in the list: the tokens of the CTAs before it
-      unsigned mine = threadIdx.x <= b ? lower : 0;
-      mine = __reduce_add_sync(0xffffffffu, mine);
-      if (lane == 0 && mine) atomicAdd(&sh.fill, mine);
+    Found f = by_count ? locate<false>(sh, row, sc, whole, cut, (u64)k, 0, 0, 0, bound)
+                       : locate<true>(sh, row, sc, whole, cut, 0, share_p, 0, 0, bound);
+    // (a row with fewer than k weighty tokens: all of them)
+    if (f.above_n + f.in_n <= kList) {
+      const unsigned upto = min(f.b, (unsigned)kBins - 1);
+      if (threadIdx.x == 0) sh.fill = f.lower_upto;
       __syncthreads();
-      row.each([&](float v, int i) {
-        if (sc.bin(v) > b || (weigh && weight_of(sc.e(v)) == 0)) return;
+      row.each_from(sc.least(upto), [&](float v, int i) {
+        if (sc.bin(v) > upto || (!by_count && weight_of(sc.e(v)) == 0)) return;
         const unsigned slot = atomicAdd(&sh.fill, 1u);
         if (slot < kList) put64(remote(&sh.list[slot], 0), order_of(v, i));
       });
       barrier();
       if (rank == 0)
-        finish(sh, reinterpret_cast<u64*>(x_s), sc, a, r, (int)listed, by_count ? k : a.n, want, by_mass, share_p, floor_e);
+        finish(sh, reinterpret_cast<u64*>(x_s), sc, a, r, (int)(f.above_n + f.in_n), by_count ? k : a.n,
+               by_count ? 0 : f.want, by_mass, share_p, floor_e);
       return;
     }
-    barrier();  // the histograms are read
-  }
-  u64 cut = ~0ull, before, mine;
-  if (by_count) cut = find_cut<false>(sh, row, sc, cut, (u64)k);
-  if (by_mass) {
-    const u64 mass = mass_upto(sh, row, sc, cut, 0.0f, before, mine);
-    cut = find_cut<true>(sh, row, sc, cut, max(scaled(mass, share_p, (1u << kGrid) - 1), 1ull));
+    if (by_count) {
+      cut = resolve<false>(sh, row, sc, f, cut);
+      if (by_mass) {
+        const u64 mass = mass_upto(sh, row, sc, cut, 0.0f, before, mine);
+        f = locate<true>(sh, row, sc, whole, cut, max(scaled(mass, share_p, (1u << kGrid) - 1), 1ull), 0, 0, 0, kBins - 1);
+        cut = resolve<true>(sh, row, sc, f, cut);
+      }
+    } else {
+      cut = resolve<true>(sh, row, sc, f, cut);
+    }
   }
   const u64 total = mass_upto(sh, row, sc, cut, floor_e, before, mine);
   const float uf = fminf(fmaxf(a.u[r], 0.0f), 1.0f);
@@ -686,7 +762,7 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
     for (int q = 0; q < 4; ++q) {
       const int i = row.index(j) + q;
       w[q] = 0;
-      if (i < a.n && order_of(v[q], i) <= cut) {
+      if (i < a.n && cut.keeps(v[q], i)) {
         const float e = sc.e(v[q]);
         if (e >= floor_e) w[q] = weight_of(e);
       }
@@ -715,9 +791,11 @@ __global__ void __launch_bounds__(kT) sample_cluster_kernel(const __grid_constan
 }
 
 cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
-  auto k = sample_cluster_kernel;
-  // (at least two units: the first CTA keeps kList masses there)
-  const int slice = std::max(((a.n + ctas - 1) / ctas + kUnit - 1) / kUnit * kUnit, 2 * kUnit);
+  const int slice = ((a.n + ctas - 1) / ctas + kUnit - 1) / kUnit * kUnit;
+  if (ctas == 1)
+    return launch_ex(sample_kernel<false>, dim3((unsigned)rows), dim3(kT), kList * sizeof(u64), st, a, slice);
+  // (at least two units: the first CTA keeps a sorted list's masses there)
+  auto k = sample_kernel<true>;
   cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * (int)sizeof(float));
   if (e != cudaSuccess) return e;
   if (ctas > 8 && (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
@@ -730,210 +808,11 @@ cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(kT);
-  cfg.dynamicSmemBytes = slice * sizeof(float);
+  cfg.dynamicSmemBytes = std::max(slice, 2 * kUnit) * sizeof(float);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = launch_overlap() ? 2 : 1;
   return cudaLaunchKernelEx(&cfg, k, a, slice);
-}
-
-}  // namespace cluster
-
-// ---------------------------------------------------------------------------
-// Rows past what a cluster holds: one CTA per row, every pass reads it again
-// ---------------------------------------------------------------------------
-__global__ void __launch_bounds__(kThreads) sample_kernel(const __grid_constant__ Args a) {
-  grid_dependency_wait();
-  allow_dependents_launch();
-  __shared__ u64 hist[256];
-  __shared__ u64 warp_mass[kWarps];
-  __shared__ int warp_ties[kWarps];
-  __shared__ unsigned max_s;
-  __shared__ int first_s;
-  __shared__ unsigned sel_key;
-  __shared__ u64 sel_rest;
-  __shared__ u64 total_s;
-  const int row = blockIdx.x, n = a.n, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const float* x = a.logits + row * a.stride;
-  if (threadIdx.x == 0) {
-    max_s = 0;
-    first_s = n;
-    total_s = 0;
-  }
-  __syncthreads();
-  unsigned mk = 0;
-  for (int i = threadIdx.x; i < n; i += kThreads) mk = max(mk, key_of(x[i]));
-  atomicMax(&max_s, __reduce_max_sync(0xffffffffu, mk));
-  __syncthreads();
-  const unsigned max_key = max_s;
-  const float max_x = value_of(max_key);
-  const float temperature = a.temperature ? a.temperature[row] : 1.0f;
-  if (max_x == -INFINITY || !(temperature > 0.0f)) {
-    for (int i = threadIdx.x; i < n; i += kThreads)
-      if (key_of(x[i]) == max_key) {
-        atomicMin(&first_s, i);
-        break;
-      }
-    __syncthreads();
-    if (threadIdx.x == 0) {
-      a.token[row] = max_x == -INFINITY ? 0 : first_s;
-      if (a.prob) a.prob[row] = max_x == -INFINITY ? 0.0f : 1.0f;
-    }
-    return;
-  }
-  const float inverse = __fdiv_rn(1.0f, temperature);
-  const int k = a.top_k ? a.top_k[row] : 0;
-  const float p = a.top_p ? a.top_p[row] : 1.0f;
-  const float floor_e = a.min_p ? fminf(a.min_p[row], 1.0f) : 0.0f;
-  // kept: keys above `cut`, and the first `ties` (by index) equal to it
-  unsigned cut = 0;
-  int ties = n;
-  if (k > 0 && k < n) {
-    // the k-th largest key, eight bits at a time
-    unsigned prefix = 0, mask = 0;
-    u64 want = k;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const unsigned key = key_of(x[i]);
-        if ((key & mask) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1ull);
-      }
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        int b = 255;
-        u64 above = 0;
-        while (b > 0 && above + hist[b] < want) above += hist[b--];
-        sel_key = prefix | ((unsigned)b << shift);
-        sel_rest = want - above;
-      }
-      __syncthreads();
-      prefix = sel_key;
-      want = sel_rest;
-      mask |= 255u << shift;
-    }
-    cut = prefix;
-    ties = (int)want;
-  }
-  if (p < 1.0f) {
-    // the total of what top-k keeps, then the key at which the running mass
-    // from the top reaches top_p of it
-    u64 mass = 0;
-    for (int i = threadIdx.x; i < n; i += kThreads) {
-      const unsigned key = key_of(x[i]);
-      if (key > cut) mass += weight_of(exp_of(key, max_key, max_x, inverse));
-    }
-    mass = warp_sum_u64(mass);
-    if (lane == 0) atomicAdd(&total_s, mass);
-    __syncthreads();
-    const u64 tie_mass = cut ? ties * weight_of(exp_of(cut, max_key, max_x, inverse)) : 0;
-    const u64 total = total_s + tie_mass;
-    const u64 share = (u64)ceilf(__fmul_rn(fmaxf(p, 0.0f), 16777216.0f));
-    u64 want = scaled(total, share, (1u << kGrid) - 1);
-    if (want == 0) want = 1;
-    unsigned prefix = 0, mask = 0;
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (threadIdx.x < 256) hist[threadIdx.x] = 0;
-      __syncthreads();
-      for (int i = threadIdx.x; i < n; i += kThreads) {
-        const unsigned key = key_of(x[i]);
-        if (key > cut && (key & mask) == prefix)
-          atomicAdd(&hist[(key >> shift) & 255], weight_of(exp_of(key, max_key, max_x, inverse)));
-      }
-      if (threadIdx.x == 0 && (cut & mask) == prefix && tie_mass) atomicAdd(&hist[(cut >> shift) & 255], tie_mass);
-      __syncthreads();
-      if (threadIdx.x == 0) {
-        int b = 255;
-        u64 above = 0;
-        while (b > 0 && above + hist[b] < want) above += hist[b--];
-        sel_key = prefix | ((unsigned)b << shift);
-        sel_rest = want - above;
-      }
-      __syncthreads();
-      prefix = sel_key;
-      want = sel_rest;
-      mask |= 255u << shift;
-    }
-    // ties at the key: as many as still start below the limit
-    const u64 each = weight_of(exp_of(prefix, max_key, max_x, inverse));
-    const u64 take = (want + each - 1) / each;
-    ties = prefix == cut ? (int)min((u64)ties, take) : (int)min((u64)n, take);
-    cut = prefix;
-  }
-  // kept weights, a contiguous share of the row per warp
-  const float cut_e = exp_of(cut, max_key, max_x, inverse);
-  const u64 cut_w = cut_e >= floor_e ? weight_of(cut_e) : 0;
-  const int share = ((n + kWarps - 1) / kWarps + 31) / 32 * 32;
-  const int i0 = min(n, warp * share), i1 = min(n, i0 + share);
-  u64 mass = 0;
-  int tied = 0;
-  for (int i = i0 + lane; i < i1; i += 32) {
-    const unsigned key = key_of(x[i]);
-    if (key > cut) {
-      const float e = exp_of(key, max_key, max_x, inverse);
-      if (e >= floor_e) mass += weight_of(e);
-    } else if (key == cut) {
-      ++tied;
-    }
-  }
-  mass = warp_sum_u64(mass);
-  tied = __reduce_add_sync(0xffffffffu, tied);
-  if (lane == 0) {
-    warp_mass[warp] = mass;
-    warp_ties[warp] = tied;
-  }
-  __syncthreads();
-  // every warp: kept mass and ties before its share, and the total
-  int my_ties = warp_ties[lane], before_ties = my_ties;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int y = __shfl_up_sync(0xffffffffu, before_ties, o);
-    if (lane >= o) before_ties += y;
-  }
-  before_ties -= my_ties;
-  const int kept_ties = max(0, min(my_ties, ties - before_ties));
-  u64 w = warp_mass[lane] + kept_ties * cut_w, upto = w;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const u64 y = __shfl_up_sync(0xffffffffu, upto, o);
-    if (lane >= o) upto += y;
-  }
-  const u64 total = __shfl_sync(0xffffffffu, upto, 31);
-  const float uf = fminf(fmaxf(a.u[row], 0.0f), 1.0f);
-  const u64 ui = min((u64)__fmul_rn(uf, 16777216.0f), (u64)(1u << kGrid) - 1);
-  const u64 aim = scaled(total, ui, 0);
-  const u64 start = __shfl_sync(0xffffffffu, upto - w, warp), mine = __shfl_sync(0xffffffffu, w, warp);
-  if (aim < start || aim >= start + mine) return;
-  // this warp holds the token: walk its share
-  u64 run = start;
-  int seen = __shfl_sync(0xffffffffu, before_ties, warp);
-  for (int i = i0 + lane; i - lane < i1; i += 32) {
-    const unsigned key = i < i1 ? key_of(x[i]) : 0;
-    const unsigned tied_lanes = __ballot_sync(0xffffffffu, i < i1 && key == cut);
-    u64 v = 0;
-    if (i < i1 && key > cut) {
-      const float e = exp_of(key, max_key, max_x, inverse);
-      if (e >= floor_e) v = weight_of(e);
-    } else if (i < i1 && key == cut && seen + __popc(tied_lanes & ((1u << lane) - 1)) < ties) {
-      v = cut_w;
-    }
-    u64 s = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const u64 y = __shfl_up_sync(0xffffffffu, s, o);
-      if (lane >= o) s += y;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, run + s > aim);
-    if (hit) {
-      if (lane == __ffs(hit) - 1) {
-        a.token[row] = i;
-        if (a.prob) a.prob[row] = __fdiv_rn((float)v, (float)total);
-      }
-      return;
-    }
-    run += __shfl_sync(0xffffffffu, s, 31);
-    seen += __popc(tied_lanes);
-  }
 }
 
 }  // namespace sample
@@ -955,15 +834,11 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
       return hyq::api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
   const hyq::sample::Args a{logits, stride, (int)n, temperature, top_k, top_p, min_p, u, token, prob};
   const cudaStream_t st = (cudaStream_t)stream;
-  namespace sc = hyq::sample::cluster;
-  cudaError_t e;
   static const char* tune = getenv("HYQ_TUNE_C");
-  const int want = tune ? atoi(tune) : 8;
-  const int ctas = (int)std::max<int64_t>(std::min<int64_t>(want, (n + sc::kUnit - 1) / sc::kUnit), (n + sc::kMaxSlice - 1) / sc::kMaxSlice);
-  if (ctas <= sc::kMaxCluster && rows <= INT32_MAX / sc::kMaxCluster)
-    e = sc::launch(a, rows, ctas, st);
-  else
-    e = hyq::launch_ex(hyq::sample::sample_kernel, dim3((unsigned)rows), dim3(hyq::sample::kThreads), 0, st, a);
+  const int want = tune ? atoi(tune) : rows >= 64 ? 1 : 8;
+  int64_t ctas = std::min<int64_t>(want, (n + hyq::sample::kUnit - 1) / hyq::sample::kUnit);
+  if (ctas > 1 && n > ctas * hyq::sample::kMaxSlice) ctas = 1;
+  const cudaError_t e = hyq::sample::launch(a, rows, (int)ctas, st);
   return e == cudaSuccess ? HYQ_OK : hyq::api_fail(HYQ_E_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
