@@ -103,7 +103,13 @@ __device__ __forceinline__ unsigned nctas() {
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
   return r;
 }
+// All threads of the row: of the cluster (STAGED), or of its one CTA.
+template <bool STAGED>
 __device__ __forceinline__ void barrier() {
+  if constexpr (!STAGED) {
+    __syncthreads();
+    return;
+  }
   asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 // The same shared address in CTA `rank`.
@@ -164,17 +170,32 @@ struct Slice {
     v.w = i + 3 < n ? __ldg(row + i + 3) : -INFINITY;
     return v;
   }
+  __device__ __forceinline__ float4 only_infinite(float4 v) const {
+    return make_float4(v.x == INFINITY ? 0.0f : -INFINITY, v.y == INFINITY ? 0.0f : -INFINITY,
+                       v.z == INFINITY ? 0.0f : -INFINITY, v.w == INFINITY ? 0.0f : -INFINITY);
+  }
+  __device__ __forceinline__ float4 load(int j) const {
+    if constexpr (STAGED) return reinterpret_cast<const float4*>(x)[32 * j + (threadIdx.x & 31)];
+    else return from_memory(x, j);
+  }
   __device__ __forceinline__ float4 at(int j) const {
-    float4 v;
-    if constexpr (STAGED) v = reinterpret_cast<const float4*>(x)[32 * j + (threadIdx.x & 31)];
-    else v = from_memory(x, j);
-    if (infinite) {
-      v.x = v.x == INFINITY ? 0.0f : -INFINITY;
-      v.y = v.y == INFINITY ? 0.0f : -INFINITY;
-      v.z = v.z == INFINITY ? 0.0f : -INFINITY;
-      v.w = v.w == INFINITY ? 0.0f : -INFINITY;
+    const float4 v = load(j);
+    return infinite ? only_infinite(v) : v;
+  }
+  // groups j0 .. j0 + N - 1, all loads issued before any value is used
+  template <int N>
+  __device__ __forceinline__ void batch(int j0, float4 (&v)[N]) const {
+    if (!STAGED && vec && j0 + N <= groups && index(j0 + N - 1) + 4 <= n) {
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        asm volatile("ld.global.nc.v4.f32 {%0, %1, %2, %3}, [%4];"
+                     : "=f"(v[q].x), "=f"(v[q].y), "=f"(v[q].z), "=f"(v[q].w)
+                     : "l"(x + index(j0 + q)));
+    } else {
+#pragma unroll
+      for (int q = 0; q < N; ++q)
+        v[q] = j0 + q < groups ? load(j0 + q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
     }
-    return v;
   }
   // f(four logits, index of the first), with several loads in flight
   template <typename F>
@@ -182,8 +203,11 @@ struct Slice {
     constexpr int AHEAD = STAGED ? 2 : 4;
     for (int j0 = 0; j0 < groups; j0 += AHEAD) {
       float4 v[AHEAD];
+      batch(j0, v);
+      if (infinite) {
 #pragma unroll
-      for (int q = 0; q < AHEAD; ++q) v[q] = j0 + q < groups ? at(j0 + q) : make_float4(-INFINITY, -INFINITY, -INFINITY, -INFINITY);
+        for (int q = 0; q < AHEAD; ++q) v[q] = only_infinite(v[q]);
+      }
 #pragma unroll
       for (int q = 0; q < AHEAD; ++q) f(v[q], index(j0 + q));
     }
@@ -193,9 +217,36 @@ struct Slice {
   __device__ __forceinline__ void each_from(float least, F f) const {
     groups_of_4([&](float4 v, int i) {
       if (fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least) {
-#pragma unroll 1
-        for (int k = 0; k < 4; ++k) f(k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w, i + k);
+        f(v.x, i);
+        f(v.y, i + 1);
+        f(v.z, i + 2);
+        f(v.w, i + 3);
       }
+    });
+  }
+  // put(slot, logit, index) for those of the groups that reach `least` and
+  // satisfy f(logit, index); slots count up from `fill`, one addition to it per
+  // warp and group.
+  template <typename F, typename P>
+  __device__ __forceinline__ void collect(float least, unsigned* fill, F f, P put) const {
+    const int lane = threadIdx.x & 31;
+    groups_of_4([&](float4 v, int i) {
+      if (!__any_sync(0xffffffffu, fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= least)) return;
+      const bool in[4] = {f(v.x, i), f(v.y, i + 1), f(v.z, i + 2), f(v.w, i + 3)};
+      const unsigned own = in[0] + in[1] + in[2] + in[3];
+      unsigned upto = own;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const unsigned y = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += y;
+      }
+      unsigned slot = 0;
+      if (lane == 31 && upto) slot = atomicAdd(fill, upto);
+      slot = __shfl_sync(0xffffffffu, slot, 31) + upto - own;
+      if (in[0]) put(slot++, v.x, i);
+      if (in[1]) put(slot++, v.y, i + 1);
+      if (in[2]) put(slot++, v.z, i + 2);
+      if (in[3]) put(slot++, v.w, i + 3);
     });
   }
 };
@@ -290,34 +341,82 @@ __device__ __forceinline__ u64 scan1(Shared& sh, u64 a, u64& total) {
   return before;
 }
 
-// Bitonic sort of list[0 .. n), n a power of two from 64 to kList, ascending,
-// by the CTA.  A warp's pairs at distances below 32 stay inside its own 64
-// entries (per turn of 512 threads), so only the longer ones meet at a barrier.
-__device__ __forceinline__ void sort_list(u64* list, int n) {
-  for (int size = 2; size <= n; size <<= 1)
+// Bitonic sort of kT P values, P consecutive ones per thread (P 2 or 4),
+// ascending: distances inside a thread in registers, inside a warp by
+// shuffles, past it through `buffer` (kT P values of shared memory).
+template <int P>
+__device__ __forceinline__ void sort_values(u64 (&v)[P], u64* buffer) {
+  const int p0 = threadIdx.x * P;
+#pragma unroll 1
+  for (int size = 2; size <= kT * P; size <<= 1)
+#pragma unroll 1
     for (int dist = size >> 1; dist > 0; dist >>= 1) {
-      if (dist >= 32) __syncthreads();
-      else __syncwarp();
-      for (int t = threadIdx.x; t < n / 2; t += kT) {
-        const int i = 2 * t - (t & (dist - 1)), j = i + dist;
-        const u64 a = list[i], b = list[j];
-        if ((a > b) == ((i & size) == 0)) {
-          list[i] = b;
-          list[j] = a;
+      const bool up = (p0 & size) == 0;
+      if (dist >= 32 * P) {
+        __syncthreads();
+#pragma unroll
+        for (int q = 0; q < P; ++q) buffer[p0 + q] = v[q];
+        __syncthreads();
+        const bool low = (p0 & dist) == 0;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const u64 other = buffer[(p0 + q) ^ dist];
+          v[q] = (low == up) == (other < v[q]) ? other : v[q];
+        }
+      } else if (dist >= P) {
+        const bool low = (p0 & dist) == 0;
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const u64 other = __shfl_xor_sync(0xffffffffu, v[q], dist / P);
+          v[q] = (low == up) == (other < v[q]) ? other : v[q];
+        }
+      } else {
+#pragma unroll
+        for (int q = 0; q < P; ++q) {
+          const int o = dist == 1 ? (q ^ 1) : (q ^ 2) % P;
+          if (o > q) {
+            const bool rising = size < P ? ((p0 + q) & size) == 0 : up;
+            const u64 a = v[q], b = v[o];
+            if ((b < a) == rising) {
+              v[q] = b;
+              v[o] = a;
+            }
+          }
         }
       }
-      if (dist >= 32) __syncthreads();
     }
   __syncthreads();
 }
-// Sorts the m entries of the list; returns the power of two they are padded to.
-__device__ __forceinline__ int sort_tokens(Shared& sh, int m) {
-  int n = 64;
-  while (n < m) n <<= 1;
-  for (int t = m + threadIdx.x; t < n; t += kT) sh.list[t] = ~0ull;
+// Sorts the m entries of the list, into the list, ~0 past them.
+template <int P>
+__device__ __forceinline__ void sort_list(Shared& sh, int m) {
+  u64 v[P];
+  const int p0 = threadIdx.x * P;
+#pragma unroll
+  for (int q = 0; q < P; ++q) v[q] = p0 + q < m ? sh.list[p0 + q] : ~0ull;
+  sort_values<P>(v, sh.list);
+#pragma unroll
+  for (int q = 0; q < P; ++q) sh.list[p0 + q] = v[q];
   __syncthreads();
-  sort_list(sh.list, n);
-  return n;
+}
+// Up to this many tokens are compared pair by pair, which costs less than a
+// sort's 45 rounds (m^2 / 512 comparisons a thread).
+constexpr int kPairs = 256;
+__device__ __forceinline__ void sort_tokens(Shared& sh, int m) {
+  if (m <= kPairs) {
+    const u64 mine = (int)threadIdx.x < m ? sh.list[threadIdx.x] : ~0ull;
+    int place = 0;
+    if ((int)threadIdx.x < m)
+      for (int j = 0; j < m; ++j) place += sh.list[j] < mine;
+    __syncthreads();
+    if ((int)threadIdx.x < m) sh.list[place] = mine;
+    else if (threadIdx.x < 2 * kT) sh.list[threadIdx.x] = ~0ull;
+    __syncthreads();
+  } else if (m <= 2 * kT) {
+    sort_list<2>(sh, m);
+  } else {
+    sort_list<4>(sh, m);
+  }
 }
 
 constexpr int kPer = kList / kT;  // tokens of a sorted list per thread
@@ -361,7 +460,7 @@ __device__ Found locate(Shared& sh, const Slice<STAGED>& row, const Scale& sc, c
     }
     atomicAdd(&sh.hist[0][b], 1u);
   });
-  barrier();
+  barrier<STAGED>();
   u64 count = 0, weight = 0;
   unsigned lower = 0;  // tokens of this thread's bin in the CTAs before this one
 #pragma unroll 4
@@ -428,16 +527,18 @@ __device__ Cut resolve(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Fo
       const int m = (int)f.in_n;
       if (threadIdx.x == 0) sh.fill = f.lower_in;
       __syncthreads();
-      row.each_from(sc.least(part.shift == 64 ? f.b : part.zbin), [&](float x, int i) {
-        if (sub_bin(sc, part, x, i) != f.b) return;
-        if (!limit.keeps(x, i) || (BY_MASS && weight_of(sc.e(x)) == 0)) return;
-        const u64 order = order_of(x, i);
-        const unsigned slot = atomicAdd(&sh.fill, 1u);
-        if (slot < kList)
-          for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order);
-      });
-      barrier();
-      const int n = sort_tokens(sh, m), per = (n + kT - 1) / kT, t0 = threadIdx.x * per;
+      row.collect(
+          sc.least(part.shift == 64 ? f.b : part.zbin), &sh.fill,
+          [&](float x, int i) {
+            return sub_bin(sc, part, x, i) == f.b && limit.keeps(x, i) && (!BY_MASS || weight_of(sc.e(x)) != 0);
+          },
+          [&](unsigned slot, float x, int i) {
+            if (slot < kList)
+              for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order_of(x, i));
+          });
+      barrier<STAGED>();
+      sort_tokens(sh, m);
+      const int per = (m + kT - 1) / kT, t0 = threadIdx.x * per;
       u64 w[kPer], mine = 0, total, last = 0;
 #pragma unroll
       for (int q = 0; q < kPer; ++q) {
@@ -460,7 +561,7 @@ __device__ Cut resolve(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Fo
       __syncthreads();
       return Cut{value_of(~(unsigned)(last >> 32)), (int)(unsigned)last};
     }
-    barrier();  // the histograms are read; divide the bin
+    barrier<STAGED>();  // the histograms are read; divide the bin
     if (part.shift == 64) {
       part.zbin = f.b;
       part.shift = 55;
@@ -507,7 +608,7 @@ __device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice<STAGED>& row, c
     for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
     put64(remote(&sh.mass_of[rank], threadIdx.x), m);
   }
-  barrier();
+  barrier<STAGED>();
   u64 total = 0;
   before = 0;
   for (unsigned c = 0; c < ctas; ++c) {
@@ -524,7 +625,8 @@ __device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice<STAGED>& row, c
 __device__ void finish(Shared& sh, u64* mass_s, const Scale& sc, const Args& a, int r, int m, int k, u64 want,
                        bool by_mass, u64 share_p, float floor_e) {
   // consecutive tokens per thread
-  const int n = sort_tokens(sh, m), per = (n + kT - 1) / kT, t0 = threadIdx.x * per;
+  sort_tokens(sh, m);
+  const int per = (m + kT - 1) / kT, t0 = threadIdx.x * per;
   u64 w[kPer], mine = 0;
   float e[kPer];
 #pragma unroll
@@ -550,20 +652,20 @@ __device__ void finish(Shared& sh, u64* mass_s, const Scale& sc, const Args& a, 
   // the kept ones in the order of their indexes
 #pragma unroll
   for (int q = 0; q < kPer; ++q)
-    if (q < per && t0 + q < n) {
+    if (q < per && t0 + q < m) {
       mass_s[t0 + q] = w[q];
-      sh.list[t0 + q] = w[q] ? (sh.list[t0 + q] << 32) | (unsigned)(t0 + q) : ~0ull;
+      sh.list[t0 + q] = w[q] ? (sh.list[t0 + q] << 32) | (unsigned)(t0 + q) : ~0ull - (unsigned)(t0 + q);
     }
   scan1(sh, mine, total);
-  sort_list(sh.list, n);
+  sort_tokens(sh, m);
   const float uf = fminf(fmaxf(a.u[r], 0.0f), 1.0f);
   const u64 ui = min((u64)__fmul_rn(uf, 16777216.0f), (u64)(1u << kGrid) - 1);
   const u64 aim = scaled(total, ui, 0);
   mine = 0;
 #pragma unroll
   for (int q = 0; q < kPer; ++q) {
-    const u64 entry = q < per && t0 + q < n ? sh.list[t0 + q] : ~0ull;
-    w[q] = entry == ~0ull ? 0 : mass_s[(unsigned)entry];
+    const u64 entry = q < per && t0 + q < m ? sh.list[t0 + q] : ~0ull;
+    w[q] = entry >> 32 == 0xffffffffu ? 0 : mass_s[(unsigned)entry];
     mine += w[q];
   }
   u64 ignored;
@@ -651,7 +753,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
     warp_max[warp] = top;
     warp_min[warp] = low;
   }
-  barrier();  // every CTA of the cluster runs before its shared memory is written to
+  barrier<STAGED>();  // every CTA of the cluster runs before its shared memory is written to
   if (threadIdx.x < ctas) {
     for (int w = 0; w < kW; ++w) {
       top = fmaxf(top, warp_max[w]);
@@ -660,7 +762,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
     put32(remote(&sh.max_of[rank], threadIdx.x), __float_as_uint(top));
     put32(remote(&sh.min_of[rank], threadIdx.x), __float_as_uint(low));
   }
-  barrier();
+  barrier<STAGED>();
   top = -INFINITY;
   low = INFINITY;
   for (unsigned c = 0; c < ctas; ++c) {
@@ -688,7 +790,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
     if (lane == 0) atomicMin(&sh.fill, first);
     __syncthreads();
     if (threadIdx.x == 0) put32(remote(&sh.first_of[rank], 0), sh.fill);
-    barrier();
+    barrier<STAGED>();
     if (rank == 0 && threadIdx.x == 0) {
       for (unsigned c = 0; c < ctas; ++c) first = min(first, sh.first_of[c]);
       a.token[r] = (int)first;
@@ -725,12 +827,13 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
       const unsigned upto = min(f.b, (unsigned)kBins - 1);
       if (threadIdx.x == 0) sh.fill = f.lower_upto;
       __syncthreads();
-      row.each_from(sc.least(upto), [&](float v, int i) {
-        if (sc.bin(v) > upto || (!by_count && weight_of(sc.e(v)) == 0)) return;
-        const unsigned slot = atomicAdd(&sh.fill, 1u);
-        if (slot < kList) put64(remote(&sh.list[slot], 0), order_of(v, i));
-      });
-      barrier();
+      row.collect(
+          sc.least(upto), &sh.fill,
+          [&](float v, int) { return sc.bin(v) <= upto && (by_count || weight_of(sc.e(v)) != 0); },
+          [&](unsigned slot, float v, int i) {
+            if (slot < kList) put64(remote(&sh.list[slot], 0), order_of(v, i));
+          });
+      barrier<STAGED>();
       if (rank == 0)
         finish(sh, reinterpret_cast<u64*>(x_s), sc, a, r, (int)(f.above_n + f.in_n), by_count ? k : a.n,
                by_count ? 0 : f.want, by_mass, share_p, floor_e);
