@@ -3,6 +3,8 @@
 #pragma once
 
 #include <cuda_runtime.h>
+
+#include <atomic>
 #include <cstdint>
 
 namespace hyq {
@@ -123,6 +125,21 @@ cudaError_t launch_ex(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, c
   cfg.attrs = attr;
   cfg.numAttrs = launch_overlap() ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, k, static_cast<KArgs>(args)...);
+}
+
+// cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel, set once per device
+// (`done` holds a bit per device ordinal; concurrent first calls may set it
+// twice).
+template <typename K>
+cudaError_t allow_smem(K k, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  cudaError_t e = cudaGetDevice(&dev);
+  if (e != cudaSuccess) return e;
+  const uint64_t bit = 1ull << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) != cudaSuccess) return e;
+  done.fetch_or(bit, std::memory_order_release);
+  return cudaSuccess;
 }
 
 }  // namespace hyq

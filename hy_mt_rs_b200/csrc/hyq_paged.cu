@@ -304,9 +304,10 @@ size_t attend_smem(int dim, int group) {
 template <bool KV16>
 cudaError_t launch_attend(const AttendArgs& a, cudaStream_t st) {
   const int group = a.heads / a.c.kv_heads, outs = (group * a.c.dim + kThreads - 1) / kThreads;
-  auto k = outs <= 4 ? attend_kernel<KV16, 4> : outs <= 8 ? attend_kernel<KV16, 8> : attend_kernel<KV16, 32>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize,
-                                       (int)attend_smem(kMaxDim, kMaxGroup));
+  const int variant = outs <= 4 ? 0 : outs <= 8 ? 1 : 2;
+  auto k = variant == 0 ? attend_kernel<KV16, 4> : variant == 1 ? attend_kernel<KV16, 8> : attend_kernel<KV16, 32>;
+  static std::atomic<uint64_t> done[3] = {};
+  const cudaError_t e = allow_smem(k, (int)attend_smem(kMaxDim, kMaxGroup), done[variant]);
   if (e != cudaSuccess) return e;
   return launch_ex(k, dim3((unsigned)a.c.tokens, (unsigned)a.c.kv_heads), dim3(kThreads),
                    attend_smem(a.c.dim, group), st, a);

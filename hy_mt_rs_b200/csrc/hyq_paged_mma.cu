@@ -764,15 +764,16 @@ cudaError_t launch(const AttendArgs& a, int64_t max_new, cudaStream_t st) {
   if (max_new * group > kRows) {
     const int64_t tiles = ((int64_t)a.c.tokens * group + kChunkRows - 1) / kChunkRows + a.c.seqs;
     auto k = chunk_kernel<DIM, KV16>;
-    if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, G::smem)) != cudaSuccess) return e;
+    static std::atomic<uint64_t> done{0};
+    if ((e = allow_smem(k, G::smem, done)) != cudaSuccess) return e;
     if ((e = launch_ex(k, dim3((unsigned)tiles, (unsigned)a.c.kv_heads), dim3(kThreads), G::smem, st, a, shift)) != cudaSuccess)
       return e;
   }
   // (one token per sequence is the fewest there can be: the rows of a
   // sequence fit one tile of 16 unless every sequence has a chunk)
   auto k = few_kernel<DIM, KV16>;
-  const int smem = G::smem + (kMaxSeqs + 1) * 4;
-  if ((e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, smem)) != cudaSuccess) return e;
+  static std::atomic<uint64_t> done{0};
+  if ((e = allow_smem(k, G::smem + (kMaxSeqs + 1) * 4, done)) != cudaSuccess) return e;
   return launch_ex(k, dim3(kMaxCtas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4, st, a, shift);
 }
 

@@ -899,7 +899,8 @@ cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
     return launch_ex(sample_kernel<false>, dim3((unsigned)rows), dim3(kT), kList * sizeof(u64), st, a, slice);
   // (at least two units: the first CTA keeps a sorted list's masses there)
   auto k = sample_kernel<true>;
-  cudaError_t e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, kMaxSlice * (int)sizeof(float));
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(k, kMaxSlice * (int)sizeof(float), done);
   if (e != cudaSuccess) return e;
   if (ctas > 8 && (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];

@@ -11,80 +11,82 @@ slot[s] of the table (row s without slots).  Indexes are device int32 tensors.
 Every call runs on the current torch CUDA stream.
 """
 import ctypes as C
+import functools
+import struct
 
 import torch
 
 from ._native import HyqError, check, lib
-from .quant import _need_cuda, _ptr, _stream
+from .quant import _need_cuda, _ptr
 
 __all__ = ["PagedCache", "rope_append", "attention", "attention_workspace"]
 
 _KV_TYPES = {torch.float32: 0, torch.float16: 1}   # HYQ_KV_F32, HYQ_KV_F16
 
+# The structures of include/hyq.h as packed bytes (a call at a decode step's
+# sizes takes a few microseconds on the device: the host side counts).
+_KV = struct.Struct("PPiiiiqqqqPqq")     # hyq_paged_kv
+_BATCH = struct.Struct("PPPqqqq")        # hyq_paged_batch
+_PAGES = struct.Struct("PPPPqqqi4x")     # hyq_pages
+_POOL = struct.Struct("Pqqqq")           # hyq_page_pool
 
-class _Kv(C.Structure):
-    """hyq_paged_kv (include/hyq.h)."""
-    _fields_ = [("k", C.c_void_p), ("v", C.c_void_p), ("dtype", C.c_int), ("kv_heads", C.c_int),
-                ("head_dim", C.c_int), ("page_size", C.c_int), ("pages", C.c_int64), ("page_stride", C.c_int64),
-                ("head_stride", C.c_int64), ("row_stride", C.c_int64), ("table", C.c_void_p), ("slots", C.c_int64),
-                ("table_width", C.c_int64)]
-
-
-class _Batch(C.Structure):
-    """hyq_paged_batch (include/hyq.h)."""
-    _fields_ = [("slot", C.c_void_p), ("row_start", C.c_void_p), ("pos", C.c_void_p), ("seqs", C.c_int64),
-                ("tokens", C.c_int64), ("max_new", C.c_int64), ("max_len", C.c_int64)]
+_current_stream = torch._C._cuda_getCurrentRawStream
 
 
-class _Pages(C.Structure):
-    """hyq_pages (include/hyq.h)."""
-    _fields_ = [("table", C.c_void_p), ("length", C.c_void_p), ("refs", C.c_void_p), ("shortage", C.c_void_p),
-                ("slots", C.c_int64), ("table_width", C.c_int64), ("pages", C.c_int64), ("page_size", C.c_int)]
+def _check_int(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
+        _need_cuda(t, name, torch.int32)
 
 
-class _Pool(C.Structure):
-    """hyq_page_pool (include/hyq.h)."""
-    _fields_ = [("base", C.c_void_p), ("planes", C.c_int64), ("plane_stride", C.c_int64), ("page_stride", C.c_int64),
-                ("page_bytes", C.c_int64)]
+def _check_f32(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous():
+        _need_cuda(t, name, torch.float32)
 
 
 def _kv(k_pages, v_pages, table):
+    """hyq_paged_kv of a layer's pages; (packed, kv_heads, page_size, head_dim, table_width)."""
     for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
         if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _KV_TYPES:
             raise HyqError(-1, f"{name}: expected a CUDA float32 or float16 tensor")
-        if t.dim() != 4 or t.stride(3) != 1:
-            raise HyqError(-2, f"{name}: expected [pages, kv_heads, page_size, head_dim], contiguous in head_dim")
-    if k_pages.shape != v_pages.shape or k_pages.stride() != v_pages.stride() or k_pages.dtype != v_pages.dtype:
+    shape, strides, dtype = k_pages.shape, k_pages.stride(), k_pages.dtype
+    if len(shape) != 4 or strides[3] != 1:
+        raise HyqError(-2, "k_pages: expected [pages, kv_heads, page_size, head_dim], contiguous in head_dim")
+    if shape != v_pages.shape or strides != v_pages.stride() or dtype != v_pages.dtype:
         raise HyqError(-2, "k_pages and v_pages differ in shape, strides or type")
-    _need_cuda(table, "table", torch.int32)
-    if table.dim() != 2:
+    _check_int(table, "table")
+    rows = table.shape
+    if len(rows) != 2:
         raise HyqError(-2, "table: expected [slots, table_width]")
-    pages, heads, page, dim = k_pages.shape
-    return _Kv(k_pages.data_ptr(), v_pages.data_ptr(), _KV_TYPES[k_pages.dtype], heads, dim, page, pages,
-               k_pages.stride(0), k_pages.stride(1), k_pages.stride(2), table.data_ptr(), table.shape[0], table.shape[1])
+    pages, heads, page, dim = shape
+    return (_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), _KV_TYPES[dtype], heads, dim, page, pages, strides[0],
+                     strides[1], strides[2], table.data_ptr(), rows[0], rows[1]), heads, page, dim, rows[1])
 
 
 def _batch(row_start, pos, slot, tokens, max_new, max_len):
-    _need_cuda(row_start, "row_start", torch.int32)
-    _need_cuda(pos, "pos", torch.int32)
+    _check_int(row_start, "row_start")
+    _check_int(pos, "pos")
     seqs = pos.numel()
     if row_start.numel() != seqs + 1:
         raise HyqError(-2, "row_start takes one more entry than pos")
     if slot is not None:
-        _need_cuda(slot, "slot", torch.int32)
+        _check_int(slot, "slot")
         if slot.numel() != seqs:
             raise HyqError(-2, "slot takes one entry per sequence")
-    return _Batch(None if slot is None else slot.data_ptr(), row_start.data_ptr(), pos.data_ptr(), seqs, tokens,
-                  max_new, max_len)
+    if max_new < 0 or max_len < 0:
+        raise HyqError(-2, "max_new and max_len are not negative")
+    return _BATCH.pack(0 if slot is None else slot.data_ptr(), row_start.data_ptr(), pos.data_ptr(), seqs, tokens,
+                       max_new, max_len)
 
 
 def _heads(t, name):
-    """[tokens, heads, head_dim] float32 activations whose heads are contiguous."""
+    """Shape and row stride of [tokens, heads, head_dim] float32 activations
+    whose heads are contiguous."""
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
         raise HyqError(-1, f"{name}: expected a CUDA float32 tensor")
-    if t.dim() != 3 or t.stride(2) != 1 or t.stride(1) != t.shape[2]:
+    shape, strides = t.shape, t.stride()
+    if len(shape) != 3 or strides[2] != 1 or (strides[1] != shape[2] and shape[1] > 1):
         raise HyqError(-2, f"{name}: expected [tokens, heads, head_dim] with contiguous heads")
-    return max(t.stride(0), t.shape[1] * t.shape[2])
+    return shape, (strides[0] if shape[0] > 1 else shape[1] * shape[2])
 
 
 def rope_append(q, k, v, k_pages, v_pages, table, row_start, pos, cos, sin, q_norm=None, k_norm=None, eps=1e-5,
@@ -94,36 +96,44 @@ def rope_append(q, k, v, k_pages, v_pages, table, row_start, pos, cos, sin, q_no
     write k and v into the pages, return the rotated queries (into `out` when
     given; q itself is allowed).  cos and sin are [positions, head_dim / 2]
     (hyq_rope_table); norm_first normalises before the rotation."""
-    kv = _kv(k_pages, v_pages, table)
-    qs, ks, vs = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
-    out = torch.empty(q.shape, device=q.device) if out is None else out
-    os = _heads(out, "out")
-    if q.shape[2] != kv.head_dim or out.shape != q.shape or k.shape != (q.shape[0], kv.kv_heads, kv.head_dim) \
-            or v.shape != k.shape:
+    kv, kv_heads, _, dim, _ = _kv(k_pages, v_pages, table)
+    (shape, qs), (k_shape, ks), (v_shape, vs) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=q.device)
+    out_shape, os = _heads(out, "out")
+    if shape[2] != dim or out_shape != shape or k_shape != (shape[0], kv_heads, dim) or v_shape != k_shape:
         raise HyqError(-2, "rope_append: shapes of q, k, v and out")
-    for t, name, shape in ((cos, "cos", None), (sin, "sin", None), (q_norm, "q_norm", (kv.head_dim,)),
-                           (k_norm, "k_norm", (kv.head_dim,))):
-        if t is None and shape:
-            continue
-        _need_cuda(t, name, torch.float32)
-        if t.shape != shape if shape else t.dim() != 2 or t.shape != cos.shape or t.shape[1] * 2 != kv.head_dim:
-            raise HyqError(-2, f"rope_append: shape of {name}")
-    # every position of a sequence is below the table's reach, so max_new and
-    # max_len (attention's bounds) are not needed here
-    b = _batch(row_start, pos, slot, q.shape[0], 0, 0)
-    opt = lambda t: C.c_void_p(None) if t is None else _ptr(t)  # noqa: E731
-    check(lib.hyq_paged_rope_append(C.byref(kv), C.byref(b), _ptr(q), qs, q.shape[1], _ptr(k), ks, _ptr(v), vs,
-                                    _ptr(cos), _ptr(sin), cos.shape[0], opt(q_norm), opt(k_norm), eps,
-                                    1 if norm_first else 0, _ptr(out), os, _stream(q.device)))
+    _check_f32(cos, "cos")
+    _check_f32(sin, "sin")
+    rows = cos.shape
+    if len(rows) != 2 or rows != sin.shape or rows[1] * 2 != dim:
+        raise HyqError(-2, "rope_append: cos and sin are [positions, head_dim / 2]")
+    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
+        if w is not None:
+            _check_f32(w, name)
+            if w.shape != (dim,):
+                raise HyqError(-2, f"rope_append: shape of {name}")
+    # (positions are checked against the table's reach on the device; max_new
+    # and max_len bound attention's work only)
+    batch = _batch(row_start, pos, slot, shape[0], 0, 0)
+    check(lib.hyq_paged_rope_append(kv, batch, q.data_ptr(), qs, shape[1], k.data_ptr(), ks, v.data_ptr(), vs,
+                                    cos.data_ptr(), sin.data_ptr(), rows[0], None if q_norm is None else q_norm.data_ptr(),
+                                    None if k_norm is None else k_norm.data_ptr(), eps, 1 if norm_first else 0,
+                                    out.data_ptr(), os, _current_stream(q.get_device())))
     return out
+
+
+@functools.lru_cache(maxsize=None)
+def _workspace_bytes(heads, head_dim):
+    n = C.c_size_t()
+    check(lib.hyq_paged_attention_workspace_bytes(heads, head_dim, C.byref(n)))
+    return n.value
 
 
 def attention_workspace(heads, head_dim, device):
     """A zeroed workspace for attention() calls with these heads (any batch);
     calls that share one must not overlap in time."""
-    n = C.c_size_t()
-    check(lib.hyq_paged_attention_workspace_bytes(heads, head_dim, C.byref(n)))
-    return torch.zeros(n.value, dtype=torch.uint8, device=device)
+    return torch.zeros(_workspace_bytes(heads, head_dim), dtype=torch.uint8, device=device)
 
 
 def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None, slot=None, out=None, workspace=None):
@@ -133,24 +143,23 @@ def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None,
     when given).  max_new and max_len bound any sequence's new tokens and its
     length after them (max_len: the table's reach by default).  workspace:
     attention_workspace(...), made here when not given."""
-    kv = _kv(k_pages, v_pages, table)
-    qs = _heads(q, "q")
-    out = torch.empty(q.shape, device=q.device) if out is None else out
-    os = _heads(out, "out")
-    if q.shape[2] != kv.head_dim or out.shape != q.shape:
+    kv, _, page, dim, width = _kv(k_pages, v_pages, table)
+    shape, qs = _heads(q, "q")
+    if out is None:
+        out = torch.empty(shape, dtype=torch.float32, device=q.device)
+    out_shape, os = _heads(out, "out")
+    if shape[2] != dim or out_shape != shape:
         raise HyqError(-2, "attention: shapes of q and out")
-    if max_len is None:
-        max_len = kv.table_width * kv.page_size
-    b = _batch(row_start, pos, slot, q.shape[0], max_new, max_len)
+    batch = _batch(row_start, pos, slot, shape[0], max_new, width * page if max_len is None else max_len)
     if workspace is None:
-        workspace = attention_workspace(q.shape[1], kv.head_dim, q.device)
-    _need_cuda(workspace, "workspace", torch.uint8)
-    need = C.c_size_t()
-    check(lib.hyq_paged_attention_workspace_bytes(q.shape[1], kv.head_dim, C.byref(need)))
-    if workspace.numel() < need.value:
-        raise HyqError(-2, f"attention: the workspace takes {need.value} bytes")
-    check(lib.hyq_paged_attention(C.byref(kv), C.byref(b), _ptr(q), qs, q.shape[1], _ptr(out), os, _ptr(workspace),
-                                  _stream(q.device)))
+        workspace = attention_workspace(shape[1], dim, q.device)
+    elif not isinstance(workspace, torch.Tensor) or not workspace.is_cuda or workspace.dtype != torch.uint8 \
+            or not workspace.is_contiguous():
+        _need_cuda(workspace, "workspace", torch.uint8)
+    if workspace.numel() < _workspace_bytes(shape[1], dim):
+        raise HyqError(-2, f"attention: the workspace takes {_workspace_bytes(shape[1], dim)} bytes")
+    check(lib.hyq_paged_attention(kv, batch, q.data_ptr(), qs, shape[1], out.data_ptr(), os, workspace.data_ptr(),
+                                  _current_stream(q.get_device())))
     return out
 
 
@@ -195,45 +204,45 @@ class PagedCache:
         n = C.c_size_t()
         check(lib.hyq_pages_workspace_bytes(self.pages, C.byref(n)))
         self._ws = torch.empty(n.value, dtype=torch.uint8, device=pool.device)
-        self._pages = _Pages(table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.shortage.data_ptr(),
-                             table.shape[0], table.shape[1], self.pages, self.page_size)
+        self._pages = _PAGES.pack(table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.shortage.data_ptr(),
+                                  table.shape[0], table.shape[1], self.pages, self.page_size)
         page = pool[0, 0, 0].numel() * pool.element_size()
-        self._pool = _Pool(pool.data_ptr(), 2 * pool.shape[0], page * self.pages, page, page)
+        self._pool = _POOL.pack(pool.data_ptr(), 2 * pool.shape[0], page * self.pages, page, page)
 
     def layer(self, i):
         """(k_pages, v_pages) of a layer."""
         return self.pool[i, 0], self.pool[i, 1]
 
     def _slots(self, *arrays):
+        n = arrays[0].numel() if isinstance(arrays[0], torch.Tensor) else 0
         for t in arrays:
-            _need_cuda(t, "slots", torch.int32)
-            if t.numel() != arrays[0].numel():
+            _check_int(t, "slots")
+            if t.numel() != n:
                 raise HyqError(-2, "PagedCache: arrays of one call differ in length")
-        return arrays[0].numel()
+        return n
 
     def reserve(self, slot, extra, pos=None):
         """Grow sequence slot[i] by extra[i] positions; their first positions
         (int32, into `pos` when given)."""
-        n = self._slots(slot, extra)
-        pos = torch.empty(n, dtype=torch.int32, device=slot.device) if pos is None else pos
-        self._slots(slot, pos)
-        check(lib.hyq_pages_reserve(C.byref(self._pages), _ptr(slot), _ptr(extra), n, _ptr(pos), _ptr(self._ws),
-                                    _stream(slot.device)))
+        if pos is None:
+            pos = torch.empty(slot.shape, dtype=torch.int32, device=slot.device)
+        n = self._slots(slot, extra, pos)
+        check(lib.hyq_pages_reserve(self._pages, slot.data_ptr(), extra.data_ptr(), n, pos.data_ptr(), _ptr(self._ws),
+                                    _current_stream(slot.get_device())))
         return pos
 
     def free(self, slot):
         """Give the sequences' pages back."""
         n = self._slots(slot)
-        check(lib.hyq_pages_free(C.byref(self._pages), _ptr(slot), n, _stream(slot.device)))
+        check(lib.hyq_pages_free(self._pages, slot.data_ptr(), n, _current_stream(slot.get_device())))
 
     def fork(self, src, dst):
         """Sequence dst[i] becomes a copy of src[i]: full pages shared, the
         partial page copied in every layer."""
         n = self._slots(src, dst)
-        check(lib.hyq_pages_fork(C.byref(self._pages), C.byref(self._pool), _ptr(src), _ptr(dst), n, _ptr(self._ws),
-                                 _stream(src.device)))
+        check(lib.hyq_pages_fork(self._pages, self._pool, src.data_ptr(), dst.data_ptr(), n, _ptr(self._ws),
+                                 _current_stream(src.get_device())))
 
     def compact(self):
         """Move the live pages to the front of the pool, in every layer."""
-        check(lib.hyq_pages_compact(C.byref(self._pages), C.byref(self._pool), _ptr(self._ws),
-                                    _stream(self.pool.device)))
+        check(lib.hyq_pages_compact(self._pages, self._pool, _ptr(self._ws), _current_stream(self.pool.get_device())))

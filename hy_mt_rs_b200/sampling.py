@@ -5,26 +5,22 @@ top-p); here one launch samples every row of a batch of logits from uniform
 numbers the caller provides, so a decode loop needs no host round trip and a
 draw can be repeated.
 """
-import ctypes as C
-
 import torch
 
 from ._native import HyqError, check, lib
-from .quant import _need_cuda, _ptr, _stream
+from .quant import _need_cuda
 
 __all__ = ["sample"]
 
+_current_stream = torch._C._cuda_getCurrentRawStream
 
-def _per_row(value, rows, dtype, name, device):
-    """A parameter as a device array of one value per row (None: off)."""
-    if value is None:
-        return None
-    if not isinstance(value, torch.Tensor):
-        return torch.full((rows,), value, dtype=dtype, device=device)
-    _need_cuda(value, name, dtype)
-    if value.numel() != rows:
+
+def _check(t, name, dtype, rows):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != dtype or not t.is_contiguous():
+        _need_cuda(t, name, dtype)
+    if t.numel() != rows:
         raise HyqError(-2, f"sample: {name} takes one value per row")
-    return value
+    return t.data_ptr()
 
 
 def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, token=None, prob=None):
@@ -39,23 +35,28 @@ def sample(logits, u, temperature=None, top_k=None, top_p=None, min_p=None, toke
     token and prob may be given to be written."""
     if not isinstance(logits, torch.Tensor) or not logits.is_cuda or logits.dtype != torch.float32:
         raise HyqError(-1, "sample: logits are a CUDA float32 tensor")
-    if logits.dim() != 2 or (logits.shape[1] > 1 and logits.stride(1) != 1):
+    shape, strides = logits.shape, logits.stride()
+    if len(shape) != 2 or (shape[1] > 1 and strides[1] != 1):
         raise HyqError(-2, "sample: logits are [rows, n] with contiguous rows")
-    rows, n = logits.shape
+    rows, n = shape
     dev = logits.device
-    _need_cuda(u, "u", torch.float32)
-    if u.numel() != rows:
-        raise HyqError(-2, "sample: u takes one number per row")
-    token = torch.empty(rows, dtype=torch.int32, device=dev) if token is None else token
-    prob = torch.empty(rows, dtype=torch.float32, device=dev) if prob is None else prob
-    _need_cuda(token, "token", torch.int32)
-    _need_cuda(prob, "prob", torch.float32)
-    if token.numel() != rows or prob.numel() != rows:
-        raise HyqError(-2, "sample: invalid output buffer")
-    params = [_per_row(temperature, rows, torch.float32, "temperature", dev),
-              _per_row(top_k, rows, torch.int32, "top_k", dev), _per_row(top_p, rows, torch.float32, "top_p", dev),
-              _per_row(min_p, rows, torch.float32, "min_p", dev)]
-    opt = lambda t: C.c_void_p(None) if t is None else _ptr(t)  # noqa: E731
-    check(lib.hyq_sample(_ptr(logits), n, max(logits.stride(0), n), rows, *(opt(t) for t in params), _ptr(u),
-                         _ptr(token), _ptr(prob), _stream(dev)))
+    kept = []   # tensors made here live until the launch
+
+    def per_row(value, name, dtype):
+        if value is None:
+            return None
+        if not isinstance(value, torch.Tensor):
+            kept.append(torch.full((rows,), value, dtype=dtype, device=dev))
+            return kept[-1].data_ptr()
+        return _check(value, name, dtype, rows)
+
+    if token is None:
+        token = torch.empty(rows, dtype=torch.int32, device=dev)
+    if prob is None:
+        prob = torch.empty(rows, dtype=torch.float32, device=dev)
+    check(lib.hyq_sample(logits.data_ptr(), n, strides[0] if rows > 1 else n, rows,
+                         per_row(temperature, "temperature", torch.float32), per_row(top_k, "top_k", torch.int32),
+                         per_row(top_p, "top_p", torch.float32), per_row(min_p, "min_p", torch.float32),
+                         _check(u, "u", torch.float32, rows), _check(token, "token", torch.int32, rows),
+                         _check(prob, "prob", torch.float32, rows), _current_stream(logits.get_device())))
     return token, prob

@@ -9,18 +9,18 @@ PTR = 0x10000     # never read: every call here is refused on the host, or has n
 
 
 def _kv(**kw):
-    from hy_mt_rs_b200.paged import _Kv
+    from hy_mt_rs_b200.paged import _KV
     d = dict(k=PTR, v=PTR, dtype=1, kv_heads=2, head_dim=128, page_size=16, pages=10, page_stride=2 * 16 * 128,
              head_stride=16 * 128, row_stride=128, table=PTR, slots=4, table_width=8)
     d.update(kw)
-    return _Kv(**d)
+    return _KV.pack(*(v or 0 for v in d.values()))
 
 
 def _batch(**kw):
-    from hy_mt_rs_b200.paged import _Batch
+    from hy_mt_rs_b200.paged import _BATCH
     d = dict(slot=None, row_start=PTR, pos=PTR, seqs=2, tokens=3, max_new=2, max_len=100)
     d.update(kw)
-    return _Batch(**d)
+    return _BATCH.pack(*(v or 0 for v in d.values()))
 
 
 KV = [(dict(k=None), INVALID), (dict(v=None), INVALID), (dict(table=None), INVALID), (dict(dtype=2), INVALID),
@@ -36,13 +36,13 @@ BATCH = [(dict(row_start=None), INVALID), (dict(pos=None), INVALID), (dict(seqs=
 
 def _attention(kv, b, q=PTR, q_stride=512, heads=4, out=PTR, out_stride=512, ws=PTR):
     from hy_mt_rs_b200._native import lib
-    return lib.hyq_paged_attention(C.byref(kv) if kv else None, C.byref(b) if b else None, q, q_stride, heads, out, out_stride, ws, None)
+    return lib.hyq_paged_attention(kv, b, q, q_stride, heads, out, out_stride, ws, None)
 
 
 def _append(kv, b, q=PTR, q_stride=512, heads=4, k=PTR, k_stride=256, v=PTR, v_stride=256, cos=PTR, sin=PTR, positions=64,
             out=PTR, out_stride=512):
     from hy_mt_rs_b200._native import lib
-    return lib.hyq_paged_rope_append(C.byref(kv) if kv else None, C.byref(b) if b else None, q, q_stride, heads, k, k_stride, v,
+    return lib.hyq_paged_rope_append(kv, b, q, q_stride, heads, k, k_stride, v,
                                      v_stride, cos, sin, positions, None, None, 1e-5, 0, out, out_stride, None)
 
 
@@ -71,31 +71,31 @@ def test_attention_workspace_bytes():
 
 
 def _pages(**kw):
-    from hy_mt_rs_b200.paged import _Pages
+    from hy_mt_rs_b200.paged import _PAGES
     d = dict(table=PTR, length=PTR, refs=PTR, shortage=PTR, slots=4, table_width=8, pages=10, page_size=16)
     d.update(kw)
-    return _Pages(**d)
+    return _PAGES.pack(*(v or 0 for v in d.values()))
 
 
 def _pool(**kw):
-    from hy_mt_rs_b200.paged import _Pool
+    from hy_mt_rs_b200.paged import _POOL
     d = dict(base=PTR, planes=4, plane_stride=10 * 4096, page_stride=4096, page_bytes=4096)
     d.update(kw)
-    return _Pool(**d)
+    return _POOL.pack(*(v or 0 for v in d.values()))
 
 
 def test_pages_checks():
     from hy_mt_rs_b200._native import lib
-    calls = [lambda p, n=1, a=PTR: lib.hyq_pages_reserve(C.byref(p), a, PTR, n, None, PTR, None),
-             lambda p, n=1, a=PTR: lib.hyq_pages_free(C.byref(p), a, n, None),
-             lambda p, n=1, a=PTR: lib.hyq_pages_fork(C.byref(p), C.byref(_pool()), a, PTR, n, PTR, None)]
+    calls = [lambda p, n=1, a=PTR: lib.hyq_pages_reserve(p, a, PTR, n, None, PTR, None),
+             lambda p, n=1, a=PTR: lib.hyq_pages_free(p, a, n, None),
+             lambda p, n=1, a=PTR: lib.hyq_pages_fork(p, _pool(), a, PTR, n, PTR, None)]
     bad = [(dict(table=None), INVALID), (dict(length=None), INVALID), (dict(refs=None), INVALID), (dict(shortage=None), INVALID),
            (dict(slots=0), SHAPE), (dict(table_width=0), SHAPE), (dict(pages=0), SHAPE), (dict(page_size=0), SHAPE),
            (dict(table_width=1 << 31), SHAPE), (dict(pages=1 << 31), SHAPE), (dict(refs=PTR + 1), ALIGN)]
     for kw, code in bad:
         for call in calls:
             assert call(_pages(**kw)) == code, kw
-        assert lib.hyq_pages_compact(C.byref(_pages(**kw)), C.byref(_pool()), PTR, None) == code
+        assert lib.hyq_pages_compact(_pages(**kw), _pool(), PTR, None) == code
     pool = [(dict(base=None), INVALID), (dict(planes=0), SHAPE), (dict(page_bytes=0), SHAPE), (dict(page_stride=16), SHAPE),
             (dict(plane_stride=16), SHAPE), (dict(base=PTR + 8), ALIGN), (dict(page_bytes=4088), ALIGN),
             (dict(plane_stride=40968), ALIGN)]
@@ -108,7 +108,7 @@ def test_pages_checks():
             assert call(_pages(), a=None) == INVALID
             assert call(_pages(), a=PTR + 2) == ALIGN
         for kw, code in pool:
-            assert lib.hyq_pages_compact(C.byref(_pages()), C.byref(_pool(**kw)), PTR, None) == code, kw
+            assert lib.hyq_pages_compact(_pages(), _pool(**kw), PTR, None) == code, kw
     n = C.c_size_t()
     assert lib.hyq_pages_workspace_bytes(10, C.byref(n)) == 0 and n.value >= 120
     assert lib.hyq_pages_workspace_bytes(0, C.byref(n)) == SHAPE
