@@ -426,7 +426,7 @@ int hyq_paged_attention_workspace_bytes(int heads, int head_dim, size_t* bytes) 
   if (!bytes) return api_fail(HYQ_E_INVALID, "paged_attention_workspace_bytes: null pointer");
   if (heads <= 0 || head_dim <= 0 || head_dim > hyq::paged::kMaxDim)
     return api_fail(HYQ_E_SHAPE, "paged_attention_workspace_bytes: shape");
-  *bytes = hyq::paged::mma_workspace_bytes(head_dim);
+  *bytes = hyq::paged::mma_workspace_bytes(head_dim) + hyq::paged::tc_workspace_bytes(head_dim);
   return HYQ_OK;
 }
 
@@ -450,7 +450,14 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
   a.ws = workspace;
   const cudaStream_t st = (cudaStream_t)stream;
   const bool kv16 = kv->dtype == HYQ_KV_F16;
-  if (hyq::paged::mma_supported(a, kv16)) return done(hyq::paged::launch_mma(a, kv16, batch->max_new, st), name);
+  if (hyq::paged::mma_supported(a, kv16)) {
+    cudaError_t e = cudaSuccess;
+    if (batch->max_new * (heads / kv->kv_heads) > hyq::paged::kFewRows)
+      e = hyq::paged::tc_supported(a, kv16) ? hyq::paged::launch_chunks_tc(a, batch->max_len, st)
+                                            : hyq::paged::launch_chunks(a, kv16, st);
+    if (e == cudaSuccess) e = hyq::paged::launch_few(a, kv16, st);
+    return done(e, name);
+  }
   return done(kv16 ? hyq::paged::launch_attend<true>(a, st) : hyq::paged::launch_attend<false>(a, st), name);
 }
 

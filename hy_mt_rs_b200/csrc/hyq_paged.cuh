@@ -83,6 +83,40 @@ __device__ __forceinline__ int checked_page(const Cache& c, int page) {
   return -1;
 }
 
+// A tile of `rows` of a sequence's (token, query head) rows of one kv head.
+// Tiles are numbered over the sequences with more than kFewRows such rows.
+constexpr int kFewRows = 16;
+
+// The sequence and the tile within it of tile `want`; false past the last.
+// By a whole warp.
+__device__ __forceinline__ bool find_tile(const Cache& c, int group, int rows, int want, int& seq, int& tile) {
+  const int lane = threadIdx.x & 31;
+  int carry = 0;
+  for (int s0 = 0; s0 < c.seqs; s0 += 32) {
+    int tiles = 0;
+    if (s0 + lane < c.seqs) {
+      const Seq s = load_seq(c, s0 + lane);
+      if (s.n * group > kFewRows) tiles = (s.n * group + rows - 1) / rows;
+    }
+    int x = tiles;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    const int before = carry + x - tiles;
+    const unsigned hit = __ballot_sync(0xffffffffu, before <= want && want < before + tiles);
+    if (hit) {
+      const int l = __ffs(hit) - 1;
+      seq = s0 + l;
+      tile = want - __shfl_sync(0xffffffffu, before, l);
+      return true;
+    }
+    carry += __shfl_sync(0xffffffffu, x, 31);
+  }
+  return false;
+}
+
 // hyq_paged_attention's activations and output.
 struct AttendArgs {
   Cache c;
@@ -101,7 +135,31 @@ constexpr int kMaxSeqs = 4096;
 // hyq_paged_mma.cu: head sizes 64 and 128 over 16-byte aligned rows.
 bool mma_supported(const AttendArgs& a, bool kv16);
 size_t mma_workspace_bytes(int dim);
-cudaError_t launch_mma(const AttendArgs& a, bool kv16, int64_t max_new, cudaStream_t st);
+cudaError_t launch_few(const AttendArgs& a, bool kv16, cudaStream_t st);    // sequences of up to kFewRows rows
+cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st); // the others
+// hyq_paged_tc.cu: the others on tcgen05 (f16 caches; the workspace past
+// mma_workspace_bytes).
+bool tc_supported(const AttendArgs& a, bool kv16);
+size_t tc_workspace_bytes(int dim);
+cudaError_t launch_chunks_tc(const AttendArgs& a, int64_t max_len, cudaStream_t st);
+
+// The non-finite values of V at positions first + 1 .. last of a sequence in
+// one column: their sum (0 when there are none).  The kernels that multiply V
+// by weights of zero take such values out first and add them back, with this,
+// for the rows that see them.
+template <bool KV16>
+__device__ __noinline__ float non_finite(const Cache& c, const Seq& s, int kvh, int first, int last, int d) {
+  float x = 0.f;
+  for (int p = first + 1; p <= last; ++p) {
+    const int page = s.pages[p / c.page_size];
+    if (page < 0 || page >= c.pages) continue;
+    const int64_t at = (int64_t)page * c.page_stride + (int64_t)kvh * c.head_stride +
+                       (int64_t)(p % c.page_size) * c.row_stride + d;
+    const float v = KV16 ? __half2float(static_cast<const __half*>(c.v)[at]) : static_cast<const float*>(c.v)[at];
+    if (!isfinite(v)) x += v;
+  }
+  return x;
+}
 
 }  // namespace paged
 }  // namespace hyq

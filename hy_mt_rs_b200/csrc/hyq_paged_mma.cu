@@ -20,7 +20,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kThreads = 32 * kWarps;
-constexpr int kRows = 16;            // query rows of a warp: (token, head) pairs
+constexpr int kRows = kFewRows;      // query rows of a warp: (token, head) pairs
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxCtas = 148 * kCtasPerSm;
 // Weights are kept 2^10 times their size, so that their lo halves stay normal
@@ -355,7 +355,7 @@ struct Feed {
   // Non-finite values of V at positions past `first` (the first new token's
   // own) become zero in shared memory: a row that does not see them would
   // multiply them by a weight of zero.  The rows that see them add them back
-  // at the end (unseen()).  Returns whether this lane found any.
+  // at the end (non_finite()).  Returns whether this lane found any.
   __device__ __forceinline__ bool clean(uint32_t dst, int p0, int first) const {
     if (p0 + G::pos - 1 <= first) return false;
     const int lane = threadIdx.x & 31;
@@ -385,22 +385,6 @@ struct Feed {
     return found;
   }
 };
-
-// The non-finite values that clean() took out past token `first`'s position,
-// for a row at token `tok` of the sequence: their sum (0 when there are none).
-template <bool KV16>
-__device__ __noinline__ float unseen(const AttendArgs& a, const Seq& s, int kvh, int first, int tok, int d) {
-  float x = 0.f;
-  for (int p = s.pos + first + 1; p <= s.pos + tok; ++p) {
-    const int page = s.pages[p / a.c.page_size];
-    if (page < 0 || page >= a.c.pages) continue;
-    const int64_t at = (int64_t)page * a.c.page_stride + (int64_t)kvh * a.c.head_stride +
-                       (int64_t)(p % a.c.page_size) * a.c.row_stride + d;
-    const float v = KV16 ? __half2float(static_cast<const __half*>(a.c.v)[at]) : static_cast<const float*>(a.c.v)[at];
-    if (!isfinite(v)) x += v;
-  }
-  return x;
-}
 
 // ---------------------------------------------------------------------------
 // Few new tokens: at most 16 (token, head) rows per kv head
@@ -565,7 +549,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
       if (whole) {
         const int tok = r / group;
         float y = sum / l;
-        if (s.n > 1) y += unseen<KV16>(a, s, kvh, 0, tok, d);
+        if (s.n > 1) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
         a.out[(int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + d] = y;
       } else {
         part[x] = sum;
@@ -628,7 +612,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
           const float inv = ml_s[0][r][1];
           const float y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
 #pragma unroll
-          for (int k = 0; k < 4; ++k) to[k] = s.n > 1 ? y[k] + unseen<KV16>(a, s, kvh, 0, tok, d + k) : y[k];
+          for (int k = 0; k < 4; ++k) to[k] = s.n > 1 ? y[k] + non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d + k) : y[k];
         }
         if (threadIdx.x == 0) counters[cf] = 0;
       }
@@ -662,26 +646,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
   }
   __syncthreads();
   if (warp == 0) {
-    int carry = 0;
-    const int want = gridDim.x - 1 - blockIdx.x;  // the last (longest) tiles first
-    for (int s0 = 0; s0 < a.c.seqs && carry <= want; s0 += 32) {
-      int tiles = 0;
-      if (s0 + lane < a.c.seqs) {
-        const Seq s = load_seq(a.c, s0 + lane);
-        if (s.n * group > kRows) tiles = (s.n * group + kChunkRows - 1) / kChunkRows;
-      }
-      int x = tiles;
-#pragma unroll
-      for (int o = 1; o < 32; o <<= 1) {
-        const int y = __shfl_up_sync(0xffffffffu, x, o);
-        if (lane >= o) x += y;
-      }
-      const int before = carry + x - tiles;
-      if (before <= want && want < before + tiles) {
-        found_s[0] = s0 + lane;
-        found_s[1] = want - before;
-      }
-      carry += __shfl_sync(0xffffffffu, x, 31);
+    int seq, tile;  // the last (longest) tiles first
+    if (find_tile(a.c, group, kChunkRows, gridDim.x - 1 - blockIdx.x, seq, tile) && lane == 0) {
+      found_s[0] = seq;
+      found_s[1] = tile;
     }
   }
   __syncthreads();
@@ -747,34 +715,36 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
         float y = rows.o[d][2 * i + j] / l;
-        if (dirty_s) y += unseen<KV16>(a, s, kvh, first_tok, tok, 8 * d + 2 * (lane & 3) + j);
+        if (dirty_s) y += non_finite<KV16>(a.c, s, kvh, s.pos + first_tok, s.pos + tok, 8 * d + 2 * (lane & 3) + j);
         to[8 * d + j] = y;
       }
     }
   }
 }
 
+int page_shift(const AttendArgs& a) {
+  return (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.c.page_size) : -1;
+}
+
 template <int DIM, bool KV16>
-cudaError_t launch(const AttendArgs& a, int64_t max_new, cudaStream_t st) {
+cudaError_t chunks(const AttendArgs& a, cudaStream_t st) {
   using G = Geo<DIM, KV16>;
-  int shift = -1;
-  if ((a.c.page_size & (a.c.page_size - 1)) == 0) shift = __builtin_ctz((unsigned)a.c.page_size);
-  const int group = a.heads / a.c.kv_heads;
-  cudaError_t e;
-  if (max_new * group > kRows) {
-    const int64_t tiles = ((int64_t)a.c.tokens * group + kChunkRows - 1) / kChunkRows + a.c.seqs;
-    auto k = chunk_kernel<DIM, KV16>;
-    static std::atomic<uint64_t> done{0};
-    if ((e = allow_smem(k, G::smem, done)) != cudaSuccess) return e;
-    if ((e = launch_ex(k, dim3((unsigned)tiles, (unsigned)a.c.kv_heads), dim3(kThreads), G::smem, st, a, shift)) != cudaSuccess)
-      return e;
-  }
-  // (one token per sequence is the fewest there can be: the rows of a
-  // sequence fit one tile of 16 unless every sequence has a chunk)
+  const int64_t tiles = ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + kChunkRows - 1) / kChunkRows + a.c.seqs;
+  auto k = chunk_kernel<DIM, KV16>;
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(k, G::smem, done);
+  if (e != cudaSuccess) return e;
+  return launch_ex(k, dim3((unsigned)tiles, (unsigned)a.c.kv_heads), dim3(kThreads), G::smem, st, a, page_shift(a));
+}
+
+template <int DIM, bool KV16>
+cudaError_t few(const AttendArgs& a, cudaStream_t st) {
+  using G = Geo<DIM, KV16>;
   auto k = few_kernel<DIM, KV16>;
   static std::atomic<uint64_t> done{0};
-  if ((e = allow_smem(k, G::smem + (kMaxSeqs + 1) * 4, done)) != cudaSuccess) return e;
-  return launch_ex(k, dim3(kMaxCtas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4, st, a, shift);
+  const cudaError_t e = allow_smem(k, G::smem + (kMaxSeqs + 1) * 4, done);
+  if (e != cudaSuccess) return e;
+  return launch_ex(k, dim3(kMaxCtas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4, st, a, page_shift(a));
 }
 
 }  // namespace
@@ -787,9 +757,14 @@ bool mma_supported(const AttendArgs& a, bool kv16) {
 
 size_t mma_workspace_bytes(int dim) { return kCounterBytes + 2 * (size_t)kMaxCtas * partial_floats(dim) * sizeof(float); }
 
-cudaError_t launch_mma(const AttendArgs& a, bool kv16, int64_t max_new, cudaStream_t st) {
-  if (a.c.dim == 128) return kv16 ? launch<128, true>(a, max_new, st) : launch<128, false>(a, max_new, st);
-  return kv16 ? launch<64, true>(a, max_new, st) : launch<64, false>(a, max_new, st);
+cudaError_t launch_few(const AttendArgs& a, bool kv16, cudaStream_t st) {
+  if (a.c.dim == 128) return kv16 ? few<128, true>(a, st) : few<128, false>(a, st);
+  return kv16 ? few<64, true>(a, st) : few<64, false>(a, st);
+}
+
+cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st) {
+  if (a.c.dim == 128) return kv16 ? chunks<128, true>(a, st) : chunks<128, false>(a, st);
+  return kv16 ? chunks<64, true>(a, st) : chunks<64, false>(a, st);
 }
 
 }  // namespace paged
