@@ -313,28 +313,28 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort_flag = 1;
         return false;
       };
+      // lo first: the large sums then take half the (cut) additions
       auto scores = [&](int w, int slot) {
         const uint32_t q = base + L::q + w * 2 * L::tile, k = base + L::ring + slot * L::tile;
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
           const uint32_t off = (t >> 2) * L::half + (t & 3) * 32;
-          mma_ss(tmem + 256 * w, desc_k_major(q + off), desc_k_major(k + off), idesc_s, t > 0);
+          mma_ss(tmem + 256 * w, desc_k_major(q + L::tile + off), desc_k_major(k + off), idesc_s, t > 0);
         }
 #pragma unroll
         for (int t = 0; t < KS; ++t) {
           const uint32_t off = (t >> 2) * L::half + (t & 3) * 32;
-          mma_ss(tmem + 256 * w, desc_k_major(q + L::tile + off), desc_k_major(k + off), idesc_s, 1);
+          mma_ss(tmem + 256 * w, desc_k_major(q + off), desc_k_major(k + off), idesc_s, 1);
         }
       };
       auto outputs = [&](int w, int slot) {
         const uint32_t v = base + L::ring + slot * L::tile, pw = tmem + 256 * w;
 #pragma unroll
-        for (int t = 0; t < kTile / 16; ++t) {  // 16 positions: hi at 32 (t / 2) + 8 (t % 2), lo 16 columns on
-          const uint64_t b = desc_mn_major(v + t * 16 * 128, L::half);
-          const uint32_t at = pw + 32 * (t >> 1) + 8 * (t & 1);
-          mma_ts(pw + 128, at, b, idesc_o, t > 0);
-          mma_ts(pw + 128, at + 16, b, idesc_o, 1);
-        }
+        for (int h = 1; h >= 0; --h)
+#pragma unroll
+          for (int t = 0; t < kTile / 16; ++t)  // 16 positions: hi at 32 (t / 2) + 8 (t % 2), lo 16 columns on
+            mma_ts(pw + 128, pw + 32 * (t >> 1) + 8 * (t & 1) + 16 * h, desc_mn_major(v + t * 16 * 128, L::half), idesc_o,
+                   h == 0 || t > 0);
       };
       bool ok = nt > 0 && wait(full(0), 0);
       if (ok) {
