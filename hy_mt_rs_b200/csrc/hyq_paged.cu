@@ -453,7 +453,7 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
   if (hyq::paged::mma_supported(a, kv16)) {
     cudaError_t e = cudaSuccess;
     if (batch->max_new * (heads / kv->kv_heads) > hyq::paged::kFewRows)
-      e = hyq::paged::tc_supported(a, kv16) ? hyq::paged::launch_chunks_tc(a, batch->max_len, st)
+      e = hyq::paged::tc_supported(a, kv16) ? hyq::paged::launch_chunks_tc(a, st)
                                             : hyq::paged::launch_chunks(a, kv16, st);
     if (e == cudaSuccess) e = hyq::paged::launch_few(a, kv16, st);
     return done(e, name);

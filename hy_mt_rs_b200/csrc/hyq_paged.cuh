@@ -141,7 +141,7 @@ cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st); // t
 // mma_workspace_bytes).
 bool tc_supported(const AttendArgs& a, bool kv16);
 size_t tc_workspace_bytes(int dim);
-cudaError_t launch_chunks_tc(const AttendArgs& a, int64_t max_len, cudaStream_t st);
+cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st);
 
 // The non-finite values of V at positions first + 1 .. last of a sequence in
 // one column: their sum (0 when there are none).  The kernels that multiply V

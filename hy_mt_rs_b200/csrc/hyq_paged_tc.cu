@@ -1,8 +1,11 @@
 // Attention of chunks of new tokens over an f16 paged cache on tcgen05, head
 // sizes 64 and 128, at f32 accuracy.
 //
-// A CTA takes two tiles of 128 (token, query head) rows of one sequence and kv
-// head, and walks the positions they see in tiles of 128.  Queries and weights
+// Work is cut into segments: two tiles of 128 (token, query head) rows of one
+// sequence and kv head, over the positions they see in tiles of 128.  All
+// segments' position tiles form one line, cut into equal ranges, one per SM
+// (plan_kernel lists the segments); a segment that spans CTAs leaves partial
+// results, which join_kernel adds up.  Queries and weights
 // are hi + lo, both f16 (22 bits), K and V exact, so a tile pair costs
 //   S = Qh K' + Ql K'   and   X = Ph V + Pl V,
 // four 128 x 128 x 128 products: twice those of plain f16 attention, which is
@@ -38,7 +41,10 @@ constexpr int kTile = 128;               // rows of a row tile, positions of a p
 constexpr int kCtaRows = 2 * kTile;
 constexpr int kThreads = 384;
 constexpr int kSlots = 3;                // tiles of K or V in shared memory
-constexpr int kMaxParts = 296;           // partial results of 256 rows in the workspace
+constexpr int kMaxCtas = 148;
+constexpr int kMaxParts = 2 * kMaxCtas;  // partial results in the workspace: a CTA's first and last piece
+constexpr int kMaxSegs = 65536;          // row tile pairs of a call
+constexpr int kMinTiles = 2;             // position tiles of a CTA, at least
 // Floats of one: outputs, then (maximum, sum) of each row, then whether a value
 // was taken out.
 __host__ __device__ constexpr size_t part_floats(int dim) { return (size_t)kCtaRows * (dim + 2) + 4; }
@@ -52,18 +58,167 @@ struct Smem {
   static constexpr int q = 0;                            // [row tile][hi, lo]
   static constexpr int ring = 4 * tile;
   static constexpr int bars = ring + kSlots * tile;
-  // full[3], empty[3], s_full[2], p_full[2], o_full[2], clean[2]
-  static constexpr int n_bars = 2 * kSlots + 8;
-  static constexpr int misc = bars + 8 * n_bars;         // tensor memory address, abort, dirty, sequence, tile
+  // full[3], empty[3], s_full[2], p_full[2], o_full[2], q_full[2], clean[2]
+  static constexpr int n_bars = 2 * kSlots + 10;
+  static constexpr int misc = bars + 8 * n_bars;         // tensor memory address, abort, first segment, dirty[2]
   static constexpr int total = misc + 32 + 1024;         // the base is moved to 1024 bytes
 };
 
+// The segments of one kv head, in global memory: segment t is row tile pair
+// tile[t] of sequence seq[t]; first[t] position tiles come before it.
+struct Plan {
+  int* count;   // segments, then the total of their tiles
+  int* seq;     // [kMaxSegs]
+  int* tile;    // [kMaxSegs]
+  int* first;   // [kMaxSegs + 1]
+};
+constexpr size_t kPlanBytes = (4 + 3 * (size_t)kMaxSegs + 4) * sizeof(int);
+inline Plan plan_of(void* ws) {
+  int* p = static_cast<int*>(ws);
+  return {p, p + 4, p + 4 + kMaxSegs, p + 4 + 2 * kMaxSegs};
+}
+
 struct Params {
   AttendArgs a;
+  Plan plan;
   int box;        // rows of a TMA box: min(page_size, 128)
-  int splits;     // parts of the positions; > 1: partial results
-  float* parts;   // [row tile pair][kv head][split] (part_floats)
+  float* parts;   // [CTA][first piece, last piece] (part_floats)
 };
+
+// Position tiles that the rows of a pair see.
+__device__ __forceinline__ int seen_tiles(const Seq& s, int group, int tile) {
+  const int last = min((tile + 1) * kCtaRows, s.n * group) - 1;
+  return (s.pos + last / group + kTile) / kTile;
+}
+
+// One CTA: the sequences' row tile pairs, then each pair's place in line.
+__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan) {
+  grid_dependency_wait();
+  allow_dependents_launch();
+  __shared__ int off_s[kMaxSeqs + 1];
+  __shared__ int warp_s[32];
+  const int group = a.heads / a.c.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  auto scan = [&](int v, int& total) {
+    int x = v;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    __syncthreads();
+    if (lane == 31) warp_s[warp] = x;
+    __syncthreads();
+    int w = warp_s[lane];
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, w, o);
+      if (lane >= o) w += y;
+    }
+    total = __shfl_sync(0xffffffffu, w, 31);
+    const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
+    return (warp ? before : 0) + x - v;
+  };
+  int segs = 0, total;
+  for (int s0 = 0; s0 < a.c.seqs; s0 += 1024) {
+    const int i = s0 + (int)threadIdx.x;
+    int n = 0;
+    if (i < a.c.seqs) {
+      const Seq s = load_seq(a.c, i);
+      if (s.n * group > kFewRows) n = (s.n * group + kCtaRows - 1) / kCtaRows;
+    }
+    const int at = segs + scan(n, total);
+    if (i < a.c.seqs) off_s[i] = at;
+    segs += total;
+  }
+  __syncthreads();
+  segs = min(segs, kMaxSegs);
+  int tiles = 0;
+  for (int t0 = 0; t0 < segs; t0 += 1024) {
+    const int t = t0 + (int)threadIdx.x;
+    int cost = 0, seq = 0, tile = 0;
+    if (t < segs) {
+      int lo = 0, hi = a.c.seqs - 1;  // the last sequence with off <= t
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (off_s[mid] <= t) lo = mid;
+        else hi = mid - 1;
+      }
+      seq = lo;
+      tile = t - off_s[lo];
+      cost = seen_tiles(load_seq(a.c, seq), group, tile);
+    }
+    const int at = tiles + scan(cost, total);
+    if (t < segs) {
+      plan.seq[t] = seq;
+      plan.tile[t] = tile;
+      plan.first[t] = at;
+    }
+    tiles += total;
+  }
+  if (threadIdx.x == 0) {
+    plan.first[segs] = tiles;
+    plan.count[0] = segs;
+    plan.count[1] = tiles;
+  }
+}
+
+// The ranges of the line: CTA c of `ctas` takes units work c / ctas ..
+struct Line {
+  int64_t work;
+  int ctas;
+  __device__ __forceinline__ int64_t begin(int c) const { return work * c / ctas; }
+  // the CTA that takes unit u
+  __device__ __forceinline__ int cta_of(int64_t u) const {
+    int c = (int)(u * ctas / work);
+    while (begin(c + 1) <= u) ++c;
+    while (c > 0 && begin(c) > u) --c;
+    return c;
+  }
+};
+__device__ __forceinline__ Line line_of(const Params& p, int grid) {
+  const int64_t work = (int64_t)p.plan.count[1] * p.a.c.kv_heads;
+  return {work, (int)min((int64_t)grid, max(work / kMinTiles, (int64_t)1))};
+}
+// The segment that holds tile x of a kv head's line; by a whole warp.
+__device__ __forceinline__ int segment_of(const Plan& plan, int x) {
+  const int lane = threadIdx.x & 31;
+  int lo = 0, n = plan.count[0];
+  for (;;) {
+    const int step = (n + 31) / 32, i = lo + lane * step;
+    const int hits = __popc(__ballot_sync(0xffffffffu, i < lo + n && plan.first[i] <= x));
+    const int next = lo + max(hits - 1, 0) * step;
+    if (step <= 1) return next;
+    n = min(step, lo + n - next);
+    lo = next;
+  }
+}
+
+// What a CTA does of a segment.
+struct Piece {
+  Seq s;
+  int kvh, r0, rows, first_tok, len, j0, nt, jm;
+  int64_t seg0;
+  bool two, whole;
+};
+__device__ __forceinline__ Piece piece_of(const Params& p, int group, int t, int kvh, int64_t at, int64_t end) {
+  Piece x;
+  const Plan& plan = p.plan;
+  const int first = plan.first[t], tiles = plan.first[t + 1] - first, tile = plan.tile[t];
+  x.s = load_seq(p.a.c, plan.seq[t]);
+  x.kvh = kvh;
+  x.seg0 = (int64_t)kvh * plan.count[1] + first;
+  x.r0 = tile * kCtaRows;
+  x.rows = min(kCtaRows, x.s.n * group - x.r0);
+  x.two = x.rows > kTile;          // the second row tile has rows
+  x.first_tok = x.r0 / group;
+  x.len = x.s.pos + (x.r0 + x.rows - 1) / group + 1;  // positions the last row sees
+  x.j0 = (int)(at - x.seg0);
+  x.nt = (int)(min(end, x.seg0 + tiles) - at);
+  x.whole = x.j0 == 0 && x.nt == tiles;
+  // tiles from here on hold positions that some row does not see
+  x.jm = max(0, (x.s.pos + x.first_tok + 1) / kTile - x.j0);
+  return x;
+}
 
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int page, uint32_t bar) {
   asm volatile(
@@ -106,29 +261,39 @@ __device__ __forceinline__ void commit(uint32_t bar) {
 __device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 
-// 32 columns of this thread's tensor memory lane.
-__device__ __forceinline__ void tmem_ld32(float (&v)[32], uint32_t a) {
+// 16 columns of this thread's tensor memory lane.
+__device__ __forceinline__ void tmem_ld(float (&v)[16], uint32_t a) {
   asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
+      "[%16];"
       : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
-        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
       : "r"(a));
 }
-__device__ __forceinline__ void tmem_st32(uint32_t a, const uint32_t (&v)[32]) {
+__device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t (&v)[16]) {
   asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16};" ::"r"(a),
       "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
       : "memory");
 }
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
+
+// f(columns, index of the first) over N columns from `a`, 16 at a time, the next
+// load in flight while one is worked on.
+template <int N, typename F>
+__device__ __forceinline__ void tmem_each(uint32_t a, F f) {
+  float v[2][16];
+  tmem_ld(v[0], a);
+#pragma unroll
+  for (int c = 0; c < N / 16; ++c) {
+    tmem_wait_ld();
+    if (c + 1 < N / 16) tmem_ld(v[(c + 1) & 1], a + 16 * (c + 1));
+    f(v[c & 1], 16 * c);
+  }
+}
 
 __device__ __forceinline__ float ex2(float x) {
   float y;
@@ -164,21 +329,25 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto s_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + w); };
   auto p_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 2 + w); };
   auto o_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 4 + w); };
-  auto clean = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 6 + (i & 1)); };  // of masked tile i
+  auto q_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 6 + w); };
+  auto clean = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 8 + (i & 1)); };  // of masked tile i
   volatile int* misc = reinterpret_cast<volatile int*>(base_g + L::misc);
   volatile int* abort_flag = misc + 1;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.heads / a.c.kv_heads, kvh = blockIdx.y;
+  const int group = a.heads / a.c.kv_heads;
 
   grid_dependency_wait();
+  allow_dependents_launch();
+  const Line line = line_of(p, gridDim.x);
+  const int cta = blockIdx.x, total = p.plan.count[1];
+  if (line.work == 0 || cta >= line.ctas) return;  // nothing allocated yet
+  const int64_t begin = line.begin(cta), end = line.begin(cta + 1);
   if (warp == 0) {
-    int seq = -1, tile = 0;  // the last (longest) tiles first
-    if (!find_tile(a.c, group, kCtaRows, gridDim.x - 1 - blockIdx.x, seq, tile)) seq = -1;
+    const int t = segment_of(p.plan, (int)(begin % total));
     if (lane == 0) {
       misc[1] = 0;
-      misc[2] = 0;
-      misc[3] = seq;
-      misc[4] = tile;
+      misc[2] = t;
+      misc[3] = misc[4] = 0;
       for (int s = 0; s < kSlots; ++s) {
         mbar_init(full(s), 1);
         mbar_init(empty(s), 3);  // the products that read it, and warps 2 and 3
@@ -187,112 +356,67 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(s_full(w), 1);
         mbar_init(p_full(w), 4);
         mbar_init(o_full(w), 1);
+        mbar_init(q_full(w), 4);
         mbar_init(clean(w), 2);
       }
       mbar_fence_init();
     }
   }
-  __syncthreads();
-  allow_dependents_launch();
-  if (misc[3] < 0) return;  // nothing allocated yet
-  const Seq s = load_seq(a.c, misc[3]);
-  const int r0 = misc[4] * kCtaRows, rows = min(kCtaRows, s.n * group - r0);
-  const bool two = rows > kTile;          // the second row tile has rows
-  const int first_tok = r0 / group, last_tok = (r0 + rows - 1) / group;
-  const int len = s.pos + last_tok + 1;   // positions the last row sees
-  const int all_tiles = (len + kTile - 1) / kTile;
-  const int j0 = (int)((int64_t)all_tiles * blockIdx.z / p.splits);
-  const int nt = (int)((int64_t)all_tiles * (blockIdx.z + 1) / p.splits) - j0;
-  // tiles from here on hold positions that some row does not see
-  const int jm = max(0, (s.pos + first_tok + 1) / kTile - j0);
-  float* part = p.splits > 1 ? p.parts + ((size_t)((gridDim.x - 1 - blockIdx.x) * gridDim.y + kvh) * p.splits + blockIdx.z) *
-                                             part_floats(DIM)
-                             : nullptr;
-
   if (warp == 1) {
     asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::misc), "r"(kTmemCols));
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
-  }
-  // The queries, a row at a time per warp: scaled to [1, 2) by a power of two
-  // that goes back into the scores, hi and lo into shared memory.
-  const int wg = warp >= 8 ? 1 : 0;                          // row tile (softmax warps)
-  const int r = r0 + wg * kTile + 32 * (warp & 3) + lane;    // row of the sequence, of this thread
-  const int tok = min(r / group, s.n - 1);
-  float factor = 1.0f;
-  if (warp >= 4 && (wg == 0 || two)) {
-    constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;  // log2(e) / sqrt(DIM)
-    constexpr int N = DIM / 32;  // values per lane
-    uint8_t* q_s = base_g + L::q + wg * 2 * L::tile;
-#pragma unroll 4
-    for (int i = 0; i < 32; ++i) {
-      const int row = 32 * (warp & 3) + i, rr = r0 + wg * kTile + row, t = rr / group;
-      float x[N], top = 0.f;
-      const float* q = a.q + (int64_t)(s.row0 + min(t, s.n - 1)) * a.q_stride + (int64_t)(kvh * group + rr % group) * DIM + N * lane;
-#pragma unroll
-      for (int k = 0; k < N; ++k) {
-        x[k] = t < s.n ? q[k] * scale : 0.f;
-        top = fmaxf(top, fabsf(x[k]));
-      }
-#pragma unroll
-      for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-      if (lane == i) factor = __uint_as_float((uint32_t)e << 23);
-      const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-      uint32_t hi[N / 2], lo[N / 2];
-#pragma unroll
-      for (int k = 0; k < N / 2; ++k) {
-        hi[k] = pack_f16(x[2 * k] * down, x[2 * k + 1] * down);
-        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-        lo[k] = pack_f16(x[2 * k] * down - f.x, x[2 * k + 1] * down - f.y);
-      }
-      const int d = N * lane, c = d >> 3;  // 16-byte chunk of the row
-      uint8_t* at = q_s + (c >> 3) * L::half + row * 128 + (((c ^ row) & 7) << 4) + (d & 7) * 2;
-#pragma unroll
-      for (int k = 0; k < N / 2; ++k) {
-        *reinterpret_cast<uint32_t*>(at + 4 * k) = hi[k];
-        *reinterpret_cast<uint32_t*>(at + L::tile + 4 * k) = lo[k];
-      }
-    }
-    fence_proxy_async_smem();
   }
   fence_before();
   __syncthreads();
   fence_after();
   const uint32_t tmem = (uint32_t)misc[0];
+  // every warp walks the same pieces: (segment, kv head), at its tile `at`
+  int t = misc[2], kvh = (int)(begin / total);
+  int64_t at = begin;
+  auto next = [&](const Piece& x) {
+    at += x.nt;
+    if (++t == p.plan.count[0]) {
+      t = 0;
+      ++kvh;
+    }
+  };
 
   if (warp < 4) {
-    // launch: 168 registers x 384 threads; 72 x 128 + 216 x 256 is the same
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    // launch: 168 registers x 384 threads; 104 x 128 + 200 x 256 is the same
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 104;");
     if (warp == 0) {
       // ------------------------------ pages in -------------------------------
       const int per = kTile / p.box;  // boxes of a tile: one lane each
       int issued = 0;
       bool ok = true;
-      for (int i = 0; i < 2 * nt && ok; ++i) {  // K and V of each tile
-        const int slot = i % kSlots, j = j0 + (i >> 1);
-        const int pos = j * kTile + lane * p.box;
-        int page = a.c.pages;  // past the pool: zeros
-        if (lane < per && pos < len) {
-          page = s.pages[pos / a.c.page_size];
-          if (page < 0 || page >= a.c.pages) {
-            atomicOr(a.c.status, DEV_BAD_ARGS);
-            page = a.c.pages;
+      while (at < end && ok) {
+        const Piece x = piece_of(p, group, t, kvh, at, end);
+        for (int i = 0; i < 2 * x.nt; ++i) {  // K and V of each tile
+          const int slot = issued % kSlots, pos = (x.j0 + (i >> 1)) * kTile + lane * p.box;
+          int page = a.c.pages;  // past the pool: zeros
+          if (lane < per && pos < x.len) {
+            page = x.s.pages[pos / a.c.page_size];
+            if (page < 0 || page >= a.c.pages) {
+              atomicOr(a.c.status, DEV_BAD_ARGS);
+              page = a.c.pages;
+            }
           }
-        }
-        if (i >= kSlots && !warp_wait(empty(slot), ((i / kSlots) - 1) & 1, abort_flag)) {
-          ok = false;
-          break;
-        }
-        if (lane == 0) mbar_arrive_expect_tx(full(slot), L::tile);
-        __syncwarp();
-        if (lane < per) {
-          const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
-          const uint32_t dst = base + L::ring + slot * L::tile + lane * p.box * 128;
+          if (issued >= kSlots && !warp_wait(empty(slot), ((issued / kSlots) - 1) & 1, abort_flag)) {
+            ok = false;
+            break;
+          }
+          if (lane == 0) mbar_arrive_expect_tx(full(slot), L::tile);
+          __syncwarp();
+          if (lane < per) {
+            const CUtensorMap* map = (i & 1) ? &map_v : &map_k;
+            const uint32_t dst = base + L::ring + slot * L::tile + lane * p.box * 128;
 #pragma unroll
-          for (int h = 0; h < HALVES; ++h)
-            tma_load_4d(dst + h * L::half, map, 64 * h, pos % a.c.page_size, kvh, page, full(slot));
+            for (int h = 0; h < HALVES; ++h)
+              tma_load_4d(dst + h * L::half, map, 64 * h, pos % a.c.page_size, x.kvh, page, full(slot));
+          }
+          ++issued;
         }
-        ++issued;
+        next(x);
       }
       if (!ok) {
         if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_EMPTY);
@@ -313,219 +437,277 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort_flag = 1;
         return false;
       };
+      // (addresses are in the low bits of a descriptor, 16 bytes a unit)
+      const uint64_t q_desc = desc_k_major(base + L::q), k_desc = desc_k_major(base + L::ring);
+      const uint64_t v_desc = desc_mn_major(base + L::ring, L::half);
       // lo first: the large sums then take half the (cut) additions
       auto scores = [&](int w, int slot) {
-        const uint32_t q = base + L::q + w * 2 * L::tile, k = base + L::ring + slot * L::tile;
-#pragma unroll
-        for (int t = 0; t < KS; ++t) {
-          const uint32_t off = (t >> 2) * L::half + (t & 3) * 32;
-          mma_ss(tmem + 256 * w, desc_k_major(q + L::tile + off), desc_k_major(k + off), idesc_s, t > 0);
-        }
-#pragma unroll
-        for (int t = 0; t < KS; ++t) {
-          const uint32_t off = (t >> 2) * L::half + (t & 3) * 32;
-          mma_ss(tmem + 256 * w, desc_k_major(q + off), desc_k_major(k + off), idesc_s, 1);
-        }
-      };
-      auto outputs = [&](int w, int slot) {
-        const uint32_t v = base + L::ring + slot * L::tile, pw = tmem + 256 * w;
+        const uint64_t q = q_desc + w * (2 * L::tile >> 4), k = k_desc + slot * (L::tile >> 4);
 #pragma unroll
         for (int h = 1; h >= 0; --h)
 #pragma unroll
-          for (int t = 0; t < kTile / 16; ++t)  // 16 positions: hi at 32 (t / 2) + 8 (t % 2), lo 16 columns on
-            mma_ts(pw + 128, pw + 32 * (t >> 1) + 8 * (t & 1) + 16 * h, desc_mn_major(v + t * 16 * 128, L::half), idesc_o,
-                   h == 0 || t > 0);
-      };
-      bool ok = nt > 0 && wait(full(0), 0);
-      if (ok) {
-        fence_after();
-        if (lane == 0) {
-          scores(0, 0);
-          commit(s_full(0));
-          if (two) {
-            scores(1, 0);
-            commit(s_full(1));
+          for (int t = 0; t < KS; ++t) {
+            const int off = ((t >> 2) * L::half + (t & 3) * 32) >> 4;
+            mma_ss(tmem + 256 * w, q + h * (L::tile >> 4) + off, k + off, idesc_s, h == 0 || t > 0);
           }
-          commit(empty(0));
-        }
-        __syncwarp();
-      }
-      for (int j = 0; j < nt && ok; ++j) {
-        const int iv = 2 * j + 1, ik = 2 * j + 2;
-        ok = wait(full(iv % kSlots), (iv / kSlots) & 1) && (j < jm || wait(clean(j - jm), ((j - jm) >> 1) & 1)) &&
-             (j + 1 >= nt || wait(full(ik % kSlots), (ik / kSlots) & 1));
-        for (int w = 0; w < (two ? 2 : 1) && ok; ++w) {
-          ok = wait(p_full(w), j & 1);
+      };
+      auto outputs = [&](int w, int slot) {
+        const uint64_t v = v_desc + slot * (L::tile >> 4);
+        const uint32_t pw = tmem + 256 * w;
+#pragma unroll
+        for (int h = 1; h >= 0; --h)
+#pragma unroll
+          for (int t = 0; t < kTile / 16; ++t)  // 16 positions: hi in 8 columns from 16 t, lo in the next 8
+            mma_ts(pw + 128, pw + 16 * t + 8 * h, v + t * (16 * 128 >> 4), idesc_o, h == 0 || t > 0);
+      };
+      int i0 = 0, masked = 0;            // ring tiles and masked tiles before this piece
+      int steps[2] = {0, 0}, pieces[2] = {0, 0};
+      bool ok = true;
+      while (at < end && ok) {
+        const Piece x = piece_of(p, group, t, kvh, at, end);
+        const int active = x.two ? 2 : 1;
+        ok = wait(full(i0 % kSlots), (i0 / kSlots) & 1);
+        for (int w = 0; w < active && ok; ++w) {
+          ok = wait(q_full(w), pieces[w] & 1);
           if (!ok) break;
           fence_after();
           if (lane == 0) {
-            outputs(w, iv % kSlots);
-            const bool last = w == (two ? 1 : 0);
-            if (last) commit(empty(iv % kSlots));
-            if (j + 1 < nt) {
-              scores(w, ik % kSlots);
-              commit(s_full(w));
-              if (last) commit(empty(ik % kSlots));
-            } else {
-              commit(o_full(w));
-            }
+            scores(w, i0 % kSlots);
+            commit(s_full(w));
+            if (w == active - 1) commit(empty(i0 % kSlots));
           }
           __syncwarp();
         }
+        for (int j = 0; j < x.nt && ok; ++j) {
+          const int iv = i0 + 2 * j + 1, ik = iv + 1;
+          ok = wait(full(iv % kSlots), (iv / kSlots) & 1);
+          if (ok && j >= x.jm) {
+            ok = wait(clean(masked), (masked >> 1) & 1);
+            ++masked;
+          }
+          ok = ok && (j + 1 >= x.nt || wait(full(ik % kSlots), (ik / kSlots) & 1));
+          for (int w = 0; w < active && ok; ++w) {
+            ok = wait(p_full(w), steps[w] & 1);
+            if (!ok) break;
+            ++steps[w];
+            fence_after();
+            if (lane == 0) {
+              outputs(w, iv % kSlots);
+              const bool last = w == active - 1;
+              if (last) commit(empty(iv % kSlots));
+              if (j + 1 < x.nt) {
+                scores(w, ik % kSlots);
+                commit(s_full(w));
+                if (last) commit(empty(ik % kSlots));
+              } else {
+                commit(o_full(w));
+              }
+            }
+            __syncwarp();
+          }
+        }
+        for (int w = 0; w < active; ++w) ++pieces[w];
+        i0 += 2 * x.nt;
+        next(x);
       }
     } else {
       // --------------------------- what rows do not see -----------------------
       // (these warps follow every tile, and hold its slot: a wait that skipped
       // phases would take an earlier one for its own)
       bool ok = true;
-      for (int i = 0; i < 2 * nt; ++i) {
-        const int slot = i % kSlots, j = i >> 1;
-        ok = warp_wait(full(slot), (i / kSlots) & 1, abort_flag);
-        if (!ok) break;
-        if (!(i & 1) || j < jm) {
-          if (lane == 0) mbar_arrive(empty(slot));
-          continue;
-        }
-        bool found = false;
-        for (int x = threadIdx.x - 64; x < kTile * 8 * HALVES; x += 64) {  // 16-byte chunks
-          const int row = (x >> 3) & (kTile - 1), pos = (j0 + j) * kTile + row;
-          if (pos <= s.pos + first_tok) continue;
-          uint4* at = reinterpret_cast<uint4*>(base_g + L::ring + slot * L::tile + x * 16);
-          uint4 v = *at;
-          uint32_t w[4] = {v.x, v.y, v.z, v.w};
-          bool bad = false;
+      int i0 = 0, masked = 0, seg = 0;
+      while (at < end && ok) {
+        const Piece x = piece_of(p, group, t, kvh, at, end);
+        ++seg;
+        for (int i = 0; i < 2 * x.nt; ++i, ++i0) {
+          const int slot = i0 % kSlots, j = i >> 1;
+          ok = warp_wait(full(slot), (i0 / kSlots) & 1, abort_flag);
+          if (!ok) break;
+          if (!(i & 1) || j < x.jm) {
+            if (lane == 0) mbar_arrive(empty(slot));
+            continue;
+          }
+          bool found = false;
+          for (int c = threadIdx.x - 64; c < kTile * 8 * HALVES; c += 64) {  // 16-byte chunks
+            const int pos = (x.j0 + j) * kTile + ((c >> 3) & (kTile - 1));
+            if (pos <= x.s.pos + x.first_tok) continue;
+            uint4* ptr = reinterpret_cast<uint4*>(base_g + L::ring + slot * L::tile + c * 16);
+            const uint4 v = *ptr;
+            uint32_t w[4] = {v.x, v.y, v.z, v.w};
+            bool bad = false;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) {
-            if ((w[k] & 0x7c00u) == 0x7c00u) w[k] &= 0xffff0000u, bad = true;
-            if ((w[k] & 0x7c000000u) == 0x7c000000u) w[k] &= 0xffffu, bad = true;
+            for (int k = 0; k < 4; ++k) {
+              if ((w[k] & 0x7c00u) == 0x7c00u) w[k] &= 0xffff0000u, bad = true;
+              if ((w[k] & 0x7c000000u) == 0x7c000000u) w[k] &= 0xffffu, bad = true;
+            }
+            if (bad) {
+              *ptr = make_uint4(w[0], w[1], w[2], w[3]);
+              found = found || pos < x.len;
+            }
           }
-          if (bad) {
-            *at = make_uint4(w[0], w[1], w[2], w[3]);
-            found = found || pos < len;
+          if (found) misc[3 + (seg & 1)] = seg;  // (at most one piece ahead of the rows that ask)
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0) {
+            mbar_arrive(clean(masked));
+            mbar_arrive(empty(slot));
           }
+          ++masked;
         }
-        if (found) misc[2] = 1;
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) {
-          mbar_arrive(clean(j - jm));
-          mbar_arrive(empty(slot));
-        }
+        next(x);
       }
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 216;");
-    if (wg == 0 || two) {
-      // -------------------------------- softmax -------------------------------
-      const uint32_t lanes = tmem + ((uint32_t)(32 * (warp & 3)) << 16), st = lanes + 256 * wg;
-      const int sees = s.pos + tok;
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // -------------------------------- softmax -------------------------------
+    const int wg = warp >= 8 ? 1 : 0;  // row tile
+    const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 * wg;
+    int steps = 0, pieces = 0, seg = 0;
+    bool ok = true;
+    while (at < end && ok) {
+      const Piece x = piece_of(p, group, t, kvh, at, end);
+      const int r = x.r0 + wg * kTile + 32 * (warp & 3) + lane;  // row of the sequence
+      const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + tok;
+      const int64_t piece_at = at;
+      const int piece_t = t, piece_kvh = kvh;
+      ++seg;
+      next(x);
+      if (wg == 1 && !x.two) continue;
+      // The queries, a row at a time per warp: scaled to [1, 2) by a power of
+      // two that goes back into the scores, hi and lo into shared memory.
+      float factor = 1.0f;
+      {
+        constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;  // log2(e) / sqrt(DIM)
+        constexpr int N = DIM / 32;  // values per lane
+        uint8_t* q_s = base_g + L::q + wg * 2 * L::tile;
+#pragma unroll 4
+        for (int i = 0; i < 32; ++i) {
+          const int row = 32 * (warp & 3) + i, rr = x.r0 + wg * kTile + row, tk = rr / group;
+          float v[N], top = 0.f;
+          const float* q = a.q + (int64_t)(x.s.row0 + min(tk, x.s.n - 1)) * a.q_stride +
+                           (int64_t)(x.kvh * group + rr % group) * DIM + N * lane;
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            v[k] = tk < x.s.n ? q[k] * scale : 0.f;
+            top = fmaxf(top, fabsf(v[k]));
+          }
+#pragma unroll
+          for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
+          const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+          if (lane == i) factor = __uint_as_float((uint32_t)e << 23);
+          const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+          uint32_t hi[N / 2], lo[N / 2];
+#pragma unroll
+          for (int k = 0; k < N / 2; ++k) {
+            hi[k] = pack_f16(v[2 * k] * down, v[2 * k + 1] * down);
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+            lo[k] = pack_f16(v[2 * k] * down - f.x, v[2 * k + 1] * down - f.y);
+          }
+          const int d = N * lane, c = d >> 3;  // 16-byte chunk of the row
+          uint8_t* to = q_s + (c >> 3) * L::half + row * 128 + (((c ^ row) & 7) << 4) + (d & 7) * 2;
+#pragma unroll
+          for (int k = 0; k < N / 2; ++k) {
+            *reinterpret_cast<uint32_t*>(to + 4 * k) = hi[k];
+            *reinterpret_cast<uint32_t*>(to + L::tile + 4 * k) = lo[k];
+          }
+        }
+        fence_proxy_async_smem();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full(wg));
+      }
       float o[DIM];
 #pragma unroll
       for (int d = 0; d < DIM; ++d) o[d] = 0.f;
       float m = -INFINITY, l = 0.f, down = 1.f;
-      bool ok = true;
-      for (int j = 0; j < nt; ++j) {
-        ok = warp_wait(s_full(wg), j & 1, abort_flag);
+      for (int j = 0; j < x.nt; ++j, ++steps) {
+        ok = warp_wait(s_full(wg), steps & 1, abort_flag);
         if (!ok) break;
         fence_after();
-        const int p0 = (j0 + j) * kTile;
-        const bool masked = j >= jm;
+        const int p0 = (x.j0 + j) * kTile;
+        const bool masked = j >= x.jm;
         float top = -INFINITY;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          tmem_ld32(v, st + 32 * c);
-          tmem_wait_ld();
+        tmem_each<kTile>(st, [&](float (&v)[16], int c) {
           if (masked) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (p0 + 32 * c + i > sees) v[i] = -INFINITY;
+            for (int i = 0; i < 16; ++i)
+              if (p0 + c + i > sees) v[i] = -INFINITY;
           }
 #pragma unroll
-          for (int i = 0; i < 32; ++i) top = fmaxf(top, v[i]);
-        }
+          for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, v[i]), v[i + 1]);
+        });
         const float now = fmaxf(m, top * factor);
         const float next_down = now == -INFINITY ? 1.f : ex2(m - now);
         const float back = kBias - (now == -INFINITY ? 0.f : now);
-        float sum = 0.f;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          float v[32];
-          uint32_t w[32];
-          tmem_ld32(v, st + 32 * c);
-          tmem_wait_ld();
+        float sum = 0.f, sum2 = 0.f;
+        tmem_each<kTile>(st, [&](float (&v)[16], int c) {
           if (masked) {
 #pragma unroll
-            for (int i = 0; i < 32; ++i)
-              if (p0 + 32 * c + i > sees) v[i] = -INFINITY;
+            for (int i = 0; i < 16; ++i)
+              if (p0 + c + i > sees) v[i] = -INFINITY;
           }
+          uint32_t w[16];
 #pragma unroll
-          for (int i = 0; i < 32; i += 2) {
+          for (int i = 0; i < 16; i += 2) {
             const float x = ex2(fmaf(v[i], factor, back)), y = ex2(fmaf(v[i + 1], factor, back));
-            sum += x + y;
+            sum += x;
+            sum2 += y;
             const float xh = high_part(x), yh = high_part(y);
             w[i >> 1] = pack_f16(xh, yh);
-            w[16 + (i >> 1)] = pack_f16(x - xh, y - yh);
+            w[8 + (i >> 1)] = pack_f16(x - xh, y - yh);
           }
-          tmem_st32(st + 32 * c, w);
-        }
-        l = fmaf(l, next_down, sum);
+          tmem_st(st + c, w);
+        });
+        l = fmaf(l, next_down, sum + sum2);
         m = now;
-        if (j > 0) {  // the tile before: its product is done (the scores came after it)
+        if (j > 0)  // the tile before: its product is done (the scores came after it)
+          tmem_each<DIM>(st + 128, [&](float (&v)[16], int c) {
 #pragma unroll
-          for (int c = 0; c < DIM / 32; ++c) {
-            float v[32];
-            tmem_ld32(v, st + 128 + 32 * c);
-            tmem_wait_ld();
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[32 * c + i] = fmaf(o[32 * c + i], down, v[i]);
-          }
-        }
+            for (int i = 0; i < 16; ++i) o[c + i] = fmaf(o[c + i], down, v[i]);
+          });
         down = next_down;
         tmem_wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(wg));
       }
-      ok = ok && nt > 0 && warp_wait(o_full(wg), 0, abort_flag);
-      if (ok) {
-        fence_after();
-#pragma unroll
-        for (int c = 0; c < DIM / 32; ++c) {
-          float v[32];
-          tmem_ld32(v, st + 128 + 32 * c);
-          tmem_wait_ld();
-#pragma unroll
-          for (int i = 0; i < 32; ++i) o[32 * c + i] = fmaf(o[32 * c + i], down, v[i]);
-        }
-      } else if (nt > 0) {
+      ok = ok && warp_wait(o_full(wg), pieces & 1, abort_flag);
+      ++pieces;
+      if (!ok) {
         if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_FULL);
         *abort_flag = 1;
+        break;
       }
-      if (r < s.n * group && (ok || nt == 0)) {
-        if (part) {
-          float* to = part + (size_t)(r - r0) * DIM;
+      fence_after();
+      tmem_each<DIM>(st + 128, [&](float (&v)[16], int c) {
 #pragma unroll
-          for (int d = 0; d < DIM; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-          float* ml = part + (size_t)kCtaRows * DIM + 2 * (r - r0);
-          ml[0] = m;
-          ml[1] = l;
-          if (r == r0) part[(size_t)kCtaRows * (DIM + 2)] = misc[2] != 0 ? 1.0f : 0.0f;
+        for (int i = 0; i < 16; ++i) o[c + i] = fmaf(o[c + i], down, v[i]);
+      });
+      const bool dirty = misc[3 + (seg & 1)] == seg;
+      if (r >= x.s.n * group) {
+        // a row past the sequence's
+      } else if (!x.whole) {
+        float* part = p.parts + (size_t)(2 * cta + (piece_at != begin)) * part_floats(DIM);
+        float* to = part + (size_t)(r - x.r0) * DIM;
+#pragma unroll
+        for (int d = 0; d < DIM; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
+        float* ml = part + (size_t)kCtaRows * DIM + 2 * (r - x.r0);
+        ml[0] = m;
+        ml[1] = l;
+        if (r == x.r0) part[(size_t)kCtaRows * (DIM + 2)] = dirty ? 1.0f : 0.0f;
+      } else {
+        float* to = a.out + (int64_t)(x.s.row0 + tok) * a.out_stride + (int64_t)(x.kvh * group + r % group) * DIM;
+        const float inv = 1.0f / l;
+        if ((reinterpret_cast<uintptr_t>(to) & 15) == 0 && !dirty) {
+#pragma unroll
+          for (int d = 0; d < DIM; d += 4)
+            *reinterpret_cast<float4*>(to + d) = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
         } else {
-          float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM;
-          const float inv = 1.0f / l;
-          const bool dirty = misc[2] != 0;
-          if ((reinterpret_cast<uintptr_t>(to) & 15) == 0 && !dirty) {
 #pragma unroll
-            for (int d = 0; d < DIM; d += 4)
-              *reinterpret_cast<float4*>(to + d) = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
-          } else {
-#pragma unroll
-            for (int d = 0; d < DIM; ++d)
-              to[d] = o[d] * inv + (dirty ? non_finite<true>(a.c, s, kvh, s.pos + first_tok, sees, d) : 0.f);
-          }
+          for (int d = 0; d < DIM; ++d)
+            to[d] = o[d] * inv + (dirty ? non_finite<true>(a.c, x.s, x.kvh, x.s.pos + x.first_tok, sees, d) : 0.f);
         }
       }
+      __syncwarp();
     }
   }
   fence_before();
@@ -536,40 +718,53 @@ __global__ void __launch_bounds__(kThreads, 1)
   }
 }
 
-// The splits of a row joined: one warp per row, in the order of the splits.
+// The pieces of the segment that starts in CTA blockIdx.x's range and goes on
+// past it (there is at most one) added up, in the order of the CTAs: a warp per
+// row, eight rows at a time; gridDim.y CTAs share the rows.
 template <int DIM>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p) {
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, int grid) {
   const AttendArgs& a = p.a;
   grid_dependency_wait();
   allow_dependents_launch();
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.c.kv_heads, kvh = blockIdx.y;
-  const int want = blockIdx.x / (kCtaRows / 8), row = blockIdx.x % (kCtaRows / 8) * 8 + warp;
-  int seq, tile;
-  if (!find_tile(a.c, group, kCtaRows, want, seq, tile)) return;
-  const Seq s = load_seq(a.c, seq);
-  const int r0 = tile * kCtaRows, r = r0 + row;
-  if (r >= s.n * group) return;
-  const float* part = p.parts + (size_t)(want * gridDim.y + kvh) * p.splits * part_floats(DIM);
-  constexpr size_t stride = part_floats(DIM);
-  const float* ml = part + (size_t)kCtaRows * DIM + 2 * row;
-  float m = lane < p.splits ? ml[lane * stride] : -INFINITY, top = m;
+  const Line line = line_of(p, grid);
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.c.kv_heads, cta = blockIdx.x;
+  if (line.work == 0 || cta >= line.ctas) return;
+  const int total = p.plan.count[1];
+  const int64_t begin = line.begin(cta), end = line.begin(cta + 1);
+  const int kvh = (int)((end - 1) / total), t = segment_of(p.plan, (int)((end - 1) % total));
+  const int64_t seg0 = (int64_t)kvh * total + p.plan.first[t], seg1 = (int64_t)kvh * total + p.plan.first[t + 1];
+  if (seg0 < begin || seg1 <= end) return;
+  const int n = line.cta_of(seg1 - 1) - cta + 1;
+  const Seq s = load_seq(a.c, p.plan.seq[t]);
+  const int r0 = p.plan.tile[t] * kCtaRows, rows = min(kCtaRows, s.n * group - r0);
+  const float* part0 = p.parts + (size_t)(2 * cta + (seg0 != begin)) * part_floats(DIM);
+  const float* part1 = p.parts + (size_t)(2 * cta) * part_floats(DIM);
+  auto part = [&](int i) { return i ? part1 + (size_t)(2 * i) * part_floats(DIM) : part0; };
+  bool dirty = false;
+  for (int i = lane; i < n; i += 32) dirty = dirty || part(i)[(size_t)kCtaRows * (DIM + 2)] != 0.f;
+  dirty = __any_sync(0xffffffffu, dirty);
+  for (int row = blockIdx.y * 8 + warp; row < rows; row += 8 * gridDim.y) {
+    const size_t ml = (size_t)kCtaRows * DIM + 2 * row;
+    float top = -INFINITY;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[ml]);
 #pragma unroll
-  for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-  const float f = m == -INFINITY ? 0.f : ex2(m - top);
-  const float l = warp_sum(lane < p.splits ? f * ml[lane * stride + 1] : 0.f);
-  constexpr int N = DIM / 32;
-  float o[N] = {};
-  for (int i = 0; i < p.splits; ++i) {
-    const float w = __shfl_sync(0xffffffffu, f, i);
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    constexpr int N = DIM / 32;
+    float o[N] = {}, l = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < n; ++i) {
+      const float* x = part(i);
+      const float f = x[ml] == -INFINITY ? 0.f : ex2(x[ml] - top);
+      l = fmaf(f, x[ml + 1], l);
 #pragma unroll
-    for (int k = 0; k < N; ++k) o[k] = fmaf(w, part[i * stride + (size_t)row * DIM + lane + 32 * k], o[k]);
+      for (int k = 0; k < N; ++k) o[k] = fmaf(f, x[(size_t)row * DIM + lane + 32 * k], o[k]);
+    }
+    const int r = r0 + row, tok = r / group, first = s.pos + r0 / group;
+    float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM;
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      to[lane + 32 * k] = o[k] / l + (dirty ? non_finite<true>(a.c, s, kvh, first, s.pos + tok, lane + 32 * k) : 0.f);
   }
-  const bool dirty = __any_sync(0xffffffffu, lane < p.splits && part[lane * stride + (size_t)kCtaRows * (DIM + 2)] != 0.f);
-  const int tok = r / group, first = s.pos + r0 / group;
-  float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM;
-#pragma unroll
-  for (int k = 0; k < N; ++k)
-    to[lane + 32 * k] = o[k] / l + (dirty ? non_finite<true>(a.c, s, kvh, first, s.pos + tok, lane + 32 * k) : 0.f);
 }
 
 PFN_cuTensorMapEncodeTiled_v12000 encode_fn() {
@@ -596,39 +791,36 @@ bool page_map(CUtensorMap* map, const void* base, const Cache& c, int box) {
 }
 
 template <int DIM>
-cudaError_t launch(const AttendArgs& a, int64_t max_len, cudaStream_t st) {
+cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   CUtensorMap mk, mv;
   Params p;
   p.a = a;
   p.box = std::min(a.c.page_size, kTile);
   if (!page_map(&mk, a.c.k, a.c, p.box) || !page_map(&mv, a.c.v, a.c, p.box)) return cudaErrorInvalidValue;
-  const int64_t tiles = ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + kCtaRows - 1) / kCtaRows + a.c.seqs;
-  // Few CTAs (a chunk of one request): the positions are cut so that every SM
-  // has one, at least four tiles each.
-  const int64_t ctas = tiles * a.c.kv_heads;
-  p.splits = (int)std::max<int64_t>(1, std::min<int64_t>({148 / ctas, kMaxParts / ctas, max_len / (4 * kTile), 32}));
-  p.parts = reinterpret_cast<float*>(static_cast<char*>(a.ws) + mma_workspace_bytes(DIM));
+  char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
+  p.plan = plan_of(ws);
+  p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
   auto k = chunk_tc_kernel<DIM>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
-  if (e != cudaSuccess) return e;
-  e = launch_ex(k, dim3((unsigned)tiles, (unsigned)a.c.kv_heads, (unsigned)p.splits), dim3(kThreads), Smem<DIM>::total, st,
-                mk, mv, p);
-  if (e != cudaSuccess || p.splits == 1) return e;
-  return launch_ex(join_kernel<DIM>, dim3((unsigned)(tiles * (kCtaRows / 8)), (unsigned)a.c.kv_heads), dim3(256), 0, st, p);
+  if (e == cudaSuccess) e = launch_ex(plan_kernel, dim3(1), dim3(1024), 0, st, a, p.plan);
+  if (e == cudaSuccess) e = launch_ex(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
+  if (e == cudaSuccess) e = launch_ex(join_kernel<DIM>, dim3(kMaxCtas, 4), dim3(256), 0, st, p, kMaxCtas);
+  return e;
 }
 
 }  // namespace
 
 bool tc_supported(const AttendArgs& a, bool kv16) {
   const int ps = a.c.page_size;
-  return kv16 && (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) && encode_fn() != nullptr;
+  const int64_t segs = ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + kCtaRows - 1) / kCtaRows + a.c.seqs;
+  return kv16 && (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) && segs <= kMaxSegs && encode_fn() != nullptr;
 }
 
-size_t tc_workspace_bytes(int dim) { return kMaxParts * part_floats(dim) * sizeof(float); }
+size_t tc_workspace_bytes(int dim) { return kPlanBytes + kMaxParts * part_floats(dim) * sizeof(float); }
 
-cudaError_t launch_chunks_tc(const AttendArgs& a, int64_t max_len, cudaStream_t st) {
-  return a.c.dim == 128 ? launch<128>(a, max_len, st) : launch<64>(a, max_len, st);
+cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st) {
+  return a.c.dim == 128 ? launch<128>(a, st) : launch<64>(a, st);
 }
 
 }  // namespace paged
