@@ -626,25 +626,30 @@ __global__ void __launch_bounds__(kThreads, 1)
         const int p0 = (x.j0 + j) * kTile;
         const bool masked = j >= x.jm;
         float top = -INFINITY;
-        tmem_each<kTile>(st, [&](float (&v)[16], int c) {
-          if (masked) {
+        // (two copies of either pass: the comparisons of a masked tile would
+        // take as long as the rest)
+        const int unseen_from = sees - p0 + 1;
+        auto mask = [&](float (&v)[16], int c) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (p0 + c + i > sees) v[i] = -INFINITY;
-          }
+          for (int i = 0; i < 16; ++i)
+            if (c + i >= unseen_from) v[i] = -INFINITY;
+        };
+        auto largest = [&](float (&v)[16]) {
 #pragma unroll
           for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, v[i]), v[i + 1]);
-        });
+        };
+        if (masked)
+          tmem_each<kTile>(st, [&](float (&v)[16], int c) {
+            mask(v, c);
+            largest(v);
+          });
+        else
+          tmem_each<kTile>(st, [&](float (&v)[16], int) { largest(v); });
         const float now = fmaxf(m, top * factor);
         const float next_down = now == -INFINITY ? 1.f : ex2(m - now);
         const float back = kBias - (now == -INFINITY ? 0.f : now);
         float sum = 0.f, sum2 = 0.f;
-        tmem_each<kTile>(st, [&](float (&v)[16], int c) {
-          if (masked) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i)
-              if (p0 + c + i > sees) v[i] = -INFINITY;
-          }
+        auto weigh = [&](float (&v)[16], int c) {
           uint32_t w[16];
 #pragma unroll
           for (int i = 0; i < 16; i += 2) {
@@ -656,7 +661,14 @@ __global__ void __launch_bounds__(kThreads, 1)
             w[8 + (i >> 1)] = pack_f16(x - xh, y - yh);
           }
           tmem_st(st + c, w);
-        });
+        };
+        if (masked)
+          tmem_each<kTile>(st, [&](float (&v)[16], int c) {
+            mask(v, c);
+            weigh(v, c);
+          });
+        else
+          tmem_each<kTile>(st, weigh);
         l = fmaf(l, next_down, sum + sum2);
         m = now;
         if (j > 0)  // the tile before: its product is done (the scores came after it)
