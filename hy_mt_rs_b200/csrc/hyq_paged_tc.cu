@@ -49,6 +49,7 @@ constexpr int kMinTiles = 2;             // position tiles of a CTA, at least
 // was taken out.
 __host__ __device__ constexpr size_t part_floats(int dim) { return (size_t)kCtaRows * (dim + 2) + 4; }
 constexpr float kBias = 10.0f;           // weights are kept 2^10 times their size (hyq_paged_mma.cu)
+constexpr float kSlack = 5.0f;           // a weight is at most 2^(kBias + kSlack): below f16's 65504
 constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DIM>
@@ -58,7 +59,7 @@ struct Smem {
   static constexpr int q = 0;                            // [row tile][hi, lo]
   static constexpr int ring = 4 * tile;
   static constexpr int bars = ring + kSlots * tile;
-  // full[3], empty[3], s_full[2], p_full[2], o_full[2], q_full[2], clean[2]
+  // full[3], empty[3], s_full[2], p_full[2], x_full[2], q_full[2], clean[2]
   static constexpr int n_bars = 2 * kSlots + 10;
   static constexpr int misc = bars + 8 * n_bars;         // tensor memory address, abort, first segment, dirty[2]
   static constexpr int total = misc + 32 + 1024;         // the base is moved to 1024 bytes
@@ -281,6 +282,26 @@ __device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t (&v)[16]) {
 __device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 
+__device__ __forceinline__ void tmem_ld(float (&v)[32], uint32_t a) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
+      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
+        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
+        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
+        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
+      : "r"(a));
+}
+__device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t (&v)[32]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
+      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
+      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
+      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
+      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
+      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
+      : "memory");
+}
 // f(columns, index of the first) over N columns from `a`, 16 at a time, the next
 // load in flight while one is worked on.
 template <int N, typename F>
@@ -328,7 +349,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto empty = [&](int s) { return base + L::bars + 8 * (kSlots + s); };
   auto s_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + w); };
   auto p_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 2 + w); };
-  auto o_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 4 + w); };
+  auto x_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 4 + w); };
   auto q_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 6 + w); };
   auto clean = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 8 + (i & 1)); };  // of masked tile i
   volatile int* misc = reinterpret_cast<volatile int*>(base_g + L::misc);
@@ -355,7 +376,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       for (int w = 0; w < 2; ++w) {
         mbar_init(s_full(w), 1);
         mbar_init(p_full(w), 4);
-        mbar_init(o_full(w), 1);
+        mbar_init(x_full(w), 1);
         mbar_init(q_full(w), 4);
         mbar_init(clean(w), 2);
       }
@@ -494,13 +515,12 @@ __global__ void __launch_bounds__(kThreads, 1)
             if (lane == 0) {
               outputs(w, iv % kSlots);
               const bool last = w == active - 1;
+              commit(x_full(w));
               if (last) commit(empty(iv % kSlots));
               if (j + 1 < x.nt) {
                 scores(w, ik % kSlots);
                 commit(s_full(w));
                 if (last) commit(empty(ik % kSlots));
-              } else {
-                commit(o_full(w));
               }
             }
             __syncwarp();
@@ -562,7 +582,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------- softmax -------------------------------
     const int wg = warp >= 8 ? 1 : 0;  // row tile
     const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 * wg;
-    int steps = 0, pieces = 0, seg = 0;
+    int steps = 0, seg = 0;
     bool ok = true;
     while (at < end && ok) {
       const Piece x = piece_of(p, group, t, kvh, at, end);
@@ -618,82 +638,133 @@ __global__ void __launch_bounds__(kThreads, 1)
       float o[DIM];
 #pragma unroll
       for (int d = 0; d < DIM; ++d) o[d] = 0.f;
+      // Weights are 2^(s - m + kBias) with a reference m that follows the row's
+      // maximum only when that is more than kSlack past it: the maximum pass
+      // over a tile's scores is then needed for the first tile alone.
       float m = -INFINITY, l = 0.f, down = 1.f;
+      // the product of the tile before, added to the row's outputs
+      auto collect = [&](int step) {
+        if (!warp_wait(x_full(wg), step & 1, abort_flag)) return false;
+        fence_after();
+        tmem_each<DIM>(st + 128, [&](float (&v)[16], int c) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[c + i] = fmaf(o[c + i], down, v[i]);
+        });
+        return true;
+      };
       for (int j = 0; j < x.nt; ++j, ++steps) {
-        ok = warp_wait(s_full(wg), steps & 1, abort_flag);
+        // (while the tensor cores are at this tile's scores)
+        ok = (j == 0 || collect(steps - 1)) && warp_wait(s_full(wg), steps & 1, abort_flag);
         if (!ok) break;
         fence_after();
-        const int p0 = (x.j0 + j) * kTile;
         const bool masked = j >= x.jm;
-        float top = -INFINITY;
-        // (two copies of either pass: the comparisons of a masked tile would
-        // take as long as the rest)
-        const int unseen_from = sees - p0 + 1;
-        auto mask = [&](float (&v)[16], int c) {
+        const int unseen_from = sees - (x.j0 + j) * kTile + 1;
+        auto mask = [&](float (&v)[32], int c) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i)
+          for (int i = 0; i < 32; ++i)
             if (c + i >= unseen_from) v[i] = -INFINITY;
         };
-        auto largest = [&](float (&v)[16]) {
+        auto largest = [&](const float (&v)[32]) {
+          float a0 = fmaxf(v[0], v[1]), a1 = fmaxf(v[2], v[3]);
 #pragma unroll
-          for (int i = 0; i < 16; i += 2) top = fmaxf(fmaxf(top, v[i]), v[i + 1]);
-        };
-        if (masked)
-          tmem_each<kTile>(st, [&](float (&v)[16], int c) {
-            mask(v, c);
-            largest(v);
-          });
-        else
-          tmem_each<kTile>(st, [&](float (&v)[16], int) { largest(v); });
-        const float now = fmaxf(m, top * factor);
-        const float next_down = now == -INFINITY ? 1.f : ex2(m - now);
-        const float back = kBias - (now == -INFINITY ? 0.f : now);
-        float sum = 0.f, sum2 = 0.f;
-        auto weigh = [&](float (&v)[16], int c) {
-          uint32_t w[16];
-#pragma unroll
-          for (int i = 0; i < 16; i += 2) {
-            const float x = ex2(fmaf(v[i], factor, back)), y = ex2(fmaf(v[i + 1], factor, back));
-            sum += x;
-            sum2 += y;
-            const float xh = high_part(x), yh = high_part(y);
-            w[i >> 1] = pack_f16(xh, yh);
-            w[8 + (i >> 1)] = pack_f16(x - xh, y - yh);
+          for (int i = 4; i < 32; i += 4) {
+            a0 = fmaxf(fmaxf(a0, v[i]), v[i + 1]);
+            a1 = fmaxf(fmaxf(a1, v[i + 2]), v[i + 3]);
           }
+          return fmaxf(a0, a1);
+        };
+        if (j == 0) {
+          float top = -INFINITY;
+#pragma unroll 1
+          for (int c = 0; c < kTile; c += 32) {
+            float v[32];
+            tmem_ld(v, st + c);
+            tmem_wait_ld();
+            if (masked) mask(v, c);
+            top = fmaxf(top, largest(v));
+          }
+          m = top * factor;
+        }
+        float back = kBias - (m == -INFINITY ? 0.f : m), sum = 0.f, sum2 = 0.f;
+        down = 1.f;
+        // 32 columns: scores to weights, hi and lo over them.  (Loops of 32
+        // columns, not unrolled, and two copies of them: the comparisons of a
+        // masked tile take as long as the rest, and the unrolled code ran out
+        // of the instruction cache.)
+        auto weigh = [&](float (&v)[32], int c) {
+          const float over = largest(v) * factor - m;
+          if (__any_sync(0xffffffffu, over > kSlack)) {
+            // raise the reference by whole powers of two; what this tile has
+            // so far follows
+            const float up = over > kSlack ? ceilf(over) : 0.f, f = ex2(-up);
+            m += up;
+            back -= up;
+            down *= f;
+            sum *= f;
+            sum2 *= f;
+            tmem_wait_st();
+#pragma unroll 1
+            for (int b = 0; b < c; b += 16) {
+              float w[16];
+              uint32_t u[16];
+              tmem_ld(w, st + b);
+              tmem_wait_ld();
+#pragma unroll
+              for (int i = 0; i < 8; ++i) {
+                const uint32_t hi = __float_as_uint(w[i]), lo = __float_as_uint(w[8 + i]);
+                const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+                const float2 a1 = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+                const float y0 = (a0.x + a1.x) * f, y1 = (a0.y + a1.y) * f, h0 = high_part(y0), h1 = high_part(y1);
+                u[i] = pack_f16(h0, h1);
+                u[8 + i] = pack_f16(y0 - h0, y1 - h1);
+              }
+              tmem_st(st + b, u);
+            }
+          }
+          uint32_t w[32];
+#pragma unroll
+          for (int g = 0; g < 32; g += 16)
+#pragma unroll
+            for (int i = 0; i < 16; i += 2) {
+              const float y0 = ex2(fmaf(v[g + i], factor, back)), y1 = ex2(fmaf(v[g + i + 1], factor, back));
+              sum += y0;
+              sum2 += y1;
+              const float h0 = high_part(y0), h1 = high_part(y1);
+              w[g + (i >> 1)] = pack_f16(h0, h1);
+              w[g + 8 + (i >> 1)] = pack_f16(y0 - h0, y1 - h1);
+            }
           tmem_st(st + c, w);
         };
-        if (masked)
-          tmem_each<kTile>(st, [&](float (&v)[16], int c) {
+        if (masked) {
+#pragma unroll 1
+          for (int c = 0; c < kTile; c += 32) {
+            float v[32];
+            tmem_ld(v, st + c);
+            tmem_wait_ld();
             mask(v, c);
             weigh(v, c);
-          });
-        else
-          tmem_each<kTile>(st, weigh);
-        l = fmaf(l, next_down, sum + sum2);
-        m = now;
-        if (j > 0)  // the tile before: its product is done (the scores came after it)
-          tmem_each<DIM>(st + 128, [&](float (&v)[16], int c) {
-#pragma unroll
-            for (int i = 0; i < 16; ++i) o[c + i] = fmaf(o[c + i], down, v[i]);
-          });
-        down = next_down;
+          }
+        } else {
+#pragma unroll 1
+          for (int c = 0; c < kTile; c += 32) {
+            float v[32];
+            tmem_ld(v, st + c);
+            tmem_wait_ld();
+            weigh(v, c);
+          }
+        }
+        l = fmaf(l, down, sum + sum2);
         tmem_wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(wg));
       }
-      ok = ok && warp_wait(o_full(wg), pieces & 1, abort_flag);
-      ++pieces;
+      ok = ok && collect(steps - 1);
       if (!ok) {
         if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_FULL);
         *abort_flag = 1;
         break;
       }
-      fence_after();
-      tmem_each<DIM>(st + 128, [&](float (&v)[16], int c) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) o[c + i] = fmaf(o[c + i], down, v[i]);
-      });
       const bool dirty = misc[3 + (seg & 1)] == seg;
       if (r >= x.s.n * group) {
         // a row past the sequence's
