@@ -328,6 +328,17 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
 // Ten mantissa bits of a weight (exact in f16 from 2^-14 up).
 __device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
+// The same value in every lane, known to be so: descriptors and addresses made
+// of such values stay in uniform registers, and a tcgen05.mma then takes 3
+// cycles to issue instead of 46 (64 to run), so that the queue of a handful
+// stays full across the waits between products.
+__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
+__device__ __forceinline__ bool elect() {
+  uint32_t p;
+  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
+  return p != 0;
+}
+
 // A wait of a whole warp: true only if every lane saw the phase complete.
 __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const volatile int* abort) {
   return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
@@ -354,7 +365,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto clean = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 8 + (i & 1)); };  // of masked tile i
   volatile int* misc = reinterpret_cast<volatile int*>(base_g + L::misc);
   volatile int* abort_flag = misc + 1;
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
   const int group = a.heads / a.c.kv_heads;
 
   grid_dependency_wait();
@@ -390,7 +401,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_before();
   __syncthreads();
   fence_after();
-  const uint32_t tmem = (uint32_t)misc[0];
+  const uint32_t tmem = (uint32_t)uniform(misc[0]);
   // every warp walks the same pieces: (segment, kv head), at its tile `at`
   int t = misc[2], kvh = (int)(begin / total);
   int64_t at = begin;
@@ -461,6 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (addresses are in the low bits of a descriptor, 16 bytes a unit)
       const uint64_t q_desc = desc_k_major(base + L::q), k_desc = desc_k_major(base + L::ring);
       const uint64_t v_desc = desc_mn_major(base + L::ring, L::half);
+      const bool one = elect();
       // lo first: the large sums then take half the (cut) additions
       auto scores = [&](int w, int slot) {
         const uint64_t q = q_desc + w * (2 * L::tile >> 4), k = k_desc + slot * (L::tile >> 4);
@@ -481,53 +493,69 @@ __global__ void __launch_bounds__(kThreads, 1)
           for (int t = 0; t < kTile / 16; ++t)  // 16 positions: hi in 8 columns from 16 t, lo in the next 8
             mma_ts(pw + 128, pw + 16 * t + 8 * h, v + t * (16 * 128 >> 4), idesc_o, h == 0 || t > 0);
       };
-      int i0 = 0, masked = 0;            // ring tiles and masked tiles before this piece
+      // slot and phase of the ring's next tile
+      int slot = 0, phase = 0, masked = 0;
+      auto advance = [&]() {
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
       int steps[2] = {0, 0}, pieces[2] = {0, 0};
       bool ok = true;
       while (at < end && ok) {
         const Piece x = piece_of(p, group, t, kvh, at, end);
-        const int active = x.two ? 2 : 1;
-        ok = wait(full(i0 % kSlots), (i0 / kSlots) & 1);
-        for (int w = 0; w < active && ok; ++w) {
+        const int active = uniform(x.two ? 2 : 1), nt = uniform(x.nt), jm = uniform(x.jm);
+        ok = wait(full(slot), phase);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (w >= active || !ok) break;
           ok = wait(q_full(w), pieces[w] & 1);
           if (!ok) break;
           fence_after();
-          if (lane == 0) {
-            scores(w, i0 % kSlots);
+          if (one) {
+            scores(w, slot);
             commit(s_full(w));
-            if (w == active - 1) commit(empty(i0 % kSlots));
+            if (w == active - 1) commit(empty(slot));
           }
           __syncwarp();
         }
-        for (int j = 0; j < x.nt && ok; ++j) {
-          const int iv = i0 + 2 * j + 1, ik = iv + 1;
-          ok = wait(full(iv % kSlots), (iv / kSlots) & 1);
-          if (ok && j >= x.jm) {
+        advance();
+        for (int j = 0; j < nt && ok; ++j) {
+          const int v_slot = slot;
+          ok = wait(full(slot), phase);
+          advance();
+          if (ok && j >= jm) {
             ok = wait(clean(masked), (masked >> 1) & 1);
             ++masked;
           }
-          ok = ok && (j + 1 >= x.nt || wait(full(ik % kSlots), (ik / kSlots) & 1));
-          for (int w = 0; w < active && ok; ++w) {
+          const int k_slot = slot;
+          if (ok && j + 1 < nt) {
+            ok = wait(full(slot), phase);
+            advance();
+          }
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (w >= active || !ok) break;
             ok = wait(p_full(w), steps[w] & 1);
             if (!ok) break;
             ++steps[w];
             fence_after();
-            if (lane == 0) {
-              outputs(w, iv % kSlots);
-              const bool last = w == active - 1;
+            if (one) {
+              outputs(w, v_slot);
               commit(x_full(w));
-              if (last) commit(empty(iv % kSlots));
-              if (j + 1 < x.nt) {
-                scores(w, ik % kSlots);
+              if (w == active - 1) commit(empty(v_slot));
+              if (j + 1 < nt) {
+                scores(w, k_slot);
                 commit(s_full(w));
-                if (last) commit(empty(ik % kSlots));
+                if (w == active - 1) commit(empty(k_slot));
               }
             }
             __syncwarp();
           }
         }
-        for (int w = 0; w < active; ++w) ++pieces[w];
-        i0 += 2 * x.nt;
+        ++pieces[0];
+        if (active == 2) ++pieces[1];
         next(x);
       }
     } else {
