@@ -40,7 +40,11 @@ struct Geo {
   static constexpr int stages = 24576 / block;        // 3 (head size 128), 6 (64)
   static constexpr int tile = kWarps * pos;           // positions of a CTA's step
   static constexpr int copies = pos * chunks / 32;    // 16-byte copies per lane, K or V
-  static constexpr int smem = kWarps * stages * block;
+  static constexpr int ring = kWarps * stages * block;
+  // 16 rows of queries (hi and lo f16, or f32), later of the warps' joined
+  // outputs, eight floats apart more than they need (banks)
+  static constexpr int pitch = DIM + 8;
+  static constexpr int smem = ring + kRows * pitch * 4;
 };
 
 __device__ __forceinline__ float ex2(float x) {
@@ -91,6 +95,67 @@ __device__ __forceinline__ void split_tf32(float x, uint32_t& hi, uint32_t& lo) 
   lo = __float_as_uint(x - __uint_as_float(hi)) & 0xffffe000u;
 }
 
+// The queries of a block of 16 (token, head) rows (block row 0 is row r0 of the
+// sequence): rows first, first + step, .. below `rows` by a warp.  First their
+// f32 values into shared memory, DIM of them per row one after another ...
+template <int DIM>
+__device__ __forceinline__ void fetch_queries(uint32_t raw_s, const AttendArgs& a, const Seq& s, int kvh, int group,
+                                              int r0, int rows, int first, int step) {
+  const int lane = threadIdx.x & 31;
+  int i = 0;
+  for (int row = first; row < rows; row += step, ++i) {
+    const int r = r0 + row, tok = r / group;
+    const float* q = a.q + (int64_t)(s.row0 + tok) * a.q_stride + (int64_t)(kvh * group + r - tok * group) * DIM + lane;
+#pragma unroll
+    for (int k = 0; k < DIM / 32; ++k)  // 4 bytes each: queries need no alignment
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(raw_s + 4 * (i * DIM + 32 * k + lane)), "l"(q + 32 * k)
+                   : "memory");
+  }
+}
+// ... then, scaled by log2(e) / sqrt(DIM), as f32, or as hi and lo f16 after an
+// exact power of two that brings the row's largest value to [1, 2) and goes back
+// into its scores, so that no query overflows f16.  Rows are DIM values in
+// 16-byte chunks xored like the cache's.
+template <int DIM, bool KV16>
+__device__ __forceinline__ void stage_queries(uint32_t q_s, float* factor_s, uint32_t raw_s, int rows, int first, int step) {
+  constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;
+  constexpr int N = DIM / 32;  // values per lane
+  const int lane = threadIdx.x & 31;
+  int i = 0;
+  for (int row = first; row < rows; row += step, ++i) {
+    float x[N], top = 0.f;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      asm volatile("ld.shared.f32 %0, [%1];" : "=f"(x[k]) : "r"(raw_s + 4 * (i * DIM + N * lane + k)) : "memory");
+      x[k] *= scale;
+      top = fmaxf(top, fabsf(x[k]));
+    }
+    const int d = N * lane;
+    if constexpr (KV16) {
+#pragma unroll
+      for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+      // exponent bits of the largest value, kept where both powers are normal
+      const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
+      const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+      if (lane == 0) factor_s[row] = __uint_as_float((uint32_t)e << 23);
+      const int c = d >> 3;
+      const uint32_t at = q_s + row * (2 * DIM) + (((c & ~7) | ((c ^ row) & 7)) << 4) + (d & 7) * 2;
+#pragma unroll
+      for (int k = 0; k < N; k += 2) {
+        uint32_t hi, lo;
+        split_f16(x[k] * down, x[k + 1] * down, hi, lo);
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 2 * k), "r"(hi) : "memory");
+        asm volatile("st.shared.u32 [%0], %1;" ::"r"(at + 2 * k + kRows * 2 * DIM), "r"(lo) : "memory");
+      }
+    } else {
+      const int c = d >> 2;
+      const uint32_t at = q_s + row * (4 * DIM) + (((c & ~7) | ((c ^ row) & 7)) << 4) + (d & 3) * 4;
+#pragma unroll
+      for (int k = 0; k < N; ++k) asm volatile("st.shared.f32 [%0], %1;" ::"r"(at + 4 * k), "f"(x[k]) : "memory");
+    }
+  }
+}
+
 // What a warp holds of its 16 rows: the queries as the left operand of the
 // score products, the running maximum and sum, and the output.  Lane l holds
 // rows l / 4 and l / 4 + 8.
@@ -104,61 +169,32 @@ struct Rows {
   float o[DIM / 8][4];
   float m[2], l[2];
 
-  // Rows r0 .. r0 + 15 of the sequence's n * group (token, head) rows; rows
-  // past them are zero.
-  __device__ __forceinline__ void load(const AttendArgs& a, const Seq& s, int kvh, int group, int r0) {
-    const int lane = threadIdx.x & 31, t = lane & 3;
-    constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;  // log2(e) / sqrt(DIM)
-    const float* q[2];
-    bool in[2];
+  // Fragments of the rows that stage_queries() left at q_s.
+  __device__ __forceinline__ void load(uint32_t q_s, const float* factor_s, const Seq& s, int group, int r0) {
+    const int lane = threadIdx.x & 31, mat = lane >> 3, row = 8 * (mat & 1) + (lane & 7);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const int r = r0 + (lane >> 2) + 8 * i, tok = r / group;
-      in[i] = tok < s.n;
-      sees[i] = s.pos + min(tok, s.n - 1);
-      q[i] = a.q + (int64_t)(s.row0 + (in[i] ? tok : 0)) * a.q_stride + (int64_t)(kvh * group + (in[i] ? r - tok * group : 0)) * DIM;
-      factor[i] = 1.0f;
+      const int r = (lane >> 2) + 8 * i;
+      sees[i] = s.pos + min((r0 + r) / group, s.n - 1);
+      factor[i] = KV16 ? factor_s[r] : 1.0f;
     }
     if constexpr (KV16) {
-      // the row's largest value to [1, 2): an exact power of two, put back in
-      // the scores, so that no query overflows f16
-      float x[DIM / 16][2][4];
-      float top[2] = {0.f, 0.f};
 #pragma unroll
-      for (int k = 0; k < DIM / 16; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) {
-            const float v = in[i] ? q[i][16 * k + 2 * t + (j & 1) + 8 * (j >> 1)] * scale : 0.f;
-            x[k][i][j] = v;
-            top[i] = fmaxf(top[i], fabsf(v));
-          }
-      float down[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 1));
-        top[i] = fmaxf(top[i], __shfl_xor_sync(0xffffffffu, top[i], 2));
-        // exponent bits of the largest value, kept where both powers are normal
-        const int e = min(max((int)(__float_as_uint(top[i]) >> 23), 1), 253);
-        factor[i] = __uint_as_float((uint32_t)e << 23);
-        down[i] = __uint_as_float((uint32_t)(254 - e) << 23);
+      for (int k = 0; k < DIM / 16; ++k) {
+        const int c = 2 * k + (mat >> 1);
+        const uint32_t at = q_s + row * (2 * DIM) + (((c & ~7) | ((c ^ row) & 7)) << 4);
+        ldsm4(qh[k], at);
+        ldsm4(ql[k], at + kRows * 2 * DIM);
       }
-#pragma unroll
-      for (int k = 0; k < DIM / 16; ++k)
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          split_f16(x[k][i][0] * down[i], x[k][i][1] * down[i], qh[k][i], ql[k][i]);
-          split_f16(x[k][i][2] * down[i], x[k][i][3] * down[i], qh[k][2 + i], ql[k][2 + i]);
-        }
     } else {
 #pragma unroll
-      for (int k = 0; k < DIM / 8; ++k)
+      for (int k = 0; k < DIM / 8; ++k) {
+        const int c = 2 * k + (mat >> 1);
+        uint32_t x[4];
+        ldsm4(x, q_s + row * (4 * DIM) + (((c & ~7) | ((c ^ row) & 7)) << 4));
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          qf[k][i] = in[i] ? q[i][8 * k + t] * scale : 0.f;
-          qf[k][2 + i] = in[i] ? q[i][8 * k + t + 4] * scale : 0.f;
-        }
+        for (int j = 0; j < 4; ++j) qf[k][j] = __uint_as_float(x[j]);
+      }
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
@@ -395,9 +431,13 @@ struct Feed {
 constexpr size_t kCounterBytes = (kMaxCtas * sizeof(unsigned) + 255) / 256 * 256;
 __host__ __device__ constexpr int partial_floats(int dim) { return kRows * (dim + 2); }
 
-// The (sequence, kv head) segments' tiles form one line, cut into equal
-// ranges, one per CTA: any mix of lengths loads every SM alike and the whole
-// cache is read once.  A segment inside one CTA's range is finished there;
+// What a segment costs beside its tiles (queries, first copies, joining the
+// warps), in tiles: the time of about four at full bandwidth.
+constexpr int kSegmentCost = 4;
+
+// The (sequence, kv head) segments' tiles, with kSegmentCost empty ones after
+// each, form one line, cut into equal ranges, one per CTA: any mix of lengths
+// loads every SM alike and the whole cache is read once.  A segment inside one CTA's range is finished there;
 // one that spans CTAs leaves partial results, and the last CTA to get there
 // adds them in the order of the CTAs (the result does not depend on which one
 // that is).  Within a tile each warp takes its own POS positions for all 16
@@ -411,6 +451,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
   extern __shared__ __align__(1024) char smem[];
   int* first_s = reinterpret_cast<int*>(smem + G::smem);  // [seqs + 1] tiles (of one kv head) before each sequence
   __shared__ float ml_s[kWarps][kRows][2];
+  __shared__ float factor_s[kRows];
   __shared__ int warp_s[kWarps];
   __shared__ int last_s;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -423,7 +464,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     int tiles = 0;
     if (i < seqs) {
       const Seq s = load_seq(a.c, i);
-      if (s.n > 0 && s.n * group <= kRows) tiles = (s.pos + s.n + G::tile - 1) / G::tile;
+      if (s.n > 0 && s.n * group <= kRows) tiles = (s.pos + s.n + G::tile - 1) / G::tile + kSegmentCost;
     }
     int x = tiles;
 #pragma unroll
@@ -464,46 +505,86 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
   unsigned* counters = static_cast<unsigned*>(a.ws);
   Rows<DIM, KV16> rows;
   const uint32_t ring = smem_addr(smem) + warp * G::stages * G::block;
-  while (at < end) {
-    while ((int64_t)first_s[si + 1] * kvh_n <= at) ++si;  // past empty sequences
-    const int tiles = first_s[si + 1] - first_s[si];
-    const int64_t s_at = (int64_t)first_s[si] * kvh_n;
-    const int kvh = (int)((at - s_at) / tiles);
-    const int64_t seg0 = s_at + (int64_t)kvh * tiles, seg1 = seg0 + tiles;
-    const int j0 = (int)(at - seg0), j1 = (int)(min(end, seg1) - seg0);
-    const Seq s = load_seq(a.c, si);
-    const Feed<DIM, KV16> feed{a, s, kvh, s.pos + s.n, shift};
-    const int step = G::tile, off = warp * G::pos;
-    // fill the ring, then one block per turn
-    int page = feed.page(j0 * step + off);
+  float* o_s = reinterpret_cast<float*>(smem + G::ring);  // [16][pitch]; the queries before
+  const int off = warp * G::pos;
+  // the piece of a segment that this CTA takes: tiles j0 .. j1 - 1 of `tiles`
+  struct {
+    Seq s;
+    int kvh, j0, j1, tiles;
+    int64_t seg0;
+  } cur, done;
+  int page = -1;  // of this lane's row in the next block to copy
+  // the piece at `at`, and its first copies
+  // (at the end of the range when only empty tiles are left)
+  auto open = [&](bool same_seq) {
+    for (;;) {
+      while ((int64_t)first_s[si + 1] * kvh_n <= at) {  // past empty sequences
+        ++si;
+        same_seq = false;
+      }
+      const int units = first_s[si + 1] - first_s[si];
+      const int64_t s_at = (int64_t)first_s[si] * kvh_n;
+      cur.tiles = units - kSegmentCost;
+      cur.kvh = (int)((at - s_at) / units);
+      cur.seg0 = s_at + (int64_t)cur.kvh * units;
+      if (at - cur.seg0 < cur.tiles) break;
+      at = cur.seg0 + units;
+      if (at >= end) return;
+    }
+    cur.j0 = (int)(at - cur.seg0);
+    cur.j1 = (int)(min(end, cur.seg0 + cur.tiles) - cur.seg0);
+    if (!same_seq) cur.s = load_seq(a.c, si);
+    const Feed<DIM, KV16> feed{a, cur.s, cur.kvh, cur.s.pos + cur.s.n, shift};
+    page = feed.page(cur.j0 * G::tile + off);
+    // (the ring's last stage is not copied to before the first turn)
+    fetch_queries<DIM>(ring + (G::stages - 1) * G::block, a, cur.s, cur.kvh, group, 0, cur.s.n * group, warp, kWarps);
+    cp_async_commit();
 #pragma unroll
     for (int i = 0; i < G::stages - 1; ++i) {
       const int now = page;
-      page = feed.page((j0 + i + 1) * step + off);
-      if (j0 + i < j1) feed.copy(ring + i * G::block, (j0 + i) * step + off, now);
+      page = feed.page((cur.j0 + i + 1) * G::tile + off);
+      if (cur.j0 + i < cur.j1) feed.copy(ring + i * G::block, (cur.j0 + i) * G::tile + off, now);
       cp_async_commit();
     }
-    rows.load(a, s, kvh, group, 0);
-    int stage = 0;
-    for (int j = j0; j < j1; ++j) {
-      const int ahead = j + G::stages - 1, now = page;
-      page = feed.page((ahead + 1) * step + off);
-      int put = stage + G::stages - 1;
-      if (put >= G::stages) put -= G::stages;
-      __syncwarp();
-      if (ahead < j1) feed.copy(ring + put * G::block, ahead * step + off, now);
-      cp_async_commit();
+  };
+  open(false);
+  while (at < end) {
+    {
+      const Seq& s = cur.s;
+      const uint32_t q_s = smem_addr(o_s);
       cp_async_wait<G::stages - 1>();
       __syncwarp();
-      const int p0 = j * step + off;
-      const bool masked = p0 + G::pos - 1 > s.pos;
-      if (masked) feed.clean(ring + stage * G::block, p0, s.pos);
-      rows.step(ring + stage * G::block, p0, masked);
-      if (++stage == G::stages) stage = 0;
+      stage_queries<DIM, KV16>(q_s, factor_s, ring + (G::stages - 1) * G::block, s.n * group, warp, kWarps);
+      __syncthreads();
+      rows.load(q_s, factor_s, s, group, 0);
+      const Feed<DIM, KV16> feed{a, s, cur.kvh, s.pos + s.n, shift};
+      int stage = 0;
+      for (int j = cur.j0; j < cur.j1; ++j) {
+        const int ahead = j + G::stages - 1, now = page;
+        page = feed.page((ahead + 1) * G::tile + off);
+        int put = stage + G::stages - 1;
+        if (put >= G::stages) put -= G::stages;
+        __syncwarp();
+        if (ahead < cur.j1) feed.copy(ring + put * G::block, ahead * G::tile + off, now);
+        cp_async_commit();
+        cp_async_wait<G::stages - 1>();
+        __syncwarp();
+        const int p0 = j * G::tile + off;
+        const bool masked = p0 + G::pos - 1 > s.pos;
+        if (masked) feed.clean(ring + stage * G::block, p0, s.pos);
+        rows.step(ring + stage * G::block, p0, masked);
+        if (++stage == G::stages) stage = 0;
+      }
     }
-    // the warps' results: maximum and sum of each row, then the outputs
-    // scaled to the common maximum, in the rings' memory
-    cp_async_wait<0>();
+    const bool second = at != begin;  // not at this CTA's range's start
+    done = cur;
+    at = cur.j1 < cur.tiles ? end : cur.seg0 + cur.tiles;
+    __syncwarp();
+    if (at < end) open(true);  // the next piece's copies run while this one is joined
+    // the warps' results: maximum and sum of each row, then the outputs scaled
+    // to the common maximum, added up warp after warp
+    const Seq& s = done.s;
+    const int kvh = done.kvh, live = s.n * group;
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       float l = rows.l[i];
@@ -515,45 +596,58 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
       }
     }
     __syncthreads();
-    constexpr int pitch = DIM + 4;
-    float* o_s = reinterpret_cast<float*>(smem);  // [warp][16][pitch]
-    static_assert(kWarps * kRows * pitch * 4 <= G::smem && kRows * kMaxCtas * 4 <= G::smem,
-                  "the rings hold the warps' outputs and a combination's weights");
+    float down[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = (lane >> 2) + 8 * i;
       float top = ml_s[0][r][0];
 #pragma unroll
       for (int w = 1; w < kWarps; ++w) top = fmaxf(top, ml_s[w][r][0]);
-      const float down = rows.m[i] == -INFINITY ? 0.f : ex2(rows.m[i] - top);
-      float* to = o_s + (warp * kRows + r) * pitch + 2 * (lane & 3);
-#pragma unroll
-      for (int d = 0; d < DIM / 8; ++d)
-        *reinterpret_cast<float2*>(to + 8 * d) = make_float2(rows.o[d][2 * i] * down, rows.o[d][2 * i + 1] * down);
+      down[i] = rows.m[i] == -INFINITY ? 0.f : ex2(rows.m[i] - top);
     }
-    __syncthreads();
-    const int live = s.n * group;
-    const bool whole = j0 == 0 && j1 == tiles;
-    float* part = parts + (size_t)(2 * cta + (at != begin)) * partial_floats(DIM);
-    for (int x = threadIdx.x; x < live * DIM; x += kThreads) {
-      const int r = x / DIM, d = x % DIM;
-      float sum = 0.f, top = -INFINITY, l = 0.f;
+#pragma unroll 1
+    for (int w = 0; w < kWarps; ++w) {
+      if (warp == w) {
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        sum += o_s[(w * kRows + r) * pitch + d];
-        top = fmaxf(top, ml_s[w][r][0]);
+        for (int i = 0; i < 2; ++i) {
+          const int r = (lane >> 2) + 8 * i;
+          if (r >= live) continue;
+          float2* to = reinterpret_cast<float2*>(o_s + r * G::pitch + 2 * (lane & 3));
+#pragma unroll
+          for (int d = 0; d < DIM / 8; ++d) {
+            const float2 before = w ? to[4 * d] : make_float2(0.f, 0.f);
+            to[4 * d] = make_float2(fmaf(rows.o[d][2 * i], down[i], before.x), fmaf(rows.o[d][2 * i + 1], down[i], before.y));
+          }
+        }
       }
+      __syncthreads();
+    }
+    const bool whole = done.j0 == 0 && done.j1 == done.tiles;
+    float* part = parts + (size_t)(2 * cta + second) * partial_floats(DIM);
+    constexpr int N = DIM / 32;  // values per lane, a warp per row
+    for (int r = warp; r < live; r += kWarps) {
+      float top = -INFINITY, l = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w][r][0]);
 #pragma unroll
       for (int w = 0; w < kWarps; ++w)
         l += ml_s[w][r][0] == -INFINITY ? 0.f : ml_s[w][r][1] * ex2(ml_s[w][r][0] - top);
+      const float* from = o_s + r * G::pitch;
       if (whole) {
         const int tok = r / group;
-        float y = sum / l;
-        if (s.n > 1) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
-        a.out[(int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + d] = y;
+        float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM;
+        const float inv = 1.0f / l;
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int d = lane + 32 * k;
+          float y = from[d] * inv;
+          if (s.n > 1) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
+          to[d] = y;
+        }
       } else {
-        part[x] = sum;
-        if (d == 0) {
+#pragma unroll
+        for (int k = 0; k < N; ++k) part[r * DIM + lane + 32 * k] = from[lane + 32 * k];
+        if (lane == 0) {
           part[kRows * DIM + 2 * r] = top;
           part[kRows * DIM + 2 * r + 1] = l;
         }
@@ -561,64 +655,63 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     }
     if (!whole) {
       // the CTAs that share the segment: cf holds its first tile, cl its last
+      const int64_t seg0 = done.seg0, seg1 = seg0 + done.tiles;
       int cf = (int)(seg0 * ctas / work);
       while (work * (cf + 1) / ctas <= seg0) ++cf;
       while (cf > 0 && work * cf / ctas > seg0) --cf;
       int cl = (int)((seg1 - 1) * ctas / work);
       while (work * (cl + 1) / ctas <= seg1 - 1) ++cl;
       while (cl > 0 && work * cl / ctas > seg1 - 1) --cl;
-      __threadfence();
+      // the CTA's stores come before the count by the barrier and this fence
       __syncthreads();
-      if (threadIdx.x == 0) last_s = atomicAdd(&counters[cf], 1u) == (unsigned)(cl - cf);
+      if (threadIdx.x == 0) {
+        __threadfence();
+        last_s = atomicAdd(&counters[cf], 1u) == (unsigned)(cl - cf);
+      }
       __syncthreads();
       if (last_s) {
         __threadfence();
         // partials cf .. cl, in order; only cf's may be its CTA's second
         const int n = cl - cf + 1;
-        const float* p0 = parts + (size_t)(2 * cf + (work * cf / ctas < seg0)) * partial_floats(DIM);
-        const float* p1 = parts + (size_t)(2 * cf) * partial_floats(DIM);
-        auto part_at = [&](int i) { return i ? p1 + (size_t)(2 * i) * partial_floats(DIM) : p0; };
-        // each row's weight of each partial, a warp per row, in the rings' memory
-        float* f_s = reinterpret_cast<float*>(smem);  // [row][n]
+        const float* part0 = parts + (size_t)(2 * cf + (work * cf / ctas < seg0)) * partial_floats(DIM);
+        const float* part1 = parts + (size_t)(2 * cf) * partial_floats(DIM);
+        auto part_at = [&](int i) { return i ? part1 + (size_t)(2 * i) * partial_floats(DIM) : part0; };
         for (int r = warp; r < live; r += kWarps) {
-          float top = -INFINITY, l = 0.f;
+          float top = -INFINITY, l = 0.f, sum[N] = {};
           for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(part_at(i) + kRows * DIM + 2 * r));
 #pragma unroll
           for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-          for (int i = lane; i < n; i += 32) {
-            const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_at(i) + kRows * DIM + 2 * r));
-            const float f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
-            f_s[r * n + i] = f;
-            l = fmaf(f, ml.y, l);
-          }
-          l = warp_sum(l);
-          if (lane == 0) ml_s[0][r][1] = 1.0f / l;
-        }
-        __syncthreads();
-        for (int x = threadIdx.x; x < live * (DIM / 4); x += kThreads) {
-          const int r = x / (DIM / 4), d = 4 * (x % (DIM / 4));
-          float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (int i0 = 0; i0 < n; i0 += 32) {
+            float f = 0.f;  // the weight of partial i0 + lane
+            if (i0 + lane < n) {
+              const float2 ml = __ldcg(reinterpret_cast<const float2*>(part_at(i0 + lane) + kRows * DIM + 2 * r));
+              f = ml.x == -INFINITY ? 0.f : ex2(ml.x - top);
+              l = fmaf(f, ml.y, l);
+            }
+            const int m = min(32, n - i0);
 #pragma unroll 8
-          for (int i = 0; i < n; ++i) {
-            const float4 v = __ldcg(reinterpret_cast<const float4*>(part_at(i) + r * DIM + d));
-            const float f = f_s[r * n + i];
-            sum.x = fmaf(f, v.x, sum.x);
-            sum.y = fmaf(f, v.y, sum.y);
-            sum.z = fmaf(f, v.z, sum.z);
-            sum.w = fmaf(f, v.w, sum.w);
-          }
-          const int tok = r / group;
-          float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + d;
-          const float inv = ml_s[0][r][1];
-          const float y[4] = {sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv};
+            for (int i = 0; i < m; ++i) {
+              const float w = __shfl_sync(0xffffffffu, f, i);
+              const float* from = part_at(i0 + i) + r * DIM + lane;
 #pragma unroll
-          for (int k = 0; k < 4; ++k) to[k] = s.n > 1 ? y[k] + non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d + k) : y[k];
+              for (int k = 0; k < N; ++k) sum[k] = fmaf(w, __ldcg(from + 32 * k), sum[k]);
+            }
+          }
+          const float inv = 1.0f / warp_sum(l);
+          const int tok = r / group;
+          float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM;
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const int d = lane + 32 * k;
+            float y = sum[k] * inv;
+            if (s.n > 1) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
+            to[d] = y;
+          }
         }
         if (threadIdx.x == 0) counters[cf] = 0;
       }
     }
-    at = seg0 + j1;
-    __syncthreads();  // the rings are free again
+    __syncthreads();  // o_s and ml_s are free again
   }
 }
 
@@ -637,6 +730,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
   allow_dependents_launch();
   extern __shared__ __align__(1024) char smem[];
   __shared__ int found_s[2];
+  __shared__ float factor_s[kWarps][kRows];
   __shared__ int dirty_s;  // clean() took something out
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.heads / a.c.kv_heads, kvh = blockIdx.y;
@@ -662,6 +756,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
   const int first_tok = min(s.n - 1, found_s[1] * kChunkRows / group);
   const Feed<DIM, KV16> feed{a, s, kvh, len, shift};
   const uint32_t ring = smem_addr(smem);
+  // the queries: each warp's own 16 rows, through its part of the ring
+  static_assert(G::stages * G::block >= 2 * kRows * DIM * 4, "a warp's queries, as they come and as they are read");
+  Rows<DIM, KV16> rows;
+  const bool any = r0 < s.n * group;
+  if (any) {
+    const uint32_t q_s = ring + warp * G::stages * G::block, raw_s = q_s + kRows * DIM * 4;
+    const int n = min(kRows, s.n * group - r0);
+    fetch_queries<DIM>(raw_s, a, s, kvh, group, r0, n, 0, 1);
+    cp_async_commit();
+    cp_async_wait<0>();
+    __syncwarp();
+    stage_queries<DIM, KV16>(q_s, factor_s[warp], raw_s, n, 0, 1);
+    __syncwarp();
+    rows.load(q_s, factor_s[warp], s, group, r0);
+  }
+  __syncthreads();
   constexpr int stage_bytes = kWarps * G::block;
   const int off = warp * G::pos;
   int page = feed.page(off);
@@ -672,9 +782,6 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
     if (i < tiles) feed.copy(ring + i * stage_bytes + warp * G::block, i * G::tile + off, now);
     cp_async_commit();
   }
-  Rows<DIM, KV16> rows;
-  rows.load(a, s, kvh, group, r0);
-  const bool any = r0 < s.n * group;
   int stage = 0;
   for (int j = 0; j < tiles; ++j) {
     cp_async_wait<G::stages - 2>();

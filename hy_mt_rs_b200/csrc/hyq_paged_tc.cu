@@ -628,7 +628,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;  // log2(e) / sqrt(DIM)
         constexpr int N = DIM / 32;  // values per lane
         uint8_t* q_s = base_g + L::q + wg * 2 * L::tile;
-#pragma unroll 4
+#pragma unroll 8
         for (int i = 0; i < 32; ++i) {
           const int row = 32 * (warp & 3) + i, rr = x.r0 + wg * kTile + row, tk = rr / group;
           float v[N], top = 0.f;
@@ -830,13 +830,16 @@ __global__ void __launch_bounds__(kThreads, 1)
 }
 
 // The pieces of the segment that starts in CTA blockIdx.x's range and goes on
-// past it (there is at most one) added up, in the order of the CTAs: a warp per
-// row, eight rows at a time; gridDim.y CTAs share the rows.
+// past it (there is at most one) added up, in the order of the CTAs; blockIdx.y
+// picks 32 of its rows.  The pieces' weights of all rows first, then four rows
+// of outputs per warp with their loads in flight together.
+constexpr int kJoinRows = 32;
 template <int DIM>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, int grid) {
   const AttendArgs& a = p.a;
   grid_dependency_wait();
   allow_dependents_launch();
+  __shared__ float f_s[kJoinRows][kMaxCtas + 1], l_s[kJoinRows];
   const Line line = line_of(p, grid);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.c.kv_heads, cta = blockIdx.x;
   if (line.work == 0 || cta >= line.ctas) return;
@@ -847,34 +850,56 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
   if (seg0 < begin || seg1 <= end) return;
   const int n = line.cta_of(seg1 - 1) - cta + 1;
   const Seq s = load_seq(a.c, p.plan.seq[t]);
-  const int r0 = p.plan.tile[t] * kCtaRows, rows = min(kCtaRows, s.n * group - r0);
+  const int r0 = p.plan.tile[t] * kCtaRows, row0 = blockIdx.y * kJoinRows;
+  const int rows = min(kJoinRows, s.n * group - r0 - row0);
+  if (rows <= 0) return;
   const float* part0 = p.parts + (size_t)(2 * cta + (seg0 != begin)) * part_floats(DIM);
   const float* part1 = p.parts + (size_t)(2 * cta) * part_floats(DIM);
   auto part = [&](int i) { return i ? part1 + (size_t)(2 * i) * part_floats(DIM) : part0; };
   bool dirty = false;
   for (int i = lane; i < n; i += 32) dirty = dirty || part(i)[(size_t)kCtaRows * (DIM + 2)] != 0.f;
   dirty = __any_sync(0xffffffffu, dirty);
-  for (int row = blockIdx.y * 8 + warp; row < rows; row += 8 * gridDim.y) {
-    const size_t ml = (size_t)kCtaRows * DIM + 2 * row;
-    float top = -INFINITY;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, part(i)[ml]);
+  // a lane per row, a warp per eighth of the pieces; then their common maximum
+  for (int x = threadIdx.x; x < n * kJoinRows; x += 256) {
+    const int row = x % kJoinRows, i = x / kJoinRows;
+    f_s[row][i] = row < rows ? part(i)[(size_t)kCtaRows * DIM + 2 * (row0 + row)] : 0.f;
+  }
+  __syncthreads();
+  for (int row = warp; row < rows; row += 8) {
+    float top = -INFINITY, l = 0.f;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, f_s[row][i]);
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    constexpr int N = DIM / 32;
-    float o[N] = {}, l = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < n; ++i) {
-      const float* x = part(i);
-      const float f = x[ml] == -INFINITY ? 0.f : ex2(x[ml] - top);
-      l = fmaf(f, x[ml + 1], l);
-#pragma unroll
-      for (int k = 0; k < N; ++k) o[k] = fmaf(f, x[(size_t)row * DIM + lane + 32 * k], o[k]);
+    for (int i = lane; i < n; i += 32) {
+      const float m = f_s[row][i], f = m == -INFINITY ? 0.f : ex2(m - top);
+      l = fmaf(f, part(i)[(size_t)kCtaRows * DIM + 2 * (row0 + row) + 1], l);
+      f_s[row][i] = f;
     }
-    const int r = r0 + row, tok = r / group, first = s.pos + r0 / group;
+    l = warp_sum(l);
+    if (lane == 0) l_s[row] = l;
+  }
+  __syncthreads();
+  constexpr int N = DIM / 32;
+  float o[4][N] = {};
+#pragma unroll 2
+  for (int i = 0; i < n; ++i) {
+    const float* x = part(i) + (size_t)row0 * DIM + lane;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      const int row = min(warp + 8 * q, rows - 1);
+      const float f = f_s[row][i];
+#pragma unroll
+      for (int k = 0; k < N; ++k) o[q][k] = fmaf(f, x[(size_t)row * DIM + 32 * k], o[q][k]);
+    }
+  }
+#pragma unroll
+  for (int q = 0; q < 4; ++q) {
+    const int row = warp + 8 * q, r = r0 + row0 + row, tok = r / group, first = s.pos + r0 / group;
+    if (row >= rows) break;
     float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM;
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      to[lane + 32 * k] = o[k] / l + (dirty ? non_finite<true>(a.c, s, kvh, first, s.pos + tok, lane + 32 * k) : 0.f);
+      to[lane + 32 * k] = o[q][k] / l_s[row] + (dirty ? non_finite<true>(a.c, s, kvh, first, s.pos + tok, lane + 32 * k) : 0.f);
   }
 }
 
@@ -916,7 +941,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
   if (e == cudaSuccess) e = launch_ex(plan_kernel, dim3(1), dim3(1024), 0, st, a, p.plan);
   if (e == cudaSuccess) e = launch_ex(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
-  if (e == cudaSuccess) e = launch_ex(join_kernel<DIM>, dim3(kMaxCtas, 4), dim3(256), 0, st, p, kMaxCtas);
+  if (e == cudaSuccess) e = launch_ex(join_kernel<DIM>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p, kMaxCtas);
   return e;
 }
 
