@@ -166,6 +166,20 @@ for _name, (_args, _res) in _SIGS.items():
     _f.restype = _res
 
 
+def load_ops():
+    """The extension module of csrc/py_ops.cpp (torch must be imported first).
+    Raises if it is missing."""
+    import importlib.util
+
+    path = os.path.join(_HERE, "lib", "_ops.so")
+    if not os.path.exists(path):
+        raise ImportError(f"_ops.so not built ({path}); run `python hy_mt_rs_b200/build.py`")
+    spec = importlib.util.spec_from_file_location("_ops", path)
+    module = importlib.util.module_from_spec(spec)
+    spec.loader.exec_module(module)
+    return module
+
+
 def exported_symbols():
     """Names this binding requires from the library."""
     return sorted(_SIGS)

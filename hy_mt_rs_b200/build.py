@@ -5,11 +5,14 @@
 (run it by path: importing the package loads the library it builds)
 
 Each csrc/*.cu is compiled with nvcc for sm_100a only and linked into
-hy_mt_rs_b200/lib/libhyq.so.  Objects go to hy_mt_rs_b200/_build/.
+hy_mt_rs_b200/lib/libhyq.so.  Objects go to hy_mt_rs_b200/_build/.  The Python
+extension of csrc/py_ops.cpp (torch tensors in, libhyq calls out) becomes
+hy_mt_rs_b200/lib/_ops.so next to it.
 """
 import concurrent.futures as cf
 import glob
 import os
+import shutil
 import subprocess
 import sys
 
@@ -17,6 +20,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 BUILD = os.path.join(HERE, "_build")
 LIB = os.path.join(HERE, "lib", "libhyq.so")
+OPS = os.path.join(HERE, "lib", "_ops.so")
 INCLUDE = os.path.join(os.path.dirname(HERE), "include")
 
 NVCC = os.environ.get("NVCC", "nvcc")
@@ -52,6 +56,26 @@ def _compile(src, verbose):
     return obj, res.stderr
 
 
+def _build_ops(force):
+    """The Python extension, against the installed torch and this Python."""
+    src = os.path.join(CSRC, "py_ops.cpp")
+    if not (force or _stale(OPS, [src, os.path.join(INCLUDE, "hyq.h")])):
+        return
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    cuda = os.path.dirname(os.path.dirname(shutil.which(NVCC) or "/usr/local/cuda/bin/nvcc"))
+    tmp = OPS + ".tmp"
+    subprocess.check_call([
+        "g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+        "-I" + os.path.join(root, "include"), "-I" + os.path.join(root, "include", "torch", "csrc", "api", "include"),
+        "-I" + sysconfig.get_paths()["include"], "-I" + os.path.join(cuda, "include"), "-I" + INCLUDE, src, "-o", tmp,
+        "-L" + os.path.dirname(LIB), "-l:libhyq.so", "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
+        "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
+    os.replace(tmp, OPS)
+
+
 def build(force=False, verbose=False):
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(os.path.dirname(LIB), exist_ok=True)
@@ -70,6 +94,7 @@ def build(force=False, verbose=False):
         cmd = [NVCC, *ARCH, "-shared", "-o", tmp, *objs, "-lcudart"]
         subprocess.check_call(cmd)
         os.replace(tmp, LIB)
+    _build_ops(force)
     if verbose:
         for log in logs:
             sys.stderr.write(log)

@@ -6,7 +6,6 @@
 
 #include <algorithm>
 #include <cstdint>
-#include <cstdlib>
 
 #include "../../include/hyq.h"
 #include "hyq_common.cuh"
@@ -938,8 +937,11 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
       return hyq::api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
   const hyq::sample::Args a{logits, stride, (int)n, temperature, top_k, top_p, min_p, u, token, prob};
   const cudaStream_t st = (cudaStream_t)stream;
-  static const char* tune = getenv("HYQ_TUNE_C");
-  const int want = tune ? atoi(tune) : rows >= 64 ? 1 : 8;
+  // CTAs per row: twelve while every CTA has an SM of its own (one row of
+  // 120,832 logits: 12.3 us, 12.5 with eight, 14.2 with four), six when the
+  // rows queue for SMs (256 rows, mixed parameters: 172 us, 190 with four or
+  // eight); fewer for short rows, one for those that do not fit.
+  const int want = rows * 12 <= 148 ? 12 : 6;
   int64_t ctas = std::min<int64_t>(want, (n + hyq::sample::kUnit - 1) / hyq::sample::kUnit);
   if (ctas > 1 && n > ctas * hyq::sample::kMaxSlice) ctas = 1;
   const cudaError_t e = hyq::sample::launch(a, rows, (int)ctas, st);

@@ -16,77 +16,16 @@ import struct
 
 import torch
 
-from ._native import HyqError, check, lib
+from ._native import HyqError, check, lib, load_ops
 from .quant import _need_cuda, _ptr
 
 __all__ = ["PagedCache", "rope_append", "attention", "attention_workspace"]
 
-_KV_TYPES = {torch.float32: 0, torch.float16: 1}   # HYQ_KV_F32, HYQ_KV_F16
-
-# The structures of include/hyq.h as packed bytes (a call at a decode step's
-# sizes takes a few microseconds on the device: the host side counts).
-_KV = struct.Struct("PPiiiiqqqqPqq")     # hyq_paged_kv
-_BATCH = struct.Struct("PPPqqqq")        # hyq_paged_batch
+_ops = load_ops()
+_KV_TYPES = (torch.float32, torch.float16)
 _PAGES = struct.Struct("PPPPqqqi4x")     # hyq_pages
 _POOL = struct.Struct("Pqqqq")           # hyq_page_pool
-
 _current_stream = torch._C._cuda_getCurrentRawStream
-
-
-def _check_int(t, name):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
-        _need_cuda(t, name, torch.int32)
-
-
-def _check_f32(t, name):
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32 or not t.is_contiguous():
-        _need_cuda(t, name, torch.float32)
-
-
-def _kv(k_pages, v_pages, table):
-    """hyq_paged_kv of a layer's pages; (packed, kv_heads, page_size, head_dim, table_width)."""
-    for t, name in ((k_pages, "k_pages"), (v_pages, "v_pages")):
-        if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype not in _KV_TYPES:
-            raise HyqError(-1, f"{name}: expected a CUDA float32 or float16 tensor")
-    shape, strides, dtype = k_pages.shape, k_pages.stride(), k_pages.dtype
-    if len(shape) != 4 or strides[3] != 1:
-        raise HyqError(-2, "k_pages: expected [pages, kv_heads, page_size, head_dim], contiguous in head_dim")
-    if shape != v_pages.shape or strides != v_pages.stride() or dtype != v_pages.dtype:
-        raise HyqError(-2, "k_pages and v_pages differ in shape, strides or type")
-    _check_int(table, "table")
-    rows = table.shape
-    if len(rows) != 2:
-        raise HyqError(-2, "table: expected [slots, table_width]")
-    pages, heads, page, dim = shape
-    return (_KV.pack(k_pages.data_ptr(), v_pages.data_ptr(), _KV_TYPES[dtype], heads, dim, page, pages, strides[0],
-                     strides[1], strides[2], table.data_ptr(), rows[0], rows[1]), heads, page, dim, rows[1])
-
-
-def _batch(row_start, pos, slot, tokens, max_new, max_len):
-    _check_int(row_start, "row_start")
-    _check_int(pos, "pos")
-    seqs = pos.numel()
-    if row_start.numel() != seqs + 1:
-        raise HyqError(-2, "row_start takes one more entry than pos")
-    if slot is not None:
-        _check_int(slot, "slot")
-        if slot.numel() != seqs:
-            raise HyqError(-2, "slot takes one entry per sequence")
-    if max_new < 0 or max_len < 0:
-        raise HyqError(-2, "max_new and max_len are not negative")
-    return _BATCH.pack(0 if slot is None else slot.data_ptr(), row_start.data_ptr(), pos.data_ptr(), seqs, tokens,
-                       max_new, max_len)
-
-
-def _heads(t, name):
-    """Shape and row stride of [tokens, heads, head_dim] float32 activations
-    whose heads are contiguous."""
-    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.float32:
-        raise HyqError(-1, f"{name}: expected a CUDA float32 tensor")
-    shape, strides = t.shape, t.stride()
-    if len(shape) != 3 or strides[2] != 1 or (strides[1] != shape[2] and shape[1] > 1):
-        raise HyqError(-2, f"{name}: expected [tokens, heads, head_dim] with contiguous heads")
-    return shape, (strides[0] if shape[0] > 1 else shape[1] * shape[2])
 
 
 def rope_append(q, k, v, k_pages, v_pages, table, row_start, pos, cos, sin, q_norm=None, k_norm=None, eps=1e-5,
@@ -96,31 +35,8 @@ def rope_append(q, k, v, k_pages, v_pages, table, row_start, pos, cos, sin, q_no
     write k and v into the pages, return the rotated queries (into `out` when
     given; q itself is allowed).  cos and sin are [positions, head_dim / 2]
     (hyq_rope_table); norm_first normalises before the rotation."""
-    kv, kv_heads, _, dim, _ = _kv(k_pages, v_pages, table)
-    (shape, qs), (k_shape, ks), (v_shape, vs) = _heads(q, "q"), _heads(k, "k"), _heads(v, "v")
-    if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=q.device)
-    out_shape, os = _heads(out, "out")
-    if shape[2] != dim or out_shape != shape or k_shape != (shape[0], kv_heads, dim) or v_shape != k_shape:
-        raise HyqError(-2, "rope_append: shapes of q, k, v and out")
-    _check_f32(cos, "cos")
-    _check_f32(sin, "sin")
-    rows = cos.shape
-    if len(rows) != 2 or rows != sin.shape or rows[1] * 2 != dim:
-        raise HyqError(-2, "rope_append: cos and sin are [positions, head_dim / 2]")
-    for w, name in ((q_norm, "q_norm"), (k_norm, "k_norm")):
-        if w is not None:
-            _check_f32(w, name)
-            if w.shape != (dim,):
-                raise HyqError(-2, f"rope_append: shape of {name}")
-    # (positions are checked against the table's reach on the device; max_new
-    # and max_len bound attention's work only)
-    batch = _batch(row_start, pos, slot, shape[0], 0, 0)
-    check(lib.hyq_paged_rope_append(kv, batch, q.data_ptr(), qs, shape[1], k.data_ptr(), ks, v.data_ptr(), vs,
-                                    cos.data_ptr(), sin.data_ptr(), rows[0], None if q_norm is None else q_norm.data_ptr(),
-                                    None if k_norm is None else k_norm.data_ptr(), eps, 1 if norm_first else 0,
-                                    out.data_ptr(), os, _current_stream(q.get_device())))
-    return out
+    return _ops.rope_append(q, k, v, k_pages, v_pages, table, row_start, pos, cos, sin, q_norm, k_norm, eps, norm_first,
+                            slot, out)
 
 
 @functools.lru_cache(maxsize=None)
@@ -143,24 +59,17 @@ def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None,
     when given).  max_new and max_len bound any sequence's new tokens and its
     length after them (max_len: the table's reach by default).  workspace:
     attention_workspace(...), made here when not given."""
-    kv, _, page, dim, width = _kv(k_pages, v_pages, table)
-    shape, qs = _heads(q, "q")
-    if out is None:
-        out = torch.empty(shape, dtype=torch.float32, device=q.device)
-    out_shape, os = _heads(out, "out")
-    if shape[2] != dim or out_shape != shape:
-        raise HyqError(-2, "attention: shapes of q and out")
-    batch = _batch(row_start, pos, slot, shape[0], max_new, width * page if max_len is None else max_len)
     if workspace is None:
-        workspace = attention_workspace(shape[1], dim, q.device)
-    elif not isinstance(workspace, torch.Tensor) or not workspace.is_cuda or workspace.dtype != torch.uint8 \
-            or not workspace.is_contiguous():
-        _need_cuda(workspace, "workspace", torch.uint8)
-    if workspace.numel() < _workspace_bytes(shape[1], dim):
-        raise HyqError(-2, f"attention: the workspace takes {_workspace_bytes(shape[1], dim)} bytes")
-    check(lib.hyq_paged_attention(kv, batch, q.data_ptr(), qs, shape[1], out.data_ptr(), os, workspace.data_ptr(),
-                                  _current_stream(q.get_device())))
-    return out
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
+            raise HyqError(-2, "q: expected [tokens, heads, head_dim] with contiguous heads")
+        workspace = attention_workspace(q.shape[1], q.shape[2], q.device)
+    return _ops.attention(q, k_pages, v_pages, table, row_start, pos, max_new, -1 if max_len is None else max_len, slot,
+                          out, workspace)
+
+
+def _check_int(t, name):
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
+        _need_cuda(t, name, torch.int32)
 
 
 class PagedCache:

@@ -609,3 +609,43 @@ def test_pages_share_then_diverge(cuda):
     for i, p in enumerate(tails):
         assert torch.equal(kp[p, :, 5], k[i].half())
         assert torch.equal(kp[p, :, :5], kp[tails[0], :, :5])
+
+
+def test_python_refusals(cuda):
+    """Shapes, types and layouts that the calls do not take."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant, sampling
+    from hy_mt_rs_b200._native import HyqError
+    s = _make(cuda, [1, 3], [20, 5], 8, 2, 64, 16, True)
+    args = lambda **kw: {**dict(q=s["q"], k_pages=s["k"], v_pages=s["v"], table=s["table"], row_start=s["row_start"],  # noqa: E731
+                                pos=s["pos"], max_new=3), **kw}
+    bad = [dict(q=s["q"].half()), dict(q=s["q"][:, :, :32]), dict(q=s["q"].transpose(0, 1)), dict(q=s["q"][:, :7]),
+           dict(k_pages=s["k"].float()), dict(v_pages=s["v"][:, :1]), dict(k_pages=s["k"].bfloat16(), v_pages=s["v"].bfloat16()),
+           dict(k_pages=s["k"].transpose(2, 3), v_pages=s["v"].transpose(2, 3)), dict(table=s["table"].long()),
+           dict(table=s["table"][0]), dict(row_start=s["row_start"][:2]), dict(pos=s["pos"].long()), dict(max_new=-1),
+           dict(max_len=10 ** 6), dict(max_len=1), dict(slot=s["pos"][:1]), dict(out=s["q"][:2]),
+           dict(workspace=torch.zeros(8, dtype=torch.uint8, device=cuda))]
+    for kw in bad:
+        with pytest.raises(HyqError):
+            paged.attention(**args(**kw))
+    cos = torch.zeros(64, 32, device=cuda)
+    k = torch.zeros(4, 2, 64, device=cuda)
+    for kw in (dict(k=k[:3]), dict(v=k[:, :1]), dict(cos=cos[:, :16]), dict(sin=cos[:10]), dict(q_norm=cos[0]),
+               dict(k_norm=cos[:2].reshape(64).half()), dict(out=torch.zeros(4, 8, 64, device=cuda).half())):
+        a = {**dict(q=s["q"], k=k, v=k, k_pages=s["k"], v_pages=s["v"], table=s["table"], row_start=s["row_start"],
+                    pos=s["pos"], cos=cos, sin=cos), **kw}
+        with pytest.raises(HyqError):
+            paged.rope_append(**a)
+    x, u = torch.zeros(3, 100, device=cuda), torch.zeros(3, device=cuda)
+    for a in ((x.half(), u), (x.t(), u), (x, u[:2]), (x, u, u[:1]), (x, u, None, u), (x, u, None, None, u.double()),
+              (x, None)):
+        with pytest.raises(HyqError):
+            sampling.sample(*a)
+    with pytest.raises(HyqError):
+        sampling.sample(x, u, token=u)
+    # nothing to do is not an error
+    empty = paged.attention(s["q"][:0], s["k"], s["v"], s["table"], s["row_start"][:1], s["pos"][:0], 0)
+    assert empty.shape == (0, 8, 64)
+    token, prob = sampling.sample(x[:0], u[:0])
+    assert token.numel() == 0 and prob.numel() == 0
+    assert quant.device_status() == 0

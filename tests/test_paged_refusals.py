@@ -1,6 +1,7 @@
 """Host checks of the paged-cache and sampling entry points: bad arguments are
 refused with a negative code and a reason before any GPU work."""
 import ctypes as C
+import struct
 
 import pytest
 
@@ -8,8 +9,11 @@ INVALID, SHAPE, ALIGN = -1, -2, -3
 PTR = 0x10000     # never read: every call here is refused on the host, or has nothing to do
 
 
+_KV = struct.Struct("PPiiiiqqqqPqq")     # hyq_paged_kv
+_BATCH = struct.Struct("PPPqqqq")        # hyq_paged_batch
+
+
 def _kv(**kw):
-    from hy_mt_rs_b200.paged import _KV
     d = dict(k=PTR, v=PTR, dtype=1, kv_heads=2, head_dim=128, page_size=16, pages=10, page_stride=2 * 16 * 128,
              head_stride=16 * 128, row_stride=128, table=PTR, slots=4, table_width=8)
     d.update(kw)
@@ -17,7 +21,6 @@ def _kv(**kw):
 
 
 def _batch(**kw):
-    from hy_mt_rs_b200.paged import _BATCH
     d = dict(slot=None, row_start=PTR, pos=PTR, seqs=2, tokens=3, max_new=2, max_len=100)
     d.update(kw)
     return _BATCH.pack(*(v or 0 for v in d.values()))
@@ -127,3 +130,27 @@ def test_sample_checks():
     assert call(rows=-1) == SHAPE and call(rows=1 << 31) == SHAPE
     assert call(logits=PTR + 2) == ALIGN and call(k=PTR + 1) == ALIGN
     assert call(rows=0) == 0      # nothing to do
+
+
+def test_python_entry_points_refuse():
+    """Tensors of the wrong kind raise HyqError before any call."""
+    import torch
+    from hy_mt_rs_b200 import paged, sampling
+    from hy_mt_rs_b200._native import HyqError
+
+    cpu = torch.zeros(2, 4, 128)
+    ints = torch.zeros(3, dtype=torch.int32)
+    with pytest.raises(HyqError):
+        paged.attention(cpu, cpu, cpu, ints, ints, ints, 1, workspace=ints)
+    with pytest.raises(HyqError):
+        paged.attention(None, cpu, cpu, ints, ints, ints, 1)
+    with pytest.raises(HyqError):
+        paged.rope_append(cpu, cpu, cpu, cpu, cpu, ints, ints, ints, cpu, cpu)
+    with pytest.raises(HyqError):
+        sampling.sample(cpu[0], ints)
+    with pytest.raises(HyqError):
+        sampling.sample(None, None, 0.5)
+    with pytest.raises(HyqError):
+        paged.PagedCache.over(cpu, ints, ints, ints)
+    with pytest.raises(TypeError):
+        paged._ops.sample(cpu)
