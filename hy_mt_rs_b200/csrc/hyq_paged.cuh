@@ -142,6 +142,9 @@ cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st); // t
 bool tc_supported(const AttendArgs& a, bool kv16);
 size_t tc_workspace_bytes(int dim);
 cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st);
+// hyq_paged_tc32.cu: the same over f32 caches, in the same workspace.
+bool tc32_supported(const AttendArgs& a);
+cudaError_t launch_chunks_tc32(const AttendArgs& a, cudaStream_t st);
 
 // The non-finite values of V at positions first + 1 .. last of a sequence in
 // one column: their sum (0 when there are none).  The kernels that multiply V

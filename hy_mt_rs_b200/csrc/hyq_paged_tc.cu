@@ -31,26 +31,15 @@
 #include <mutex>
 
 #include "hyq_kernels.h"
-#include "hyq_paged.cuh"
+#include "hyq_paged_tc.cuh"
 
 namespace hyq {
 namespace paged {
 namespace {
 
-constexpr int kTile = 128;               // rows of a row tile, positions of a position tile
-constexpr int kCtaRows = 2 * kTile;
+constexpr int kCtaRows = 2 * kTile;      // rows of a segment
 constexpr int kThreads = 384;
 constexpr int kSlots = 3;                // tiles of K or V in shared memory
-constexpr int kMaxCtas = 148;
-constexpr int kMaxParts = 2 * kMaxCtas;  // partial results in the workspace: a CTA's first and last piece
-constexpr int kMaxSegs = 65536;          // row tile pairs of a call
-constexpr int kMinTiles = 2;             // position tiles of a CTA, at least
-// Floats of one: outputs, then (maximum, sum) of each row, then whether a value
-// was taken out.
-__host__ __device__ constexpr size_t part_floats(int dim) { return (size_t)kCtaRows * (dim + 2) + 4; }
-constexpr float kBias = 10.0f;           // weights are kept 2^10 times their size (hyq_paged_mma.cu)
-constexpr float kSlack = 5.0f;           // a weight is at most 2^(kBias + kSlack): below f16's 65504
-constexpr float kLog2e = 1.4426950408889634f;
 
 template <int DIM>
 struct Smem {
@@ -65,283 +54,12 @@ struct Smem {
   static constexpr int total = misc + 32 + 1024;         // the base is moved to 1024 bytes
 };
 
-// The segments of one kv head, in global memory: segment t is row tile pair
-// tile[t] of sequence seq[t]; first[t] position tiles come before it.
-struct Plan {
-  int* count;   // segments, then the total of their tiles
-  int* seq;     // [kMaxSegs]
-  int* tile;    // [kMaxSegs]
-  int* first;   // [kMaxSegs + 1]
-};
-constexpr size_t kPlanBytes = (4 + 3 * (size_t)kMaxSegs + 4) * sizeof(int);
-inline Plan plan_of(void* ws) {
-  int* p = static_cast<int*>(ws);
-  return {p, p + 4, p + 4 + kMaxSegs, p + 4 + 2 * kMaxSegs};
-}
-
-struct Params {
-  AttendArgs a;
-  Plan plan;
-  int box;        // rows of a TMA box: min(page_size, 128)
-  float* parts;   // [CTA][first piece, last piece] (part_floats)
-};
-
-// Position tiles that the rows of a pair see.
-__device__ __forceinline__ int seen_tiles(const Seq& s, int group, int tile) {
-  const int last = min((tile + 1) * kCtaRows, s.n * group) - 1;
-  return (s.pos + last / group + kTile) / kTile;
-}
-
-// One CTA: the sequences' row tile pairs, then each pair's place in line.
-__global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan) {
-  grid_dependency_wait();
-  allow_dependents_launch();
-  __shared__ int off_s[kMaxSeqs + 1];
-  __shared__ int warp_s[32];
-  const int group = a.heads / a.c.kv_heads, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  auto scan = [&](int v, int& total) {
-    int x = v;
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, x, o);
-      if (lane >= o) x += y;
-    }
-    __syncthreads();
-    if (lane == 31) warp_s[warp] = x;
-    __syncthreads();
-    int w = warp_s[lane];
-#pragma unroll
-    for (int o = 1; o < 32; o <<= 1) {
-      const int y = __shfl_up_sync(0xffffffffu, w, o);
-      if (lane >= o) w += y;
-    }
-    total = __shfl_sync(0xffffffffu, w, 31);
-    const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
-    return (warp ? before : 0) + x - v;
-  };
-  int segs = 0, total;
-  for (int s0 = 0; s0 < a.c.seqs; s0 += 1024) {
-    const int i = s0 + (int)threadIdx.x;
-    int n = 0;
-    if (i < a.c.seqs) {
-      const Seq s = load_seq(a.c, i);
-      if (s.n * group > kFewRows) n = (s.n * group + kCtaRows - 1) / kCtaRows;
-    }
-    const int at = segs + scan(n, total);
-    if (i < a.c.seqs) off_s[i] = at;
-    segs += total;
-  }
-  __syncthreads();
-  segs = min(segs, kMaxSegs);
-  int tiles = 0;
-  for (int t0 = 0; t0 < segs; t0 += 1024) {
-    const int t = t0 + (int)threadIdx.x;
-    int cost = 0, seq = 0, tile = 0;
-    if (t < segs) {
-      int lo = 0, hi = a.c.seqs - 1;  // the last sequence with off <= t
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (off_s[mid] <= t) lo = mid;
-        else hi = mid - 1;
-      }
-      seq = lo;
-      tile = t - off_s[lo];
-      cost = seen_tiles(load_seq(a.c, seq), group, tile);
-    }
-    const int at = tiles + scan(cost, total);
-    if (t < segs) {
-      plan.seq[t] = seq;
-      plan.tile[t] = tile;
-      plan.first[t] = at;
-    }
-    tiles += total;
-  }
-  if (threadIdx.x == 0) {
-    plan.first[segs] = tiles;
-    plan.count[0] = segs;
-    plan.count[1] = tiles;
-  }
-}
-
-// The ranges of the line: CTA c of `ctas` takes units work c / ctas ..
-struct Line {
-  int64_t work;
-  int ctas;
-  __device__ __forceinline__ int64_t begin(int c) const { return work * c / ctas; }
-  // the CTA that takes unit u
-  __device__ __forceinline__ int cta_of(int64_t u) const {
-    int c = (int)(u * ctas / work);
-    while (begin(c + 1) <= u) ++c;
-    while (c > 0 && begin(c) > u) --c;
-    return c;
-  }
-};
-__device__ __forceinline__ Line line_of(const Params& p, int grid) {
-  const int64_t work = (int64_t)p.plan.count[1] * p.a.c.kv_heads;
-  return {work, (int)min((int64_t)grid, max(work / kMinTiles, (int64_t)1))};
-}
-// The segment that holds tile x of a kv head's line; by a whole warp.
-__device__ __forceinline__ int segment_of(const Plan& plan, int x) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = plan.count[0];
-  for (;;) {
-    const int step = (n + 31) / 32, i = lo + lane * step;
-    const int hits = __popc(__ballot_sync(0xffffffffu, i < lo + n && plan.first[i] <= x));
-    const int next = lo + max(hits - 1, 0) * step;
-    if (step <= 1) return next;
-    n = min(step, lo + n - next);
-    lo = next;
-  }
-}
-
-// What a CTA does of a segment.
-struct Piece {
-  Seq s;
-  int kvh, r0, rows, first_tok, len, j0, nt, jm;
-  int64_t seg0;
-  bool two, whole;
-};
-__device__ __forceinline__ Piece piece_of(const Params& p, int group, int t, int kvh, int64_t at, int64_t end) {
-  Piece x;
-  const Plan& plan = p.plan;
-  const int first = plan.first[t], tiles = plan.first[t + 1] - first, tile = plan.tile[t];
-  x.s = load_seq(p.a.c, plan.seq[t]);
-  x.kvh = kvh;
-  x.seg0 = (int64_t)kvh * plan.count[1] + first;
-  x.r0 = tile * kCtaRows;
-  x.rows = min(kCtaRows, x.s.n * group - x.r0);
-  x.two = x.rows > kTile;          // the second row tile has rows
-  x.first_tok = x.r0 / group;
-  x.len = x.s.pos + (x.r0 + x.rows - 1) / group + 1;  // positions the last row sees
-  x.j0 = (int)(at - x.seg0);
-  x.nt = (int)(min(end, x.seg0 + tiles) - at);
-  x.whole = x.j0 == 0 && x.nt == tiles;
-  // tiles from here on hold positions that some row does not see
-  x.jm = max(0, (x.s.pos + x.first_tok + 1) / kTile - x.j0);
-  return x;
-}
-
 __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map, int x, int row, int head, int page, uint32_t bar) {
   asm volatile(
       "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], "
       "[%6];" ::"r"(dst),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(row), "r"(head), "r"(page), "r"(bar)
       : "memory");
-}
-
-// Shared-memory operand descriptors, 128-byte swizzle, version 1.  Rows of 64
-// f16 along the inner (K) dimension: 8-row groups 1024 bytes apart.
-__device__ __forceinline__ uint64_t desc_k_major(uint32_t a) {
-  return (uint64_t)((a >> 4) & 0x3fffu) | ((uint64_t)1 << 16) | ((uint64_t)(1024 >> 4) << 32) | ((uint64_t)1 << 46) |
-         ((uint64_t)2 << 61);
-}
-// V as the right operand: rows are the inner (K) dimension, 64 columns of N
-// contiguous; the next 64 columns `half` bytes further, 8-row groups 1024.
-__device__ __forceinline__ uint64_t desc_mn_major(uint32_t a, uint32_t half) {
-  return (uint64_t)((a >> 4) & 0x3fffu) | ((uint64_t)(half >> 4) << 16) | ((uint64_t)(1024 >> 4) << 32) |
-         ((uint64_t)1 << 46) | ((uint64_t)2 << 61);
-}
-
-__device__ __forceinline__ void mma_ss(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}" ::"r"(d),
-      "l"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void mma_ts(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate) {
-  asm volatile(
-      "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}" ::"r"(d),
-      "r"(a), "l"(b), "r"(idesc), "r"(accumulate)
-      : "memory");
-}
-__device__ __forceinline__ void commit(uint32_t bar) {
-  asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-
-// 16 columns of this thread's tensor memory lane.
-__device__ __forceinline__ void tmem_ld(float (&v)[16], uint32_t a) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x16.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15}, "
-      "[%16];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15])
-      : "r"(a));
-}
-__device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t (&v)[16]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16};" ::"r"(a),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15])
-      : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tmem_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-__device__ __forceinline__ void tmem_ld(float (&v)[32], uint32_t a) {
-  asm volatile(
-      "tcgen05.ld.sync.aligned.32x32b.x32.b32 {%0, %1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31}, [%32];"
-      : "=f"(v[0]), "=f"(v[1]), "=f"(v[2]), "=f"(v[3]), "=f"(v[4]), "=f"(v[5]), "=f"(v[6]), "=f"(v[7]), "=f"(v[8]),
-        "=f"(v[9]), "=f"(v[10]), "=f"(v[11]), "=f"(v[12]), "=f"(v[13]), "=f"(v[14]), "=f"(v[15]), "=f"(v[16]),
-        "=f"(v[17]), "=f"(v[18]), "=f"(v[19]), "=f"(v[20]), "=f"(v[21]), "=f"(v[22]), "=f"(v[23]), "=f"(v[24]),
-        "=f"(v[25]), "=f"(v[26]), "=f"(v[27]), "=f"(v[28]), "=f"(v[29]), "=f"(v[30]), "=f"(v[31])
-      : "r"(a));
-}
-__device__ __forceinline__ void tmem_st(uint32_t a, const uint32_t (&v)[32]) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-      "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};" ::"r"(a),
-      "r"(v[0]), "r"(v[1]), "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7]), "r"(v[8]), "r"(v[9]),
-      "r"(v[10]), "r"(v[11]), "r"(v[12]), "r"(v[13]), "r"(v[14]), "r"(v[15]), "r"(v[16]), "r"(v[17]), "r"(v[18]),
-      "r"(v[19]), "r"(v[20]), "r"(v[21]), "r"(v[22]), "r"(v[23]), "r"(v[24]), "r"(v[25]), "r"(v[26]), "r"(v[27]),
-      "r"(v[28]), "r"(v[29]), "r"(v[30]), "r"(v[31])
-      : "memory");
-}
-// f(columns, index of the first) over N columns from `a`, 16 at a time, the next
-// load in flight while one is worked on.
-template <int N, typename F>
-__device__ __forceinline__ void tmem_each(uint32_t a, F f) {
-  float v[2][16];
-  tmem_ld(v[0], a);
-#pragma unroll
-  for (int c = 0; c < N / 16; ++c) {
-    tmem_wait_ld();
-    if (c + 1 < N / 16) tmem_ld(v[(c + 1) & 1], a + 16 * (c + 1));
-    f(v[c & 1], 16 * c);
-  }
-}
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-// Ten mantissa bits of a weight (exact in f16 from 2^-14 up).
-__device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
-
-// The same value in every lane, known to be so: descriptors and addresses made
-// of such values stay in uniform registers, and a tcgen05.mma then takes 3
-// cycles to issue instead of 46 (64 to run), so that the queue of a handful
-// stays full across the waits between products.
-__device__ __forceinline__ int uniform(int v) { return __shfl_sync(0xffffffffu, v, 0); }
-__device__ __forceinline__ bool elect() {
-  uint32_t p;
-  asm volatile("{\n\t.reg .pred q;\n\telect.sync _|q, 0xffffffff;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(p));
-  return p != 0;
-}
-
-// A wait of a whole warp: true only if every lane saw the phase complete.
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const volatile int* abort) {
-  return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort));
 }
 
 template <int DIM>
@@ -422,7 +140,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int issued = 0;
       bool ok = true;
       while (at < end && ok) {
-        const Piece x = piece_of(p, group, t, kvh, at, end);
+        const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
         for (int i = 0; i < 2 * x.nt; ++i) {  // K and V of each tile
           const int slot = issued % kSlots, pos = (x.j0 + (i >> 1)) * kTile + lane * p.box;
           int page = a.c.pages;  // past the pool: zeros
@@ -504,7 +222,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int steps[2] = {0, 0}, pieces[2] = {0, 0};
       bool ok = true;
       while (at < end && ok) {
-        const Piece x = piece_of(p, group, t, kvh, at, end);
+        const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
         const int active = uniform(x.two ? 2 : 1), nt = uniform(x.nt), jm = uniform(x.jm);
         ok = wait(full(slot), phase);
 #pragma unroll
@@ -565,7 +283,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       int i0 = 0, masked = 0, seg = 0;
       while (at < end && ok) {
-        const Piece x = piece_of(p, group, t, kvh, at, end);
+        const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
         ++seg;
         for (int i = 0; i < 2 * x.nt; ++i, ++i0) {
           const int slot = i0 % kSlots, j = i >> 1;
@@ -613,62 +331,18 @@ __global__ void __launch_bounds__(kThreads, 1)
     int steps = 0, seg = 0;
     bool ok = true;
     while (at < end && ok) {
-      const Piece x = piece_of(p, group, t, kvh, at, end);
+      const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
       const int r = x.r0 + wg * kTile + 32 * (warp & 3) + lane;  // row of the sequence
       const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + tok;
       const int64_t piece_at = at;
-      const int piece_t = t, piece_kvh = kvh;
       ++seg;
       next(x);
       if (wg == 1 && !x.two) continue;
-      // The queries, a row at a time per warp: scaled to [1, 2) by a power of
-      // two that goes back into the scores, hi and lo into shared memory.
-      float factor = 1.0f;
-      {
-        constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;  // log2(e) / sqrt(DIM)
-        constexpr int N = DIM / 32;  // values per lane
-        uint8_t* q_s = base_g + L::q + wg * 2 * L::tile;
-#pragma unroll 8
-        for (int i = 0; i < 32; ++i) {
-          const int row = 32 * (warp & 3) + i, rr = x.r0 + wg * kTile + row, tk = rr / group;
-          float v[N], top = 0.f;
-          const float* q = a.q + (int64_t)(x.s.row0 + min(tk, x.s.n - 1)) * a.q_stride +
-                           (int64_t)(x.kvh * group + rr % group) * DIM + N * lane;
-#pragma unroll
-          for (int k = 0; k < N; ++k) {
-            v[k] = tk < x.s.n ? q[k] * scale : 0.f;
-            top = fmaxf(top, fabsf(v[k]));
-          }
-#pragma unroll
-          for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-          const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-          if (lane == i) factor = __uint_as_float((uint32_t)e << 23);
-          const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-          uint32_t hi[N / 2], lo[N / 2];
-#pragma unroll
-          for (int k = 0; k < N / 2; ++k) {
-            hi[k] = pack_f16(v[2 * k] * down, v[2 * k + 1] * down);
-            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-            lo[k] = pack_f16(v[2 * k] * down - f.x, v[2 * k + 1] * down - f.y);
-          }
-          const int d = N * lane, c = d >> 3;  // 16-byte chunk of the row
-          uint8_t* to = q_s + (c >> 3) * L::half + row * 128 + (((c ^ row) & 7) << 4) + (d & 7) * 2;
-#pragma unroll
-          for (int k = 0; k < N / 2; ++k) {
-            *reinterpret_cast<uint32_t*>(to + 4 * k) = hi[k];
-            *reinterpret_cast<uint32_t*>(to + L::tile + 4 * k) = lo[k];
-          }
-        }
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(q_full(wg));
-      }
+      const float factor = stage_rows<DIM>(a, x, group, x.r0 + wg * kTile, base_g + L::q + wg * 2 * L::tile);
+      if (lane == 0) mbar_arrive(q_full(wg));
       float o[DIM];
 #pragma unroll
       for (int d = 0; d < DIM; ++d) o[d] = 0.f;
-      // Weights are 2^(s - m + kBias) with a reference m that follows the row's
-      // maximum only when that is more than kSlack past it: the maximum pass
-      // over a tile's scores is then needed for the first tile alone.
       float m = -INFINITY, l = 0.f, down = 1.f;
       // the product of the tile before, added to the row's outputs
       auto collect = [&](int step) {
@@ -685,103 +359,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         ok = (j == 0 || collect(steps - 1)) && warp_wait(s_full(wg), steps & 1, abort_flag);
         if (!ok) break;
         fence_after();
-        const bool masked = j >= x.jm;
-        const int unseen_from = sees - (x.j0 + j) * kTile + 1;
-        auto mask = [&](float (&v)[32], int c) {
-#pragma unroll
-          for (int i = 0; i < 32; ++i)
-            if (c + i >= unseen_from) v[i] = -INFINITY;
-        };
-        auto largest = [&](const float (&v)[32]) {
-          float a0 = fmaxf(v[0], v[1]), a1 = fmaxf(v[2], v[3]);
-#pragma unroll
-          for (int i = 4; i < 32; i += 4) {
-            a0 = fmaxf(fmaxf(a0, v[i]), v[i + 1]);
-            a1 = fmaxf(fmaxf(a1, v[i + 2]), v[i + 3]);
-          }
-          return fmaxf(a0, a1);
-        };
-        if (j == 0) {
-          float top = -INFINITY;
-#pragma unroll 1
-          for (int c = 0; c < kTile; c += 32) {
-            float v[32];
-            tmem_ld(v, st + c);
-            tmem_wait_ld();
-            if (masked) mask(v, c);
-            top = fmaxf(top, largest(v));
-          }
-          m = top * factor;
-        }
-        float back = kBias - (m == -INFINITY ? 0.f : m), sum = 0.f, sum2 = 0.f;
-        down = 1.f;
-        // 32 columns: scores to weights, hi and lo over them.  (Loops of 32
-        // columns, not unrolled, and two copies of them: the comparisons of a
-        // masked tile take as long as the rest, and the unrolled code ran out
-        // of the instruction cache.)
-        auto weigh = [&](float (&v)[32], int c) {
-          const float over = largest(v) * factor - m;
-          if (__any_sync(0xffffffffu, over > kSlack)) {
-            // raise the reference by whole powers of two; what this tile has
-            // so far follows
-            const float up = over > kSlack ? ceilf(over) : 0.f, f = ex2(-up);
-            m += up;
-            back -= up;
-            down *= f;
-            sum *= f;
-            sum2 *= f;
-            tmem_wait_st();
-#pragma unroll 1
-            for (int b = 0; b < c; b += 16) {
-              float w[16];
-              uint32_t u[16];
-              tmem_ld(w, st + b);
-              tmem_wait_ld();
-#pragma unroll
-              for (int i = 0; i < 8; ++i) {
-                const uint32_t hi = __float_as_uint(w[i]), lo = __float_as_uint(w[8 + i]);
-                const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-                const float2 a1 = __half22float2(*reinterpret_cast<const __half2*>(&lo));
-                const float y0 = (a0.x + a1.x) * f, y1 = (a0.y + a1.y) * f, h0 = high_part(y0), h1 = high_part(y1);
-                u[i] = pack_f16(h0, h1);
-                u[8 + i] = pack_f16(y0 - h0, y1 - h1);
-              }
-              tmem_st(st + b, u);
-            }
-          }
-          uint32_t w[32];
-#pragma unroll
-          for (int g = 0; g < 32; g += 16)
-#pragma unroll
-            for (int i = 0; i < 16; i += 2) {
-              const float y0 = ex2(fmaf(v[g + i], factor, back)), y1 = ex2(fmaf(v[g + i + 1], factor, back));
-              sum += y0;
-              sum2 += y1;
-              const float h0 = high_part(y0), h1 = high_part(y1);
-              w[g + (i >> 1)] = pack_f16(h0, h1);
-              w[g + 8 + (i >> 1)] = pack_f16(y0 - h0, y1 - h1);
-            }
-          tmem_st(st + c, w);
-        };
-        if (masked) {
-#pragma unroll 1
-          for (int c = 0; c < kTile; c += 32) {
-            float v[32];
-            tmem_ld(v, st + c);
-            tmem_wait_ld();
-            mask(v, c);
-            weigh(v, c);
-          }
-        } else {
-#pragma unroll 1
-          for (int c = 0; c < kTile; c += 32) {
-            float v[32];
-            tmem_ld(v, st + c);
-            tmem_wait_ld();
-            weigh(v, c);
-          }
-        }
-        l = fmaf(l, down, sum + sum2);
+        scores_to_weights(st, j == 0, j >= x.jm, sees - (x.j0 + j) * kTile + 1, factor, m, l, down, [](float (&)[32], int) {});
         tmem_wait_st();
         fence_before();
         __syncwarp();
@@ -794,30 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const bool dirty = misc[3 + (seg & 1)] == seg;
-      if (r >= x.s.n * group) {
-        // a row past the sequence's
-      } else if (!x.whole) {
-        float* part = p.parts + (size_t)(2 * cta + (piece_at != begin)) * part_floats(DIM);
-        float* to = part + (size_t)(r - x.r0) * DIM;
-#pragma unroll
-        for (int d = 0; d < DIM; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-        float* ml = part + (size_t)kCtaRows * DIM + 2 * (r - x.r0);
-        ml[0] = m;
-        ml[1] = l;
-        if (r == x.r0) part[(size_t)kCtaRows * (DIM + 2)] = dirty ? 1.0f : 0.0f;
-      } else {
-        float* to = a.out + (int64_t)(x.s.row0 + tok) * a.out_stride + (int64_t)(x.kvh * group + r % group) * DIM;
-        const float inv = 1.0f / l;
-        if ((reinterpret_cast<uintptr_t>(to) & 15) == 0 && !dirty) {
-#pragma unroll
-          for (int d = 0; d < DIM; d += 4)
-            *reinterpret_cast<float4*>(to + d) = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
-        } else {
-#pragma unroll
-          for (int d = 0; d < DIM; ++d)
-            to[d] = o[d] * inv + (dirty ? non_finite<true>(a.c, x.s, x.kvh, x.s.pos + x.first_tok, sees, d) : 0.f);
-        }
-      }
+      store_row<DIM, kCtaRows, true>(p, x, group, cta, piece_at != begin, r, o, m, l, dirty);
       __syncwarp();
     }
   }
@@ -826,80 +381,6 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 1) {
     fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
-  }
-}
-
-// The pieces of the segment that starts in CTA blockIdx.x's range and goes on
-// past it (there is at most one) added up, in the order of the CTAs; blockIdx.y
-// picks 32 of its rows.  The pieces' weights of all rows first, then four rows
-// of outputs per warp with their loads in flight together.
-constexpr int kJoinRows = 32;
-template <int DIM>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, int grid) {
-  const AttendArgs& a = p.a;
-  grid_dependency_wait();
-  allow_dependents_launch();
-  __shared__ float f_s[kJoinRows][kMaxCtas + 1], l_s[kJoinRows];
-  const Line line = line_of(p, grid);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.c.kv_heads, cta = blockIdx.x;
-  if (line.work == 0 || cta >= line.ctas) return;
-  const int total = p.plan.count[1];
-  const int64_t begin = line.begin(cta), end = line.begin(cta + 1);
-  const int kvh = (int)((end - 1) / total), t = segment_of(p.plan, (int)((end - 1) % total));
-  const int64_t seg0 = (int64_t)kvh * total + p.plan.first[t], seg1 = (int64_t)kvh * total + p.plan.first[t + 1];
-  if (seg0 < begin || seg1 <= end) return;
-  const int n = line.cta_of(seg1 - 1) - cta + 1;
-  const Seq s = load_seq(a.c, p.plan.seq[t]);
-  const int r0 = p.plan.tile[t] * kCtaRows, row0 = blockIdx.y * kJoinRows;
-  const int rows = min(kJoinRows, s.n * group - r0 - row0);
-  if (rows <= 0) return;
-  const float* part0 = p.parts + (size_t)(2 * cta + (seg0 != begin)) * part_floats(DIM);
-  const float* part1 = p.parts + (size_t)(2 * cta) * part_floats(DIM);
-  auto part = [&](int i) { return i ? part1 + (size_t)(2 * i) * part_floats(DIM) : part0; };
-  bool dirty = false;
-  for (int i = lane; i < n; i += 32) dirty = dirty || part(i)[(size_t)kCtaRows * (DIM + 2)] != 0.f;
-  dirty = __any_sync(0xffffffffu, dirty);
-  // a lane per row, a warp per eighth of the pieces; then their common maximum
-  for (int x = threadIdx.x; x < n * kJoinRows; x += 256) {
-    const int row = x % kJoinRows, i = x / kJoinRows;
-    f_s[row][i] = row < rows ? part(i)[(size_t)kCtaRows * DIM + 2 * (row0 + row)] : 0.f;
-  }
-  __syncthreads();
-  for (int row = warp; row < rows; row += 8) {
-    float top = -INFINITY, l = 0.f;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, f_s[row][i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    for (int i = lane; i < n; i += 32) {
-      const float m = f_s[row][i], f = m == -INFINITY ? 0.f : ex2(m - top);
-      l = fmaf(f, part(i)[(size_t)kCtaRows * DIM + 2 * (row0 + row) + 1], l);
-      f_s[row][i] = f;
-    }
-    l = warp_sum(l);
-    if (lane == 0) l_s[row] = l;
-  }
-  __syncthreads();
-  constexpr int N = DIM / 32;
-  float o[4][N] = {};
-#pragma unroll 2
-  for (int i = 0; i < n; ++i) {
-    const float* x = part(i) + (size_t)row0 * DIM + lane;
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int row = min(warp + 8 * q, rows - 1);
-      const float f = f_s[row][i];
-#pragma unroll
-      for (int k = 0; k < N; ++k) o[q][k] = fmaf(f, x[(size_t)row * DIM + 32 * k], o[q][k]);
-    }
-  }
-#pragma unroll
-  for (int q = 0; q < 4; ++q) {
-    const int row = warp + 8 * q, r = r0 + row0 + row, tok = r / group, first = s.pos + r0 / group;
-    if (row >= rows) break;
-    float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM;
-#pragma unroll
-    for (int k = 0; k < N; ++k)
-      to[lane + 32 * k] = o[q][k] / l_s[row] + (dirty ? non_finite<true>(a.c, s, kvh, first, s.pos + tok, lane + 32 * k) : 0.f);
   }
 }
 
@@ -939,9 +420,9 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   auto k = chunk_tc_kernel<DIM>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
-  if (e == cudaSuccess) e = launch_ex(plan_kernel, dim3(1), dim3(1024), 0, st, a, p.plan);
+  if (e == cudaSuccess) e = launch_ex(plan_kernel<kCtaRows>, dim3(1), dim3(1024), 0, st, a, p.plan);
   if (e == cudaSuccess) e = launch_ex(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
-  if (e == cudaSuccess) e = launch_ex(join_kernel<DIM>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p, kMaxCtas);
+  if (e == cudaSuccess) e = launch_ex(join_kernel<DIM, kCtaRows, true>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p, kMaxCtas);
   return e;
 }
 
@@ -953,7 +434,7 @@ bool tc_supported(const AttendArgs& a, bool kv16) {
   return kv16 && (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) && segs <= kMaxSegs && encode_fn() != nullptr;
 }
 
-size_t tc_workspace_bytes(int dim) { return kPlanBytes + kMaxParts * part_floats(dim) * sizeof(float); }
+size_t tc_workspace_bytes(int dim) { return kPlanBytes + kMaxParts * part_floats<kCtaRows>(dim) * sizeof(float); }
 
 cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st) {
   return a.c.dim == 128 ? launch<128>(a, st) : launch<64>(a, st);
