@@ -113,7 +113,8 @@ bool launch_overlap();
 // on: such kernels wait for their predecessor grid (griddepcontrol.wait)
 // before touching memory, and let their own dependents launch early.
 template <typename... KArgs, typename... Args>
-cudaError_t launch_ex(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+cudaError_t launch_dependent(bool overlap, void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st,
+                             Args... args) {
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[0].val.programmaticStreamSerializationAllowed = 1;
@@ -123,8 +124,20 @@ cudaError_t launch_ex(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, c
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = launch_overlap() ? 1 : 0;
+  cfg.numAttrs = overlap ? 1 : 0;
   return cudaLaunchKernelEx(&cfg, k, static_cast<KArgs>(args)...);
+}
+
+template <typename... KArgs, typename... Args>
+cudaError_t launch_ex(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+  return launch_dependent(launch_overlap(), k, grid, block, smem, st, args...);
+}
+
+// A call's second and later kernels: whatever the setting, since the kernel
+// before is the call's own.
+template <typename... KArgs, typename... Args>
+cudaError_t launch_next(void (*k)(KArgs...), dim3 grid, dim3 block, size_t smem, cudaStream_t st, Args... args) {
+  return launch_dependent(true, k, grid, block, smem, st, args...);
 }
 
 // cudaFuncAttributeMaxDynamicSharedMemorySize of a kernel, set once per device

@@ -452,11 +452,12 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
   const bool kv16 = kv->dtype == HYQ_KV_F16;
   if (hyq::paged::mma_supported(a, kv16)) {
     cudaError_t e = cudaSuccess;
-    if (batch->max_new * (heads / kv->kv_heads) > hyq::paged::kFewRows)
+    const bool more = batch->max_new * (heads / kv->kv_heads) > hyq::paged::kFewRows;
+    if (more)
       e = kv16 && hyq::paged::tc_supported(a, kv16)  ? hyq::paged::launch_chunks_tc(a, st)
           : !kv16 && hyq::paged::tc32_supported(a) ? hyq::paged::launch_chunks_tc32(a, st)
                                                    : hyq::paged::launch_chunks(a, kv16, st);
-    if (e == cudaSuccess) e = hyq::paged::launch_few(a, kv16, st);
+    if (e == cudaSuccess) e = hyq::paged::launch_few(a, kv16, more, st);
     return done(e, name);
   }
   return done(kv16 ? hyq::paged::launch_attend<true>(a, st) : hyq::paged::launch_attend<false>(a, st), name);

@@ -135,7 +135,8 @@ constexpr int kMaxSeqs = 4096;
 // hyq_paged_mma.cu: head sizes 64 and 128 over 16-byte aligned rows.
 bool mma_supported(const AttendArgs& a, bool kv16);
 size_t mma_workspace_bytes(int dim);
-cudaError_t launch_few(const AttendArgs& a, bool kv16, cudaStream_t st);    // sequences of up to kFewRows rows
+// Sequences of up to kFewRows rows; `next`: after the launch of the others.
+cudaError_t launch_few(const AttendArgs& a, bool kv16, bool next, cudaStream_t st);
 cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st); // the others
 // hyq_paged_tc.cu: the others on tcgen05 (f16 caches; the workspace past
 // mma_workspace_bytes).

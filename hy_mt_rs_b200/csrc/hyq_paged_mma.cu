@@ -845,13 +845,14 @@ cudaError_t chunks(const AttendArgs& a, cudaStream_t st) {
 }
 
 template <int DIM, bool KV16>
-cudaError_t few(const AttendArgs& a, cudaStream_t st) {
+cudaError_t few(const AttendArgs& a, bool next, cudaStream_t st) {
   using G = Geo<DIM, KV16>;
   auto k = few_kernel<DIM, KV16>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(k, G::smem + (kMaxSeqs + 1) * 4, done);
   if (e != cudaSuccess) return e;
-  return launch_ex(k, dim3(kMaxCtas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4, st, a, page_shift(a));
+  return launch_dependent(next || launch_overlap(), k, dim3(kMaxCtas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4, st,
+                          a, page_shift(a));
 }
 
 }  // namespace
@@ -864,9 +865,9 @@ bool mma_supported(const AttendArgs& a, bool kv16) {
 
 size_t mma_workspace_bytes(int dim) { return kCounterBytes + 2 * (size_t)kMaxCtas * partial_floats(dim) * sizeof(float); }
 
-cudaError_t launch_few(const AttendArgs& a, bool kv16, cudaStream_t st) {
-  if (a.c.dim == 128) return kv16 ? few<128, true>(a, st) : few<128, false>(a, st);
-  return kv16 ? few<64, true>(a, st) : few<64, false>(a, st);
+cudaError_t launch_few(const AttendArgs& a, bool kv16, bool next, cudaStream_t st) {
+  if (a.c.dim == 128) return kv16 ? few<128, true>(a, next, st) : few<128, false>(a, next, st);
+  return kv16 ? few<64, true>(a, next, st) : few<64, false>(a, next, st);
 }
 
 cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st) {

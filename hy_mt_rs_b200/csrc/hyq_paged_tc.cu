@@ -50,7 +50,7 @@ struct Smem {
   static constexpr int bars = ring + kSlots * tile;
   // full[3], empty[3], s_full[2], p_full[2], x_full[2], q_full[2], clean[2]
   static constexpr int n_bars = 2 * kSlots + 10;
-  static constexpr int misc = bars + 8 * n_bars;         // tensor memory address, abort, first segment, dirty[2]
+  static constexpr int misc = bars + 8 * n_bars;         // tensor memory address, abort, unused, dirty[2]
   static constexpr int total = misc + 32 + 1024;         // the base is moved to 1024 bytes
 };
 
@@ -88,15 +88,13 @@ __global__ void __launch_bounds__(kThreads, 1)
 
   grid_dependency_wait();
   allow_dependents_launch();
-  const Line line = line_of(p, gridDim.x);
-  const int cta = blockIdx.x, total = p.plan.count[1];
-  if (line.work == 0 || cta >= line.ctas) return;  // nothing allocated yet
-  const int64_t begin = line.begin(cta), end = line.begin(cta + 1);
+  const int cta = blockIdx.x;
+  const Start start = p.plan.start[cta];
+  const int64_t begin = start.begin, end = p.plan.start[cta + 1].begin;
+  if (begin == end) return;  // nothing allocated yet
   if (warp == 0) {
-    const int t = segment_of(p.plan, (int)(begin % total));
     if (lane == 0) {
       misc[1] = 0;
-      misc[2] = t;
       misc[3] = misc[4] = 0;
       for (int s = 0; s < kSlots; ++s) {
         mbar_init(full(s), 1);
@@ -121,7 +119,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   fence_after();
   const uint32_t tmem = (uint32_t)uniform(misc[0]);
   // every warp walks the same pieces: (segment, kv head), at its tile `at`
-  int t = misc[2], kvh = (int)(begin / total);
+  int t = start.t, kvh = start.kvh;
   int64_t at = begin;
   auto next = [&](const Piece& x) {
     at += x.nt;
@@ -372,8 +370,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const bool dirty = misc[3 + (seg & 1)] == seg;
-      store_row<DIM, kCtaRows, true>(p, x, group, cta, piece_at != begin, r, o, m, l, dirty);
-      __syncwarp();
+      store_rows<DIM, kCtaRows, true>(p, x, group, cta, piece_at != begin, r, base_g + L::q + wg * 2 * L::tile, o, m, l, dirty);
     }
   }
   fence_before();
@@ -421,8 +418,8 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
   if (e == cudaSuccess) e = launch_ex(plan_kernel<kCtaRows>, dim3(1), dim3(1024), 0, st, a, p.plan);
-  if (e == cudaSuccess) e = launch_ex(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
-  if (e == cudaSuccess) e = launch_ex(join_kernel<DIM, kCtaRows, true>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p, kMaxCtas);
+  if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
+  if (e == cudaSuccess) e = launch_next(join_kernel<DIM, kCtaRows, true>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p);
   return e;
 }
 

@@ -16,7 +16,8 @@ constexpr int kTile = 128;               // rows of a row tile, positions of a p
 constexpr int kMaxCtas = 148;
 constexpr int kMaxParts = 2 * kMaxCtas;  // partial results in the workspace: a CTA's first and last piece
 constexpr int kMaxSegs = 65536;          // segments of a call
-constexpr int kMinTiles = 2;             // position tiles of a CTA, at least
+constexpr int kMinTiles = 2;             // cost of a CTA's range, at least
+constexpr int kSegTiles = 1;             // cost of a segment, in tiles
 // Floats of a partial result of a segment of ROWS rows: outputs, then
 // (maximum, sum) of each row, then whether a value was taken out.
 template <int ROWS>
@@ -27,18 +28,29 @@ constexpr float kBias = 10.0f;           // weights are kept 2^10 times their si
 constexpr float kSlack = 5.0f;           // a weight is at most 2^(kBias + kSlack): below f16's 65504
 constexpr float kLog2e = 1.4426950408889634f;
 
-// The segments of one kv head, in global memory: segment t is the
-// tile[t]-th of sequence seq[t]; first[t] position tiles come before it.
-struct Plan {
-  int* count;   // segments, then the total of their tiles
-  int* seq;     // [kMaxSegs]
-  int* tile;    // [kMaxSegs]
-  int* first;   // [kMaxSegs + 1]
+// A segment: its sequence (n rows of tokens from row0 at pos, pages in `slot`),
+// which of the sequence's it is, and the position tiles that come before and
+// up to its end among one kv head's.
+struct alignas(16) Segment {
+  int row0, n, pos, slot;
+  int tile, first, end, unused;
 };
-constexpr size_t kPlanBytes = (4 + 3 * (size_t)kMaxSegs + 4) * sizeof(int);
+// Where a CTA's range begins: position tile `begin` of all kv heads', in
+// segment t of kv head kvh.
+struct alignas(16) Start {
+  int64_t begin;
+  int t, kvh;
+};
+struct Plan {
+  int* count;      // segments, then the total of their tiles
+  Start* start;    // [kMaxCtas + 1]
+  Segment* seg;    // [kMaxSegs]
+};
+constexpr size_t kPlanBytes = 16 + (kMaxCtas + 1) * sizeof(Start) + (size_t)kMaxSegs * sizeof(Segment);
 inline Plan plan_of(void* ws) {
-  int* p = static_cast<int*>(ws);
-  return {p, p + 4, p + 4 + kMaxSegs, p + 4 + 2 * kMaxSegs};
+  char* p = static_cast<char*>(ws);
+  return {reinterpret_cast<int*>(p), reinterpret_cast<Start*>(p + 16),
+          reinterpret_cast<Segment*>(p + 16 + (kMaxCtas + 1) * sizeof(Start))};
 }
 
 struct Params {
@@ -55,7 +67,9 @@ __device__ __forceinline__ int seen_tiles(const Seq& s, int group, int tile) {
   return (s.pos + last / group + kTile) / kTile;
 }
 
-// One CTA: the sequences' segments, then each one's place in line.
+// One CTA: the sequences' segments, each one's place in line, and the CTAs'
+// ranges of it.  The line is cut by equal cost, kSegTiles more than its tiles
+// for each segment (its queries in, its results out, a start of the pipeline).
 template <int ROWS>
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan) {
   grid_dependency_wait();
@@ -101,6 +115,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
   for (int t0 = 0; t0 < segs; t0 += 1024) {
     const int t = t0 + (int)threadIdx.x;
     int cost = 0, seq = 0, tile = 0;
+    Seq s{};
     if (t < segs) {
       int lo = 0, hi = a.c.seqs - 1;  // the last sequence with off <= t
       while (lo < hi) {
@@ -110,51 +125,32 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
       }
       seq = lo;
       tile = t - off_s[lo];
-      cost = seen_tiles<ROWS>(load_seq(a.c, seq), group, tile);
+      s = load_seq(a.c, seq);
+      cost = seen_tiles<ROWS>(s, group, tile);
     }
     const int at = tiles + scan(cost, total);
-    if (t < segs) {
-      plan.seq[t] = seq;
-      plan.tile[t] = tile;
-      plan.first[t] = at;
-    }
+    if (t < segs) plan.seg[t] = {s.row0, s.n, s.pos, a.c.slot ? a.c.slot[seq] : seq, tile, at, at + cost, 0};
     tiles += total;
   }
+  __syncthreads();
+  if (threadIdx.x <= kMaxCtas) {
+    const int64_t per = tiles + (int64_t)kSegTiles * segs, work = per * a.c.kv_heads;
+    const int64_t ctas = min((int64_t)kMaxCtas, max(work / kMinTiles, (int64_t)1));
+    const int64_t unit = work * min((int64_t)threadIdx.x, ctas) / ctas;
+    const int kvh = per ? (int)(unit / per) : 0;
+    const int64_t rest = unit - kvh * per;
+    int lo = 0, hi = segs - 1;  // the last segment that begins at `rest` or before
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (plan.seg[mid].first + (int64_t)kSegTiles * mid <= rest) lo = mid;
+      else hi = mid - 1;
+    }
+    const int first = segs ? plan.seg[lo].first : 0;
+    plan.start[threadIdx.x] = {(int64_t)kvh * tiles + first + max(rest - first - (int64_t)kSegTiles * (lo + 1), (int64_t)0), lo, kvh};
+  }
   if (threadIdx.x == 0) {
-    plan.first[segs] = tiles;
     plan.count[0] = segs;
     plan.count[1] = tiles;
-  }
-}
-
-// The ranges of the line: CTA c of `ctas` takes units work c / ctas ..
-struct Line {
-  int64_t work;
-  int ctas;
-  __device__ __forceinline__ int64_t begin(int c) const { return work * c / ctas; }
-  // the CTA that takes unit u
-  __device__ __forceinline__ int cta_of(int64_t u) const {
-    int c = (int)(u * ctas / work);
-    while (begin(c + 1) <= u) ++c;
-    while (c > 0 && begin(c) > u) --c;
-    return c;
-  }
-};
-__device__ __forceinline__ Line line_of(const Params& p, int grid) {
-  const int64_t work = (int64_t)p.plan.count[1] * p.a.c.kv_heads;
-  return {work, (int)min((int64_t)grid, max(work / kMinTiles, (int64_t)1))};
-}
-// The segment that holds tile x of a kv head's line; by a whole warp.
-__device__ __forceinline__ int segment_of(const Plan& plan, int x) {
-  const int lane = threadIdx.x & 31;
-  int lo = 0, n = plan.count[0];
-  for (;;) {
-    const int step = (n + 31) / 32, i = lo + lane * step;
-    const int hits = __popc(__ballot_sync(0xffffffffu, i < lo + n && plan.first[i] <= x));
-    const int next = lo + max(hits - 1, 0) * step;
-    if (step <= 1) return next;
-    n = min(step, lo + n - next);
-    lo = next;
   }
 }
 
@@ -169,8 +165,10 @@ template <int ROWS>
 __device__ __forceinline__ Piece piece_of(const Params& p, int group, int t, int kvh, int64_t at, int64_t end) {
   Piece x;
   const Plan& plan = p.plan;
-  const int first = plan.first[t], tiles = plan.first[t + 1] - first, tile = plan.tile[t];
-  x.s = load_seq(p.a.c, plan.seq[t]);
+  const int4* seg = reinterpret_cast<const int4*>(plan.seg + t);
+  const int4 s = seg[0], place = seg[1];
+  const int tile = place.x, first = place.y, tiles = place.z - place.y;
+  x.s = {s.x, s.y, s.z, p.a.c.table + (int64_t)s.w * p.a.c.width};
   x.kvh = kvh;
   x.seg0 = (int64_t)kvh * plan.count[1] + first;
   x.r0 = tile * ROWS;
@@ -303,44 +301,71 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, const v
 
 // A row tile's queries, 32 rows by each of four warps: rows r0 .. of the
 // segment's (token, head) rows, scaled to [1, 2) by a power of two that goes
-// back into the scores (the result, for the thread's own row), hi and lo as
-// right-hand tiles at q_s.
+// back into the scores (the result, for the thread's own row), hi and lo to
+// q_s.  The rows come as they are, all in flight together, to the places that
+// their own halves then take.
 template <int DIM>
 __device__ __forceinline__ float stage_rows(const AttendArgs& a, const Piece& x, int group, int r0, uint8_t* q_s) {
   constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;  // log2(e) / sqrt(DIM)
-  constexpr int N = DIM / 32;  // values per lane
+  constexpr int N = DIM / 32, kLanes = DIM / 4;  // values per lane; lanes per row of 16-byte pieces
   constexpr int half = kTile * 128, tile = half * (DIM / 64);
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int lane = threadIdx.x & 31, row0 = threadIdx.x & 96;
+  const int rr = r0 + row0 + lane, tk = rr / group;
+  const int64_t mine =
+      tk < x.s.n ? (int64_t)(x.s.row0 + tk) * a.q_stride + (int64_t)(x.kvh * group + rr - tk * group) * DIM : -1;
+  const bool vec = ((reinterpret_cast<uintptr_t>(a.q) | (uintptr_t)a.q_stride * 4) & 15) == 0;
+  q_s += row0 * 128;
+  const int c = lane % kLanes;
+#pragma unroll 4
+  for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
+    const int64_t off = __shfl_sync(0xffffffffu, mine, i);
+    const float* from = a.q + max(off, (int64_t)0) + 4 * c;
+    const uint32_t to = smem_addr(q_s) + i * 128 + (c >> 3) * half + (((c ^ i) & 7) << 4), n = off >= 0 ? 4 : 0;
+    if (vec) {
+      asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(4 * n) : "memory");
+    } else {
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4 * k), "l"(from + k), "r"(n) : "memory");
+    }
+  }
+  asm volatile("cp.async.wait_all;" ::: "memory");
+  __syncwarp();
   float factor = 1.0f;
-#pragma unroll 8
-  for (int i = 0; i < 32; ++i) {
-    const int row = 32 * (warp & 3) + i, rr = r0 + row, tk = rr / group;
-    float v[N], top = 0.f;
-    const float* q = a.q + (int64_t)(x.s.row0 + min(tk, x.s.n - 1)) * a.q_stride +
-                     (int64_t)(x.kvh * group + rr % group) * DIM + N * lane;
+  const int d = N * lane;
+#pragma unroll 1
+  for (int i0 = 0; i0 < 32; i0 += 4) {
+    float v[4][N];
 #pragma unroll
-    for (int k = 0; k < N; ++k) {
-      v[k] = tk < x.s.n ? q[k] * scale : 0.f;
-      top = fmaxf(top, fabsf(v[k]));
+    for (int i = 0; i < 4; ++i) {
+      const uint8_t* from = q_s + (i0 + i) * 128 + (d >> 5) * half + ((((d >> 2) ^ (i0 + i)) & 7) << 4) + (d & 3) * 4;
+#pragma unroll
+      for (int k = 0; k < N; ++k) v[i][k] = reinterpret_cast<const float*>(from)[k] * scale;
     }
+    __syncwarp();
 #pragma unroll
-    for (int w = 16; w > 0; w >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, w));
-    const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
-    if (lane == i) factor = __uint_as_float((uint32_t)e << 23);
-    const float down = __uint_as_float((uint32_t)(254 - e) << 23);
-    uint32_t hi[N / 2], lo[N / 2];
+    for (int i = 0; i < 4; ++i) {
+      uint32_t bits = 0;
 #pragma unroll
-    for (int k = 0; k < N / 2; ++k) {
-      hi[k] = pack_f16(v[2 * k] * down, v[2 * k + 1] * down);
-      const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
-      lo[k] = pack_f16(v[2 * k] * down - f.x, v[2 * k + 1] * down - f.y);
-    }
-    const int d = N * lane, c = d >> 3;  // 16-byte chunk of the row
-    uint8_t* to = q_s + (c >> 3) * half + row * 128 + (((c ^ row) & 7) << 4) + (d & 7) * 2;
+      for (int k = 0; k < N; ++k) bits = max(bits, __float_as_uint(v[i][k]) & 0x7fffffffu);
+      const int e = min(max((int)(__reduce_max_sync(0xffffffffu, bits) >> 23), 1), 253);
+      if (lane == i0 + i) factor = __uint_as_float((uint32_t)e << 23);
+      const float down = __uint_as_float((uint32_t)(254 - e) << 23);
+      uint32_t hi[N / 2], lo[N / 2];
 #pragma unroll
-    for (int k = 0; k < N / 2; ++k) {
-      *reinterpret_cast<uint32_t*>(to + 4 * k) = hi[k];
-      *reinterpret_cast<uint32_t*>(to + tile + 4 * k) = lo[k];
+      for (int k = 0; k < N / 2; ++k) {
+        hi[k] = pack_f16(v[i][2 * k] * down, v[i][2 * k + 1] * down);
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi[k]));
+        lo[k] = pack_f16(v[i][2 * k] * down - f.x, v[i][2 * k + 1] * down - f.y);
+      }
+      uint8_t* to = q_s + (i0 + i) * 128 + (d >> 6) * half + ((((d >> 3) ^ (i0 + i)) & 7) << 4) + (d & 7) * 2;
+      if constexpr (N == 4) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(hi[0], hi[1]);
+        *reinterpret_cast<uint2*>(to + tile) = make_uint2(lo[0], lo[1]);
+      } else {
+        *reinterpret_cast<uint32_t*>(to) = hi[0];
+        *reinterpret_cast<uint32_t*>(to + tile) = lo[0];
+      }
     }
   }
   fence_proxy_async_smem();
@@ -458,59 +483,87 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
   l = fmaf(l, down, sum + sum2);
 }
 
-// A row's result of a piece: its output, or a partial result.
+// The results of a warp's 32 rows of a piece, row r this thread's: outputs, or
+// a partial result.  They go through the rows' own places in q_s, whose
+// queries no product reads any more, so that rows are written whole.
 template <int DIM, int ROWS, bool KV16>
-__device__ __forceinline__ void store_row(const Params& p, const Piece& x, int group, int cta, bool second, int r,
-                                          const float (&o)[DIM], float m, float l, bool dirty) {
+__device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int group, int cta, bool second, int r,
+                                           uint8_t* q_s, const float (&o)[DIM], float m, float l, bool dirty) {
+  constexpr int half = kTile * 128, kLanes = DIM / 4;  // lanes of a row
   const AttendArgs& a = p.a;
-  if (r >= x.s.n * group) return;  // a row past the sequence's
-  const int tok = r / group;
-  if (!x.whole) {
-    float* part = p.parts + (size_t)(2 * cta + second) * part_floats<ROWS>(DIM);
-    float* to = part + (size_t)(r - x.r0) * DIM;
-#pragma unroll
-    for (int d = 0; d < DIM; d += 4) *reinterpret_cast<float4*>(to + d) = make_float4(o[d], o[d + 1], o[d + 2], o[d + 3]);
-    float* ml = part + (size_t)ROWS * DIM + 2 * (r - x.r0);
-    ml[0] = m;
-    ml[1] = l;
+  const int lane = threadIdx.x & 31, row0 = threadIdx.x & 96, tok = r / group;
+  const bool in = r < x.s.n * group;
+  float* part = p.parts + (size_t)(2 * cta + second) * part_floats<ROWS>(DIM);
+  int64_t mine = -1;
+  if (in && x.whole) {
+    mine = (int64_t)(x.s.row0 + tok) * a.out_stride + (int64_t)(x.kvh * group + r - tok * group) * DIM;
+  } else if (in) {
+    mine = (int64_t)(r - x.r0) * DIM;
+    *reinterpret_cast<float2*>(part + (size_t)ROWS * DIM + 2 * (r - x.r0)) = make_float2(m, l);
     if (KV16 && r == x.r0) part[(size_t)ROWS * (DIM + 2)] = dirty ? 1.0f : 0.0f;
-    return;
   }
-  float* to = a.out + (int64_t)(x.s.row0 + tok) * a.out_stride + (int64_t)(x.kvh * group + r % group) * DIM;
-  const float inv = 1.0f / l;
-  if ((reinterpret_cast<uintptr_t>(to) & 15) == 0 && !dirty) {
+  const float inv = x.whole ? 1.0f / l : 1.0f;
+  uint8_t* row = q_s + (row0 + lane) * 128;
 #pragma unroll
-    for (int d = 0; d < DIM; d += 4)
-      *reinterpret_cast<float4*>(to + d) = make_float4(o[d] * inv, o[d + 1] * inv, o[d + 2] * inv, o[d + 3] * inv);
-  } else {
-#pragma unroll
-    for (int d = 0; d < DIM; ++d)
-      to[d] = o[d] * inv + (dirty ? non_finite<KV16>(a.c, x.s, x.kvh, x.s.pos + x.first_tok, x.s.pos + tok, d) : 0.f);
+  for (int c = 0; c < DIM / 4; ++c)
+    *reinterpret_cast<float4*>(row + (c >> 3) * half + (((c ^ lane) & 7) << 4)) =
+        make_float4(o[4 * c] * inv, o[4 * c + 1] * inv, o[4 * c + 2] * inv, o[4 * c + 3] * inv);
+  __syncwarp();
+  float* to = x.whole ? a.out : part;
+  const bool vec = !x.whole || ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)a.out_stride * 4) & 15) == 0;
+  dirty = dirty && x.whole;
+  const int c = lane % kLanes;
+#pragma unroll 4
+  for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
+    const int64_t off = __shfl_sync(0xffffffffu, mine, i);
+    const int tk = __shfl_sync(0xffffffffu, tok, i);
+    float4 f = *reinterpret_cast<const float4*>(q_s + (row0 + i) * 128 + (c >> 3) * half + (((c ^ i) & 7) << 4));
+    if (off < 0) continue;
+    if (KV16 && dirty) {
+      auto more = [&](int k) { return non_finite<KV16>(a.c, x.s, x.kvh, x.s.pos + x.first_tok, x.s.pos + tk, 4 * c + k); };
+      f.x += more(0), f.y += more(1), f.z += more(2), f.w += more(3);
+    }
+    float* y = to + off + 4 * c;
+    if (vec) {
+      *reinterpret_cast<float4*>(y) = f;
+    } else {
+      y[0] = f.x, y[1] = f.y, y[2] = f.z, y[3] = f.w;
+    }
   }
+  __syncwarp();
 }
 
 // The pieces of the segment that starts in CTA blockIdx.x's range and goes on
 // past it (there is at most one) added up, in the order of the CTAs; blockIdx.y
-// picks 32 of its rows.  The pieces' weights of all rows first, then four rows
-// of outputs per warp with their loads in flight together.
+// picks 32 of its rows.  The pieces' factors of all rows first, then four rows
+// of outputs per warp with the loads of four pieces in flight together.
 constexpr int kJoinRows = 32;
 template <int DIM, int ROWS, bool KV16>
-__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p, int grid) {
+__global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p) {
   const AttendArgs& a = p.a;
   grid_dependency_wait();
   allow_dependents_launch();
-  __shared__ float f_s[kJoinRows][kMaxCtas + 1], l_s[kJoinRows];
-  const Line line = line_of(p, grid);
+  __shared__ float2 ml_s[kMaxCtas][kJoinRows];  // maximum (then factor) and sum
+  __shared__ float l_s[kJoinRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, group = a.heads / a.c.kv_heads, cta = blockIdx.x;
-  if (line.work == 0 || cta >= line.ctas) return;
+  const int64_t begin = p.plan.start[cta].begin, end = p.plan.start[cta + 1].begin;
+  if (begin == end) return;
+  // the segment of tile end - 1: the one before the next range's, if that
+  // range begins with one
   const int total = p.plan.count[1];
-  const int64_t begin = line.begin(cta), end = line.begin(cta + 1);
-  const int kvh = (int)((end - 1) / total), t = segment_of(p.plan, (int)((end - 1) % total));
-  const int64_t seg0 = (int64_t)kvh * total + p.plan.first[t], seg1 = (int64_t)kvh * total + p.plan.first[t + 1];
-  if (seg0 < begin || seg1 <= end) return;
-  const int n = line.cta_of(seg1 - 1) - cta + 1;
-  const Seq s = load_seq(a.c, p.plan.seq[t]);
-  const int r0 = p.plan.tile[t] * ROWS, row0 = blockIdx.y * kJoinRows;
+  int t = p.plan.start[cta + 1].t, kvh = p.plan.start[cta + 1].kvh;
+  if ((int64_t)kvh * total + p.plan.seg[t].first == end) return;  // it ends with this range
+  const int64_t seg0 = (int64_t)kvh * total + p.plan.seg[t].first, seg1 = (int64_t)kvh * total + p.plan.seg[t].end;
+  if (seg0 < begin) return;
+  int n = 1;  // and the ranges that begin inside it
+  for (int c = cta + 1; c < kMaxCtas; c += 32) {
+    const int hits = __popc(__ballot_sync(0xffffffffu, c + lane < kMaxCtas && p.plan.start[c + lane].begin < seg1));
+    n += hits;
+    if (hits < 32) break;
+  }
+  const int4 seq = *reinterpret_cast<const int4*>(p.plan.seg + t);
+  const Seq s{seq.x, seq.y, seq.z, a.c.table + (int64_t)seq.w * a.c.width};
+  const int r0 = p.plan.seg[t].tile * ROWS, row0 = blockIdx.y * kJoinRows;
   const int rows = min(kJoinRows, s.n * group - r0 - row0);
   if (rows <= 0) return;
   const float* part0 = p.parts + (size_t)(2 * cta + (seg0 != begin)) * part_floats<ROWS>(DIM);
@@ -518,48 +571,55 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
   auto part = [&](int i) { return i ? part1 + (size_t)(2 * i) * part_floats<ROWS>(DIM) : part0; };
   bool dirty = false;
   for (int i = lane; KV16 && i < n; i += 32) dirty = dirty || part(i)[(size_t)ROWS * (DIM + 2)] != 0.f;
-  dirty = __any_sync(0xffffffffu, dirty);
-  // a lane per row, a warp per eighth of the pieces; then their common maximum
   for (int x = threadIdx.x; x < n * kJoinRows; x += 256) {
     const int row = x % kJoinRows, i = x / kJoinRows;
-    f_s[row][i] = row < rows ? part(i)[(size_t)ROWS * DIM + 2 * (row0 + row)] : 0.f;
+    ml_s[i][row] = row < rows ? reinterpret_cast<const float2*>(part(i) + (size_t)ROWS * DIM)[row0 + row] : make_float2(0.f, 1.f);
   }
+  dirty = __any_sync(0xffffffffu, dirty);
   __syncthreads();
-  for (int row = warp; row < rows; row += 8) {
+  // a thread per row: the pieces' factors
+  if (threadIdx.x < kJoinRows) {
+    const int row = threadIdx.x;
     float top = -INFINITY, l = 0.f;
-    for (int i = lane; i < n; i += 32) top = fmaxf(top, f_s[row][i]);
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    for (int i = lane; i < n; i += 32) {
-      const float m = f_s[row][i], f = m == -INFINITY ? 0.f : ex2(m - top);
-      l = fmaf(f, part(i)[(size_t)ROWS * DIM + 2 * (row0 + row) + 1], l);
-      f_s[row][i] = f;
+    for (int i = 0; i < n; ++i) top = fmaxf(top, ml_s[i][row].x);
+    for (int i = 0; i < n; ++i) {
+      const float2 v = ml_s[i][row];
+      const float f = v.x == -INFINITY ? 0.f : ex2(v.x - top);
+      l = fmaf(f, v.y, l);
+      ml_s[i][row].x = f;
     }
-    l = warp_sum(l);
-    if (lane == 0) l_s[row] = l;
+    l_s[row] = l;
   }
   __syncthreads();
-  constexpr int N = DIM / 32;
+  constexpr int N = DIM / 32;  // neighbouring values per lane, rows warp, warp + 8 ..
   float o[4][N] = {};
-#pragma unroll 2
+#pragma unroll 4
   for (int i = 0; i < n; ++i) {
-    const float* x = part(i) + (size_t)row0 * DIM + lane;
+    const float* x = part(i) + (size_t)row0 * DIM + N * lane;
 #pragma unroll
     for (int q = 0; q < 4; ++q) {
       const int row = min(warp + 8 * q, rows - 1);
-      const float f = f_s[row][i];
+      const float f = ml_s[i][row].x;
+      float v[N];
+      if constexpr (N == 4) {
+        const float4 y = *reinterpret_cast<const float4*>(x + (size_t)row * DIM);
+        v[0] = y.x, v[1] = y.y, v[2] = y.z, v[3] = y.w;
+      } else {
+        const float2 y = *reinterpret_cast<const float2*>(x + (size_t)row * DIM);
+        v[0] = y.x, v[1] = y.y;
+      }
 #pragma unroll
-      for (int k = 0; k < N; ++k) o[q][k] = fmaf(f, x[(size_t)row * DIM + 32 * k], o[q][k]);
+      for (int k = 0; k < N; ++k) o[q][k] = fmaf(f, v[k], o[q][k]);
     }
   }
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int row = warp + 8 * q, r = r0 + row0 + row, tok = r / group, first = s.pos + r0 / group;
     if (row >= rows) break;
-    float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM;
+    float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM + N * lane;
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      to[lane + 32 * k] = o[q][k] / l_s[row] + (dirty ? non_finite<KV16>(a.c, s, kvh, first, s.pos + tok, lane + 32 * k) : 0.f);
+      to[k] = o[q][k] / l_s[row] + (dirty ? non_finite<KV16>(a.c, s, kvh, first, s.pos + tok, N * lane + k) : 0.f);
   }
 }
 

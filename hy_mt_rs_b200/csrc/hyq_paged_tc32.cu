@@ -46,7 +46,7 @@ struct Smem {
   static constexpr int bars = top + 2 * kSplitWarps * 8;
   // k_full, v_full, v_top, p_full, x_full, s_full[2]
   static constexpr int n_bars = 7;
-  // tensor memory address, abort, first segment, then [2] of: tile that is left
+  // tensor memory address, abort, unused, then [2] of: tile that is left
   // out (its number + 1), scale of X
   static constexpr int misc = bars + 8 * n_bars;
   static constexpr int total = misc + 32 + 1024;         // the base is moved to 1024 bytes
@@ -114,16 +114,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
 
   grid_dependency_wait();
   allow_dependents_launch();
-  const Line line = line_of(p, gridDim.x);
-  const int cta = blockIdx.x, total = p.plan.count[1];
-  if (line.work == 0 || cta >= line.ctas) return;  // nothing allocated yet
-  const int64_t begin = line.begin(cta), end = line.begin(cta + 1);
+  const int cta = blockIdx.x;
+  const Start start = p.plan.start[cta];
+  const int64_t begin = start.begin, end = p.plan.start[cta + 1].begin;
+  if (begin == end) return;  // nothing allocated yet
   const int tiles = uniform((int)(end - begin));
   if (warp == 0) {
-    const int t = segment_of(p.plan, (int)(begin % total));
     if (lane == 0) {
       misc[1] = 0;
-      misc[2] = t;
       misc[3] = misc[4] = 0;
       mbar_init(k_full, kSplitWarps + 4);  // K is there, and the queries: the softmax warps
       mbar_init(v_full, kSplitWarps);
@@ -143,7 +141,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
   __syncthreads();
   fence_after();
   const uint32_t tmem = (uint32_t)uniform(misc[0]);
-  int t = misc[2], kvh = (int)(begin / total);
+  int t = start.t, kvh = start.kvh;
   int64_t at = begin;
   auto next = [&](const Piece& x) {
     at += x.nt;
@@ -408,8 +406,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       }
       if (ok) collect();
       if (!ok) break;
-      store_row<DIM, kRows, false>(p, x, group, cta, second, r, o, m, l, false);
-      __syncwarp();
+      store_rows<DIM, kRows, false>(p, x, group, cta, second, r, base_g + L::q, o, m, l, false);
     }
   }
   if (!ok) {
@@ -436,9 +433,9 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
   if (e == cudaSuccess) e = launch_ex(plan_kernel<kRows>, dim3(1), dim3(1024), 0, st, a, p.plan);
-  if (e == cudaSuccess) e = launch_ex(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
+  if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
   if (e == cudaSuccess)
-    e = launch_ex(join_kernel<DIM, kRows, false>, dim3(kMaxCtas, kRows / kJoinRows), dim3(256), 0, st, p, kMaxCtas);
+    e = launch_next(join_kernel<DIM, kRows, false>, dim3(kMaxCtas, kRows / kJoinRows), dim3(256), 0, st, p);
   return e;
 }
 

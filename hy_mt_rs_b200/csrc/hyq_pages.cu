@@ -335,7 +335,7 @@ int done(cudaError_t e, const char* name) {
 
 cudaError_t launch_copy(const hyq::pages::Table& t, const hyq::pages::Pool& pool, const hyq::pages::Plan& w, bool rename,
                         cudaStream_t st) {
-  return hyq::launch_ex(hyq::pages::copy_kernel, dim3(148 * 8), dim3(256), 0, st, t, pool, w, rename);
+  return hyq::launch_next(hyq::pages::copy_kernel, dim3(148 * 8), dim3(256), 0, st, t, pool, w, rename);
 }
 
 }  // namespace
