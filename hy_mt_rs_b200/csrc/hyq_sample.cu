@@ -17,7 +17,6 @@ namespace sample {
 using u64 = unsigned long long;
 
 constexpr int kGrid = 24;              // u and top_p in steps of 2^-24
-constexpr int kWeightBits = 40;        // the largest logit weighs 2^40
 
 struct Args {
   const float* logits;
@@ -42,14 +41,41 @@ __device__ __forceinline__ float value_of(unsigned key) {
   return __uint_as_float((key & 0x80000000u) ? (key & 0x7fffffffu) : ~key);
 }
 
-// floor(2^40 e) of 0 <= e <= 1 by its bits (a conversion to 64 bits runs at a
-// fraction of the rate)
-__device__ __forceinline__ u64 weight_of(float e) {
-  const unsigned b = __float_as_uint(e);
-  const int up = (int)(b >> 23) - (127 - kWeightBits + 23);
-  const unsigned m = (b & 0x7fffffu) | 0x800000u;
-  return up >= 0 ? (u64)m << up : up > -24 ? (u64)(m >> -up) : 0;
+// floor(2^40 e) of 0 <= e <= 1 without 64-bit arithmetic or conversions: e 2^20
+// is split at the nearest whole number, both parts read from the low bits of a
+// sum with 2^23 or 1.5 2^23; the second is rounded down, so that the pair is
+// exact.
+constexpr unsigned kHighBase = 0x4b000000u, kLowBase = 0x4b400000u;
+__device__ __forceinline__ void weight_parts(float e, unsigned& high, unsigned& low) {
+  const float t = __fmul_rn(e, 1048576.0f), h = __fadd_rn(t, 8388608.0f);
+  high = __float_as_uint(h);
+  low = __float_as_uint(__fmaf_rd(__fsub_rn(t, __fsub_rn(h, 8388608.0f)), 1048576.0f, 12582912.0f));
 }
+__device__ __forceinline__ u64 weight_of(float e) {
+  unsigned high, low;
+  weight_parts(e, high, low);
+  return (u64)((int64_t)(int)(high - kHighBase) * (1 << 20) + (int)(low - kLowBase));
+}
+// A sum of weights: the parts' own bits are added up, and their bases taken out
+// every 2,048 terms at most (4,095 would still fit).
+struct WeightSum {
+  unsigned high = 0, low = 0, terms = 0;
+  u64 whole = 0;
+  __device__ __forceinline__ void add(float e) {
+    unsigned h, l;
+    weight_parts(e, h, l);
+    high += h;
+    low += l;
+  }
+  __device__ __forceinline__ void added(unsigned n) {
+    terms += n;
+    if (terms >= 2048) flush();
+  }
+  __device__ __forceinline__ void flush() {
+    whole += (u64)((int64_t)(high - terms * kHighBase) * (1 << 20) + (int)(low - terms * kLowBase));
+    high = low = terms = 0;
+  }
+};
 
 // floor(a * m / 2^24) for m <= 2^24 (a below 2^64 / 2^24 in the low part only)
 __device__ __forceinline__ u64 scaled(u64 a, u64 m, u64 round) {
@@ -65,22 +91,32 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 // A row is worked on by a cluster of CTAs, a slice each.  With few rows the
 // slices are staged in shared memory (the row is read from memory once and
 // the passes below read it from there); with many, or a row too long for
-// that, one CTA takes a whole row and reads it again from L2 in each pass, so
-// that every SM has rows of its own and nothing waits for another CTA.  What
-// the CTAs of a row tell one another goes through distributed shared memory,
-// one cluster barrier per exchange:
+// that, each pass reads them from memory again, and a greedy row or one with a
+// top-k of up to kDirect is left to the cluster's first CTA.  What the CTAs of a
+// row tell one another goes through distributed shared memory, one cluster
+// barrier per exchange:
 //   1. the largest and the smallest logit;
-//   2. with top-k or top-p, a histogram of z = (max - logit) / temperature
-//      over at most 28 (past it a weight is 0: e^-28 < 2^-40) in 512 equal
-//      bins; every CTA adds up all of them and finds the bin in which the
-//      k-th logit, or the top_p of the mass, falls;
-//   3. the tokens up to that bin, usually a few hundred at most, go to the
-//      first CTA of the cluster, which sorts them and finishes the row alone.
+//   2. with top-k, a bound from the threads' own maxima; one CTA alone then
+//      takes the tokens up to it (step 4).  Several, or a top-k past kDirect: a
+//      histogram of z = (max - logit) / temperature over at most 28 (past it a
+//      weight is 0: e^-28 < 2^-40) in 512 equal bins; every CTA adds up all of
+//      them and finds the bin in which the k-th logit falls;
+//   3. with top-p alone, the masses of sixteen ranges of z, then the histogram,
+//      with masses, of the one in which the top_p of the mass falls;
+//   4. the tokens up to that bin, usually a few hundred at most, go to the
+//      first CTA of the cluster, which finds the cuts among them and finishes
+//      the row alone.
 // Where they are more than kList (a wide nucleus, ties), the exact cut is
 // found over the whole cluster instead: the bin's own tokens, listed in every
 // CTA, are sorted by value and index; a bin with too many is divided again by
 // the bits of the key, then by index.  Then each CTA adds up its kept mass,
 // and the one that holds the draw walks its part.
+//
+// What bounds it: one row is latency (13 us for 0.5 MB: a handful of exchanges
+// and scans); many rows, the passes over them: 256 rows of 120,832 logits (124
+// MB) take 24 us greedy (one pass, 5.2 TB/s), 47 us with top-k 40 (two), 100 us
+// without filters (exponentials of all, 31 M in one pass), 180 us with top-p
+// alone (five passes).
 
 constexpr int kT = 512;                // threads of a CTA
 constexpr int kW = kT / 32;
@@ -89,8 +125,11 @@ constexpr int kBins = 512;
 static_assert(kBins == kT, "one bin per thread");
 constexpr int kList = 2048;            // tokens the first CTA sorts
 constexpr int kMaxCluster = 16;
-constexpr int kMaxSlice = 24 * kUnit;  // floats: 192 KB
+constexpr int kMaxSlice = 16 * kUnit;  // floats: 128 KB
 constexpr float kSpan = 28.0f;
+constexpr int kCoarse = 16;            // ranges of bins (with one or the other shift)
+constexpr int kFine = kCoarse * kBins;
+static_assert(kCoarse == kW, "a warp adds up a range");
 
 __device__ __forceinline__ unsigned ctarank() {
   unsigned r;
@@ -102,10 +141,9 @@ __device__ __forceinline__ unsigned nctas() {
   asm("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
   return r;
 }
-// All threads of the row: of the cluster (STAGED), or of its one CTA.
-template <bool STAGED>
-__device__ __forceinline__ void barrier() {
-  if constexpr (!STAGED) {
+// All threads of the row's `ctas`.
+__device__ __forceinline__ void barrier(unsigned ctas) {
+  if (ctas == 1) {
     __syncthreads();
     return;
   }
@@ -123,6 +161,11 @@ __device__ __forceinline__ void put64(uint32_t a, u64 v) {
 __device__ __forceinline__ void put32(uint32_t a, unsigned v) {
   asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(a), "r"(v) : "memory");
 }
+__device__ __forceinline__ u64 get64(uint32_t a) {
+  u64 v;
+  asm volatile("ld.shared::cluster.u64 %0, [%1];" : "=l"(v) : "r"(a) : "memory");
+  return v;
+}
 __device__ __forceinline__ unsigned get32(uint32_t a) {
   unsigned v;
   asm volatile("ld.shared::cluster.u32 %0, [%1];" : "=r"(v) : "r"(a) : "memory");
@@ -138,11 +181,12 @@ struct Shared {
   unsigned first_of[kMaxCluster];
   u64 mass_of[kMaxCluster];
   u64 warp_a[kW], warp_b[kW];
+  u64 range_of[kMaxCluster][kCoarse], range[kCoarse];
   unsigned fill;                // entries of the list so far
-  unsigned bin, lower_in;
+  int bin;
+  unsigned lower_in, above;     // above: this CTA's tokens before the bins
   u64 above_n, above_w, in_n;
 };
-static_assert(2 * kUnit * sizeof(float) >= kList * sizeof(u64), "the masses of a sorted list");
 // Logits of a slice up to which the sums of 14-bit parts stay below 2^32;
 // past it (one CTA, a longer row) the masses are 64-bit atomics.
 constexpr int kPartMax = 1 << 18;
@@ -158,6 +202,7 @@ struct Slice {
   int first;       // index in the row of this thread's first four
   int n, groups;
   bool vec, infinite;
+  unsigned ctas;   // that share the row
   __device__ __forceinline__ int index(int j) const { return first + 128 * j; }
   __device__ __forceinline__ float4 from_memory(const float* row, int j) const {
     const int i = index(j);
@@ -260,17 +305,23 @@ struct Cut {
 
 struct Scale {
   float max, inverse, bins;
+  int base, shift;  // bins of 2^shift steps from `base` on
   __device__ __forceinline__ float e(float x) const {
     return fmaxf(expf(__fmul_rn(__fsub_rn(x, max), inverse)), 0.0f);  // (0 for NaN)
   }
   // a logit below which every bin is past `b` (two bins of slack for rounding)
-  __device__ __forceinline__ float least(unsigned b) const { return max - (float)(b + 2) / bins * 1.0001f; }
-  // (max - x) / temperature in bins, to the nearest whole number (the sum with
-  // 2^23 rounds it into the low bits): monotone in the logit; kBins and more:
-  // no weight.  `bins` carries the 1 / temperature.
-  __device__ __forceinline__ unsigned bin(float x) const {
-    return __float_as_uint(fminf(__fmul_rn(__fsub_rn(max, x), bins), 4.0f * kBins) + 8388608.0f) & 0x7fffffu;
+  __device__ __forceinline__ float least(int b) const {
+    return max - (float)((base + b + 2) << shift) / bins * 1.0001f;
   }
+  // (max - x) / temperature in 2^13 steps over the span, to the nearest whole
+  // number (the sum with 2^23 rounds it into the low bits): monotone in the
+  // logit; kFine and more: no weight.  `bins` carries the 1 / temperature.
+  __device__ __forceinline__ unsigned fine(float x) const {
+    return __float_as_uint(fminf(__fmul_rn(__fsub_rn(max, x), bins), 4.0f * kFine) + 8388608.0f) & 0x7fffffu;
+  }
+  // the bin of the range that is looked at: below 0 before it, kBins and more
+  // past it
+  __device__ __forceinline__ int bin(float x) const { return (int)(fine(x) >> shift) - base; }
 };
 
 // Order of the tokens: larger logits first, ties by index.
@@ -279,17 +330,17 @@ __device__ __forceinline__ u64 order_of(float x, int index) { return ((u64)~key_
 // Which part of the row is divided next: all of it by z, or a z bin and leading
 // bits of the order, 9 at a time.
 struct Part {
-  unsigned zbin;
+  int zbin;
   u64 prefix, mask;
   int shift;  // of the next 9 bits; 64: by z
 };
 
-__device__ __forceinline__ unsigned sub_bin(const Scale& sc, const Part& p, float x, int index) {
-  const unsigned z = sc.bin(x);
+__device__ __forceinline__ int sub_bin(const Scale& sc, const Part& p, float x, int index) {
+  const int z = sc.bin(x);
   if (p.shift == 64) return z;
   const u64 order = order_of(x, index);
   if (z != p.zbin || (order & p.mask) != p.prefix) return kBins;
-  return (unsigned)(order >> p.shift) & (kBins - 1);
+  return (int)(order >> p.shift) & (kBins - 1);
 }
 
 // Exclusive sums over the CTA's bins of two values, one bin per thread.
@@ -423,29 +474,78 @@ constexpr int kPer = kList / kT;  // tokens of a sorted list per thread
 // Where a cut falls: bin `b` of a part, the tokens and the mass before it, its
 // own tokens, and this CTA's place among them (of the bin, of all up to it).
 struct Found {
-  unsigned b;
+  int b;
   u64 above_n, above_w, in_n, want;
   unsigned lower_in, lower_upto;
 };
 
+// For a cut by mass of a whole row: the sixteenth of the span in which it
+// falls becomes the scale's bins, so that only the tokens there go into
+// locate()'s histogram (its shared-memory atomics cost more than the
+// exponentials).  The sums are each thread's own, in shared memory at `own`
+// (kCoarse x kT), and need no atomics.  Returns the mass before the range; want:
+// `share` of the row's.
+template <bool STAGED>
+__device__ u64 coarse_range(Shared& sh, const Slice<STAGED>& row, Scale& sc, u64* own, u64 share, u64& want) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned rank = ctarank(), ctas = row.ctas;
+#pragma unroll
+  for (int j = 0; j < kCoarse; ++j) own[j * kT + threadIdx.x] = 0;
+  row.groups_of_4([&](float4 v, int) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const float x = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w;
+      const unsigned j = sc.fine(x) / kBins;
+      if (j < kCoarse) own[j * kT + threadIdx.x] += weight_of(sc.e(x));
+    }
+  });
+  __syncthreads();
+  u64 m = 0;
+#pragma unroll
+  for (int q = 0; q < kT / 32; ++q) m += own[warp * kT + 32 * q + lane];
+  m = warp_sum_u64(m);
+  if (lane < ctas) put64(remote(&sh.range_of[rank][warp], lane), m);
+  barrier(row.ctas);
+  if (threadIdx.x < kCoarse) {
+    m = 0;
+    for (unsigned c = 0; c < ctas; ++c) m += sh.range_of[c][threadIdx.x];
+    sh.range[threadIdx.x] = m;
+  }
+  __syncthreads();
+  u64 total = 0, before = 0;
+#pragma unroll
+  for (int j = 0; j < kCoarse; ++j) total += sh.range[j];
+  want = max(scaled(total, share, (1u << kGrid) - 1), 1ull);
+  int j = 0;
+  while (j < kCoarse - 1 && before + sh.range[j] < want) before += sh.range[j++];
+  sc.base = j * kBins;
+  sc.shift = 0;
+  return before;
+}
+
 // Finds the bin of `part` in which token number `want`, or (BY_MASS) the
-// `want`-th unit of mass, falls, among the tokens up to `limit`; with BY_MASS
-// and want 0, want is `share` of the part's mass.  b = kBins: there are fewer.
-// Bins past `bound` are known not to matter.
+// `want`-th unit of mass, falls, among the tokens up to `limit`.  b = kBins:
+// there are fewer.  Bins past `bound` are known not to matter.
 template <bool BY_MASS, bool STAGED>
 __device__ Found locate(Shared& sh, const Slice<STAGED>& row, const Scale& sc, const Part& part, Cut limit, u64 want,
-                        u64 share, u64 above_n, u64 above_w, unsigned bound) {
-  const unsigned rank = ctarank(), ctas = nctas();
+                        u64 above_n, u64 above_w, int bound) {
+  const unsigned rank = ctarank(), ctas = row.ctas;
   for (int i = threadIdx.x; i < (BY_MASS ? 4 : 1) * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
   if (threadIdx.x == 0) {
     sh.bin = kBins;
     sh.fill = 0;
+    sh.above = 0;
   }
   __syncthreads();
   const bool all = part.shift == 64 && limit.all();
+  unsigned over = 0;  // tokens before the bins
   row.each_from(sc.least(bound), [&](float x, int i) {
-    const unsigned b = all ? sc.bin(x) : sub_bin(sc, part, x, i);
+    const int b = all ? sc.bin(x) : sub_bin(sc, part, x, i);
     if (b > bound || (!all && !limit.keeps(x, i))) return;
+    if (BY_MASS && b < 0) {
+      ++over;
+      return;
+    }
     if constexpr (BY_MASS) {
       const u64 w = weight_of(sc.e(x));
       if (w == 0) return;
@@ -459,8 +559,13 @@ __device__ Found locate(Shared& sh, const Slice<STAGED>& row, const Scale& sc, c
     }
     atomicAdd(&sh.hist[0][b], 1u);
   });
-  barrier<STAGED>();
+  if constexpr (BY_MASS) {
+    over = __reduce_add_sync(0xffffffffu, over);
+    if ((threadIdx.x & 31) == 0 && over) atomicAdd(&sh.above, over);
+  }
+  barrier(row.ctas);
   u64 count = 0, weight = 0;
+  unsigned lower_over = 0;
   unsigned lower = 0;  // tokens of this thread's bin in the CTAs before this one
 #pragma unroll 4
   for (unsigned c = 0; c < ctas; ++c) {
@@ -469,19 +574,19 @@ __device__ Found locate(Shared& sh, const Slice<STAGED>& row, const Scale& sc, c
     if (c < rank) lower += in;
     count += in;
     if constexpr (BY_MASS) {
+      over = get32(remote(&sh.above, c));
+      if (c < rank) lower_over += over;
+      above_n += over;
+    }
+    if constexpr (BY_MASS) {
       if (row.groups * (128 * kW) <= kPartMax)
         weight += (u64)get32(h + 4 * kBins) + ((u64)get32(h + 8 * kBins) << 14) + ((u64)get32(h + 12 * kBins) << 28);
       else
-        weight += reinterpret_cast<const u64*>(&sh.hist[2][0])[threadIdx.x];  // (a cluster of one)
+        weight += get64(remote(reinterpret_cast<u64*>(&sh.hist[2][0]) + threadIdx.x, c));
     }
   }
   u64 before_n, before_w;
   scan2(sh, count, weight, before_n, before_w);
-  if (BY_MASS && want == 0) {
-    u64 mass = 0;
-    for (int w = 0; w < kW; ++w) mass += sh.warp_b[w];
-    want = max(scaled(mass, share, (1u << kGrid) - 1), 1ull);
-  }
   before_n += above_n;
   before_w += above_w;
   if (BY_MASS ? before_w < want && before_w + weight >= want : before_n < want && before_n + count >= want) {
@@ -506,11 +611,11 @@ __device__ Found locate(Shared& sh, const Slice<STAGED>& row, const Scale& sc, c
     f.in_n = sh.in_n;
     f.lower_in = sh.lower_in;
   }
-  unsigned mine = threadIdx.x < f.b ? lower : 0;
+  unsigned mine = (int)threadIdx.x < f.b ? lower : 0;
   mine = __reduce_add_sync(0xffffffffu, mine);
   if ((threadIdx.x & 31) == 0 && mine) atomicAdd(&sh.fill, mine);
   __syncthreads();
-  f.lower_upto = sh.fill + f.lower_in;
+  f.lower_upto = sh.fill + f.lower_in + lower_over;
   __syncthreads();
   return f;
 }
@@ -518,7 +623,7 @@ __device__ Found locate(Shared& sh, const Slice<STAGED>& row, const Scale& sc, c
 // The exact cut inside a bin that locate() found.
 template <bool BY_MASS, bool STAGED>
 __device__ Cut resolve(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Found f, Cut limit) {
-  const unsigned ctas = nctas();
+  const unsigned ctas = row.ctas;
   Part part{0, 0, 0, 64};
   // (8 levels divide a 64-bit order to single tokens; the bound is for safety)
   for (int level = 0; level < 10 && f.b < kBins; ++level) {
@@ -535,7 +640,7 @@ __device__ Cut resolve(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Fo
             if (slot < kList)
               for (unsigned c = 0; c < ctas; ++c) put64(remote(&sh.list[slot], c), order_of(x, i));
           });
-      barrier<STAGED>();
+      barrier(row.ctas);
       sort_tokens(sh, m);
       const int per = (m + kT - 1) / kT, t0 = threadIdx.x * per;
       u64 w[kPer], mine = 0, total, last = 0;
@@ -560,7 +665,7 @@ __device__ Cut resolve(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Fo
       __syncthreads();
       return Cut{value_of(~(unsigned)(last >> 32)), (int)(unsigned)last};
     }
-    barrier<STAGED>();  // the histograms are read; divide the bin
+    barrier(row.ctas);  // the histograms are read; divide the bin
     if (part.shift == 64) {
       part.zbin = f.b;
       part.shift = 55;
@@ -569,7 +674,7 @@ __device__ Cut resolve(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Fo
       part.mask |= (u64)(kBins - 1) << part.shift;
       part.shift = part.shift >= 9 ? part.shift - 9 : 0;
     }
-    f = locate<BY_MASS>(sh, row, sc, part, limit, f.want, 0, f.above_n, f.above_w, kBins - 1);
+    f = locate<BY_MASS>(sh, row, sc, part, limit, f.want, f.above_n, f.above_w, kBins - 1);
   }
   return limit;  // fewer, or lighter, than what is wanted: all
 }
@@ -579,26 +684,22 @@ __device__ Cut resolve(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Fo
 template <bool STAGED>
 __device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice<STAGED>& row, const Scale& sc, Cut cut, float floor_e,
                                          u64& before, u64& mine) {
-  const unsigned rank = ctarank(), ctas = nctas();
+  const unsigned rank = ctarank(), ctas = row.ctas;
   const int warp = threadIdx.x >> 5;
-  u64 m = 0;
+  u64 m;
+  WeightSum sum;
   const bool all = cut.all();
-  if (all) {
-    row.groups_of_4([&](float4 v, int) {
+  row.groups_of_4([&](float4 v, int i) {
+    if (!all && !(fmaxf(fmaxf(v.x, v.y), fmaxf(v.z, v.w)) >= cut.x)) return;
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const float e = sc.e(k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w);
-        m += e >= floor_e ? weight_of(e) : 0;
-      }
-    });
-  } else {
-    row.each_from(cut.x, [&](float x, int i) {
-      if (!cut.keeps(x, i)) return;
-      const float e = sc.e(x);
-      if (e >= floor_e) m += weight_of(e);
-    });
-  }
-  mine = warp_sum_u64(m);
+    for (int k = 0; k < 4; ++k) {
+      const float x = k == 0 ? v.x : k == 1 ? v.y : k == 2 ? v.z : v.w, e = sc.e(x);
+      sum.add(e >= floor_e && (all || cut.keeps(x, i + k)) ? e : 0.0f);
+    }
+    sum.added(4);
+  });
+  sum.flush();
+  mine = warp_sum_u64(sum.whole);
   __syncthreads();
   if ((threadIdx.x & 31) == 0) sh.warp_a[warp] = mine;
   __syncthreads();
@@ -607,7 +708,7 @@ __device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice<STAGED>& row, c
     for (int w = 0; w < kW; ++w) m += sh.warp_a[w];
     put64(remote(&sh.mass_of[rank], threadIdx.x), m);
   }
-  barrier<STAGED>();
+  barrier(row.ctas);
   u64 total = 0;
   before = 0;
   for (unsigned c = 0; c < ctas; ++c) {
@@ -618,11 +719,142 @@ __device__ __forceinline__ u64 mass_upto(Shared& sh, const Slice<STAGED>& row, c
   return total;
 }
 
+// The unit of a row's mass that is drawn.
+__device__ __forceinline__ u64 aim_of(const Args& a, int r, u64 total) {
+  const float uf = fminf(fmaxf(a.u[r], 0.0f), 1.0f);
+  return scaled(total, min((u64)__fmul_rn(uf, 16777216.0f), (u64)(1u << kGrid) - 1), 0);
+}
+__device__ __forceinline__ u64 weight_in(const Shared& sh, int b) {
+  return (u64)sh.hist[1][b] + ((u64)sh.hist[2][b] << 14) + ((u64)sh.hist[3][b] << 28);
+}
+__device__ __forceinline__ void add_weight(Shared& sh, int b, u64 w) {
+  atomicAdd(&sh.hist[1][b], (unsigned)(w & 0x3fff));
+  atomicAdd(&sh.hist[2][b], (unsigned)(w >> 14 & 0x3fff));
+  atomicAdd(&sh.hist[3][b], (unsigned)(w >> 28));
+}
+
+// finish() without sorting, for more than kPairs tokens: the cuts' bins from a
+// histogram of the list, the cuts themselves by comparing the tokens of one bin;
+// then the masses of 512 ranges of indexes, and the tokens of the one that
+// holds the draw.  False, with nothing done, if a bin has more than kPairs.
+__device__ bool finish_by_bins(Shared& sh, u64* few, const Scale& sc, const Args& a, int r, int m, int k, u64 want,
+                               bool by_mass, u64 share_p, float floor_e) {
+  u64* few_w = few + kList;
+  u64 order[kPer], w[kPer];
+  int bin[kPer];
+  for (int i = threadIdx.x; i < 4 * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    const int t = threadIdx.x + q * kT;
+    order[q] = t < m ? sh.list[t] : ~0ull;
+    w[q] = 0;
+    bin[q] = kBins;
+    if (t < m) {
+      const float x = value_of(~(unsigned)(order[q] >> 32));
+      w[q] = weight_of(sc.e(x));
+      bin[q] = min((int)(sc.fine(x) / kCoarse), kBins - 1);
+      atomicAdd(&sh.hist[0][bin[q]], 1u);
+      add_weight(sh, bin[q], w[q]);
+    }
+  }
+  __syncthreads();
+  const u64 count = sh.hist[0][threadIdx.x], weight = weight_in(sh, threadIdx.x);
+  u64 before_n, before_w;
+  scan2(sh, count, weight, before_n, before_w);
+  u64 total = 0;
+  for (int i = 0; i < kW; ++i) total += sh.warp_b[i];
+  // tokens of the bin that thread `at` found, and their number
+  auto gather = [&](bool at, u64 cut) {
+    if (threadIdx.x == 0) sh.fill = 0;
+    if (at) {
+      sh.bin = threadIdx.x;
+      sh.above_n = before_n;
+      sh.above_w = before_w;
+    }
+    __syncthreads();
+    const int b = sh.bin;
+#pragma unroll
+    for (int q = 0; q < kPer; ++q)
+      if (bin[q] == b && order[q] <= cut) {
+        const unsigned slot = atomicAdd(&sh.fill, 1u);
+        few[slot] = order[q];
+        few_w[slot] = w[q];
+      }
+    __syncthreads();
+    return (int)sh.fill;
+  };
+  u64 cut = ~0ull;  // the last token that is kept
+  if (k < m) {
+    const int n = gather(before_n < (u64)k && before_n + count >= (u64)k, cut);
+    if (n > kPairs) return false;
+    if ((int)threadIdx.x < n) {
+      u64 lighter = 0;
+      int place = (int)sh.above_n;
+      for (int j = 0; j < n; ++j)
+        if (few[j] < few[threadIdx.x]) {
+          ++place;
+          lighter += few_w[j];
+        }
+      if (place == k - 1) {
+        sh.warp_a[0] = few[threadIdx.x];
+        sh.warp_a[1] = sh.above_w + lighter + few_w[threadIdx.x];
+      }
+    }
+    __syncthreads();
+    cut = sh.warp_a[0];
+    total = sh.warp_a[1];
+    __syncthreads();
+  }
+  if (by_mass) {
+    if (want == 0) want = max(scaled(total, share_p, (1u << kGrid) - 1), 1ull);
+    const int n = gather(before_w < want && before_w + weight >= want, cut);
+    if (n > kPairs) return false;
+    if ((int)threadIdx.x < n) {
+      u64 at = sh.above_w;
+      for (int j = 0; j < n; ++j)
+        if (few[j] < few[threadIdx.x]) at += few_w[j];
+      if (at < want && at + few_w[threadIdx.x] >= want) sh.warp_a[0] = few[threadIdx.x];
+    }
+    __syncthreads();
+    cut = sh.warp_a[0];
+    __syncthreads();
+  }
+  // the draw, in the order of the indexes
+  const int width = (a.n + kBins - 1) / kBins;
+  for (int i = threadIdx.x; i < 4 * kBins; i += kT) (&sh.hist[0][0])[i] = 0;
+  __syncthreads();
+#pragma unroll
+  for (int q = 0; q < kPer; ++q) {
+    bin[q] = kBins;
+    if (w[q] && order[q] <= cut && sc.e(value_of(~(unsigned)(order[q] >> 32))) >= floor_e) {
+      bin[q] = (int)((unsigned)order[q] / (unsigned)width);
+      add_weight(sh, bin[q], w[q]);
+    }
+  }
+  __syncthreads();
+  const u64 mine = weight_in(sh, threadIdx.x);
+  before_w = scan1(sh, mine, total);
+  const u64 aim = aim_of(a, r, total);
+  const int n = gather(aim >= before_w && aim < before_w + mine, ~0ull);
+  for (int i = threadIdx.x; i < n; i += kT) {
+    u64 at = sh.above_w;
+    for (int j = 0; j < n; ++j)
+      if ((unsigned)few[j] < (unsigned)few[i]) at += few_w[j];
+    if (aim >= at && aim < at + few_w[i]) {
+      a.token[r] = (int)(unsigned)few[i];
+      if (a.prob) a.prob[r] = __fdiv_rn((float)few_w[i], (float)total);
+    }
+  }
+  return true;
+}
+
 // The rest of a row by one CTA: list[0 .. m) holds the order of every token
 // that can be kept.  `k`: keep at most that many; `want`: then those whose
 // predecessors weigh less (0: not yet known, top_p of what k keeps).
 __device__ void finish(Shared& sh, u64* mass_s, const Scale& sc, const Args& a, int r, int m, int k, u64 want,
                        bool by_mass, u64 share_p, float floor_e) {
+  if (m > kPairs && finish_by_bins(sh, mass_s, sc, a, r, m, k, want, by_mass, share_p, floor_e)) return;
   // consecutive tokens per thread
   sort_tokens(sh, m);
   const int per = (m + kT - 1) / kT, t0 = threadIdx.x * per;
@@ -657,9 +889,7 @@ __device__ void finish(Shared& sh, u64* mass_s, const Scale& sc, const Args& a, 
     }
   scan1(sh, mine, total);
   sort_tokens(sh, m);
-  const float uf = fminf(fmaxf(a.u[r], 0.0f), 1.0f);
-  const u64 ui = min((u64)__fmul_rn(uf, 16777216.0f), (u64)(1u << kGrid) - 1);
-  const u64 aim = scaled(total, ui, 0);
+  const u64 aim = aim_of(a, r, total);
   mine = 0;
 #pragma unroll
   for (int q = 0; q < kPer; ++q) {
@@ -679,13 +909,13 @@ __device__ void finish(Shared& sh, u64* mass_s, const Scale& sc, const Args& a, 
   }
 }
 
-// The bin up to which the first k logits of the row lie, at least: the k-th
-// largest of the threads' own maxima (this CTA alone holds k logits there).
-__device__ __forceinline__ unsigned local_bound(Shared& sh, const Scale& sc, float thread_max, int k) {
+// The bin of the k-th largest of the threads' own maxima: this CTA alone holds k
+// logits up to there.
+__device__ __forceinline__ int local_bound(Shared& sh, const Scale& sc, float thread_max, int k) {
   sh.hist[0][threadIdx.x] = 0;
   if (threadIdx.x == 0) sh.bin = kBins - 1;
   __syncthreads();
-  const unsigned b = sc.bin(thread_max);
+  const int b = sc.bin(thread_max);
   if (b < kBins) atomicAdd(&sh.hist[0][b], 1u);
   __syncthreads();
   const u64 count = sh.hist[0][threadIdx.x];
@@ -693,10 +923,16 @@ __device__ __forceinline__ unsigned local_bound(Shared& sh, const Scale& sc, flo
   const u64 before = scan1(sh, count, total);
   if (before < (u64)k && before + count >= (u64)k) sh.bin = threadIdx.x;
   __syncthreads();
-  const unsigned bound = sh.bin;
+  const int bound = sh.bin;
   __syncthreads();
   return bound;
 }
+
+// Of a row's kT threads' maxima, which one has about 1.3 k + 16 logits up to it,
+// if they lie at random: k of them nearly always, and kList hardly ever (for
+// k <= kDirect).
+constexpr int kDirect = 1400;
+__device__ __forceinline__ int likely(int k) { return (int)(kT * (1.0f - __expf(-(1.3f * k + 16.0f) / kT))); }
 
 // STAGED: a cluster per row, the slices in shared memory (after the sorted
 // list's masses).  Otherwise one CTA per row.
@@ -706,13 +942,22 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
   allow_dependents_launch();
   __shared__ Shared sh;
   extern __shared__ __align__(16) float x_s[];
-  const unsigned rank = ctarank(), ctas = nctas();
-  const int r = blockIdx.x / ctas, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const unsigned rank = ctarank();
+  const int r = blockIdx.x / nctas(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float* x = a.logits + r * a.stride;
+  const float temperature = a.temperature ? a.temperature[r] : 1.0f;
+  const int k = a.top_k ? a.top_k[r] : 0;
+  const bool by_count = k > 0 && k < a.n;
+  unsigned ctas = nctas();
+  if (!STAGED && (!(temperature > 0.0f) || (by_count && k <= kDirect))) {  // one pass more than the maximum's, at most
+    if (rank != 0) return;
+    ctas = 1;
+    slice = (a.n + kUnit - 1) / kUnit * kUnit;
+  }
   const int share = slice / kW;  // of a warp
   float* mine_s = x_s + warp * share;
   Slice<STAGED> row{STAGED ? mine_s : x, (int)rank * slice + warp * share + 4 * lane, a.n, share / 128,
-                    (reinterpret_cast<uintptr_t>(x) & 15) == 0, false};
+                    (reinterpret_cast<uintptr_t>(x) & 15) == 0, false, ctas};
   float top = -INFINITY, low = INFINITY;
   int top_group = 0;  // where this thread first saw its largest
   for (int j0 = 0; j0 < row.groups; j0 += 4) {
@@ -752,7 +997,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
     warp_max[warp] = top;
     warp_min[warp] = low;
   }
-  barrier<STAGED>();  // every CTA of the cluster runs before its shared memory is written to
+  barrier(row.ctas);  // every CTA of the cluster runs before its shared memory is written to
   if (threadIdx.x < ctas) {
     for (int w = 0; w < kW; ++w) {
       top = fmaxf(top, warp_max[w]);
@@ -761,14 +1006,13 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
     put32(remote(&sh.max_of[rank], threadIdx.x), __float_as_uint(top));
     put32(remote(&sh.min_of[rank], threadIdx.x), __float_as_uint(low));
   }
-  barrier<STAGED>();
+  barrier(row.ctas);
   top = -INFINITY;
   low = INFINITY;
   for (unsigned c = 0; c < ctas; ++c) {
     top = fmaxf(top, sh.max_of[c]);
     low = fminf(low, sh.min_of[c]);
   }
-  const float temperature = a.temperature ? a.temperature[r] : 1.0f;
   if (top == -INFINITY) {
     if (rank == 0 && threadIdx.x == 0) {
       a.token[r] = 0;
@@ -789,7 +1033,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
     if (lane == 0) atomicMin(&sh.fill, first);
     __syncthreads();
     if (threadIdx.x == 0) put32(remote(&sh.first_of[rank], 0), sh.fill);
-    barrier<STAGED>();
+    barrier(row.ctas);
     if (rank == 0 && threadIdx.x == 0) {
       for (unsigned c = 0; c < ctas; ++c) first = min(first, sh.first_of[c]);
       a.token[r] = (int)first;
@@ -808,22 +1052,49 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
   sc.max = top;
   sc.inverse = fminf(__fdiv_rn(1.0f, temperature), 3e38f);
   const float span = (top - low) * sc.inverse;
-  sc.bins = fminf((kBins - 1) / fminf(fmaxf(span, 1e-20f), kSpan) * sc.inverse, 1e38f);
-  const int k = a.top_k ? a.top_k[r] : 0;
+  sc.bins = fminf((kFine - 1) / fminf(fmaxf(span, 1e-20f), kSpan) * sc.inverse, 1e38f);
+  sc.base = 0;
+  sc.shift = 4;
   const float p = a.top_p ? a.top_p[r] : 1.0f;
   const float floor_e = a.min_p ? fminf(a.min_p[r], 1.0f) : 0.0f;
-  const bool by_count = k > 0 && k < a.n, by_mass = p < 1.0f;
+  const bool by_mass = p < 1.0f;
   const u64 share_p = by_mass ? (u64)ceilf(__fmul_rn(fmaxf(p, 0.0f), 16777216.0f)) : 0;
   Cut cut{-INFINITY, INT32_MAX};
   u64 before, mine;
   if (by_count || by_mass) {
     const Part whole{0, 0, 0, 64};
-    const unsigned bound = by_count && k <= kT / 2 ? local_bound(sh, sc, own_max, k) : kBins - 1;
-    Found f = by_count ? locate<false>(sh, row, sc, whole, cut, (u64)k, 0, 0, 0, bound)
-                       : locate<true>(sh, row, sc, whole, cut, 0, share_p, 0, 0, bound);
+    int bound = kBins - 1;
+    if (by_count && k <= kDirect) {
+      bound = local_bound(sh, sc, own_max, k <= kT / 2 ? k : likely(k));
+      if (ctas == 1) {
+        if (threadIdx.x == 0) sh.fill = 0;
+        __syncthreads();
+        row.collect(sc.least(bound), &sh.fill, [&](float v, int) { return sc.bin(v) <= bound; },
+                    [&](unsigned slot, float v, int i) {
+                      if (slot < kList) sh.list[slot] = order_of(v, i);
+                    });
+        __syncthreads();
+        const unsigned n = sh.fill;
+        __syncthreads();
+        if (n <= kList && (n >= (unsigned)k || bound == kBins - 1)) {
+          finish(sh, reinterpret_cast<u64*>(x_s), sc, a, r, (int)n, k, 0, by_mass, share_p, floor_e);
+          return;
+        }
+      }
+      if (k > kT / 2) bound = kBins - 1;  // a guess that did not hold
+    }
+    u64 want = (u64)k;
+    Found f;
+    if (by_count) {
+      f = locate<false>(sh, row, sc, whole, cut, want, 0, 0, bound);
+    } else {
+      u64* own = reinterpret_cast<u64*>(x_s + (STAGED ? slice : 0));
+      const u64 above_w = coarse_range(sh, row, sc, own, share_p, want);
+      f = locate<true>(sh, row, sc, whole, cut, want, 0, above_w, bound);
+    }
     // (a row with fewer than k weighty tokens: all of them)
     if (f.above_n + f.in_n <= kList) {
-      const unsigned upto = min(f.b, (unsigned)kBins - 1);
+      const int upto = min(f.b, kBins - 1);
       if (threadIdx.x == 0) sh.fill = f.lower_upto;
       __syncthreads();
       row.collect(
@@ -832,17 +1103,17 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
           [&](unsigned slot, float v, int i) {
             if (slot < kList) put64(remote(&sh.list[slot], 0), order_of(v, i));
           });
-      barrier<STAGED>();
+      barrier(row.ctas);
       if (rank == 0)
         finish(sh, reinterpret_cast<u64*>(x_s), sc, a, r, (int)(f.above_n + f.in_n), by_count ? k : a.n,
-               by_count ? 0 : f.want, by_mass, share_p, floor_e);
+               by_count ? 0 : want, by_mass, share_p, floor_e);
       return;
     }
     if (by_count) {
       cut = resolve<false>(sh, row, sc, f, cut);
       if (by_mass) {
         const u64 mass = mass_upto(sh, row, sc, cut, 0.0f, before, mine);
-        f = locate<true>(sh, row, sc, whole, cut, max(scaled(mass, share_p, (1u << kGrid) - 1), 1ull), 0, 0, 0, kBins - 1);
+        f = locate<true>(sh, row, sc, whole, cut, max(scaled(mass, share_p, (1u << kGrid) - 1), 1ull), 0, 0, kBins - 1);
         cut = resolve<true>(sh, row, sc, f, cut);
       }
     } else {
@@ -850,9 +1121,7 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
     }
   }
   const u64 total = mass_upto(sh, row, sc, cut, floor_e, before, mine);
-  const float uf = fminf(fmaxf(a.u[r], 0.0f), 1.0f);
-  const u64 ui = min((u64)__fmul_rn(uf, 16777216.0f), (u64)(1u << kGrid) - 1);
-  const u64 aim = scaled(total, ui, 0);
+  const u64 aim = aim_of(a, r, total);
   if (aim < before || aim >= before + mine) return;
   // this warp holds the token: index order is group by group of 128
   u64 run = before;
@@ -892,14 +1161,16 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
   }
 }
 
-cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
+constexpr int kOwnBytes = kCoarse * kT * sizeof(u64);  // coarse_range's sums
+static_assert(kOwnBytes >= 2 * kList * (int)sizeof(u64), "finish()'s lists");
+
+cudaError_t launch(const Args& a, int64_t rows, int ctas, bool staged, cudaStream_t st) {
   const int slice = ((a.n + ctas - 1) / ctas + kUnit - 1) / kUnit * kUnit;
-  if (ctas == 1)
-    return launch_ex(sample_kernel<false>, dim3((unsigned)rows), dim3(kT), kList * sizeof(u64), st, a, slice);
-  // (at least two units: the first CTA keeps a sorted list's masses there)
-  auto k = sample_kernel<true>;
-  static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(k, kMaxSlice * (int)sizeof(float), done);
+  auto k = staged ? sample_kernel<true> : sample_kernel<false>;
+  static std::atomic<uint64_t> done[2];
+  // (finish() keeps a list's masses where the slices, or the sums, were)
+  const int most = staged ? kMaxSlice * (int)sizeof(float) + kOwnBytes : kOwnBytes;
+  cudaError_t e = allow_smem(k, most, done[staged]);
   if (e != cudaSuccess) return e;
   if (ctas > 8 && (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
   cudaLaunchAttribute attr[2];
@@ -911,7 +1182,7 @@ cudaError_t launch(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)(rows * ctas));
   cfg.blockDim = dim3(kT);
-  cfg.dynamicSmemBytes = std::max(slice, 2 * kUnit) * sizeof(float);
+  cfg.dynamicSmemBytes = kOwnBytes + (staged ? slice * sizeof(float) : 0);
   cfg.stream = st;
   cfg.attrs = attr;
   cfg.numAttrs = launch_overlap() ? 2 : 1;
@@ -937,14 +1208,17 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
       return hyq::api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
   const hyq::sample::Args a{logits, stride, (int)n, temperature, top_k, top_p, min_p, u, token, prob};
   const cudaStream_t st = (cudaStream_t)stream;
-  // CTAs per row: twelve while every CTA has an SM of its own (one row of
-  // 120,832 logits: 12.3 us, 12.5 with eight, 14.2 with four), six when the
-  // rows queue for SMs (256 rows, mixed parameters: 172 us, 190 with four or
-  // eight); fewer for short rows, one for those that do not fit.
-  const int want = rows * 12 <= 148 ? 12 : 6;
-  int64_t ctas = std::min<int64_t>(want, (n + hyq::sample::kUnit - 1) / hyq::sample::kUnit);
-  if (ctas > 1 && n > ctas * hyq::sample::kMaxSlice) ctas = 1;
-  const cudaError_t e = hyq::sample::launch(a, rows, (int)ctas, st);
+  // Few rows: as many CTAs per row as there are SMs for, the slices in their
+  // shared memory (256 rows of 120,832 logits cut to n; temperature 0.7, top-k
+  // 40, top-p 0.9 / mixed parameters): n = 1: 14 / 15 us with eight, 16 / 16 with
+  // four; 16: 16 / 27 us with six, 24 / 25 with eight; 32: 17 / 59 us with four,
+  // 26 / 53 with six, 30 / 59 with six from memory.  Many rows: four per row, from
+  // memory (64: 30 / 67 us, 32 / 59 staged; 128: 47 / 77 us, 58 / 94 staged; 256:
+  // 84 / 116 us; 64 / 144 with two, 94 / 137 with eight).
+  const int64_t units = (n + hyq::sample::kUnit - 1) / hyq::sample::kUnit;
+  const int ctas = (int)std::min<int64_t>(rows <= 12 ? 8 : rows <= 16 ? 6 : 4, units);
+  const bool staged = rows <= 32 && ctas > 1 && n <= (int64_t)ctas * hyq::sample::kMaxSlice;
+  const cudaError_t e = hyq::sample::launch(a, rows, ctas, staged, st);
   return e == cudaSuccess ? HYQ_OK : hyq::api_fail(HYQ_E_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
