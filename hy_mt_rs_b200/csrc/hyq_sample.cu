@@ -92,8 +92,8 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 // slices are staged in shared memory (the row is read from memory once and
 // the passes below read it from there); with many, or a row too long for
 // that, each pass reads them from memory again, and a greedy row or one with a
-// top-k of up to kDirect is left to the cluster's first CTA.  What the CTAs of a
-// row tell one another goes through distributed shared memory, one cluster
+// top-k of up to kDirect has one CTA, in a launch of its own.  What the CTAs of
+// a row tell one another goes through distributed shared memory, one cluster
 // barrier per exchange:
 //   1. the largest and the smallest logit;
 //   2. with top-k, a bound from the threads' own maxima; one CTA alone then
@@ -114,9 +114,9 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 //
 // What bounds it: one row is latency (13 us for 0.5 MB: a handful of exchanges
 // and scans); many rows, the passes over them: 256 rows of 120,832 logits (124
-// MB) take 24 us greedy (one pass, 5.2 TB/s), 47 us with top-k 40 (two), 100 us
-// without filters (exponentials of all, 31 M in one pass), 180 us with top-p
-// alone (five passes).
+// MB) take 24 us greedy (one pass, 5.2 TB/s), 47 us with top-k 40 (two), 92 us
+// without filters (two, 31 M exponentials), 187 us with top-p 0.9 at 0.7 (four)
+// and 300 us at 1.0 (six: the nucleus is 14,000 tokens wide).
 
 constexpr int kT = 512;                // threads of a CTA
 constexpr int kW = kT / 32;
@@ -934,26 +934,23 @@ __device__ __forceinline__ int local_bound(Shared& sh, const Scale& sc, float th
 constexpr int kDirect = 1400;
 __device__ __forceinline__ int likely(int k) { return (int)(kT * (1.0f - __expf(-(1.3f * k + 16.0f) / kT))); }
 
-// STAGED: a cluster per row, the slices in shared memory (after the sorted
-// list's masses).  Otherwise one CTA per row.
+// Rows that take one pass more than the maximum's at most: greedy ones, and
+// those with a top-k whose candidates one CTA collects at once.
+__device__ __forceinline__ bool light(const Args& a, int r) {
+  const int k = a.top_k ? a.top_k[r] : 0;
+  return (a.temperature && !(a.temperature[r] > 0.0f)) || (k > 0 && k < a.n && k <= kDirect);
+}
+
+// A row by `ctas` CTAs, `slice` logits each; STAGED: kept in shared memory at
+// x_s.  The sums and lists come after them.
 template <bool STAGED>
-__global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ Args a, int slice) {
-  grid_dependency_wait();
-  allow_dependents_launch();
-  __shared__ Shared sh;
-  extern __shared__ __align__(16) float x_s[];
+__device__ __forceinline__ void sample_row(Shared& sh, float* x_s, const Args& a, int r, unsigned ctas, int slice) {
   const unsigned rank = ctarank();
-  const int r = blockIdx.x / nctas(), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const float* x = a.logits + r * a.stride;
   const float temperature = a.temperature ? a.temperature[r] : 1.0f;
   const int k = a.top_k ? a.top_k[r] : 0;
   const bool by_count = k > 0 && k < a.n;
-  unsigned ctas = nctas();
-  if (!STAGED && (!(temperature > 0.0f) || (by_count && k <= kDirect))) {  // one pass more than the maximum's, at most
-    if (rank != 0) return;
-    ctas = 1;
-    slice = (a.n + kUnit - 1) / kUnit * kUnit;
-  }
   const int share = slice / kW;  // of a warp
   float* mine_s = x_s + warp * share;
   Slice<STAGED> row{STAGED ? mine_s : x, (int)rank * slice + warp * share + 4 * lane, a.n, share / 128,
@@ -1163,16 +1160,41 @@ __global__ void __launch_bounds__(kT, 2) sample_kernel(const __grid_constant__ A
 
 constexpr int kOwnBytes = kCoarse * kT * sizeof(u64);  // coarse_range's sums
 static_assert(kOwnBytes >= 2 * kList * (int)sizeof(u64), "finish()'s lists");
+__host__ __device__ inline int slice_of(int n, int ctas) { return ((n + ctas - 1) / ctas + kUnit - 1) / kUnit * kUnit; }
 
-cudaError_t launch(const Args& a, int64_t rows, int ctas, bool staged, cudaStream_t st) {
-  const int slice = ((a.n + ctas - 1) / ctas + kUnit - 1) / kUnit * kUnit;
-  auto k = staged ? sample_kernel<true> : sample_kernel<false>;
-  static std::atomic<uint64_t> done[2];
-  // (finish() keeps a list's masses where the slices, or the sums, were)
-  const int most = staged ? kMaxSlice * (int)sizeof(float) + kOwnBytes : kOwnBytes;
-  cudaError_t e = allow_smem(k, most, done[staged]);
-  if (e != cudaSuccess) return e;
-  if (ctas > 8 && (e = cudaFuncSetAttribute(k, cudaFuncAttributeNonPortableClusterSizeAllowed, 1)) != cudaSuccess) return e;
+// A cluster per row, its slices in shared memory.
+__global__ void __launch_bounds__(kT, 2) staged_kernel(const __grid_constant__ Args a) {
+  grid_dependency_wait();
+  allow_dependents_launch();
+  __shared__ Shared sh;
+  extern __shared__ __align__(16) float x_s[];
+  sample_row<true>(sh, x_s, a, blockIdx.x / nctas(), nctas(), slice_of(a.n, nctas()));
+}
+
+// A CTA per light row.
+__global__ void __launch_bounds__(kT, 2) light_kernel(const __grid_constant__ Args a) {
+  grid_dependency_wait();
+  allow_dependents_launch();
+  __shared__ Shared sh;
+  extern __shared__ __align__(16) float x_s[];
+  if (light(a, blockIdx.x)) sample_row<false>(sh, x_s, a, blockIdx.x, 1, slice_of(a.n, 1));
+}
+
+// A cluster per other row, next to light_kernel: this one does not wait for that
+// to start (when it may, every CTA of that has seen what came before them
+// both), and ends after it, so that what waits for this kernel has waited for
+// both.
+__global__ void __launch_bounds__(kT, 2) wide_kernel(const __grid_constant__ Args a) {
+  allow_dependents_launch();
+  __shared__ Shared sh;
+  extern __shared__ __align__(16) float x_s[];
+  const int r = blockIdx.x / nctas();
+  if (!light(a, r)) sample_row<false>(sh, x_s, a, r, nctas(), slice_of(a.n, nctas()));
+  if (blockIdx.x == 0) grid_dependency_wait();
+}
+
+template <typename K, typename... X>
+cudaError_t launch_clusters(K k, int grid, int ctas, int smem, bool overlap, cudaStream_t st, X... x) {
   cudaLaunchAttribute attr[2];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = (unsigned)ctas;
@@ -1180,13 +1202,30 @@ cudaError_t launch(const Args& a, int64_t rows, int ctas, bool staged, cudaStrea
   attr[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
   attr[1].val.programmaticStreamSerializationAllowed = 1;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(rows * ctas));
+  cfg.gridDim = dim3((unsigned)grid);
   cfg.blockDim = dim3(kT);
-  cfg.dynamicSmemBytes = kOwnBytes + (staged ? slice * sizeof(float) : 0);
+  cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cfg.attrs = attr;
-  cfg.numAttrs = launch_overlap() ? 2 : 1;
-  return cudaLaunchKernelEx(&cfg, k, a, slice);
+  cfg.numAttrs = overlap ? 2 : 1;
+  return cudaLaunchKernelEx(&cfg, k, x...);
+}
+
+cudaError_t launch_staged(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
+  static std::atomic<uint64_t> done{0};
+  const cudaError_t e = allow_smem(staged_kernel, kMaxSlice * (int)sizeof(float) + kOwnBytes, done);
+  if (e != cudaSuccess) return e;
+  return launch_clusters(staged_kernel, (int)rows * ctas, ctas, slice_of(a.n, ctas) * (int)sizeof(float) + kOwnBytes,
+                         launch_overlap(), st, a);
+}
+
+cudaError_t launch_rows(const Args& a, int64_t rows, int ctas, cudaStream_t st) {
+  static std::atomic<uint64_t> done[2];
+  cudaError_t e = allow_smem(light_kernel, kOwnBytes, done[0]);
+  if (e == cudaSuccess) e = allow_smem(wide_kernel, kOwnBytes, done[1]);
+  if (e == cudaSuccess) e = launch_ex(light_kernel, dim3((unsigned)rows), dim3(kT), kOwnBytes, st, a);
+  if (e == cudaSuccess) e = launch_clusters(wide_kernel, (int)rows * ctas, ctas, kOwnBytes, true, st, a);
+  return e;
 }
 
 }  // namespace sample
@@ -1209,16 +1248,17 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
   const hyq::sample::Args a{logits, stride, (int)n, temperature, top_k, top_p, min_p, u, token, prob};
   const cudaStream_t st = (cudaStream_t)stream;
   // Few rows: as many CTAs per row as there are SMs for, the slices in their
-  // shared memory (256 rows of 120,832 logits cut to n; temperature 0.7, top-k
-  // 40, top-p 0.9 / mixed parameters): n = 1: 14 / 15 us with eight, 16 / 16 with
-  // four; 16: 16 / 27 us with six, 24 / 25 with eight; 32: 17 / 59 us with four,
-  // 26 / 53 with six, 30 / 59 with six from memory.  Many rows: four per row, from
-  // memory (64: 30 / 67 us, 32 / 59 staged; 128: 47 / 77 us, 58 / 94 staged; 256:
-  // 84 / 116 us; 64 / 144 with two, 94 / 137 with eight).
+  // shared memory.  Many: one per light row, four per other row, from memory.
+  // Measured at 120,832 logits (temperature 0.7, top-k 40, top-p 0.9 / mixed
+  // parameters / top-p 0.9 alone, us): 1 row 14 / 15 / 21 with eight, 16 / 16 / 24
+  // with four; 16 rows 16 / 27 / 34 with six, 24 / 25 / 46 with eight; 32 rows 17
+  // / 58 / 48 with four, 23 / 66 / 60 (48 rows) from memory; 64 rows 32 / 59 / 81
+  // staged, 23 / 72 / 61 from memory; 256 rows 123 / 162 / 259 staged, 45 / 104 /
+  // 187 from memory, 84 / 115 / 182 in one launch with idle CTAs on light rows.
   const int64_t units = (n + hyq::sample::kUnit - 1) / hyq::sample::kUnit;
   const int ctas = (int)std::min<int64_t>(rows <= 12 ? 8 : rows <= 16 ? 6 : 4, units);
   const bool staged = rows <= 32 && ctas > 1 && n <= (int64_t)ctas * hyq::sample::kMaxSlice;
-  const cudaError_t e = hyq::sample::launch(a, rows, ctas, staged, st);
+  const cudaError_t e = staged ? hyq::sample::launch_staged(a, rows, ctas, st) : hyq::sample::launch_rows(a, rows, ctas, st);
   return e == cudaSuccess ? HYQ_OK : hyq::api_fail(HYQ_E_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 

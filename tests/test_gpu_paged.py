@@ -649,3 +649,27 @@ def test_python_refusals(cuda):
     token, prob = sampling.sample(x[:0], u[:0])
     assert token.numel() == 0 and prob.numel() == 0
     assert quant.device_status() == 0
+
+
+@pytest.mark.parametrize("kv16", [True, False])
+def test_attention_launch_overlap(cuda, kv16):
+    """The chain of a call's kernels and the next call's, launched early."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant
+    s = _make(cuda, [1, 150, 3, 700], [300, 20, 70, 500], 16, 4, 128, 32, kv16, seed=5)
+    ws = paged.attention_workspace(16, 128, cuda)
+    want = _attend(s, workspace=ws).clone()
+    q = s["q"].clone()
+    out, again = torch.empty_like(want), torch.empty_like(want)
+    quant.set_launch_overlap(True)
+    try:
+        for _ in range(10):
+            s["q"].copy_(q * 2)
+            _attend(s, out=out, workspace=ws)
+            s["q"].copy_(q)
+            _attend(s, out=out, workspace=ws)
+            _attend(s, out=again, workspace=ws)
+            assert torch.equal(out, want) and torch.equal(again, want)
+    finally:
+        quant.set_launch_overlap(False)
+    assert quant.device_status() == 0

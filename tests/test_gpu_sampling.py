@@ -181,3 +181,34 @@ def test_repeats_and_streams(cuda):
     assert torch.equal(first, again)
     one = torch.cat([sampling.sample(x[i:i + 1], u[i:i + 1], 1.0, 0, 0.95)[0] for i in range(64)])
     assert torch.equal(first, one)      # a row's token does not depend on the batch
+
+
+@pytest.mark.parametrize("rows", [3, 40, 150])
+def test_launch_overlap(cuda, rows):
+    """With kernels launched before their predecessors have ended, what follows
+    a call still sees its tokens, and a call what precedes it."""
+    import torch
+    from hy_mt_rs_b200 import quant, sampling
+    g = torch.Generator(device=cuda).manual_seed(rows)
+    logits = torch.randn(rows, 30011, generator=g, device=cuda) * 3
+    u = torch.rand(rows, generator=g, device=cuda)
+    i = torch.arange(rows, device=cuda)
+    temperature = torch.tensor([0.0, 0.8, 1.2, 1.0], device=cuda)[i % 4]
+    top_k = torch.tensor([0, 40, 500], dtype=torch.int32, device=cuda)[i % 3]
+    top_p = torch.tensor([1.0, 0.9], device=cuda)[i % 2]
+    want, _ = sampling.sample(logits, u, temperature, top_k, top_p)
+    second, _ = sampling.sample(logits.roll(1, 0).contiguous(), u, temperature, top_k, top_p)
+    x, token, again = torch.empty_like(logits), torch.empty_like(want), torch.empty_like(want)
+    quant.set_launch_overlap(True)
+    try:
+        for _ in range(10):
+            token.fill_(-1)
+            x.copy_(logits)
+            sampling.sample(x, u, temperature, top_k, top_p, token=token)
+            sampling.sample(x, u, temperature, top_k, top_p, token=again)
+            x.copy_(logits.roll(1, 0))
+            assert torch.equal(token, want) and torch.equal(again, want)
+            sampling.sample(x, u, temperature, top_k, top_p, token=token)
+            assert torch.equal(token, second)
+    finally:
+        quant.set_launch_overlap(False)
