@@ -454,9 +454,10 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
     cudaError_t e = cudaSuccess;
     const bool more = batch->max_new * (heads / kv->kv_heads) > hyq::paged::kFewRows;
     if (more)
-      e = kv16 && hyq::paged::tc_supported(a, kv16)  ? hyq::paged::launch_chunks_tc(a, st)
-          : !kv16 && hyq::paged::tc32_supported(a) ? hyq::paged::launch_chunks_tc32(a, st)
-                                                   : hyq::paged::launch_chunks(a, kv16, st);
+      e = hyq::paged::chunks_short(a, kv16, batch->max_len) ? hyq::paged::launch_chunks(a, kv16, st)
+          : kv16 && hyq::paged::tc_supported(a, kv16)       ? hyq::paged::launch_chunks_tc(a, st)
+          : !kv16 && hyq::paged::tc32_supported(a)          ? hyq::paged::launch_chunks_tc32(a, st)
+                                                            : hyq::paged::launch_chunks(a, kv16, st);
     if (e == cudaSuccess) e = hyq::paged::launch_few(a, kv16, more, st);
     return done(e, name);
   }

@@ -829,6 +829,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
   }
 }
 
+int64_t chunk_tiles(const AttendArgs& a) {
+  return ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + kChunkRows - 1) / kChunkRows + a.c.seqs;
+}
+
 int page_shift(const AttendArgs& a) {
   return (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.c.page_size) : -1;
 }
@@ -836,7 +840,7 @@ int page_shift(const AttendArgs& a) {
 template <int DIM, bool KV16>
 cudaError_t chunks(const AttendArgs& a, cudaStream_t st) {
   using G = Geo<DIM, KV16>;
-  const int64_t tiles = ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + kChunkRows - 1) / kChunkRows + a.c.seqs;
+  const int64_t tiles = chunk_tiles(a);
   auto k = chunk_kernel<DIM, KV16>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(k, G::smem, done);
@@ -861,6 +865,12 @@ bool mma_supported(const AttendArgs& a, bool kv16) {
   const int64_t strides = (a.c.page_stride | a.c.head_stride | a.c.row_stride) * (kv16 ? 2 : 4);
   return (a.c.dim == 64 || a.c.dim == 128) && strides % 16 == 0 &&
          (reinterpret_cast<uintptr_t>(a.c.k) | reinterpret_cast<uintptr_t>(a.c.v)) % 16 == 0;
+}
+
+bool chunks_short(const AttendArgs& a, bool kv16, int64_t max_len) {
+  const int64_t tiles = (chunk_tiles(a) - a.c.seqs / 2) * a.c.kv_heads;  // sequences' last tiles are half full
+  const int64_t rounds = (tiles + kMaxCtas - 1) / kMaxCtas;
+  return rounds * max_len <= (kv16 ? 350 : 64);
 }
 
 size_t mma_workspace_bytes(int dim) { return kCounterBytes + 2 * (size_t)kMaxCtas * partial_floats(dim) * sizeof(float); }
