@@ -18,7 +18,8 @@
 //                undone in its column of scores; V one for the tile, known
 //                when all warps have seen their part, undone in X;
 //   warp 12      the products S, into two buffers in turn;
-//   warp 13      the products X.
+//   warp 13      the products X, likewise: a tile's is added to the outputs while
+//                the next tile's weights are multiplied.
 //
 // A tile with an infinity or NaN, or whose positions' largest values of V are
 // more than 2^14 apart, is left out of the products (V and the weights are
@@ -44,8 +45,8 @@ struct Smem {
   static constexpr int scale = 6 * tile;                 // [2][128]: 2^-n of K's positions
   static constexpr int top = scale + 2 * kTile * 4;      // [2][8 warps] largest, smallest bits of V
   static constexpr int bars = top + 2 * kSplitWarps * 8;
-  // k_full, v_full, v_top, p_full, x_full, s_full[2]
-  static constexpr int n_bars = 7;
+  // k_full, v_full, v_top, p_full, s_full[2], x_full[2]
+  static constexpr int n_bars = 8;
   // tensor memory address, abort, unused, then [2] of: tile that is left
   // out (its number + 1), scale of X
   static constexpr int misc = bars + 8 * n_bars;
@@ -96,14 +97,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
   using L = Smem<DIM>;
   constexpr int KS = DIM / 16;            // steps of 16 along the head
   constexpr int N = DIM / 32;             // values of a lane
-  constexpr uint32_t kTmemCols = 512;     // S and P twice 128, X
+  constexpr uint32_t kTmemCols = 512;     // S and P twice 128, X twice 128
   const AttendArgs& a = p.a;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* base_g = smem_raw + (base - raw);
-  const uint32_t k_full = base + L::bars, v_full = k_full + 8, v_top = k_full + 16, p_full = k_full + 24,
-                 x_full = k_full + 32;
-  auto s_full = [&](int i) { return k_full + 40 + 8 * (i & 1); };  // tile i: phase i / 2
+  const uint32_t k_full = base + L::bars, v_full = k_full + 8, v_top = k_full + 16, p_full = k_full + 24;
+  auto s_full = [&](int i) { return k_full + 32 + 8 * (i & 1); };  // of tile i: phase i / 2
+  auto x_full = [&](int i) { return k_full + 48 + 8 * (i & 1); };
   float* scale_s = reinterpret_cast<float*>(base_g + L::scale);
   volatile int* misc = reinterpret_cast<volatile int*>(base_g + L::misc);
   volatile int* abort_flag = misc + 1;
@@ -127,9 +128,10 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       mbar_init(v_full, kSplitWarps);
       mbar_init(v_top, kSplitWarps);
       mbar_init(p_full, 4);
-      mbar_init(x_full, 1);
-      mbar_init(s_full(0), 1);
-      mbar_init(s_full(1), 1);
+      for (int i = 0; i < 2; ++i) {
+        mbar_init(s_full(i), 1);
+        mbar_init(x_full(i), 1);
+      }
       mbar_fence_init();
     }
   }
@@ -192,9 +194,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
           for (int h = 0; h < 3; ++h)
 #pragma unroll
             for (int s = 0; s < kTile / 16; ++s)  // 16 positions: hi in 8 columns from 16 s, lo in the next 8
-              mma_ts(tmem + 256, pw + 16 * s + (h == 0 ? 8 : 0), v + (h == 1 ? L::tile >> 4 : 0) + s * (16 * 128 >> 4), idesc_o,
+              mma_ts(tmem + 256 + 128 * (i & 1), pw + 16 * s + (h == 0 ? 8 : 0), v + (h == 1 ? L::tile >> 4 : 0) + s * (16 * 128 >> 4), idesc_o,
                      h > 0 || s > 0);
-          commit(x_full);
+          commit(x_full(i));
         }
         __syncwarp();
       }
@@ -221,15 +223,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       const float* row = static_cast<const float*>(from) + o + N * lane;
 #pragma unroll
       for (int k = 0; k < N; ++k) v[k] = 0.f;
-      if (o >= 0) {
-        if constexpr (N == 4) {
-          const float4 f = *reinterpret_cast<const float4*>(row);
-          v[0] = f.x, v[1] = f.y, v[2] = f.z, v[3] = f.w;
-        } else {
-          const float2 f = *reinterpret_cast<const float2*>(row);
-          v[0] = f.x, v[1] = f.y;
-        }
-      }
+      // (predicated, not branched around: branches would keep the rows apart)
+      if constexpr (N == 4)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.s64 p, %4, 0;\n\t@p ld.global.v4.f32 {%0, %1, %2, %3}, [%5];\n\t}"
+                     : "+f"(v[0]), "+f"(v[1]), "+f"(v[N - 2]), "+f"(v[N - 1])
+                     : "l"(o), "l"(row));
+      else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.s64 p, %2, 0;\n\t@p ld.global.v2.f32 {%0, %1}, [%3];\n\t}"
+                     : "+f"(v[0]), "+f"(v[1])
+                     : "l"(o), "l"(row));
     };
     float kr[kPart / 2][N], vr[kPart][N];
     int64_t here = place(), there = -1;
@@ -251,14 +253,17 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       }
       if (i > 0 && !wait(s_full(i - 1), (i - 1) >> 1)) break;
       auto put_keys = [&](int r0) {
+        uint32_t top[kPart / 2], own = 0;  // own: of row r0 + lane
 #pragma unroll
         for (int r = 0; r < kPart / 2; ++r) {
-          const uint32_t top = row_top(kr[r]);
-          if (lane == 0) {
-            scale_s[(i & 1) * kTile + row0 + r0 + r] = unscale_of(top);
-            if (top >= 0x7f800000u) out_s[i & 1] = i + 1;
-          }
-          put_row<DIM>(k_s, row0 + r0 + r, kr[r], scale_of(top));
+          top[r] = row_top(kr[r]);
+          own = lane == r ? top[r] : own;
+        }
+#pragma unroll
+        for (int r = 0; r < kPart / 2; ++r) put_row<DIM>(k_s, row0 + r0 + r, kr[r], scale_of(top[r]));
+        if (lane < kPart / 2) {
+          scale_s[(i & 1) * kTile + row0 + r0 + lane] = unscale_of(own);
+          if (own >= 0x7f800000u) out_s[i & 1] = i + 1;
         }
       };
       put_keys(0);
@@ -294,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       if (lane == 0) mbar_arrive(k_full);
 #pragma unroll
       for (int r = 0; r < kPart / 2; ++r) load(kr[r], a.c.k, there, r);
-      if (i > 0 && !wait(x_full, i - 1)) break;
+      if (i > 0 && !wait(x_full(i - 1), (i - 1) >> 1)) break;
       if (out) {
 #pragma unroll
         for (int r = 0; r < kPart; ++r)
@@ -328,25 +333,28 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
 #pragma unroll
       for (int d = 0; d < DIM; ++d) o[d] = 0.f;
       float m = -INFINITY, l = 0.f, down = 1.f, back = 1.f;
-      // the product of the tile before, added to the row's outputs
-      auto collect = [&]() {
-        if (!wait(x_full, i - 1)) return;
+      // the product of tile i - 1, which was weighed with `down` and `back`,
+      // added to the row's outputs
+      auto collect = [&](float down, float back) {
+        if (!wait(x_full(i - 1), (i - 1) >> 1)) return;
         fence_after();
-        tmem_each<DIM>(tmem + lanes + 256, [&](float (&v)[16], int c) {
+        tmem_each<DIM>(tmem + lanes + 256 + 128 * ((i - 1) & 1), [&](float (&v)[16], int c) {
 #pragma unroll
           for (int k = 0; k < 16; ++k) o[c + k] = fmaf(v[k], back, o[c + k] * down);
         });
       };
       for (int j = 0; j < x.nt; ++j, ++i) {
-        if (j > 0) collect();
         // (the second: this warp has part in that phase, and reads what came with it)
         if (!wait(s_full(i), i >> 1) || !wait(k_full, i)) break;
         fence_after();
         if (j + 1 < x.nt && lane == 0) mbar_arrive(k_full);  // the next tile's queries are there
         const uint32_t st = tmem + lanes + 128 * (i & 1);
         const int p0 = (x.j0 + j) * kTile;
+        const float before_down = down, before_back = back;
+        const bool out = uniform(out_s[i & 1]) == i + 1;
         back = back_s[i & 1];
-        if (uniform(out_s[i & 1]) == i + 1) {
+        if (out) {
+          if (j > 0) collect(before_down, before_back);
           constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;
           const float* q = a.q + (int64_t)(x.s.row0 + tok) * a.q_stride + (int64_t)(x.kvh * group + r % group) * DIM;
 #pragma unroll 1
@@ -403,8 +411,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full);
+        if (j > 0 && !out) collect(before_down, before_back);
       }
-      if (ok) collect();
+      if (ok) collect(down, back);
       if (!ok) break;
       store_rows<DIM, kRows, false>(p, x, group, cta, second, r, base_g + L::q, o, m, l, false);
     }
