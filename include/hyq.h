@@ -445,7 +445,8 @@ int hyq_argmax(const float* x, int64_t n, int32_t* token, int32_t* pos, int pos_
  *   (none is allowed), at positions pos[s], pos[s] + 1, ...; its table row is
  *   slot[s], or s when slot is NULL.  `tokens` is the number of rows of the
  *   activations (rows outside every sequence are left alone), max_new bounds
- *   any sequence's new tokens and max_len any pos[s] + new tokens.
+ *   any sequence's new tokens and max_len any pos[s] + new tokens (the closer,
+ *   the better the choice of kernels).  At most 4096 sequences.
  * A sequence whose table row, pages or positions are out of range is skipped
  * and raises HYQ_DEV_BAD_ARGS (see hyq_device_status). */
 #define HYQ_KV_F32 0
@@ -486,7 +487,8 @@ int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, 
  * pages already.  out [tokens, heads, head_dim], rows out_stride floats apart.
  * f32 accuracy over either cache type.  Values past a token's position (page
  * tails, later tokens of its chunk) never reach its output, whatever they
- * hold.  head_dim at most 256, at most 16 query heads per kv head.
+ * hold.  head_dim at most 256, at most 16 query heads per kv head.  (Outputs
+ * are kept 2^10 times their size inside: values from 2^113 up overflow.)
  * workspace: hyq_paged_attention_workspace_bytes bytes (independent of the
  * batch), 16-byte aligned, zero before the first call (every call leaves its
  * counters zero again); calls that share one must not overlap in time. */
@@ -554,7 +556,7 @@ int hyq_pages_compact(const hyq_pages* p, const hyq_page_pool* pool, void* works
  * steps of 2^-24, so the token does not depend on the order of summation.
  * prob (may be NULL): the token's share of the kept weights.  NaN logits
  * count as -inf; a row without a logit above -inf gives token 0, prob 0;
- * logits of +inf share the whole weight. */
+ * logits of +inf share the whole weight.  n is below 2^23. */
 int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, const float* temperature,
                const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
                float* prob, void* stream);

@@ -673,3 +673,38 @@ def test_attention_launch_overlap(cuda, kv16):
     finally:
         quant.set_launch_overlap(False)
     assert quant.device_status() == 0
+
+
+@pytest.mark.parametrize("dim", [128, 64])
+@pytest.mark.parametrize("keys,values", [(0, 6), (10, 0), (10, 20), (0, 40)])
+def test_attention_positions_of_different_sizes(cuda, dim, keys, values):
+    """An f32 cache whose positions differ by powers of two: keys and values
+    are split after a scale for each position or tile, which must lose nothing
+    (the bound is relative to each row's own sum of p |v|)."""
+    import torch
+    s = _make(cuda, [200, 3, 40], [150, 100, 300], 8, 2, dim, 32, False, seed=keys + values)
+    g = torch.Generator(device=cuda).manual_seed(1)
+    size = s["k"].shape[0], 1, s["k"].shape[2], 1
+    up = torch.randint(-keys, keys + 1, size, generator=g, device=cuda).float()
+    s["k"] *= torch.exp2(up - keys)         # scores stay of ordinary size
+    s["v"] *= torch.exp2(torch.randint(-values, values + 1, size, generator=g, device=cuda).float())
+    got = _attend(s)
+    ref, tol = _reference(s)
+    err = (got.double() - ref).abs()
+    assert (err <= tol).all(), float((err / tol).max())
+
+
+@pytest.mark.parametrize("kv16,huge", [(True, 65504.0), (False, 1e30)])
+def test_attention_huge_later_token(cuda, kv16, huge):
+    """A finite, huge key and value of a later token leaves the tokens before it
+    as they were."""
+    s = _make(cuda, [200], [50], 8, 2, 128, 32, kv16, seed=9)
+    clean = dict(s, k=s["k"].clone(), v=s["v"].clone())
+    p = 50 + 133
+    page = int(s["table"][0, p // 32])
+    s["k"][page, :, p % 32] = -huge
+    s["v"][page, :, p % 32] = huge
+    got = _attend(s)
+    ref, tol = _reference(clean)
+    assert ((got[:133].double() - ref[:133]).abs() <= tol[:133]).all()
+    assert got.isfinite().all()
