@@ -454,14 +454,16 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
   const cudaStream_t st = (cudaStream_t)stream;
   const bool kv16 = kv->dtype == HYQ_KV_F16;
   if (hyq::paged::mma_supported(a, kv16)) {
-    cudaError_t e = cudaSuccess;
-    const bool more = batch->max_new * (heads / kv->kv_heads) > hyq::paged::kFewRows;
-    if (more)
-      e = hyq::paged::chunks_short(a, kv16, batch->max_len) ? hyq::paged::launch_chunks(a, kv16, st)
-          : kv16 && hyq::paged::tc_supported(a, kv16)       ? hyq::paged::launch_chunks_tc(a, st)
-          : !kv16 && hyq::paged::tc32_supported(a)          ? hyq::paged::launch_chunks_tc32(a, st)
-                                                            : hyq::paged::launch_chunks(a, kv16, st);
-    if (e == cudaSuccess) e = hyq::paged::launch_few(a, kv16, more, st);
+    cudaError_t e;
+    if (batch->max_new * (heads / kv->kv_heads) <= hyq::paged::kFewRows) {
+      e = hyq::paged::launch_few(a, kv16, false, st);
+    } else if (hyq::paged::chunks_short(a, kv16, batch->max_len) ||
+               !(kv16 ? hyq::paged::tc_supported(a) : hyq::paged::tc32_supported(a))) {
+      e = hyq::paged::launch_chunks(a, kv16, st);
+      if (e == cudaSuccess) e = hyq::paged::launch_few(a, kv16, true, st);
+    } else {
+      e = kv16 ? hyq::paged::launch_chunks_tc(a, st) : hyq::paged::launch_chunks_tc32(a, st);
+    }
     return done(e, name);
   }
   return done(kv16 ? hyq::paged::launch_attend<true>(a, st) : hyq::paged::launch_attend<false>(a, st), name);

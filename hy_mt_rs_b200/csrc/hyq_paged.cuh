@@ -135,8 +135,9 @@ constexpr int kMaxSeqs = 4096;
 // hyq_paged_mma.cu: head sizes 64 and 128 over 16-byte aligned rows.
 bool mma_supported(const AttendArgs& a, bool kv16);
 size_t mma_workspace_bytes(int dim);
-// Sequences of up to kFewRows rows; `next`: after the launch of the others.
-cudaError_t launch_few(const AttendArgs& a, bool kv16, bool next, cudaStream_t st);
+// Sequences of up to kFewRows rows; `beside`: next to the kernel that the same
+// call launched before.
+cudaError_t launch_few(const AttendArgs& a, bool kv16, bool beside, cudaStream_t st);
 cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st);  // the others
 // Whether that is faster than the kernels on tcgen05: one launch instead of
 // three, but every CTA goes through its rows' positions alone, at 0.04 us (f16
@@ -147,8 +148,8 @@ cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st);  // 
 // 21; 8 tokens at 100, 8 sequences 29 / 22.
 bool chunks_short(const AttendArgs& a, bool kv16, int64_t max_len);
 // hyq_paged_tc.cu: the others on tcgen05 (f16 caches; the workspace past
-// mma_workspace_bytes).
-bool tc_supported(const AttendArgs& a, bool kv16);
+// mma_workspace_bytes), and launch_few beside their first kernel.
+bool tc_supported(const AttendArgs& a);
 size_t tc_workspace_bytes(int dim);
 cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st);
 // hyq_paged_tc32.cu: the same over f32 caches, in the same workspace.

@@ -451,10 +451,13 @@ constexpr int kSegmentCost = 4;
 // that is).  Within a tile each warp takes its own POS positions for all 16
 // rows, through its own ring of asynchronous copies; the warps meet at the
 // end of a segment.
+// `beside`: the kernel before is the same call's and has nothing that this one
+// reads: it starts without waiting for that (when it may, every CTA of that has
+// seen what came before them both), and ends after it.
 template <int DIM, bool KV16>
-__global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_constant__ AttendArgs a, int shift) {
+__global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_constant__ AttendArgs a, int shift, bool beside) {
   using G = Geo<DIM, KV16>;
-  grid_dependency_wait();
+  if (!beside) grid_dependency_wait();
   allow_dependents_launch();
   extern __shared__ __align__(1024) char smem[];
   int* first_s = reinterpret_cast<int*>(smem + G::smem);  // [seqs + 1] tiles (of one kv head) before each sequence
@@ -495,7 +498,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
   __syncthreads();
   const int64_t work = (int64_t)carry * kvh_n;
   const int ctas = (int)min((int64_t)gridDim.x, work), cta = blockIdx.x;
-  if (cta >= ctas) return;
+  if (cta >= ctas) {
+    if (beside && cta == 0) grid_dependency_wait();
+    return;
+  }
   int64_t at = work * cta / ctas;
   const int64_t end = work * (cta + 1) / ctas;
   const int64_t begin = at;
@@ -721,6 +727,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     }
     __syncthreads();  // o_s and ml_s are free again
   }
+  if (beside && cta == 0) grid_dependency_wait();
 }
 
 // ---------------------------------------------------------------------------
@@ -858,14 +865,14 @@ cudaError_t chunks(const AttendArgs& a, cudaStream_t st) {
 }
 
 template <int DIM, bool KV16>
-cudaError_t few(const AttendArgs& a, bool next, cudaStream_t st) {
+cudaError_t few(const AttendArgs& a, bool beside, cudaStream_t st) {
   using G = Geo<DIM, KV16>;
   auto k = few_kernel<DIM, KV16>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(k, G::smem + (kMaxSeqs + 1) * 4, done);
   if (e != cudaSuccess) return e;
-  return launch_dependent(next || launch_overlap(), k, dim3(kMaxCtas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4, st,
-                          a, page_shift(a));
+  return launch_dependent(beside || launch_overlap(), k, dim3(kMaxCtas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4, st,
+                          a, page_shift(a), beside);
 }
 
 }  // namespace
@@ -884,9 +891,9 @@ bool chunks_short(const AttendArgs& a, bool kv16, int64_t max_len) {
 
 size_t mma_workspace_bytes(int dim) { return kCounterBytes + 2 * (size_t)kMaxCtas * partial_floats(dim) * sizeof(float); }
 
-cudaError_t launch_few(const AttendArgs& a, bool kv16, bool next, cudaStream_t st) {
-  if (a.c.dim == 128) return kv16 ? few<128, true>(a, next, st) : few<128, false>(a, next, st);
-  return kv16 ? few<64, true>(a, next, st) : few<64, false>(a, next, st);
+cudaError_t launch_few(const AttendArgs& a, bool kv16, bool beside, cudaStream_t st) {
+  if (a.c.dim == 128) return kv16 ? few<128, true>(a, beside, st) : few<128, false>(a, beside, st);
+  return kv16 ? few<64, true>(a, beside, st) : few<64, false>(a, beside, st);
 }
 
 cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st) {

@@ -423,6 +423,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
   if (e == cudaSuccess) e = launch_ex(plan_kernel<kCtaRows>, dim3(1), dim3(1024), 0, st, a, p.plan);
+  if (e == cudaSuccess) e = launch_few(a, true, true, st);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
   if (e == cudaSuccess) e = launch_next(join_kernel<DIM, kCtaRows, true>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p);
   return e;
@@ -430,10 +431,10 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-bool tc_supported(const AttendArgs& a, bool kv16) {
+bool tc_supported(const AttendArgs& a) {
   const int ps = a.c.page_size;
   const int64_t segs = ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + kCtaRows - 1) / kCtaRows + a.c.seqs;
-  return kv16 && (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) && segs <= kMaxSegs && encode_fn() != nullptr;
+  return (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) && segs <= kMaxSegs && encode_fn() != nullptr;
 }
 
 size_t tc_workspace_bytes(int dim) { return kPlanBytes + kMaxParts * part_floats<kCtaRows>(dim) * sizeof(float); }
