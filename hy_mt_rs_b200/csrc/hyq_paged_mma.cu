@@ -9,7 +9,7 @@
 // lo.lo is left out: three products each.  The tensor cores cut their sums
 // instead of rounding them, which over a long context adds up (8e-6 at 1,100
 // positions), so each block's output is added to the running one in f32
-// arithmetic.  Weights are 2^(x - m): the scores carry log2(e) through the
+// arithmetic, and within a block small products go first.  Weights are 2^(x - m): the scores carry log2(e) through the
 // queries.
 //
 // Few tokens, bound by memory: 64 requests of 90 to 4,000 positions (16 query
@@ -247,7 +247,8 @@ struct Rows {
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[n][j] = (s[n][j] + lo[n][j]) * factor[j >> 1];
     } else {
-      float lo[4] = {0.f, 0.f, 0.f, 0.f}, lo2[4] = {0.f, 0.f, 0.f, 0.f};
+      // (the large products in two sums: half as many cut additions in each)
+      float lo[4] = {}, lo2[4] = {}, odd[4] = {};
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[0][j] = 0.f;
 #pragma unroll
@@ -262,13 +263,13 @@ struct Rows {
           for (int j = 0; j < 4; ++j) split_tf32(qf[2 * k + h][j], qh_[j], ql_[j]);
 #pragma unroll
           for (int j = 0; j < 2; ++j) split_tf32(__uint_as_float(b[2 * h + j]), bh[j], bl[j]);
-          mma_tf32(s[0], qh_, bh[0], bh[1]);
+          mma_tf32(h ? odd : s[0], qh_, bh[0], bh[1]);
           mma_tf32(lo, qh_, bl[0], bl[1]);
           mma_tf32(lo2, ql_, bh[0], bh[1]);
         }
       }
 #pragma unroll
-      for (int j = 0; j < 4; ++j) s[0][j] += lo[j] + lo2[j];
+      for (int j = 0; j < 4; ++j) s[0][j] += odd[j] + (lo[j] + lo2[j]);
     }
     if (masked) {
 #pragma unroll
@@ -315,10 +316,10 @@ struct Rows {
         uint32_t b[4];
         ldsm4_t(b, v_s + row * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4));
         float x[2][4] = {};
-        mma_f16(x[0], ph, b[0], b[1]);
-        mma_f16(x[1], ph, b[2], b[3]);
         mma_f16(x[0], pl, b[0], b[1]);
         mma_f16(x[1], pl, b[2], b[3]);
+        mma_f16(x[0], ph, b[0], b[1]);
+        mma_f16(x[1], ph, b[2], b[3]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
           o[2 * d][j] = fmaf(o[2 * d][j], down[j >> 1], x[0][j]);
@@ -347,9 +348,9 @@ struct Rows {
           split_tf32(y, bh[j], bl[j]);
         }
         float x[4] = {};
-        mma_tf32(x, ph, bh[0], bh[1]);
         mma_tf32(x, ph, bl[0], bl[1]);
         mma_tf32(x, pl, bh[0], bh[1]);
+        mma_tf32(x, ph, bh[0], bh[1]);
 #pragma unroll
         for (int j = 0; j < 4; ++j) o[d][j] = fmaf(o[d][j], down[j >> 1], x[j]);
       }
