@@ -436,9 +436,10 @@ struct Feed {
 // ---------------------------------------------------------------------------
 
 // Workspace: one counter per CTA, then two partial results per CTA: 16 rows of
-// DIM outputs, then the rows' (maximum, sum).
+// DIM outputs, then the rows' (maximum, sum), then whether clean() took a value
+// out.
 constexpr size_t kCounterBytes = (kMaxCtas * sizeof(unsigned) + 255) / 256 * 256;
-__host__ __device__ constexpr int partial_floats(int dim) { return kRows * (dim + 2); }
+__host__ __device__ constexpr int partial_floats(int dim) { return kRows * (dim + 2) + 4; }
 
 // What a segment costs beside its tiles (queries, first copies, joining the
 // warps), in tiles: the time of about four at full bandwidth.
@@ -466,6 +467,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
   __shared__ float factor_s[kRows];
   __shared__ int warp_s[kWarps];
   __shared__ int last_s;
+  __shared__ int dirty_s;  // the last piece (of this CTA's) that clean() took a value out of
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int group = a.heads / a.c.kv_heads, seqs = a.c.seqs, kvh_n = a.c.kv_heads;
   // prefix sum of the sequences' tiles; sequences with more rows are the
@@ -495,7 +497,10 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     if (i < seqs) first_s[i] = before + x - tiles;
     __syncthreads();
   }
-  if (threadIdx.x == 0) first_s[seqs] = carry;
+  if (threadIdx.x == 0) {
+    first_s[seqs] = carry;
+    dirty_s = 0;
+  }
   __syncthreads();
   const int64_t work = (int64_t)carry * kvh_n;
   const int ctas = (int)min((int64_t)gridDim.x, work), cta = blockIdx.x;
@@ -563,7 +568,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     }
   };
   open(false);
-  while (at < end) {
+  for (int piece = 1; at < end; ++piece) {
     {
       const Seq& s = cur.s;
       const uint32_t q_s = smem_addr(o_s);
@@ -586,7 +591,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
         __syncwarp();
         const int p0 = j * G::tile + off;
         const bool masked = p0 + G::pos - 1 > s.pos;
-        if (masked) feed.clean(ring + stage * G::block, p0, s.pos);
+        if (masked && feed.clean(ring + stage * G::block, p0, s.pos)) dirty_s = piece;
         rows.step(ring + stage * G::block, p0, masked);
         if (++stage == G::stages) stage = 0;
       }
@@ -637,7 +642,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
       }
       __syncthreads();
     }
-    const bool whole = done.j0 == 0 && done.j1 == done.tiles;
+    const bool whole = done.j0 == 0 && done.j1 == done.tiles, dirty = dirty_s == piece;
     float* part = parts + (size_t)(2 * cta + second) * partial_floats(DIM);
     constexpr int N = DIM / 32;  // values per lane, a warp per row
     for (int r = warp; r < live; r += kWarps) {
@@ -656,7 +661,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
         for (int k = 0; k < N; ++k) {
           const int d = lane + 32 * k;
           float y = from[d] * inv;
-          if (s.n > 1) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
+          if (dirty) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
           to[d] = y;
         }
       } else {
@@ -669,6 +674,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
       }
     }
     if (!whole) {
+      if (s.n > 1 && threadIdx.x == 0) part[kRows * (DIM + 2)] = dirty ? 1.0f : 0.0f;
       // the CTAs that share the segment: cf holds its first tile, cl its last
       const int64_t seg0 = done.seg0, seg1 = seg0 + done.tiles;
       int cf = (int)(seg0 * ctas / work);
@@ -691,6 +697,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
         const float* part0 = parts + (size_t)(2 * cf + (work * cf / ctas < seg0)) * partial_floats(DIM);
         const float* part1 = parts + (size_t)(2 * cf) * partial_floats(DIM);
         auto part_at = [&](int i) { return i ? part1 + (size_t)(2 * i) * partial_floats(DIM) : part0; };
+        bool any = false;  // a piece was dirty
+        for (int i = lane; s.n > 1 && i < n; i += 32) any = any || __ldcg(part_at(i) + kRows * (DIM + 2)) != 0.f;
+        any = __any_sync(0xffffffffu, any);
         for (int r = warp; r < live; r += kWarps) {
           float top = -INFINITY, l = 0.f, sum[N] = {};
           for (int i = lane; i < n; i += 32) top = fmaxf(top, __ldcg(part_at(i) + kRows * DIM + 2 * r));
@@ -719,7 +728,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
           for (int k = 0; k < N; ++k) {
             const int d = lane + 32 * k;
             float y = sum[k] * inv;
-            if (s.n > 1) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
+            if (any) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
             to[d] = y;
           }
         }

@@ -708,3 +708,20 @@ def test_attention_huge_later_token(cuda, kv16, huge):
     ref, tol = _reference(clean)
     assert ((got[:133].double() - ref[:133]).abs() <= tol[:133]).all()
     assert got.isfinite().all()
+
+
+@pytest.mark.parametrize("kv16", [True, False])
+@pytest.mark.parametrize("new,ctx,at", [(3, 1500, 1), (4, 700, 3), (2, 3000, 0)])
+def test_attention_few_later_tokens_do_not_leak(cuda, new, ctx, at, kv16):
+    """The same where a sequence's positions are split over many CTAs: an
+    infinity in a new token's values reaches it and the later ones only."""
+    s = _make(cuda, [1, new, 2], [900, ctx, 40], 8, 2, 128, 32, kv16, seed=at)
+    clean = dict(s, k=s["k"].clone(), v=s["v"].clone())
+    p = ctx + at
+    s["v"][int(s["table"][1, p // 32]), :, p % 32, 77] = float("inf")
+    got = _attend(s)
+    ref, tol = _reference(clean)
+    rows = list(range(1 + at, 1 + new))           # of sequence 1, from that token on
+    ok = (got.double() - ref).abs() <= tol
+    ok[rows, :, 77] = ~got[rows, :, 77].isfinite()
+    assert ok.all()
