@@ -24,13 +24,15 @@ class PagedBatch:
     (either architecture; the cache type and the products' precision are the
     model's).
 
-    slots: requests at a time.  They share `pages` pages of page_size
+    slots: requests at a time, at most 1024.  They share `pages` pages of page_size
     positions (by default enough for every slot to reach cfg.positions).
     chunk: prompt tokens that generate() feeds in a step, next to the tokens of
     the requests that decode already."""
 
     def __init__(self, model, slots, pages=None, page_size=64, chunk=256):
         cfg, dev = model.cfg, model.device
+        if not 1 <= slots <= 1024:
+            raise ValueError("1 to 1024 slots")
         self.m, self.slots, self.chunk = model, slots, chunk
         width = -(-cfg.positions // page_size)
         self.cache = paged.PagedCache(len(model.layers), cfg.kv_heads, cfg.head_dim, pages or slots * width, page_size,
