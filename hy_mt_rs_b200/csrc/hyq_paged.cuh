@@ -148,7 +148,7 @@ cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st);  // 
 // 21; 8 tokens at 100, 8 sequences 29 / 22.
 bool chunks_short(const AttendArgs& a, bool kv16, int64_t max_len);
 // hyq_paged_tc.cu: the others on tcgen05 (f16 caches; the workspace past
-// mma_workspace_bytes), and launch_few beside their first kernel.
+// mma_workspace_bytes), and launch_few beside them.
 bool tc_supported(const AttendArgs& a);
 size_t tc_workspace_bytes(int dim);
 cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st);

@@ -447,8 +447,8 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
   if (e == cudaSuccess) e = launch_ex(plan_kernel<kRows>, dim3(1), dim3(1024), 0, st, a, p.plan);
-  if (e == cudaSuccess) e = launch_few(a, false, true, st);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
+  if (e == cudaSuccess) e = launch_few(a, false, true, st);
   if (e == cudaSuccess)
     e = launch_next(join_kernel<DIM, kRows, false>, dim3(kMaxCtas, kRows / kJoinRows), dim3(256), 0, st, p);
   return e;
