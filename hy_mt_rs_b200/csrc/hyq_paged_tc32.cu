@@ -50,8 +50,8 @@ struct Smem {
   static constexpr int scale = 6 * tile;                 // [2][128]: 2^-n of K's positions
   static constexpr int top = scale + 2 * kTile * 4;      // [2][8 warps] largest, smallest bits of V
   static constexpr int bars = top + 2 * kSplitWarps * 8;
-  // k_full, v_full, v_top, p_full, s_full[2], x_full[2]
-  static constexpr int n_bars = 8;
+  // k_full, v_full, v_top, p_full[2], s_full[2], x_full[2]
+  static constexpr int n_bars = 9;
   // tensor memory address, abort, unused, then [2] of: tile that is left
   // out (its number + 1), scale of X
   static constexpr int misc = bars + 8 * n_bars;
@@ -107,9 +107,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   const uint32_t raw = smem_addr(smem_raw), base = (raw + 1023u) & ~1023u;
   uint8_t* base_g = smem_raw + (base - raw);
-  const uint32_t k_full = base + L::bars, v_full = k_full + 8, v_top = k_full + 16, p_full = k_full + 24;
-  auto s_full = [&](int i) { return k_full + 32 + 8 * (i & 1); };  // of tile i: phase i / 2
-  auto x_full = [&](int i) { return k_full + 48 + 8 * (i & 1); };
+  const uint32_t k_full = base + L::bars, v_full = k_full + 8, v_top = k_full + 16;
+  // Of tile i: phase i / 2.  (Two of p_full as well: a softmax warp may be done
+  // with tile i + 1 before another is with i, and its arrival must not count for
+  // i; with i + 2 it is done only after X(i), which takes all of i's.)
+  auto p_full = [&](int i) { return k_full + 24 + 8 * (i & 1); };
+  auto s_full = [&](int i) { return k_full + 40 + 8 * (i & 1); };
+  auto x_full = [&](int i) { return k_full + 56 + 8 * (i & 1); };
   float* scale_s = reinterpret_cast<float*>(base_g + L::scale);
   volatile int* misc = reinterpret_cast<volatile int*>(base_g + L::misc);
   volatile int* abort_flag = misc + 1;
@@ -132,8 +136,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       mbar_init(k_full, kSplitWarps + 4);  // K is there, and the queries: the softmax warps
       mbar_init(v_full, kSplitWarps);
       mbar_init(v_top, kSplitWarps);
-      mbar_init(p_full, 4);
       for (int i = 0; i < 2; ++i) {
+        mbar_init(p_full(i), 4);
         mbar_init(s_full(i), 1);
         mbar_init(x_full(i), 1);
       }
@@ -191,7 +195,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       }
     } else if (warp == 13) {
       const uint64_t v = desc_mn_major(base + L::v, L::half);
-      for (int i = 0; i < tiles && wait(v_full, i) && wait(p_full, i); ++i) {
+      for (int i = 0; i < tiles && wait(v_full, i) && wait(p_full(i), i >> 1); ++i) {
         fence_after();
         if (one) {
           const uint32_t pw = tmem + 128 * (i & 1);
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
         tmem_wait_st();
         fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(p_full);
+        if (lane == 0) mbar_arrive(p_full(i));
         if (j > 0 && !out) collect(before_down, before_back);
       }
       if (ok) collect(down, back);

@@ -1,0 +1,109 @@
+"""Paged attention at its edges, each case with the kernel that it must reach:
+infinities in cached values, scores of any size, keys that are NaN, values that
+a row does not see in every kernel, bad page entries, graph capture."""
+import math
+
+import pytest
+
+from test_gpu_paged import _attend, _int, _make
+
+pytestmark = pytest.mark.gpu
+
+# new tokens, context and page size that lead to each kernel, with 8 query and 2
+# kv heads, max_len the longest sequence: (kernel, f16 cache, new, ctx, page, dim)
+FEW = [("few_kernel", True, [1, 3], [700, 90], 32, 128), ("few_kernel", True, [4], [5000], 64, 64),
+       ("few_kernel", False, [1, 3], [700, 90], 32, 128), ("few_kernel", False, [2], [3000], 16, 64)]
+CHUNK = [("chunk_kernel", True, [40, 1], [200, 90], 32, 128), ("chunk_kernel", True, [150], [500], 48, 64),
+         ("chunk_kernel", False, [40], [20], 32, 128)]
+TC = [("chunk_tc_kernel", True, [200, 2], [500, 70], 32, 128), ("chunk_tc_kernel", True, [300], [1900], 128, 64),
+      ("chunk_tc_kernel", True, [64] * 40, [400] * 40, 16, 64)]
+TC32 = [("chunk_tc32_kernel", False, [200, 2], [500, 70], 32, 128), ("chunk_tc32_kernel", False, [130], [1900], 48, 64),
+        ("chunk_tc32_kernel", False, [32] * 40, [400] * 40, 16, 64)]
+OTHER = [("attend_kernel", True, [5, 1], [200, 90], 16, 80), ("attend_kernel", False, [3], [300], 7, 128 + 32)]
+ALL = FEW + CHUNK + TC + TC32 + OTHER
+
+
+def _ids(case):
+    return f"{case[0]}-{'f16' if case[1] else 'f32'}-{case[2][0]}x{len(case[2])}at{case[3][0]}-p{case[4]}-d{case[5]}"
+
+
+def _case(dev, case, **kw):
+    _, kv16, new, ctx, page, dim = case
+    return _make(dev, new, ctx, 8, 2, dim, page, kv16, seed=dim + sum(ctx), **kw)
+
+
+def _run(case, s, reaches=True, **kw):
+    """The call's output; `reaches`: the kernel that the case is for must be
+    among those that ran."""
+    import torch
+    from torch.profiler import ProfilerActivity, profile
+    length = max(n + c for n, c in zip(s["new"], s["ctx"]))
+    with profile(activities=[ProfilerActivity.CUDA]) as p:
+        out = _attend(s, max_len=length, **kw)
+        torch.cuda.synchronize()
+    names = [e.name for e in p.events()]
+    if reaches:
+        assert any(case[0] + "<" in n for n in names), names
+    return out
+
+
+def _at(s, i, p):
+    """Page and row of position p of sequence i."""
+    return int(s["table"][s["slots"][i], p // s["page"]]), p % s["page"]
+
+
+def _exact(s, drop=()):
+    """The output in 64 bits, without the positions in `drop`, and the bound of
+    test_gpu_paged._reference: products to 21 bits and sums in f32 put a score
+    off by at most (2^-21 + dim 2^-24) sum|q k| / sqrt(dim), which counts twice
+    in a weight; 2^-18 for the roundings of weights and sums.  Queries are kept
+    to 2^-25 of their row's largest value at least: that times sum|k| on top."""
+    import torch
+    q = s["q"].double()
+    heads, dim = q.shape[1:]
+    group = heads // s["k"].shape[1]
+    out, tol = torch.zeros_like(q), torch.zeros_like(q)
+    for i, (n, c) in enumerate(zip(s["new"], s["ctx"])):
+        a = s["starts"][i]
+        held = s["table"][s["slots"][i], :-(-(n + c) // s["page"])].long()
+        kept = torch.tensor([p for p in range(n + c) if p not in set(drop)], device=q.device)
+        hide = kept[None] > torch.arange(c, n + c, device=q.device)[:, None]
+        for h in range(heads):
+            k = s["k"][held, h // group].double().reshape(-1, dim)[kept]
+            v = s["v"][held, h // group].double().reshape(-1, dim)[kept]
+            x = q[a:a + n, h] @ k.T / math.sqrt(dim)
+            p = torch.softmax(x.masked_fill(hide, -math.inf), -1)
+            rows = q[a:a + n, h].abs()
+            off = (2.0 ** -21 + dim * 2.0 ** -24) * (rows @ k.abs().T) + 2.0 ** -25 * rows.amax(-1, keepdim=True) * k.abs().sum(-1)
+            off = (off / math.sqrt(dim)).masked_fill(hide, 0).amax(-1, keepdim=True)
+            out[a:a + n, h] = p @ v
+            tol[a:a + n, h] = (p @ v.abs()) * (2 * off + 2.0 ** -18)
+    return out, tol
+
+
+def _within(got, ref, tol):
+    err = (got.double() - ref).abs()
+    assert (err <= tol).all(), float((err / tol.clamp(min=1e-30)).max())
+
+
+# ---------------------------------------------------------------- values
+@pytest.mark.parametrize("bad", [math.inf, math.nan])
+@pytest.mark.parametrize("case", TC32, ids=_ids)
+def test_f32_tiles_left_out_of_the_products(cuda, case, bad):
+    """A tile of an f32 cache with a value that is not finite is gone through
+    position by position, in a time of its own for each warp: that value is its
+    column's output, every other one is right, call after call."""
+    s = _case(cuda, case)
+    ref, tol = _exact(s)
+    for i, (n, c) in enumerate(zip(s["new"], s["ctx"])):
+        if n > 4:
+            for p in (0, c // 2):
+                page, row = _at(s, i, p)
+                s["v"][page, :, row, 3] = bad
+    chunked = [r for n, a in zip(s["new"], s["starts"]) if n > 4 for r in range(a, a + n)]
+    for _ in range(10):
+        got = _run(case, s)
+        col = got[chunked, :, 3]
+        assert (col.isnan() if math.isnan(bad) else col == bad).all()
+        got[chunked, :, 3] = ref[chunked, :, 3].float()
+        _within(got, ref, tol)
