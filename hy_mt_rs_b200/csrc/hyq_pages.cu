@@ -121,6 +121,12 @@ __device__ bool slots_ok(const Table& t, const int32_t* slot, int n, const int32
   return __syncthreads_and(ok);
 }
 
+// A reserve or fork with a bad sequence (one thread).
+__device__ __forceinline__ void refuse(const Table& t) {
+  *t.shortage = HYQ_PAGES_REFUSED;
+  atomicOr(t.status, DEV_BAD_ARGS);
+}
+
 __global__ void __launch_bounds__(kThreads)
     reserve_kernel(Table t, const int32_t* slot, const int32_t* extra, int n, int32_t* pos, Plan w) {
   grid_dependency_wait();
@@ -137,8 +143,9 @@ __global__ void __launch_bounds__(kThreads)
     ok = before >= 0 && add >= 0 && after <= (int64_t)t.width * t.page_size;
     if (ok) need = (int)((after + t.page_size - 1) / t.page_size) - held;
   }
-  if (!__syncthreads_and(ok)) {
-    if (i == 0) atomicOr(t.status, DEV_BAD_ARGS);
+  if (!__syncthreads_and(ok)) {  // what goes on with these positions skips the sequences
+    if (pos && i < n) pos[i] = -1;
+    if (i == 0) refuse(t);
     return;
   }
   int total;
@@ -188,7 +195,7 @@ __global__ void __launch_bounds__(kThreads)
     part = ok && len % t.page_size != 0;
   }
   if (!__syncthreads_and(ok)) {
-    if (i == 0) atomicOr(t.status, DEV_BAD_ARGS);
+    if (i == 0) refuse(t);
     return;
   }
   for (int s = i >> 5; s < n; s += kThreads / 32) release(t, dst[s]);

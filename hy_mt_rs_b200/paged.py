@@ -19,7 +19,9 @@ import torch
 from ._native import HyqError, check, lib, load_ops
 from .quant import _need_cuda, _ptr
 
-__all__ = ["PagedCache", "rope_append", "attention", "attention_workspace"]
+__all__ = ["PagedCache", "REFUSED", "rope_append", "attention", "attention_workspace"]
+
+REFUSED = 2147483647    # HYQ_PAGES_REFUSED
 
 _ops = load_ops()
 _KV_TYPES = (torch.float32, torch.float16)
@@ -83,7 +85,10 @@ class PagedCache:
     pages with another slot; free() gives them back; compact() moves the live
     pages to the front of the pool.  Nothing synchronises with the host:
     `shortage` holds the number of pages the last reserve or fork lacked (it
-    then changed nothing, or left the forks empty)."""
+    then changed nothing, or left the forks empty), or REFUSED after one with a
+    slot that is repeated or out of range, or that would pass its table row
+    (nothing changed; a reserve's positions are -1, which rope_append and
+    attention skip).  `changes` counts the calls that changed lengths."""
 
     def __init__(self, layers, kv_heads, head_dim, pages, page_size, slots, table_width, device, dtype=torch.float16):
         z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=device)  # noqa: E731
@@ -109,6 +114,7 @@ class PagedCache:
             raise HyqError(-2, "PagedCache: shapes of pool, table, length and refs")
         self.pool, self.table, self.length, self.refs = pool, table, length, refs
         self.page_size, self.pages, self.slots = pool.shape[4], pool.shape[2], table.shape[0]
+        self.changes = 0
         self.shortage = torch.zeros(1, dtype=torch.int32, device=pool.device)
         n = C.c_size_t()
         check(lib.hyq_pages_workspace_bytes(self.pages, C.byref(n)))
@@ -136,6 +142,7 @@ class PagedCache:
         if pos is None:
             pos = torch.empty(slot.shape, dtype=torch.int32, device=slot.device)
         n = self._slots(slot, extra, pos)
+        self.changes += 1
         check(lib.hyq_pages_reserve(self._pages, slot.data_ptr(), extra.data_ptr(), n, pos.data_ptr(), _ptr(self._ws),
                                     _current_stream(slot.get_device())))
         return pos
@@ -143,12 +150,14 @@ class PagedCache:
     def free(self, slot):
         """Give the sequences' pages back."""
         n = self._slots(slot)
+        self.changes += 1
         check(lib.hyq_pages_free(self._pages, slot.data_ptr(), n, _current_stream(slot.get_device())))
 
     def fork(self, src, dst):
         """Sequence dst[i] becomes a copy of src[i]: full pages shared, the
         partial page copied in every layer."""
         n = self._slots(src, dst)
+        self.changes += 1
         check(lib.hyq_pages_fork(self._pages, self._pool, src.data_ptr(), dst.data_ptr(), n, _ptr(self._ws),
                                  _current_stream(src.get_device())))
 

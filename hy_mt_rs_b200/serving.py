@@ -41,6 +41,34 @@ class PagedBatch:
         self.cos, self.sin = model.cos.view(cfg.positions, half), model.sin.view(cfg.positions, half)
         self.workspace = paged.attention_workspace(cfg.heads, cfg.head_dim, dev)
         self.acts = _Acts(cfg, slots + chunk, dev)
+        self._known([0] * slots)
+
+    def _state(self):
+        return self.cache.changes, self.cache.length._version
+
+    def _known(self, held):
+        """The slots' lengths after the calls so far: exact, or past the cache's
+        where pages were short."""
+        self._held, self._held_at = held, self._state()
+
+    def _fork(self, src, dst):
+        self.cache.fork(*self._ints(src, dst))
+        held = list(self._held)
+        for a, b in zip(src, dst):
+            held[b] = self._held[a]
+        self._known(held)
+
+    def _lengths_after(self, slots, lengths):
+        """The requests' lengths after `lengths` more tokens; ValueError if one
+        would pass the model's positions.  The cache's own lengths are read (the
+        host waits) only where they changed by other hands, or to refuse."""
+        after = [self._held[s] + n for s, n in zip(slots, lengths)]
+        if self._held_at != self._state() or max(after) > self.m.cfg.positions:
+            self._known(self.cache.length.tolist())
+            after = [self._held[s] + n for s, n in zip(slots, lengths)]
+            if max(after) > self.m.cfg.positions:
+                raise ValueError(f"a request would pass the model's {self.m.cfg.positions} positions")
+        return after
 
     def _ints(self, *lists):
         """Device int32 arrays of some host lists, by one copy."""
@@ -52,17 +80,26 @@ class PagedBatch:
         lists; ids: the tokens of all, one request after another, device
         int32), append them to the cache, and return the logits of each
         request's last token, [len(slots), vocab].  cache.shortage tells
-        afterwards whether the pages sufficed."""
+        afterwards whether the pages sufficed.  A slot given twice or out of
+        range, or a request that would pass the model's positions, is refused
+        (ValueError) before anything changes."""
         m, cfg, dev = self.m, self.m.cfg, self.m.device
         rows, n = sum(lengths), len(slots)
         if n == 0 or len(lengths) != n or min(lengths) < 1 or ids.numel() != rows:
             raise ValueError("at least one new token per request, and one id per new token")
+        if len(set(slots)) != n or min(slots) < 0 or max(slots) >= self.slots:
+            raise ValueError(f"slots of a step are distinct, from 0 to {self.slots - 1}")
+        after = self._lengths_after(slots, lengths)
         if rows > self.acts.M:
             self.acts = _Acts(cfg, rows, dev)
         a = self.acts
         ends = torch.tensor(lengths).cumsum(0).tolist()
         slot, extra, row_start = self._ints(slots, lengths, [0] + ends)
         pos = self.cache.reserve(slot, extra)
+        held = list(self._held)
+        for s, length in zip(slots, after):
+            held[s] = length
+        self._known(held)
         q, k, v, attended = (t[:rows].view(rows, -1, cfg.head_dim) for t in (a.q, a.k, a.v, a.attended))
         logits = torch.empty(n, cfg.vocab, device=dev)
         st, fused = m._stream(), m.precision == quant.GEMM_F32
@@ -116,6 +153,7 @@ class PagedBatch:
         made = {}                                                           # decoding slot: its tokens so far
         short = torch.zeros(1, dtype=torch.int32, device=dev)
         self.cache.free(self._ints(range(self.slots))[0])
+        self._known([0] * self.slots)
         while True:
             # a token of every decoding request, then prompt tokens
             slots = [s for s, count in made.items() if count < n_new]
@@ -139,8 +177,8 @@ class PagedBatch:
             logits = self.step(slots, lengths, torch.cat(parts))
             torch.maximum(short, self.cache.shortage, out=short)
             if complete and answers > 1:
-                self.cache.fork(*self._ints([i * answers for i in complete for _ in range(1, answers)],
-                                            [i * answers + j for i in complete for j in range(1, answers)]))
+                self._fork([i * answers for i in complete for _ in range(1, answers)],
+                           [i * answers + j for i in complete for j in range(1, answers)])
                 torch.maximum(short, self.cache.shortage, out=short)
             if not sources:
                 continue

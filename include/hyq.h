@@ -519,9 +519,14 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
  * When reserve or fork would need more pages than are free, nothing grows
  * (fork: the dsts end up empty) and *shortage receives the number missing;
  * otherwise it receives 0.  A bad slot, an overlong table row or a repeated
- * slot leaves everything as it was and raises HYQ_DEV_BAD_ARGS.
+ * slot leaves the tables and lengths of all as they were and raises
+ * HYQ_DEV_BAD_ARGS; reserve and fork then write HYQ_PAGES_REFUSED to *shortage,
+ * and reserve -1 to every pos[i], at which hyq_paged_rope_append and
+ * hyq_paged_attention skip the sequence.
  * workspace: hyq_pages_workspace_bytes bytes, 16-byte aligned, no initial
  * value needed. */
+#define HYQ_PAGES_REFUSED 2147483647
+
 typedef struct hyq_pages {
   int32_t *table, *length, *refs, *shortage;
   int64_t slots, table_width, pages;

@@ -1,0 +1,71 @@
+"""PagedBatch.step: arguments that must not reach the cache, and the lengths it
+keeps for the attention calls."""
+import numpy as np
+import pytest
+
+from test_gpu_serving import _alone, _close, _model
+
+pytestmark = pytest.mark.gpu
+
+
+def _put(x, cuda):
+    import torch
+    return torch.tensor(x, dtype=torch.int32, device=cuda)
+
+
+@pytest.mark.parametrize("kv16", [True, False])
+def test_step_refuses_what_would_spoil_others(cuda, kv16):
+    """A request at the end of the positions, a slot given twice, out of range:
+    ValueError before any launch; the other requests' pages stay bit for bit
+    and their next logits are what they would have been."""
+    import torch
+    from hy_mt_rs_b200 import quant
+    from hy_mt_rs_b200.serving import PagedBatch
+
+    model = _model(cuda, "dense", kv16)
+    end = model.cfg.positions
+    rng = np.random.default_rng(5)
+    prompts = [rng.integers(0, model.cfg.vocab, n).tolist() for n in (30, 21, end)]
+    batches = [PagedBatch(model, 4, page_size=16) for _ in range(2)]
+    for b in batches:
+        b.step([0, 1, 2], [30, 21, end], _put(sum(prompts, []), cuda))
+    batch, other = batches
+    pool = batch.cache.pool.clone()
+    state = [t.clone() for t in (batch.cache.table, batch.cache.length, batch.cache.refs)]
+    for slots, lengths in (([0, 1, 2], [1, 1, 1]), ([0, 1, 0], [1, 1, 1]), ([0, 4], [1, 1]), ([0, -1], [1, 1]),
+                           ([0, 3], [1, end + 1]), ([1, 0], [end - 20, 1])):
+        with pytest.raises(ValueError):
+            batch.step(slots, lengths, _put([1] * sum(lengths), cuda))
+        assert torch.equal(batch.cache.pool, pool)
+        for a, b in zip(state, (batch.cache.table, batch.cache.length, batch.cache.refs)):
+            assert torch.equal(a, b)
+    ids = _put([11, 12], cuda)
+    assert torch.equal(batch.step([0, 1], [1, 1], ids), other.step([0, 1], [1, 1], ids))
+    assert quant.device_status() == 0
+
+
+def test_lengths_follow_the_cache(cuda):
+    """Slots freed or forked through the cache itself, and steps that found no
+    pages, neither refuse a request that fits nor let one through that does
+    not."""
+    from hy_mt_rs_b200 import quant
+    from hy_mt_rs_b200.serving import PagedBatch
+
+    model = _model(cuda, "dense", True)
+    end = model.cfg.positions
+    batch = PagedBatch(model, 3, page_size=16, pages=end // 16 + 2)
+    batch.step([0], [end], _put([1] * end, cuda))
+    with pytest.raises(ValueError):
+        batch.step([0], [1], _put([1], cuda))
+    batch.cache.free(_put([0], cuda))
+    batch.step([0], [end - 1], _put([1] * (end - 1), cuda))
+    batch.cache.fork(_put([0], cuda), _put([1], cuda))
+    batch.step([1], [1], _put([1], cuda))
+    with pytest.raises(ValueError):
+        batch.step([1], [1], _put([1], cuda))
+    batch.step([2], [end], _put([1] * end, cuda))       # no pages are left for that many
+    assert batch.cache.shortage.item() > 0
+    quant.device_status()
+    batch.step([2], [10], _put([1] * 10, cuda))         # but for these
+    assert batch.cache.shortage.item() == 0 and batch.cache.length.tolist() == [end - 1, end, 10]
+    assert quant.device_status() == 0
