@@ -32,7 +32,9 @@ constexpr int kRows = kFewRows;      // query rows of a warp: (token, head) pair
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxCtas = 148 * kCtasPerSm;
 // Weights are kept 2^10 times their size, so that their lo halves stay normal
-// f16 numbers down to 2^-24 of the largest.
+// f16 numbers down to 2^-24 of the largest: they are 2^(s - m) with a reference
+// m of 10 below the row's maximum, rounded up, so that no weight passes 2^10
+// (and f16's range) however coarse the scores are.
 constexpr float kBias = 10.0f;
 constexpr float kLog2e = 1.4426950408889634f;
 
@@ -175,7 +177,7 @@ struct Rows {
   float factor[2];                      // 2^e taken out of a row's queries (f16)
   int sees[2];                          // last position each row sees
   float o[DIM / 8][4];
-  float m[2], l[2];
+  float m[2], l[2];                     // reference and sum of the weights
 
   // Fragments of the rows that stage_queries() left at q_s.
   __device__ __forceinline__ void load(uint32_t q_s, const float* factor_s, const Seq& s, int group, int r0) {
@@ -290,14 +292,14 @@ struct Rows {
     float down[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float now = fmaxf(m[i], top[i]);
+      const float now = fmaxf(m[i], __fsub_ru(top[i], kBias));
       down[i] = now == -INFINITY ? 1.0f : ex2(m[i] - now);
       m[i] = now;
       l[i] *= down[i];
     }
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float base = (m[i] == -INFINITY ? 0.f : m[i]) - kBias;
+      const float base = m[i] == -INFINITY ? 0.f : m[i];
 #pragma unroll
       for (int n = 0; n < NT; ++n)
 #pragma unroll

@@ -373,13 +373,18 @@ __device__ __forceinline__ float stage_rows(const AttendArgs& a, const Piece& x,
   return factor;
 }
 
+// The reference of weights whose largest score is `top`: rounded up, so that no
+// weight passes 2^kBias however coarse the scores are, and kept with the bias
+// taken off, so that a weight is 2^(s - m) to the last bit of s and m.
+__device__ __forceinline__ float reference(float top) { return __fsub_ru(top, kBias); }
+
 // One row's scores of a tile, in tensor memory at `st`, to weights, hi and lo
-// (8 columns each for 16 positions), over them.  Weights are
-// 2^(s - m + kBias) with a reference m that follows the row's maximum only
-// when that is more than kSlack past it: the maximum pass over a tile's scores
-// is then needed for a row's first tile alone.  l is the sum of the weights so
-// far, `down` what the outputs so far are to be multiplied by.  scale(v, c)
-// is applied to the scores of columns c .. c + 31 before `factor`.
+// (8 columns each for 16 positions), over them.  Weights are 2^(s - m) with a
+// reference m kBias below the row's maximum (reference()) that follows it only
+// when that is more than kSlack further up: the maximum pass over a tile's
+// scores is then needed for a row's first tile alone.  l is the sum of the
+// weights so far, `down` what the outputs so far are to be multiplied by.
+// scale(v, c) is applied to the scores of columns c .. c + 31 before `factor`.
 template <typename Scale>
 __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool masked, int unseen_from, float factor, float& m,
                                                   float& l, float& down, Scale scale) {
@@ -408,22 +413,30 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
       if (masked) mask(v, c);
       top = fmaxf(top, largest(v));
     }
-    m = top * factor;
+    m = reference(top * factor);
   }
-  float back = kBias - (m == -INFINITY ? 0.f : m), sum = 0.f, sum2 = 0.f;
+  float back = m == -INFINITY ? 0.f : -m, sum = 0.f, sum2 = 0.f;
   down = 1.f;
   // 32 columns: scores to weights, hi and lo over them.  (Loops of 32
   // columns, not unrolled, and two copies of them: the comparisons of a
   // masked tile take as long as the rest, and the unrolled code ran out
   // of the instruction cache.)
   auto weigh = [&](float (&v)[32], int c) {
-    const float over = largest(v) * factor - m;
+    const float top = largest(v) * factor, over = top - m - kBias;
     if (__any_sync(0xffffffffu, over > kSlack)) {
-      // raise the reference by whole powers of two; what this tile has
-      // so far follows
-      const float up = over > kSlack ? ceilf(over) : 0.f, f = ex2(-up);
-      m += up;
-      back -= up;
+      // raise the reference, by whole powers of two where what there is so far
+      // still counts (2^-64 of it does not: nor does a sum from before the first
+      // score above -inf); what this tile has so far follows
+      float f = 1.f;
+      if (over > 64.f) {
+        f = 0.f;
+        m = reference(top);
+      } else if (over > kSlack) {
+        const float before = m;
+        m = fmaxf(m + ceilf(over), reference(top));
+        f = ex2(before - m);
+      }
+      back = m == -INFINITY ? 0.f : -m;
       down *= f;
       sum *= f;
       sum2 *= f;

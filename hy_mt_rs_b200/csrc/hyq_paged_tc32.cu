@@ -382,15 +382,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
             }
             s *= scale;
             if (m == -INFINITY) {
-              m = s;
-            } else if (s > m + kSlack) {
-              const float f = ex2(m - s);
-              m = s;
+              m = reference(s);
+            } else if (s - m > kBias + kSlack) {
+              const float f = ex2(m - reference(s));
+              m = reference(s);
               l *= f;
 #pragma unroll
               for (int d = 0; d < DIM; ++d) o[d] *= f;
             }
-            const float w = s == -INFINITY ? 0.f : ex2(s - m + kBias);
+            const float w = s == -INFINITY ? 0.f : ex2(s - m);
             l += w;
 #pragma unroll
             for (int d = 0; d < DIM / 4; ++d) {

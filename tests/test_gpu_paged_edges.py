@@ -107,3 +107,71 @@ def test_f32_tiles_left_out_of_the_products(cuda, case, bad):
         assert (col.isnan() if math.isnan(bad) else col == bad).all()
         got[chunked, :, 3] = ref[chunked, :, 3].float()
         _within(got, ref, tol)
+
+
+# ---------------------------------------------------------------- scores
+def _longer(case):
+    """The case without its sequences of fewer than 140 cached positions."""
+    kept = [(n, c) for n, c in zip(case[2], case[3]) if c >= 140]
+    return (*case[:2], [n for n, _ in kept], [c for _, c in kept], *case[4:])
+
+
+@pytest.mark.parametrize("low", [-20.0, -1e3, -65504.0])
+@pytest.mark.parametrize("case", [c for c in ALL if max(c[3]) >= 200], ids=_ids)
+def test_lowest_keys_then_ordinary_ones(cuda, case, low):
+    """The first 130 positions score far below the others, in the manner of a
+    mask of the type's lowest value (f32 caches: times 1e27 as well): weights
+    of zero to 64 bits, and the others' are as if they were not there."""
+    case = _longer(case)
+    _, kv16, new, ctx, page, dim = case
+    for up in (1.0,) if kv16 else (1.0, 1e27):
+        s = _case(cuda, case)
+        s["q"][..., 0] = 1000.0 if low == -20.0 else 20.0
+        s["k"][..., 0] *= 0.01      # of the ordinary positions
+        for i in range(len(ctx)):
+            for p in range(130):
+                pg, row = _at(s, i, p)
+                s["k"][pg, :, row, 0] = low * up
+        ref, tol = _exact(s, drop=range(130))
+        _within(_run(case, s), ref, tol)
+
+
+@pytest.mark.parametrize("size", [9.0e5, 2.5e7, 4.0e7, 9.0e7, 1.8e8, 3.0e9, -9.0e5, -2.5e7, -4.0e7, -1.8e8, -3.0e9])
+@pytest.mark.parametrize("case", ALL, ids=_ids)
+def test_equal_scores_of_any_size(cuda, case, size):
+    """Equal scores, however large, are equal weights: the mean of the values
+    seen, to 2^-18 of the mean magnitude (weights) and 2^-24 for each position
+    (a sum in f32)."""
+    import torch
+    s = _case(cuda, case)
+    s["q"].zero_()
+    s["q"][..., 0] = size * math.sqrt(case[5]) / math.log2(math.e) / 1024
+    s["k"].zero_()
+    s["k"][..., 0] = 1024.0
+    got = _run(case, s)
+    for i, (n, c, a) in enumerate(zip(s["new"], s["ctx"], s["starts"])):
+        held = s["table"][s["slots"][i], :-(-(n + c) // s["page"])].long()
+        v = s["v"][held].double().transpose(1, 2).flatten(0, 1)[:n + c]     # [positions, kv heads, dim]
+        count = torch.arange(1, n + c + 1, device=v.device)[:, None, None]
+        mean, size_of = (x.cumsum(0) / count for x in (v, v.abs()))
+        for h in range(8):
+            err = (got[a:a + n, h].double() - mean[c:, h // 4]).abs()
+            tol = (2.0 ** -18 + 2.0 ** -24 * count[c:, 0]) * size_of[c:, h // 4]
+            assert (err <= tol).all(), float(err.max())
+
+
+@pytest.mark.parametrize("case", [c for c in TC if c[3][0] >= 400] + [c for c in TC32 if c[3][0] >= 400], ids=_ids)
+def test_scores_below_every_number_first(cuda, case):
+    """The first 130 positions' scores overflow to -inf: weights of zero."""
+    case = _longer(case)
+    _, kv16, new, ctx, page, dim = case
+    s = _case(cuda, case)
+    s["k"][..., 0] = 0.0
+    s["q"].zero_()
+    s["q"][..., 0] = 1e36           # finite scores are all 0: the mean of the values
+    for i in range(len(ctx)):
+        for p in range(130):
+            pg, row = _at(s, i, p)
+            s["k"][pg, :, row, 0] = -65504.0 if kv16 else -math.inf
+    ref, tol = _exact(dict(s, q=s["q"] * 0), drop=range(130))
+    _within(_run(case, s), ref, tol)
