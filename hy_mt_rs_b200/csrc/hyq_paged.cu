@@ -296,7 +296,14 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
 #pragma unroll
   for (int j = 0; j < OUTS; ++j) {
     const int i = threadIdx.x + j * kThreads;
-    if (i < G * dim) a.out[t * a.out_stride + (int64_t)kvh * G * dim + i] = o[j] / l_s[i / dim];
+    if (i >= G * dim) break;
+    const float l = l_s[i / dim];
+    float y = o[j] / l;
+    if (!isfinite(y) && isfinite(l)) {
+      const float x = non_finite<KV16, 1>(a.c, sq, kvh, -1, seen - 1, i % dim).v[0];
+      if (x != 0.f) y = x;
+    }
+    a.out[t * a.out_stride + (int64_t)kvh * G * dim + i] = y;
   }
 }
 

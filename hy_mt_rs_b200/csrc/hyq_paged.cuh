@@ -156,20 +156,40 @@ cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st);
 bool tc32_supported(const AttendArgs& a);
 cudaError_t launch_chunks_tc32(const AttendArgs& a, cudaStream_t st);
 
-// The non-finite values of V at positions first + 1 .. last of a sequence in
-// one column: their sum (0 when there are none).  The kernels that multiply V
-// by weights of zero take such values out first and add them back, with this,
+// The non-finite values of V at positions first + 1 .. last of a sequence, in N
+// neighbouring columns: their sums (0 where there are none).  An infinity that
+// a row sees is its output whatever the weight, which is above zero: products
+// do not give that (the halves of a split weight or value, and weights that
+// round to zero, make NaN of it), so rows whose output is not finite though the
+// sum of their weights is get it from here.  Likewise the kernels that multiply
+// V by weights of zero take such values out first and add them back, with this,
 // for the rows that see them.
-template <bool KV16>
-__device__ __noinline__ float non_finite(const Cache& c, const Seq& s, int kvh, int first, int last, int d) {
-  float x = 0.f;
-  for (int p = first + 1; p <= last; ++p) {
-    const int page = s.pages[p / c.page_size];
-    if (page < 0 || page >= c.pages) continue;
-    const int64_t at = (int64_t)page * c.page_stride + (int64_t)kvh * c.head_stride +
-                       (int64_t)(p % c.page_size) * c.row_stride + d;
-    const float v = KV16 ? __half2float(static_cast<const __half*>(c.v)[at]) : static_cast<const float*>(c.v)[at];
-    if (!isfinite(v)) x += v;
+template <int N>
+struct Sums {
+  float v[N];
+};
+template <bool KV16, int N>
+__device__ __noinline__ Sums<N> non_finite(const Cache& c, const Seq& s, int kvh, int first, int last, int d) {
+  constexpr int AHEAD = 8;  // positions whose loads are in flight together
+  Sums<N> x{};
+  for (int p0 = first + 1; p0 <= last; p0 += AHEAD) {
+    float v[AHEAD][N];
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i) {
+      const int p = min(p0 + i, last), page = s.pages[p / c.page_size];
+      const bool in = p0 + i <= last && page >= 0 && page < c.pages;
+      const int64_t at = in ? (int64_t)page * c.page_stride + (int64_t)kvh * c.head_stride +
+                                  (int64_t)(p % c.page_size) * c.row_stride + d
+                            : 0;
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        v[i][k] = !in ? 0.f : KV16 ? __half2float(static_cast<const __half*>(c.v)[at + k]) : static_cast<const float*>(c.v)[at + k];
+    }
+#pragma unroll
+    for (int i = 0; i < AHEAD; ++i)
+#pragma unroll
+      for (int k = 0; k < N; ++k)
+        if (!isfinite(v[i][k])) x.v[k] += v[i][k];
   }
   return x;
 }

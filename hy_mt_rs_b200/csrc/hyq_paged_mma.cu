@@ -433,6 +433,19 @@ struct Feed {
   }
 };
 
+// An output y of a row that sees positions up to `last`, l the sum of its
+// weights; `dirty`: values at positions past `first` were taken out.
+template <bool KV16>
+__device__ __forceinline__ float settled(float y, float l, bool dirty, const Cache& c, const Seq& s, int kvh, int first, int last,
+                                         int d) {
+  if (!isfinite(y) && isfinite(l)) {
+    const float x = non_finite<KV16, 1>(c, s, kvh, -1, first, d).v[0];
+    if (x != 0.f) y = x;
+  }
+  if (dirty) y += non_finite<KV16, 1>(c, s, kvh, first, last, d).v[0];
+  return y;
+}
+
 // ---------------------------------------------------------------------------
 // Few new tokens: at most 16 (token, head) rows per kv head
 // ---------------------------------------------------------------------------
@@ -652,8 +665,8 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) top = fmaxf(top, ml_s[w][r][0]);
 #pragma unroll
-      for (int w = 0; w < kWarps; ++w)
-        l += ml_s[w][r][0] == -INFINITY ? 0.f : ml_s[w][r][1] * ex2(ml_s[w][r][0] - top);
+      for (int w = 0; w < kWarps; ++w)  // (a warp without a score above -inf has 0, or NaN to pass on)
+        l = fmaf(ml_s[w][r][1], ml_s[w][r][0] == -INFINITY ? 0.f : ex2(ml_s[w][r][0] - top), l);
       const float* from = o_s + r * G::pitch;
       if (whole) {
         const int tok = r / group;
@@ -662,9 +675,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           const int d = lane + 32 * k;
-          float y = from[d] * inv;
-          if (dirty) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
-          to[d] = y;
+          to[d] = settled<KV16>(from[d] * inv, l, dirty, a.c, s, kvh, s.pos, s.pos + tok, d);
         }
       } else {
 #pragma unroll
@@ -723,15 +734,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
               for (int k = 0; k < N; ++k) sum[k] = fmaf(w, __ldcg(from + 32 * k), sum[k]);
             }
           }
-          const float inv = 1.0f / warp_sum(l);
+          l = warp_sum(l);
+          const float inv = 1.0f / l;
           const int tok = r / group;
           float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM;
 #pragma unroll
           for (int k = 0; k < N; ++k) {
             const int d = lane + 32 * k;
-            float y = sum[k] * inv;
-            if (any) y += non_finite<KV16>(a.c, s, kvh, s.pos, s.pos + tok, d);
-            to[d] = y;
+            to[d] = settled<KV16>(sum[k] * inv, l, any, a.c, s, kvh, s.pos, s.pos + tok, d);
           }
         }
         if (threadIdx.x == 0) counters[cf] = 0;
@@ -845,14 +855,23 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
     const int r = r0 + (lane >> 2) + 8 * i, tok = r / group;
     if (tok >= s.n) continue;
     float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + 2 * (lane & 3);
+    bool odd = dirty_s;
 #pragma unroll
     for (int d = 0; d < DIM / 8; ++d) {
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        float y = rows.o[d][2 * i + j] / l;
-        if (dirty_s) y += non_finite<KV16>(a.c, s, kvh, s.pos + first_tok, s.pos + tok, 8 * d + 2 * (lane & 3) + j);
+        const float y = rows.o[d][2 * i + j] / l;
+        odd = odd || !isfinite(y);
         to[8 * d + j] = y;
       }
+    }
+    if (odd) {
+#pragma unroll 1
+      for (int d = 0; d < DIM / 8; ++d)
+#pragma unroll 1
+        for (int j = 0; j < 2; ++j)
+          to[8 * d + j] = settled<KV16>(to[8 * d + j], l, dirty_s, a.c, s, kvh, s.pos + first_tok, s.pos + tok,
+                                        8 * d + 2 * (lane & 3) + j);
     }
   }
 }

@@ -524,18 +524,14 @@ __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int 
   __syncwarp();
   float* to = x.whole ? a.out : part;
   const bool vec = !x.whole || ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)a.out_stride * 4) & 15) == 0;
-  dirty = dirty && x.whole;
   const int c = lane % kLanes;
+  bool odd = dirty;
 #pragma unroll 4
   for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
     const int64_t off = __shfl_sync(0xffffffffu, mine, i);
-    const int tk = __shfl_sync(0xffffffffu, tok, i);
-    float4 f = *reinterpret_cast<const float4*>(q_s + (row0 + i) * 128 + (c >> 3) * half + (((c ^ i) & 7) << 4));
+    const float4 f = *reinterpret_cast<const float4*>(q_s + (row0 + i) * 128 + (c >> 3) * half + (((c ^ i) & 7) << 4));
     if (off < 0) continue;
-    if (KV16 && dirty) {
-      auto more = [&](int k) { return non_finite<KV16>(a.c, x.s, x.kvh, x.s.pos + x.first_tok, x.s.pos + tk, 4 * c + k); };
-      f.x += more(0), f.y += more(1), f.z += more(2), f.w += more(3);
-    }
+    odd = odd || !isfinite((f.x + f.y) + (f.z + f.w));
     float* y = to + off + 4 * c;
     if (vec) {
       *reinterpret_cast<float4*>(y) = f;
@@ -544,6 +540,23 @@ __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int 
     }
   }
   __syncwarp();
+  if (!x.whole || !__any_sync(0xffffffffu, odd)) return;
+  // infinities and NaN of V that the rows see (non_finite())
+  const int first = x.s.pos + x.first_tok;
+  const Sums<4> before = non_finite<KV16, 4>(a.c, x.s, x.kvh, -1, first, 4 * c);
+#pragma unroll 1
+  for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
+    const int64_t off = __shfl_sync(0xffffffffu, mine, i);
+    const int last = x.s.pos + __shfl_sync(0xffffffffu, tok, i);
+    const float sum = __shfl_sync(0xffffffffu, l, i);
+    if (off >= 0 && isfinite(sum)) {
+      const Sums<4> own = non_finite<KV16, 4>(a.c, x.s, x.kvh, first, last, 4 * c);
+#pragma unroll
+      for (int k = 0; k < 4; ++k)
+        if (before.v[k] + own.v[k] != 0.f) to[off + 4 * c + k] = before.v[k] + own.v[k];
+    }
+    __syncwarp();
+  }
 }
 
 // The pieces of the segment that starts in CTA blockIdx.x's range and goes on
@@ -625,14 +638,34 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
       for (int k = 0; k < N; ++k) o[q][k] = fmaf(f, v[k], o[q][k]);
     }
   }
+  auto place = [&](int r) {
+    return a.out + (int64_t)(s.row0 + r / group) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM + N * lane;
+  };
+  bool odd = dirty;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
-    const int row = warp + 8 * q, r = r0 + row0 + row, tok = r / group, first = s.pos + r0 / group;
+    const int row = warp + 8 * q;
     if (row >= rows) break;
-    float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM + N * lane;
+    float* to = place(r0 + row0 + row);
+    const float l = l_s[row];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const float y = o[q][k] / l;
+      odd = odd || !isfinite(y);
+      to[k] = y;
+    }
+  }
+  if (!odd) return;
+  const int first = s.pos + r0 / group;
+  const Sums<N> before = non_finite<KV16, N>(a.c, s, kvh, -1, first, N * lane);
+#pragma unroll 1
+  for (int row = warp; row < rows; row += 8) {
+    if (!isfinite(l_s[row])) continue;
+    float* to = place(r0 + row0 + row);
+    const Sums<N> own = non_finite<KV16, N>(a.c, s, kvh, first, s.pos + (r0 + row0 + row) / group, N * lane);
 #pragma unroll
     for (int k = 0; k < N; ++k)
-      to[k] = o[q][k] / l_s[row] + (dirty ? non_finite<KV16>(a.c, s, kvh, first, s.pos + tok, N * lane + k) : 0.f);
+      if (before.v[k] + own.v[k] != 0.f) to[k] = before.v[k] + own.v[k];
   }
 }
 

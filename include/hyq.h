@@ -485,10 +485,13 @@ int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, 
  * (attention_into, model.rs:949-1021): the token at position p of sequence s
  * sees the sequence's positions 0 ..= p, whose keys and values must be in the
  * pages already.  out [tokens, heads, head_dim], rows out_stride floats apart.
- * f32 accuracy over either cache type.  Values past a token's position (page
- * tails, later tokens of its chunk) never reach its output, whatever they
- * hold.  head_dim at most 256, at most 16 query heads per kv head.  (Outputs
- * are kept 2^10 times their size inside: values from 2^113 up overflow.)
+ * f32 accuracy over either cache type.  Keys and values past a token's position
+ * (page tails, later tokens of its chunk) never reach its output, whatever they
+ * hold.  Every weight counts as above zero: an infinity in a value that a token
+ * sees is its output, infinities of both signs and NaN make NaN.  A NaN key
+ * makes the rows that see it NaN, and an infinite one may.  head_dim at most
+ * 256, at most 16 query heads per kv head.  (Outputs are kept 2^10 times their
+ * size inside: values from 2^113 up overflow.)
  * workspace: hyq_paged_attention_workspace_bytes bytes (independent of the
  * batch), 16-byte aligned, zero before the first call (every call leaves its
  * counters zero again); calls that share one must not overlap in time. */

@@ -109,6 +109,61 @@ def test_f32_tiles_left_out_of_the_products(cuda, case, bad):
         _within(got, ref, tol)
 
 
+@pytest.mark.parametrize("case", ALL, ids=_ids)
+def test_infinities_in_cached_values(cuda, case):
+    """Every weight is above zero, so an infinity in a value that a token sees
+    is its output, two of different sign and a NaN are NaN; other columns and
+    other kv heads are as without."""
+    from hy_mt_rs_b200 import quant
+    s = _case(cuda, case)
+    ref, tol = _exact(s)
+    put = [(0, 3, math.inf), (0, 5, -math.inf), (1, 6, math.inf), (9, 6, -math.inf), (11, 8, math.nan)]
+    for i, c in enumerate(s["ctx"]):
+        for p, d, x in put:
+            page, row = _at(s, i, p)
+            s["v"][page, 1, row, d] = x
+    got = _run(case, s)
+    rows = got[:, 4:]       # the query heads of kv head 1
+    assert (rows[..., 3] == math.inf).all() and (rows[..., 5] == -math.inf).all()
+    assert rows[..., 6].isnan().all() and rows[..., 8].isnan().all()
+    for d in (3, 5, 6, 8):
+        rows[..., d] = ref[:, 4:, d].float()
+    _within(got, ref, tol)
+    assert quant.device_status() == 0
+
+
+LATER = [("few_kernel", True, [4], [600], 32, 128), ("few_kernel", False, [3], [1500], 32, 64),
+         ("chunk_kernel", True, [100], [100], 32, 128), ("chunk_kernel", False, [50], [10], 16, 64),
+         ("chunk_tc_kernel", True, [200], [500], 32, 128), ("chunk_tc_kernel", True, [200], [3000], 64, 64),
+         ("chunk_tc_kernel", True, [600], [0], 128, 128), ("chunk_tc_kernel", True, [64, 3, 65, 64, 1] * 20, [400] * 100, 16, 64),
+         ("chunk_tc32_kernel", False, [200], [500], 32, 128), ("chunk_tc32_kernel", False, [200], [3000], 64, 64),
+         ("attend_kernel", True, [9], [60], 16, 40)]
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("case", LATER, ids=_ids)
+def test_later_values_do_not_leak(cuda, case, bad):
+    """A non-finite value of a new token is the output of the tokens from its
+    position on, in its column, and reaches nothing else; what lies past every
+    sequence holds anything."""
+    s = _case(cuda, case, fill=bad)
+    clean = dict(s, k=s["k"].nan_to_num(0, 0, 0), v=s["v"].nan_to_num(0, 0, 0))
+    ref, tol = _exact(clean)
+    want = ref.clone()
+    for i, (n, c, a) in enumerate(zip(s["new"], s["ctx"], s["starts"])):
+        at = (2 * n) // 3
+        page, row = _at(s, i, c + at)
+        s["v"][page, :, row, 7] = bad
+        want[a + at:a + n, :, 7] = bad
+    got = _run(case, s)
+    col = got[..., 7].clone()
+    hit = ~want[..., 7].isfinite()
+    assert (col[hit].isnan() if math.isnan(bad) else col[hit] == bad).all()
+    col[hit] = ref[..., 7][hit].float()
+    got[..., 7] = col
+    _within(got, ref, tol)
+
+
 # ---------------------------------------------------------------- scores
 def _longer(case):
     """The case without its sequences of fewer than 140 cached positions."""
