@@ -271,7 +271,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
 #pragma unroll
       for (int w = 16; w > 0; w >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, w));
       const float before = m_s[g], now = fmaxf(before, m);
-      const float e = now == -INFINITY ? 0.f : expf(x - now);
+      const float e = x == -INFINITY ? 0.f : expf(x - now);  // (NaN scores stay NaN)
       const float sum = warp_sum(e);
       __syncwarp();
       e_s[g * kChunk + (threadIdx.x & 31)] = e;

@@ -132,6 +132,21 @@ def test_infinities_in_cached_values(cuda, case):
     assert quant.device_status() == 0
 
 
+@pytest.mark.parametrize("case", ALL, ids=_ids)
+def test_nan_keys_outweigh_infinite_values(cuda, case):
+    """NaN scores make a row NaN, also where its values hold an infinity and
+    where whole blocks of positions are NaN."""
+    for n in (1, 64, 130):
+        s = _case(cuda, case)
+        for i, c in enumerate(s["ctx"]):
+            page, row = _at(s, i, 0)
+            s["v"][page, :, row, 3] = math.inf
+            for p in range(min(n, c)):
+                page, row = _at(s, i, p)
+                s["k"][page, :, row, 1] = math.nan
+        assert _run(case, s).isnan().all()
+
+
 LATER = [("few_kernel", True, [4], [600], 32, 128), ("few_kernel", False, [3], [1500], 32, 64),
          ("chunk_kernel", True, [100], [100], 32, 128), ("chunk_kernel", False, [50], [10], 16, 64),
          ("chunk_tc_kernel", True, [200], [500], 32, 128), ("chunk_tc_kernel", True, [200], [3000], 64, 64),
