@@ -250,8 +250,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
       const int64_t at = (int64_t)max(page, 0) * a.c.page_stride + (int64_t)kvh * a.c.head_stride +
                          (int64_t)(p % a.c.page_size) * a.c.row_stride;
       for (int d = threadIdx.x & 31; d < dim; d += 32) {
-        k_s[i * ks + d] = load_kv<KV16>(a.c.k, at + d);
-        v_s[i * ks + d] = load_kv<KV16>(a.c.v, at + d);
+        k_s[i * ks + d] = page < 0 ? 0.f : load_kv<KV16>(a.c.k, at + d);
+        v_s[i * ks + d] = page < 0 ? 0.f : load_kv<KV16>(a.c.v, at + d);
       }
     }
     __syncthreads();

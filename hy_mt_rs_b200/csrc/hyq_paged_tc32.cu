@@ -369,15 +369,15 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
 #pragma unroll 1
           for (int pos = p0; pos < min(p0 + kTile, sees + 1); ++pos) {
             const int page = x.s.pages[pos / a.c.page_size];
-            if (page < 0 || page >= a.c.pages) continue;
-            const int64_t row = (int64_t)page * a.c.page_stride + (int64_t)x.kvh * a.c.head_stride +
+            const bool in = page >= 0 && page < a.c.pages;  // (no page: zeros, as for the products)
+            const int64_t row = (int64_t)(in ? page : 0) * a.c.page_stride + (int64_t)x.kvh * a.c.head_stride +
                                 (int64_t)(pos % a.c.page_size) * a.c.row_stride;
             const float4* kf = reinterpret_cast<const float4*>(static_cast<const float*>(a.c.k) + row);
             const float4* vf = reinterpret_cast<const float4*>(static_cast<const float*>(a.c.v) + row);
             float s = 0.f;
 #pragma unroll 4
             for (int d = 0; d < DIM / 4; ++d) {
-              const float4 f = kf[d];
+              const float4 f = in ? kf[d] : make_float4(0.f, 0.f, 0.f, 0.f);
               s = fmaf(q[4 * d], f.x, fmaf(q[4 * d + 1], f.y, fmaf(q[4 * d + 2], f.z, fmaf(q[4 * d + 3], f.w, s))));
             }
             s *= scale;
@@ -394,7 +394,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
             l += w;
 #pragma unroll
             for (int d = 0; d < DIM / 4; ++d) {
-              const float4 f = vf[d];
+              const float4 f = in ? vf[d] : make_float4(0.f, 0.f, 0.f, 0.f);
               o[4 * d] = fmaf(w, f.x, o[4 * d]);
               o[4 * d + 1] = fmaf(w, f.y, o[4 * d + 1]);
               o[4 * d + 2] = fmaf(w, f.z, o[4 * d + 2]);

@@ -447,8 +447,9 @@ int hyq_argmax(const float* x, int64_t n, int32_t* token, int32_t* pos, int pos_
  *   activations (rows outside every sequence are left alone), max_new bounds
  *   any sequence's new tokens and max_len any pos[s] + new tokens (the closer,
  *   the better the choice of kernels).  At most 4096 sequences.
- * A sequence whose table row, pages or positions are out of range is skipped
- * and raises HYQ_DEV_BAD_ARGS (see hyq_device_status). */
+ * A sequence whose table row or positions are out of range is skipped, and a
+ * table entry that is no page of the pool counts as one of zeros (appending
+ * skips its tokens); both raise HYQ_DEV_BAD_ARGS (see hyq_device_status). */
 #define HYQ_KV_F32 0
 #define HYQ_KV_F16 1
 

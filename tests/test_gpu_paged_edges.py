@@ -245,3 +245,52 @@ def test_scores_below_every_number_first(cuda, case):
             s["k"][pg, :, row, 0] = -65504.0 if kv16 else -math.inf
     ref, tol = _exact(dict(s, q=s["q"] * 0), drop=range(130))
     _within(_run(case, s), ref, tol)
+
+
+# ------------------------------------------------------- bad arguments on the device
+BAD = [("few_kernel", True, [1, 2, 1], [50, 300, 40], 16, 128), ("few_kernel", False, [1, 2, 1], [50, 300, 40], 16, 64),
+       ("chunk_kernel", True, [40, 30, 40], [50, 100, 9], 16, 128), ("chunk_kernel", False, [9, 12, 9], [30, 40, 8], 16, 64),
+       ("chunk_tc_kernel", True, [100, 90, 80], [500, 700, 9], 16, 128), ("chunk_tc_kernel", True, [100, 90, 80], [500, 700, 9], 128, 64),
+       ("chunk_tc32_kernel", False, [100, 90, 80], [500, 700, 9], 16, 128), ("chunk_tc32_kernel", False, [70, 70, 70], [400, 300, 9], 48, 64),
+       ("attend_kernel", True, [1, 4, 3], [50, 100, 9], 16, 48), ("attend_kernel", False, [1, 4, 3], [50, 100, 9], 16, 96)]
+
+
+@pytest.mark.parametrize("infinite", [False, True])
+@pytest.mark.parametrize("entry", [-1, -5, 1 << 30, None])
+@pytest.mark.parametrize("case", BAD, ids=_ids)
+def test_bad_page_entries_read_as_zeros(cuda, case, entry, infinite):
+    """A table entry that names no page: its positions count as keys and values
+    of zero (no other request's are read), beside an infinity in the same tile
+    too; the other sequences are as they were, HYQ_DEV_BAD_ARGS is raised."""
+    import torch
+    from hy_mt_rs_b200 import quant
+    s = _case(cuda, case)
+    s["k"][0] = 3.0
+    s["v"][0] = 1e4             # a page that must not be read
+    taken = s["table"].clone()
+    # no sequence holds page 0: swap it for a free one
+    free = sorted(set(range(s["k"].shape[0])) - set(taken[taken >= 0].tolist()))
+    if 0 not in free:
+        s["table"][taken == 0] = free[-1]
+    if infinite:
+        page, row = _at(s, 1, 0)
+        s["v"][page, :, row, 3] = math.inf
+    good = _run(case, s)
+    assert quant.device_status() == 0
+    a, b = s["starts"][1], s["starts"][2]
+    t = dict(s, table=s["table"].clone())
+    t["table"][1, 1] = s["k"].shape[0] if entry is None else entry
+    out = torch.zeros_like(good)
+    _run(case, t, out=out)
+    assert quant.device_status() == 8
+    assert torch.equal(out[:a], good[:a]) and torch.equal(out[b:], good[b:])
+    # zeros in their place, on a page of their own
+    z = dict(s, table=s["table"].clone(), k=torch.cat([s["k"], torch.zeros_like(s["k"][:1])]),
+             v=torch.cat([s["v"], torch.zeros_like(s["v"][:1])]))
+    z["table"][1, 1] = s["k"].shape[0]
+    z["v"].nan_to_num_(posinf=0.0)
+    ref, tol = _exact(z)
+    if infinite:
+        assert (out[a:b, :, 3] == math.inf).all()
+        out[a:b, :, 3] = ref[a:b, :, 3].float()
+    _within(out[a:b], ref[a:b], tol[a:b])
