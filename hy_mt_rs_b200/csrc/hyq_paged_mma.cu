@@ -494,6 +494,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     if (i < seqs) {
       const Seq s = load_seq(a.c, i);
       if (s.n > 0 && s.n * group <= kRows) tiles = (s.pos + s.n + G::tile - 1) / G::tile + kSegmentCost;
+      else if (s.n > 0 && !beside) atomicOr(a.c.status, DEV_BAD_ARGS);  // max_new was too small: nobody takes it
     }
     int x = tiles;
 #pragma unroll

@@ -445,8 +445,9 @@ int hyq_argmax(const float* x, int64_t n, int32_t* token, int32_t* pos, int pos_
  *   (none is allowed), at positions pos[s], pos[s] + 1, ...; its table row is
  *   slot[s], or s when slot is NULL.  `tokens` is the number of rows of the
  *   activations (rows outside every sequence are left alone), max_new bounds
- *   any sequence's new tokens and max_len any pos[s] + new tokens (the closer,
- *   the better the choice of kernels).  At most 4096 sequences.
+ *   any sequence's new tokens (attention may skip one with more, and then raises
+ *   HYQ_DEV_BAD_ARGS) and max_len any pos[s] + new tokens (the closer, the better
+ *   the choice of kernels).  At most 4096 sequences.
  * A sequence whose table row or positions are out of range is skipped, and a
  * table entry that is no page of the pool counts as one of zeros (appending
  * skips its tokens); both raise HYQ_DEV_BAD_ARGS (see hyq_device_status). */

@@ -294,3 +294,18 @@ def test_bad_page_entries_read_as_zeros(cuda, case, entry, infinite):
         assert (out[a:b, :, 3] == math.inf).all()
         out[a:b, :, 3] = ref[a:b, :, 3].float()
     _within(out[a:b], ref[a:b], tol[a:b])
+
+
+@pytest.mark.parametrize("kv16", [True, False])
+def test_more_tokens_than_max_new_are_reported(cuda, kv16):
+    """max_new too small for a sequence raises HYQ_DEV_BAD_ARGS; the others are
+    right."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant
+    s = _make(cuda, [1, 40, 2], [50, 20, 300], 8, 2, 128, 16, kv16)
+    ref, tol = _exact(s)
+    out = torch.zeros_like(s["q"])
+    paged.attention(s["q"], s["k"], s["v"], s["table"], s["row_start"], s["pos"], 2, out=out)
+    assert quant.device_status() == 8
+    for rows in (slice(0, 1), slice(41, 43)):
+        _within(out[rows], ref[rows], tol[rows])
