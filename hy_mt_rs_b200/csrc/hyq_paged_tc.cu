@@ -55,7 +55,7 @@ struct Smem {
   static constexpr int bars = ring + kSlots * tile;
   // full[3], empty[3], s_full[2], p_full[2], x_full[2], q_full[2], clean[2]
   static constexpr int n_bars = 2 * kSlots + 10;
-  static constexpr int misc = bars + 8 * n_bars;         // tensor memory address, abort, unused, dirty[2]
+  static constexpr int misc = bars + 8 * n_bars;         // tensor memory address, abort, unused, dirty
   static constexpr int total = misc + 32 + 1024;         // the base is moved to 1024 bytes
 };
 
@@ -100,7 +100,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   if (warp == 0) {
     if (lane == 0) {
       misc[1] = 0;
-      misc[3] = misc[4] = 0;
+      misc[3] = 0;
       for (int s = 0; s < kSlots; ++s) {
         mbar_init(full(s), 1);
         mbar_init(empty(s), 3);  // the products that read it, and warps 2 and 3
@@ -284,10 +284,9 @@ __global__ void __launch_bounds__(kThreads, 1)
       // (these warps follow every tile, and hold its slot: a wait that skipped
       // phases would take an earlier one for its own)
       bool ok = true;
-      int i0 = 0, masked = 0, seg = 0;
+      int i0 = 0, masked = 0;
       while (at < end && ok) {
         const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
-        ++seg;
         for (int i = 0; i < 2 * x.nt; ++i, ++i0) {
           const int slot = i0 % kSlots, j = i >> 1;
           ok = warp_wait(full(slot), (i0 / kSlots) & 1, abort_flag);
@@ -314,7 +313,7 @@ __global__ void __launch_bounds__(kThreads, 1)
               found = found || pos < x.len;
             }
           }
-          if (found) misc[3 + (seg & 1)] = seg;  // (at most one piece ahead of the rows that ask)
+          if (found) misc[3] = 1;  // (from here on: these warps may be pieces ahead of the rows that ask)
           fence_proxy_async_smem();
           __syncwarp();
           if (lane == 0) {
@@ -331,14 +330,13 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------- softmax -------------------------------
     const int wg = warp >= 8 ? 1 : 0;  // row tile
     const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 * wg;
-    int steps = 0, seg = 0;
+    int steps = 0;
     bool ok = true;
     while (at < end && ok) {
       const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
       const int r = x.r0 + wg * kTile + 32 * (warp & 3) + lane;  // row of the sequence
       const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + tok;
       const int64_t piece_at = at;
-      ++seg;
       next(x);
       if (wg == 1 && !x.two) continue;
       const float factor = stage_rows<DIM>(a, x, group, x.r0 + wg * kTile, base_g + L::q + wg * 2 * L::tile);
@@ -374,7 +372,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         *abort_flag = 1;
         break;
       }
-      const bool dirty = misc[3 + (seg & 1)] == seg;
+      const bool dirty = misc[3] != 0;
       store_rows<DIM, kCtaRows, true>(p, x, group, cta, piece_at != begin, r, base_g + L::q + wg * 2 * L::tile, o, m, l, dirty);
     }
   }

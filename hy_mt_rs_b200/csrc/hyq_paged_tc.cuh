@@ -19,7 +19,7 @@ constexpr int kMaxSegs = 65536;          // segments of a call
 constexpr int kMinTiles = 2;             // cost of a CTA's range, at least
 constexpr int kSegTiles = 1;             // cost of a segment, in tiles
 // Floats of a partial result of a segment of ROWS rows: outputs, then
-// (maximum, sum) of each row, then whether a value was taken out.
+// (maximum, sum) of each row, then whether a value may have been taken out.
 template <int ROWS>
 __host__ __device__ constexpr size_t part_floats(int dim) {
   return (size_t)ROWS * (dim + 2) + 4;
@@ -525,7 +525,7 @@ __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int 
   float* to = x.whole ? a.out : part;
   const bool vec = !x.whole || ((reinterpret_cast<uintptr_t>(a.out) | (uintptr_t)a.out_stride * 4) & 15) == 0;
   const int c = lane % kLanes;
-  bool odd = dirty;
+  bool odd = false;
 #pragma unroll 4
   for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
     const int64_t off = __shfl_sync(0xffffffffu, mine, i);
@@ -540,10 +540,13 @@ __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int 
     }
   }
   __syncwarp();
-  if (!x.whole || !__any_sync(0xffffffffu, odd)) return;
-  // infinities and NaN of V that the rows see (non_finite())
+  odd = __any_sync(0xffffffffu, odd);
+  if (!x.whole || !(odd || dirty)) return;
+  // infinities and NaN of V that the rows see (non_finite()); one that all see
+  // shows in their outputs
   const int first = x.s.pos + x.first_tok;
-  const Sums<4> before = non_finite<KV16, 4>(a.c, x.s, x.kvh, -1, first, 4 * c);
+  Sums<4> before{};
+  if (odd) before = non_finite<KV16, 4>(a.c, x.s, x.kvh, -1, first, 4 * c);
 #pragma unroll 1
   for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
     const int64_t off = __shfl_sync(0xffffffffu, mine, i);
@@ -641,7 +644,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
   auto place = [&](int r) {
     return a.out + (int64_t)(s.row0 + r / group) * a.out_stride + (int64_t)(kvh * group + r % group) * DIM + N * lane;
   };
-  bool odd = dirty;
+  bool odd = false;
 #pragma unroll
   for (int q = 0; q < 4; ++q) {
     const int row = warp + 8 * q;
@@ -655,9 +658,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
       to[k] = y;
     }
   }
-  if (!odd) return;
+  if (!odd && !dirty) return;
   const int first = s.pos + r0 / group;
-  const Sums<N> before = non_finite<KV16, N>(a.c, s, kvh, -1, first, N * lane);
+  Sums<N> before{};
+  if (odd) before = non_finite<KV16, N>(a.c, s, kvh, -1, first, N * lane);
 #pragma unroll 1
   for (int row = warp; row < rows; row += 8) {
     if (!isfinite(l_s[row])) continue;

@@ -179,6 +179,26 @@ def test_later_values_do_not_leak(cuda, case, bad):
     _within(got, ref, tol)
 
 
+def test_taken_out_values_of_neighbouring_pieces(cuda):
+    """Segments of two and of one row tile in turn, a non-finite value in every
+    other one's new tokens: each row gets its own back, call after call."""
+    case = ("chunk_tc_kernel", True, [64, 6, 64, 5] * 40, [90, 20, 300, 400] * 40, 16, 64)
+    s = _case(cuda, case)
+    ref, tol = _exact(s)
+    want = ref.clone()
+    for i, (n, c, a) in enumerate(zip(s["new"], s["ctx"], s["starts"])):
+        if i % 4 in (0, 3):
+            page, row = _at(s, i, c + n - 2)
+            s["v"][page, :, row, i % 64] = math.inf
+            want[a + n - 2:a + n, :, i % 64] = math.inf
+    hit = ~want.isfinite()
+    for _ in range(10):
+        got = _run(case, s)
+        assert (got[hit] == math.inf).all()
+        got[hit] = ref[hit].float()
+        _within(got, ref, tol)
+
+
 # ---------------------------------------------------------------- scores
 def _longer(case):
     """The case without its sequences of fewer than 140 cached positions."""
