@@ -53,14 +53,6 @@ const at::Tensor& plain(PyObject* o, const char* name, at::ScalarType type) {
   if (!t.is_contiguous()) refuse(HYQ_E_INVALID, std::string(name) + ": expected a contiguous tensor");
   return t;
 }
-// A contiguous tensor of `n` values, or null for None.
-const void* optional(PyObject* o, const char* name, at::ScalarType type, int64_t n) {
-  if (o == Py_None) return nullptr;
-  const at::Tensor& t = plain(o, name, type);
-  if (t.numel() != n) refuse(HYQ_E_SHAPE, std::string(name) + ": expected " + std::to_string(n) + " values");
-  return t.data_ptr();
-}
-
 int64_t whole(PyObject* o) {
   const long long v = PyLong_AsLongLong(o);
   if (v == -1 && PyErr_Occurred()) throw Refused{0, ""};
@@ -75,6 +67,15 @@ double number(PyObject* o) {
 // One device for all of a call's tensors.
 void same_device(const at::Tensor& a, const at::Tensor& b, const char* name) {
   if (a.device() != b.device()) refuse(HYQ_E_INVALID, std::string(name) + ": on another device");
+}
+
+// A contiguous tensor of `n` values on the device of `like`, or null for None.
+const void* optional(PyObject* o, const at::Tensor& like, const char* name, at::ScalarType type, int64_t n) {
+  if (o == Py_None) return nullptr;
+  const at::Tensor& t = plain(o, name, type);
+  same_device(like, t, name);
+  if (t.numel() != n) refuse(HYQ_E_SHAPE, std::string(name) + ": expected " + std::to_string(n) + " values");
+  return t.data_ptr();
 }
 
 hyq_paged_kv make_kv(const at::Tensor& q, PyObject* k_pages, PyObject* v_pages, PyObject* table) {
@@ -104,7 +105,7 @@ hyq_paged_batch make_batch(const at::Tensor& q, PyObject* row_start, PyObject* p
   if (r.numel() != seqs + 1) refuse(HYQ_E_SHAPE, "row_start takes one more entry than pos");
   same_device(q, r, "row_start");
   same_device(q, p, "pos");
-  const void* s = optional(slot, "slot", at::kInt, seqs);
+  const void* s = optional(slot, q, "slot", at::kInt, seqs);
   return {static_cast<const int32_t*>(s), static_cast<const int32_t*>(r.data_ptr()),
           static_cast<const int32_t*>(p.data_ptr()), seqs, tokens, max_new, max_len};
 }
@@ -189,12 +190,13 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
       refuse(HYQ_E_SHAPE, "rope_append: cos and sin are [positions, head_dim / 2]");
     same_device(q, cos, "cos");
     same_device(q, sin, "sin");
+    const void* q_norm = optional(a[10], q, "q_norm", at::kFloat, kv.head_dim);
+    const void* k_norm = optional(a[11], q, "k_norm", at::kFloat, kv.head_dim);
     check(hyq_paged_rope_append(
         &kv, &batch, static_cast<const float*>(q.data_ptr()), qs, (int)q.size(1), static_cast<const float*>(k.data_ptr()), ks,
         static_cast<const float*>(v.data_ptr()), vs, static_cast<const float*>(cos.data_ptr()),
         static_cast<const float*>(sin.data_ptr()), cos.size(0),
-        static_cast<const float*>(optional(a[10], "q_norm", at::kFloat, kv.head_dim)),
-        static_cast<const float*>(optional(a[11], "k_norm", at::kFloat, kv.head_dim)), (float)number(a[12]),
+        static_cast<const float*>(q_norm), static_cast<const float*>(k_norm), (float)number(a[12]),
         PyObject_IsTrue(a[13]), static_cast<float*>(out.data_ptr()), row_stride(out, "out"), stream_of(q)));
     return THPVariable_Wrap(out);
   });
@@ -207,14 +209,16 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (x.dim() != 2 || (x.size(1) > 1 && x.stride(1) != 1)) refuse(HYQ_E_SHAPE, "sample: logits are [rows, n] with contiguous rows");
     const int64_t rows = x.size(0), cols = x.size(1);
     if (a[1] == Py_None) refuse(HYQ_E_INVALID, "u: expected a CUDA tensor");
-    const void* u = optional(a[1], "u", at::kFloat, rows);
+    const void* u = optional(a[1], x, "u", at::kFloat, rows);
+    const void* temperature = optional(a[2], x, "temperature", at::kFloat, rows);
+    const void* top_k = optional(a[3], x, "top_k", at::kInt, rows);
+    const void* top_p = optional(a[4], x, "top_p", at::kFloat, rows);
+    const void* min_p = optional(a[5], x, "min_p", at::kFloat, rows);
     const at::Tensor token = output(a[6], x, {rows}, at::kInt, "token"), prob = output(a[7], x, {rows}, at::kFloat, "prob");
     if (!token.is_contiguous() || !prob.is_contiguous()) refuse(HYQ_E_INVALID, "sample: expected contiguous outputs");
     check(hyq_sample(static_cast<const float*>(x.data_ptr()), cols, rows > 1 ? x.stride(0) : cols, rows,
-                     static_cast<const float*>(optional(a[2], "temperature", at::kFloat, rows)),
-                     static_cast<const int32_t*>(optional(a[3], "top_k", at::kInt, rows)),
-                     static_cast<const float*>(optional(a[4], "top_p", at::kFloat, rows)),
-                     static_cast<const float*>(optional(a[5], "min_p", at::kFloat, rows)), static_cast<const float*>(u),
+                     static_cast<const float*>(temperature), static_cast<const int32_t*>(top_k),
+                     static_cast<const float*>(top_p), static_cast<const float*>(min_p), static_cast<const float*>(u),
                      static_cast<int32_t*>(token.data_ptr()), static_cast<float*>(prob.data_ptr()), stream_of(x)));
     PyObject *t = THPVariable_Wrap(token), *p = THPVariable_Wrap(prob);
     PyObject* both = t && p ? PyTuple_Pack(2, t, p) : nullptr;

@@ -109,6 +109,7 @@ class PagedCache:
         _need_cuda(pool, "pool")
         for t, name in ((table, "table"), (length, "length"), (refs, "refs")):
             _need_cuda(t, name, torch.int32)
+            self._same_device(t, pool, name)
         if pool.dim() != 6 or pool.shape[1] != 2 or table.dim() != 2 or length.numel() != table.shape[0] \
                 or refs.numel() != pool.shape[2]:
             raise HyqError(-2, "PagedCache: shapes of pool, table, length and refs")
@@ -124,6 +125,11 @@ class PagedCache:
         page = pool[0, 0, 0].numel() * pool.element_size()
         self._pool = _POOL.pack(pool.data_ptr(), 2 * pool.shape[0], page * self.pages, page, page)
 
+    @staticmethod
+    def _same_device(t, like, name):
+        if t.device != like.device:
+            raise HyqError(-1, f"{name}: on another device")
+
     def layer(self, i):
         """(k_pages, v_pages) of a layer."""
         return self.pool[i, 0], self.pool[i, 1]
@@ -132,6 +138,7 @@ class PagedCache:
         n = arrays[0].numel() if isinstance(arrays[0], torch.Tensor) else 0
         for t in arrays:
             _check_int(t, "slots")
+            self._same_device(t, self.pool, "slots")
             if t.numel() != n:
                 raise HyqError(-2, "PagedCache: arrays of one call differ in length")
         return n
@@ -139,9 +146,10 @@ class PagedCache:
     def reserve(self, slot, extra, pos=None):
         """Grow sequence slot[i] by extra[i] positions; their first positions
         (int32, into `pos` when given)."""
+        n = self._slots(slot, extra)
         if pos is None:
             pos = torch.empty(slot.shape, dtype=torch.int32, device=slot.device)
-        n = self._slots(slot, extra, pos)
+        self._slots(slot, pos)
         self.changes += 1
         check(lib.hyq_pages_reserve(self._pages, slot.data_ptr(), extra.data_ptr(), n, pos.data_ptr(), _ptr(self._ws),
                                     _current_stream(slot.get_device())))
