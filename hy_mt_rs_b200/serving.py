@@ -13,8 +13,9 @@ them, hyq_paged_rope_append and hyq_paged_attention over the requests' pages
 import torch
 
 from . import paged, quant, sampling
-from ._native import check, lib
+from ._native import HyqError, check, lib
 from .model import _Acts, _add_norm, _gate_up_normed, _matmul_normed, _p, _qkv_normed
+from .quant import _need_cuda
 
 __all__ = ["PagedBatch"]
 
@@ -33,6 +34,8 @@ class PagedBatch:
         cfg, dev = model.cfg, model.device
         if not 1 <= slots <= 1024:
             raise ValueError("1 to 1024 slots")
+        if chunk < 1 or page_size < 1:
+            raise ValueError("at least one position of a page and one prompt token of a step")
         self.m, self.slots, self.chunk = model, slots, chunk
         width = -(-cfg.positions // page_size)
         self.cache = paged.PagedCache(len(model.layers), cfg.kv_heads, cfg.head_dim, pages or slots * width, page_size,
@@ -84,6 +87,9 @@ class PagedBatch:
         range, or a request that would pass the model's positions, is refused
         (ValueError) before anything changes."""
         m, cfg, dev = self.m, self.m.cfg, self.m.device
+        _need_cuda(ids, "ids", torch.int32)
+        if ids.device != self.cache.pool.device:
+            raise HyqError(-1, "ids: on another device")
         rows, n = sum(lengths), len(slots)
         if n == 0 or len(lengths) != n or min(lengths) < 1 or ids.numel() != rows:
             raise ValueError("at least one new token per request, and one id per new token")

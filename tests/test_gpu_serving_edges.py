@@ -69,3 +69,20 @@ def test_lengths_follow_the_cache(cuda):
     batch.step([2], [10], _put([1] * 10, cuda))         # but for these
     assert batch.cache.shortage.item() == 0 and batch.cache.length.tolist() == [end - 1, end, 10]
     assert quant.device_status() == 0
+
+
+def test_arguments_are_checked(cuda):
+    import torch
+    from hy_mt_rs_b200._native import HyqError
+    from hy_mt_rs_b200.serving import PagedBatch
+
+    model = _model(cuda, "dense", True)
+    for kw in (dict(chunk=0), dict(chunk=-4), dict(page_size=0)):
+        with pytest.raises(ValueError):
+            PagedBatch(model, 2, **{"page_size": 16, **kw})
+    batch = PagedBatch(model, 2, page_size=16)
+    for ids in (torch.zeros(2, dtype=torch.int64, device=cuda), torch.zeros(2, dtype=torch.int32),
+                torch.zeros(4, dtype=torch.int32, device=cuda)[::2]):
+        with pytest.raises(HyqError):
+            batch.step([0], [2], ids)
+    assert batch.cache.length.tolist() == [0, 0]
