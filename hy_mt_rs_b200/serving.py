@@ -119,7 +119,7 @@ class PagedBatch:
                 paged.rope_append(q, k, v, k_pages, v_pages, self.cache.table, row_start, pos, self.cos, self.sin,
                                   W["q_norm"], W["k_norm"], cfg.eps, bool(m.norm_first), slot=slot, out=q)
                 paged.attention(q, k_pages, v_pages, self.cache.table, row_start, pos, max(lengths),
-                                slot=slot, out=attended, workspace=self.workspace)
+                                max(after), slot=slot, out=attended, workspace=self.workspace)
                 check(lib.hyq_matmul(W["o"].handle, _p(a.attended), rows, _p(a.projected), st))
                 if "moe" in W:
                     _add_norm(_p(a.hidden), _p(a.projected), _p(W["ffn_norm"]), cfg.hidden, rows, cfg.eps,

@@ -71,6 +71,28 @@ def test_lengths_follow_the_cache(cuda):
     assert quant.device_status() == 0
 
 
+@pytest.mark.parametrize("kv16", [True, False])
+def test_attention_gets_the_longest_length(cuda, kv16, monkeypatch):
+    """The bound that the choice of attention kernels goes by."""
+    from hy_mt_rs_b200 import paged
+    from hy_mt_rs_b200.serving import PagedBatch
+
+    model = _model(cuda, "dense", kv16)
+    batch = PagedBatch(model, 3, page_size=16)
+    seen, call = [], paged.attention
+
+    def record(*a, **kw):
+        seen.append((a[6], a[7] if len(a) > 7 else kw.get("max_len")))
+        return call(*a, **kw)
+
+    monkeypatch.setattr(paged, "attention", record)
+    batch.step([0, 2], [20, 9], _put([1] * 29, cuda))
+    batch.step([0, 1], [1, 7], _put([1] * 8, cuda))
+    batch.step([2], [1], _put([1], cuda))
+    n = len(model.layers)
+    assert seen == [(20, 20)] * n + [(7, 21)] * n + [(1, 10)] * n
+
+
 def test_arguments_are_checked(cuda):
     import torch
     from hy_mt_rs_b200._native import HyqError
@@ -86,3 +108,32 @@ def test_arguments_are_checked(cuda):
         with pytest.raises(HyqError):
             batch.step([0], [2], ids)
     assert batch.cache.length.tolist() == [0, 0]
+
+
+@pytest.mark.parametrize("kv16", [True, False])
+def test_long_contexts_match_single_requests(cuda, kv16):
+    """Prompts past the lengths of the one-launch chunk kernel, in chunks, beside
+    short ones (tolerances of test_gpu_serving)."""
+    import torch
+    from hy_mt_rs_b200 import quant
+    from hy_mt_rs_b200.model import DenseConfig, DenseModel, random_weights
+    from hy_mt_rs_b200.serving import PagedBatch
+
+    cfg = DenseConfig(layers=3, vocab=8192, ffn=2048, positions=1024)
+    weights = random_weights(cfg, cuda, seed=12)
+    torch.cuda.synchronize()
+    model = DenseModel(cfg, weights, cuda, kv16=kv16, gemm_precision=quant.GEMM_F32)
+    tol = 1e-3 if kv16 else 1e-4
+    rng = np.random.default_rng(6)
+    prompts = [rng.integers(0, cfg.vocab, n).tolist() for n in (700, 20, 450)]
+    ids, logits = _alone(model, prompts, 3)
+    batch = PagedBatch(model, 3, page_size=32)
+    batch.step([0], [300], _put(prompts[0][:300], cuda))
+    batch.step([0, 2], [399, 449], _put(prompts[0][300:699] + prompts[2][:449], cuda))
+    got = batch.step([1, 0, 2], [20, 1, 1], _put(prompts[1] + prompts[0][699:] + prompts[2][449:], cuda)).cpu().numpy()
+    for g, r in zip(got, (1, 0, 2)):
+        assert _close(g, logits[r][0], tol), r
+    got = batch.step([0, 1, 2], [1] * 3, _put([i[0] for i in ids], cuda)).cpu().numpy()
+    for r, g in enumerate(got):
+        assert _close(g, logits[r][1], tol), r
+    assert quant.device_status() == 0
