@@ -41,8 +41,13 @@ __host__ __device__ inline Plan plan_of(void* ws, int64_t pages) {
   return {p, p + 4, p + 4 + pages, p + 4 + 2 * pages};
 }
 
-// Exclusive prefix sum of one value per thread over the CTA (1024 threads);
-// every thread gets the total.
+// Sum of two counts of pages, at most kMost: 1,024 sequences may ask for more
+// than 2^31 together, and must not seem to ask for few.
+constexpr unsigned kMost = HYQ_PAGES_REFUSED - 1;
+__device__ __forceinline__ int sum_of(int a, int b) { return (int)min((unsigned)a + (unsigned)b, kMost); }
+
+// Exclusive prefix sum of one value per thread over the CTA (1024 threads),
+// right while the total is below kMost; every thread gets the total.
 __device__ __forceinline__ int block_scan(int v, int& total) {
   __shared__ int warp_s[kThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -50,7 +55,7 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x += y;
+    if (lane >= o) x = sum_of(x, y);
   }
   if (lane == 31) warp_s[warp] = x;
   __syncthreads();
@@ -58,12 +63,12 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w += y;
+    if (lane >= o) w = sum_of(w, y);
   }
   total = __shfl_sync(0xffffffffu, w, 31);
   const int base = warp == 0 ? 0 : __shfl_sync(0xffffffffu, w, warp - 1);
   __syncthreads();  // warp_s may be written again
-  return base + x - v;
+  return sum_of(base, x) - v;
 }
 
 // The `need` lowest-numbered free pages, in ascending order, into list (as
@@ -148,7 +153,7 @@ __global__ void __launch_bounds__(kThreads)
     if (i == 0) refuse(t);
     return;
   }
-  int total;
+  int total;  // (kMost is more than there can be pages)
   const int at = block_scan(need, total);
   at_s[i] = at;
   const int found = total ? find_free(t.refs, t.pages, total, w.to) : 0;

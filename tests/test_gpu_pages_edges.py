@@ -46,3 +46,22 @@ def test_refused_fork_says_so(cuda):
         assert cache.shortage.item() == paged.REFUSED and quant.device_status() == 8
     cache.fork(_int([0], cuda), _int([1], cuda))
     assert cache.shortage.item() == 0 and quant.device_status() == 0
+
+
+def test_reserve_of_more_than_2_to_the_31_pages(cuda):
+    """1,024 sequences that ask for 2^21 + 1 pages each: short, and nothing
+    grows.  (The table is 8.6 GB, of which the call reads nothing.)"""
+    import torch
+    from hy_mt_rs_b200 import paged, quant
+    width, pages = (1 << 21) + 1, 64
+    z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=cuda)  # noqa: E731
+    table = torch.empty(1024, width, dtype=torch.int32, device=cuda)
+    cache = paged.PagedCache.over(torch.zeros(1, 2, pages, 1, 1, 8, dtype=torch.float16, device=cuda), table, z(1024), z(pages))
+    slot = torch.arange(1024, dtype=torch.int32, device=cuda)
+    pos = cache.reserve(slot, torch.full_like(slot, width))
+    assert (pos == 0).all() and cache.shortage.item() == paged.REFUSED - 1 - pages
+    assert (cache.length == 0).all() and (cache.refs == 0).all()
+    cache.reserve(slot[:3], torch.full_like(slot[:3], 21))
+    assert cache.shortage.item() == 0 and cache.refs.sum().item() == 63
+    assert table[:3, :21].flatten().tolist() == list(range(63))
+    assert quant.device_status() == 0
