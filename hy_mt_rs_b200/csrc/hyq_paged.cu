@@ -335,14 +335,15 @@ using hyq::api_fail;
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-int make_cache(const hyq_paged_kv* kv, const hyq_paged_batch* b, int heads, const char* name, hyq::paged::Cache& c) {
+int make_cache(const hyq_paged_kv* kv, const hyq_paged_batch* b, int heads, const char* name, bool attends,
+               hyq::paged::Cache& c) {
   if (!kv || !b || !kv->k || !kv->v || !kv->table || (b->seqs > 0 && (!b->row_start || !b->pos)))
     return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
   if (kv->dtype != HYQ_KV_F32 && kv->dtype != HYQ_KV_F16)
     return api_fail(HYQ_E_INVALID, "%s: unknown cache type %d", name, kv->dtype);
   if (kv->kv_heads <= 0 || kv->head_dim <= 0 || kv->page_size <= 0 || kv->pages <= 0 || kv->pages > INT32_MAX ||
       kv->slots <= 0 || kv->slots > INT32_MAX || kv->table_width <= 0 ||
-      kv->table_width > INT32_MAX / kv->page_size)
+      kv->table_width > (INT32_MAX - hyq::paged::kPastEnd) / kv->page_size)
     return api_fail(HYQ_E_SHAPE, "%s: shape of the cache", name);
   if (heads <= 0 || heads % kv->kv_heads)
     return api_fail(HYQ_E_SHAPE, "%s: %d query heads over %d kv heads", name, heads, kv->kv_heads);
@@ -354,6 +355,9 @@ int make_cache(const hyq_paged_kv* kv, const hyq_paged_batch* b, int heads, cons
   if (b->seqs < 0 || b->seqs > hyq::paged::kMaxSeqs || b->tokens < 0 || b->tokens > INT32_MAX || b->max_new < 0 ||
       b->max_len < b->max_new || b->max_len > kv->table_width * kv->page_size)
     return api_fail(HYQ_E_SHAPE, "%s: shape of the batch", name);
+  if (attends && !hyq::paged::sums_fit(b->seqs, kv->table_width * kv->page_size))
+    return api_fail(HYQ_E_SHAPE, "%s: %lld sequences of up to %lld positions: more than the kernels' sums hold", name,
+                    (long long)b->seqs, (long long)(kv->table_width * kv->page_size));
   if (!b->slot && b->seqs > kv->slots)
     return api_fail(HYQ_E_SHAPE, "%s: %lld sequences, %lld table rows", name, (long long)b->seqs, (long long)kv->slots);
   const size_t esize = kv->dtype == HYQ_KV_F16 ? 2 : 4;
@@ -395,7 +399,7 @@ int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, 
                           void* stream) {
   const char* name = "paged_rope_append";
   hyq::paged::AppendArgs a{};
-  const int rc = make_cache(kv, batch, heads, name, a.c);
+  const int rc = make_cache(kv, batch, heads, name, false, a.c);
   if (rc) return rc;
   if (batch->seqs == 0 || batch->tokens == 0) return HYQ_OK;
   if (!q || !k || !v || !cos_tab || !sin_tab || !q_out) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
@@ -444,7 +448,7 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
                         int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
   const char* name = "paged_attention";
   hyq::paged::AttendArgs a{};
-  const int rc = make_cache(kv, batch, heads, name, a.c);
+  const int rc = make_cache(kv, batch, heads, name, true, a.c);
   if (rc) return rc;
   if (batch->seqs == 0 || batch->tokens == 0 || batch->max_new == 0) return HYQ_OK;
   if (!q || !out || !workspace) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);

@@ -128,6 +128,10 @@ struct AttendArgs {
   void* ws;
 };
 
+// The kernels round a sequence's length up to tiles and look some tiles ahead, in
+// 32 bits: a table row ends this far below 2^31.
+constexpr int kPastEnd = 4096;
+
 // Largest number of sequences of a call (the kernels keep a prefix sum over
 // them in shared memory).
 constexpr int kMaxSeqs = 4096;
@@ -135,6 +139,9 @@ constexpr int kMaxSeqs = 4096;
 // hyq_paged_mma.cu: head sizes 64 and 128 over 16-byte aligned rows.
 bool mma_supported(const AttendArgs& a, bool kv16);
 size_t mma_workspace_bytes(int dim);
+// Whether launch_few's 32-bit sum of tiles holds that many sequences of any
+// length up to `reach` (4,096 of 16 million positions).
+bool sums_fit(int64_t seqs, int64_t reach);
 // Sequences of up to kFewRows rows; `beside`: next to the kernel that the same
 // call launched before.
 cudaError_t launch_few(const AttendArgs& a, bool kv16, bool beside, cudaStream_t st);

@@ -915,6 +915,11 @@ bool mma_supported(const AttendArgs& a, bool kv16) {
          (reinterpret_cast<uintptr_t>(a.c.k) | reinterpret_cast<uintptr_t>(a.c.v)) % 16 == 0;
 }
 
+bool sums_fit(int64_t seqs, int64_t reach) {
+  constexpr int tile = Geo<128, false>::tile;  // the smaller one
+  return seqs * (reach / tile + 1 + kSegmentCost) <= INT32_MAX;
+}
+
 bool chunks_short(const AttendArgs& a, bool kv16, int64_t max_len) {
   const int64_t tiles = (chunk_tiles(a) - a.c.seqs / 2) * a.c.kv_heads;  // sequences' last tiles are half full
   const int64_t rounds = (tiles + kMaxCtas - 1) / kMaxCtas;

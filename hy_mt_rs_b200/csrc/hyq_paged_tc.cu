@@ -431,8 +431,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
 
 bool tc_supported(const AttendArgs& a) {
   const int ps = a.c.page_size;
-  const int64_t segs = ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + kCtaRows - 1) / kCtaRows + a.c.seqs;
-  return (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) && segs <= kMaxSegs && encode_fn() != nullptr;
+  return (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) && plan_fits<kCtaRows>(a) && encode_fn() != nullptr;
 }
 
 size_t tc_workspace_bytes(int dim) { return kPlanBytes + kMaxParts * part_floats<kCtaRows>(dim) * sizeof(float); }

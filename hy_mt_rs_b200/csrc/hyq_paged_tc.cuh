@@ -60,6 +60,14 @@ struct Params {
   float* parts;   // [CTA][first piece, last piece] (part_floats)
 };
 
+// Whether the plan holds a call's segments of ROWS rows: their number, and the
+// 32-bit sum of their tiles at any length.
+template <int ROWS>
+inline bool plan_fits(const AttendArgs& a) {
+  const int64_t segs = ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + ROWS - 1) / ROWS + a.c.seqs;
+  return segs <= kMaxSegs && segs * ((int64_t)a.c.width * a.c.page_size / kTile + 1 + kSegTiles) <= INT32_MAX;
+}
+
 // Position tiles that the rows of a segment see.
 template <int ROWS>
 __device__ __forceinline__ int seen_tiles(const Seq& s, int group, int tile) {

@@ -460,9 +460,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
 
 }  // namespace
 
-bool tc32_supported(const AttendArgs& a) {
-  return ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + kRows - 1) / kRows + a.c.seqs <= kMaxSegs;
-}
+bool tc32_supported(const AttendArgs& a) { return plan_fits<kRows>(a); }
 
 cudaError_t launch_chunks_tc32(const AttendArgs& a, cudaStream_t st) {
   return a.c.dim == 128 ? launch<128>(a, st) : launch<64>(a, st);

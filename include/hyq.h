@@ -447,7 +447,9 @@ int hyq_argmax(const float* x, int64_t n, int32_t* token, int32_t* pos, int pos_
  *   activations (rows outside every sequence are left alone), max_new bounds
  *   any sequence's new tokens (attention may skip one with more, and then raises
  *   HYQ_DEV_BAD_ARGS) and max_len any pos[s] + new tokens (the closer, the better
- *   the choice of kernels).  At most 4096 sequences.
+ *   the choice of kernels).  At most 4096 sequences (attention: fewer where a
+ *   table row has more than 2^24 positions); a table row ends 4096 positions
+ *   below 2^31.
  * A sequence whose table row or positions are out of range is skipped, and a
  * table entry that is no page of the pool counts as one of zeros (appending
  * skips its tokens); both raise HYQ_DEV_BAD_ARGS (see hyq_device_status). */
