@@ -1237,7 +1237,7 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
                const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
                float* prob, void* stream) {
   const char* name = "sample";
-  if (n <= 0 || n >= 1 << 23 || rows < 0 || rows > INT32_MAX || stride < n)
+  if (n <= 0 || n >= 1 << 23 || rows < 0 || rows > INT32_MAX / 8 || stride < n)  // (up to 8 CTAs a row)
     return hyq::api_fail(HYQ_E_SHAPE, "%s: shape (1 to 8388607 logits a row)", name);
   if (rows == 0) return HYQ_OK;
   if (!logits || !u || !token) return hyq::api_fail(HYQ_E_INVALID, "%s: null pointer", name);
