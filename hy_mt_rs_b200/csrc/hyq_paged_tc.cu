@@ -175,9 +175,12 @@ __global__ void __launch_bounds__(kThreads, 1)
         if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_EMPTY);
         *abort_flag = 1;
       }
-      // no copy may land after this CTA is gone
-      for (int i = max(0, issued - kSlots); i < issued; ++i)
-        if (!warp_wait(full(i % kSlots), (i / kSlots) & 1, nullptr) && lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_DRAIN);
+      // no copy may land after this CTA is gone, and no product's arrival
+      for (int i = max(0, issued - kSlots); i < issued; ++i) {
+        const bool in = warp_wait(full(i % kSlots), (i / kSlots) & 1, nullptr);
+        const bool out = warp_wait(empty(i % kSlots), (i / kSlots) & 1, abort_flag);
+        if (!(in && out) && lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_DRAIN);
+      }
     } else if (warp == 1) {
       // ------------------------------ products -------------------------------
       // f32 sums, f16 operands, M 128; N 128 positions, or DIM columns with V
