@@ -329,3 +329,43 @@ def test_more_tokens_than_max_new_are_reported(cuda, kv16):
     assert quant.device_status() == 8
     for rows in (slice(0, 1), slice(41, 43)):
         _within(out[rows], ref[rows], tol[rows])
+
+
+# ---------------------------------------------------------------- graphs
+GRAPH = [("chunk_tc_kernel", True, [200, 1, 3], [500, 900, 70], 32, 128), ("chunk_kernel", True, [40, 1], [100, 90], 32, 128),
+         ("chunk_tc32_kernel", False, [130, 2, 1], [500, 90, 700], 32, 128), ("chunk_kernel", False, [30, 2], [10, 5], 32, 64)]
+
+
+@pytest.mark.parametrize("overlap", [False, True])
+@pytest.mark.parametrize("case", GRAPH, ids=_ids)
+def test_chunk_calls_in_a_graph(cuda, case, overlap):
+    """Two chunk calls captured with their programmatic edges, replayed while
+    the positions change in place."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant
+    s = _case(cuda, case)
+    ws = paged.attention_workspace(8, case[5], cuda)
+    length = max(n + c for n, c in zip(s["new"], s["ctx"]))
+    out, again = torch.empty_like(s["q"]), torch.empty_like(s["q"])
+    _run(case, s, out=out, workspace=ws)
+    quant.set_launch_overlap(overlap)
+    try:
+        g, st = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(g, stream=st):
+            _attend(s, out=out, workspace=ws, max_len=length)
+            _attend(dict(s, q=out), out=again, workspace=ws, max_len=length)
+    finally:
+        quant.set_launch_overlap(False)
+    for less in (0, 1, 5):
+        s["ctx"] = [max(c - less, 0) for c in case[3]]
+        s["pos"].copy_(_int(s["ctx"], cuda))
+        out.zero_()
+        for _ in range(3):
+            g.replay()
+        torch.cuda.synchronize()
+        ref, tol = _exact(s)
+        _within(out, ref, tol)
+        ref, tol = _exact(dict(s, q=out))
+        _within(again, ref, tol)
+    assert quant.device_status() == 0
