@@ -19,6 +19,7 @@
 // Chunks, bound by the products and by each CTA's own walk over the positions:
 // 200 tokens at 0 21 us, 8 sequences of 40 at 100 20 us (f16); longer ones go to
 // the kernels on tcgen05.
+#include "../../include/hyq.h"
 #include "hyq_kernels.h"
 #include "hyq_paged.cuh"
 
@@ -453,7 +454,8 @@ __device__ __forceinline__ float settled(float y, float l, bool dirty, const Cac
 // Workspace: one counter per CTA, then two partial results per CTA: 16 rows of
 // DIM outputs, then the rows' (maximum, sum), then whether clean() took a value
 // out.
-constexpr size_t kCounterBytes = (kMaxCtas * sizeof(unsigned) + 255) / 256 * 256;
+constexpr size_t kCounterBytes = HYQ_PAGED_ATTENTION_ZEROED;
+static_assert(kCounterBytes >= kMaxCtas * sizeof(unsigned), "a counter per CTA");
 __host__ __device__ constexpr int partial_floats(int dim) { return kRows * (dim + 2) + 4; }
 
 // What a segment costs beside its tiles (queries, first copies, joining the

@@ -27,6 +27,7 @@ _ops = load_ops()
 _KV_TYPES = (torch.float32, torch.float16)
 _PAGES = struct.Struct("PPPPqqqi4x")     # hyq_pages
 _POOL = struct.Struct("Pqqqq")           # hyq_page_pool
+_ZEROED = 4096                           # HYQ_PAGED_ATTENTION_ZEROED
 _current_stream = torch._C._cuda_getCurrentRawStream
 
 
@@ -49,9 +50,11 @@ def _workspace_bytes(heads, head_dim):
 
 
 def attention_workspace(heads, head_dim, device):
-    """A zeroed workspace for attention() calls with these heads (any batch);
-    calls that share one must not overlap in time."""
-    return torch.zeros(_workspace_bytes(heads, head_dim), dtype=torch.uint8, device=device)
+    """A workspace for attention() calls with these heads (any batch), zero where
+    the calls need it; calls that share one must not overlap in time."""
+    workspace = torch.empty(_workspace_bytes(heads, head_dim), dtype=torch.uint8, device=device)
+    workspace[:_ZEROED].zero_()
+    return workspace
 
 
 def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None, slot=None, out=None, workspace=None):

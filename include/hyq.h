@@ -497,8 +497,11 @@ int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, 
  * 256, at most 16 query heads per kv head.  (Outputs are kept 2^10 times their
  * size inside: values from 2^113 up overflow.)
  * workspace: hyq_paged_attention_workspace_bytes bytes (independent of the
- * batch), 16-byte aligned, zero before the first call (every call leaves its
- * counters zero again); calls that share one must not overlap in time. */
+ * batch), 16-byte aligned, its first HYQ_PAGED_ATTENTION_ZEROED bytes zero
+ * before the first call (every call leaves them zero again); calls that share
+ * one must not overlap in time. */
+#define HYQ_PAGED_ATTENTION_ZEROED 4096
+
 int hyq_paged_attention_workspace_bytes(int heads, int head_dim, size_t* bytes);
 int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
                         int heads, float* out, int64_t out_stride, void* workspace, void* stream);

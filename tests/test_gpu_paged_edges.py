@@ -369,3 +369,19 @@ def test_chunk_calls_in_a_graph(cuda, case, overlap):
         ref, tol = _exact(dict(s, q=out))
         _within(again, ref, tol)
     assert quant.device_status() == 0
+
+
+@pytest.mark.parametrize("case", [FEW[1], FEW[3], TC[0], TC32[1]], ids=_ids)
+def test_workspace_of_used_memory(cuda, case):
+    """A workspace in memory that holds NaN and large numbers: only its first
+    bytes are zero."""
+    import torch
+    from hy_mt_rs_b200 import paged
+    s = _case(cuda, case)
+    ref, tol = _exact(s)
+    for x in (math.nan, 1e38):
+        ws = paged.attention_workspace(8, case[5], cuda)
+        ws[4096:] = torch.full((ws.numel() // 4,), x, device=cuda).view(torch.uint8)[:ws.numel() - 4096]
+        _within(_run(case, s, workspace=ws), ref, tol)
+        _within(_run(case, s, workspace=ws), ref, tol)
+        assert int(ws[:4096].amax()) == 0
