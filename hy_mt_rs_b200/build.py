@@ -15,6 +15,7 @@ import os
 import shutil
 import subprocess
 import sys
+from importlib import metadata
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -57,9 +58,12 @@ def _compile(src, verbose):
 
 
 def _build_ops(force):
-    """The Python extension, against the installed torch and this Python."""
+    """The Python extension, against the installed torch and this Python (whose
+    versions are kept beside the objects: it fits no others)."""
     src = os.path.join(CSRC, "py_ops.cpp")
-    if not (force or _stale(OPS, [src, os.path.join(INCLUDE, "hyq.h")])):
+    note, against = os.path.join(BUILD, "ops.against"), f"torch {metadata.version('torch')}, Python {sys.version}"
+    if not (force or _stale(OPS, [src, os.path.join(INCLUDE, "hyq.h")]) or not os.path.exists(note)
+            or open(note).read() != against):
         return
     import sysconfig
 
@@ -74,6 +78,8 @@ def _build_ops(force):
         "-L" + os.path.dirname(LIB), "-l:libhyq.so", "-L" + os.path.join(root, "lib"), "-ltorch_python", "-ltorch_cpu",
         "-lc10", "-lc10_cuda", "-Wl,-rpath,$ORIGIN"])
     os.replace(tmp, OPS)
+    with open(note, "w") as f:
+        f.write(against)
 
 
 def build(force=False, verbose=False):
