@@ -163,6 +163,26 @@ cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st);
 bool tc32_supported(const AttendArgs& a);
 cudaError_t launch_chunks_tc32(const AttendArgs& a, cudaStream_t st);
 
+// Weights are 2^(s - m) of the scores s, which carry log2(e) through the queries,
+// with a reference m of 10 below the row's maximum: kept 2^10 times their size,
+// their lo halves stay normal f16 numbers down to 2^-24 of the largest.  The
+// reference is rounded up, so that no weight passes 2^10 (and f16's range)
+// however coarse the scores are, and kept with the bias taken off, so that a
+// weight is 2^(s - m) to the last bit of s and m.
+constexpr float kBias = 10.0f;
+constexpr float kLog2e = 1.4426950408889634f;
+__device__ __forceinline__ float reference(float top) { return __fsub_ru(top, kBias); }
+
+__device__ __forceinline__ float ex2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  const __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
 // The non-finite values of V at positions first + 1 .. last of a sequence, in N
 // neighbouring columns: their sums (0 where there are none).  An infinity that
 // a row sees is its output whatever the weight, which is above zero: products

@@ -32,12 +32,6 @@ constexpr int kThreads = 32 * kWarps;
 constexpr int kRows = kFewRows;      // query rows of a warp: (token, head) pairs
 constexpr int kCtasPerSm = 2;
 constexpr int kMaxCtas = 148 * kCtasPerSm;
-// Weights are kept 2^10 times their size, so that their lo halves stay normal
-// f16 numbers down to 2^-24 of the largest: they are 2^(s - m) with a reference
-// m of 10 below the row's maximum, rounded up, so that no weight passes 2^10
-// (and f16's range) however coarse the scores are.
-constexpr float kBias = 10.0f;
-constexpr float kLog2e = 1.4426950408889634f;
 
 // A warp's block of positions: POS rows of K, then of V, in 16-byte chunks
 // whose low three index bits are xored with the row (reads by ldmatrix and by
@@ -57,12 +51,6 @@ struct Geo {
   static constexpr int pitch = DIM + 8;
   static constexpr int smem = ring + kRows * pitch * 4;
 };
-
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -92,10 +80,6 @@ __device__ __forceinline__ void copy16(uint32_t dst, const void* src, int bytes)
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes) : "memory");
 }
 
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 __device__ __forceinline__ void split_f16(float a, float b, uint32_t& hi, uint32_t& lo) {
   hi = pack_f16(a, b);
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hi));
@@ -293,7 +277,7 @@ struct Rows {
     float down[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
-      const float now = fmaxf(m[i], __fsub_ru(top[i], kBias));
+      const float now = fmaxf(m[i], reference(top[i]));
       down[i] = now == -INFINITY ? 1.0f : ex2(m[i] - now);
       m[i] = now;
       l[i] *= down[i];

@@ -24,9 +24,7 @@ template <int ROWS>
 __host__ __device__ constexpr size_t part_floats(int dim) {
   return (size_t)ROWS * (dim + 2) + 4;
 }
-constexpr float kBias = 10.0f;           // weights are kept 2^10 times their size (hyq_paged_mma.cu)
 constexpr float kSlack = 5.0f;           // a weight is at most 2^(kBias + kSlack): below f16's 65504
-constexpr float kLog2e = 1.4426950408889634f;
 
 // A segment: its sequence (n rows of tokens from row0 at pos, pages in `slot`),
 // which of the sequence's it is, and the position tiles that come before and
@@ -279,15 +277,6 @@ __device__ __forceinline__ void tmem_each(uint32_t a, F f) {
   }
 }
 
-__device__ __forceinline__ float ex2(float x) {
-  float y;
-  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
-  const __half2 h = __floats2half2_rn(lo, hi);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
 // Ten mantissa bits of a weight (exact in f16 from 2^-14 up).
 __device__ __forceinline__ float high_part(float x) { return __uint_as_float(__float_as_uint(x) & 0xffffe000u); }
 
@@ -380,11 +369,6 @@ __device__ __forceinline__ float stage_rows(const AttendArgs& a, const Piece& x,
   __syncwarp();
   return factor;
 }
-
-// The reference of weights whose largest score is `top`: rounded up, so that no
-// weight passes 2^kBias however coarse the scores are, and kept with the bias
-// taken off, so that a weight is 2^(s - m) to the last bit of s and m.
-__device__ __forceinline__ float reference(float top) { return __fsub_ru(top, kBias); }
 
 // One row's scores of a tile, in tensor memory at `st`, to weights, hi and lo
 // (8 columns each for 16 positions), over them.  Weights are 2^(s - m) with a
