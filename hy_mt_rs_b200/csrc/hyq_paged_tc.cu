@@ -418,7 +418,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   p.box = std::min(a.c.page_size, kTile);
   if (!page_map(&mk, a.c.k, a.c, p.box) || !page_map(&mv, a.c.v, a.c, p.box)) return cudaErrorInvalidValue;
   char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
-  p.plan = plan_of(ws);
+  p.plan = plan_of<kCtaRows>(a, ws);
   p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
   auto k = chunk_tc_kernel<DIM>;
   static std::atomic<uint64_t> done{0};

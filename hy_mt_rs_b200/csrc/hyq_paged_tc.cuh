@@ -43,12 +43,18 @@ struct Plan {
   int* count;      // segments, then the total of their tiles
   Start* start;    // [kMaxCtas + 1]
   Segment* seg;    // [kMaxSegs]
+  int most;        // segments that the rows of the call can make
 };
 constexpr size_t kPlanBytes = 16 + (kMaxCtas + 1) * sizeof(Start) + (size_t)kMaxSegs * sizeof(Segment);
-inline Plan plan_of(void* ws) {
+template <int ROWS>
+inline int64_t most_segments(const AttendArgs& a) {
+  return ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + ROWS - 1) / ROWS + a.c.seqs;
+}
+template <int ROWS>
+inline Plan plan_of(const AttendArgs& a, void* ws) {
   char* p = static_cast<char*>(ws);
   return {reinterpret_cast<int*>(p), reinterpret_cast<Start*>(p + 16),
-          reinterpret_cast<Segment*>(p + 16 + (kMaxCtas + 1) * sizeof(Start))};
+          reinterpret_cast<Segment*>(p + 16 + (kMaxCtas + 1) * sizeof(Start)), (int)most_segments<ROWS>(a)};
 }
 
 struct Params {
@@ -62,7 +68,7 @@ struct Params {
 // 32-bit sum of their tiles at any length.
 template <int ROWS>
 inline bool plan_fits(const AttendArgs& a) {
-  const int64_t segs = ((int64_t)a.c.tokens * (a.heads / a.c.kv_heads) + ROWS - 1) / ROWS + a.c.seqs;
+  const int64_t segs = most_segments<ROWS>(a);
   return segs <= kMaxSegs && segs * ((int64_t)a.c.width * a.c.page_size / kTile + 1 + kSegTiles) <= INT32_MAX;
 }
 
@@ -116,7 +122,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
     segs += total;
   }
   __syncthreads();
-  segs = min(segs, kMaxSegs);
+  segs = min(segs, plan.most);  // (more: rows of several sequences, row_start not ascending)
   int tiles = 0;
   for (int t0 = 0; t0 < segs; t0 += 1024) {
     const int t = t0 + (int)threadIdx.x;

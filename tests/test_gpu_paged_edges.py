@@ -385,3 +385,18 @@ def test_workspace_of_used_memory(cuda, case):
         _within(_run(case, s, workspace=ws), ref, tol)
         _within(_run(case, s, workspace=ws), ref, tol)
         assert int(ws[:4096].amax()) == 0
+
+
+@pytest.mark.parametrize("case", [FEW[0], CHUNK[0], TC[0], TC32[0], OTHER[0]], ids=_ids)
+def test_descending_row_starts_are_reported(cuda, case):
+    """row_start that goes back gives rows to several sequences and others a
+    negative number: HYQ_DEV_BAD_ARGS, and nothing past the rows is written."""
+    import torch
+    from hy_mt_rs_b200 import quant
+    s = _case(cuda, case)
+    n, seqs = s["new"][0], 40
+    t = dict(s, row_start=_int([0, n] * seqs, cuda), pos=s["pos"][:1].repeat(2 * seqs - 1), slots=None,
+             slot=torch.zeros(2 * seqs - 1, dtype=torch.int32, device=cuda))
+    buf = torch.full((n + 8, 8, case[5]), 7.0, device=cuda)
+    _run((case[0], *case[1:]), dict(t, q=s["q"][:n]), out=buf[:n])
+    assert (buf[n:] == 7).all() and quant.device_status() == 8
