@@ -41,13 +41,17 @@ __host__ __device__ inline Plan plan_of(void* ws, int64_t pages) {
   return {p, p + 4, p + 4 + pages, p + 4 + 2 * pages};
 }
 
-// Sum of two counts of pages, at most kMost: 1,024 sequences may ask for more
-// than 2^31 together, and must not seem to ask for few.
+// Sum of two counts, CAPPED at kMost: 1,024 sequences may ask for more than 2^31
+// pages together, and must not seem to ask for few.
 constexpr unsigned kMost = HYQ_PAGES_REFUSED - 1;
-__device__ __forceinline__ int sum_of(int a, int b) { return (int)min((unsigned)a + (unsigned)b, kMost); }
+template <bool CAPPED>
+__device__ __forceinline__ int sum_of(int a, int b) {
+  return CAPPED ? (int)min((unsigned)a + (unsigned)b, kMost) : a + b;
+}
 
 // Exclusive prefix sum of one value per thread over the CTA (1024 threads),
 // right while the total is below kMost; every thread gets the total.
+template <bool CAPPED = false>
 __device__ __forceinline__ int block_scan(int v, int& total) {
   __shared__ int warp_s[kThreads / 32];
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
@@ -55,7 +59,7 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, x, o);
-    if (lane >= o) x = sum_of(x, y);
+    if (lane >= o) x = sum_of<CAPPED>(x, y);
   }
   if (lane == 31) warp_s[warp] = x;
   __syncthreads();
@@ -63,12 +67,12 @@ __device__ __forceinline__ int block_scan(int v, int& total) {
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) {
     const int y = __shfl_up_sync(0xffffffffu, w, o);
-    if (lane >= o) w = sum_of(w, y);
+    if (lane >= o) w = sum_of<CAPPED>(w, y);
   }
   total = __shfl_sync(0xffffffffu, w, 31);
   const int base = warp == 0 ? 0 : __shfl_sync(0xffffffffu, w, warp - 1);
   __syncthreads();  // warp_s may be written again
-  return sum_of(base, x) - v;
+  return sum_of<CAPPED>(base, x) - v;
 }
 
 // The `need` lowest-numbered free pages, in ascending order, into list (as
@@ -154,7 +158,7 @@ __global__ void __launch_bounds__(kThreads)
     return;
   }
   int total;  // (kMost is more than there can be pages)
-  const int at = block_scan(need, total);
+  const int at = block_scan<true>(need, total);
   at_s[i] = at;
   const int found = total ? find_free(t.refs, t.pages, total, w.to) : 0;
   if (pos && i < n) pos[i] = before;
