@@ -43,7 +43,8 @@ __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
 // rotated pair meet in one thread: no value leaves its registers between the
 // load and the store.  Each group takes BATCH heads at a time, their loads in
 // flight together, and with those of the tables.  Bound by memory: 8,208 tokens
-// of 32 query and 8 kv heads of 128 into an f32 cache (403 MB) 84 us, 4.8 TB/s
+// of 32 query and 8 kv heads of 128 into an f32 cache (403 MB) 84 us, 4.8 TB/s, in
+// accesses of 4 bytes a lane, 64 contiguous bytes of a head, with 35 % of the warps
 // (108 us with registers for six CTAs an SM instead of three); 64 tokens 3.6 us.
 template <int DIM, bool KV16>
 __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant__ AppendArgs a) {

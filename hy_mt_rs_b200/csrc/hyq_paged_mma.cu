@@ -13,8 +13,8 @@
 // queries.
 //
 // Few tokens, bound by memory: 64 requests of 90 to 4,000 positions (16 query
-// and 4 kv heads of 128, f16, 269 MB) 53.5 us, 5.0 TB/s; 4 of 60,000 to 100,000
-// (32 and 8 heads, 1.3 GB) 205 to 215 us, 6.1 to 6.4 TB/s; one of 512 positions (f32) 10.7 us,
+// and 4 kv heads of 128, f16, 269 MB) 54 us, 5.0 TB/s; 4 of 60,000 to 100,000
+// (32 and 8 heads, 1.3 GB) 205 to 215 us, 6.1 to 6.4 TB/s; one of 512 positions (f32) 10.4 to 11.1 us,
 // all latency: the plan of the line, the copies, the partial results' join.
 // Chunks, bound by the products and by each CTA's own walk over the positions:
 // 200 tokens at 0 21 us, 8 sequences of 40 at 100 20 us (f16); longer ones go to

@@ -11,8 +11,10 @@
 // four 128 x 128 x 128 products: twice those of plain f16 attention, which is
 // what bounds the kernel (half the tensor cores' f16 rate), together with the
 // power limit.  4,096 tokens over 12,288 positions, 32 query and 8 kv heads of
-// 128: 1.45 to 1.65 ms from box to box, 580 to 660 TFLOP/s of 2 x 2 x heads x
-// head size x pairs, 70 to 80 % of half the measured 1,657.  Two row tiles, so
+// 128: 1.43 ms at 1,965 MHz (ten calls after a pause), 1.64 ms back to back, where
+// the card draws 989 W of its 1,000 and holds 1,507 to 1,575 MHz: 585 to 670
+// TFLOP/s of 2 x 2 x heads x head size x pairs, 71 to 81 % of half the measured
+// 1,657 (tensor pipe 69 % busy).  Two row tiles, so
 // that one's products run under the other's softmax; a tile's 32 steps of 16 take
 // 64 cycles each, its softmax about as long.
 //

@@ -22,7 +22,7 @@
 //                the next tile's weights are multiplied.
 //
 // Three chunks of 201 to 256 tokens over up to 2,300 positions, 16 query and 4
-// kv heads of 128: 65 us with plan and join (the warp-level kernel on tf32 took
+// kv heads of 128: 63 us with plan and join (the warp-level kernel on tf32 took
 // 470).  A CTA's start takes 10 us and a tile of positions 5 us, the chain of its
 // split, scores, weights and outputs; the six products alone take 1.6.
 //

@@ -281,7 +281,8 @@ struct Pool {
 // since the divisions that name it by its number took as long as the copy.
 // Two waves of CTAs, so that the SMs that are done first get more (500 MB of
 // moves 90 us, 5.8 TB/s; 98 with one wave; 67 MB of copies of one page for each
-// of 8 forks 15 us with fork_kernel, 17 with four waves or 4 KB at a time).
+// of 8 forks 15 to 16 us with fork_kernel, 2 more with four waves or 4 KB at a
+// time).
 constexpr int kCopyThreads = 256, kCopyEach = 4, kCopyCtas = 148 * 16;
 __global__ void __launch_bounds__(kCopyThreads) copy_kernel(Table t, Pool pool, Plan w, bool rename) {
   grid_dependency_wait();

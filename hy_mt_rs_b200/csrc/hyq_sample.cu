@@ -112,7 +112,7 @@ __device__ __forceinline__ u64 warp_sum_u64(u64 v) {
 // the bits of the key, then by index.  Then each CTA adds up its kept mass,
 // and the one that holds the draw walks its part.
 //
-// What bounds it: one row is latency (13 us for 0.5 MB: a handful of exchanges
+// What bounds it: one row is latency (14 us for 0.5 MB: a handful of exchanges
 // and scans); many rows, the passes over them: 256 rows of 120,832 logits (124
 // MB) take 24 us greedy (one pass, 5.2 TB/s), 47 us with top-k 40 (two), 92 us
 // without filters (two, 31 M exponentials), 187 us with top-p 0.9 at 0.7 (four)
