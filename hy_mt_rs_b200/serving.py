@@ -47,7 +47,8 @@ class PagedBatch:
         self._known([0] * slots)
 
     def _state(self):
-        return self.cache.changes, self.cache.length._version
+        length = self.cache.length
+        return self.cache.changes, 0 if length.is_inference() else length._version
 
     def _known(self, held):
         """The slots' lengths after the calls so far: exact, or past the cache's

@@ -137,3 +137,19 @@ def test_long_contexts_match_single_requests(cuda, kv16):
     for r, g in enumerate(got):
         assert _close(g, logits[r][1], tol), r
     assert quant.device_status() == 0
+
+
+def test_under_inference_mode(cuda):
+    """A batch made and stepped where tensors have no version counter."""
+    import torch
+    from hy_mt_rs_b200.serving import PagedBatch
+
+    model = _model(cuda, "dense", True)
+    with torch.inference_mode():
+        batch = PagedBatch(model, 2, page_size=16)
+        batch.step([0], [5], _put([1] * 5, cuda))
+        batch.step([0, 1], [1, 3], _put([1] * 4, cuda))
+        assert len(batch.generate([[1, 2, 3]], 4, answers=2)[0][1]) == 4
+    other = PagedBatch(model, 2, page_size=16)
+    other.step([0], [5], _put([1] * 5, cuda))
+    assert batch.generate([[5, 6]], 3) == other.generate([[5, 6]], 3)
