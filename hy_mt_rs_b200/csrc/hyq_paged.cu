@@ -29,11 +29,12 @@ struct AppendArgs {
   int norm_first;
   float* q_out;
   int64_t out_stride;
+  bool vec;  // 8-bit: the codes of a row are 8-byte aligned
 };
 
-template <bool KV16>
+template <Kv KV>
 __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
-  if constexpr (KV16) static_cast<__half*>(base)[i] = __float2half_rn(x);
+  if constexpr (KV == kF16) static_cast<__half*>(base)[i] = __float2half_rn(x);
   else static_cast<float*>(base)[i] = x;
 }
 
@@ -46,9 +47,12 @@ __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
 // of 32 query and 8 kv heads of 128 into an f32 cache (403 MB) 84 us, 4.8 TB/s, in
 // accesses of 4 bytes a lane, 64 contiguous bytes of a head, with 35 % of the warps
 // (108 us with registers for six CTAs an SM instead of three); 64 tokens 3.6 us.
-template <int DIM, bool KV16>
+// Into an 8-bit cache a head's largest magnitude comes from its 16 lanes, and the
+// codes go through shared memory, so that a lane writes neighbouring ones.
+template <int DIM, Kv KV>
 __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int EL = DIM / 16, BATCH = 3;
+  __shared__ __align__(8) uint8_t codes_s[is_8bit(KV) ? 256 : 8][is_8bit(KV) ? EL : 8];  // DIM of each group of 16 lanes
   grid_dependency_wait();
   allow_dependents_launch();
   const int t = blockIdx.x, l = threadIdx.x & 15, part = threadIdx.x >> 4;
@@ -92,6 +96,7 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
     sn[i] = a.sin_tab[(int64_t)pos * (DIM / 2) + l + 16 * i];
   }
   const int64_t row = (int64_t)page * a.c.page_stride + (int64_t)(pos % a.c.page_size) * a.c.row_stride;
+  const int64_t scales = is_8bit(KV) ? scale_at(a.c, page, 0, pos % a.c.page_size) : 0;
   for (int u0 = part; u0 - part < units; u0 += 16 * BATCH) {
     if (u0 != part) load(u0);
 #pragma unroll
@@ -121,6 +126,23 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
         }
       }
       if (!a.norm_first) norm();
+      uint32_t top = 0;
+      if constexpr (is_8bit(KV)) {
+#pragma unroll
+        for (int i = 0; i < EL; ++i) top = max(top, __float_as_uint(x[b][i]) & 0x7fffffffu);
+#pragma unroll
+        for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
+      }
+      if (is_8bit(KV)) __syncwarp();  // the codes of the heads before are out
+      const float scale = is_8bit(KV) ? row_scale<KV>(top) : 1.f;
+      if constexpr (is_8bit(KV)) {
+        uint8_t* mine = codes_s[threadIdx.x & ~15];
+        if (!is_q && u < units) {
+#pragma unroll
+          for (int i = 0; i < EL; ++i) mine[l + 16 * i] = encode<KV>(x[b][i], scale);
+        }
+        __syncwarp();
+      }
       if (u >= units) continue;
       if (is_q) {
         float* to = a.q_out + t * a.out_stride + u * DIM + l;
@@ -129,8 +151,22 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
       } else {
         const int kh = (u - a.heads) % a.c.kv_heads;
         const int64_t to = row + kh * a.c.head_stride + l;
+        void* base = rotated ? a.c.k : a.c.v;
+        if constexpr (is_8bit(KV)) {
+          uint8_t* y = static_cast<uint8_t*>(base) + to + (EL - 1) * l;
+          const uint8_t* from = codes_s[threadIdx.x];
+          if (a.vec) {
+            if constexpr (EL == 8) *reinterpret_cast<uint2*>(y) = *reinterpret_cast<const uint2*>(from);
+            else *reinterpret_cast<uint32_t*>(y) = *reinterpret_cast<const uint32_t*>(from);
+          } else {
 #pragma unroll
-        for (int i = 0; i < EL; ++i) store_kv<KV16>(rotated ? a.c.k : a.c.v, to + 16 * i, x[b][i]);
+            for (int i = 0; i < EL; ++i) y[i] = from[i];
+          }
+          if (l == 0) (rotated ? a.c.k_scale : a.c.v_scale)[scales + kh * a.c.scale_head_stride] = scale;
+        } else {
+#pragma unroll
+          for (int i = 0; i < EL; ++i) store_kv<KV>(base, to + 16 * i, x[b][i]);
+        }
       }
     }
   }
@@ -138,7 +174,7 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
 
 // Any other even head size: a warp per head at a time, the head in
 // shared memory; sums in the order of dot_x86.
-template <bool KV16>
+template <Kv KV>
 __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ AppendArgs a) {
   grid_dependency_wait();
   allow_dependents_launch();
@@ -158,11 +194,23 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   const float* cs = a.cos_tab + (int64_t)pos * half;
   const float* sn = a.sin_tab + (int64_t)pos * half;
   const int64_t row = (int64_t)page * a.c.page_stride + (int64_t)(pos % a.c.page_size) * a.c.row_stride;
+  // a head's values into an 8-bit cache
+  auto quantise = [&](const float* x, void* base, float* scale_base, int kh) {
+    uint32_t top = 0;
+    for (int i = lane; i < dim; i += 32) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    const float scale = row_scale<KV>(__reduce_max_sync(0xffffffffu, top));
+    for (int i = lane; i < dim; i += 32) static_cast<uint8_t*>(base)[row + kh * a.c.head_stride + i] = encode<KV>(x[i], scale);
+    if (lane == 0) scale_base[scale_at(a.c, page, kh, pos % a.c.page_size)] = scale;
+  };
   for (int u = warp; u < a.heads + 2 * a.c.kv_heads; u += 8) {
     if (u >= a.heads + a.c.kv_heads) {  // a value head: copied as it is
       const int kh = u - a.heads - a.c.kv_heads;
       const float* x = a.v + t * a.v_stride + kh * dim;
-      for (int i = lane; i < dim; i += 32) store_kv<KV16>(a.c.v, row + kh * a.c.head_stride + i, x[i]);
+      if constexpr (is_8bit(KV)) {
+        quantise(x, a.c.v, a.c.v_scale, kh);
+      } else {
+        for (int i = lane; i < dim; i += 32) store_kv<KV>(a.c.v, row + kh * a.c.head_stride + i, x[i]);
+      }
       continue;
     }
     const bool is_q = u < a.heads;
@@ -188,9 +236,13 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
       }
       __syncwarp();
     }
+    if (is_8bit(KV) && !is_q) {
+      if constexpr (is_8bit(KV)) quantise(h, a.c.k, a.c.k_scale, kh);
+      continue;
+    }
     for (int i = lane; i < dim; i += 32) {
       if (is_q) a.q_out[t * a.out_stride + u * dim + i] = h[i];
-      else store_kv<KV16>(a.c.k, row + kh * a.c.head_stride + i, h[i]);
+      else store_kv<KV>(a.c.k, row + kh * a.c.head_stride + i, h[i]);
     }
   }
 }
@@ -199,10 +251,11 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
 // Attention
 // ---------------------------------------------------------------------------
 
-template <bool KV16>
+template <Kv KV>
 __device__ __forceinline__ float load_kv(const void* base, int64_t i) {
-  if constexpr (KV16) return __half2float(static_cast<const __half*>(base)[i]);
-  else return static_cast<const float*>(base)[i];
+  if constexpr (KV == kF16) return __half2float(static_cast<const __half*>(base)[i]);
+  else if constexpr (KV == kF32) return static_cast<const float*>(base)[i];
+  else return code_value<KV>(static_cast<const uint8_t*>(base)[i]);
 }
 
 // Any head size, strides and page size.  One CTA per (row, kv head): chunks
@@ -210,11 +263,12 @@ __device__ __forceinline__ float load_kv(const void* base, int64_t i) {
 // position) score, a running maximum and sum per query head (online softmax),
 // OUTS outputs of the group's heads x dim per thread in registers.  Reads
 // only positions the row sees.  For what the others do not take: head sizes
-// other than 64 and 128, rows that are not 16-byte aligned.
+// other than 64 and 128, rows that are not 16-byte aligned.  (Of an 8-bit cache it
+// stages code * scale.)
 constexpr int kChunk = 32;
 constexpr int kThreads = 128;
 
-template <bool KV16, int OUTS>
+template <Kv KV, int OUTS>
 __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant__ AttendArgs a) {
   grid_dependency_wait();
   allow_dependents_launch();
@@ -250,9 +304,19 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
       const int p = p0 + i, page = checked_page(a.c, sq.pages[p / a.c.page_size]);
       const int64_t at = (int64_t)max(page, 0) * a.c.page_stride + (int64_t)kvh * a.c.head_stride +
                          (int64_t)(p % a.c.page_size) * a.c.row_stride;
+      float k_unit = 1.f, v_unit = 1.f;
+      if constexpr (is_8bit(KV)) {
+        const int64_t s = scale_at(a.c, max(page, 0), kvh, p % a.c.page_size);
+        k_unit = page < 0 ? 0.f : a.c.k_scale[s];
+        v_unit = page < 0 ? 0.f : a.c.v_scale[s];
+      }
       for (int d = threadIdx.x & 31; d < dim; d += 32) {
-        k_s[i * ks + d] = page < 0 ? 0.f : load_kv<KV16>(a.c.k, at + d);
-        v_s[i * ks + d] = page < 0 ? 0.f : load_kv<KV16>(a.c.v, at + d);
+        k_s[i * ks + d] = page < 0 ? 0.f : load_kv<KV>(a.c.k, at + d);
+        v_s[i * ks + d] = page < 0 ? 0.f : load_kv<KV>(a.c.v, at + d);
+        if constexpr (is_8bit(KV)) {
+          k_s[i * ks + d] *= k_unit;
+          v_s[i * ks + d] *= v_unit;
+        }
       }
     }
     __syncthreads();
@@ -300,8 +364,8 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
     if (i >= G * dim) break;
     const float l = l_s[i / dim];
     float y = o[j] / l;
-    if (!isfinite(y) && isfinite(l)) {
-      const float x = non_finite<KV16, 1>(a.c, sq, kvh, -1, seen - 1, i % dim).v[0];
+    if (!is_8bit(KV) && !isfinite(y) && isfinite(l)) {
+      const float x = non_finite<KV == kF16, 1>(a.c, sq, kvh, -1, seen - 1, i % dim).v[0];
       if (x != 0.f) y = x;
     }
     a.out[t * a.out_stride + (int64_t)kvh * G * dim + i] = y;
@@ -312,16 +376,87 @@ size_t attend_smem(int dim, int group) {
   return sizeof(float) * ((2 * kChunk + group) * (size_t)(dim + 1) + (size_t)group * (kChunk + 3));
 }
 
-template <bool KV16>
+template <Kv KV>
 cudaError_t launch_attend(const AttendArgs& a, cudaStream_t st) {
   const int group = a.heads / a.c.kv_heads, outs = (group * a.c.dim + kThreads - 1) / kThreads;
   const int variant = outs <= 4 ? 0 : outs <= 8 ? 1 : 2;
-  auto k = variant == 0 ? attend_kernel<KV16, 4> : variant == 1 ? attend_kernel<KV16, 8> : attend_kernel<KV16, 32>;
+  auto k = variant == 0 ? attend_kernel<KV, 4> : variant == 1 ? attend_kernel<KV, 8> : attend_kernel<KV, 32>;
   static std::atomic<uint64_t> done[3] = {};
   const cudaError_t e = allow_smem(k, (int)attend_smem(kMaxDim, kMaxGroup), done[variant]);
   if (e != cudaSuccess) return e;
   return launch_ex(k, dim3((unsigned)a.c.tokens, (unsigned)a.c.kv_heads), dim3(kThreads),
                    attend_smem(a.c.dim, group), st, a);
+}
+
+// ---------------------------------------------------------------------------
+// Reading rows back
+// ---------------------------------------------------------------------------
+
+struct GatherArgs {
+  Cache c;
+  void* k;
+  void* v;
+  int64_t k_stride, v_stride;  // elements
+  bool vec;                    // four values of a row at a time are aligned, in and out
+};
+
+// One CTA per row of the output, a warp per (kv head, K or V), four values a lane
+// (or one, where they are not aligned).  Bound by memory.
+template <Kv KV, typename T>
+__global__ void __launch_bounds__(256) gather_kernel(const __grid_constant__ GatherArgs a) {
+  grid_dependency_wait();
+  allow_dependents_launch();
+  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = a.c.dim;
+  const int s = seq_of_row(a.c, t);
+  if (s < 0) return;
+  const Seq sq = load_seq(a.c, s);
+  if (t - sq.row0 >= sq.n) return;
+  const int pos = sq.pos + (t - sq.row0), in_page = pos % a.c.page_size;
+  const int page = checked_page(a.c, sq.pages[pos / a.c.page_size]);
+  for (int u = warp; u < 2 * a.c.kv_heads; u += 8) {
+    const bool is_k = u < a.c.kv_heads;
+    const int kh = is_k ? u : u - a.c.kv_heads;
+    const void* base = is_k ? a.c.k : a.c.v;
+    T* to = static_cast<T*>(is_k ? a.k : a.v) + t * (is_k ? a.k_stride : a.v_stride) + (int64_t)kh * dim;
+    const int64_t at = (int64_t)max(page, 0) * a.c.page_stride + (int64_t)kh * a.c.head_stride + (int64_t)in_page * a.c.row_stride;
+    float unit = 1.f;
+    if constexpr (is_8bit(KV)) unit = page < 0 ? 0.f : (is_k ? a.c.k_scale : a.c.v_scale)[scale_at(a.c, page, kh, in_page)];
+    auto value = [&](float x) { return page < 0 ? 0.f : x * unit; };
+    if (a.vec) {
+      for (int d = 4 * lane; d < dim; d += 128) {
+        float x[4];
+        if constexpr (KV == kF32) {
+          const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at + d);
+          x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
+        } else if constexpr (KV == kF16) {
+          const uint2 h = *reinterpret_cast<const uint2*>(static_cast<const __half*>(base) + at + d);
+          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
+          x[0] = f0.x, x[1] = f0.y, x[2] = f1.x, x[3] = f1.y;
+        } else {
+          const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(base) + at + d);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[i] = code_value<KV>((uint8_t)(w >> (8 * i)));
+        }
+        if constexpr (sizeof(T) == 4)
+          *reinterpret_cast<float4*>(to + d) = make_float4(value(x[0]), value(x[1]), value(x[2]), value(x[3]));
+        else
+          *reinterpret_cast<uint2*>(to + d) = make_uint2(pack_f16(value(x[0]), value(x[1])), pack_f16(value(x[2]), value(x[3])));
+      }
+    } else {
+      for (int d = lane; d < dim; d += 32) to[d] = (T)value(load_kv<KV>(base, at + d));
+    }
+  }
+}
+
+template <Kv KV>
+cudaError_t launch_gather(const GatherArgs& a, bool f16, cudaStream_t st) {
+  return launch_ex(f16 ? gather_kernel<KV, __half> : gather_kernel<KV, float>, dim3((unsigned)a.c.tokens), dim3(256), 0, st, a);
+}
+
+template <Kv KV>
+cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
+  auto kern = a.c.dim == 128 ? append_rows_kernel<128, KV> : a.c.dim == 64 ? append_rows_kernel<64, KV> : append_kernel<KV>;
+  return launch_ex(kern, dim3((unsigned)a.c.tokens), dim3(256), 0, st, a);
 }
 
 }  // namespace paged
@@ -336,12 +471,17 @@ using hyq::api_fail;
 
 bool aligned(const void* p, size_t a) { return reinterpret_cast<uintptr_t>(p) % a == 0; }
 
-int make_cache(const hyq_paged_kv* kv, const hyq_paged_batch* b, int heads, const char* name, bool attends,
-               hyq::paged::Cache& c) {
+// kv8: the same cache's scales, where the call takes 8-bit ones.
+int make_cache(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_paged_batch* b, int heads, const char* name,
+               bool attends, hyq::paged::Cache& c) {
   if (!kv || !b || !kv->k || !kv->v || !kv->table || (b->seqs > 0 && (!b->row_start || !b->pos)))
     return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
-  if (kv->dtype != HYQ_KV_F32 && kv->dtype != HYQ_KV_F16)
+  const bool coded = kv8 && (kv->dtype == HYQ_KV_I8 || kv->dtype == HYQ_KV_F8);
+  if (kv->dtype != HYQ_KV_F32 && kv->dtype != HYQ_KV_F16 && !coded)
     return api_fail(HYQ_E_INVALID, "%s: unknown cache type %d", name, kv->dtype);
+  if (coded && (!kv8->k_scale || !kv8->v_scale)) return api_fail(HYQ_E_INVALID, "%s: an 8-bit cache without scales", name);
+  if (coded && (kv8->scale_page_stride <= 0 || kv8->scale_head_stride <= 0 || kv8->scale_row_stride <= 0))
+    return api_fail(HYQ_E_SHAPE, "%s: strides of the scales", name);
   if (kv->kv_heads <= 0 || kv->head_dim <= 0 || kv->page_size <= 0 || kv->pages <= 0 || kv->pages > INT32_MAX ||
       kv->slots <= 0 || kv->slots > INT32_MAX || kv->table_width <= 0 ||
       kv->table_width > (INT32_MAX - hyq::paged::kPastEnd) / kv->page_size)
@@ -361,7 +501,9 @@ int make_cache(const hyq_paged_kv* kv, const hyq_paged_batch* b, int heads, cons
                     (long long)b->seqs, (long long)(kv->table_width * kv->page_size));
   if (!b->slot && b->seqs > kv->slots)
     return api_fail(HYQ_E_SHAPE, "%s: %lld sequences, %lld table rows", name, (long long)b->seqs, (long long)kv->slots);
-  const size_t esize = kv->dtype == HYQ_KV_F16 ? 2 : 4;
+  const size_t esize = hyq::paged::value_bytes((hyq::paged::Kv)kv->dtype);
+  if (coded && (!aligned(kv8->k_scale, 4) || !aligned(kv8->v_scale, 4)))
+    return api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
   if (!aligned(kv->k, esize) || !aligned(kv->v, esize) || !aligned(kv->table, 4) || !aligned(b->row_start, 4) ||
       !aligned(b->pos, 4) || !aligned(b->slot, 4))
     return api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
@@ -382,6 +524,13 @@ int make_cache(const hyq_paged_kv* kv, const hyq_paged_batch* b, int heads, cons
   c.pos = b->pos;
   c.seqs = (int)b->seqs;
   c.tokens = (int)b->tokens;
+  if (coded) {
+    c.k_scale = kv8->k_scale;
+    c.v_scale = kv8->v_scale;
+    c.scale_page_stride = kv8->scale_page_stride;
+    c.scale_head_stride = kv8->scale_head_stride;
+    c.scale_row_stride = kv8->scale_row_stride;
+  }
   return hyq::api_status_word(&c.status);
 }
 
@@ -389,18 +538,14 @@ int done(cudaError_t e, const char* name) {
   return e == cudaSuccess ? HYQ_OK : api_fail(HYQ_E_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }
 
-}  // namespace
-
-extern "C" {
-
-int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
-                          int heads, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+int rope_append(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                int heads, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                           const float* cos_tab, const float* sin_tab, int64_t positions, const float* q_norm,
                           const float* k_norm, float eps, int norm_first, float* q_out, int64_t out_stride,
                           void* stream) {
   const char* name = "paged_rope_append";
   hyq::paged::AppendArgs a{};
-  const int rc = make_cache(kv, batch, heads, name, false, a.c);
+  const int rc = make_cache(kv, kv8, batch, heads, name, false, a.c);
   if (rc) return rc;
   if (batch->seqs == 0 || batch->tokens == 0) return HYQ_OK;
   if (!q || !k || !v || !cos_tab || !sin_tab || !q_out) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
@@ -430,26 +575,21 @@ int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, 
   a.q_out = q_out;
   a.out_stride = out_stride;
   using namespace hyq::paged;
-  const bool kv16 = kv->dtype == HYQ_KV_F16;
-  auto kern = kv->head_dim == 128  ? (kv16 ? append_rows_kernel<128, true> : append_rows_kernel<128, false>)
-              : kv->head_dim == 64 ? (kv16 ? append_rows_kernel<64, true> : append_rows_kernel<64, false>)
-                                   : (kv16 ? append_kernel<true> : append_kernel<false>);
-  return done(hyq::launch_ex(kern, dim3((unsigned)batch->tokens), dim3(256), 0, (cudaStream_t)stream, a), name);
+  a.vec = a.c.dim % 8 == 0 && ((a.c.page_stride | a.c.head_stride | a.c.row_stride) & 7) == 0 && aligned(a.c.k, 8) && aligned(a.c.v, 8);
+  const cudaStream_t st = (cudaStream_t)stream;
+  switch (kv->dtype) {
+    case kF32: return done(launch_append<kF32>(a, st), name);
+    case kF16: return done(launch_append<kF16>(a, st), name);
+    case kI8: return done(launch_append<kI8>(a, st), name);
+    default: return done(launch_append<kF8>(a, st), name);
+  }
 }
 
-int hyq_paged_attention_workspace_bytes(int heads, int head_dim, size_t* bytes) {
-  if (!bytes) return api_fail(HYQ_E_INVALID, "paged_attention_workspace_bytes: null pointer");
-  if (heads <= 0 || head_dim <= 0 || head_dim > hyq::paged::kMaxDim)
-    return api_fail(HYQ_E_SHAPE, "paged_attention_workspace_bytes: shape");
-  *bytes = hyq::paged::mma_workspace_bytes(head_dim) + hyq::paged::tc_workspace_bytes(head_dim);
-  return HYQ_OK;
-}
-
-int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
-                        int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
+int attention(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+              int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
   const char* name = "paged_attention";
   hyq::paged::AttendArgs a{};
-  const int rc = make_cache(kv, batch, heads, name, true, a.c);
+  const int rc = make_cache(kv, kv8, batch, heads, name, true, a.c);
   if (rc) return rc;
   if (batch->seqs == 0 || batch->tokens == 0 || batch->max_new == 0) return HYQ_OK;
   if (!q || !out || !workspace) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
@@ -464,21 +604,96 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
   a.out_stride = out_stride;
   a.ws = workspace;
   const cudaStream_t st = (cudaStream_t)stream;
-  const bool kv16 = kv->dtype == HYQ_KV_F16;
-  if (hyq::paged::mma_supported(a, kv16)) {
+  using namespace hyq::paged;
+  const Kv type = (Kv)kv->dtype;
+  if (mma_supported(a, type)) {
     cudaError_t e;
-    if (batch->max_new * (heads / kv->kv_heads) <= hyq::paged::kFewRows) {
-      e = hyq::paged::launch_few(a, kv16, false, st);
-    } else if (hyq::paged::chunks_short(a, kv16, batch->max_len) ||
-               !(kv16 ? hyq::paged::tc_supported(a) : hyq::paged::tc32_supported(a))) {
-      e = hyq::paged::launch_chunks(a, kv16, st);
-      if (e == cudaSuccess) e = hyq::paged::launch_few(a, kv16, true, st);
+    if (batch->max_new * (heads / kv->kv_heads) <= kFewRows) {
+      e = launch_few(a, type, false, st);
+    } else if (is_8bit(type) || chunks_short(a, type, batch->max_len) || !(type == kF16 ? tc_supported(a) : tc32_supported(a))) {
+      e = launch_chunks(a, type, st);
+      if (e == cudaSuccess) e = launch_few(a, type, true, st);
     } else {
-      e = kv16 ? hyq::paged::launch_chunks_tc(a, st) : hyq::paged::launch_chunks_tc32(a, st);
+      e = type == kF16 ? launch_chunks_tc(a, st) : launch_chunks_tc32(a, st);
     }
     return done(e, name);
   }
-  return done(kv16 ? hyq::paged::launch_attend<true>(a, st) : hyq::paged::launch_attend<false>(a, st), name);
+  switch (type) {
+    case kF32: return done(launch_attend<kF32>(a, st), name);
+    case kF16: return done(launch_attend<kF16>(a, st), name);
+    case kI8: return done(launch_attend<kI8>(a, st), name);
+    default: return done(launch_attend<kF8>(a, st), name);
+  }
+}
+
+}  // namespace
+
+extern "C" {
+
+int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                          int heads, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                          const float* cos_tab, const float* sin_tab, int64_t positions, const float* q_norm,
+                          const float* k_norm, float eps, int norm_first, float* q_out, int64_t out_stride,
+                          void* stream) {
+  return rope_append(kv, nullptr, batch, q, q_stride, heads, k, k_stride, v, v_stride, cos_tab, sin_tab, positions, q_norm, k_norm,
+                     eps, norm_first, q_out, out_stride, stream);
+}
+
+int hyq_paged_rope_append_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                              int heads, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                              const float* cos_tab, const float* sin_tab, int64_t positions, const float* q_norm,
+                              const float* k_norm, float eps, int norm_first, float* q_out, int64_t out_stride,
+                              void* stream) {
+  return rope_append(kv ? &kv->kv : nullptr, kv, batch, q, q_stride, heads, k, k_stride, v, v_stride, cos_tab, sin_tab, positions,
+                     q_norm, k_norm, eps, norm_first, q_out, out_stride, stream);
+}
+
+int hyq_paged_attention_workspace_bytes(int heads, int head_dim, size_t* bytes) {
+  if (!bytes) return api_fail(HYQ_E_INVALID, "paged_attention_workspace_bytes: null pointer");
+  if (heads <= 0 || head_dim <= 0 || head_dim > hyq::paged::kMaxDim)
+    return api_fail(HYQ_E_SHAPE, "paged_attention_workspace_bytes: shape");
+  *bytes = hyq::paged::mma_workspace_bytes(head_dim) + hyq::paged::tc_workspace_bytes(head_dim);
+  return HYQ_OK;
+}
+
+int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                        int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
+  return attention(kv, nullptr, batch, q, q_stride, heads, out, out_stride, workspace, stream);
+}
+
+int hyq_paged_attention_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                            int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
+  return attention(kv ? &kv->kv : nullptr, kv, batch, q, q_stride, heads, out, out_stride, workspace, stream);
+}
+
+int hyq_paged_gather(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, int f16, void* k, int64_t k_stride, void* v,
+                     int64_t v_stride, void* stream) {
+  const char* name = "paged_gather";
+  using namespace hyq::paged;
+  GatherArgs a{};
+  const int rc = make_cache(kv ? &kv->kv : nullptr, kv, batch, kv ? kv->kv.kv_heads : 1, name, false, a.c);
+  if (rc) return rc;
+  if (batch->seqs == 0 || batch->tokens == 0) return HYQ_OK;
+  if (!k || !v) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
+  const int64_t width = (int64_t)a.c.kv_heads * a.c.dim;
+  if (k_stride < width || v_stride < width) return api_fail(HYQ_E_SHAPE, "%s: shape of the outputs", name);
+  const size_t esize = f16 ? 2 : 4;
+  if (!aligned(k, esize) || !aligned(v, esize)) return api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
+  const Kv type = (Kv)kv->kv.dtype;
+  a.k = k;
+  a.v = v;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  const size_t in = 4 * value_bytes(type);
+  a.vec = ((a.c.dim | a.c.page_stride | a.c.head_stride | a.c.row_stride | k_stride | v_stride) & 3) == 0 && aligned(a.c.k, in) &&
+          aligned(a.c.v, in) && aligned(k, 4 * esize) && aligned(v, 4 * esize);
+  const cudaStream_t st = (cudaStream_t)stream;
+  switch (type) {
+    case kF32: return done(launch_gather<kF32>(a, f16, st), name);
+    case kF16: return done(launch_gather<kF16>(a, f16, st), name);
+    case kI8: return done(launch_gather<kI8>(a, f16, st), name);
+    default: return done(launch_gather<kF8>(a, f16, st), name);
+  }
 }
 
 }  // extern "C"

@@ -3,6 +3,7 @@
 #pragma once
 
 #include <cuda_fp16.h>
+#include <cuda_fp8.h>
 #include <cuda_runtime.h>
 
 #include <cstdint>
@@ -14,6 +15,12 @@ namespace paged {
 
 constexpr int kMaxDim = 256;
 constexpr int kMaxGroup = 16;  // query heads per kv head
+
+// Type of a cache (HYQ_KV_*).  A row of an 8-bit one is dim codes and one f32
+// scale: a value is code * scale.
+enum Kv { kF32 = 0, kF16 = 1, kI8 = 2, kF8 = 3 };
+__host__ __device__ constexpr bool is_8bit(Kv kv) { return kv == kI8 || kv == kF8; }
+__host__ __device__ constexpr int value_bytes(Kv kv) { return kv == kF32 ? 4 : kv == kF16 ? 2 : 1; }
 
 // hyq_paged_kv + hyq_paged_batch (include/hyq.h), as the kernels take them.
 struct Cache {
@@ -29,6 +36,9 @@ struct Cache {
   const int32_t* pos;        // [seqs]
   int seqs, tokens;
   unsigned* status;
+  float* k_scale;  // 8-bit caches: a scale per row
+  float* v_scale;
+  int64_t scale_page_stride, scale_head_stride, scale_row_stride;  // elements
 };
 
 // One sequence's new tokens.
@@ -83,6 +93,51 @@ __device__ __forceinline__ int checked_page(const Cache& c, int page) {
   return -1;
 }
 
+// Four codes of an 8-bit cache as two f16 pairs: bytes 0 and 2 in `even`, 1 and 3
+// in `odd`, exactly.  int8: 1024 + 128 + code is built in the bits of an f16 and
+// 1152 taken off.  e4m3: its exponent and mantissa bits are an f16's three places
+// further up, which makes 2^-8 of the value (code_unit(); subnormals too); there is no
+// code for NaN, 0x7f and 0xff are +-480.
+template <Kv KV>
+__device__ __forceinline__ void decode4(uint32_t w, uint32_t& even, uint32_t& odd) {
+  if constexpr (KV == kI8) {
+    const __half2 off = __floats2half2_rn(1152.f, 1152.f);
+    const uint32_t e = (w & 0x00ff00ffu) ^ 0x64806480u, o = ((w >> 8) & 0x00ff00ffu) ^ 0x64806480u;
+    const __half2 he = __hsub2(*reinterpret_cast<const __half2*>(&e), off), ho = __hsub2(*reinterpret_cast<const __half2*>(&o), off);
+    even = *reinterpret_cast<const uint32_t*>(&he);
+    odd = *reinterpret_cast<const uint32_t*>(&ho);
+  } else {
+    even = ((w << 8) & 0x80008000u) | ((w << 7) & 0x3f803f80u);
+    odd = (w & 0x80008000u) | ((w >> 1) & 0x3f803f80u);
+  }
+}
+template <Kv KV>
+__device__ __forceinline__ constexpr float code_unit() { return KV == kF8 ? 256.f : 1.f; }
+template <Kv KV>
+__device__ __forceinline__ float code_value(uint8_t c) {
+  if constexpr (KV == kI8) return (float)(int8_t)c;
+  const __half_raw h{(unsigned short)(((c & 0x80u) << 8) | ((c & 0x7fu) << 7))};
+  return 256.f * __half2float(h);
+}
+// Scales of a row (element offset for page, kv head and row in the page).
+__device__ __forceinline__ int64_t scale_at(const Cache& c, int page, int kvh, int row) {
+  return (int64_t)page * c.scale_page_stride + (int64_t)kvh * c.scale_head_stride + (int64_t)row * c.scale_row_stride;
+}
+// The scale of a row whose largest magnitude has these bits: NaN for a row with
+// an infinity or NaN, which then reads back as NaN throughout.
+template <Kv KV>
+__device__ __forceinline__ float row_scale(uint32_t top) {
+  return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(top), KV == kI8 ? 127.f : 448.f);
+}
+// Code of x in a row of this scale: the nearest, ties to even.
+template <Kv KV>
+__device__ __forceinline__ uint8_t encode(float x, float scale) {
+  if (!(scale > 0.f)) return 0;  // zeros, or a row that reads back as NaN
+  const float y = __fdiv_rn(x, scale);
+  if constexpr (KV == kI8) return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(y)));
+  return (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+}
+
 // A tile of `rows` of a sequence's (token, query head) rows of one kv head.
 // Tiles are numbered over the sequences with more than kFewRows such rows.
 constexpr int kFewRows = 16;
@@ -126,6 +181,9 @@ struct AttendArgs {
   float* out;
   int64_t out_stride;
   void* ws;
+  // attention over a part of the positions only (null otherwise):
+  const int32_t* first;  // [seqs] a sequence's positions from here on
+  float2* ml;            // [tokens, heads] each output's reference and sum of weights, written with it
 };
 
 // The kernels round a sequence's length up to tiles and look some tiles ahead, in
@@ -137,15 +195,15 @@ constexpr int kPastEnd = 4096;
 constexpr int kMaxSeqs = 4096;
 
 // hyq_paged_mma.cu: head sizes 64 and 128 over 16-byte aligned rows.
-bool mma_supported(const AttendArgs& a, bool kv16);
+bool mma_supported(const AttendArgs& a, Kv kv);
 size_t mma_workspace_bytes(int dim);
 // Whether launch_few's 32-bit sum of tiles holds that many sequences of any
 // length up to `reach` (4,096 of 16 million positions).
 bool sums_fit(int64_t seqs, int64_t reach);
 // Sequences of up to kFewRows rows; `beside`: next to the kernel that the same
 // call launched before.
-cudaError_t launch_few(const AttendArgs& a, bool kv16, bool beside, cudaStream_t st);
-cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st);  // the others
+cudaError_t launch_few(const AttendArgs& a, Kv kv, bool beside, cudaStream_t st);
+cudaError_t launch_chunks(const AttendArgs& a, Kv kv, cudaStream_t st);  // the others
 // Whether that is faster than the kernels on tcgen05: one launch instead of
 // three, but every CTA goes through its rows' positions alone, at 0.04 us (f16
 // caches) or 0.16 us (f32) for each.  Measured with 16 query and 4 kv heads, us
@@ -153,7 +211,7 @@ cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st);  // 
 // 28; 5 tokens at 300, 64 sequences 31 / 51; 64 tokens at 500 36 / 34; 40 tokens
 // at 300, 32 sequences 60 / 48; f32, 16 tokens at 0 13 / 21; 64 tokens at 0 21 /
 // 21; 8 tokens at 100, 8 sequences 29 / 22.
-bool chunks_short(const AttendArgs& a, bool kv16, int64_t max_len);
+bool chunks_short(const AttendArgs& a, Kv kv, int64_t max_len);
 // hyq_paged_tc.cu: the others on tcgen05 (f16 caches; the workspace past
 // mma_workspace_bytes), and launch_few beside them.
 bool tc_supported(const AttendArgs& a);

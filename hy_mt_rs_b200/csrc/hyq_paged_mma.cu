@@ -35,14 +35,16 @@ constexpr int kMaxCtas = 148 * kCtasPerSm;
 
 // A warp's block of positions: POS rows of K, then of V, in 16-byte chunks
 // whose low three index bits are xored with the row (reads by ldmatrix and by
-// words then fall into distinct banks).  8 KB for head size 128.
-template <int DIM, bool KV16>
+// words then fall into distinct banks; 8-bit caches: place()).  8 KB for head
+// size 128.
+template <int DIM, Kv KV>
 struct Geo {
-  static constexpr int pos = KV16 ? 16 : 8;
-  static constexpr int row_bytes = DIM * (KV16 ? 2 : 4);
+  static constexpr int pos = is_8bit(KV) ? 32 : KV == kF16 ? 16 : 8;
+  static constexpr int row_bytes = DIM * value_bytes(KV);
   static constexpr int chunks = row_bytes / 16;
-  static constexpr int block = 2 * pos * row_bytes;
-  static constexpr int stages = 24576 / block;        // 3 (head size 128), 6 (64)
+  static constexpr int scales = 2 * pos * row_bytes;   // 8-bit: K's, then V's, behind the codes
+  static constexpr int block = scales + (is_8bit(KV) ? 2 * pos * 4 : 0);
+  static constexpr int stages = (is_8bit(KV) ? 25344 : 24576) / block;  // 3 (head size 128), 6 or 5 (64)
   static constexpr int tile = kWarps * pos;           // positions of a CTA's step
   static constexpr int copies = pos * chunks / 32;    // 16-byte copies per lane, K or V
   static constexpr int ring = kWarps * stages * block;
@@ -51,6 +53,15 @@ struct Geo {
   static constexpr int pitch = DIM + 8;
   static constexpr int smem = ring + kRows * pitch * 4;
 };
+
+// Place of chunk c of row `row` of an 8-bit cache's K or V.  The products' operands
+// come by 16-byte (V of head size 64: 8-byte) loads of a whole warp: of K, chunks
+// 0 .. 3 of eight neighbouring rows, of V, neighbouring chunks of every other row.
+template <int DIM>
+__device__ __forceinline__ int place(int row, int c, bool v) {
+  if constexpr (DIM == 128) return row * 128 + ((c ^ (v ? row & 7 : (row & 1) << 2)) << 4);
+  else return (row >> 1) * 128 + (((((row & 1) << 2) | c) ^ (((row >> 1) & 3) << 1)) << 4);
+}
 
 __device__ __forceinline__ void ldsm4(uint32_t (&r)[4], uint32_t a) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
@@ -111,7 +122,7 @@ __device__ __forceinline__ void fetch_queries(uint32_t raw_s, const AttendArgs& 
 // exact power of two that brings the row's largest value to [1, 2) and goes back
 // into its scores, so that no query overflows f16.  Rows are DIM values in
 // 16-byte chunks xored like the cache's.
-template <int DIM, bool KV16>
+template <int DIM, Kv KV>
 __device__ __forceinline__ void stage_queries(uint32_t q_s, float* factor_s, uint32_t raw_s, int rows, int first, int step) {
   constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;
   constexpr int N = DIM / 32;  // values per lane
@@ -126,13 +137,28 @@ __device__ __forceinline__ void stage_queries(uint32_t q_s, float* factor_s, uin
       top = fmaxf(top, fabsf(x[k]));
     }
     const int d = N * lane;
-    if constexpr (KV16) {
+    if constexpr (KV != kF32) {
 #pragma unroll
       for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
       // exponent bits of the largest value, kept where both powers are normal
       const int e = min(max((int)(__float_as_uint(top) >> 23), 1), 253);
       const float down = __uint_as_float((uint32_t)(254 - e) << 23);
       if (lane == 0) factor_s[row] = __uint_as_float((uint32_t)e << 23);
+      if constexpr (is_8bit(KV)) {
+        // in the order in which K's codes meet them: of 16 codes that a lane t of
+        // four loads, bytes 0 and 2 of word i are inner indexes 2 t and 2 t + 1
+        // of step i, bytes 1 and 3 the ones 8 further
+#pragma unroll
+        for (int k = 0; k < N; ++k) {
+          const int y = d + k, e16 = 16 * (4 * (y >> 6) + ((y >> 2) & 3)) + 2 * ((y >> 4) & 3) + ((y >> 1) & 1) + 8 * (y & 1);
+          const int c = e16 >> 3;
+          const uint32_t at = q_s + row * (2 * DIM) + (((c & ~7) | ((c ^ row) & 7)) << 4) + (e16 & 7) * 2;
+          const __half hi = __float2half_rn(x[k] * down), lo = __float2half_rn(x[k] * down - __half2float(hi));
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(at), "h"(__half_as_ushort(hi)) : "memory");
+          asm volatile("st.shared.u16 [%0], %1;" ::"r"(at + kRows * 2 * DIM), "h"(__half_as_ushort(lo)) : "memory");
+        }
+        continue;
+      }
       const int c = d >> 3;
       const uint32_t at = q_s + row * (2 * DIM) + (((c & ~7) | ((c ^ row) & 7)) << 4) + (d & 7) * 2;
 #pragma unroll
@@ -154,12 +180,13 @@ __device__ __forceinline__ void stage_queries(uint32_t q_s, float* factor_s, uin
 // What a warp holds of its 16 rows: the queries as the left operand of the
 // score products, the running maximum and sum, and the output.  Lane l holds
 // rows l / 4 and l / 4 + 8.
-template <int DIM, bool KV16>
+template <int DIM, Kv KV>
 struct Rows {
-  uint32_t qh[KV16 ? DIM / 16 : 1][4];  // f16: hi and lo fragments
-  uint32_t ql[KV16 ? DIM / 16 : 1][4];
-  float qf[KV16 ? 1 : DIM / 8][4];      // f32: split where they are used
-  float factor[2];                      // 2^e taken out of a row's queries (f16)
+  static constexpr bool F32 = KV == kF32;
+  uint32_t qh[F32 ? 1 : DIM / 16][4];   // hi and lo fragments
+  uint32_t ql[F32 ? 1 : DIM / 16][4];
+  float qf[F32 ? DIM / 8 : 1][4];       // f32: split where they are used
+  float factor[2];                      // 2^e taken out of a row's queries (not f32)
   int sees[2];                          // last position each row sees
   float o[DIM / 8][4];
   float m[2], l[2];                     // reference and sum of the weights
@@ -171,9 +198,9 @@ struct Rows {
     for (int i = 0; i < 2; ++i) {
       const int r = (lane >> 2) + 8 * i;
       sees[i] = s.pos + min((r0 + r) / group, s.n - 1);
-      factor[i] = KV16 ? factor_s[r] : 1.0f;
+      factor[i] = F32 ? 1.0f : factor_s[r];
     }
-    if constexpr (KV16) {
+    if constexpr (!F32) {
 #pragma unroll
       for (int k = 0; k < DIM / 16; ++k) {
         const int c = 2 * k + (mat >> 1);
@@ -205,12 +232,41 @@ struct Rows {
   // One block of positions p0 .. p0 + POS - 1 (K at k_s, V behind it); with
   // `masked`, positions a row does not see are left out.
   __device__ __forceinline__ void step(uint32_t k_s, int p0, bool masked) {
-    using G = Geo<DIM, KV16>;
+    using G = Geo<DIM, KV>;
     const int lane = threadIdx.x & 31, t = lane & 3;
     const uint32_t v_s = k_s + G::pos * G::row_bytes;
     constexpr int NT = G::pos / 8;  // score tiles of 8 positions
     float s[NT][4];
-    if constexpr (KV16) {
+    if constexpr (is_8bit(KV)) {
+      float lo[NT][4];
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = lo[n][j] = 0.f;
+#pragma unroll
+        for (int h = 0; h < DIM / 64; ++h) {
+          uint32_t w[4];
+          asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                       : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3])
+                       : "r"(k_s + place<DIM>(8 * n + (lane >> 2), 4 * h + t, false))
+                       : "memory");
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            uint32_t b0, b1;
+            decode4<KV>(w[i], b0, b1);
+            mma_f16(s[n], qh[4 * h + i], b0, b1);
+            mma_f16(lo[n], ql[4 * h + i], b0, b1);
+          }
+        }
+      }
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float ks[2];
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];" : "=f"(ks[0]), "=f"(ks[1]) : "r"(k_s + G::scales + 4 * (8 * n + 2 * t)) : "memory");
+#pragma unroll
+        for (int j = 0; j < 4; ++j) s[n][j] = (s[n][j] + lo[n][j]) * (factor[j >> 1] * code_unit<KV>()) * ks[j & 1];
+      }
+    } else if constexpr (KV == kF16) {
       float lo[NT][4];
 #pragma unroll
       for (int n = 0; n < NT; ++n) {
@@ -293,7 +349,86 @@ struct Rows {
           l[i] += s[n][2 * i + j];
         }
     }
-    if constexpr (KV16) {
+    if constexpr (is_8bit(KV)) {
+      // Weights times V's scales, in the unit of the block's largest of each row (a
+      // power of two that goes back into the block's product), so that whatever the
+      // weights and scales are, no product that counts in the block falls below f16.
+      float back[2], p[NT][4], most[2] = {0.f, 0.f};
+#pragma unroll
+      for (int n = 0; n < NT; ++n) {
+        float vs[2];
+        asm volatile("ld.shared.v2.f32 {%0, %1}, [%2];"
+                     : "=f"(vs[0]), "=f"(vs[1])
+                     : "r"(k_s + G::scales + 4 * (G::pos + 8 * n + 2 * t))
+                     : "memory");
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          p[n][j] = masked && p0 + 8 * n + 2 * t + (j & 1) > sees[j >> 1] ? 0.f : s[n][j] * vs[j & 1];
+          most[j >> 1] = fmaxf(most[j >> 1], p[n][j]);
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 1));
+        most[i] = fmaxf(most[i], __shfl_xor_sync(0xffffffffu, most[i], 2));
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const uint32_t e = min(max(__float_as_uint(most[i]) >> 23, 1u), 253u);
+        const float unit = __uint_as_float((254u - e) << 23);
+        back[i] = __uint_as_float(e << 23) * code_unit<KV>();
+#pragma unroll
+        for (int n = 0; n < NT; ++n)
+#pragma unroll
+          for (int j = 0; j < 2; ++j) p[n][2 * i + j] *= unit;
+      }
+      float x[DIM / 8][4];
+#pragma unroll
+      for (int d = 0; d < DIM / 8; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) x[d][j] = 0.f;
+      // A column n of step d stands for value (DIM / 8) n + d of the head: a lane's
+      // loads are neighbouring values of four positions.
+#pragma unroll
+      for (int b = 0; b < NT / 2; ++b) {
+        uint32_t ph[4], pl[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) split_f16(p[2 * b + (j >> 1)][2 * (j & 1)], p[2 * b + (j >> 1)][2 * (j & 1) + 1], ph[j], pl[j]);
+        constexpr int W = DIM / 32;  // words of a lane's values
+        uint32_t w[4][W];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const int row = 16 * b + 2 * t + (r & 1) + 8 * (r >> 1);
+          if constexpr (W == 4)
+            asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                         : "=r"(w[r][0]), "=r"(w[r][1]), "=r"(w[r][W - 2]), "=r"(w[r][W - 1])
+                         : "r"(v_s + place<DIM>(row, lane >> 2, true))
+                         : "memory");
+          else
+            asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];"
+                         : "=r"(w[r][0]), "=r"(w[r][1])
+                         : "r"(v_s + place<DIM>(row, lane >> 3, true) + 8 * ((lane >> 2) & 1))
+                         : "memory");
+        }
+#pragma unroll
+        for (int c = 0; c < W; ++c)
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {  // values 4 c + 2 h and the next, of two positions each
+            uint32_t b0[2], b1[2];
+            decode4<KV>(__byte_perm(w[0][c], w[1][c], h ? 0x7632 : 0x5410), b0[0], b0[1]);
+            decode4<KV>(__byte_perm(w[2][c], w[3][c], h ? 0x7632 : 0x5410), b1[0], b1[1]);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+              mma_f16(x[4 * c + 2 * h + k], pl, b0[k], b1[k]);
+              mma_f16(x[4 * c + 2 * h + k], ph, b0[k], b1[k]);
+            }
+          }
+      }
+#pragma unroll
+      for (int d = 0; d < DIM / 8; ++d)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) o[d][j] = fmaf(o[d][j], down[j >> 1], x[d][j] * back[j >> 1]);
+    } else if constexpr (KV == kF16) {
       uint32_t ph[4], pl[4];
 #pragma unroll
       for (int j = 0; j < 4; ++j) split_f16(s[j >> 1][2 * (j & 1)], s[j >> 1][2 * (j & 1) + 1], ph[j], pl[j]);
@@ -346,9 +481,9 @@ struct Rows {
 };
 
 // The copies of a warp's block of positions into its stage.
-template <int DIM, bool KV16>
+template <int DIM, Kv KV>
 struct Feed {
-  using G = Geo<DIM, KV16>;
+  using G = Geo<DIM, KV>;
   const AttendArgs& a;
   const Seq& s;
   int kvh, len, shift;
@@ -371,7 +506,7 @@ struct Feed {
         atomicOr(a.c.status, DEV_BAD_ARGS);
       }
     }
-    constexpr int esize = KV16 ? 2 : 4;
+    constexpr int esize = value_bytes(KV);
     const char* k = static_cast<const char*>(a.c.k);
     const char* v = static_cast<const char*>(a.c.v);
 #pragma unroll
@@ -379,16 +514,31 @@ struct Feed {
       const int x = i * 32 + lane, row = x / G::chunks, c = x % G::chunks;
       const int64_t off = __shfl_sync(0xffffffffu, at, row) * esize + 16 * c;
       const int n = __shfl_sync(0xffffffffu, ok, row);
-      const uint32_t to = dst + row * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4);
-      copy16(to, k + (n ? off : 0), n);
-      copy16(to + G::pos * G::row_bytes, v + (n ? off : 0), n);
+      if constexpr (is_8bit(KV)) {
+        copy16(dst + place<DIM>(row, c, false), k + (n ? off : 0), n);
+        copy16(dst + G::pos * G::row_bytes + place<DIM>(row, c, true), v + (n ? off : 0), n);
+      } else {
+        const uint32_t to = dst + row * G::row_bytes + (((c & ~7) | ((c ^ row) & 7)) << 4);
+        copy16(to, k + (n ? off : 0), n);
+        copy16(to + G::pos * G::row_bytes, v + (n ? off : 0), n);
+      }
+    }
+    if constexpr (is_8bit(KV)) {
+      const int row = shift >= 0 ? p & ((1 << shift) - 1) : p % a.c.page_size;
+      const int64_t from = ok ? scale_at(a.c, page, kvh, row) : 0;
+      const uint32_t to = dst + G::scales + 4 * lane;
+      const int n = ok ? 4 : 0;
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(a.c.k_scale + from), "r"(n) : "memory");
+      asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to + 4 * G::pos), "l"(a.c.v_scale + from), "r"(n) : "memory");
     }
   }
   // Non-finite values of V at positions past `first` (the first new token's
   // own) become zero in shared memory: a row that does not see them would
   // multiply them by a weight of zero.  The rows that see them add them back
   // at the end (non_finite()).  Returns whether this lane found any.
+  // (An 8-bit cache has none: what is not finite there is a row's scale.)
   __device__ __forceinline__ bool clean(uint32_t dst, int p0, int first) const {
+    if constexpr (is_8bit(KV)) return false;
     if (p0 + G::pos - 1 <= first) return false;
     const int lane = threadIdx.x & 31;
     bool found = false;
@@ -402,7 +552,7 @@ struct Feed {
       bool bad = false;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if constexpr (KV16) {
+        if constexpr (KV == kF16) {
           if ((w[j] & 0x7c00u) == 0x7c00u) w[j] &= 0xffff0000u, bad = true;
           if ((w[j] & 0x7c000000u) == 0x7c000000u) w[j] &= 0xffffu, bad = true;
         } else {
@@ -420,9 +570,11 @@ struct Feed {
 
 // An output y of a row that sees positions up to `last`, l the sum of its
 // weights; `dirty`: values at positions past `first` were taken out.
-template <bool KV16>
+template <Kv KV>
 __device__ __forceinline__ float settled(float y, float l, bool dirty, const Cache& c, const Seq& s, int kvh, int first, int last,
                                          int d) {
+  if constexpr (is_8bit(KV)) return y;
+  constexpr bool KV16 = KV == kF16;
   if (!isfinite(y) && isfinite(l)) {
     const float x = non_finite<KV16, 1>(c, s, kvh, -1, first, d).v[0];
     if (x != 0.f) y = x;
@@ -442,6 +594,12 @@ constexpr size_t kCounterBytes = HYQ_PAGED_ATTENTION_ZEROED;
 static_assert(kCounterBytes >= kMaxCtas * sizeof(unsigned), "a counter per CTA");
 __host__ __device__ constexpr int partial_floats(int dim) { return kRows * (dim + 2) + 4; }
 
+// Where value d of a head stands in a row of the warps' joined outputs.
+template <int DIM, Kv KV>
+__device__ __forceinline__ int column(int d) {
+  return is_8bit(KV) ? 8 * (d % (DIM / 8)) + d / (DIM / 8) : d;
+}
+
 // What a segment costs beside its tiles (queries, first copies, joining the
 // warps), in tiles: the time of about four at full bandwidth.
 constexpr int kSegmentCost = 4;
@@ -457,9 +615,10 @@ constexpr int kSegmentCost = 4;
 // `beside`: the kernel before is the same call's and has nothing that this one
 // reads: it starts without waiting for that (when it may, every CTA of that has
 // seen what came before them both), and ends after it.
-template <int DIM, bool KV16>
+// PART: only a sequence's positions from a.first on, and a.ml is written too.
+template <int DIM, Kv KV, bool PART>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_constant__ AttendArgs a, int shift, bool beside) {
-  using G = Geo<DIM, KV16>;
+  using G = Geo<DIM, KV>;
   if (!beside) grid_dependency_wait();
   allow_dependents_launch();
   extern __shared__ __align__(1024) char smem[];
@@ -479,7 +638,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     int tiles = 0;
     if (i < seqs) {
       const Seq s = load_seq(a.c, i);
-      if (s.n > 0 && s.n * group <= kRows) tiles = (s.pos + s.n + G::tile - 1) / G::tile + kSegmentCost;
+      if (s.n > 0 && s.n * group <= kRows) tiles = (s.pos + s.n - (PART ? a.first[i] : 0) + G::tile - 1) / G::tile + kSegmentCost;
       else if (s.n > 0 && !beside) atomicOr(a.c.status, DEV_BAD_ARGS);  // max_new was too small: nobody takes it
     }
     int x = tiles;
@@ -525,14 +684,14 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
   }
   float* parts = reinterpret_cast<float*>(static_cast<char*>(a.ws) + kCounterBytes);
   unsigned* counters = static_cast<unsigned*>(a.ws);
-  Rows<DIM, KV16> rows;
+  Rows<DIM, KV> rows;
   const uint32_t ring = smem_addr(smem) + warp * G::stages * G::block;
   float* o_s = reinterpret_cast<float*>(smem + G::ring);  // [16][pitch]; the queries before
   const int off = warp * G::pos;
   // the piece of a segment that this CTA takes: tiles j0 .. j1 - 1 of `tiles`
   struct {
     Seq s;
-    int kvh, j0, j1, tiles;
+    int kvh, j0, j1, tiles, first;  // (first: position of tile 0)
     int64_t seg0;
   } cur, done;
   int page = -1;  // of this lane's row in the next block to copy
@@ -555,17 +714,20 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
     }
     cur.j0 = (int)(at - cur.seg0);
     cur.j1 = (int)(min(end, cur.seg0 + cur.tiles) - cur.seg0);
-    if (!same_seq) cur.s = load_seq(a.c, si);
-    const Feed<DIM, KV16> feed{a, cur.s, cur.kvh, cur.s.pos + cur.s.n, shift};
-    page = feed.page(cur.j0 * G::tile + off);
+    if (!same_seq) {
+      cur.s = load_seq(a.c, si);
+      cur.first = PART ? a.first[si] + off : off;
+    }
+    const Feed<DIM, KV> feed{a, cur.s, cur.kvh, cur.s.pos + cur.s.n, shift};
+    page = feed.page(cur.j0 * G::tile + cur.first);
     // (the ring's last stage is not copied to before the first turn)
     fetch_queries<DIM>(ring + (G::stages - 1) * G::block, a, cur.s, cur.kvh, group, 0, cur.s.n * group, warp, kWarps);
     cp_async_commit();
 #pragma unroll
     for (int i = 0; i < G::stages - 1; ++i) {
       const int now = page;
-      page = feed.page((cur.j0 + i + 1) * G::tile + off);
-      if (cur.j0 + i < cur.j1) feed.copy(ring + i * G::block, (cur.j0 + i) * G::tile + off, now);
+      page = feed.page((cur.j0 + i + 1) * G::tile + cur.first);
+      if (cur.j0 + i < cur.j1) feed.copy(ring + i * G::block, (cur.j0 + i) * G::tile + cur.first, now);
       cp_async_commit();
     }
   };
@@ -576,22 +738,22 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
       const uint32_t q_s = smem_addr(o_s);
       cp_async_wait<G::stages - 1>();
       __syncwarp();
-      stage_queries<DIM, KV16>(q_s, factor_s, ring + (G::stages - 1) * G::block, s.n * group, warp, kWarps);
+      stage_queries<DIM, KV>(q_s, factor_s, ring + (G::stages - 1) * G::block, s.n * group, warp, kWarps);
       __syncthreads();
       rows.load(q_s, factor_s, s, group, 0);
-      const Feed<DIM, KV16> feed{a, s, cur.kvh, s.pos + s.n, shift};
+      const Feed<DIM, KV> feed{a, s, cur.kvh, s.pos + s.n, shift};
       int stage = 0;
       for (int j = cur.j0; j < cur.j1; ++j) {
         const int ahead = j + G::stages - 1, now = page;
-        page = feed.page((ahead + 1) * G::tile + off);
+        page = feed.page((ahead + 1) * G::tile + cur.first);
         int put = stage + G::stages - 1;
         if (put >= G::stages) put -= G::stages;
         __syncwarp();
-        if (ahead < cur.j1) feed.copy(ring + put * G::block, ahead * G::tile + off, now);
+        if (ahead < cur.j1) feed.copy(ring + put * G::block, ahead * G::tile + cur.first, now);
         cp_async_commit();
         cp_async_wait<G::stages - 1>();
         __syncwarp();
-        const int p0 = j * G::tile + off;
+        const int p0 = j * G::tile + cur.first;
         const bool masked = p0 + G::pos - 1 > s.pos;
         if (masked && feed.clean(ring + stage * G::block, p0, s.pos)) dirty_s = piece;
         rows.step(ring + stage * G::block, p0, masked);
@@ -662,11 +824,12 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
 #pragma unroll
         for (int k = 0; k < N; ++k) {
           const int d = lane + 32 * k;
-          to[d] = settled<KV16>(from[d] * inv, l, dirty, a.c, s, kvh, s.pos, s.pos + tok, d);
+          to[d] = settled<KV>(from[column<DIM, KV>(d)] * inv, l, dirty, a.c, s, kvh, s.pos, s.pos + tok, d);
         }
+        if (PART && lane == 0) a.ml[(int64_t)(s.row0 + tok) * a.heads + kvh * group + r - tok * group] = make_float2(top, l);
       } else {
 #pragma unroll
-        for (int k = 0; k < N; ++k) part[r * DIM + lane + 32 * k] = from[lane + 32 * k];
+        for (int k = 0; k < N; ++k) part[r * DIM + lane + 32 * k] = from[column<DIM, KV>(lane + 32 * k)];
         if (lane == 0) {
           part[kRows * DIM + 2 * r] = top;
           part[kRows * DIM + 2 * r + 1] = l;
@@ -728,8 +891,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) few_kernel(const __grid_
 #pragma unroll
           for (int k = 0; k < N; ++k) {
             const int d = lane + 32 * k;
-            to[d] = settled<KV16>(sum[k] * inv, l, any, a.c, s, kvh, s.pos, s.pos + tok, d);
+            to[d] = settled<KV>(sum[k] * inv, l, any, a.c, s, kvh, s.pos, s.pos + tok, d);
           }
+          if (PART && lane == 0) a.ml[(int64_t)(s.row0 + tok) * a.heads + kvh * group + r - tok * group] = make_float2(top, l);
         }
         if (threadIdx.x == 0) counters[cf] = 0;
       }
@@ -748,9 +912,9 @@ constexpr int kChunkRows = kWarps * kRows;
 // Grid (row tiles, kv heads): tile x belongs to the sequence whose tiles
 // (64 rows each) contain it.  The four warps share every tile of positions, each
 // copying a quarter of it.
-template <int DIM, bool KV16>
+template <int DIM, Kv KV>
 __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __grid_constant__ AttendArgs a, int shift) {
-  using G = Geo<DIM, KV16>;
+  using G = Geo<DIM, KV>;
   grid_dependency_wait();
   allow_dependents_launch();
   extern __shared__ __align__(1024) char smem[];
@@ -779,11 +943,11 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
   const int last_tok = min(s.n - 1, (found_s[1] * kChunkRows + kChunkRows - 1) / group);
   const int len = s.pos + last_tok + 1, tiles = (len + G::tile - 1) / G::tile;
   const int first_tok = min(s.n - 1, found_s[1] * kChunkRows / group);
-  const Feed<DIM, KV16> feed{a, s, kvh, len, shift};
+  const Feed<DIM, KV> feed{a, s, kvh, len, shift};
   const uint32_t ring = smem_addr(smem);
   // the queries: each warp's own 16 rows, through its part of the ring
   static_assert(G::stages * G::block >= 2 * kRows * DIM * 4, "a warp's queries, as they come and as they are read");
-  Rows<DIM, KV16> rows;
+  Rows<DIM, KV> rows;
   const bool any = r0 < s.n * group;
   if (any) {
     const uint32_t q_s = ring + warp * G::stages * G::block, raw_s = q_s + kRows * DIM * 4;
@@ -792,7 +956,7 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
     cp_async_commit();
     cp_async_wait<0>();
     __syncwarp();
-    stage_queries<DIM, KV16>(q_s, factor_s[warp], raw_s, n, 0, 1);
+    stage_queries<DIM, KV>(q_s, factor_s[warp], raw_s, n, 0, 1);
     __syncwarp();
     rows.load(q_s, factor_s[warp], s, group, r0);
   }
@@ -841,7 +1005,9 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
     l += __shfl_xor_sync(0xffffffffu, l, 2);
     const int r = r0 + (lane >> 2) + 8 * i, tok = r / group;
     if (tok >= s.n) continue;
-    float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM + 2 * (lane & 3);
+    float* to = a.out + (int64_t)(s.row0 + tok) * a.out_stride + (int64_t)(kvh * group + r - tok * group) * DIM;
+    // value d, j of a lane's row
+    auto value = [&](int d, int j) { return is_8bit(KV) ? DIM / 8 * (2 * (lane & 3) + j) + d : 8 * d + 2 * (lane & 3) + j; };
     bool odd = dirty_s;
 #pragma unroll
     for (int d = 0; d < DIM / 8; ++d) {
@@ -849,16 +1015,16 @@ __global__ void __launch_bounds__(kThreads, kCtasPerSm) chunk_kernel(const __gri
       for (int j = 0; j < 2; ++j) {
         const float y = rows.o[d][2 * i + j] / l;
         odd = odd || !isfinite(y);
-        to[8 * d + j] = y;
+        to[value(d, j)] = y;
       }
     }
-    if (odd) {
+    if (!is_8bit(KV) && odd) {
 #pragma unroll 1
       for (int d = 0; d < DIM / 8; ++d)
 #pragma unroll 1
         for (int j = 0; j < 2; ++j)
-          to[8 * d + j] = settled<KV16>(to[8 * d + j], l, dirty_s, a.c, s, kvh, s.pos + first_tok, s.pos + tok,
-                                        8 * d + 2 * (lane & 3) + j);
+          to[value(d, j)] =
+              settled<KV>(to[value(d, j)], l, dirty_s, a.c, s, kvh, s.pos + first_tok, s.pos + tok, value(d, j));
     }
   }
 }
@@ -871,21 +1037,21 @@ int page_shift(const AttendArgs& a) {
   return (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.c.page_size) : -1;
 }
 
-template <int DIM, bool KV16>
+template <int DIM, Kv KV>
 cudaError_t chunks(const AttendArgs& a, cudaStream_t st) {
-  using G = Geo<DIM, KV16>;
+  using G = Geo<DIM, KV>;
   const int64_t tiles = chunk_tiles(a);
-  auto k = chunk_kernel<DIM, KV16>;
+  auto k = chunk_kernel<DIM, KV>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(k, G::smem, done);
   if (e != cudaSuccess) return e;
   return launch_ex(k, dim3((unsigned)tiles, (unsigned)a.c.kv_heads), dim3(kThreads), G::smem, st, a, page_shift(a));
 }
 
-template <int DIM, bool KV16>
+template <int DIM, Kv KV, bool PART>
 cudaError_t few(const AttendArgs& a, bool beside, cudaStream_t st) {
-  using G = Geo<DIM, KV16>;
-  auto k = few_kernel<DIM, KV16>;
+  using G = Geo<DIM, KV>;
+  auto k = few_kernel<DIM, KV, PART>;
   static std::atomic<uint64_t> done{0};
   const cudaError_t e = allow_smem(k, G::smem + (kMaxSeqs + 1) * 4, done);
   if (e != cudaSuccess) return e;
@@ -893,35 +1059,47 @@ cudaError_t few(const AttendArgs& a, bool beside, cudaStream_t st) {
                           a, page_shift(a), beside);
 }
 
+template <Kv KV>
+cudaError_t few(const AttendArgs& a, bool beside, cudaStream_t st) {
+  if (a.first) return a.c.dim == 128 ? few<128, KV, true>(a, beside, st) : few<64, KV, true>(a, beside, st);
+  return a.c.dim == 128 ? few<128, KV, false>(a, beside, st) : few<64, KV, false>(a, beside, st);
+}
+
+template <Kv KV>
+cudaError_t chunks(const AttendArgs& a, cudaStream_t st) {
+  return a.c.dim == 128 ? chunks<128, KV>(a, st) : chunks<64, KV>(a, st);
+}
+
 }  // namespace
 
-bool mma_supported(const AttendArgs& a, bool kv16) {
-  const int64_t strides = (a.c.page_stride | a.c.head_stride | a.c.row_stride) * (kv16 ? 2 : 4);
+bool mma_supported(const AttendArgs& a, Kv kv) {
+  const int64_t strides = (a.c.page_stride | a.c.head_stride | a.c.row_stride) * value_bytes(kv);
   return (a.c.dim == 64 || a.c.dim == 128) && strides % 16 == 0 &&
          (reinterpret_cast<uintptr_t>(a.c.k) | reinterpret_cast<uintptr_t>(a.c.v)) % 16 == 0;
 }
 
 bool sums_fit(int64_t seqs, int64_t reach) {
-  constexpr int tile = Geo<128, false>::tile;  // the smaller one
+  constexpr int tile = Geo<128, kF32>::tile;  // the smallest one
   return seqs * (reach / tile + 1 + kSegmentCost) <= INT32_MAX;
 }
 
-bool chunks_short(const AttendArgs& a, bool kv16, int64_t max_len) {
+bool chunks_short(const AttendArgs& a, Kv kv, int64_t max_len) {
   const int64_t tiles = (chunk_tiles(a) - a.c.seqs / 2) * a.c.kv_heads;  // sequences' last tiles are half full
   const int64_t rounds = (tiles + kMaxCtas - 1) / kMaxCtas;
-  return rounds * max_len <= (kv16 ? 350 : 64);
+  return rounds * max_len <= (kv == kF32 ? 64 : 350);
 }
 
 size_t mma_workspace_bytes(int dim) { return kCounterBytes + 2 * (size_t)kMaxCtas * partial_floats(dim) * sizeof(float); }
 
-cudaError_t launch_few(const AttendArgs& a, bool kv16, bool beside, cudaStream_t st) {
-  if (a.c.dim == 128) return kv16 ? few<128, true>(a, beside, st) : few<128, false>(a, beside, st);
-  return kv16 ? few<64, true>(a, beside, st) : few<64, false>(a, beside, st);
+cudaError_t launch_few(const AttendArgs& a, Kv kv, bool beside, cudaStream_t st) {
+  return kv == kF32   ? few<kF32>(a, beside, st)
+         : kv == kF16 ? few<kF16>(a, beside, st)
+         : kv == kI8  ? few<kI8>(a, beside, st)
+                      : few<kF8>(a, beside, st);
 }
 
-cudaError_t launch_chunks(const AttendArgs& a, bool kv16, cudaStream_t st) {
-  if (a.c.dim == 128) return kv16 ? chunks<128, true>(a, st) : chunks<128, false>(a, st);
-  return kv16 ? chunks<64, true>(a, st) : chunks<64, false>(a, st);
+cudaError_t launch_chunks(const AttendArgs& a, Kv kv, cudaStream_t st) {
+  return kv == kF32 ? chunks<kF32>(a, st) : kv == kF16 ? chunks<kF16>(a, st) : kv == kI8 ? chunks<kI8>(a, st) : chunks<kF8>(a, st);
 }
 
 }  // namespace paged

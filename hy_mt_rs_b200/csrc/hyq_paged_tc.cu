@@ -427,7 +427,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
   if (e == cudaSuccess) e = launch_ex(plan_kernel<kCtaRows>, dim3(1), dim3(1024), 0, st, a, p.plan);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
-  if (e == cudaSuccess) e = launch_few(a, true, true, st);
+  if (e == cudaSuccess) e = launch_few(a, kF16, true, st);
   if (e == cudaSuccess) e = launch_next(join_kernel<DIM, kCtaRows, true>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p);
   return e;
 }

@@ -78,10 +78,18 @@ const void* optional(PyObject* o, const at::Tensor& like, const char* name, at::
   return t.data_ptr();
 }
 
-hyq_paged_kv make_kv(const at::Tensor& q, PyObject* k_pages, PyObject* v_pages, PyObject* table) {
+// A layer's pages, and the scales of 8-bit ones (None otherwise).
+hyq_paged_kv8 make_kv(const at::Tensor& q, PyObject* k_pages, PyObject* v_pages, PyObject* table, PyObject* k_scale,
+                      PyObject* v_scale) {
   const at::Tensor &k = tensor(k_pages, "k_pages"), &v = tensor(v_pages, "v_pages");
   const at::ScalarType type = k.scalar_type();
-  if (type != at::kFloat && type != at::kHalf) refuse(HYQ_E_INVALID, "k_pages: expected a CUDA float32 or float16 tensor");
+  const int kv_type = type == at::kFloat  ? HYQ_KV_F32
+                      : type == at::kHalf ? HYQ_KV_F16
+                      : type == at::kChar ? HYQ_KV_I8
+                                          : HYQ_KV_F8;
+  const bool coded = kv_type == HYQ_KV_I8 || kv_type == HYQ_KV_F8;
+  if (kv_type == HYQ_KV_F8 && type != at::kFloat8_e4m3fn)
+    refuse(HYQ_E_INVALID, "k_pages: expected a CUDA float32, float16, int8 or float8_e4m3fn tensor");
   if (k.dim() != 4 || k.stride(3) != 1)
     refuse(HYQ_E_SHAPE, "k_pages: expected [pages, kv_heads, page_size, head_dim], contiguous in head_dim");
   if (v.scalar_type() != type || v.sizes() != k.sizes() || v.strides() != k.strides())
@@ -93,9 +101,25 @@ hyq_paged_kv make_kv(const at::Tensor& q, PyObject* k_pages, PyObject* v_pages, 
   same_device(q, t, "table");
   for (int i = 1; i < 4; ++i)
     if (k.size(i) > INT32_MAX) refuse(HYQ_E_SHAPE, "k_pages: shape");
-  return {k.data_ptr(), v.data_ptr(), type == at::kHalf ? HYQ_KV_F16 : HYQ_KV_F32, (int)k.size(1), (int)k.size(3),
-          (int)k.size(2), k.size(0), k.stride(0), k.stride(1), k.stride(2),
-          static_cast<const int32_t*>(t.data_ptr()), t.size(0), t.size(1)};
+  hyq_paged_kv8 kv{{k.data_ptr(), v.data_ptr(), kv_type, (int)k.size(1), (int)k.size(3), (int)k.size(2), k.size(0), k.stride(0),
+                    k.stride(1), k.stride(2), static_cast<const int32_t*>(t.data_ptr()), t.size(0), t.size(1)},
+                   nullptr, nullptr, 0, 0, 0};
+  if (!coded) {
+    if (k_scale != Py_None || v_scale != Py_None) refuse(HYQ_E_INVALID, "k_scale, v_scale: these pages have none");
+    return kv;
+  }
+  const at::Tensor &ks = typed(k_scale, "k_scale", at::kFloat), &vs = typed(v_scale, "v_scale", at::kFloat);
+  same_device(q, ks, "k_scale");
+  same_device(q, vs, "v_scale");
+  if (ks.dim() != 3 || ks.size(0) != k.size(0) || ks.size(1) != k.size(1) || ks.size(2) != k.size(2))
+    refuse(HYQ_E_SHAPE, "k_scale: expected [pages, kv_heads, page_size]");
+  if (vs.sizes() != ks.sizes() || vs.strides() != ks.strides()) refuse(HYQ_E_SHAPE, "k_scale and v_scale differ in shape or strides");
+  kv.k_scale = static_cast<float*>(ks.data_ptr());
+  kv.v_scale = static_cast<float*>(vs.data_ptr());
+  kv.scale_page_stride = ks.stride(0);
+  kv.scale_head_stride = ks.stride(1);
+  kv.scale_row_stride = ks.stride(2);
+  return kv;
 }
 
 hyq_paged_batch make_batch(const at::Tensor& q, PyObject* row_start, PyObject* pos, PyObject* slot, int64_t tokens,
@@ -131,6 +155,14 @@ void check(int rc) {
   if (rc != HYQ_OK) refuse(rc, hyq_last_error());
 }
 
+PyObject* pair(const at::Tensor& a, const at::Tensor& b) {
+  PyObject *x = THPVariable_Wrap(a), *y = THPVariable_Wrap(b);
+  PyObject* both = x && y ? PyTuple_Pack(2, x, y) : nullptr;
+  Py_XDECREF(x);
+  Py_XDECREF(y);
+  return both;
+}
+
 template <typename F>
 PyObject* guarded(Py_ssize_t given, Py_ssize_t wanted, F f) {
   if (given != wanted) {
@@ -148,11 +180,12 @@ PyObject* guarded(Py_ssize_t given, Py_ssize_t wanted, F f) {
 }
 
 // q, k_pages, v_pages, table, row_start, pos, max_new, max_len (-1: the table's
-// reach), slot, out, workspace
+// reach), slot, out, workspace, k_scale, v_scale
 PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 11, [&]() -> PyObject* {
+  return guarded(n, 13, [&]() -> PyObject* {
     const at::Tensor& q = typed(a[0], "q", at::kFloat);
-    const hyq_paged_kv kv = make_kv(q, a[1], a[2], a[3]);
+    const hyq_paged_kv8 kv8 = make_kv(q, a[1], a[2], a[3], a[11], a[12]);
+    const hyq_paged_kv& kv = kv8.kv;
     const int64_t qs = row_stride(q, "q"), max_len = whole(a[7]);
     const hyq_paged_batch batch = make_batch(q, a[4], a[5], a[8], q.size(0), whole(a[6]),
                                              max_len < 0 ? kv.table_width * kv.page_size : max_len);
@@ -163,18 +196,38 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     size_t bytes = 0;
     check(hyq_paged_attention_workspace_bytes((int)q.size(1), kv.head_dim, &bytes));
     if ((size_t)ws.numel() < bytes) refuse(HYQ_E_SHAPE, "attention: the workspace takes " + std::to_string(bytes) + " bytes");
-    check(hyq_paged_attention(&kv, &batch, static_cast<const float*>(q.data_ptr()), qs, (int)q.size(1),
-                              static_cast<float*>(out.data_ptr()), row_stride(out, "out"), ws.data_ptr(), stream_of(q)));
+    check(hyq_paged_attention_kv8(&kv8, &batch, static_cast<const float*>(q.data_ptr()), qs, (int)q.size(1),
+                                  static_cast<float*>(out.data_ptr()), row_stride(out, "out"), ws.data_ptr(), stream_of(q)));
     return THPVariable_Wrap(out);
   });
 }
 
+// k_pages, v_pages, table, row_start, pos, tokens (-1: k_out's), f16, slot, k_out,
+// v_out, k_scale, v_scale
+PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 12, [&]() -> PyObject* {
+    const at::Tensor& pages = tensor(a[0], "k_pages");
+    const hyq_paged_kv8 kv = make_kv(pages, a[0], a[1], a[2], a[10], a[11]);
+    const int64_t tokens = whole(a[5]);
+    const bool f16 = PyObject_IsTrue(a[6]);
+    if (tokens < 0 || tokens > INT32_MAX) refuse(HYQ_E_SHAPE, "gather: tokens");
+    const hyq_paged_batch batch = make_batch(pages, a[3], a[4], a[7], tokens, 0, 0);
+    const at::ScalarType type = f16 ? at::kHalf : at::kFloat;
+    const at::Tensor k = output(a[8], pages, {tokens, kv.kv.kv_heads, kv.kv.head_dim}, type, "k_out"),
+                     v = output(a[9], pages, {tokens, kv.kv.kv_heads, kv.kv.head_dim}, type, "v_out");
+    check(hyq_paged_gather(&kv, &batch, f16, k.data_ptr(), row_stride(k, "k_out"), v.data_ptr(), row_stride(v, "v_out"),
+                           stream_of(pages)));
+    return pair(k, v);
+  });
+}
+
 // q, k, v, k_pages, v_pages, table, row_start, pos, cos, sin, q_norm, k_norm,
-// eps, norm_first, slot, out
+// eps, norm_first, slot, out, k_scale, v_scale
 PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded(n, 16, [&]() -> PyObject* {
+  return guarded(n, 18, [&]() -> PyObject* {
     const at::Tensor &q = typed(a[0], "q", at::kFloat), &k = typed(a[1], "k", at::kFloat), &v = typed(a[2], "v", at::kFloat);
-    const hyq_paged_kv kv = make_kv(q, a[3], a[4], a[5]);
+    const hyq_paged_kv8 kv8 = make_kv(q, a[3], a[4], a[5], a[16], a[17]);
+    const hyq_paged_kv& kv = kv8.kv;
     const int64_t qs = row_stride(q, "q"), ks = row_stride(k, "k"), vs = row_stride(v, "v");
     // (positions are checked against the table's reach on the device; max_new
     // and max_len bound attention's work only)
@@ -192,8 +245,8 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     same_device(q, sin, "sin");
     const void* q_norm = optional(a[10], q, "q_norm", at::kFloat, kv.head_dim);
     const void* k_norm = optional(a[11], q, "k_norm", at::kFloat, kv.head_dim);
-    check(hyq_paged_rope_append(
-        &kv, &batch, static_cast<const float*>(q.data_ptr()), qs, (int)q.size(1), static_cast<const float*>(k.data_ptr()), ks,
+    check(hyq_paged_rope_append_kv8(
+        &kv8, &batch, static_cast<const float*>(q.data_ptr()), qs, (int)q.size(1), static_cast<const float*>(k.data_ptr()), ks,
         static_cast<const float*>(v.data_ptr()), vs, static_cast<const float*>(cos.data_ptr()),
         static_cast<const float*>(sin.data_ptr()), cos.size(0),
         static_cast<const float*>(q_norm), static_cast<const float*>(k_norm), (float)number(a[12]),
@@ -220,16 +273,13 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
                      static_cast<const float*>(temperature), static_cast<const int32_t*>(top_k),
                      static_cast<const float*>(top_p), static_cast<const float*>(min_p), static_cast<const float*>(u),
                      static_cast<int32_t*>(token.data_ptr()), static_cast<float*>(prob.data_ptr()), stream_of(x)));
-    PyObject *t = THPVariable_Wrap(token), *p = THPVariable_Wrap(prob);
-    PyObject* both = t && p ? PyTuple_Pack(2, t, p) : nullptr;
-    Py_XDECREF(t);
-    Py_XDECREF(p);
-    return both;
+    return pair(token, prob);
   });
 }
 
 PyMethodDef methods[] = {
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(attention)), METH_FASTCALL, nullptr},
+    {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gather)), METH_FASTCALL, nullptr},
     {"rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rope_append)), METH_FASTCALL, nullptr},
     {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sample)), METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};

@@ -4,7 +4,9 @@ tokens, and reserving, freeing, forking and compacting the pages on the device.
 
 A layer's keys and values are tensors [pages, kv_heads, page_size, head_dim]
 (float32 or float16; any strides with a contiguous last dimension, so a
-permuted [pages, page_size, kv_heads, head_dim] tensor works too).  A batch of
+permuted [pages, page_size, kv_heads, head_dim] tensor works too), or 8-bit codes
+(int8 or float8_e4m3fn) of that shape with float32 scales k_scale and v_scale
+[pages, kv_heads, page_size], any strides: a value is code * scale.  A batch of
 new tokens is ragged: rows row_start[s] .. row_start[s + 1] - 1 of the
 activations belong to sequence s, at positions pos[s] ..; its pages are row
 slot[s] of the table (row s without slots).  Indexes are device int32 tensors.
@@ -19,7 +21,7 @@ import torch
 from ._native import HyqError, check, lib, load_ops
 from .quant import _need_cuda, _ptr
 
-__all__ = ["PagedCache", "REFUSED", "rope_append", "attention", "attention_workspace"]
+__all__ = ["PagedCache", "REFUSED", "rope_append", "gather", "attention", "attention_workspace"]
 
 REFUSED = 2147483647    # HYQ_PAGES_REFUSED
 
@@ -32,14 +34,27 @@ _current_stream = torch._C._cuda_getCurrentRawStream
 
 
 def rope_append(q, k, v, k_pages, v_pages, table, row_start, pos, cos, sin, q_norm=None, k_norm=None, eps=1e-5,
-                norm_first=False, slot=None, out=None):
+                norm_first=False, slot=None, out=None, k_scale=None, v_scale=None):
     """hyq_paged_rope_append: rotate and normalise the heads of q [tokens,
     heads, head_dim] and k [tokens, kv_heads, head_dim] at their positions,
     write k and v into the pages, return the rotated queries (into `out` when
     given; q itself is allowed).  cos and sin are [positions, head_dim / 2]
-    (hyq_rope_table); norm_first normalises before the rotation."""
+    (hyq_rope_table); norm_first normalises before the rotation.  Into 8-bit
+    pages the rows are quantised, with their scales to k_scale and v_scale."""
     return _ops.rope_append(q, k, v, k_pages, v_pages, table, row_start, pos, cos, sin, q_norm, k_norm, eps, norm_first,
-                            slot, out)
+                            slot, out, k_scale, v_scale)
+
+
+def gather(k_pages, v_pages, table, row_start, pos, tokens, slot=None, dtype=torch.float32, k_out=None, v_out=None,
+           k_scale=None, v_scale=None):
+    """hyq_paged_gather: the keys and values that the pages hold at positions
+    pos[s] .. of each sequence, as rope_append's k and v [tokens, kv_heads,
+    head_dim] lay there (into k_out and v_out when given), float32 or float16.
+    For a sequence's rows outside the pages: another cache, the host."""
+    if dtype not in (torch.float32, torch.float16):
+        raise HyqError(-1, f"dtype: expected float32 or float16, got {dtype}")
+    return _ops.gather(k_pages, v_pages, table, row_start, pos, tokens, dtype == torch.float16, slot, k_out, v_out, k_scale,
+                       v_scale)
 
 
 @functools.lru_cache(maxsize=None)
@@ -57,7 +72,8 @@ def attention_workspace(heads, head_dim, device):
     return workspace
 
 
-def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None, slot=None, out=None, workspace=None):
+def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None, slot=None, out=None, workspace=None,
+              k_scale=None, v_scale=None):
     """hyq_paged_attention: causal grouped-query attention of the rotated
     queries q [tokens, heads, head_dim] over the pages, which hold the new
     tokens' keys and values already; [tokens, heads, head_dim] (into `out`
@@ -69,7 +85,7 @@ def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None,
             raise HyqError(-2, "q: expected [tokens, heads, head_dim] with contiguous heads")
         workspace = attention_workspace(q.shape[1], q.shape[2], q.device)
     return _ops.attention(q, k_pages, v_pages, table, row_start, pos, max_new, -1 if max_len is None else max_len, slot,
-                          out, workspace)
+                          out, workspace, k_scale, v_scale)
 
 
 def _check_int(t, name):

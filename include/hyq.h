@@ -506,6 +506,48 @@ int hyq_paged_attention_workspace_bytes(int heads, int head_dim, size_t* bytes);
 int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
                         int heads, float* out, int64_t out_stride, void* workspace, void* stream);
 
+/* --- 8-bit caches ------------------------------------------------------------
+ * hyq_paged_kv8: a cache of any type, with the scales that the 8-bit types
+ * HYQ_KV_I8 (int8) and HYQ_KV_F8 (e4m3) need: a row (one position of one kv head,
+ * of k or of v) is head_dim codes, described by `kv`, and one f32 scale, at
+ * page * scale_page_stride + head * scale_head_stride + row * scale_row_stride of
+ * k_scale or v_scale; a value is code * scale.  (For the other types the scales
+ * are not read.)
+ * Appending sets scale = the row's largest magnitude / 127 (int8) or / 448
+ * (e4m3), in f32, and each code to the one nearest to value / scale, ties to
+ * even; a row of zeros has scale 0.  A row with an infinity or NaN has codes 0
+ * and a NaN scale: it reads back as NaN throughout.  Attention makes NaN of rows
+ * that see such a position, and of no others.  The codes 0x7f and 0xff of e4m3,
+ * which appending does not write, count as +-480. */
+#define HYQ_KV_I8 2
+#define HYQ_KV_F8 3
+
+typedef struct hyq_paged_kv8 {
+  hyq_paged_kv kv;
+  float *k_scale, *v_scale;
+  int64_t scale_page_stride, scale_head_stride, scale_row_stride; /* in elements */
+} hyq_paged_kv8;
+
+/* hyq_paged_rope_append and hyq_paged_attention over such a cache.  The queries
+ * that come out are hyq_paged_rope_append's, bit for bit; attention has f32
+ * accuracy over the values that the codes stand for. */
+int hyq_paged_rope_append_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                              int heads, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
+                              const float* cos_tab, const float* sin_tab, int64_t positions, const float* q_norm,
+                              const float* k_norm, float eps, int norm_first, float* q_out, int64_t out_stride,
+                              void* stream);
+int hyq_paged_attention_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                            int heads, float* out, int64_t out_stride, void* workspace, void* stream);
+
+/* Rows of a cache of any type as values: positions pos[s], pos[s] + 1, .. of
+ * each sequence (the batch's rows, as hyq_paged_rope_append takes them; they need
+ * not be new) into k and v [tokens, kv_heads, head_dim], f32 or, with f16, IEEE
+ * binary16 (rounded to nearest); rows k_stride and v_stride values apart.  Rows
+ * outside every sequence are left alone; a table entry that is no page gives
+ * zeros and raises HYQ_DEV_BAD_ARGS.  max_new and max_len are not used. */
+int hyq_paged_gather(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, int f16, void* k, int64_t k_stride, void* v,
+                     int64_t v_stride, void* stream);
+
 /* --- Pages of a cache: reserve, free, fork, compact ------------------------
  * Device-side bookkeeping of the table above, and the page copies it needs
  * (no counterpart in the reference).  hyq_pages: the table [slots,
