@@ -118,6 +118,7 @@ _SIGS = {
     "hyq_pages_free": ([_vp, _vp, _i64, _vp], C.c_int),
     "hyq_pages_fork": ([_vp, _vp, _vp, _vp, _i64, _vp, _vp], C.c_int),
     "hyq_pages_compact": ([_vp, _vp, _vp, _vp], C.c_int),
+    "hyq_logits_adjust": ([_vp, _i64, _i64, _i64, _vp, _vp, _i64, _vp], C.c_int),
     "hyq_sample": ([_vp, _i64, _i64, _i64, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp], C.c_int),
     "hyq_gguf_open": ([C.c_char_p, C.c_int, C.POINTER(C.c_void_p)], C.c_int),
     "hyq_gguf_close": ([_vp], None),

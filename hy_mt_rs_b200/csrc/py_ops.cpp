@@ -5,6 +5,7 @@
 #include <Python.h>
 
 #include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/autograd/python_variable.h>
 
@@ -196,6 +197,7 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     size_t bytes = 0;
     check(hyq_paged_attention_workspace_bytes((int)q.size(1), kv.head_dim, &bytes));
     if ((size_t)ws.numel() < bytes) refuse(HYQ_E_SHAPE, "attention: the workspace takes " + std::to_string(bytes) + " bytes");
+    const c10::cuda::CUDAGuard device(q.device());
     check(hyq_paged_attention_kv8(&kv8, &batch, static_cast<const float*>(q.data_ptr()), qs, (int)q.size(1),
                                   static_cast<float*>(out.data_ptr()), row_stride(out, "out"), ws.data_ptr(), stream_of(q)));
     return THPVariable_Wrap(out);
@@ -215,6 +217,7 @@ PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const at::ScalarType type = f16 ? at::kHalf : at::kFloat;
     const at::Tensor k = output(a[8], pages, {tokens, kv.kv.kv_heads, kv.kv.head_dim}, type, "k_out"),
                      v = output(a[9], pages, {tokens, kv.kv.kv_heads, kv.kv.head_dim}, type, "v_out");
+    const c10::cuda::CUDAGuard device(pages.device());
     check(hyq_paged_gather(&kv, &batch, f16, k.data_ptr(), row_stride(k, "k_out"), v.data_ptr(), row_stride(v, "v_out"),
                            stream_of(pages)));
     return pair(k, v);
@@ -245,6 +248,7 @@ PyObject* rope_append(PyObject*, PyObject* const* a, Py_ssize_t n) {
     same_device(q, sin, "sin");
     const void* q_norm = optional(a[10], q, "q_norm", at::kFloat, kv.head_dim);
     const void* k_norm = optional(a[11], q, "k_norm", at::kFloat, kv.head_dim);
+    const c10::cuda::CUDAGuard device(q.device());
     check(hyq_paged_rope_append_kv8(
         &kv8, &batch, static_cast<const float*>(q.data_ptr()), qs, (int)q.size(1), static_cast<const float*>(k.data_ptr()), ks,
         static_cast<const float*>(v.data_ptr()), vs, static_cast<const float*>(cos.data_ptr()),
@@ -269,6 +273,7 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
     const void* min_p = optional(a[5], x, "min_p", at::kFloat, rows);
     const at::Tensor token = output(a[6], x, {rows}, at::kInt, "token"), prob = output(a[7], x, {rows}, at::kFloat, "prob");
     if (!token.is_contiguous() || !prob.is_contiguous()) refuse(HYQ_E_INVALID, "sample: expected contiguous outputs");
+    const c10::cuda::CUDAGuard device(x.device());
     check(hyq_sample(static_cast<const float*>(x.data_ptr()), cols, rows > 1 ? x.stride(0) : cols, rows,
                      static_cast<const float*>(temperature), static_cast<const int32_t*>(top_k),
                      static_cast<const float*>(top_p), static_cast<const float*>(min_p), static_cast<const float*>(u),
@@ -277,7 +282,69 @@ PyObject* sample(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// [rows, columns] whose rows are contiguous; their distance.
+int64_t matrix_stride(const at::Tensor& t, const char* name) {
+  if (t.dim() != 2 || (t.size(1) > 1 && t.stride(1) != 1))
+    refuse(HYQ_E_SHAPE, std::string(name) + ": expected a matrix with contiguous rows");
+  return t.size(0) > 1 ? t.stride(0) : t.size(1);
+}
+
+// logits, history, length, prompt, slot, repetition, presence, frequency,
+// bias_start, bias_token, bias_value, mask, mask_row, out
+PyObject* adjust(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 14, [&]() -> PyObject* {
+    const at::Tensor& x = typed(a[0], "logits", at::kFloat);
+    const int64_t stride = matrix_stride(x, "logits"), rows = x.size(0), cols = x.size(1);
+    hyq_adjust p{};
+    if (a[1] != Py_None) {
+      const at::Tensor& h = typed(a[1], "history", at::kInt);
+      same_device(x, h, "history");
+      p.history_stride = matrix_stride(h, "history");
+      p.history = static_cast<const int32_t*>(h.data_ptr());
+      p.slots = h.size(0);
+      p.history_width = h.size(1);
+      if (a[2] == Py_None) refuse(HYQ_E_INVALID, "length: expected a CUDA tensor");
+      p.length = static_cast<const int32_t*>(optional(a[2], x, "length", at::kInt, p.slots));
+      p.prompt = static_cast<const int32_t*>(optional(a[3], x, "prompt", at::kInt, p.slots));
+      p.slot = static_cast<const int32_t*>(optional(a[4], x, "slot", at::kInt, rows));
+    } else {
+      for (int i = 2; i < 8; ++i)
+        if (a[i] != Py_None) refuse(HYQ_E_INVALID, "adjust: lengths and penalties go with a history");
+    }
+    p.repetition = static_cast<const float*>(optional(a[5], x, "repetition", at::kFloat, rows));
+    p.presence = static_cast<const float*>(optional(a[6], x, "presence", at::kFloat, rows));
+    p.frequency = static_cast<const float*>(optional(a[7], x, "frequency", at::kFloat, rows));
+    if (a[8] != Py_None) {
+      const at::Tensor& t = plain(a[9], "bias tokens", at::kInt);
+      same_device(x, t, "bias tokens");
+      p.bias_count = t.numel();
+      p.bias_start = static_cast<const int32_t*>(optional(a[8], x, "bias starts", at::kInt, rows + 1));
+      p.bias_token = static_cast<const int32_t*>(t.data_ptr());
+      if (a[10] == Py_None) refuse(HYQ_E_INVALID, "bias values: expected a CUDA tensor");
+      p.bias_value = static_cast<const float*>(optional(a[10], x, "bias values", at::kFloat, p.bias_count));
+      if (p.bias_count == 0) p.bias_start = nullptr;
+    }
+    if (a[11] != Py_None) {
+      const at::Tensor& m = typed(a[11], "mask", at::kInt);
+      same_device(x, m, "mask");
+      p.mask_stride = matrix_stride(m, "mask");
+      if (m.size(1) < (cols + 31) / 32) refuse(HYQ_E_SHAPE, "mask: expected [masks, (n + 31) / 32]");
+      p.mask = static_cast<const int32_t*>(m.data_ptr());
+      p.masks = m.size(0);
+      p.mask_row = static_cast<const int32_t*>(optional(a[12], x, "mask_row", at::kInt, rows));
+    } else if (a[12] != Py_None) {
+      refuse(HYQ_E_INVALID, "adjust: mask_row goes with a mask");
+    }
+    const at::Tensor out = output(a[13], x, x.sizes(), at::kFloat, "out");
+    const c10::cuda::CUDAGuard device(x.device());
+    check(hyq_logits_adjust(static_cast<const float*>(x.data_ptr()), cols, stride, rows, &p, static_cast<float*>(out.data_ptr()),
+                            matrix_stride(out, "out"), stream_of(x)));
+    return THPVariable_Wrap(out);
+  });
+}
+
 PyMethodDef methods[] = {
+    {"adjust", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(adjust)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(attention)), METH_FASTCALL, nullptr},
     {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gather)), METH_FASTCALL, nullptr},
     {"rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rope_append)), METH_FASTCALL, nullptr},

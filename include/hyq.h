@@ -618,6 +618,45 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
                const int32_t* top_k, const float* top_p, const float* min_p, const float* u, int32_t* token,
                float* prob, void* stream);
 
+/* --- Logits before sampling: penalties, biases, masks ------------------------
+ * (The reference's Sampler has the repetition penalty, generation.rs, on the
+ * host.)  Row r of `rows` rows of n logits (rows `stride` floats apart) goes to
+ * out (rows out_stride apart; logits itself is allowed) as, in f32 and in this
+ * order:
+ *   penalties  the row's history is row slot[r] (r without slots; negative:
+ *              none) of history [slots, history_width] (rows history_stride
+ *              apart): its first length[slot] tokens, of which the first
+ *              prompt[slot] (0 without) are the prompt's and the others, the
+ *              made ones, come after.  A token of the history: l / repetition[r]
+ *              where l > 0, l * repetition[r] elsewhere; one that was made c > 0
+ *              times: then l - (frequency[r] * c + presence[r]).  A repetition
+ *              that is not above 0 is off, as is 1;
+ *   biases     l + bias_value[i] for the last i of bias_start[r] ..
+ *              bias_start[r + 1] - 1 whose bias_token[i] it is;
+ *   mask       -inf where bit (token % 32) of word token / 32 of mask row
+ *              mask_row[r] (r without; negative: none) is 0; words past n are not
+ *              read.
+ * Any of the arrays' pointers may be NULL for what is not wanted (a penalty
+ * needs a history).  Tokens that are none of the n are skipped.  NaN stays NaN.
+ * A slot or mask row past the last, a length outside 0 .. history_width and
+ * bias entries outside 0 .. bias_count - 1 leave that part out for the row and
+ * raise HYQ_DEV_BAD_ARGS. */
+typedef struct hyq_adjust {
+  const int32_t* history;
+  int64_t slots, history_width, history_stride;
+  const int32_t *slot, *length, *prompt;           /* [rows], [slots], [slots] */
+  const float *repetition, *presence, *frequency;  /* [rows] each */
+  const int32_t *bias_start, *bias_token;          /* [rows + 1], [bias_count] */
+  const float* bias_value;                         /* [bias_count] */
+  int64_t bias_count;
+  const int32_t* mask;                             /* [masks, (n + 31) / 32] */
+  int64_t masks, mask_stride;                      /* in words */
+  const int32_t* mask_row;                         /* [rows] */
+} hyq_adjust;
+
+int hyq_logits_adjust(const float* logits, int64_t n, int64_t stride, int64_t rows, const hyq_adjust* adjust, float* out,
+                      int64_t out_stride, void* stream);
+
 /* --- GGUF v3 model files (gguf.rs:50-210) --------------------------------
  * hyq_gguf_open maps the file read-only and checks it as the reference does
  * (header bounds, metadata types, alignment, tensor table, Tencent legacy
