@@ -112,6 +112,8 @@ _SIGS = {
     "hyq_paged_rope_append_kv8": ([_vp, _vp, _vp, _i64, C.c_int, _vp, _i64, _vp, _i64, _vp, _vp, _i64, _vp, _vp, C.c_float,
                                    C.c_int, _vp, _i64, _vp], C.c_int),
     "hyq_paged_attention_kv8": ([_vp, _vp, _vp, _i64, C.c_int, _vp, _i64, _vp, _vp], C.c_int),
+    "hyq_paged_attention_shared_workspace_bytes": ([C.c_int, C.c_int, _i64, C.POINTER(C.c_size_t)], C.c_int),
+    "hyq_paged_attention_shared": ([_vp, _vp, _vp, _vp, _i64, _i64, _vp, _i64, C.c_int, _vp, _i64, _vp, _vp], C.c_int),
     "hyq_paged_gather": ([_vp, _vp, C.c_int, _vp, _i64, _vp, _i64, _vp], C.c_int),
     "hyq_pages_workspace_bytes": ([_i64, C.POINTER(C.c_size_t)], C.c_int),
     "hyq_pages_reserve": ([_vp, _vp, _vp, _i64, _vp, _vp, _vp], C.c_int),

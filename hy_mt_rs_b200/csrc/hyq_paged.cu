@@ -5,6 +5,7 @@
 #include "../../include/hyq.h"
 #include "hyq_kernels.h"
 #include "hyq_paged.cuh"
+#include "hyq_paged_shared.h"
 
 namespace hyq {
 namespace paged {
@@ -585,10 +586,11 @@ int rope_append(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_page
   }
 }
 
-int attention(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
-              int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
-  const char* name = "paged_attention";
-  hyq::paged::AttendArgs a{};
+// The checks of an attention call; `nothing`: it has nothing to do.
+int attend_args(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+                int heads, float* out, int64_t out_stride, void* workspace, const char* name, hyq::paged::AttendArgs& a,
+                bool& nothing) {
+  nothing = true;
   const int rc = make_cache(kv, kv8, batch, heads, name, true, a.c);
   if (rc) return rc;
   if (batch->seqs == 0 || batch->tokens == 0 || batch->max_new == 0) return HYQ_OK;
@@ -603,18 +605,22 @@ int attention(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_paged_
   a.out = out;
   a.out_stride = out_stride;
   a.ws = workspace;
-  const cudaStream_t st = (cudaStream_t)stream;
+  nothing = false;
+  return HYQ_OK;
+}
+
+int attend(const hyq::paged::AttendArgs& a, hyq::paged::Kv type, int64_t max_new, int64_t max_len, const char* name,
+           cudaStream_t st) {
   using namespace hyq::paged;
-  const Kv type = (Kv)kv->dtype;
   if (mma_supported(a, type)) {
     cudaError_t e;
-    if (batch->max_new * (heads / kv->kv_heads) <= kFewRows) {
+    if (max_new * (a.heads / a.c.kv_heads) <= kFewRows) {
       e = launch_few(a, type, false, st);
-    } else if (is_8bit(type) || chunks_short(a, type, batch->max_len) || !(type == kF16 ? tc_supported(a) : tc32_supported(a))) {
+    } else if (chunks_short(a, type, max_len) || !chunks_tc_supported(a, type)) {
       e = launch_chunks(a, type, st);
       if (e == cudaSuccess) e = launch_few(a, type, true, st);
     } else {
-      e = type == kF16 ? launch_chunks_tc(a, st) : launch_chunks_tc32(a, st);
+      e = launch_chunks_tc(a, type, st);
     }
     return done(e, name);
   }
@@ -624,6 +630,16 @@ int attention(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_paged_
     case kI8: return done(launch_attend<kI8>(a, st), name);
     default: return done(launch_attend<kF8>(a, st), name);
   }
+}
+
+int attention(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
+              int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
+  const char* name = "paged_attention";
+  hyq::paged::AttendArgs a{};
+  bool nothing;
+  const int rc = attend_args(kv, kv8, batch, q, q_stride, heads, out, out_stride, workspace, name, a, nothing);
+  if (rc || nothing) return rc;
+  return attend(a, (hyq::paged::Kv)kv->dtype, batch->max_new, batch->max_len, name, (cudaStream_t)stream);
 }
 
 }  // namespace
@@ -664,6 +680,41 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
 int hyq_paged_attention_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
                             int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
   return attention(kv ? &kv->kv : nullptr, kv, batch, q, q_stride, heads, out, out_stride, workspace, stream);
+}
+
+int hyq_paged_attention_shared_workspace_bytes(int heads, int head_dim, int64_t tokens, size_t* bytes) {
+  const char* name = "paged_attention_shared_workspace_bytes";
+  if (!bytes) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
+  if (heads <= 0 || heads > 1 << 16 || head_dim <= 0 || head_dim > hyq::paged::kMaxDim || tokens < 0 || tokens > INT32_MAX)
+    return api_fail(HYQ_E_SHAPE, "%s: shape", name);
+  *bytes = hyq::paged::shared_workspace_bytes(heads, head_dim, tokens);
+  return HYQ_OK;
+}
+
+int hyq_paged_attention_shared(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const int32_t* group_start,
+                               const int32_t* shared, int64_t groups, int64_t max_shared, const float* q, int64_t q_stride,
+                               int heads, float* out, int64_t out_stride, void* workspace, void* stream) {
+  const char* name = "paged_attention_shared";
+  using namespace hyq::paged;
+  AttendArgs a{};
+  bool nothing;
+  const int rc = attend_args(kv ? &kv->kv : nullptr, kv, batch, q, q_stride, heads, out, out_stride, workspace, name, a, nothing);
+  if (rc || nothing) return rc;
+  if (groups < 0 || groups > kMaxSeqs || max_shared < 0 || max_shared > batch->max_len)
+    return api_fail(HYQ_E_SHAPE, "%s: shape of the groups", name);
+  if (batch->max_new * (heads / kv->kv.kv_heads) > kFewRows)
+    return api_fail(HYQ_E_SHAPE, "%s: at most %d rows (new tokens x query heads per kv head) of a sequence", name, kFewRows);
+  if (groups > 0 && (!group_start || !shared)) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
+  if (!aligned(group_start, 4) || !aligned(shared, 4))
+    return api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
+  const Kv type = (Kv)kv->kv.dtype;
+  const cudaStream_t st = (cudaStream_t)stream;
+  if (groups == 0 || max_shared == 0 || !shared_supported(a, type))
+    return attend(a, type, batch->max_new, batch->max_len, name, st);
+  a.groups.start = group_start;
+  a.groups.shared = shared;
+  a.groups.n = (int)groups;
+  return done(launch_shared(a, type, st), name);
 }
 
 int hyq_paged_gather(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, int f16, void* k, int64_t k_stride, void* v,

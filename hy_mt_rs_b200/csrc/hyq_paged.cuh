@@ -172,6 +172,19 @@ __device__ __forceinline__ bool find_tile(const Cache& c, int group, int rows, i
   return false;
 }
 
+// Groups of sequences with a prefix in common (n 0: none), for the kernels that
+// take the prefixes; `out` and `ml` are those of the sequences' own positions then.
+struct Groups {
+  const int32_t* start;   // [n + 1] first sequence of each
+  const int32_t* shared;  // [n] positions in common
+  int n;
+  int32_t* first;         // [seqs], [tokens] prefix that a sequence, a token takes from its group
+  int32_t* token_prefix;
+  float* out;
+  int64_t out_stride;
+  float2* ml;
+};
+
 // hyq_paged_attention's activations and output.
 struct AttendArgs {
   Cache c;
@@ -184,6 +197,7 @@ struct AttendArgs {
   // attention over a part of the positions only (null otherwise):
   const int32_t* first;  // [seqs] a sequence's positions from here on
   float2* ml;            // [tokens, heads] each output's reference and sum of weights, written with it
+  Groups groups;
 };
 
 // The kernels round a sequence's length up to tiles and look some tiles ahead, in
@@ -220,6 +234,18 @@ cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st);
 // hyq_paged_tc32.cu: the same over f32 caches, in the same workspace.
 bool tc32_supported(const AttendArgs& a);
 cudaError_t launch_chunks_tc32(const AttendArgs& a, cudaStream_t st);
+
+// hyq_paged_tc8.cu: the same over 8-bit caches.
+bool tc8_supported(const AttendArgs& a);
+cudaError_t launch_chunks_tc8(const AttendArgs& a, Kv kv, cudaStream_t st);
+
+// The kernels on tcgen05 for a cache type.
+inline bool chunks_tc_supported(const AttendArgs& a, Kv kv) {
+  return kv == kF16 ? tc_supported(a) : kv == kF32 ? tc32_supported(a) : tc8_supported(a);
+}
+inline cudaError_t launch_chunks_tc(const AttendArgs& a, Kv kv, cudaStream_t st) {
+  return kv == kF16 ? launch_chunks_tc(a, st) : kv == kF32 ? launch_chunks_tc32(a, st) : launch_chunks_tc8(a, kv, st);
+}
 
 // Weights are 2^(s - m) of the scores s, which carry log2(e) through the queries,
 // with a reference m of 10 below the row's maximum: kept 2^10 times their size,

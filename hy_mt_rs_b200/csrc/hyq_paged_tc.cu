@@ -340,7 +340,7 @@ __global__ void __launch_bounds__(kThreads, 1)
     while (at < end && ok) {
       const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
       const int r = x.r0 + wg * kTile + 32 * (warp & 3) + lane;  // row of the sequence
-      const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + tok;
+      const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + x.step * tok;
       const int64_t piece_at = at;
       next(x);
       if (wg == 1 && !x.two) continue;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         break;
       }
       const bool dirty = misc[3] != 0;
-      store_rows<DIM, kCtaRows, true>(p, x, group, cta, piece_at != begin, r, base_g + L::q + wg * 2 * L::tile, o, m, l, dirty);
+      store_rows<DIM, kCtaRows, kF16>(p, x, group, cta, piece_at != begin, r, base_g + L::q + wg * 2 * L::tile, o, m, l, dirty);
     }
   }
   fence_before();
@@ -425,10 +425,10 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   auto k = chunk_tc_kernel<DIM>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
-  if (e == cudaSuccess) e = launch_ex(plan_kernel<kCtaRows>, dim3(1), dim3(1024), 0, st, a, p.plan);
+  if (e == cudaSuccess) e = launch_plan<kCtaRows>(a, p.plan, st);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
-  if (e == cudaSuccess) e = launch_few(a, kF16, true, st);
-  if (e == cudaSuccess) e = launch_next(join_kernel<DIM, kCtaRows, true>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p);
+  if (e == cudaSuccess) e = launch_beside(a, kF16, st);
+  if (e == cudaSuccess) e = launch_next(join_kernel<DIM, kCtaRows, kF16>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p);
   return e;
 }
 

@@ -1,5 +1,5 @@
 // What the tcgen05 attention kernels share (f16 caches: hyq_paged_tc.cu, f32
-// caches: hyq_paged_tc32.cu): the plan of a call's work, the join of partial
+// caches: hyq_paged_tc32.cu, 8-bit ones: hyq_paged_tc8.cu): the plan of a call's work, the join of partial
 // results, operand descriptors, tensor memory access.
 #pragma once
 
@@ -27,11 +27,13 @@ __host__ __device__ constexpr size_t part_floats(int dim) {
 constexpr float kSlack = 5.0f;           // a weight is at most 2^(kBias + kSlack): below f16's 65504
 
 // A segment: its sequence (n rows of tokens from row0 at pos, pages in `slot`),
-// which of the sequence's it is, and the position tiles that come before and
-// up to its end among one kv head's.
+// which of the sequence's it is, the position tiles that come before and up to
+// its end among one kv head's, and how many positions further a token sees than
+// the one before: 1, or 0 where it is a group's tokens over their prefix (all see
+// positions 0 .. pos).
 struct alignas(16) Segment {
   int row0, n, pos, slot;
-  int tile, first, end, unused;
+  int tile, first, end, step;
 };
 // Where a CTA's range begins: position tile `begin` of all kv heads', in
 // segment t of kv head kvh.
@@ -74,15 +76,18 @@ inline bool plan_fits(const AttendArgs& a) {
 
 // Position tiles that the rows of a segment see.
 template <int ROWS>
-__device__ __forceinline__ int seen_tiles(const Seq& s, int group, int tile) {
+__device__ __forceinline__ int seen_tiles(const Seq& s, int group, int tile, int step) {
   const int last = min((tile + 1) * ROWS, s.n * group) - 1;
-  return (s.pos + last / group + kTile) / kTile;
+  return (s.pos + step * (last / group) + kTile) / kTile;
 }
 
 // One CTA: the sequences' segments, each one's place in line, and the CTAs'
 // ranges of it.  The line is cut by equal cost, kSegTiles more than its tiles
 // for each segment (its queries in, its results out, a start of the pipeline).
-template <int ROWS>
+// PREFIX: the segments are those of the groups' prefixes, and each sequence's and
+// each token's prefix is written down; a group whose prefix some sequence of it does
+// not hold (DEV_BAD_ARGS), or that is a single sequence, has none.
+template <int ROWS, bool PREFIX>
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan) {
   grid_dependency_wait();
   allow_dependents_launch();
@@ -109,16 +114,73 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
     const int before = __shfl_sync(0xffffffffu, w, max(warp - 1, 0));
     return (warp ? before : 0) + x - v;
   };
+  const Groups& g = a.groups;
+  const int units = PREFIX ? g.n : a.c.seqs;
+  if constexpr (PREFIX) {
+    for (int i = threadIdx.x; i < a.c.tokens; i += 1024) g.token_prefix[i] = 0;
+    bool bad = false;
+    for (int i = threadIdx.x; i < units; i += 1024) {
+      const int first = g.start[i], last = g.start[i + 1], p = g.shared[i];
+      bad = bad || first < 0 || first > last || last > a.c.seqs || p < 0;
+      off_s[i] = last - first > 1 ? p : 0;
+    }
+    if (__syncthreads_or(bad)) {  // no groups then
+      if (threadIdx.x == 0) atomicOr(a.c.status, DEV_BAD_ARGS);
+      for (int i = threadIdx.x; i < units; i += 1024) off_s[i] = 0;
+      __syncthreads();
+    }
+    // (twice over the sequences: a group's prefix holds when all of it have been seen)
+#pragma unroll 1
+    for (int turn = 0; turn < 2; ++turn) {
+      for (int i = threadIdx.x; i < a.c.seqs; i += 1024) {
+        int lo = 0, hi = units - 1;  // the last group that starts at or before i
+        while (lo < hi) {
+          const int mid = (lo + hi + 1) >> 1;
+          if (g.start[mid] <= i) lo = mid;
+          else hi = mid - 1;
+        }
+        const bool in = g.start[lo] <= i && i < g.start[lo + 1];
+        const Seq s = load_seq(a.c, i);
+        if (turn == 0) {
+          const int slot = a.c.slot ? a.c.slot[i] : i;
+          if (in && off_s[lo] > 0 &&
+              (a.c.row_start[i + 1] - a.c.row_start[i] != s.n || slot < 0 || slot >= a.c.slots || s.pos < off_s[lo] ||
+               (int64_t)s.pos + s.n > (int64_t)a.c.width * a.c.page_size || s.n * group > kFewRows)) {
+            atomicOr(a.c.status, DEV_BAD_ARGS);
+            atomicExch(&off_s[lo], 0);
+          }
+        } else {
+          const int p = in ? off_s[lo] : 0;
+          g.first[i] = p;
+          if (s.n * group > kFewRows) atomicOr(a.c.status, DEV_BAD_ARGS);  // max_new was too small: nobody takes it
+          for (int t = 0; p > 0 && t < s.n; ++t) g.token_prefix[s.row0 + t] = p;
+        }
+      }
+      __syncthreads();
+    }
+  }
+  // unit i, its prefix (off_s[i] before off_s becomes the prefix sum, else its segments' pos)
+  auto load = [&](int i, int prefix) {
+    if constexpr (!PREFIX) return load_seq(a.c, i);
+    Seq s{};
+    if (prefix > 0) {
+      const int first = g.start[i];
+      s.row0 = a.c.row_start[first];
+      s.n = a.c.row_start[g.start[i + 1]] - s.row0;
+      s.pos = prefix - 1;
+    }
+    return s;
+  };
   int segs = 0, total;
-  for (int s0 = 0; s0 < a.c.seqs; s0 += 1024) {
+  for (int s0 = 0; s0 < units; s0 += 1024) {
     const int i = s0 + (int)threadIdx.x;
     int n = 0;
-    if (i < a.c.seqs) {
-      const Seq s = load_seq(a.c, i);
-      if (s.n * group > kFewRows) n = (s.n * group + ROWS - 1) / ROWS;
+    if (i < units) {
+      const Seq s = load(i, PREFIX ? off_s[i] : 0);
+      if (s.n * group > (PREFIX ? 0 : kFewRows)) n = (s.n * group + ROWS - 1) / ROWS;
     }
     const int at = segs + scan(n, total);
-    if (i < a.c.seqs) off_s[i] = at;
+    if (i < units) off_s[i] = at;
     segs += total;
   }
   __syncthreads();
@@ -129,7 +191,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
     int cost = 0, seq = 0, tile = 0;
     Seq s{};
     if (t < segs) {
-      int lo = 0, hi = a.c.seqs - 1;  // the last sequence with off <= t
+      int lo = 0, hi = units - 1;  // the last sequence with off <= t
       while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (off_s[mid] <= t) lo = mid;
@@ -137,11 +199,12 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
       }
       seq = lo;
       tile = t - off_s[lo];
-      s = load_seq(a.c, seq);
-      cost = seen_tiles<ROWS>(s, group, tile);
+      if constexpr (PREFIX) seq = g.start[lo];
+      s = load(lo, PREFIX ? g.first[seq] : 0);
+      cost = seen_tiles<ROWS>(s, group, tile, !PREFIX);
     }
     const int at = tiles + scan(cost, total);
-    if (t < segs) plan.seg[t] = {s.row0, s.n, s.pos, a.c.slot ? a.c.slot[seq] : seq, tile, at, at + cost, 0};
+    if (t < segs) plan.seg[t] = {s.row0, s.n, s.pos, a.c.slot ? a.c.slot[seq] : seq, tile, at, at + cost, !PREFIX};
     tiles += total;
   }
   __syncthreads();
@@ -166,10 +229,27 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
   }
 }
 
+template <int ROWS>
+cudaError_t launch_plan(const AttendArgs& a, const Plan& plan, cudaStream_t st) {
+  if (a.groups.n) return launch_ex(plan_kernel<ROWS, true>, dim3(1), dim3(1024), 0, st, a, plan);
+  return launch_ex(plan_kernel<ROWS, false>, dim3(1), dim3(1024), 0, st, a, plan);
+}
+// The few-token kernel that a call's chunks' kernel starts beside it: the sequences
+// with few rows, or, for groups' prefixes, all sequences' own positions.
+inline cudaError_t launch_beside(const AttendArgs& a, Kv kv, cudaStream_t st) {
+  if (!a.groups.n) return launch_few(a, kv, true, st);
+  AttendArgs own = a;
+  own.first = a.groups.first;
+  own.out = a.groups.out;
+  own.out_stride = a.groups.out_stride;
+  own.ml = a.groups.ml;
+  return launch_few(own, kv, true, st);
+}
+
 // What a CTA does of a segment.
 struct Piece {
   Seq s;
-  int kvh, r0, rows, first_tok, len, j0, nt, jm;
+  int kvh, r0, rows, first_tok, len, j0, nt, jm, step;
   int64_t seg0;
   bool two, whole;
 };
@@ -186,8 +266,9 @@ __device__ __forceinline__ Piece piece_of(const Params& p, int group, int t, int
   x.r0 = tile * ROWS;
   x.rows = min(ROWS, x.s.n * group - x.r0);
   x.two = x.rows > kTile;          // the second row tile has rows
-  x.first_tok = x.r0 / group;
-  x.len = x.s.pos + (x.r0 + x.rows - 1) / group + 1;  // positions the last row sees
+  x.step = place.w;
+  x.first_tok = x.step * (x.r0 / group);
+  x.len = x.s.pos + x.step * ((x.r0 + x.rows - 1) / group) + 1;  // positions the last row sees
   x.j0 = (int)(at - x.seg0);
   x.nt = (int)(min(end, x.seg0 + tiles) - at);
   x.whole = x.j0 == 0 && x.nt == tiles;
@@ -383,9 +464,14 @@ __device__ __forceinline__ float stage_rows(const AttendArgs& a, const Piece& x,
 // scores is then needed for a row's first tile alone.  l is the sum of the
 // weights so far, `down` what the outputs so far are to be multiplied by.
 // scale(v, c) is applied to the scores of columns c .. c + 31 before `factor`.
-template <typename Scale>
+// With VALUES the columns have factors up to 1 of their own, values[c], in a unit of
+// the tile, 2^lift: weights are 2^(s + lift - m), what is stored of them is times
+// those, and l is the sum of 2^(s - m).  (The reference then follows what the
+// stored products can be at most, over all tiles, whatever their units.)
+template <bool VALUES = false, typename Scale>
 __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool masked, int unseen_from, float factor, float& m,
-                                                  float& l, float& down, Scale scale) {
+                                                  float& l, float& down, Scale scale, const float* values = nullptr,
+                                                  float lift = 0.f) {
   auto mask = [&](float (&v)[32], int c) {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
@@ -411,16 +497,16 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
       if (masked) mask(v, c);
       top = fmaxf(top, largest(v));
     }
-    m = reference(top * factor);
+    m = reference(VALUES ? fmaf(top, factor, lift) : top * factor);
   }
-  float back = m == -INFINITY ? 0.f : -m, sum = 0.f, sum2 = 0.f;
+  float back = (m == -INFINITY ? 0.f : -m) + (VALUES ? lift : 0.f), sum = 0.f, sum2 = 0.f;
   down = 1.f;
   // 32 columns: scores to weights, hi and lo over them.  (Loops of 32
   // columns, not unrolled, and two copies of them: the comparisons of a
   // masked tile take as long as the rest, and the unrolled code ran out
   // of the instruction cache.)
   auto weigh = [&](float (&v)[32], int c) {
-    const float top = largest(v) * factor, over = top - m - kBias;
+    const float top = VALUES ? fmaf(largest(v), factor, lift) : largest(v) * factor, over = top - m - kBias;
     if (__any_sync(0xffffffffu, over > kSlack)) {
       // raise the reference, by whole powers of two where what there is so far
       // still counts (2^-64 of it does not: nor does a sum from before the first
@@ -434,7 +520,7 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
         m = fmaxf(m + ceilf(over), reference(top));
         f = ex2(before - m);
       }
-      back = m == -INFINITY ? 0.f : -m;
+      back = (m == -INFINITY ? 0.f : -m) + (VALUES ? lift : 0.f);
       down *= f;
       sum *= f;
       sum2 *= f;
@@ -462,9 +548,14 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
     for (int g = 0; g < 32; g += 16)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        const float y0 = ex2(fmaf(v[g + i], factor, back)), y1 = ex2(fmaf(v[g + i + 1], factor, back));
+        float y0 = ex2(fmaf(v[g + i], factor, back)), y1 = ex2(fmaf(v[g + i + 1], factor, back));
         sum += y0;
         sum2 += y1;
+        if constexpr (VALUES) {
+          const float2 f = *reinterpret_cast<const float2*>(values + c + g + i);
+          y0 *= f.x;
+          y1 *= f.y;
+        }
         const float h0 = high_part(y0), h1 = high_part(y1);
         w[g + (i >> 1)] = pack_f16(h0, h1);
         w[g + 8 + (i >> 1)] = pack_f16(y0 - h0, y1 - h1);
@@ -491,13 +582,13 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
       weigh(v, c);
     }
   }
-  l = fmaf(l, down, sum + sum2);
+  l = fmaf(l, down, VALUES ? (sum + sum2) * __uint_as_float((uint32_t)(127 - (int)lift) << 23) : sum + sum2);
 }
 
 // The results of a warp's 32 rows of a piece, row r this thread's: outputs, or
 // a partial result.  They go through the rows' own places in q_s, whose
 // queries no product reads any more, so that rows are written whole.
-template <int DIM, int ROWS, bool KV16>
+template <int DIM, int ROWS, Kv KV>
 __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int group, int cta, bool second, int r,
                                            uint8_t* q_s, const float (&o)[DIM], float m, float l, bool dirty) {
   constexpr int half = kTile * 128, kLanes = DIM / 4;  // lanes of a row
@@ -507,11 +598,12 @@ __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int 
   float* part = p.parts + (size_t)(2 * cta + second) * part_floats<ROWS>(DIM);
   int64_t mine = -1;
   if (in && x.whole) {
+    if (a.ml) a.ml[(int64_t)(x.s.row0 + tok) * a.heads + x.kvh * group + r - tok * group] = make_float2(m, l);
     mine = (int64_t)(x.s.row0 + tok) * a.out_stride + (int64_t)(x.kvh * group + r - tok * group) * DIM;
   } else if (in) {
     mine = (int64_t)(r - x.r0) * DIM;
     *reinterpret_cast<float2*>(part + (size_t)ROWS * DIM + 2 * (r - x.r0)) = make_float2(m, l);
-    if (KV16 && r == x.r0) part[(size_t)ROWS * (DIM + 2)] = dirty ? 1.0f : 0.0f;
+    if (KV == kF16 && r == x.r0) part[(size_t)ROWS * (DIM + 2)] = dirty ? 1.0f : 0.0f;
   }
   const float inv = x.whole ? 1.0f / l : 1.0f;
   uint8_t* row = q_s + (row0 + lane) * 128;
@@ -539,7 +631,8 @@ __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int 
   }
   __syncwarp();
   odd = __any_sync(0xffffffffu, odd);
-  if (!x.whole || !(odd || dirty)) return;
+  if (is_8bit(KV) || !x.whole || !(odd || dirty)) return;
+  constexpr bool KV16 = KV == kF16;
   // infinities and NaN of V that the rows see (non_finite()); one that all see
   // shows in their outputs
   const int first = x.s.pos + x.first_tok;
@@ -548,7 +641,7 @@ __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int 
 #pragma unroll 1
   for (int i = lane / kLanes; i < 32; i += 32 / kLanes) {
     const int64_t off = __shfl_sync(0xffffffffu, mine, i);
-    const int last = x.s.pos + __shfl_sync(0xffffffffu, tok, i);
+    const int last = x.s.pos + x.step * __shfl_sync(0xffffffffu, tok, i);
     const float sum = __shfl_sync(0xffffffffu, l, i);
     if (off >= 0 && isfinite(sum)) {
       const Sums<4> own = non_finite<KV16, 4>(a.c, x.s, x.kvh, first, last, 4 * c);
@@ -565,7 +658,7 @@ __device__ __forceinline__ void store_rows(const Params& p, const Piece& x, int 
 // picks 32 of its rows.  The pieces' factors of all rows first, then four rows
 // of outputs per warp with the loads of four pieces in flight together.
 constexpr int kJoinRows = 32;
-template <int DIM, int ROWS, bool KV16>
+template <int DIM, int ROWS, Kv KV>
 __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Params p) {
   const AttendArgs& a = p.a;
   grid_dependency_wait();
@@ -589,6 +682,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
     if (hits < 32) break;
   }
   const int4 seq = *reinterpret_cast<const int4*>(p.plan.seg + t);
+  const int step = p.plan.seg[t].step;
   const Seq s{seq.x, seq.y, seq.z, a.c.table + (int64_t)seq.w * a.c.width};
   const int r0 = p.plan.seg[t].tile * ROWS, row0 = blockIdx.y * kJoinRows;
   const int rows = min(kJoinRows, s.n * group - r0 - row0);
@@ -597,7 +691,7 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
   const float* part1 = p.parts + (size_t)(2 * cta) * part_floats<ROWS>(DIM);
   auto part = [&](int i) { return i ? part1 + (size_t)(2 * i) * part_floats<ROWS>(DIM) : part0; };
   bool dirty = false;
-  for (int i = lane; KV16 && i < n; i += 32) dirty = dirty || part(i)[(size_t)ROWS * (DIM + 2)] != 0.f;
+  for (int i = lane; KV == kF16 && i < n; i += 32) dirty = dirty || part(i)[(size_t)ROWS * (DIM + 2)] != 0.f;
   for (int x = threadIdx.x; x < n * kJoinRows; x += 256) {
     const int row = x % kJoinRows, i = x / kJoinRows;
     ml_s[i][row] = row < rows ? reinterpret_cast<const float2*>(part(i) + (size_t)ROWS * DIM)[row0 + row] : make_float2(0.f, 1.f);
@@ -616,6 +710,10 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
       ml_s[i][row].x = f;
     }
     l_s[row] = l;
+    if (a.ml && row < rows) {
+      const int r = r0 + row0 + row, tok = r / group;
+      a.ml[(int64_t)(s.row0 + tok) * a.heads + kvh * group + r - tok * group] = make_float2(top, l);
+    }
   }
   __syncthreads();
   constexpr int N = DIM / 32;  // neighbouring values per lane, rows warp, warp + 8 ..
@@ -656,15 +754,16 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
       to[k] = y;
     }
   }
-  if (!odd && !dirty) return;
-  const int first = s.pos + r0 / group;
+  if (is_8bit(KV) || (!odd && !dirty)) return;
+  constexpr bool KV16 = KV == kF16;
+  const int first = s.pos + step * (r0 / group);
   Sums<N> before{};
   if (odd) before = non_finite<KV16, N>(a.c, s, kvh, -1, first, N * lane);
 #pragma unroll 1
   for (int row = warp; row < rows; row += 8) {
     if (!isfinite(l_s[row])) continue;
     float* to = place(r0 + row0 + row);
-    const Sums<N> own = non_finite<KV16, N>(a.c, s, kvh, first, s.pos + (r0 + row0 + row) / group, N * lane);
+    const Sums<N> own = non_finite<KV16, N>(a.c, s, kvh, first, s.pos + step * ((r0 + row0 + row) / group), N * lane);
 #pragma unroll
     for (int k = 0; k < N; ++k)
       if (before.v[k] + own.v[k] != 0.f) to[k] = before.v[k] + own.v[k];

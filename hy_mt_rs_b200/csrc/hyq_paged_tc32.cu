@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
     while (at < end && ok) {
       const Piece x = piece_of<kRows>(p, group, t, kvh, at, end);
       const int r = x.r0 + 32 * warp + lane;  // row of the sequence
-      const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + tok;
+      const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + x.step * tok;
       const bool second = at != begin;
       next(x);
       const float factor = stage_rows<DIM>(a, x, group, x.r0, base_g + L::q);
@@ -424,7 +424,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       }
       if (ok) collect(down, back);
       if (!ok) break;
-      store_rows<DIM, kRows, false>(p, x, group, cta, second, r, base_g + L::q, o, m, l, false);
+      store_rows<DIM, kRows, kF32>(p, x, group, cta, second, r, base_g + L::q, o, m, l, false);
     }
   }
   if (!ok) {
@@ -450,11 +450,11 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   auto k = chunk_tc32_kernel<DIM>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
-  if (e == cudaSuccess) e = launch_ex(plan_kernel<kRows>, dim3(1), dim3(1024), 0, st, a, p.plan);
+  if (e == cudaSuccess) e = launch_plan<kRows>(a, p.plan, st);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
-  if (e == cudaSuccess) e = launch_few(a, kF32, true, st);
+  if (e == cudaSuccess) e = launch_beside(a, kF32, st);
   if (e == cudaSuccess)
-    e = launch_next(join_kernel<DIM, kRows, false>, dim3(kMaxCtas, kRows / kJoinRows), dim3(256), 0, st, p);
+    e = launch_next(join_kernel<DIM, kRows, kF32>, dim3(kMaxCtas, kRows / kJoinRows), dim3(256), 0, st, p);
   return e;
 }
 

@@ -1,0 +1,506 @@
+// Attention of chunks of new tokens over an 8-bit paged cache on tcgen05, head
+// sizes 64 and 128, at f32 accuracy over the values that the codes stand for.
+//
+// The f16 kernel's line of segments, products and softmax (hyq_paged_tc.cu,
+// hyq_paged_tc.cuh): a code is a whole f16 number (or 2^-8 of an e4m3 value), so the
+// products are the same four, S = Qh K' + Ql K' and X = Ph V + Pl V.  K's scales
+// multiply the columns of S.  V's go into the weights, as f16 pairs in the unit of
+// the tile's largest scale; the running reference of a row counts that unit in
+// (scores_to_weights()), so that tiles of any units may follow each other.
+//
+//   warp 1       tcgen05.mma, as in the f16 kernel;
+//   warps 4-7    codes and scales from global memory (a tile's while the tensor
+//                cores are at the one before), to f16 in a ring of three tiles of K
+//                and V, in the layout that TMA gives the f16 kernel;
+//   warps 8-11, 12-15   softmax of row tile 0 and 1, a thread per row.
+//
+// A tile whose scales of V are more than 2^10 apart, or not finite at a position of
+// the sequence, is left out of the products (its weights are zeros there); each
+// softmax thread then goes through the positions that its row sees, in f32.
+#include "hyq_paged_tc.cuh"
+
+namespace hyq {
+namespace paged {
+namespace {
+
+constexpr int kCtaRows = 2 * kTile;      // rows of a segment
+constexpr int kThreads = 512;
+constexpr int kSlots = 3;                // tiles of K or V in shared memory
+constexpr int kSpread = 10;              // of the exponents of a tile's scales of V
+
+template <int DIM>
+struct Smem {
+  static constexpr int half = kTile * 128;               // 128 rows of 64 f16
+  static constexpr int tile = half * (DIM / 64);         // K, V, or one half (hi or lo) of a Q tile
+  static constexpr int q = 0;                            // [row tile][hi, lo]
+  static constexpr int ring = 4 * tile;
+  static constexpr int k_scale = ring + kSlots * tile;   // [2][128]: of tile i in i & 1
+  static constexpr int v_scale = k_scale + 2 * kTile * 4;
+  static constexpr int top = v_scale + 2 * kTile * 4;    // [2][4 warps] largest and smallest scale's bits
+  static constexpr int bars = top + 2 * 4 * 8;
+  // full[3], empty[3], s_full[2], p_full[2], x_full[2], q_full[2], scales[2]
+  static constexpr int n_bars = 2 * kSlots + 10;
+  // tensor memory address, abort, then [2] of: tile that is left out (its number +
+  // 1), exponent of the tile's unit
+  static constexpr int misc = bars + 8 * n_bars;
+  static constexpr int total = misc + 32;
+};
+
+// (the base is aligned to 1024 bytes by its declaration, and checked)
+template <int DIM, Kv KV>
+__global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_constant__ Params p) {
+  using L = Smem<DIM>;
+  constexpr int KS = DIM / 16;            // steps of 16 along the head
+  constexpr uint32_t kTmemCols = 512;
+  const AttendArgs& a = p.a;
+  extern __shared__ __align__(1024) uint8_t smem[];
+  const uint32_t base = smem_addr(smem);
+  auto full = [&](int s) { return base + L::bars + 8 * s; };
+  auto empty = [&](int s) { return base + L::bars + 8 * (kSlots + s); };
+  auto s_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + w); };
+  auto p_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 2 + w); };
+  auto x_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 4 + w); };
+  auto q_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 6 + w); };
+  auto scales = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 8 + (i & 1)); };  // of tile i: phase i / 2
+  float* k_scale_s = reinterpret_cast<float*>(smem + L::k_scale);
+  float* v_scale_s = reinterpret_cast<float*>(smem + L::v_scale);
+  volatile int* misc = reinterpret_cast<volatile int*>(smem + L::misc);
+  volatile int* abort_flag = misc + 1;
+  volatile int* out_s = misc + 2;
+  volatile int* lift_s = misc + 4;
+  const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
+  const int group = a.heads / a.c.kv_heads;
+
+  grid_dependency_wait();
+  allow_dependents_launch();
+  const int cta = blockIdx.x;
+  const Start start = p.plan.start[cta];
+  const int64_t begin = start.begin, end = p.plan.start[cta + 1].begin;
+  if (begin == end) return;  // nothing allocated yet
+  if (base & 1023u) {        // (the swizzled layouts need it)
+    if (threadIdx.x == 0) atomicOr(a.c.status, DEV_BAD_ARGS);
+    return;
+  }
+  if (warp == 0) {
+    if (lane == 0) {
+      misc[1] = 0;
+      misc[2] = misc[3] = 0;
+      for (int s = 0; s < kSlots; ++s) {
+        mbar_init(full(s), 4);
+        mbar_init(empty(s), 1);
+      }
+      for (int w = 0; w < 2; ++w) {
+        mbar_init(s_full(w), 1);
+        mbar_init(p_full(w), 4);
+        mbar_init(x_full(w), 1);
+        mbar_init(q_full(w), 4);
+        mbar_init(scales(w), 4);
+      }
+      mbar_fence_init();
+    }
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(base + L::misc), "r"(kTmemCols));
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+  }
+  fence_before();
+  __syncthreads();
+  fence_after();
+  const uint32_t tmem = (uint32_t)uniform(misc[0]);
+  // every warp walks the same pieces: (segment, kv head), at its tile `at`
+  int t = start.t, kvh = start.kvh;
+  int64_t at = begin;
+  auto next = [&](const Piece& x) {
+    at += x.nt;
+    if (++t == p.plan.count[0]) {
+      t = 0;
+      ++kvh;
+    }
+  };
+
+  // launch: 128 registers x 512 threads = (40 + 72 + 2 x 200) x 128
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    if (warp == 1) {
+      // ------------------------------ products -------------------------------
+      // f32 sums, f16 operands, M 128; N 128 positions, or DIM columns with V
+      // along its rows (bit 16)
+      constexpr uint32_t idesc_s = (1u << 4) | ((uint32_t)(kTile >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+      constexpr uint32_t idesc_o = (1u << 4) | (1u << 16) | ((uint32_t)(DIM >> 3) << 17) | ((uint32_t)(kTile >> 4) << 24);
+      auto wait = [&](uint32_t bar, uint32_t parity) {
+        if (warp_wait(bar, parity, abort_flag)) return true;
+        if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_FULL);
+        *abort_flag = 1;
+        return false;
+      };
+      const uint64_t q_desc = desc_k_major(base + L::q), k_desc = desc_k_major(base + L::ring);
+      const uint64_t v_desc = desc_mn_major(base + L::ring, L::half);
+      const bool one = elect();
+      // lo first: the large sums then take half the (cut) additions
+      auto scores = [&](int w, int slot) {
+        const uint64_t q = q_desc + w * (2 * L::tile >> 4), k = k_desc + slot * (L::tile >> 4);
+#pragma unroll
+        for (int h = 1; h >= 0; --h)
+#pragma unroll
+          for (int t = 0; t < KS; ++t) {
+            const int off = ((t >> 2) * L::half + (t & 3) * 32) >> 4;
+            mma_ss(tmem + 256 * w, q + h * (L::tile >> 4) + off, k + off, idesc_s, h == 0 || t > 0);
+          }
+      };
+      auto outputs = [&](int w, int slot) {
+        const uint64_t v = v_desc + slot * (L::tile >> 4);
+        const uint32_t pw = tmem + 256 * w;
+#pragma unroll
+        for (int h = 1; h >= 0; --h)
+#pragma unroll
+          for (int t = 0; t < kTile / 16; ++t)  // 16 positions: hi in 8 columns from 16 t, lo in the next 8
+            mma_ts(pw + 128, pw + 16 * t + 8 * h, v + t * (16 * 128 >> 4), idesc_o, h == 0 || t > 0);
+      };
+      // slot and phase of the ring's next tile
+      int slot = 0, phase = 0;
+      auto advance = [&]() {
+        if (++slot == kSlots) {
+          slot = 0;
+          phase ^= 1;
+        }
+      };
+      int steps[2] = {0, 0}, pieces[2] = {0, 0}, issued = 0;
+      bool ok = true;
+      while (at < end && ok) {
+        const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+        const int active = uniform(x.two ? 2 : 1), nt = uniform(x.nt);
+        ok = wait(full(slot), phase);
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {
+          if (w >= active || !ok) break;
+          ok = wait(q_full(w), pieces[w] & 1);
+          if (!ok) break;
+          fence_after();
+          if (one) {
+            scores(w, slot);
+            commit(s_full(w));
+            if (w == active - 1) commit(empty(slot));
+          }
+          __syncwarp();
+        }
+        if (ok) ++issued;
+        advance();
+        for (int j = 0; j < nt && ok; ++j) {
+          const int v_slot = slot;
+          ok = wait(full(slot), phase);
+          advance();
+          const int k_slot = slot;
+          if (ok && j + 1 < nt) {
+            ok = wait(full(slot), phase);
+            advance();
+          }
+#pragma unroll
+          for (int w = 0; w < 2; ++w) {
+            if (w >= active || !ok) break;
+            ok = wait(p_full(w), steps[w] & 1);
+            if (!ok) break;
+            ++steps[w];
+            fence_after();
+            if (one) {
+              outputs(w, v_slot);
+              commit(x_full(w));
+              if (w == active - 1) commit(empty(v_slot));
+              if (j + 1 < nt) {
+                scores(w, k_slot);
+                commit(s_full(w));
+                if (w == active - 1) commit(empty(k_slot));
+              }
+            }
+            __syncwarp();
+          }
+          if (ok) issued += j + 1 < nt ? 2 : 1;
+        }
+        ++pieces[0];
+        if (active == 2) ++pieces[1];
+        next(x);
+      }
+      // no product's arrival may come after this CTA is gone
+      for (int i = max(0, issued - kSlots); i < issued; ++i)
+        if (!warp_wait(empty(i % kSlots), (i / kSlots) & 1, nullptr) && lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_DRAIN);
+    }
+  } else if (warp < 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    // ------------------------------- K and V --------------------------------
+    constexpr int LPR = DIM / 16;         // lanes of a row, 16 codes each
+    constexpr int RPI = 32 / LPR, IT = LPR;
+    const int lw = warp - 4, pos_in = threadIdx.x - 128;
+    uint2* top_s = reinterpret_cast<uint2*>(smem + L::top);
+    Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+    const int tiles = uniform((int)(end - begin));
+    int j = 0, issued = 0, lift = 0;
+    bool ok = true;
+    uint4 r[IT];
+    // where row `row` of the tile begins, or -1
+    auto page_row = [&](int row, int& in_page) {
+      const int pos = (x.j0 + j) * kTile + row;
+      in_page = pos % a.c.page_size;
+      return pos < x.len ? checked_page(a.c, x.s.pages[pos / a.c.page_size]) : -1;
+    };
+    int64_t here = -1;    // of row (lane / RPI) of the warp's (lane % RPI)th rows
+    float ks = 0.f, vs = 0.f;
+    bool held = false;    // this thread's position is one of the sequence's
+    auto open = [&]() {
+      int in_page, page = page_row((lane / RPI) * 4 * RPI + lw * RPI + lane % RPI, in_page);
+      here = page < 0 ? -1
+                      : (int64_t)page * a.c.page_stride + (int64_t)x.kvh * a.c.head_stride + (int64_t)in_page * a.c.row_stride;
+      page = page_row(pos_in, in_page);
+      held = page >= 0;
+      const int64_t at_scale = held ? scale_at(a.c, page, x.kvh, in_page) : 0;
+      ks = held ? a.c.k_scale[at_scale] : 0.f;
+      vs = held ? a.c.v_scale[at_scale] : 0.f;
+    };
+    auto load = [&](const void* from) {
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int64_t o = __shfl_sync(0xffffffffu, here, i * RPI + lane / LPR);
+        const uint8_t* row = static_cast<const uint8_t*>(from) + max(o, (int64_t)0) + 16 * (lane % LPR);
+        r[i] = o >= 0 ? *reinterpret_cast<const uint4*>(row) : make_uint4(0, 0, 0, 0);
+      }
+    };
+    auto take = [&]() {  // the ring's next slot
+      const int slot = issued % kSlots;
+      ok = issued < kSlots || warp_wait(empty(slot), ((issued / kSlots) - 1) & 1, abort_flag);
+      ++issued;
+      return slot;
+    };
+    auto put = [&](int slot) {
+      uint8_t* to = smem + L::ring + slot * L::tile;
+      const int c0 = 2 * (lane % LPR);
+      const bool swap = DIM == 128 && (c0 & 8);  // the two chunks in turn: distinct banks
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int row = i * 4 * RPI + lw * RPI + lane / LPR;
+        uint32_t w[8];
+        const uint32_t in[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+#pragma unroll
+        for (int k = 0; k < 4; ++k) decode4<KV>(__byte_perm(in[k], 0, 0x3120), w[2 * k], w[2 * k + 1]);
+        uint8_t* line = to + (c0 >> 3) * L::half + row * 128;
+        const int even = ((c0 & 7) ^ (row & 7)) << 4, odd = (((c0 & 7) | 1) ^ (row & 7)) << 4;
+        const uint4 lo = make_uint4(w[0], w[1], w[2], w[3]), hi = make_uint4(w[4], w[5], w[6], w[7]);
+        *reinterpret_cast<uint4*>(line + (swap ? odd : even)) = swap ? hi : lo;
+        *reinterpret_cast<uint4*>(line + (swap ? even : odd)) = swap ? lo : hi;
+      }
+      fence_proxy_async_smem();
+    };
+    open();
+    load(a.c.k);
+#pragma unroll 1
+    for (int i = 0; i < tiles; ++i) {
+      const int k_slot = take();
+      if (!ok) break;
+      // (the softmax of tile i - 2 is done: its V's slot is free)
+      const uint32_t bits = __float_as_uint(vs);
+      const bool usable = bits - 1u < 0x7f7fffffu;  // positive and finite
+      const uint32_t most = __reduce_max_sync(0xffffffffu, usable ? bits : 0u),
+                     least = __reduce_min_sync(0xffffffffu, usable ? bits : 0x7f800000u);
+      const bool bad = __any_sync(0xffffffffu, held && !isfinite(vs));
+      if (lane == 0) top_s[(i & 1) * 4 + lw] = make_uint2(most, bad ? 0u : least);
+      put(k_slot);
+      asm volatile("bar.sync 1, 128;" ::: "memory");
+      uint32_t top = 0, low = 0x7f800000u;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint2 o = top_s[(i & 1) * 4 + w];
+        top = max(top, o.x);
+        low = min(low, o.y);
+      }
+      // the unit: above the largest scale (a tile of zeros keeps the one before)
+      if (top) lift = min(max((int)(top >> 23) - 126, -100), 100);
+      const float unit = code_unit<KV>(), down = __uint_as_float((uint32_t)(127 - lift) << 23);
+      k_scale_s[(i & 1) * kTile + pos_in] = ks * unit;
+      v_scale_s[(i & 1) * kTile + pos_in] = isfinite(vs) ? vs * down : 0.f;
+      if (pos_in == 0) {
+        lift_s[i & 1] = lift;
+        out_s[i & 1] = low == 0u || (top && (top >> 23) > (low >> 23) + kSpread) ? i + 1 : 0;
+      }
+      __syncwarp();
+      if (lane == 0) {
+        mbar_arrive(scales(i));
+        mbar_arrive(full(k_slot));
+      }
+      load(a.c.v);
+      const int v_slot = take();
+      if (!ok) break;
+      put(v_slot);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full(v_slot));
+      if (i + 1 < tiles) {
+        if (++j == x.nt) {
+          next(x);
+          x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+          j = 0;
+        }
+        open();
+        load(a.c.k);
+      }
+    }
+    if (!ok) {
+      if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_EMPTY);
+      *abort_flag = 1;
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 200;");
+    // -------------------------------- softmax -------------------------------
+    const int wg = warp >= 12 ? 1 : 0;  // row tile
+    const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 * wg;
+    int steps = 0, tile = 0;  // this row tile's steps, all tiles of the CTA
+    bool ok = true;
+    while (at < end && ok) {
+      const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+      const int r = x.r0 + wg * kTile + 32 * (warp & 3) + lane;  // row of the sequence
+      const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + x.step * tok;
+      const int64_t piece_at = at;
+      next(x);
+      if (wg == 1 && !x.two) {
+        tile += x.nt;
+        continue;
+      }
+      const float factor = stage_rows<DIM>(a, x, group, x.r0 + wg * kTile, smem + L::q + wg * 2 * L::tile);
+      if (lane == 0) mbar_arrive(q_full(wg));
+      float o[DIM];
+#pragma unroll
+      for (int d = 0; d < DIM; ++d) o[d] = 0.f;
+      float m = -INFINITY, l = 0.f, down = 1.f;
+      // the product of the tile before, added to the row's outputs
+      auto collect = [&](int step) {
+        if (!warp_wait(x_full(wg), step & 1, abort_flag)) return false;
+        fence_after();
+        tmem_each<DIM>(st + 128, [&](float (&v)[16], int c) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) o[c + i] = fmaf(o[c + i], down, v[i]);
+        });
+        return true;
+      };
+      for (int j = 0; j < x.nt; ++j, ++steps, ++tile) {
+        // (while the tensor cores are at this tile's scores, which follow its scales:
+        // the wait for those skips no phase)
+        ok = (j == 0 || collect(steps - 1)) && warp_wait(s_full(wg), steps & 1, abort_flag) &&
+             warp_wait(scales(tile), (tile >> 1) & 1, abort_flag);
+        if (!ok) break;
+        fence_after();
+        const int p0 = (x.j0 + j) * kTile;
+        const float* ks = k_scale_s + (tile & 1) * kTile;
+        if (uniform(out_s[tile & 1]) == tile + 1) {
+          // in f32, each position in the unit of its own scale
+          constexpr float scale = (DIM == 128 ? 0.08838834764831845f : 0.125f) * kLog2e;
+          const float* q = a.q + (int64_t)(x.s.row0 + tok) * a.q_stride + (int64_t)(x.kvh * group + r % group) * DIM;
+          const float lift = (float)lift_s[tile & 1];
+#pragma unroll 1
+          for (int pos = p0; pos < min(p0 + kTile, sees + 1); ++pos) {
+            const int page = x.s.pages[pos / a.c.page_size], in_page = pos % a.c.page_size;
+            const bool in = page >= 0 && page < a.c.pages;  // (no page: zeros, as for the products)
+            const int64_t row = (int64_t)(in ? page : 0) * a.c.page_stride + (int64_t)x.kvh * a.c.head_stride +
+                                (int64_t)in_page * a.c.row_stride;
+            const uint32_t* kc = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.c.k) + row);
+            const uint32_t* vc = reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(a.c.v) + row);
+            const float v_unit = in ? a.c.v_scale[scale_at(a.c, page, x.kvh, in_page)] : 0.f;
+            float s = 0.f;
+#pragma unroll 4
+            for (int d = 0; d < DIM / 4; ++d) {
+              const uint32_t w = in ? kc[d] : 0u;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) s = fmaf(q[4 * d + i], code_value<KV>((uint8_t)(w >> (8 * i))), s);
+            }
+            s *= scale * (ks[pos - p0] / code_unit<KV>());
+            const bool usable = v_unit > 0.f && isfinite(v_unit);
+            const float own = usable ? fminf(fmaxf((float)((int)(__float_as_uint(v_unit) >> 23) - 126), -100.f), 100.f) : lift;
+            const float u = s + own, back = __uint_as_float((uint32_t)(127 - (int)own) << 23);
+            if (m == -INFINITY) {
+              m = reference(u);
+            } else if (u - m > kBias + kSlack) {
+              const float f = ex2(m - reference(u));
+              m = reference(u);
+              l *= f;
+#pragma unroll
+              for (int d = 0; d < DIM; ++d) o[d] *= f;
+            }
+            const float w = u == -INFINITY ? 0.f : ex2(u - m);
+            l = fmaf(w, back, l);
+            const float wv = w * (v_unit * back);
+#pragma unroll
+            for (int d = 0; d < DIM / 4; ++d) {
+              const uint32_t c = in ? vc[d] : 0u;
+#pragma unroll
+              for (int i = 0; i < 4; ++i) o[4 * d + i] = fmaf(wv, code_value<KV>((uint8_t)(c >> (8 * i))) / code_unit<KV>(), o[4 * d + i]);
+            }
+          }
+          __syncwarp();
+          down = 1.f;
+          const uint32_t zero[16] = {};
+#pragma unroll 1
+          for (int c = 0; c < kTile; c += 16) tmem_st(st + c, zero);
+        } else {
+          scores_to_weights<true>(
+              st, j == 0, j >= x.jm, sees - p0 + 1, factor, m, l, down,
+              [&](float (&v)[32], int c) {
+                const float4* f4 = reinterpret_cast<const float4*>(ks + c);
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                  const float4 f = f4[k];
+                  v[4 * k] *= f.x, v[4 * k + 1] *= f.y, v[4 * k + 2] *= f.z, v[4 * k + 3] *= f.w;
+                }
+              },
+              v_scale_s + (tile & 1) * kTile, (float)lift_s[tile & 1]);
+        }
+        tmem_wait_st();
+        fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(p_full(wg));
+      }
+      ok = ok && collect(steps - 1);
+      if (!ok) {
+        if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_FULL);
+        *abort_flag = 1;
+        break;
+      }
+      if constexpr (KV == kF8) {
+#pragma unroll
+        for (int d = 0; d < DIM; ++d) o[d] *= code_unit<KV>();
+      }
+      store_rows<DIM, kCtaRows, KV>(p, x, group, cta, piece_at != begin, r, smem + L::q + wg * 2 * L::tile, o, m, l, false);
+    }
+  }
+  fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(kTmemCols));
+  }
+}
+
+template <int DIM, Kv KV>
+cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
+  Params p;
+  p.a = a;
+  p.box = 0;
+  char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
+  p.plan = plan_of<kCtaRows>(a, ws);
+  p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
+  auto k = chunk_tc8_kernel<DIM, KV>;
+  static std::atomic<uint64_t> done{0};
+  cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
+  if (e == cudaSuccess) e = launch_plan<kCtaRows>(a, p.plan, st);
+  if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
+  if (e == cudaSuccess) e = launch_beside(a, KV, st);
+  if (e == cudaSuccess) e = launch_next(join_kernel<DIM, kCtaRows, KV>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p);
+  return e;
+}
+
+template <Kv KV>
+cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
+  return a.c.dim == 128 ? launch<128, KV>(a, st) : launch<64, KV>(a, st);
+}
+
+}  // namespace
+
+bool tc8_supported(const AttendArgs& a) { return plan_fits<kCtaRows>(a); }
+
+cudaError_t launch_chunks_tc8(const AttendArgs& a, Kv kv, cudaStream_t st) { return kv == kI8 ? launch<kI8>(a, st) : launch<kF8>(a, st); }
+
+}  // namespace paged
+}  // namespace hyq

@@ -204,7 +204,38 @@ PyObject* attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
-// k_pages, v_pages, table, row_start, pos, tokens (-1: k_out's), f16, slot, k_out,
+// q, k_pages, v_pages, table, row_start, pos, group_start, shared, max_new, max_len
+// (-1: the table's reach), max_shared (-1: max_len), slot, out, workspace, k_scale,
+// v_scale
+PyObject* attention_shared(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded(n, 16, [&]() -> PyObject* {
+    const at::Tensor& q = typed(a[0], "q", at::kFloat);
+    const hyq_paged_kv8 kv8 = make_kv(q, a[1], a[2], a[3], a[14], a[15]);
+    const hyq_paged_kv& kv = kv8.kv;
+    const int64_t qs = row_stride(q, "q"), given = whole(a[9]), max_len = given < 0 ? kv.table_width * kv.page_size : given;
+    const int64_t max_shared = whole(a[10]);
+    const hyq_paged_batch batch = make_batch(q, a[4], a[5], a[11], q.size(0), whole(a[8]), max_len);
+    if (q.size(2) != kv.head_dim) refuse(HYQ_E_SHAPE, "attention_shared: head_dim of q and the pages");
+    const at::Tensor &start = plain(a[6], "group_start", at::kInt), &shared = plain(a[7], "shared", at::kInt);
+    same_device(q, start, "group_start");
+    same_device(q, shared, "shared");
+    if (start.numel() != shared.numel() + 1) refuse(HYQ_E_SHAPE, "group_start takes one more entry than shared");
+    const at::Tensor out = output(a[12], q, q.sizes(), at::kFloat, "out");
+    const at::Tensor& ws = plain(a[13], "workspace", at::kByte);
+    same_device(q, ws, "workspace");
+    size_t bytes = 0;
+    check(hyq_paged_attention_shared_workspace_bytes((int)q.size(1), kv.head_dim, q.size(0), &bytes));
+    if ((size_t)ws.numel() < bytes) refuse(HYQ_E_SHAPE, "attention_shared: the workspace takes " + std::to_string(bytes) + " bytes");
+    const c10::cuda::CUDAGuard device(q.device());
+    check(hyq_paged_attention_shared(&kv8, &batch, static_cast<const int32_t*>(start.data_ptr()),
+                                     static_cast<const int32_t*>(shared.data_ptr()), shared.numel(), max_shared < 0 ? max_len : max_shared,
+                                     static_cast<const float*>(q.data_ptr()), qs, (int)q.size(1), static_cast<float*>(out.data_ptr()),
+                                     row_stride(out, "out"), ws.data_ptr(), stream_of(q)));
+    return THPVariable_Wrap(out);
+  });
+}
+
+// k_pages, v_pages, table, row_start, pos, tokens, f16, slot, k_out,
 // v_out, k_scale, v_scale
 PyObject* gather(PyObject*, PyObject* const* a, Py_ssize_t n) {
   return guarded(n, 12, [&]() -> PyObject* {
@@ -346,6 +377,7 @@ PyObject* adjust(PyObject*, PyObject* const* a, Py_ssize_t n) {
 PyMethodDef methods[] = {
     {"adjust", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(adjust)), METH_FASTCALL, nullptr},
     {"attention", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(attention)), METH_FASTCALL, nullptr},
+    {"attention_shared", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(attention_shared)), METH_FASTCALL, nullptr},
     {"gather", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(gather)), METH_FASTCALL, nullptr},
     {"rope_append", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(rope_append)), METH_FASTCALL, nullptr},
     {"sample", reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(sample)), METH_FASTCALL, nullptr},

@@ -21,7 +21,8 @@ import torch
 from ._native import HyqError, check, lib, load_ops
 from .quant import _need_cuda, _ptr
 
-__all__ = ["PagedCache", "REFUSED", "rope_append", "gather", "attention", "attention_workspace"]
+__all__ = ["PagedCache", "REFUSED", "rope_append", "gather", "attention", "attention_workspace",
+           "attention_shared", "attention_shared_workspace"]
 
 REFUSED = 2147483647    # HYQ_PAGES_REFUSED
 
@@ -91,6 +92,34 @@ def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None,
 def _check_int(t, name):
     if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dtype != torch.int32 or not t.is_contiguous():
         _need_cuda(t, name, torch.int32)
+
+
+def attention_shared_workspace(heads, head_dim, tokens, device):
+    """A workspace for attention_shared() calls with these heads and at most so
+    many tokens; calls that share one must not overlap in time."""
+    n = C.c_size_t()
+    check(lib.hyq_paged_attention_shared_workspace_bytes(heads, head_dim, tokens, C.byref(n)))
+    workspace = torch.empty(n.value, dtype=torch.uint8, device=device)
+    workspace[:_ZEROED].zero_()
+    return workspace
+
+
+def attention_shared(q, k_pages, v_pages, table, row_start, pos, group_start, shared, max_new, max_len=None, max_shared=None,
+                     slot=None, out=None, workspace=None, k_scale=None, v_scale=None):
+    """hyq_paged_attention_shared: attention() of few new tokens (max_new times
+    the query heads per kv head at most 16) where groups of sequences share a
+    prefix, which is read once per group.  Group g is the sequences
+    group_start[g] .. group_start[g + 1] - 1; their first shared[g] positions
+    hold the same keys and values, read through the first one's pages.
+    max_shared bounds shared (max_len by default).  workspace:
+    attention_shared_workspace(...), made here when not given."""
+    if workspace is None:
+        if not isinstance(q, torch.Tensor) or q.dim() != 3:
+            raise HyqError(-2, "q: expected [tokens, heads, head_dim] with contiguous heads")
+        workspace = attention_shared_workspace(q.shape[1], q.shape[2], q.shape[0], q.device)
+    return _ops.attention_shared(q, k_pages, v_pages, table, row_start, pos, group_start, shared, max_new,
+                                 -1 if max_len is None else max_len, -1 if max_shared is None else max_shared, slot, out,
+                                 workspace, k_scale, v_scale)
 
 
 class PagedCache:

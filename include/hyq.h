@@ -539,6 +539,28 @@ int hyq_paged_rope_append_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* ba
 int hyq_paged_attention_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
                             int heads, float* out, int64_t out_stride, void* workspace, void* stream);
 
+/* Attention of sequences that share a prefix (answers forked from one prompt,
+ * requests behind one system prompt), the prefix read once per group: what
+ * hyq_paged_attention_kv8 gives for the same batch, in other roundings.
+ * Group g is the sequences group_start[g] .. group_start[g + 1] - 1 of the batch
+ * (`groups` of them, in order; sequences outside all are on their own), whose
+ * positions 0 .. shared[g] - 1 hold the same keys and values: they are read
+ * through the table row of the group's first sequence.  shared[g] is at most the
+ * pos of each of its sequences (else the group has no prefix: its sequences are
+ * taken each on their own, and HYQ_DEV_BAD_ARGS is raised; a group_start that
+ * does not ascend from 0 to seqs does that to all groups).  Every cache type; for
+ * few new tokens: max_new times the query heads per kv head is at most 16.
+ * max_shared bounds any shared[g] (a prefix past it counts all the same).
+ * Head sizes other than 64 and 128, and pages that the chunks' kernels do not take
+ * (f16: page_size 16, 32, 64 or a multiple of 128), go through
+ * hyq_paged_attention_kv8 instead.
+ * workspace: hyq_paged_attention_shared_workspace_bytes bytes for at least the
+ * batch's tokens, under hyq_paged_attention's rules. */
+int hyq_paged_attention_shared_workspace_bytes(int heads, int head_dim, int64_t tokens, size_t* bytes);
+int hyq_paged_attention_shared(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const int32_t* group_start,
+                               const int32_t* shared, int64_t groups, int64_t max_shared, const float* q, int64_t q_stride,
+                               int heads, float* out, int64_t out_stride, void* workspace, void* stream);
+
 /* Rows of a cache of any type as values: positions pos[s], pos[s] + 1, .. of
  * each sequence (the batch's rows, as hyq_paged_rope_append takes them; they need
  * not be new) into k and v [tokens, kv_heads, head_dim], f32 or, with f16, IEEE
