@@ -615,10 +615,10 @@ int attend(const hyq::paged::AttendArgs& a, hyq::paged::Kv type, int64_t max_new
   if (mma_supported(a, type)) {
     cudaError_t e;
     if (max_new * (a.heads / a.c.kv_heads) <= kFewRows) {
-      e = launch_few(a, type, false, st);
+      e = launch_few(a, type, max_new, false, st);
     } else if (chunks_short(a, type, max_len) || !chunks_tc_supported(a, type)) {
       e = launch_chunks(a, type, st);
-      if (e == cudaSuccess) e = launch_few(a, type, true, st);
+      if (e == cudaSuccess) e = launch_few(a, type, max_new, true, st);
     } else {
       e = launch_chunks_tc(a, type, st);
     }
@@ -714,6 +714,7 @@ int hyq_paged_attention_shared(const hyq_paged_kv8* kv, const hyq_paged_batch* b
   a.groups.start = group_start;
   a.groups.shared = shared;
   a.groups.n = (int)groups;
+  a.groups.max_new = batch->max_new;
   return done(launch_shared(a, type, st), name);
 }
 

@@ -183,6 +183,7 @@ struct Groups {
   float* out;
   int64_t out_stride;
   float2* ml;
+  int64_t max_new;        // of any sequence
 };
 
 // hyq_paged_attention's activations and output.
@@ -214,9 +215,9 @@ size_t mma_workspace_bytes(int dim);
 // Whether launch_few's 32-bit sum of tiles holds that many sequences of any
 // length up to `reach` (4,096 of 16 million positions).
 bool sums_fit(int64_t seqs, int64_t reach);
-// Sequences of up to kFewRows rows; `beside`: next to the kernel that the same
-// call launched before.
-cudaError_t launch_few(const AttendArgs& a, Kv kv, bool beside, cudaStream_t st);
+// Sequences of up to kFewRows rows (and, when that is less, as many as max_new tokens
+// have); `beside`: next to the kernel that the same call launched before.
+cudaError_t launch_few(const AttendArgs& a, Kv kv, int64_t max_new, bool beside, cudaStream_t st);
 cudaError_t launch_chunks(const AttendArgs& a, Kv kv, cudaStream_t st);  // the others
 // Whether that is faster than the kernels on tcgen05: one launch instead of
 // three, but every CTA goes through its rows' positions alone, at 0.04 us (f16
@@ -254,6 +255,7 @@ inline cudaError_t launch_chunks_tc(const AttendArgs& a, Kv kv, cudaStream_t st)
 // however coarse the scores are, and kept with the bias taken off, so that a
 // weight is 2^(s - m) to the last bit of s and m.
 constexpr float kBias = 10.0f;
+constexpr float kSlack = 5.0f;  // where the reference lags behind: a weight is at most 2^(kBias + kSlack), below f16's 65504
 constexpr float kLog2e = 1.4426950408889634f;
 __device__ __forceinline__ float reference(float top) { return __fsub_ru(top, kBias); }
 

@@ -24,7 +24,6 @@ template <int ROWS>
 __host__ __device__ constexpr size_t part_floats(int dim) {
   return (size_t)ROWS * (dim + 2) + 4;
 }
-constexpr float kSlack = 5.0f;           // a weight is at most 2^(kBias + kSlack): below f16's 65504
 
 // A segment: its sequence (n rows of tokens from row0 at pos, pages in `slot`),
 // which of the sequence's it is, the position tiles that come before and up to
@@ -237,13 +236,13 @@ cudaError_t launch_plan(const AttendArgs& a, const Plan& plan, cudaStream_t st) 
 // The few-token kernel that a call's chunks' kernel starts beside it: the sequences
 // with few rows, or, for groups' prefixes, all sequences' own positions.
 inline cudaError_t launch_beside(const AttendArgs& a, Kv kv, cudaStream_t st) {
-  if (!a.groups.n) return launch_few(a, kv, true, st);
+  if (!a.groups.n) return launch_few(a, kv, kFewRows, true, st);
   AttendArgs own = a;
   own.first = a.groups.first;
   own.out = a.groups.out;
   own.out_stride = a.groups.out_stride;
   own.ml = a.groups.ml;
-  return launch_few(own, kv, true, st);
+  return launch_few(own, kv, a.groups.max_new, true, st);
 }
 
 // What a CTA does of a segment.
