@@ -2,10 +2,12 @@
 // (include/hyq.h states the rule).
 //
 // A CTA takes a slice of a row: it asks for its logits first, and while they
-// come counts the slice's tokens among the row's history and finds the last bias
-// entry of each in shared memory (whole numbers: the order of the atomics does
-// not matter).  Bound by memory, 8 bytes a logit; the history is read by every
-// slice of its row, mostly from L2.
+// come counts the slice's tokens among the row's history in shared memory (whole
+// numbers: the order of the atomics does not matter).  Biases, which are few, come
+// after the slice is out: the last entry of each token is found in the counts' place.
+// Bound by memory, 8 bytes a logit; the history is read by every slice of its row,
+// mostly from L2, so slices are as long as registers hold, unless a call has too few
+// to fill the SMs with.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -19,8 +21,6 @@ namespace hyq {
 namespace logits {
 
 constexpr int kThreads = 256;
-constexpr int kPer = 16;                      // logits of a thread
-constexpr int kSlice = kThreads * kPer;
 constexpr unsigned kSeen = 0x80000000u;       // of a count: the token stands in the prompt
 
 struct Args {
@@ -46,12 +46,13 @@ __device__ __forceinline__ void each(const int32_t* list, int count, F f) {
   for (; i < count; i += kThreads) f(list[i], i);
 }
 
-__global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant__ Args a) {
+// PER: logits of a thread.
+template <int PER>
+__global__ void __launch_bounds__(kThreads, PER == 32 ? 4 : 8) adjust_kernel(const __grid_constant__ Args a) {
+  constexpr int kPer = PER, kSlice = kThreads * PER;
   grid_dependency_wait();
   allow_dependents_launch();
-  extern __shared__ __align__(16) unsigned smem[];
-  unsigned* count_s = smem;             // [kSlice]
-  unsigned* bias_s = smem + kSlice;     // [kSlice] last entry of each token, + 1 (with biases)
+  __shared__ __align__(16) unsigned count_s[kSlice];
   const int r = blockIdx.x / a.slices, lo = (blockIdx.x - r * a.slices) * kSlice, size = min(kSlice, a.n - lo);
   const float* x = a.x + r * a.x_stride + lo;
   float* out = a.out + r * a.out_stride + lo;
@@ -115,12 +116,8 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant_
   }
   // (uniform over the CTA from here on)
   if (length > 0) {
-    for (int i = threadIdx.x; i < kSlice / 4; i += kThreads) reinterpret_cast<uint4*>(count_s)[i] = make_uint4(0, 0, 0, 0);
-  }
-  if (biases > 0) {
-    for (int i = threadIdx.x; i < kSlice / 4; i += kThreads) reinterpret_cast<uint4*>(bias_s)[i] = make_uint4(0, 0, 0, 0);
-  }
-  if (length > 0 || biases > 0) {
+#pragma unroll
+    for (int i = 0; i < kPer / 4; ++i) reinterpret_cast<uint4*>(count_s)[threadIdx.x + i * kThreads] = make_uint4(0, 0, 0, 0);
     __syncthreads();
     each(past, length, [&](int t, int i) {
       const unsigned j = (unsigned)t - (unsigned)lo;
@@ -128,19 +125,14 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant_
       if (i < prompt) atomicOr(&count_s[j], kSeen);
       else atomicAdd(&count_s[j], 1u);
     });
-    each(p.bias_token + bias0, biases, [&](int t, int i) {
-      const unsigned j = (unsigned)t - (unsigned)lo;
-      if (j < (unsigned)size) atomicMax(&bias_s[j], (unsigned)i + 1);
-    });
     __syncthreads();
   }
-  auto adjust = [&](float y, unsigned count, unsigned bias, bool allowed) {
+  auto adjust = [&](float y, unsigned count, bool allowed) {
     if (count) {
       y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
       const unsigned made = count & ~kSeen;
       if (made) y = __fsub_rn(y, __fadd_rn(__fmul_rn(frequency, (float)made), presence));
     }
-    if (bias) y = __fadd_rn(y, p.bias_value[bias0 + bias - 1]);
     return allowed ? y : -INFINITY;
   };
   if (vec) {
@@ -148,15 +140,14 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant_
     for (int k = 0; k < kPer; k += 4) {
       const int j = at(k);
       if (j >= size) break;
-      uint4 c = make_uint4(0, 0, 0, 0), b = c;
+      uint4 c = make_uint4(0, 0, 0, 0);
       if (length > 0) c = *reinterpret_cast<const uint4*>(count_s + j);
-      if (biases > 0) b = *reinterpret_cast<const uint4*>(bias_s + j);
       const unsigned w = words ? (unsigned)words[(lo + j) >> 5] >> ((lo + j) & 31) : 0xfu;
-      if ((c.x | c.y | c.z | c.w | b.x | b.y | b.z | b.w) != 0 || (w & 0xfu) != 0xfu) {
-        v[k] = adjust(v[k], c.x, b.x, w & 1u);
-        v[k + 1] = adjust(v[k + 1], c.y, b.y, w & 2u);
-        v[k + 2] = adjust(v[k + 2], c.z, b.z, w & 4u);
-        v[k + 3] = adjust(v[k + 3], c.w, b.w, w & 8u);
+      if ((c.x | c.y | c.z | c.w) != 0 || (w & 0xfu) != 0xfu) {
+        v[k] = adjust(v[k], c.x, w & 1u);
+        v[k + 1] = adjust(v[k + 1], c.y, w & 2u);
+        v[k + 2] = adjust(v[k + 2], c.z, w & 4u);
+        v[k + 3] = adjust(v[k + 3], c.w, w & 8u);
       }
       if (j + 3 < size) {
         *reinterpret_cast<float4*>(out + j) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
@@ -171,11 +162,34 @@ __global__ void __launch_bounds__(kThreads) adjust_kernel(const __grid_constant_
     for (int k = 0; k < kPer; ++k) {
       const int j = at(k);
       if (j >= size) break;
-      const unsigned c = length > 0 ? count_s[j] : 0u, b = biases > 0 ? bias_s[j] : 0u;
+      const unsigned c = length > 0 ? count_s[j] : 0u;
       const unsigned w = words ? (unsigned)words[(lo + j) >> 5] >> ((lo + j) & 31) : 1u;
-      out[j] = c || b || !(w & 1u) ? adjust(v[k], c, b, w & 1u) : v[k];
+      out[j] = c || !(w & 1u) ? adjust(v[k], c, w & 1u) : v[k];
     }
   }
+  if (biases == 0) return;
+  // f(index of the token in the slice, entry) for the row's entries in this slice
+  auto entries = [&](auto f) {
+    each(p.bias_token + bias0, biases, [&](int t, int i) {
+      const unsigned j = (unsigned)t - (unsigned)lo;
+      if (j < (unsigned)size) f(j, (unsigned)i);
+    });
+  };
+  __syncthreads();
+  entries([&](unsigned j, unsigned) { count_s[j] = 0; });
+  __syncthreads();
+  entries([&](unsigned j, unsigned i) { atomicMax(&count_s[j], i + 1); });
+  __syncthreads();
+  entries([&](unsigned j, unsigned i) {
+    const bool allowed = !words || ((unsigned)words[(lo + j) >> 5] >> ((lo + j) & 31) & 1u);
+    if (count_s[j] == i + 1 && allowed) out[j] = __fadd_rn(out[j], p.bias_value[bias0 + i]);
+  });
+}
+
+template <int PER>
+cudaError_t launch(Args a, int64_t rows, int64_t slices, cudaStream_t st) {
+  a.slices = (int)slices;
+  return launch_ex(adjust_kernel<PER>, dim3((unsigned)(rows * slices)), dim3(kThreads), 0, st, a);
 }
 
 }  // namespace logits
@@ -187,8 +201,9 @@ extern "C" int hyq_logits_adjust(const float* logits, int64_t n, int64_t stride,
   const char* name = "logits_adjust";
   auto aligned = [](const void* p) { return reinterpret_cast<uintptr_t>(p) % 4 == 0; };
   if (!adjust) return hyq::api_fail(HYQ_E_INVALID, "%s: null pointer", name);
-  const int64_t slices = (n + kSlice - 1) / kSlice;
-  if (n <= 0 || n > INT32_MAX - kSlice || stride < n || out_stride < n || rows < 0 || rows > INT32_MAX / slices)
+  constexpr int kLong = 32, kShort = 8;  // logits of a thread
+  const int64_t slices = (n + kThreads * kLong - 1) / (kThreads * kLong), shorter = (n + kThreads * kShort - 1) / (kThreads * kShort);
+  if (n <= 0 || n > INT32_MAX - kThreads * kLong || stride < n || out_stride < n || rows < 0 || rows > INT32_MAX / shorter)
     return hyq::api_fail(HYQ_E_SHAPE, "%s: shape of the logits", name);
   const hyq_adjust& p = *adjust;
   if (rows == 0) return HYQ_OK;
@@ -207,10 +222,11 @@ extern "C" int hyq_logits_adjust(const float* logits, int64_t n, int64_t stride,
                         (const void*)p.bias_start, (const void*)p.bias_token, (const void*)p.bias_value, (const void*)p.mask,
                         (const void*)p.mask_row})
     if (!aligned(q)) return hyq::api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
-  Args a{logits, out, stride, out_stride, (int)n, (int)slices, p, nullptr};
+  Args a{logits, out, stride, out_stride, (int)n, 0, p, nullptr};
   const int rc = hyq::api_status_word(&a.status);
   if (rc) return rc;
-  const size_t smem = (p.bias_start ? 2 : 1) * kSlice * sizeof(unsigned);
-  const cudaError_t e = hyq::launch_ex(adjust_kernel, dim3((unsigned)(rows * slices)), dim3(kThreads), smem, (cudaStream_t)stream, a);
+  // TUNE
+  const cudaStream_t st = (cudaStream_t)stream;
+  const cudaError_t e = rows * slices >= 2 * 148 ? launch<kLong>(a, rows, slices, st) : launch<kShort>(a, rows, shorter, st);
   return e == cudaSuccess ? HYQ_OK : hyq::api_fail(HYQ_E_CUDA, "%s: %s", name, cudaGetErrorString(e));
 }

@@ -135,12 +135,12 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
         for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       }
       if (is_8bit(KV)) __syncwarp();  // the codes of the heads before are out
-      const float scale = is_8bit(KV) ? row_scale<KV>(top) : 1.f;
+      const RowCode code = is_8bit(KV) ? row_code<KV>(top) : RowCode{};
       if constexpr (is_8bit(KV)) {
         uint8_t* mine = codes_s[threadIdx.x & ~15];
         if (!is_q && u < units) {
 #pragma unroll
-          for (int i = 0; i < EL; ++i) mine[l + 16 * i] = encode<KV>(x[b][i], scale);
+          for (int i = 0; i < EL; ++i) mine[l + 16 * i] = encode<KV>(x[b][i], code.inverse);
         }
         __syncwarp();
       }
@@ -163,7 +163,7 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
 #pragma unroll
             for (int i = 0; i < EL; ++i) y[i] = from[i];
           }
-          if (l == 0) (rotated ? a.c.k_scale : a.c.v_scale)[scales + kh * a.c.scale_head_stride] = scale;
+          if (l == 0) (rotated ? a.c.k_scale : a.c.v_scale)[scales + kh * a.c.scale_head_stride] = code.scale;
         } else {
 #pragma unroll
           for (int i = 0; i < EL; ++i) store_kv<KV>(base, to + 16 * i, x[b][i]);
@@ -199,9 +199,9 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   auto quantise = [&](const float* x, void* base, float* scale_base, int kh) {
     uint32_t top = 0;
     for (int i = lane; i < dim; i += 32) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
-    const float scale = row_scale<KV>(__reduce_max_sync(0xffffffffu, top));
-    for (int i = lane; i < dim; i += 32) static_cast<uint8_t*>(base)[row + kh * a.c.head_stride + i] = encode<KV>(x[i], scale);
-    if (lane == 0) scale_base[scale_at(a.c, page, kh, pos % a.c.page_size)] = scale;
+    const RowCode code = row_code<KV>(__reduce_max_sync(0xffffffffu, top));
+    for (int i = lane; i < dim; i += 32) static_cast<uint8_t*>(base)[row + kh * a.c.head_stride + i] = encode<KV>(x[i], code.inverse);
+    if (lane == 0) scale_base[scale_at(a.c, page, kh, pos % a.c.page_size)] = code.scale;
   };
   for (int u = warp; u < a.heads + 2 * a.c.kv_heads; u += 8) {
     if (u >= a.heads + a.c.kv_heads) {  // a value head: copied as it is
@@ -398,60 +398,86 @@ struct GatherArgs {
   void* k;
   void* v;
   int64_t k_stride, v_stride;  // elements
-  bool vec;                    // four values of a row at a time are aligned, in and out
+  bool vec;                    // 16 bytes of a row at a time are aligned, in and out
 };
 
-// One CTA per row of the output, a warp per (kv head, K or V), four values a lane
-// (or one, where they are not aligned).  Bound by memory.
+// A warp per row of the output, 16 bytes of the cache a lane (or one value, where
+// they are not aligned), four loads in flight.  Bound by memory.
+constexpr int kGatherThreads = 64;
+
 template <Kv KV, typename T>
-__global__ void __launch_bounds__(256) gather_kernel(const __grid_constant__ GatherArgs a) {
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(const __grid_constant__ GatherArgs a) {
   grid_dependency_wait();
   allow_dependents_launch();
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, dim = a.c.dim;
+  const int t = blockIdx.x * (kGatherThreads / 32) + (threadIdx.x >> 5), lane = threadIdx.x & 31, dim = a.c.dim;
+  if (t >= a.c.tokens) return;
   const int s = seq_of_row(a.c, t);
   if (s < 0) return;
   const Seq sq = load_seq(a.c, s);
   if (t - sq.row0 >= sq.n) return;
   const int pos = sq.pos + (t - sq.row0), in_page = pos % a.c.page_size;
   const int page = checked_page(a.c, sq.pages[pos / a.c.page_size]);
-  for (int u = warp; u < 2 * a.c.kv_heads; u += 8) {
-    const bool is_k = u < a.c.kv_heads;
-    const int kh = is_k ? u : u - a.c.kv_heads;
-    const void* base = is_k ? a.c.k : a.c.v;
-    T* to = static_cast<T*>(is_k ? a.k : a.v) + t * (is_k ? a.k_stride : a.v_stride) + (int64_t)kh * dim;
-    const int64_t at = (int64_t)max(page, 0) * a.c.page_stride + (int64_t)kh * a.c.head_stride + (int64_t)in_page * a.c.row_stride;
-    float unit = 1.f;
-    if constexpr (is_8bit(KV)) unit = page < 0 ? 0.f : (is_k ? a.c.k_scale : a.c.v_scale)[scale_at(a.c, page, kh, in_page)];
-    auto value = [&](float x) { return page < 0 ? 0.f : x * unit; };
-    if (a.vec) {
-      for (int d = 4 * lane; d < dim; d += 128) {
-        float x[4];
-        if constexpr (KV == kF32) {
-          const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(base) + at + d);
-          x[0] = f.x, x[1] = f.y, x[2] = f.z, x[3] = f.w;
-        } else if constexpr (KV == kF16) {
-          const uint2 h = *reinterpret_cast<const uint2*>(static_cast<const __half*>(base) + at + d);
-          const float2 f0 = __half22float2(*reinterpret_cast<const __half2*>(&h.x)), f1 = __half22float2(*reinterpret_cast<const __half2*>(&h.y));
-          x[0] = f0.x, x[1] = f0.y, x[2] = f1.x, x[3] = f1.y;
-        } else {
-          const uint32_t w = *reinterpret_cast<const uint32_t*>(static_cast<const uint8_t*>(base) + at + d);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) x[i] = code_value<KV>((uint8_t)(w >> (8 * i)));
-        }
-        if constexpr (sizeof(T) == 4)
-          *reinterpret_cast<float4*>(to + d) = make_float4(value(x[0]), value(x[1]), value(x[2]), value(x[3]));
-        else
-          *reinterpret_cast<uint2*>(to + d) = make_uint2(pack_f16(value(x[0]), value(x[1])), pack_f16(value(x[2]), value(x[3])));
-      }
-    } else {
-      for (int d = lane; d < dim; d += 32) to[d] = (T)value(load_kv<KV>(base, at + d));
+  const int64_t row = (int64_t)max(page, 0) * a.c.page_stride + (int64_t)in_page * a.c.row_stride;
+  // unit u of `per` values: head u / units of K, then of V
+  auto each = [&](int per, auto f) {
+    const int units = dim / per, all = 2 * a.c.kv_heads * units;
+#pragma unroll 4
+    for (int u = lane; u < all; u += 32) {
+      const int head = u / units, d = (u - head * units) * per;
+      const bool is_k = head < a.c.kv_heads;
+      const int kh = is_k ? head : head - a.c.kv_heads;
+      float unit = 1.f;
+      if constexpr (is_8bit(KV)) unit = page < 0 ? 0.f : (is_k ? a.c.k_scale : a.c.v_scale)[scale_at(a.c, page, kh, in_page)];
+      T* to = static_cast<T*>(is_k ? a.k : a.v) + t * (is_k ? a.k_stride : a.v_stride) + (int64_t)kh * dim + d;
+      f(is_k ? a.c.k : a.c.v, row + (int64_t)kh * a.c.head_stride + d, unit, to);
     }
+  };
+  if (a.vec) {
+    constexpr int PER = 16 / value_bytes(KV);
+    each(PER, [&](const void* base, int64_t at, float unit, T* to) {
+      const uint4 w = *reinterpret_cast<const uint4*>(static_cast<const char*>(base) + at * value_bytes(KV));
+      const uint32_t in[4] = {w.x, w.y, w.z, w.w};
+      float x[PER];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (KV == kF32) {
+          x[i] = __uint_as_float(in[i]);
+        } else if constexpr (KV == kF16) {
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&in[i]));
+          x[2 * i] = f.x, x[2 * i + 1] = f.y;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k) x[4 * i + k] = code_value<KV>((uint8_t)(in[i] >> (8 * k))) * unit;
+        }
+      }
+      if (page < 0) {
+#pragma unroll
+        for (int i = 0; i < PER; ++i) x[i] = 0.f;
+      }
+      if constexpr (sizeof(T) == 4) {
+#pragma unroll
+        for (int i = 0; i < PER; i += 4) *reinterpret_cast<float4*>(to + i) = make_float4(x[i], x[i + 1], x[i + 2], x[i + 3]);
+      } else if constexpr (PER == 4) {
+        *reinterpret_cast<uint2*>(to) = make_uint2(pack_f16(x[0], x[1]), pack_f16(x[2], x[3]));
+      } else {
+#pragma unroll
+        for (int i = 0; i < PER; i += 8)
+          *reinterpret_cast<uint4*>(to + i) = make_uint4(pack_f16(x[i], x[i + 1]), pack_f16(x[i + 2], x[i + 3]),
+                                                         pack_f16(x[i + 4], x[i + 5]), pack_f16(x[i + 6], x[i + 7]));
+      }
+    });
+  } else {
+    each(1, [&](const void* base, int64_t at, float unit, T* to) {
+      *to = (T)(page < 0 ? 0.f : load_kv<KV>(base, at) * unit);
+    });
   }
 }
 
 template <Kv KV>
 cudaError_t launch_gather(const GatherArgs& a, bool f16, cudaStream_t st) {
-  return launch_ex(f16 ? gather_kernel<KV, __half> : gather_kernel<KV, float>, dim3((unsigned)a.c.tokens), dim3(256), 0, st, a);
+  constexpr int per = kGatherThreads / 32;
+  return launch_ex(f16 ? gather_kernel<KV, __half> : gather_kernel<KV, float>, dim3((unsigned)((a.c.tokens + per - 1) / per)),
+                   dim3(kGatherThreads), 0, st, a);
 }
 
 template <Kv KV>
@@ -736,9 +762,10 @@ int hyq_paged_gather(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, int 
   a.v = v;
   a.k_stride = k_stride;
   a.v_stride = v_stride;
-  const size_t in = 4 * value_bytes(type);
-  a.vec = ((a.c.dim | a.c.page_stride | a.c.head_stride | a.c.row_stride | k_stride | v_stride) & 3) == 0 && aligned(a.c.k, in) &&
-          aligned(a.c.v, in) && aligned(k, 4 * esize) && aligned(v, 4 * esize);
+  const int per = 16 / value_bytes(type), align = f16 && per == 4 ? 8 : 16;  // values of 16 bytes; alignment of what they make
+  a.vec = (a.c.dim | a.c.page_stride | a.c.head_stride | a.c.row_stride) % per == 0 && aligned(a.c.k, 16) && aligned(a.c.v, 16) &&
+          a.c.dim * esize % align == 0 && k_stride * esize % align == 0 && v_stride * esize % align == 0 && aligned(k, align) &&
+          aligned(v, align);
   const cudaStream_t st = (cudaStream_t)stream;
   switch (type) {
     case kF32: return done(launch_gather<kF32>(a, f16, st), name);

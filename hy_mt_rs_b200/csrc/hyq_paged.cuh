@@ -123,17 +123,24 @@ __device__ __forceinline__ float code_value(uint8_t c) {
 __device__ __forceinline__ int64_t scale_at(const Cache& c, int page, int kvh, int row) {
   return (int64_t)page * c.scale_page_stride + (int64_t)kvh * c.scale_head_stride + (int64_t)row * c.scale_row_stride;
 }
-// The scale of a row whose largest magnitude has these bits: NaN for a row with
-// an infinity or NaN, which then reads back as NaN throughout.
+// A row's scale, and what takes its values to codes, from the bits of its largest
+// magnitude: NaN and 0 for a row with an infinity or NaN, which then reads back as
+// NaN throughout; 0 and 0 for one of zeros, or below 2^-90.
+struct RowCode {
+  float scale, inverse;
+};
 template <Kv KV>
-__device__ __forceinline__ float row_scale(uint32_t top) {
-  return top >= 0x7f800000u ? __uint_as_float(0x7fc00000u) : __fdiv_rn(__uint_as_float(top), KV == kI8 ? 127.f : 448.f);
+__device__ __forceinline__ RowCode row_code(uint32_t top) {
+  constexpr float largest = KV == kI8 ? 127.f : 448.f;
+  if (top >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f};
+  if (top < (127u - 90u) << 23) return {0.f, 0.f};
+  const float x = __uint_as_float(top);
+  return {__fdiv_rn(x, largest), __fdiv_rn(largest, x)};
 }
-// Code of x in a row of this scale: the nearest, ties to even.
+// Code of x in a row with this inverse: the nearest to their product, ties to even.
 template <Kv KV>
-__device__ __forceinline__ uint8_t encode(float x, float scale) {
-  if (!(scale > 0.f)) return 0;  // zeros, or a row that reads back as NaN
-  const float y = __fdiv_rn(x, scale);
+__device__ __forceinline__ uint8_t encode(float x, float inverse) {
+  const float y = inverse == 0.f ? 0.f : __fmul_rn(x, inverse);
   if constexpr (KV == kI8) return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(y)));
   return (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
 }

@@ -514,9 +514,10 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
  * k_scale or v_scale; a value is code * scale.  (For the other types the scales
  * are not read.)
  * Appending sets scale = the row's largest magnitude / 127 (int8) or / 448
- * (e4m3), in f32, and each code to the one nearest to value / scale, ties to
- * even; a row of zeros has scale 0.  A row with an infinity or NaN has codes 0
- * and a NaN scale: it reads back as NaN throughout.  Attention makes NaN of rows
+ * (e4m3), and each code to the one nearest to value * (127 or 448 / that
+ * magnitude), ties to even, each step in f32; a row of magnitudes below 2^-90 has
+ * scale and codes 0.  A row with an infinity or NaN has codes 0 and a NaN scale:
+ * it reads back as NaN throughout.  Attention makes NaN of rows
  * that see such a position, and of no others.  The codes 0x7f and 0xff of e4m3,
  * which appending does not write, count as +-480. */
 #define HYQ_KV_I8 2

@@ -33,12 +33,14 @@ def _quantise(x, kind):
     import torch
     dtype, largest = _types()[kind]
     x = x.cpu()
-    scale = x.abs().amax(-1) / largest
-    y = x / torch.where(scale > 0, scale, 1.0)[..., None]
+    top = x.abs().amax(-1)
+    top = torch.where(top < 2.0 ** -90, 0.0, top)
+    scale = top / largest
+    y = x * torch.where(top > 0, largest / top, 0.0)[..., None]
     codes = y.round().clamp(-127, 127).to(dtype) if kind == "i8" else y.to(dtype)
     bad = ~torch.isfinite(x).all(-1)
     scale[bad] = math.nan
-    codes.view(torch.uint8)[bad] = 0
+    codes.view(torch.uint8)[bad | (top == 0)] = 0    # (not -0)
     return codes, scale
 
 
