@@ -735,13 +735,15 @@ int hyq_paged_attention_shared(const hyq_paged_kv8* kv, const hyq_paged_batch* b
     return api_fail(HYQ_E_ALIGN, "%s: a pointer is not aligned to its element size", name);
   const Kv type = (Kv)kv->kv.dtype;
   const cudaStream_t st = (cudaStream_t)stream;
-  if (groups == 0 || max_shared == 0 || !shared_supported(a, type))
-    return attend(a, type, batch->max_new, batch->max_len, name, st);
   a.groups.start = group_start;
   a.groups.shared = shared;
   a.groups.n = (int)groups;
   a.groups.max_new = batch->max_new;
-  return done(launch_shared(a, type, st), name);
+  if (groups == 0 || max_shared == 0 || !shared_supported(a, type)) {
+    a.groups = {};
+    return attend(a, type, batch->max_new, batch->max_len, name, st);
+  }
+  return done(launch_shared(a, type, max_shared, st), name);
 }
 
 int hyq_paged_gather(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, int f16, void* k, int64_t k_stride, void* v,

@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
       __syncwarp();
       stage_queries<DIM, KV, kRows>(q_s, factor_s, ring + (G::stages - 1) * G::block, s.n * group, warp, kWarps);
       __syncthreads();
-      rows.load(q_s, factor_s, s, group, 0);
+      rows.load(q_s, factor_s, s, group, 0, s.n * group);
       const Feed<DIM, KV, NB> feed{a, s, cur.kvh, s.pos + s.n, shift};
       int stage = 0;
       for (int j = cur.j0; j < cur.j1; ++j) {
@@ -398,7 +398,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV>::ctas) chunk_kernel(con
     __syncwarp();
     stage_queries<DIM, KV>(q_s, factor_s[warp], raw_s, n, 0, 1);
     __syncwarp();
-    rows.load(q_s, factor_s[warp], s, group, r0);
+    rows.load(q_s, factor_s[warp], s, group, r0, n);
   }
   __syncthreads();
   constexpr int stage_bytes = kWarps * G::block;

@@ -3,6 +3,7 @@
 // all of it); each sequence's own positions by the few-token kernel beside it.
 // Both leave normalised outputs with their references and sums of weights, which
 // merge_kernel puts together.
+#include <algorithm>
 #include <cmath>
 
 #include "../../include/hyq.h"
@@ -56,17 +57,20 @@ size_t rounded(size_t n) { return (n + 255) / 256 * 256; }
 
 }  // namespace
 
+// The few-token kernel's counters, which stay zero between calls, come first in a
+// workspace; what follows them is one way's or the other's.
 size_t shared_workspace_bytes(int heads, int dim, int64_t tokens) {
   const size_t rows = (size_t)tokens * heads;
-  return rounded(mma_workspace_bytes(dim) + tc_workspace_bytes(dim)) + rounded(rows * dim * sizeof(float)) + 2 * rounded(rows * sizeof(float2)) +
-         rounded(kMaxSeqs * sizeof(int32_t)) + rounded(tokens * sizeof(int32_t));
+  const size_t chunks = rounded(rows * dim * sizeof(float)) + 2 * rounded(rows * sizeof(float2)) + rounded(kMaxSeqs * sizeof(int32_t)) +
+                        rounded(tokens * sizeof(int32_t));
+  return rounded(mma_workspace_bytes(dim) + tc_workspace_bytes(dim)) + std::max(chunks, line_workspace_bytes(heads, dim, tokens));
 }
 
-bool shared_supported(const AttendArgs& a, Kv kv) {
-  return mma_supported(a, kv) && chunks_tc_supported(a, kv);
-}
+bool shared_supported(const AttendArgs& a, Kv kv) { return line_supported(a, kv) || (mma_supported(a, kv) && chunks_tc_supported(a, kv)); }
 
-cudaError_t launch_shared(const AttendArgs& given, Kv kv, cudaStream_t st) {
+cudaError_t launch_shared(const AttendArgs& given, Kv kv, int64_t max_shared, cudaStream_t st) {
+  if (line_supported(given, kv) && (!chunks_tc_supported(given, kv) || true))
+    return launch_line(given, kv, static_cast<char*>(given.ws) + rounded(mma_workspace_bytes(given.c.dim) + tc_workspace_bytes(given.c.dim)), st);
   AttendArgs a = given;  // the prefixes' pass
   const size_t rows = (size_t)a.c.tokens * a.heads;
   char* p = static_cast<char*>(a.ws) + rounded(mma_workspace_bytes(a.c.dim) + tc_workspace_bytes(a.c.dim));
