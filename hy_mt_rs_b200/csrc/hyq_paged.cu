@@ -743,7 +743,7 @@ int hyq_paged_attention_shared(const hyq_paged_kv8* kv, const hyq_paged_batch* b
     a.groups = {};
     return attend(a, type, batch->max_new, batch->max_len, name, st);
   }
-  return done(launch_shared(a, type, max_shared, st), name);
+  return done(launch_shared(a, type, st), name);
 }
 
 int hyq_paged_gather(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, int f16, void* k, int64_t k_stride, void* v,

@@ -185,8 +185,8 @@ struct Groups {
   const int32_t* start;   // [n + 1] first sequence of each
   const int32_t* shared;  // [n] positions in common
   int n;
-  int32_t* first;         // [seqs], [tokens] prefix that a sequence, a token takes from its group
-  int32_t* token_prefix;
+  int32_t* first;         // [seqs] prefix that a sequence takes from its group (0: none)
+  int2* token;            // [tokens] first segment of a token's group (-1: none), its place among the group's
   float* out;
   int64_t out_stride;
   float2* ml;

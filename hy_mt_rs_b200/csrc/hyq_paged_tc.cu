@@ -428,7 +428,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   if (e == cudaSuccess) e = launch_plan<kCtaRows>(a, p.plan, st);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
   if (e == cudaSuccess) e = launch_beside(a, kF16, st);
-  if (e == cudaSuccess) e = launch_next(join_kernel<DIM, kCtaRows, kF16>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p);
+  if (e == cudaSuccess) e = launch_last<DIM, kCtaRows, kF16>(p, st);
   return e;
 }
 

@@ -17,6 +17,7 @@ constexpr int kMaxCtas = 148;
 constexpr int kMaxParts = 2 * kMaxCtas;  // partial results in the workspace: a CTA's first and last piece
 constexpr int kMaxSegs = 65536;          // segments of a call
 constexpr int kMinTiles = 2;             // cost of a CTA's range, at least
+constexpr int kMinPrefixTiles = 4;       // of prefixes: the few-token kernel beside has work for the other SMs
 constexpr int kSegTiles = 1;             // cost of a segment, in tiles
 // Floats of a partial result of a segment of ROWS rows: outputs, then
 // (maximum, sum) of each row, then whether a value may have been taken out.
@@ -116,7 +117,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
   const Groups& g = a.groups;
   const int units = PREFIX ? g.n : a.c.seqs;
   if constexpr (PREFIX) {
-    for (int i = threadIdx.x; i < a.c.tokens; i += 1024) g.token_prefix[i] = 0;
+    for (int i = threadIdx.x; i < a.c.tokens; i += 1024) g.token[i] = make_int2(-1, 0);
     bool bad = false;
     for (int i = threadIdx.x; i < units; i += 1024) {
       const int first = g.start[i], last = g.start[i + 1], p = g.shared[i];
@@ -152,7 +153,6 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
           const int p = in ? off_s[lo] : 0;
           g.first[i] = p;
           if (s.n * group > kFewRows) atomicOr(a.c.status, DEV_BAD_ARGS);  // max_new was too small: nobody takes it
-          for (int t = 0; p > 0 && t < s.n; ++t) g.token_prefix[s.row0 + t] = p;
         }
       }
       __syncthreads();
@@ -183,6 +183,19 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
     segs += total;
   }
   __syncthreads();
+  if constexpr (PREFIX) {
+    for (int i = threadIdx.x; i < a.c.seqs; i += 1024) {
+      if (g.first[i] == 0) continue;
+      int lo = 0, hi = units - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (g.start[mid] <= i) lo = mid;
+        else hi = mid - 1;
+      }
+      const int row0 = a.c.row_start[g.start[lo]];
+      for (int t = a.c.row_start[i]; t < a.c.row_start[i + 1]; ++t) g.token[t] = make_int2(off_s[lo], t - row0);
+    }
+  }
   segs = min(segs, plan.most);  // (more: rows of several sequences, row_start not ascending)
   int tiles = 0;
   for (int t0 = 0; t0 < segs; t0 += 1024) {
@@ -209,7 +222,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
   __syncthreads();
   if (threadIdx.x <= kMaxCtas) {
     const int64_t per = tiles + (int64_t)kSegTiles * segs, work = per * a.c.kv_heads;
-    const int64_t ctas = min((int64_t)kMaxCtas, max(work / kMinTiles, (int64_t)1));
+    const int64_t ctas = min((int64_t)kMaxCtas, max(work / (PREFIX ? kMinPrefixTiles : kMinTiles), (int64_t)1));
     const int64_t unit = work * min((int64_t)threadIdx.x, ctas) / ctas;
     const int kvh = per ? (int)(unit / per) : 0;
     const int64_t rest = unit - kvh * per;
@@ -767,6 +780,122 @@ __global__ void __launch_bounds__(256) join_kernel(const __grid_constant__ Param
     for (int k = 0; k < N; ++k)
       if (before.v[k] + own.v[k] != 0.f) to[k] = before.v[k] + own.v[k];
   }
+}
+
+// The outputs of groups' tokens: what the prefix's pieces and the sequence's own
+// positions (in groups.out, normalised) left, a warp per (token, head):
+// y = (w0 y0 + w1 y1) / (w0 + w1), w = l 2^(m - max).  An output that is not finite
+// stays so whatever its weight, which is above zero.
+template <int DIM, int ROWS, Kv KV>
+__global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ Params p) {
+  constexpr int N = DIM / 32, kAhead = 8;
+  grid_dependency_wait();
+  allow_dependents_launch();
+  const AttendArgs& a = p.a;
+  const int lane = threadIdx.x & 31, unit = blockIdx.x * 4 + (threadIdx.x >> 5), t = unit / a.heads, h = unit - t * a.heads;
+  if (t >= a.c.tokens) return;
+  const int2 token = a.groups.token[t];
+  if (token.x < 0) return;
+  const int group = a.heads / a.c.kv_heads, kvh = h / group, r = token.y * group + h - kvh * group, seg = token.x + r / ROWS;
+  const int64_t row = (int64_t)t * a.heads + h;
+  const Segment& segment = p.plan.seg[seg];
+  const int total = p.plan.count[1];
+  const int64_t seg0 = (int64_t)kvh * total + segment.first, seg1 = (int64_t)kvh * total + segment.end;
+  float* out = a.groups.out + t * a.groups.out_stride + (int64_t)h * DIM + lane;
+  const float2 own = a.groups.ml[row];
+  float y[2][N];
+#pragma unroll
+  for (int k = 0; k < N; ++k) y[1][k] = out[32 * k];
+  // the CTAs of the segment's pieces: from the last that begins at its first tile or
+  // before
+  int c0 = -1, n = 0;
+#pragma unroll
+  for (int c = 0; c < kMaxCtas; c += 32) {
+    const int64_t begin = c + lane < kMaxCtas ? p.plan.start[c + lane].begin : INT64_MAX;
+    c0 += __popc(__ballot_sync(0xffffffffu, begin <= seg0));
+    n += __popc(__ballot_sync(0xffffffffu, begin > seg0 && begin < seg1));
+  }
+  float2 ml = make_float2(-INFINITY, 0.f);
+  if (n == 0) {  // inside one range: finished there
+    ml = a.ml[row];
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[0][k] = a.out[row * DIM + lane + 32 * k];
+  } else {
+    const float* part0 = p.parts + (size_t)(2 * c0 + (seg0 != p.plan.start[c0].begin)) * part_floats<ROWS>(DIM);
+    const float* part1 = p.parts + (size_t)(2 * c0) * part_floats<ROWS>(DIM);
+    auto part = [&](int i) { return i ? part1 + (size_t)(2 * i) * part_floats<ROWS>(DIM) : part0; };
+    const int in = r % ROWS;
+    ++n;
+    float top = -INFINITY, l = 0.f;
+    for (int i = lane; i < n; i += 32) top = fmaxf(top, reinterpret_cast<const float2*>(part(i) + (size_t)ROWS * DIM)[in].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+#pragma unroll
+    for (int k = 0; k < N; ++k) y[0][k] = 0.f;
+#pragma unroll 1
+    for (int i0 = 0; i0 < n; i0 += 32) {
+      float f = 0.f;  // the weight of piece i0 + lane
+      if (i0 + lane < n) {
+        const float2 v = reinterpret_cast<const float2*>(part(i0 + lane) + (size_t)ROWS * DIM)[in];
+        f = v.x == -INFINITY ? 0.f : ex2(v.x - top);
+        l += v.x == -INFINITY ? v.y : f * v.y;  // (without a score above -inf: 0, or NaN to pass on)
+      }
+      const int m = min(32, n - i0);
+#pragma unroll 1
+      for (int i1 = 0; i1 < m; i1 += kAhead) {
+        float x[kAhead][N];
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const float* from = part(i0 + min(i1 + i, m - 1)) + (size_t)in * DIM + lane;
+#pragma unroll
+          for (int k = 0; k < N; ++k) x[i][k] = from[32 * k];
+        }
+#pragma unroll
+        for (int i = 0; i < kAhead; ++i) {
+          const float w = __shfl_sync(0xffffffffu, f, (i1 + i) & 31);
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (i1 + i < m) y[0][k] = fmaf(w, x[i][k], y[0][k]);
+        }
+      }
+    }
+    ml = make_float2(top, warp_sum(l));
+    const float inv = 1.0f / ml.y;
+    bool odd = false;
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      y[0][k] *= inv;
+      odd = odd || !isfinite(y[0][k]);
+    }
+    if (!is_8bit(KV) && odd && isfinite(ml.y)) {
+      const Seq s{segment.row0, segment.n, segment.pos, a.c.table + (int64_t)segment.slot * a.c.width};
+#pragma unroll 1
+      for (int k = 0; k < N; ++k) {
+        const float x = non_finite<KV == kF16, 1>(a.c, s, kvh, -1, s.pos, lane + 32 * k).v[0];
+        if (x != 0.f) y[0][k] = x;
+      }
+    }
+  }
+  const float top = fmaxf(ml.x, own.x);
+  // (a part without a score above -inf has no weight, or NaN to pass on)
+  const bool none[2] = {ml.x == -INFINITY && ml.y == 0.f, own.x == -INFINITY && own.y == 0.f};
+  const float w0 = ml.x == -INFINITY ? ml.y : ml.y * ex2(ml.x - top), w1 = own.x == -INFINITY ? own.y : own.y * ex2(own.x - top);
+  const float inv = 1.0f / (w0 + w1);
+#pragma unroll
+  for (int k = 0; k < N; ++k) {
+    const float f0 = none[0] ? 0.f : isfinite(y[0][k]) ? y[0][k] * (w0 * inv) : y[0][k];
+    const float f1 = none[1] ? 0.f : isfinite(y[1][k]) ? y[1][k] * (w1 * inv) : y[1][k];
+    out[32 * k] = none[0] && none[1] ? inv * 0.f : f0 + f1;
+  }
+}
+
+// A call's last kernel: the join of pieces, or the merge of prefixes and sequences.
+template <int DIM, int ROWS, Kv KV>
+cudaError_t launch_last(const Params& p, cudaStream_t st) {
+  if (!p.a.groups.n)
+    return launch_next(join_kernel<DIM, ROWS, KV>, dim3(kMaxCtas, ROWS / kJoinRows), dim3(256), 0, st, p);
+  const int64_t units = (int64_t)p.a.c.tokens * p.a.heads;
+  return launch_next(merge_kernel<DIM, ROWS, KV>, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, st, p);
 }
 
 }  // namespace

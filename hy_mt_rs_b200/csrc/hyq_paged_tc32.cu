@@ -453,8 +453,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   if (e == cudaSuccess) e = launch_plan<kRows>(a, p.plan, st);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
   if (e == cudaSuccess) e = launch_beside(a, kF32, st);
-  if (e == cudaSuccess)
-    e = launch_next(join_kernel<DIM, kRows, kF32>, dim3(kMaxCtas, kRows / kJoinRows), dim3(256), 0, st, p);
+  if (e == cudaSuccess) e = launch_last<DIM, kRows, kF32>(p, st);
   return e;
 }
 

@@ -487,7 +487,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   if (e == cudaSuccess) e = launch_plan<kCtaRows>(a, p.plan, st);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
   if (e == cudaSuccess) e = launch_beside(a, KV, st);
-  if (e == cudaSuccess) e = launch_next(join_kernel<DIM, kCtaRows, KV>, dim3(kMaxCtas, kCtaRows / kJoinRows), dim3(256), 0, st, p);
+  if (e == cudaSuccess) e = launch_last<DIM, kCtaRows, KV>(p, st);
   return e;
 }
 
