@@ -476,14 +476,9 @@ __device__ __forceinline__ float stage_rows(const AttendArgs& a, const Piece& x,
 // scores is then needed for a row's first tile alone.  l is the sum of the
 // weights so far, `down` what the outputs so far are to be multiplied by.
 // scale(v, c) is applied to the scores of columns c .. c + 31 before `factor`.
-// With VALUES the columns have factors up to 1 of their own, values[c], in a unit of
-// the tile, 2^lift: weights are 2^(s + lift - m), what is stored of them is times
-// those, and l is the sum of 2^(s - m).  (The reference then follows what the
-// stored products can be at most, over all tiles, whatever their units.)
-template <bool VALUES = false, typename Scale>
+template <typename Scale>
 __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool masked, int unseen_from, float factor, float& m,
-                                                  float& l, float& down, Scale scale, const float* values = nullptr,
-                                                  float lift = 0.f) {
+                                                  float& l, float& down, Scale scale) {
   auto mask = [&](float (&v)[32], int c) {
 #pragma unroll
     for (int i = 0; i < 32; ++i)
@@ -509,16 +504,16 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
       if (masked) mask(v, c);
       top = fmaxf(top, largest(v));
     }
-    m = reference(VALUES ? fmaf(top, factor, lift) : top * factor);
+    m = reference(top * factor);
   }
-  float back = (m == -INFINITY ? 0.f : -m) + (VALUES ? lift : 0.f), sum = 0.f, sum2 = 0.f;
+  float back = m == -INFINITY ? 0.f : -m, sum = 0.f, sum2 = 0.f;
   down = 1.f;
   // 32 columns: scores to weights, hi and lo over them.  (Loops of 32
   // columns, not unrolled, and two copies of them: the comparisons of a
   // masked tile take as long as the rest, and the unrolled code ran out
   // of the instruction cache.)
   auto weigh = [&](float (&v)[32], int c) {
-    const float top = VALUES ? fmaf(largest(v), factor, lift) : largest(v) * factor, over = top - m - kBias;
+    const float top = largest(v) * factor, over = top - m - kBias;
     if (__any_sync(0xffffffffu, over > kSlack)) {
       // raise the reference, by whole powers of two where what there is so far
       // still counts (2^-64 of it does not: nor does a sum from before the first
@@ -532,7 +527,7 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
         m = fmaxf(m + ceilf(over), reference(top));
         f = ex2(before - m);
       }
-      back = (m == -INFINITY ? 0.f : -m) + (VALUES ? lift : 0.f);
+      back = m == -INFINITY ? 0.f : -m;
       down *= f;
       sum *= f;
       sum2 *= f;
@@ -560,14 +555,9 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
     for (int g = 0; g < 32; g += 16)
 #pragma unroll
       for (int i = 0; i < 16; i += 2) {
-        float y0 = ex2(fmaf(v[g + i], factor, back)), y1 = ex2(fmaf(v[g + i + 1], factor, back));
+        const float y0 = ex2(fmaf(v[g + i], factor, back)), y1 = ex2(fmaf(v[g + i + 1], factor, back));
         sum += y0;
         sum2 += y1;
-        if constexpr (VALUES) {
-          const float2 f = *reinterpret_cast<const float2*>(values + c + g + i);
-          y0 *= f.x;
-          y1 *= f.y;
-        }
         const float h0 = high_part(y0), h1 = high_part(y1);
         w[g + (i >> 1)] = pack_f16(h0, h1);
         w[g + 8 + (i >> 1)] = pack_f16(y0 - h0, y1 - h1);
@@ -594,7 +584,7 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
       weigh(v, c);
     }
   }
-  l = fmaf(l, down, VALUES ? (sum + sum2) * __uint_as_float((uint32_t)(127 - (int)lift) << 23) : sum + sum2);
+  l = fmaf(l, down, sum + sum2);
 }
 
 // The results of a warp's 32 rows of a piece, row r this thread's: outputs, or

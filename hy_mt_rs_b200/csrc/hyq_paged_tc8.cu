@@ -6,7 +6,7 @@
 // products are the same four, S = Qh K' + Ql K' and X = Ph V + Pl V.  K's scales
 // multiply the columns of S.  V's go into the weights, as f16 pairs in the unit of
 // the tile's largest scale; the running reference of a row counts that unit in
-// (scores_to_weights()), so that tiles of any units may follow each other.
+// (code_scores_to_weights()), so that tiles of any units may follow each other.
 //
 //   warp 1       tcgen05.mma, as in the f16 kernel;
 //   warps 4-7    codes and scales from global memory (a tile's while the tensor
@@ -45,6 +45,144 @@ struct Smem {
   static constexpr int misc = bars + 8 * n_bars;
   static constexpr int total = misc + 32;
 };
+
+// Two f32 at a time.
+__device__ __forceinline__ uint64_t pair(float a, float b) { return (uint64_t)__float_as_uint(a) | (uint64_t)__float_as_uint(b) << 32; }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t sub2(uint64_t a, uint64_t b) {
+  uint64_t d;
+  asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+  return d;
+}
+__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
+  uint64_t d;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
+  return d;
+}
+__device__ __forceinline__ float low(uint64_t a) { return __uint_as_float((uint32_t)a); }
+__device__ __forceinline__ float high(uint64_t a) { return __uint_as_float((uint32_t)(a >> 32)); }
+
+// scores_to_weights() over codes: the columns' scores are times ks[c], and the
+// weights times vs[c], up to 1, V's scales in the tile's unit 2^lift.  A weight is
+// 2^(s + lift - m) before that, and l the sum of 2^(s - m): the reference follows what
+// the stored products can be at most, over all tiles, whatever their units.
+__device__ __forceinline__ void code_scores_to_weights(uint32_t st, bool first, bool masked, int unseen_from, float factor, float& m,
+                                                       float& l, float& down, const float* ks, const float* vs, float lift) {
+  // the scores of columns c .. c + 31, and the largest
+  auto scores = [&](uint64_t (&u)[16], int c) {
+    float v[32];
+    tmem_ld(v, st + c);
+    const float4* k4 = reinterpret_cast<const float4*>(ks + c);
+    float4 k[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) k[i] = k4[i];
+    tmem_wait_ld();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      u[2 * i] = mul2(pair(v[4 * i], v[4 * i + 1]), pair(k[i & 3].x, k[i & 3].y));
+      u[2 * i + 1] = mul2(pair(v[4 * i + 2], v[4 * i + 3]), pair(k[i & 3].z, k[i & 3].w));
+      if (i < 4) k[i] = k4[i + 4];
+    }
+    if (masked) {
+#pragma unroll
+      for (int i = 0; i < 16; ++i)
+        u[i] = pair(c + 2 * i >= unseen_from ? -INFINITY : low(u[i]), c + 2 * i + 1 >= unseen_from ? -INFINITY : high(u[i]));
+    }
+    float a[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) a[i] = fmaxf(low(u[i]), high(u[i]));
+#pragma unroll
+    for (int i = 4; i < 16; ++i) a[i & 3] = fmaxf(fmaxf(a[i & 3], low(u[i])), high(u[i]));
+    return fmaxf(fmaxf(a[0], a[1]), fmaxf(a[2], a[3]));
+  };
+  if (first) {
+    float top = -INFINITY;
+#pragma unroll 1
+    for (int c = 0; c < kTile; c += 32) {
+      uint64_t u[16];
+      top = fmaxf(top, scores(u, c));
+    }
+    m = reference(fmaf(top, factor, lift));
+  }
+  const uint64_t factors = pair(factor, factor);
+  float back = (m == -INFINITY ? 0.f : -m) + lift;
+  uint64_t sum = 0, sum2 = 0;
+  down = 1.f;
+#pragma unroll 1
+  for (int c = 0; c < kTile; c += 32) {
+    uint64_t u[16];
+    const float top = fmaf(scores(u, c), factor, lift), over = top - m - kBias;
+    if (__any_sync(0xffffffffu, over > kSlack)) {
+      // raise the reference, by whole powers of two where what there is so far
+      // still counts; what this tile has so far follows
+      float f = 1.f;
+      if (over > 64.f) {
+        f = 0.f;
+        m = reference(top);
+      } else if (over > kSlack) {
+        const float before = m;
+        m = fmaxf(m + ceilf(over), reference(top));
+        f = ex2(before - m);
+      }
+      back = (m == -INFINITY ? 0.f : -m) + lift;
+      down *= f;
+      sum = mul2(sum, pair(f, f));
+      sum2 = mul2(sum2, pair(f, f));
+      tmem_wait_st();
+#pragma unroll 1
+      for (int b = 0; b < c; b += 16) {
+        float w[16];
+        uint32_t x[16];
+        tmem_ld(w, st + b);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const uint32_t hi = __float_as_uint(w[i]), lo = __float_as_uint(w[8 + i]);
+          const float2 a0 = __half22float2(*reinterpret_cast<const __half2*>(&hi));
+          const float2 a1 = __half22float2(*reinterpret_cast<const __half2*>(&lo));
+          const float y0 = (a0.x + a1.x) * f, y1 = (a0.y + a1.y) * f, h0 = high_part(y0), h1 = high_part(y1);
+          x[i] = pack_f16(h0, h1);
+          x[8 + i] = pack_f16(y0 - h0, y1 - h1);
+        }
+        tmem_st(st + b, x);
+      }
+    }
+    const uint64_t backs = pair(back, back);
+    const float4* v4 = reinterpret_cast<const float4*>(vs + c);
+#pragma unroll
+    for (int g = 0; g < 2; ++g) {
+      float4 f4[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) f4[i] = v4[4 * g + i];
+      uint32_t w[16];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint64_t e = fma2(u[8 * g + i], factors, backs);
+        const uint64_t y = pair(ex2(low(e)), ex2(high(e)));
+        if (i & 1) sum2 = add2(sum2, y);
+        else sum = add2(sum, y);
+        const float4 f = f4[i >> 1];
+        const uint64_t z = mul2(y, i & 1 ? pair(f.z, f.w) : pair(f.x, f.y));
+        const float h0 = high_part(low(z)), h1 = high_part(high(z));
+        const uint64_t rest = sub2(z, pair(h0, h1));
+        w[i] = pack_f16(h0, h1);
+        w[8 + i] = pack_f16(low(rest), high(rest));
+      }
+      tmem_st(st + c + 16 * g, w);
+    }
+  }
+  sum = add2(sum, sum2);
+  l = fmaf(l, down, (low(sum) + high(sum)) * __uint_as_float((uint32_t)(127 - (int)lift) << 23));
+}
 
 // (the base is aligned to 1024 bytes by its declaration, and checked)
 template <int DIM, Kv KV>
@@ -118,9 +256,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
     }
   };
 
-  // launch: 128 registers x 512 threads = (40 + 72 + 2 x 200) x 128
+  // launch: 128 registers x 512 threads = (48 + 64 + 2 x 200) x 128
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
     if (warp == 1) {
       // ------------------------------ products -------------------------------
       // f32 sums, f16 operands, M 128; N 128 positions, or DIM columns with V
@@ -224,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         if (!warp_wait(empty(i % kSlots), (i / kSlots) & 1, nullptr) && lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
     // ------------------------------- K and V --------------------------------
     constexpr int LPR = DIM / 16;         // lanes of a row, 16 codes each
     constexpr int RPI = 32 / LPR, IT = LPR;
@@ -234,73 +372,85 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
     const int tiles = uniform((int)(end - begin));
     int j = 0, issued = 0, lift = 0;
     bool ok = true;
-    uint4 r[IT];
-    // where row `row` of the tile begins, or -1
-    auto page_row = [&](int row, int& in_page) {
-      const int pos = (x.j0 + j) * kTile + row;
-      in_page = pos % a.c.page_size;
-      return pos < x.len ? checked_page(a.c, x.s.pages[pos / a.c.page_size]) : -1;
+    // A lane's position is pos_in of the tile; its warp puts the 32 rows of its lanes.
+    const int shift = p.box;
+    auto entry = [&](int j) {  // of that position in its sequence's table row, -1: none
+      const int pos = (x.j0 + j) * kTile + pos_in;
+      return pos < x.len ? x.s.pages[shift >= 0 ? pos >> shift : pos / a.c.page_size] : -1;
     };
-    int64_t here = -1;    // of row (lane / RPI) of the warp's (lane % RPI)th rows
+    int64_t here = -1;     // where the position's row begins, or -1
     float ks = 0.f, vs = 0.f;
-    bool held = false;    // this thread's position is one of the sequence's
+    bool held = false;     // it is one of the sequence's
+    int ahead = entry(0);  // the next tile's
     auto open = [&]() {
-      int in_page, page = page_row((lane / RPI) * 4 * RPI + lw * RPI + lane % RPI, in_page);
-      here = page < 0 ? -1
-                      : (int64_t)page * a.c.page_stride + (int64_t)x.kvh * a.c.head_stride + (int64_t)in_page * a.c.row_stride;
-      page = page_row(pos_in, in_page);
+      const int pos = (x.j0 + j) * kTile + pos_in, in_page = shift >= 0 ? pos & ((1 << shift) - 1) : pos % a.c.page_size;
+      const int page = pos < x.len ? checked_page(a.c, ahead) : -1;
       held = page >= 0;
+      here = held ? (int64_t)page * a.c.page_stride + (int64_t)x.kvh * a.c.head_stride + (int64_t)in_page * a.c.row_stride : -1;
       const int64_t at_scale = held ? scale_at(a.c, page, x.kvh, in_page) : 0;
       ks = held ? a.c.k_scale[at_scale] : 0.f;
       vs = held ? a.c.v_scale[at_scale] : 0.f;
     };
-    auto load = [&](const void* from) {
+    // A lane's 16 codes of the warp's rows become two 16-byte chunks of f16; the codes
+    // come to the place of one of them (`mine`; the other's beside, so that lanes meet
+    // distinct banks), where the same lane takes them from.
+    const int c0 = 2 * (lane % LPR);
+    auto line = [&](int slot, int row) { return base + L::ring + slot * L::tile + (c0 >> 3) * L::half + row * 128; };
+    auto mine = [&](int row) { return (((c0 & 7) | (DIM == 128 ? c0 >> 3 : 0)) ^ (row & 7)) << 4; };
+    auto row_of = [&](int i) { return 32 * lw + i * RPI + lane / LPR; };
+    // the next operand's codes asked for, into the ring's next slot
+    auto ask = [&](const void* from) {
+      const int slot = issued % kSlots;
+      ok = issued < kSlots || warp_wait(empty(slot), ((issued / kSlots) - 1) & 1, abort_flag);
+      if (!ok) return;
+      ++issued;
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
         const int64_t o = __shfl_sync(0xffffffffu, here, i * RPI + lane / LPR);
         const uint8_t* row = static_cast<const uint8_t*>(from) + max(o, (int64_t)0) + 16 * (lane % LPR);
-        r[i] = o >= 0 ? *reinterpret_cast<const uint4*>(row) : make_uint4(0, 0, 0, 0);
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(line(slot, row_of(i)) + mine(row_of(i))), "l"(row),
+                     "r"(o >= 0 ? 16 : 0)
+                     : "memory");
       }
+      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    auto take = [&]() {  // the ring's next slot
-      const int slot = issued % kSlots;
-      ok = issued < kSlots || warp_wait(empty(slot), ((issued / kSlots) - 1) & 1, abort_flag);
-      ++issued;
-      return slot;
-    };
-    auto put = [&](int slot) {
-      uint8_t* to = smem + L::ring + slot * L::tile;
-      const int c0 = 2 * (lane % LPR);
-      const bool swap = DIM == 128 && (c0 & 8);  // the two chunks in turn: distinct banks
+    // operand n's codes (all but the last `left` asked for have come) to f16
+    auto put = [&](int n, bool left) {
+      if (left) asm volatile("cp.async.wait_group 1;" ::: "memory");
+      else asm volatile("cp.async.wait_group 0;" ::: "memory");
+      const int slot = n % kSlots;
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
-        const int row = i * 4 * RPI + lw * RPI + lane / LPR;
-        uint32_t w[8];
-        const uint32_t in[4] = {r[i].x, r[i].y, r[i].z, r[i].w};
+        const uint32_t to = line(slot, row_of(i)), at = mine(row_of(i));
+        uint32_t in[4], w[8];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(in[0]), "=r"(in[1]), "=r"(in[2]), "=r"(in[3]) : "r"(to + at) : "memory");
 #pragma unroll
         for (int k = 0; k < 4; ++k) decode4<KV>(__byte_perm(in[k], 0, 0x3120), w[2 * k], w[2 * k + 1]);
-        uint8_t* line = to + (c0 >> 3) * L::half + row * 128;
-        const int even = ((c0 & 7) ^ (row & 7)) << 4, odd = (((c0 & 7) | 1) ^ (row & 7)) << 4;
-        const uint4 lo = make_uint4(w[0], w[1], w[2], w[3]), hi = make_uint4(w[4], w[5], w[6], w[7]);
-        *reinterpret_cast<uint4*>(line + (swap ? odd : even)) = swap ? hi : lo;
-        *reinterpret_cast<uint4*>(line + (swap ? even : odd)) = swap ? lo : hi;
+        const bool second = DIM == 128 && (c0 & 8);  // this lane's place is that of its second chunk
+#pragma unroll
+        for (int k = 0; k < 2; ++k) {
+          const bool hi = (k == 0) == second;
+          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (k == 0 ? at : at ^ 16)), "r"(hi ? w[4] : w[0]),
+                       "r"(hi ? w[5] : w[1]), "r"(hi ? w[6] : w[2]), "r"(hi ? w[7] : w[3])
+                       : "memory");
+        }
       }
       fence_proxy_async_smem();
     };
     open();
-    load(a.c.k);
+    ask(a.c.k);
+    ask(a.c.v);
+    ahead = entry(1);
 #pragma unroll 1
-    for (int i = 0; i < tiles; ++i) {
-      const int k_slot = take();
-      if (!ok) break;
-      // (the softmax of tile i - 2 is done: its V's slot is free)
+    for (int i = 0; i < tiles && ok; ++i) {
+      // (asked for behind V of tile i - 2, whose products followed that tile's softmax)
       const uint32_t bits = __float_as_uint(vs);
       const bool usable = bits - 1u < 0x7f7fffffu;  // positive and finite
       const uint32_t most = __reduce_max_sync(0xffffffffu, usable ? bits : 0u),
                      least = __reduce_min_sync(0xffffffffu, usable ? bits : 0x7f800000u);
       const bool bad = __any_sync(0xffffffffu, held && !isfinite(vs));
       if (lane == 0) top_s[(i & 1) * 4 + lw] = make_uint2(most, bad ? 0u : least);
-      put(k_slot);
+      put(2 * i, true);
       asm volatile("bar.sync 1, 128;" ::: "memory");
       uint32_t top = 0, low = 0x7f800000u;
 #pragma unroll
@@ -321,24 +471,27 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(scales(i));
-        mbar_arrive(full(k_slot));
+        mbar_arrive(full((2 * i) % kSlots));
       }
-      load(a.c.v);
-      const int v_slot = take();
-      if (!ok) break;
-      put(v_slot);
-      __syncwarp();
-      if (lane == 0) mbar_arrive(full(v_slot));
-      if (i + 1 < tiles) {
+      const bool more = i + 1 < tiles;
+      if (more) {
         if (++j == x.nt) {
           next(x);
           x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
           j = 0;
+          ahead = entry(0);
         }
         open();
-        load(a.c.k);
+        ask(a.c.k);
+        if (!ok) break;
+        ahead = entry(j + 1);
       }
+      put(2 * i + 1, more);
+      __syncwarp();
+      if (lane == 0) mbar_arrive(full((2 * i + 1) % kSlots));
+      if (more) ask(a.c.v);
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok) {
       if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_EMPTY);
       *abort_flag = 1;
@@ -435,17 +588,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
 #pragma unroll 1
           for (int c = 0; c < kTile; c += 16) tmem_st(st + c, zero);
         } else {
-          scores_to_weights<true>(
-              st, j == 0, j >= x.jm, sees - p0 + 1, factor, m, l, down,
-              [&](float (&v)[32], int c) {
-                const float4* f4 = reinterpret_cast<const float4*>(ks + c);
-#pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                  const float4 f = f4[k];
-                  v[4 * k] *= f.x, v[4 * k + 1] *= f.y, v[4 * k + 2] *= f.z, v[4 * k + 3] *= f.w;
-                }
-              },
-              v_scale_s + (tile & 1) * kTile, (float)lift_s[tile & 1]);
+          code_scores_to_weights(st, j == 0, j >= x.jm, sees - p0 + 1, factor, m, l, down, ks, v_scale_s + (tile & 1) * kTile,
+                                 (float)lift_s[tile & 1]);
         }
         tmem_wait_st();
         fence_before();
@@ -477,7 +621,7 @@ template <int DIM, Kv KV>
 cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   Params p;
   p.a = a;
-  p.box = 0;
+  p.box = (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.c.page_size) : -1;
   char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
   p.plan = plan_of<kCtaRows>(a, ws);
   p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
