@@ -256,9 +256,9 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
     }
   };
 
-  // launch: 128 registers x 512 threads = (48 + 64 + 2 x 200) x 128
+  // launch: 128 registers x 512 threads = (40 + 72 + 2 x 200) x 128
   if (warp < 4) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 48;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 40;");
     if (warp == 1) {
       // ------------------------------ products -------------------------------
       // f32 sums, f16 operands, M 128; N 128 positions, or DIM columns with V
@@ -362,7 +362,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         if (!warp_wait(empty(i % kSlots), (i / kSlots) & 1, nullptr) && lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_DRAIN);
     }
   } else if (warp < 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 64;");
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 72;");
     // ------------------------------- K and V --------------------------------
     constexpr int LPR = DIM / 16;         // lanes of a row, 16 codes each
     constexpr int RPI = 32 / LPR, IT = LPR;
@@ -391,66 +391,77 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
       ks = held ? a.c.k_scale[at_scale] : 0.f;
       vs = held ? a.c.v_scale[at_scale] : 0.f;
     };
-    // A lane's 16 codes of the warp's rows become two 16-byte chunks of f16; the codes
-    // come to the place of one of them (`mine`; the other's beside, so that lanes meet
-    // distinct banks), where the same lane takes them from.
+    // A lane's 16 codes of each of the warp's rows become two 16-byte chunks of f16.  K's
+    // wait in registers for their slot, which comes free half a tile before the tensor
+    // cores want them; V's, which have a tile and a half, come to the place of one of
+    // the chunks (`mine`), where the same lane takes them from.  (The other chunk's place
+    // for half the lanes: they meet distinct banks.)
     const int c0 = 2 * (lane % LPR);
+    const bool second = DIM == 128 && (c0 & 8);
     auto line = [&](int slot, int row) { return base + L::ring + slot * L::tile + (c0 >> 3) * L::half + row * 128; };
-    auto mine = [&](int row) { return (((c0 & 7) | (DIM == 128 ? c0 >> 3 : 0)) ^ (row & 7)) << 4; };
+    auto mine = [&](int row) { return (((c0 & 7) | (second ? 1 : 0)) ^ (row & 7)) << 4; };
     auto row_of = [&](int i) { return 32 * lw + i * RPI + lane / LPR; };
-    // the next operand's codes asked for, into the ring's next slot
-    auto ask = [&](const void* from) {
-      const int slot = issued % kSlots;
-      ok = issued < kSlots || warp_wait(empty(slot), ((issued / kSlots) - 1) & 1, abort_flag);
-      if (!ok) return;
-      ++issued;
+    uint4 kr[IT];
+    auto load_keys = [&]() {
 #pragma unroll
       for (int i = 0; i < IT; ++i) {
         const int64_t o = __shfl_sync(0xffffffffu, here, i * RPI + lane / LPR);
-        const uint8_t* row = static_cast<const uint8_t*>(from) + max(o, (int64_t)0) + 16 * (lane % LPR);
+        const uint8_t* row = static_cast<const uint8_t*>(a.c.k) + o + 16 * (lane % LPR);
+        kr[i] = make_uint4(0, 0, 0, 0);
+        // (predicated, not branched around: branches would keep the rows apart)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ge.s64 p, %4, 0;\n\t@p ld.global.v4.u32 {%0, %1, %2, %3}, [%5];\n\t}"
+                     : "+r"(kr[i].x), "+r"(kr[i].y), "+r"(kr[i].z), "+r"(kr[i].w)
+                     : "l"(o), "l"(row));
+      }
+    };
+    auto take = [&]() {  // the ring's next slot
+      const int slot = issued % kSlots;
+      ok = issued < kSlots || warp_wait(empty(slot), ((issued / kSlots) - 1) & 1, abort_flag);
+      ++issued;
+      return slot;
+    };
+    auto ask_values = [&](int slot) {
+#pragma unroll
+      for (int i = 0; i < IT; ++i) {
+        const int64_t o = __shfl_sync(0xffffffffu, here, i * RPI + lane / LPR);
+        const uint8_t* row = static_cast<const uint8_t*>(a.c.v) + max(o, (int64_t)0) + 16 * (lane % LPR);
         asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(line(slot, row_of(i)) + mine(row_of(i))), "l"(row),
                      "r"(o >= 0 ? 16 : 0)
                      : "memory");
       }
-      asm volatile("cp.async.commit_group;" ::: "memory");
     };
-    // operand n's codes (all but the last `left` asked for have come) to f16
-    auto put = [&](int n, bool left) {
-      if (left) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 0;" ::: "memory");
-      const int slot = n % kSlots;
+    // 16 codes of row_of(i) to f16
+    auto put = [&](int slot, int i, uint32_t x, uint32_t y, uint32_t z, uint32_t u) {
+      const uint32_t to = line(slot, row_of(i)), at = mine(row_of(i));
+      const uint32_t in[4] = {x, y, z, u};
+      uint32_t w[8];
 #pragma unroll
-      for (int i = 0; i < IT; ++i) {
-        const uint32_t to = line(slot, row_of(i)), at = mine(row_of(i));
-        uint32_t in[4], w[8];
-        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(in[0]), "=r"(in[1]), "=r"(in[2]), "=r"(in[3]) : "r"(to + at) : "memory");
+      for (int k = 0; k < 4; ++k) decode4<KV>(__byte_perm(in[k], 0, 0x3120), w[2 * k], w[2 * k + 1]);
 #pragma unroll
-        for (int k = 0; k < 4; ++k) decode4<KV>(__byte_perm(in[k], 0, 0x3120), w[2 * k], w[2 * k + 1]);
-        const bool second = DIM == 128 && (c0 & 8);  // this lane's place is that of its second chunk
-#pragma unroll
-        for (int k = 0; k < 2; ++k) {
-          const bool hi = (k == 0) == second;
-          asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (k == 0 ? at : at ^ 16)), "r"(hi ? w[4] : w[0]),
-                       "r"(hi ? w[5] : w[1]), "r"(hi ? w[6] : w[2]), "r"(hi ? w[7] : w[3])
-                       : "memory");
-        }
+      for (int k = 0; k < 2; ++k) {
+        const bool hi = (k == 0) == second;
+        asm volatile("st.shared.v4.u32 [%0], {%1, %2, %3, %4};" ::"r"(to + (k == 0 ? at : at ^ 16)), "r"(hi ? w[4] : w[0]),
+                     "r"(hi ? w[5] : w[1]), "r"(hi ? w[6] : w[2]), "r"(hi ? w[7] : w[3])
+                     : "memory");
       }
-      fence_proxy_async_smem();
     };
     open();
-    ask(a.c.k);
-    ask(a.c.v);
+    load_keys();
     ahead = entry(1);
 #pragma unroll 1
-    for (int i = 0; i < tiles && ok; ++i) {
-      // (asked for behind V of tile i - 2, whose products followed that tile's softmax)
+    for (int i = 0; i < tiles; ++i) {
       const uint32_t bits = __float_as_uint(vs);
       const bool usable = bits - 1u < 0x7f7fffffu;  // positive and finite
       const uint32_t most = __reduce_max_sync(0xffffffffu, usable ? bits : 0u),
                      least = __reduce_min_sync(0xffffffffu, usable ? bits : 0x7f800000u);
       const bool bad = __any_sync(0xffffffffu, held && !isfinite(vs));
       if (lane == 0) top_s[(i & 1) * 4 + lw] = make_uint2(most, bad ? 0u : least);
-      put(2 * i, true);
+      const int k_slot = take();
+      if (!ok) break;
+      // (V of tile i - 2 was there, whose products followed that tile's softmax)
+#pragma unroll
+      for (int r = 0; r < IT; ++r) put(k_slot, r, kr[r].x, kr[r].y, kr[r].z, kr[r].w);
+      fence_proxy_async_smem();
       asm volatile("bar.sync 1, 128;" ::: "memory");
       uint32_t top = 0, low = 0x7f800000u;
 #pragma unroll
@@ -471,10 +482,13 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) {
         mbar_arrive(scales(i));
-        mbar_arrive(full((2 * i) % kSlots));
+        mbar_arrive(full(k_slot));
       }
-      const bool more = i + 1 < tiles;
-      if (more) {
+      const int v_slot = take();
+      if (!ok) break;
+      ask_values(v_slot);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (i + 1 < tiles) {
         if (++j == x.nt) {
           next(x);
           x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
@@ -482,14 +496,22 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
           ahead = entry(0);
         }
         open();
-        ask(a.c.k);
-        if (!ok) break;
+        load_keys();
         ahead = entry(j + 1);
       }
-      put(2 * i + 1, more);
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+#pragma unroll
+      for (int r = 0; r < IT; ++r) {
+        uint32_t in[4];
+        asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                     : "=r"(in[0]), "=r"(in[1]), "=r"(in[2]), "=r"(in[3])
+                     : "r"(line(v_slot, row_of(r)) + mine(row_of(r)))
+                     : "memory");
+        put(v_slot, r, in[0], in[1], in[2], in[3]);
+      }
+      fence_proxy_async_smem();
       __syncwarp();
-      if (lane == 0) mbar_arrive(full((2 * i + 1) % kSlots));
-      if (more) ask(a.c.v);
+      if (lane == 0) mbar_arrive(full(v_slot));
     }
     asm volatile("cp.async.wait_all;" ::: "memory");
     if (!ok) {
