@@ -46,18 +46,19 @@ namespace {
 
 constexpr int kCtaRows = 2 * kTile;      // rows of a segment
 constexpr int kThreads = 384;
-constexpr int kSlots = 3;                // tiles of K or V in shared memory
 
-template <int DIM>
+template <int DIM, bool PREFIX>
 struct Smem {
+  static constexpr int slots = PREFIX ? kPrefixSlots : 3;
   static constexpr int half = kTile * 128;               // 128 rows of 64 f16
   static constexpr int tile = half * (DIM / 64);         // K, V, or one half (hi or lo) of a Q tile
   static constexpr int q = 0;                            // [row tile][hi, lo]
-  static constexpr int ring = 4 * tile;
-  static constexpr int bars = ring + kSlots * tile;
-  // full[3], empty[3], s_full[2], p_full[2], x_full[2], q_full[2], clean[2]
-  static constexpr int n_bars = 2 * kSlots + 10;
-  static constexpr int misc = bars + 8 * n_bars;         // tensor memory address, abort, unused, dirty
+  static constexpr int ring = (PREFIX ? 2 : 4) * tile;
+  static constexpr int bars = ring + slots * tile;
+  // full[slots], empty[slots], s_full[2], p_full[2], x_full[2], q_full[2], clean[2], half[2]
+  static constexpr int n_bars = 2 * slots + 12;
+  static constexpr int factors = bars + 8 * n_bars;      // (prefixes) powers of two of the rows' queries
+  static constexpr int misc = factors + (PREFIX ? kTile * 4 : 0);         // tensor memory address, abort, unused, dirty
   static constexpr int total = misc + 32 + 1024;         // the base is moved to 1024 bytes
 };
 
@@ -69,11 +70,12 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
       : "memory");
 }
 
-template <int DIM>
+template <int DIM, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 1)
     chunk_tc_kernel(const __grid_constant__ CUtensorMap map_k, const __grid_constant__ CUtensorMap map_v,
                     const __grid_constant__ Params p) {
-  using L = Smem<DIM>;
+  using L = Smem<DIM, PREFIX>;
+  constexpr int kSlots = L::slots, ROWS = PREFIX ? kPrefixRows : kCtaRows;
   constexpr int KS = DIM / 16;            // steps of 16 along the head
   constexpr int HALVES = DIM / 64;
   constexpr uint32_t kTmemCols = 512;
@@ -87,6 +89,7 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto p_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 2 + w); };
   auto x_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 4 + w); };
   auto q_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 6 + w); };
+  auto half = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 10 + w); };  // given, taken (split pieces)
   auto clean = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 8 + (i & 1)); };  // of masked tile i
   volatile int* misc = reinterpret_cast<volatile int*>(base_g + L::misc);
   volatile int* abort_flag = misc + 1;
@@ -113,6 +116,7 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(x_full(w), 1);
         mbar_init(q_full(w), 4);
         mbar_init(clean(w), 2);
+        mbar_init(half(w), 4);
       }
       mbar_fence_init();
     }
@@ -145,7 +149,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       int issued = 0;
       bool ok = true;
       while (at < end && ok) {
-        const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+        const Piece x = piece_of<ROWS, PREFIX>(p, group, t, kvh, at, end);
         for (int i = 0; i < 2 * x.nt; ++i) {  // K and V of each tile
           const int slot = issued % kSlots, pos = (x.j0 + (i >> 1)) * kTile + lane * p.box;
           int page = a.c.pages;  // past the pool: zeros
@@ -201,7 +205,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       const bool one = elect();
       // lo first: the large sums then take half the (cut) additions
       auto scores = [&](int w, int slot) {
-        const uint64_t q = q_desc + w * (2 * L::tile >> 4), k = k_desc + slot * (L::tile >> 4);
+        const uint64_t q = q_desc + (PREFIX ? 0 : w) * (2 * L::tile >> 4), k = k_desc + slot * (L::tile >> 4);
 #pragma unroll
         for (int h = 1; h >= 0; --h)
 #pragma unroll
@@ -220,7 +224,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             mma_ts(pw + 128, pw + 16 * t + 8 * h, v + t * (16 * 128 >> 4), idesc_o, h == 0 || t > 0);
       };
       // slot and phase of the ring's next tile
-      int slot = 0, phase = 0, masked = 0;
+      int slot = 0, phase = 0, masked = 0, operand = 0;
       auto advance = [&]() {
         if (++slot == kSlots) {
           slot = 0;
@@ -230,8 +234,50 @@ __global__ void __launch_bounds__(kThreads, 1)
       int steps[2] = {0, 0}, pieces[2] = {0, 0};
       bool ok = true;
       while (at < end && ok) {
-        const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+        const Piece x = piece_of<ROWS, PREFIX>(p, group, t, kvh, at, end);
         const int active = uniform(x.two ? 2 : 1), nt = uniform(x.nt), jm = uniform(x.jm);
+        if constexpr (PREFIX) {
+          // tile j is group j % 2's; operands 2 j (K) and 2 j + 1 (V) behind `operand`
+          const int first = operand;
+          operand += 2 * nt;
+          auto scores_of = [&](int j) {
+            const int n = first + 2 * j, w = j & 1;
+            ok = wait(full(n % kSlots), (n / kSlots) & 1);
+            if (!ok) return;
+            fence_after();
+            if (one) {
+              scores(w, n % kSlots);
+              commit(s_full(w));
+              commit(empty(n % kSlots));
+            }
+            __syncwarp();
+          };
+          ok = wait(q_full(0), pieces[0] & 1);
+          ++pieces[0];
+          if (ok) scores_of(0);
+          if (ok && nt > 1) scores_of(1);
+          for (int j = 0; j < nt && ok; ++j) {
+            const int n = first + 2 * j + 1, w = j & 1;
+            ok = wait(full(n % kSlots), (n / kSlots) & 1);
+            if (ok && j >= jm) {
+              ok = wait(clean(masked), (masked >> 1) & 1);
+              ++masked;
+            }
+            ok = ok && wait(p_full(w), steps[w] & 1);
+            if (!ok) break;
+            ++steps[w];
+            fence_after();
+            if (one) {
+              outputs(w, n % kSlots);
+              commit(x_full(w));
+              commit(empty(n % kSlots));
+            }
+            __syncwarp();
+            if (j + 2 < nt) scores_of(j + 2);
+          }
+          next(x);
+          continue;
+        }
         ok = wait(full(slot), phase);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
@@ -291,7 +337,7 @@ __global__ void __launch_bounds__(kThreads, 1)
       bool ok = true;
       int i0 = 0, masked = 0;
       while (at < end && ok) {
-        const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+        const Piece x = piece_of<ROWS, PREFIX>(p, group, t, kvh, at, end);
         for (int i = 0; i < 2 * x.nt; ++i, ++i0) {
           const int slot = i0 % kSlots, j = i >> 1;
           ok = warp_wait(full(slot), (i0 / kSlots) & 1, abort_flag);
@@ -335,17 +381,27 @@ __global__ void __launch_bounds__(kThreads, 1)
     // -------------------------------- softmax -------------------------------
     const int wg = warp >= 8 ? 1 : 0;  // row tile
     const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 * wg;
-    int steps = 0;
+    int steps = 0, splits = 0;
     bool ok = true;
     while (at < end && ok) {
-      const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
-      const int r = x.r0 + wg * kTile + 32 * (warp & 3) + lane;  // row of the sequence
+      const Piece x = piece_of<ROWS, PREFIX>(p, group, t, kvh, at, end);
+      const int r0 = x.r0 + (PREFIX ? 0 : wg * kTile), r = r0 + 32 * (warp & 3) + lane;  // row of the sequence
       const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + x.step * tok;
       const int64_t piece_at = at;
       next(x);
-      if (wg == 1 && !x.two) continue;
-      const float factor = stage_rows<DIM>(a, x, group, x.r0 + wg * kTile, base_g + L::q + wg * 2 * L::tile);
-      if (lane == 0) mbar_arrive(q_full(wg));
+      if (!PREFIX && wg == 1 && !x.two) continue;
+      float factor;
+      float* factor_s = reinterpret_cast<float*>(base_g + L::factors) + 32 * (warp & 3) + lane;
+      uint8_t* q_s = base_g + L::q + (PREFIX ? 0 : wg) * 2 * L::tile;
+      if (!PREFIX || wg == 0) {
+        factor = stage_rows<DIM>(a, x, group, r0, q_s);
+        if (PREFIX) *factor_s = factor;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full(wg));
+      } else {
+        ok = warp_wait(q_full(0), splits & 1, abort_flag);
+        factor = *factor_s;
+      }
       float o[DIM];
 #pragma unroll
       for (int d = 0; d < DIM; ++d) o[d] = 0.f;
@@ -360,25 +416,41 @@ __global__ void __launch_bounds__(kThreads, 1)
         });
         return true;
       };
-      for (int j = 0; j < x.nt; ++j, ++steps) {
+      const int j0 = PREFIX ? wg : 0, by = PREFIX ? 2 : 1;
+      for (int j = j0; j < x.nt && ok; j += by, ++steps) {
         // (while the tensor cores are at this tile's scores)
-        ok = (j == 0 || collect(steps - 1)) && warp_wait(s_full(wg), steps & 1, abort_flag);
+        ok = (j == j0 || collect(steps - 1)) && warp_wait(s_full(wg), steps & 1, abort_flag);
         if (!ok) break;
         fence_after();
-        scores_to_weights(st, j == 0, j >= x.jm, sees - (x.j0 + j) * kTile + 1, factor, m, l, down, [](float (&)[32], int) {});
+        scores_to_weights(st, j == j0, j >= x.jm, sees - (x.j0 + j) * kTile + 1, factor, m, l, down, [](float (&)[32], int) {});
         tmem_wait_st();
         fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(wg));
       }
-      ok = ok && collect(steps - 1);
+      ok = ok && (j0 >= x.nt || collect(steps - 1));
+      if (PREFIX && ok) {
+        if (wg == 1) {
+          give_half<DIM>(st, o, m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(half(0));
+          ok = warp_wait(half(1), splits & 1, abort_flag);
+        } else {
+          ok = warp_wait(half(0), splits & 1, abort_flag);
+          if (ok) take_half<DIM>(st + 256, o, m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(half(1));
+        }
+        ++splits;
+      }
       if (!ok) {
         if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_FULL);
         *abort_flag = 1;
         break;
       }
+      if (PREFIX && wg == 1) continue;
       const bool dirty = misc[3] != 0;
-      store_rows<DIM, kCtaRows, kF16>(p, x, group, cta, piece_at != begin, r, base_g + L::q + wg * 2 * L::tile, o, m, l, dirty);
+      store_rows<DIM, ROWS, kF16>(p, x, group, cta, piece_at != begin, r, q_s, o, m, l, dirty);
     }
   }
   fence_before();
@@ -412,23 +484,24 @@ bool page_map(CUtensorMap* map, const void* base, const Cache& c, int box) {
                      CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
-template <int DIM>
+template <int DIM, bool PREFIX>
 cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   CUtensorMap mk, mv;
+  constexpr int ROWS = PREFIX ? kPrefixRows : kCtaRows;
   Params p;
   p.a = a;
   p.box = std::min(a.c.page_size, kTile);
   if (!page_map(&mk, a.c.k, a.c, p.box) || !page_map(&mv, a.c.v, a.c, p.box)) return cudaErrorInvalidValue;
   char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
-  p.plan = plan_of<kCtaRows>(a, ws);
+  p.plan = plan_of<ROWS>(a, ws);
   p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
-  auto k = chunk_tc_kernel<DIM>;
+  auto k = chunk_tc_kernel<DIM, PREFIX>;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
-  if (e == cudaSuccess) e = launch_plan<kCtaRows>(a, p.plan, st);
-  if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, mk, mv, p);
+  cudaError_t e = allow_smem(k, Smem<DIM, PREFIX>::total, done);
+  if (e == cudaSuccess) e = launch_plan<ROWS, PREFIX>(a, p.plan, st);
+  if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM, PREFIX>::total, st, mk, mv, p);
   if (e == cudaSuccess) e = launch_beside(a, kF16, st);
-  if (e == cudaSuccess) e = launch_last<DIM, kCtaRows, kF16>(p, st);
+  if (e == cudaSuccess) e = launch_last<DIM, ROWS, PREFIX, kF16>(p, st);
   return e;
 }
 
@@ -436,13 +509,15 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
 
 bool tc_supported(const AttendArgs& a) {
   const int ps = a.c.page_size;
-  return (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) && plan_fits<kCtaRows>(a) && encode_fn() != nullptr;
+  return (ps == 16 || ps == 32 || ps == 64 || ps % kTile == 0) &&
+         (a.groups.n ? plan_fits<kPrefixRows>(a) : plan_fits<kCtaRows>(a)) && encode_fn() != nullptr;
 }
 
 size_t tc_workspace_bytes(int dim) { return kPlanBytes + kMaxParts * part_floats<kCtaRows>(dim) * sizeof(float); }
 
 cudaError_t launch_chunks_tc(const AttendArgs& a, cudaStream_t st) {
-  return a.c.dim == 128 ? launch<128>(a, st) : launch<64>(a, st);
+  if (a.groups.n) return a.c.dim == 128 ? launch<128, true>(a, st) : launch<64, true>(a, st);
+  return a.c.dim == 128 ? launch<128, false>(a, st) : launch<64, false>(a, st);
 }
 
 }  // namespace paged

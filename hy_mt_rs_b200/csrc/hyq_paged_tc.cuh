@@ -241,10 +241,9 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
   }
 }
 
-template <int ROWS>
+template <int ROWS, bool PREFIX>
 cudaError_t launch_plan(const AttendArgs& a, const Plan& plan, cudaStream_t st) {
-  if (a.groups.n) return launch_ex(plan_kernel<ROWS, true>, dim3(1), dim3(1024), 0, st, a, plan);
-  return launch_ex(plan_kernel<ROWS, false>, dim3(1), dim3(1024), 0, st, a, plan);
+  return launch_ex(plan_kernel<ROWS, PREFIX>, dim3(1), dim3(1024), 0, st, a, plan);
 }
 // The few-token kernel that a call's chunks' kernel starts beside it: the sequences
 // with few rows, or, for groups' prefixes, all sequences' own positions.
@@ -265,7 +264,7 @@ struct Piece {
   int64_t seg0;
   bool two, whole;
 };
-template <int ROWS>
+template <int ROWS, bool PREFIX>
 __device__ __forceinline__ Piece piece_of(const Params& p, int group, int t, int kvh, int64_t at, int64_t end) {
   Piece x;
   const Plan& plan = p.plan;
@@ -278,7 +277,7 @@ __device__ __forceinline__ Piece piece_of(const Params& p, int group, int t, int
   x.r0 = tile * ROWS;
   x.rows = min(ROWS, x.s.n * group - x.r0);
   x.two = x.rows > kTile;          // the second row tile has rows
-  x.step = place.w;
+  x.step = !PREFIX;
   x.first_tok = x.step * (x.r0 / group);
   x.len = x.s.pos + x.step * ((x.r0 + x.rows - 1) / group) + 1;  // positions the last row sees
   x.j0 = (int)(at - x.seg0);
@@ -587,6 +586,44 @@ __device__ __forceinline__ void scores_to_weights(uint32_t st, bool first, bool 
   l = fmaf(l, down, sum + sum2);
 }
 
+// Prefixes of f16 and 8-bit caches: a segment is one row tile, whose position tiles
+// go to the two softmax groups in turn, so that one's products run under the other's
+// softmax; the second tile of Q leaves room for five tiles of K and V.
+constexpr int kPrefixRows = kTile, kPrefixSlots = 5;
+// The groups' halves of a row are put together at the end: the second group's outputs
+// go to its own columns of tensor memory (`st`: scores, then outputs) with reference
+// and sum, and the first adds them to its own (`st`: the second's).
+template <int DIM>
+__device__ __forceinline__ void give_half(uint32_t st, const float (&o)[DIM], float m, float l) {
+#pragma unroll
+  for (int c = 0; c < DIM; c += 16) {
+    uint32_t v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = __float_as_uint(o[c + i]);
+    tmem_st(st + kTile + c, v);
+  }
+  uint32_t v[16] = {__float_as_uint(m), __float_as_uint(l)};
+  tmem_st(st, v);
+  tmem_wait_st();
+  fence_before();
+}
+template <int DIM>
+__device__ __forceinline__ void take_half(uint32_t st, float (&o)[DIM], float& m, float& l) {
+  fence_after();
+  float v[16];
+  tmem_ld(v, st);
+  tmem_wait_ld();
+  const float top = fmaxf(m, v[0]), f0 = m == -INFINITY ? 0.f : ex2(m - top), f1 = v[0] == -INFINITY ? 0.f : ex2(v[0] - top);
+  // (without a score above -inf: a sum of 0, or NaN to pass on)
+  l = (m == -INFINITY ? l : l * f0) + (v[0] == -INFINITY ? v[1] : v[1] * f1);
+  m = top;
+  tmem_each<DIM>(st + kTile, [&](float (&x)[16], int c) {
+#pragma unroll
+    for (int i = 0; i < 16; ++i) o[c + i] = fmaf(x[i], f1, o[c + i] * f0);
+  });
+  fence_before();
+}
+
 // The results of a warp's 32 rows of a piece, row r this thread's: outputs, or
 // a partial result.  They go through the rows' own places in q_s, whose
 // queries no product reads any more, so that rows are written whole.
@@ -880,12 +917,14 @@ __global__ void __launch_bounds__(128) merge_kernel(const __grid_constant__ Para
 }
 
 // A call's last kernel: the join of pieces, or the merge of prefixes and sequences.
-template <int DIM, int ROWS, Kv KV>
+template <int DIM, int ROWS, bool PREFIX, Kv KV>
 cudaError_t launch_last(const Params& p, cudaStream_t st) {
-  if (!p.a.groups.n)
+  if constexpr (PREFIX) {
+    const int64_t units = (int64_t)p.a.c.tokens * p.a.heads;
+    return launch_next(merge_kernel<DIM, ROWS, KV>, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, st, p);
+  } else {
     return launch_next(join_kernel<DIM, ROWS, KV>, dim3(kMaxCtas, ROWS / kJoinRows), dim3(256), 0, st, p);
-  const int64_t units = (int64_t)p.a.c.tokens * p.a.heads;
-  return launch_next(merge_kernel<DIM, ROWS, KV>, dim3((unsigned)((units + 3) / 4)), dim3(128), 0, st, p);
+  }
 }
 
 }  // namespace

@@ -97,7 +97,7 @@ __device__ __forceinline__ uint32_t exponent(uint32_t top) { return max(min(top 
 __device__ __forceinline__ float scale_of(uint32_t top) { return __uint_as_float((268u - exponent(top)) << 23); }
 __device__ __forceinline__ float unscale_of(uint32_t top) { return __uint_as_float((exponent(top) - 14u) << 23); }
 
-template <int DIM>
+template <int DIM, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_constant__ Params p) {
   using L = Smem<DIM>;
   constexpr int KS = DIM / 16;            // steps of 16 along the head
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
     uint8_t* k_s = base_g + L::k;
     uint8_t* v_s = base_g + L::v;
     uint2* top_s = reinterpret_cast<uint2*>(base_g + L::top);
-    Piece x = piece_of<kRows>(p, group, t, kvh, at, end);
+    Piece x = piece_of<kRows, PREFIX>(p, group, t, kvh, at, end);
     int j = 0;
     // where position row0 + lane % 16 of the tile begins, or -1
     auto place = [&]() {
@@ -253,7 +253,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
       if (i + 1 < tiles) {
         if (++j == x.nt) {
           next(x);
-          x = piece_of<kRows>(p, group, t, kvh, at, end);
+          x = piece_of<kRows, PREFIX>(p, group, t, kvh, at, end);
           j = 0;
         }
         there = place();
@@ -331,7 +331,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
     const uint32_t lanes = (uint32_t)(32 * warp) << 16;
     int i = 0;
     while (at < end && ok) {
-      const Piece x = piece_of<kRows>(p, group, t, kvh, at, end);
+      const Piece x = piece_of<kRows, PREFIX>(p, group, t, kvh, at, end);
       const int r = x.r0 + 32 * warp + lane;  // row of the sequence
       const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + x.step * tok;
       const bool second = at != begin;
@@ -439,7 +439,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc32_kernel(const __grid_co
   }
 }
 
-template <int DIM>
+template <int DIM, bool PREFIX>
 cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   Params p;
   p.a = a;
@@ -447,13 +447,13 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
   p.plan = plan_of<kRows>(a, ws);
   p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
-  auto k = chunk_tc32_kernel<DIM>;
+  auto k = chunk_tc32_kernel<DIM, PREFIX>;
   static std::atomic<uint64_t> done{0};
   cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
-  if (e == cudaSuccess) e = launch_plan<kRows>(a, p.plan, st);
+  if (e == cudaSuccess) e = launch_plan<kRows, PREFIX>(a, p.plan, st);
   if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
   if (e == cudaSuccess) e = launch_beside(a, kF32, st);
-  if (e == cudaSuccess) e = launch_last<DIM, kRows, kF32>(p, st);
+  if (e == cudaSuccess) e = launch_last<DIM, kRows, PREFIX, kF32>(p, st);
   return e;
 }
 
@@ -462,7 +462,8 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
 bool tc32_supported(const AttendArgs& a) { return plan_fits<kRows>(a); }
 
 cudaError_t launch_chunks_tc32(const AttendArgs& a, cudaStream_t st) {
-  return a.c.dim == 128 ? launch<128>(a, st) : launch<64>(a, st);
+  if (a.groups.n) return a.c.dim == 128 ? launch<128, true>(a, st) : launch<64, true>(a, st);
+  return a.c.dim == 128 ? launch<128, false>(a, st) : launch<64, false>(a, st);
 }
 
 }  // namespace paged

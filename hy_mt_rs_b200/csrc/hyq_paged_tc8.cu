@@ -25,24 +25,25 @@ namespace {
 
 constexpr int kCtaRows = 2 * kTile;      // rows of a segment
 constexpr int kThreads = 512;
-constexpr int kSlots = 3;                // tiles of K or V in shared memory
 constexpr int kSpread = 10;              // of the exponents of a tile's scales of V
 
-template <int DIM>
+template <int DIM, bool PREFIX>
 struct Smem {
+  static constexpr int slots = PREFIX ? kPrefixSlots : 3;
   static constexpr int half = kTile * 128;               // 128 rows of 64 f16
   static constexpr int tile = half * (DIM / 64);         // K, V, or one half (hi or lo) of a Q tile
   static constexpr int q = 0;                            // [row tile][hi, lo]
-  static constexpr int ring = 4 * tile;
-  static constexpr int k_scale = ring + kSlots * tile;   // [2][128]: of tile i in i & 1
+  static constexpr int ring = (PREFIX ? 2 : 4) * tile;
+  static constexpr int k_scale = ring + slots * tile;   // [2][128]: of tile i in i & 1
   static constexpr int v_scale = k_scale + 2 * kTile * 4;
   static constexpr int top = v_scale + 2 * kTile * 4;    // [2][4 warps] largest and smallest scale's bits
   static constexpr int bars = top + 2 * 4 * 8;
-  // full[3], empty[3], s_full[2], p_full[2], x_full[2], q_full[2], scales[2]
-  static constexpr int n_bars = 2 * kSlots + 10;
+  // full[slots], empty[slots], s_full[2], p_full[2], x_full[2], q_full[2], scales[2], half[2]
+  static constexpr int n_bars = 2 * slots + 12;
   // tensor memory address, abort, then [2] of: tile that is left out (its number +
   // 1), exponent of the tile's unit
-  static constexpr int misc = bars + 8 * n_bars;
+  static constexpr int factors = bars + 8 * n_bars;      // (prefixes) powers of two of the rows' queries
+  static constexpr int misc = factors + (PREFIX ? kTile * 4 : 0);
   static constexpr int total = misc + 32;
 };
 
@@ -185,9 +186,10 @@ __device__ __forceinline__ void code_scores_to_weights(uint32_t st, bool first, 
 }
 
 // (the base is aligned to 1024 bytes by its declaration, and checked)
-template <int DIM, Kv KV>
+template <int DIM, Kv KV, bool PREFIX>
 __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_constant__ Params p) {
-  using L = Smem<DIM>;
+  using L = Smem<DIM, PREFIX>;
+  constexpr int kSlots = L::slots, ROWS = PREFIX ? kPrefixRows : kCtaRows;
   constexpr int KS = DIM / 16;            // steps of 16 along the head
   constexpr uint32_t kTmemCols = 512;
   const AttendArgs& a = p.a;
@@ -199,6 +201,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
   auto p_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 2 + w); };
   auto x_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 4 + w); };
   auto q_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 6 + w); };
+  auto half = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 10 + w); };  // given, taken (split pieces)
   auto scales = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 8 + (i & 1)); };  // of tile i: phase i / 2
   float* k_scale_s = reinterpret_cast<float*>(smem + L::k_scale);
   float* v_scale_s = reinterpret_cast<float*>(smem + L::v_scale);
@@ -233,6 +236,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         mbar_init(x_full(w), 1);
         mbar_init(q_full(w), 4);
         mbar_init(scales(w), 4);
+        mbar_init(half(w), 4);
       }
       mbar_fence_init();
     }
@@ -276,7 +280,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
       const bool one = elect();
       // lo first: the large sums then take half the (cut) additions
       auto scores = [&](int w, int slot) {
-        const uint64_t q = q_desc + w * (2 * L::tile >> 4), k = k_desc + slot * (L::tile >> 4);
+        const uint64_t q = q_desc + (PREFIX ? 0 : w) * (2 * L::tile >> 4), k = k_desc + slot * (L::tile >> 4);
 #pragma unroll
         for (int h = 1; h >= 0; --h)
 #pragma unroll
@@ -295,7 +299,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
             mma_ts(pw + 128, pw + 16 * t + 8 * h, v + t * (16 * 128 >> 4), idesc_o, h == 0 || t > 0);
       };
       // slot and phase of the ring's next tile
-      int slot = 0, phase = 0;
+      int slot = 0, phase = 0, operand = 0;
       auto advance = [&]() {
         if (++slot == kSlots) {
           slot = 0;
@@ -305,8 +309,48 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
       int steps[2] = {0, 0}, pieces[2] = {0, 0}, issued = 0;
       bool ok = true;
       while (at < end && ok) {
-        const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+        const Piece x = piece_of<ROWS, PREFIX>(p, group, t, kvh, at, end);
         const int active = uniform(x.two ? 2 : 1), nt = uniform(x.nt);
+        if constexpr (PREFIX) {
+          // tile j is group j % 2's; operands 2 j (K) and 2 j + 1 (V) behind `operand`
+          const int first = operand;
+          operand += 2 * nt;
+          auto scores_of = [&](int j) {
+            const int n = first + 2 * j, w = j & 1;
+            ok = wait(full(n % kSlots), (n / kSlots) & 1);
+            if (!ok) return;
+            fence_after();
+            if (one) {
+              scores(w, n % kSlots);
+              commit(s_full(w));
+              commit(empty(n % kSlots));
+            }
+            __syncwarp();
+            ++issued;
+          };
+          ok = wait(q_full(0), pieces[0] & 1);
+          ++pieces[0];
+          if (ok) scores_of(0);
+          if (ok && nt > 1) scores_of(1);
+          for (int j = 0; j < nt && ok; ++j) {
+            const int n = first + 2 * j + 1, w = j & 1;
+            ok = wait(full(n % kSlots), (n / kSlots) & 1);
+            ok = ok && wait(p_full(w), steps[w] & 1);
+            if (!ok) break;
+            ++steps[w];
+            fence_after();
+            if (one) {
+              outputs(w, n % kSlots);
+              commit(x_full(w));
+              commit(empty(n % kSlots));
+            }
+            __syncwarp();
+            ++issued;
+            if (j + 2 < nt) scores_of(j + 2);
+          }
+          next(x);
+          continue;
+        }
         ok = wait(full(slot), phase);
 #pragma unroll
         for (int w = 0; w < 2; ++w) {
@@ -368,7 +412,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
     constexpr int RPI = 32 / LPR, IT = LPR;
     const int lw = warp - 4, pos_in = threadIdx.x - 128;
     uint2* top_s = reinterpret_cast<uint2*>(smem + L::top);
-    Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+    Piece x = piece_of<ROWS, PREFIX>(p, group, t, kvh, at, end);
     const int tiles = uniform((int)(end - begin));
     int j = 0, issued = 0, lift = 0;
     bool ok = true;
@@ -470,6 +514,20 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         top = max(top, o.x);
         low = min(low, o.y);
       }
+      int v_slot = 0;
+      auto ask = [&]() {
+        v_slot = take();
+        if (!ok) return;
+        ask_values(v_slot);
+        asm volatile("cp.async.commit_group;" ::: "memory");
+      };
+      if constexpr (PREFIX) {
+        // (here the ring alone does not say that the softmax of tile i - 2, whose scales
+        // these replace, is done: its V's products do)
+        ask();
+        if (ok && i >= 2) ok = warp_wait(empty((2 * i - 3) % kSlots), ((2 * i - 3) / kSlots) & 1, abort_flag);
+        if (!ok) break;
+      }
       // the unit: above the largest scale (a tile of zeros keeps the one before)
       if (top) lift = min(max((int)(top >> 23) - 126, -100), 100);
       const float unit = code_unit<KV>(), down = __uint_as_float((uint32_t)(127 - lift) << 23);
@@ -484,14 +542,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         mbar_arrive(scales(i));
         mbar_arrive(full(k_slot));
       }
-      const int v_slot = take();
-      if (!ok) break;
-      ask_values(v_slot);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      if constexpr (!PREFIX) {
+        ask();
+        if (!ok) break;
+      }
       if (i + 1 < tiles) {
         if (++j == x.nt) {
           next(x);
-          x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
+          x = piece_of<ROWS, PREFIX>(p, group, t, kvh, at, end);
           j = 0;
           ahead = entry(0);
         }
@@ -523,20 +581,29 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
     // -------------------------------- softmax -------------------------------
     const int wg = warp >= 12 ? 1 : 0;  // row tile
     const uint32_t st = tmem + ((uint32_t)(32 * (warp & 3)) << 16) + 256 * wg;
-    int steps = 0, tile = 0;  // this row tile's steps, all tiles of the CTA
+    int steps = 0, tiles = 0, splits = 0;  // this row tile's steps, all tiles of the pieces before
     bool ok = true;
     while (at < end && ok) {
-      const Piece x = piece_of<kCtaRows>(p, group, t, kvh, at, end);
-      const int r = x.r0 + wg * kTile + 32 * (warp & 3) + lane;  // row of the sequence
+      const Piece x = piece_of<ROWS, PREFIX>(p, group, t, kvh, at, end);
+      const int r0 = x.r0 + (PREFIX ? 0 : wg * kTile), r = r0 + 32 * (warp & 3) + lane;  // row of the sequence
       const int tok = min(r / group, x.s.n - 1), sees = x.s.pos + x.step * tok;
       const int64_t piece_at = at;
       next(x);
-      if (wg == 1 && !x.two) {
-        tile += x.nt;
-        continue;
+      const int tile0 = tiles;
+      tiles += x.nt;
+      if (!PREFIX && wg == 1 && !x.two) continue;
+      float factor;
+      float* factor_s = reinterpret_cast<float*>(smem + L::factors) + 32 * (warp & 3) + lane;
+      uint8_t* q_s = smem + L::q + (PREFIX ? 0 : wg) * 2 * L::tile;
+      if (!PREFIX || wg == 0) {
+        factor = stage_rows<DIM>(a, x, group, r0, q_s);
+        if (PREFIX) *factor_s = factor;
+        __syncwarp();
+        if (lane == 0) mbar_arrive(q_full(wg));
+      } else {
+        ok = warp_wait(q_full(0), splits & 1, abort_flag);
+        factor = *factor_s;
       }
-      const float factor = stage_rows<DIM>(a, x, group, x.r0 + wg * kTile, smem + L::q + wg * 2 * L::tile);
-      if (lane == 0) mbar_arrive(q_full(wg));
       float o[DIM];
 #pragma unroll
       for (int d = 0; d < DIM; ++d) o[d] = 0.f;
@@ -551,10 +618,12 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         });
         return true;
       };
-      for (int j = 0; j < x.nt; ++j, ++steps, ++tile) {
+      const int j0 = PREFIX ? wg : 0, by = PREFIX ? 2 : 1;
+      for (int j = j0; j < x.nt && ok; j += by, ++steps) {
+        const int tile = tile0 + j;
         // (while the tensor cores are at this tile's scores, which follow its scales:
         // the wait for those skips no phase)
-        ok = (j == 0 || collect(steps - 1)) && warp_wait(s_full(wg), steps & 1, abort_flag) &&
+        ok = (j == j0 || collect(steps - 1)) && warp_wait(s_full(wg), steps & 1, abort_flag) &&
              warp_wait(scales(tile), (tile >> 1) & 1, abort_flag);
         if (!ok) break;
         fence_after();
@@ -610,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
 #pragma unroll 1
           for (int c = 0; c < kTile; c += 16) tmem_st(st + c, zero);
         } else {
-          code_scores_to_weights(st, j == 0, j >= x.jm, sees - p0 + 1, factor, m, l, down, ks, v_scale_s + (tile & 1) * kTile,
+          code_scores_to_weights(st, j == j0, j >= x.jm, sees - p0 + 1, factor, m, l, down, ks, v_scale_s + (tile & 1) * kTile,
                                  (float)lift_s[tile & 1]);
         }
         tmem_wait_st();
@@ -618,17 +687,32 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         __syncwarp();
         if (lane == 0) mbar_arrive(p_full(wg));
       }
-      ok = ok && collect(steps - 1);
+      ok = ok && (j0 >= x.nt || collect(steps - 1));
+      if (PREFIX && ok) {
+        if (wg == 1) {
+          give_half<DIM>(st, o, m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(half(0));
+          ok = warp_wait(half(1), splits & 1, abort_flag);
+        } else {
+          ok = warp_wait(half(0), splits & 1, abort_flag);
+          if (ok) take_half<DIM>(st + 256, o, m, l);
+          __syncwarp();
+          if (lane == 0) mbar_arrive(half(1));
+        }
+        ++splits;
+      }
       if (!ok) {
         if (lane == 0) atomicOr(a.c.status, DEV_TIMEOUT_FULL);
         *abort_flag = 1;
         break;
       }
+      if (PREFIX && wg == 1) continue;
       if constexpr (KV == kF8) {
 #pragma unroll
         for (int d = 0; d < DIM; ++d) o[d] *= code_unit<KV>();
       }
-      store_rows<DIM, kCtaRows, KV>(p, x, group, cta, piece_at != begin, r, smem + L::q + wg * 2 * L::tile, o, m, l, false);
+      store_rows<DIM, ROWS, KV>(p, x, group, cta, piece_at != begin, r, q_s, o, m, l, false);
     }
   }
   fence_before();
@@ -639,32 +723,34 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
   }
 }
 
-template <int DIM, Kv KV>
+template <int DIM, Kv KV, bool PREFIX>
 cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
+  constexpr int ROWS = PREFIX ? kPrefixRows : kCtaRows;
   Params p;
   p.a = a;
   p.box = (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.c.page_size) : -1;
   char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
-  p.plan = plan_of<kCtaRows>(a, ws);
+  p.plan = plan_of<ROWS>(a, ws);
   p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
-  auto k = chunk_tc8_kernel<DIM, KV>;
+  auto k = chunk_tc8_kernel<DIM, KV, PREFIX>;
   static std::atomic<uint64_t> done{0};
-  cudaError_t e = allow_smem(k, Smem<DIM>::total, done);
-  if (e == cudaSuccess) e = launch_plan<kCtaRows>(a, p.plan, st);
-  if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM>::total, st, p);
+  cudaError_t e = allow_smem(k, Smem<DIM, PREFIX>::total, done);
+  if (e == cudaSuccess) e = launch_plan<ROWS, PREFIX>(a, p.plan, st);
+  if (e == cudaSuccess) e = launch_next(k, dim3(kMaxCtas), dim3(kThreads), Smem<DIM, PREFIX>::total, st, p);
   if (e == cudaSuccess) e = launch_beside(a, KV, st);
-  if (e == cudaSuccess) e = launch_last<DIM, kCtaRows, KV>(p, st);
+  if (e == cudaSuccess) e = launch_last<DIM, ROWS, PREFIX, KV>(p, st);
   return e;
 }
 
 template <Kv KV>
 cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
-  return a.c.dim == 128 ? launch<128, KV>(a, st) : launch<64, KV>(a, st);
+  if (a.groups.n) return a.c.dim == 128 ? launch<128, KV, true>(a, st) : launch<64, KV, true>(a, st);
+  return a.c.dim == 128 ? launch<128, KV, false>(a, st) : launch<64, KV, false>(a, st);
 }
 
 }  // namespace
 
-bool tc8_supported(const AttendArgs& a) { return plan_fits<kCtaRows>(a); }
+bool tc8_supported(const AttendArgs& a) { return a.groups.n ? plan_fits<kPrefixRows>(a) : plan_fits<kCtaRows>(a); }
 
 cudaError_t launch_chunks_tc8(const AttendArgs& a, Kv kv, cudaStream_t st) { return kv == kI8 ? launch<kI8>(a, st) : launch<kF8>(a, st); }
 
