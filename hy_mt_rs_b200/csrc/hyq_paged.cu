@@ -739,7 +739,7 @@ int hyq_paged_attention_shared(const hyq_paged_kv8* kv, const hyq_paged_batch* b
   a.groups.shared = shared;
   a.groups.n = (int)groups;
   a.groups.max_new = batch->max_new;
-  if (groups == 0 || max_shared == 0 || !shared_supported(a, type)) {
+  if (!shared_supported(a, type) || !worth_sharing(a, type, groups, max_shared)) {
     a.groups = {};
     return attend(a, type, batch->max_new, batch->max_len, name, st);
   }

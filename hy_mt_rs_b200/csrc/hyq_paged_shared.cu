@@ -18,6 +18,17 @@ size_t shared_workspace_bytes(int heads, int dim, int64_t tokens) {
          rounded(kMaxSeqs * sizeof(int32_t)) + rounded(tokens * sizeof(int2));
 }
 
+// Whether a call's prefixes are worth their own kernels: reading them for every
+// sequence costs 5 to 6 TB/s of L2, which reaches the three launches' own time at about
+// 150 MB.  Measured with 16 query and 4 kv heads, one group, shared / each on its own,
+// us: f16, 16 sequences of 2,000 (61 MB) 43 / 23, 32 (127 MB) 44 / 33, 64 (258 MB) 45 /
+// 51, 16 of 8,000 (246 MB) 37 / 47; int8, 32 of 2,000 (65 MB) 45 / 34, 64 (133 MB) 47 /
+// 51, 64 of 8,000 57 / 138; f32, 16 of 2,000 (123 MB) 46 / 41, 32 (254 MB) 48 / 69.
+bool worth_sharing(const AttendArgs& a, Kv kv, int64_t groups, int64_t max_shared) {
+  const int64_t row = 2 * ((int64_t)a.c.dim * value_bytes(kv) + (is_8bit(kv) ? 4 : 0)) * a.c.kv_heads;
+  return groups > 0 && (a.c.seqs - groups) * max_shared * row >= 150000000;
+}
+
 bool shared_supported(const AttendArgs& a, Kv kv) { return mma_supported(a, kv) && chunks_tc_supported(a, kv); }
 
 cudaError_t launch_shared(const AttendArgs& given, Kv kv, cudaStream_t st) {

@@ -17,7 +17,6 @@ constexpr int kMaxCtas = 148;
 constexpr int kMaxParts = 2 * kMaxCtas;  // partial results in the workspace: a CTA's first and last piece
 constexpr int kMaxSegs = 65536;          // segments of a call
 constexpr int kMinTiles = 2;             // cost of a CTA's range, at least
-constexpr int kMinPrefixTiles = 4;       // of prefixes: the few-token kernel beside has work for the other SMs
 constexpr int kSegTiles = 1;             // cost of a segment, in tiles
 // Floats of a partial result of a segment of ROWS rows: outputs, then
 // (maximum, sum) of each row, then whether a value may have been taken out.
@@ -46,6 +45,7 @@ struct Plan {
   Start* start;    // [kMaxCtas + 1]
   Segment* seg;    // [kMaxSegs]
   int most;        // segments that the rows of the call can make
+  int least;       // prefixes: tiles of a CTA's range, at least (more: there is other work for the SMs left)
 };
 constexpr size_t kPlanBytes = 16 + (kMaxCtas + 1) * sizeof(Start) + (size_t)kMaxSegs * sizeof(Segment);
 template <int ROWS>
@@ -56,7 +56,7 @@ template <int ROWS>
 inline Plan plan_of(const AttendArgs& a, void* ws) {
   char* p = static_cast<char*>(ws);
   return {reinterpret_cast<int*>(p), reinterpret_cast<Start*>(p + 16),
-          reinterpret_cast<Segment*>(p + 16 + (kMaxCtas + 1) * sizeof(Start)), (int)most_segments<ROWS>(a)};
+          reinterpret_cast<Segment*>(p + 16 + (kMaxCtas + 1) * sizeof(Start)), (int)most_segments<ROWS>(a), 0};
 }
 
 struct Params {
@@ -222,7 +222,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
   __syncthreads();
   if (threadIdx.x <= kMaxCtas) {
     const int64_t per = tiles + (int64_t)kSegTiles * segs, work = per * a.c.kv_heads;
-    const int64_t ctas = min((int64_t)kMaxCtas, max(work / (PREFIX ? kMinPrefixTiles : kMinTiles), (int64_t)1));
+    const int64_t ctas = min((int64_t)kMaxCtas, max(work / (PREFIX ? plan.least : kMinTiles), (int64_t)1));
     const int64_t unit = work * min((int64_t)threadIdx.x, ctas) / ctas;
     const int kvh = per ? (int)(unit / per) : 0;
     const int64_t rest = unit - kvh * per;

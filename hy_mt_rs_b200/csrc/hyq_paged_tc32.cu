@@ -446,6 +446,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   p.box = 0;
   char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
   p.plan = plan_of<kRows>(a, ws);
+  p.plan.least = 4;
   p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
   auto k = chunk_tc32_kernel<DIM, PREFIX>;
   static std::atomic<uint64_t> done{0};

@@ -731,6 +731,7 @@ cudaError_t launch(const AttendArgs& a, cudaStream_t st) {
   p.box = (a.c.page_size & (a.c.page_size - 1)) == 0 ? __builtin_ctz((unsigned)a.c.page_size) : -1;
   char* ws = static_cast<char*>(a.ws) + mma_workspace_bytes(DIM);
   p.plan = plan_of<ROWS>(a, ws);
+  p.plan.least = 8;
   p.parts = reinterpret_cast<float*>(ws + kPlanBytes);
   auto k = chunk_tc8_kernel<DIM, KV, PREFIX>;
   static std::atomic<uint64_t> done{0};

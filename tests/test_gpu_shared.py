@@ -26,13 +26,16 @@ def _make(dev, groups, heads, kvh, dim, page, kind, seed=0, own_pages=(), layout
     seqs = [(p, behind, new, i) for i, (p, members) in enumerate(groups) for behind, new in members]
     counts = [-(-(p + behind + new) // page) for p, behind, new, _ in seqs]
     pages = sum(counts) + 5
+    # a table so wide that the call's bound on the prefixes makes them worth their own kernels
+    row = 2 * kvh * {"f32": 4 * dim, "f16": 2 * dim}.get(kind, dim + 4)
+    width = max(max(counts) + 1, -(-150000000 // (max(1, len(seqs) - len(groups)) * row * page)) + 1)
     held = list(range(pages))
     rng.shuffle(held)
     shape = (pages, kvh, page, dim) if layout == "hnd" else (pages, page, kvh, dim)
     pools = [torch.randn(*shape, generator=g, device=dev) for _ in range(2)]
     if layout != "hnd":
         pools = [x.permute(0, 2, 1, 3) for x in pools]
-    table = torch.full((len(seqs), max(counts) + 1), -1, dtype=torch.int32)
+    table = torch.full((len(seqs), width), -1, dtype=torch.int32)
     at, first = 0, {}
     for s, ((p, behind, new, i), c) in enumerate(zip(seqs, counts)):
         mine = held[at:at + c]
@@ -128,6 +131,17 @@ def test_layout_slots_copies_outputs(cuda, kind):
     _close(got[:t], s)
     plain = paged.attention(s["q"], s["k_pages"], s["v_pages"], s["table"], s["row_start"], s["pos"], 4, slot=s["slot"], **s["kv"])
     _close(plain, s)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_small_prefixes_are_attention(cuda, kind):
+    """A call whose prefixes are not worth it gives attention()'s bits."""
+    import torch
+    from hy_mt_rs_b200 import paged
+    s = _make(cuda, [(200, [(9, 1), (0, 2), (50, 1)]), (333, [(1, 1), (70, 4)])], 16, 4, 128, 16, kind, seed=3)
+    plain = paged.attention(s["q"], s["k_pages"], s["v_pages"], s["table"], s["row_start"], s["pos"], 4, 500, **s["kv"])
+    assert torch.equal(_attend(s, max_len=500, max_shared=333), plain)
+    assert not torch.equal(_attend(s), plain)     # the other tests' way
 
 
 @pytest.mark.parametrize("kind", KINDS)
