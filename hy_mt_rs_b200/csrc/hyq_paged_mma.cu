@@ -61,24 +61,35 @@ constexpr int kSegmentCost = 4;
 // reads: it starts without waiting for that (when it may, every CTA of that has
 // seen what came before them both), and ends after it.
 // PART: only a sequence's positions from a.first on, and a.ml is written too.
-// NB 1: for sequences of up to 8 rows.
+// NB 1: a sequence with more than eight rows counts as several, of as many tokens as
+// eight rows hold each (at most `shares`).
 template <int DIM, Kv KV, bool PART, int NB>
 __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
-    few_kernel(const __grid_constant__ AttendArgs a, int shift, bool beside) {
+    few_kernel(const __grid_constant__ AttendArgs a, int shift, bool beside, int shares) {
   using G = Geo<DIM, KV, NB>;
   using R = RowsOf<DIM, KV, NB>;
   constexpr int kRows = G::rows;
   if (!beside) grid_dependency_wait();
   allow_dependents_launch();
   extern __shared__ __align__(1024) char smem[];
-  int* first_s = reinterpret_cast<int*>(smem + G::smem);  // [seqs + 1] tiles (of one kv head) before each sequence
+  int* first_s = reinterpret_cast<int*>(smem + G::smem);  // [seqs + 1] tiles (of one kv head) before each sequence (or share)
   __shared__ float ml_s[kWarps][kRows][2];
   __shared__ float factor_s[kRows];
   __shared__ int warp_s[kWarps];
   __shared__ int last_s;
   __shared__ int dirty_s;  // the last piece (of this CTA's) that clean() took a value out of
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int group = a.heads / a.c.kv_heads, seqs = a.c.seqs, kvh_n = a.c.kv_heads;
+  const int group = a.heads / a.c.kv_heads, seqs = NB == 1 ? a.c.seqs * shares : a.c.seqs, kvh_n = a.c.kv_heads;
+  auto load = [&](int i) {
+    if (NB > 1 || shares == 1) return load_seq(a.c, i);
+    Seq s = load_seq(a.c, i / shares);
+    if (s.n * group > kFewRows) return s;
+    const int before = min(i % shares * (kRows / group), s.n);
+    s.row0 += before;
+    s.pos += before;
+    s.n = min(s.n - before, kRows / group);
+    return s;
+  };
   // prefix sum of the sequences' tiles; sequences with more rows are the
   // chunk kernel's
   int carry = 0;
@@ -86,8 +97,8 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
     const int i = s0 + (int)threadIdx.x;
     int tiles = 0;
     if (i < seqs) {
-      const Seq s = load_seq(a.c, i);
-      if (s.n > 0 && s.n * group <= kRows) tiles = (s.pos + s.n - (PART ? a.first[i] : 0) + G::tile - 1) / G::tile + kSegmentCost;
+      const Seq s = load(i);
+      if (s.n > 0 && s.n * group <= kRows) tiles = (s.pos + s.n - (PART ? a.first[NB == 1 ? i / shares : i] : 0) + G::tile - 1) / G::tile + kSegmentCost;
       else if (s.n > 0 && !beside) atomicOr(a.c.status, DEV_BAD_ARGS);  // max_new was too small: nobody takes it
     }
     int x = tiles;
@@ -164,8 +175,8 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
     cur.j0 = (int)(at - cur.seg0);
     cur.j1 = (int)(min(end, cur.seg0 + cur.tiles) - cur.seg0);
     if (!same_seq) {
-      cur.s = load_seq(a.c, si);
-      cur.first = PART ? a.first[si] + off : off;
+      cur.s = load(si);
+      cur.first = PART ? a.first[NB == 1 ? si / shares : si] + off : off;
     }
     const Feed<DIM, KV, NB> feed{a, cur.s, cur.kvh, cur.s.pos + cur.s.n, shift};
     page = feed.page(cur.j0 * G::tile + cur.first);
@@ -484,27 +495,30 @@ cudaError_t chunks(const AttendArgs& a, cudaStream_t st) {
 }
 
 template <int DIM, Kv KV, bool PART, int NB>
-cudaError_t few(const AttendArgs& a, bool beside, cudaStream_t st) {
+cudaError_t few(const AttendArgs& a, int shares, bool beside, cudaStream_t st) {
   using G = Geo<DIM, KV, NB>;
   auto k = few_kernel<DIM, KV, PART, NB>;
   static std::atomic<uint64_t> done{0};
-  const cudaError_t e = allow_smem(k, G::smem + (kMaxSeqs + 1) * 4, done);
+  const cudaError_t e = allow_smem(k, G::smem + ((NB == 1 ? 3 : 1) * kMaxSeqs + 1) * 4, done);
   if (e != cudaSuccess) return e;
-  return launch_dependent(beside || launch_overlap(), k, dim3(kSms * G::ctas), dim3(kThreads), (size_t)G::smem + (a.c.seqs + 1) * 4,
-                          st, a, page_shift(a), beside);
+  return launch_dependent(beside || launch_overlap(), k, dim3(kSms * G::ctas), dim3(kThreads),
+                          (size_t)G::smem + (shares * a.c.seqs + 1) * 4, st, a, page_shift(a), beside, shares);
 }
 
 template <int DIM, Kv KV, int NB>
-cudaError_t few(const AttendArgs& a, bool beside, cudaStream_t st) {
-  return a.first ? few<DIM, KV, true, NB>(a, beside, st) : few<DIM, KV, false, NB>(a, beside, st);
+cudaError_t few(const AttendArgs& a, int shares, bool beside, cudaStream_t st) {
+  return a.first ? few<DIM, KV, true, NB>(a, shares, beside, st) : few<DIM, KV, false, NB>(a, shares, beside, st);
 }
 
 template <Kv KV>
 cudaError_t few(const AttendArgs& a, int64_t rows, bool beside, cudaStream_t st) {
   if constexpr (is_8bit(KV)) {
-    if (rows <= 8) return a.c.dim == 128 ? few<128, KV, 1>(a, beside, st) : few<64, KV, 1>(a, beside, st);
+    const int group = a.heads / a.c.kv_heads;
+    const int shares = group > 8 ? 1 : std::max(1, ((int)rows / group + 8 / group - 1) / (8 / group));  // 3 at most
+    if (group <= 8)
+      return a.c.dim == 128 ? few<128, KV, 1>(a, shares, beside, st) : few<64, KV, 1>(a, shares, beside, st);
   }
-  return a.c.dim == 128 ? few<128, KV, 2>(a, beside, st) : few<64, KV, 2>(a, beside, st);
+  return a.c.dim == 128 ? few<128, KV, 2>(a, 1, beside, st) : few<64, KV, 2>(a, 1, beside, st);
 }
 
 template <Kv KV>
