@@ -28,6 +28,7 @@ REFUSED = 2147483647    # HYQ_PAGES_REFUSED
 
 _ops = load_ops()
 _KV_TYPES = (torch.float32, torch.float16)
+_CODES = (torch.int8, torch.float8_e4m3fn)      # 8-bit caches
 _PAGES = struct.Struct("PPPPqqqi4x")     # hyq_pages
 _POOL = struct.Struct("Pqqqq")           # hyq_page_pool
 _ZEROED = 4096                           # HYQ_PAGED_ATTENTION_ZEROED
@@ -126,7 +127,10 @@ class PagedCache:
     """Pages of every layer's keys and values, and the device tables that say
     which sequence holds which: `pool` [layers, 2, pages, kv_heads, page_size,
     head_dim] (layer(i) gives its keys and values), `table` [slots,
-    table_width] (-1: unused), `length` [slots] and `refs` [pages].
+    table_width] (-1: unused), `length` [slots] and `refs` [pages].  dtype int8 or
+    float8_e4m3fn: an 8-bit cache, whose pool is [layers, 2, pages, bytes] (uint8),
+    a page's codes and then its scales, so that page copies move both (layer(i)
+    gives the codes, scales(i) their scales).
 
     A slot is a sequence.  reserve() before each step makes room for its new
     tokens and returns the positions they start at; fork() shares a sequence's
@@ -140,6 +144,18 @@ class PagedCache:
 
     def __init__(self, layers, kv_heads, head_dim, pages, page_size, slots, table_width, device, dtype=torch.float16):
         z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=device)  # noqa: E731
+        if dtype in _CODES:
+            up = lambda n: -(-n // 16) * 16  # noqa: E731
+            rows = kv_heads * page_size
+            scales = up(rows * head_dim)
+            pool = torch.zeros(layers, 2, pages, scales + up(4 * rows), dtype=torch.uint8, device=device)
+            coded = pool[..., :rows * head_dim].view(dtype).as_strided(
+                (layers, 2, pages, kv_heads, page_size, head_dim),
+                (*pool.stride()[:3], page_size * head_dim, head_dim, 1))
+            scale = pool.view(torch.float32).as_strided(
+                (layers, 2, pages, kv_heads, page_size), (*(n // 4 for n in pool.stride()[:3]), page_size, 1), scales // 4)
+            self._init(coded, z(slots, table_width) - 1, z(slots), z(pages), pool, scale)
+            return
         self._init(torch.zeros(layers, 2, pages, kv_heads, page_size, head_dim, dtype=dtype, device=device),
                    z(slots, table_width) - 1, z(slots), z(pages))
 
@@ -151,17 +167,18 @@ class PagedCache:
         cache._init(pool, table, length, refs)
         return cache
 
-    def _init(self, pool, table, length, refs):
-        if not isinstance(pool, torch.Tensor) or pool.dtype not in _KV_TYPES:
+    def _init(self, pool, table, length, refs, raw=None, scale=None):
+        if not isinstance(pool, torch.Tensor) or pool.dtype not in (_KV_TYPES if raw is None else _CODES):
             raise HyqError(-1, "pool: expected a CUDA float32 or float16 tensor")
-        _need_cuda(pool, "pool")
+        _need_cuda(pool if raw is None else raw, "pool")
         for t, name in ((table, "table"), (length, "length"), (refs, "refs")):
             _need_cuda(t, name, torch.int32)
             self._same_device(t, pool, name)
         if pool.dim() != 6 or pool.shape[1] != 2 or table.dim() != 2 or length.numel() != table.shape[0] \
                 or refs.numel() != pool.shape[2]:
             raise HyqError(-2, "PagedCache: shapes of pool, table, length and refs")
-        self.pool, self.table, self.length, self.refs = pool, table, length, refs
+        self.pool, self.table, self.length, self.refs = pool if raw is None else raw, table, length, refs
+        self._pages_of, self._scale = pool, scale
         self.page_size, self.pages, self.slots = pool.shape[4], pool.shape[2], table.shape[0]
         self.changes = 0
         self.shortage = torch.zeros(1, dtype=torch.int32, device=pool.device)
@@ -170,7 +187,7 @@ class PagedCache:
         self._ws = torch.empty(n.value, dtype=torch.uint8, device=pool.device)
         self._pages = _PAGES.pack(table.data_ptr(), length.data_ptr(), refs.data_ptr(), self.shortage.data_ptr(),
                                   table.shape[0], table.shape[1], self.pages, self.page_size)
-        page = pool[0, 0, 0].numel() * pool.element_size()
+        page = self.pool[0, 0, 0].numel() * pool.element_size()
         self._pool = _POOL.pack(pool.data_ptr(), 2 * pool.shape[0], page * self.pages, page, page)
 
     @staticmethod
@@ -180,7 +197,11 @@ class PagedCache:
 
     def layer(self, i):
         """(k_pages, v_pages) of a layer."""
-        return self.pool[i, 0], self.pool[i, 1]
+        return self._pages_of[i, 0], self._pages_of[i, 1]
+
+    def scales(self, i):
+        """(k_scale, v_scale) of a layer of an 8-bit cache, else (None, None)."""
+        return (None, None) if self._scale is None else (self._scale[i, 0], self._scale[i, 1])
 
     def _slots(self, *arrays):
         n = arrays[0].numel() if isinstance(arrays[0], torch.Tensor) else 0

@@ -6,8 +6,9 @@ The reference serves one Session per request (README.md:139-141), each with a
 contiguous cache (model.rs:116-120) and a Sampler on the host (generation.rs).
 Here a step runs the batched forward (model.rs:549-646) over the new rows of
 all requests at once: hyq_embed and the batched products as DenseBatch runs
-them, hyq_paged_rope_append and hyq_paged_attention over the requests' pages
-(hy_mt_rs_b200.paged), and hyq_sample for the next tokens
+them, hyq_paged_rope_append and hyq_paged_attention (hyq_paged_attention_shared where
+requests were forked from one another) over the requests' pages
+(hy_mt_rs_b200.paged), and hyq_logits_adjust and hyq_sample for the next tokens
 (hy_mt_rs_b200.sampling).
 """
 import torch
@@ -22,15 +23,15 @@ __all__ = ["PagedBatch"]
 
 class PagedBatch:
     """Requests in the slots of a PagedCache, over a DenseModel's weights
-    (either architecture; the cache type and the products' precision are the
-    model's).
+    (either architecture; the products' precision is the model's).
 
     slots: requests at a time, at most 1024.  They share `pages` pages of page_size
     positions (by default enough for every slot to reach cfg.positions).
     chunk: prompt tokens that generate() feeds in a step, next to the tokens of
-    the requests that decode already."""
+    the requests that decode already.  kv_dtype: the cache's type, the model's by
+    default; torch.int8 and torch.float8_e4m3fn are 8-bit caches (paged)."""
 
-    def __init__(self, model, slots, pages=None, page_size=64, chunk=256):
+    def __init__(self, model, slots, pages=None, page_size=64, chunk=256, kv_dtype=None):
         cfg, dev = model.cfg, model.device
         if not 1 <= slots <= 1024:
             raise ValueError("1 to 1024 slots")
@@ -39,10 +40,11 @@ class PagedBatch:
         self.m, self.slots, self.chunk = model, slots, chunk
         width = -(-cfg.positions // page_size)
         self.cache = paged.PagedCache(len(model.layers), cfg.kv_heads, cfg.head_dim, pages or slots * width, page_size,
-                                      slots, width, dev, dtype=model.kv_dtype)
+                                      slots, width, dev, dtype=kv_dtype or model.kv_dtype)
         half = cfg.head_dim // 2
         self.cos, self.sin = model.cos.view(cfg.positions, half), model.sin.view(cfg.positions, half)
-        self.workspace = paged.attention_workspace(cfg.heads, cfg.head_dim, dev)
+        self._few = 16 // (cfg.heads // cfg.kv_heads)     # tokens of a request that attention_shared takes
+        self.workspace = paged.attention_shared_workspace(cfg.heads, cfg.head_dim, slots * max(self._few, 1), dev)
         self.acts = _Acts(cfg, slots + chunk, dev)
         self._known([0] * slots)
 
@@ -50,17 +52,36 @@ class PagedBatch:
         length = self.cache.length
         return self.cache.changes, 0 if length.is_inference() else length._version
 
-    def _known(self, held):
+    def _known(self, held, prefix=None):
         """The slots' lengths after the calls so far: exact, or past the cache's
-        where pages were short."""
-        self._held, self._held_at = held, self._state()
+        where pages were short; and of slots forked from one another a key and
+        the positions that all with this key have in common."""
+        self._held, self._held_at, self._prefix = held, self._state(), prefix or {}
 
     def _fork(self, src, dst):
         self.cache.fork(*self._ints(src, dst))
-        held = list(self._held)
+        held, prefix = list(self._held), dict(self._prefix)
+        for b in dst:
+            prefix.pop(b, None)
         for a, b in zip(src, dst):
             held[b] = self._held[a]
-        self._known(held)
+            prefix[b] = prefix.setdefault(a, (object(), self._held[a]))
+        self._known(held, prefix)
+
+    def _groups(self, slots, lengths):
+        """Neighbouring requests of a step that share a prefix, for
+        paged.attention_shared: (starts, shared), or None if there are none or
+        some request has more tokens than that takes."""
+        if not self._prefix or max(lengths) > self._few:
+            return None
+        starts, shared, last = [], [], None
+        for i, s in enumerate(slots):
+            key, n = self._prefix.get(s, (None, 0))
+            if key is None or key is not last:
+                starts.append(i)
+                shared.append(n)
+            last = key
+        return None if len(starts) == len(slots) else (starts + [len(slots)], shared)
 
     def _lengths_after(self, slots, lengths):
         """The requests' lengths after `lengths` more tokens; ValueError if one
@@ -101,12 +122,14 @@ class PagedBatch:
             self.acts = _Acts(cfg, rows, dev)
         a = self.acts
         ends = torch.tensor(lengths).cumsum(0).tolist()
-        slot, extra, row_start = self._ints(slots, lengths, [0] + ends)
+        groups = self._groups(slots, lengths)
+        starts, shared = groups or ([], [])
+        slot, extra, row_start, starts, shared = self._ints(slots, lengths, [0] + ends, starts, shared)
         pos = self.cache.reserve(slot, extra)
         held = list(self._held)
         for s, length in zip(slots, after):
             held[s] = length
-        self._known(held)
+        self._known(held, self._prefix)
         q, k, v, attended = (t[:rows].view(rows, -1, cfg.head_dim) for t in (a.q, a.k, a.v, a.attended))
         logits = torch.empty(n, cfg.vocab, device=dev)
         st, fused = m._stream(), m.precision == quant.GEMM_F32
@@ -115,12 +138,20 @@ class PagedBatch:
             delta = None
             for i, W in enumerate(m.layers):
                 k_pages, v_pages = self.cache.layer(i)
+                k_scale, v_scale = self.cache.scales(i)
                 _qkv_normed(fused, W, _p(a.hidden), delta, _p(W["input_norm"]), cfg.eps, rows, _p(a.normalized),
                             (_p(a.q), _p(a.k), _p(a.v)), st)
                 paged.rope_append(q, k, v, k_pages, v_pages, self.cache.table, row_start, pos, self.cos, self.sin,
-                                  W["q_norm"], W["k_norm"], cfg.eps, bool(m.norm_first), slot=slot, out=q)
-                paged.attention(q, k_pages, v_pages, self.cache.table, row_start, pos, max(lengths),
-                                max(after), slot=slot, out=attended, workspace=self.workspace)
+                                  W["q_norm"], W["k_norm"], cfg.eps, bool(m.norm_first), slot=slot, out=q,
+                                  k_scale=k_scale, v_scale=v_scale)
+                if groups:
+                    paged.attention_shared(q, k_pages, v_pages, self.cache.table, row_start, pos, starts, shared, max(lengths),
+                                           max(after), max(groups[1]), slot=slot, out=attended, workspace=self.workspace,
+                                           k_scale=k_scale, v_scale=v_scale)
+                else:
+                    paged.attention(q, k_pages, v_pages, self.cache.table, row_start, pos, max(lengths),
+                                    max(after), slot=slot, out=attended, workspace=self.workspace, k_scale=k_scale,
+                                    v_scale=v_scale)
                 check(lib.hyq_matmul(W["o"].handle, _p(a.attended), rows, _p(a.projected), st))
                 if "moe" in W:
                     _add_norm(_p(a.hidden), _p(a.projected), _p(W["ffn_norm"]), cfg.hidden, rows, cfg.eps,
@@ -139,12 +170,18 @@ class PagedBatch:
                            st)
         return logits
 
-    def generate(self, prompts, n_new, answers=1, temperature=0.0, top_k=None, top_p=None, min_p=None, seed=0):
+    def generate(self, prompts, n_new, answers=1, temperature=0.0, top_k=None, top_p=None, min_p=None, seed=0,
+                 repetition=None, presence=None, frequency=None, bias=None, mask=None):
         """n_new tokens of each of `answers` answers to each prompt (lists of
         ids): [prompt][answer][token].  A prompt's answers share its full pages
         (PagedCache.fork).  The sampling parameters hold for all requests
         (temperature 0: greedy); `seed` seeds the uniform numbers.  The tokens
-        stay on the device until the end."""
+        stay on the device until the end.
+
+        repetition, presence and frequency (numbers): penalties of the tokens of
+        the prompt and the answer so far; bias: {token: value}; mask [1 or prompts,
+        (vocab + 31) // 32] (int32): the tokens that all requests, or each
+        prompt's, may take (sampling.adjust states the rules)."""
         dev, used = self.m.device, len(prompts) * answers
         if not prompts or min(len(p) for p in prompts) < 1 or answers < 1 or n_new < 1:
             raise ValueError("at least one prompt token, answer and new token")
@@ -161,6 +198,15 @@ class PagedBatch:
         short = torch.zeros(1, dtype=torch.int32, device=dev)
         self.cache.free(self._ints(range(self.slots))[0])
         self._known([0] * self.slots)
+        penalties = dict(repetition=repetition, presence=presence, frequency=frequency)
+        history = None
+        if any(p is not None for p in penalties.values()):
+            history = torch.full((self.slots, self.m.cfg.positions), -1, dtype=torch.int32, device=dev)
+            for i, ids in enumerate(prompt_ids):
+                history[i * answers:(i + 1) * answers, :ids.numel()] = ids
+            told = self._ints([len(prompts[min(s, used - 1) // answers]) for s in range(self.slots)])[0]   # the prompts' lengths
+        if bias:
+            bias_token, bias_value = self._ints(bias.keys())[0], torch.tensor(list(bias.values()), dtype=torch.float32).to(dev)
         while True:
             # a token of every decoding request, then prompt tokens
             slots = [s for s, count in made.items() if count < n_new]
@@ -191,8 +237,23 @@ class PagedBatch:
                 continue
             row, slot, column = self._ints([r for r, _ in sources], [s for _, s in sources],
                                            [made.get(s, 0) for _, s in sources])
-            token, _ = sampling.sample(logits.index_select(0, row), torch.rand(len(sources), generator=random, device=dev),
-                                       temperature, top_k, top_p, min_p)
+            picked = logits.index_select(0, row)
+            if history is not None or bias or mask is not None:
+                n, more = len(sources), {}
+                if history is not None:
+                    length = told.clone()
+                    length[slot.long()] += column
+                    more.update(history=history, length=length, prompt=told, slot=slot, **penalties)
+                if bias:
+                    more["bias"] = (torch.arange(n + 1, dtype=torch.int32, device=dev) * len(bias), bias_token.repeat(n),
+                                    bias_value.repeat(n))
+                if mask is not None:
+                    more.update(mask=mask, mask_row=slot // answers if mask.shape[0] > 1 else torch.zeros_like(slot))
+                sampling.adjust(picked, **more, out=picked)
+            token, _ = sampling.sample(picked, torch.rand(len(sources), generator=random, device=dev), temperature, top_k, top_p,
+                                       min_p)
+            if history is not None:
+                history[slot.long(), (told[slot.long()] + column).long()] = token
             latest[slot.long()] = token
             out[slot.long(), column.long()] = token
             for _, s in sources:
