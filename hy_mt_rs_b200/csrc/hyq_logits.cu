@@ -1,13 +1,14 @@
 // Penalties for repeated tokens, biases and masks on rows of logits, in one pass
 // (include/hyq.h states the rule).
 //
-// A CTA takes a slice of a row: it asks for its logits first, and while they
-// come counts the slice's tokens among the row's history in shared memory (whole
-// numbers: the order of the atomics does not matter).  Biases, which are few, come
-// after the slice is out: the last entry of each token is found in the counts' place.
-// Bound by memory, 8 bytes a logit; the history is read by every slice of its row,
-// mostly from L2, so slices are as long as registers hold, unless a call has too few
-// to fill the SMs with.
+// A CTA takes a slice of a row: it copies it, masked, while the row's history comes,
+// and then changes the logits of the slice's tokens in that (noted down in shared
+// memory as they come), each once, by whoever of their occurrences takes the count
+// (whole numbers: the order of the atomics does not matter); the last bias entry of
+// each token likewise.  Bound by
+// memory, 8 bytes a logit; the history is read by every slice of its row, mostly from
+// L2, so slices are as long as registers hold, unless a call has too few to fill the SMs
+// with.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -32,27 +33,17 @@ struct Args {
   unsigned* status;
 };
 
-// The tokens of a list from thread to thread, four loads in flight: f(token, index).
-template <typename F>
-__device__ __forceinline__ void each(const int32_t* list, int count, F f) {
-  int i = threadIdx.x;
-  for (; i + 3 * kThreads < count; i += 4 * kThreads) {
-    int32_t t[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) t[k] = list[i + k * kThreads];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) f(t[k], i + k * kThreads);
-  }
-  for (; i < count; i += kThreads) f(list[i], i);
-}
-
 // PER: logits of a thread.
 template <int PER>
 __global__ void __launch_bounds__(kThreads, PER == 32 ? 4 : 8) adjust_kernel(const __grid_constant__ Args a) {
   constexpr int kPer = PER, kSlice = kThreads * PER;
   grid_dependency_wait();
   allow_dependents_launch();
-  __shared__ __align__(16) unsigned count_s[kSlice];
+  __shared__ unsigned count_s[kSlice];
+  constexpr int kNotes = 4096;
+  __shared__ uint16_t note_s[kNotes];  // the slice's tokens in the history: place, from 0x8000 up in the prompt
+  __shared__ int notes_s;
+  static_assert(kSlice <= 0x8000, "a place in 15 bits");
   const int r = blockIdx.x / a.slices, lo = (blockIdx.x - r * a.slices) * kSlice, size = min(kSlice, a.n - lo);
   const float* x = a.x + r * a.x_stride + lo;
   float* out = a.out + r * a.out_stride + lo;
@@ -75,79 +66,60 @@ __global__ void __launch_bounds__(kThreads, PER == 32 ? 4 : 8) adjust_kernel(con
 #pragma unroll
     for (int k = 0; k < kPer; ++k) v[k] = at(k) < size ? x[at(k)] : 0.f;
   }
+  if (threadIdx.x == 0) notes_s = 0;
+  __syncthreads();
   const hyq_adjust& p = a.a;
   auto bad = [&] {
     if (threadIdx.x == 0) atomicOr(a.status, DEV_BAD_ARGS);
   };
-  // the row's history
+  // what the row has, each list's loads as early as what they need is there
   float rep = p.repetition ? p.repetition[r] : 1.f;
-  if (!(rep > 0.f)) rep = 1.f;
   const float presence = p.presence ? p.presence[r] : 0.f, frequency = p.frequency ? p.frequency[r] : 0.f;
+  const int slot = !p.history ? -1 : p.slot ? p.slot[r] : r, mask = !p.mask ? -1 : p.mask_row ? p.mask_row[r] : r;
+  int bias0 = p.bias_start ? p.bias_start[r] : 0, biases = p.bias_start ? p.bias_start[r + 1] - bias0 : 0;
+  if (!(rep > 0.f)) rep = 1.f;
   const int32_t* past = nullptr;
   int length = 0, prompt = 0;
-  if (p.history && (rep != 1.f || presence != 0.f || frequency != 0.f)) {
-    const int slot = p.slot ? p.slot[r] : r;
-    if (slot >= p.slots) {
+  if (slot >= p.slots && slot >= 0) bad();
+  if (slot >= 0 && slot < p.slots && (rep != 1.f || presence != 0.f || frequency != 0.f)) {
+    length = p.length[slot];
+    prompt = p.prompt ? p.prompt[slot] : 0;
+    if (length < 0 || length > p.history_width) {
       bad();
-    } else if (slot >= 0) {
-      length = p.length[slot];
-      prompt = p.prompt ? p.prompt[slot] : 0;
-      if (length < 0 || length > p.history_width) {
-        bad();
-        length = 0;
-      }
-      past = p.history + slot * p.history_stride;
+      length = 0;
     }
+    past = p.history + slot * p.history_stride;
   }
-  int biases = 0, bias0 = 0;
-  if (p.bias_start) {
-    bias0 = p.bias_start[r];
-    biases = p.bias_start[r + 1] - bias0;
-    if (bias0 < 0 || biases < 0 || (int64_t)bias0 + biases > p.bias_count) {
-      bad();
-      biases = 0;
-    }
+  if (bias0 < 0 || biases < 0 || (int64_t)bias0 + biases > p.bias_count) {
+    bad();
+    biases = 0;
   }
-  const int32_t* words = nullptr;
-  if (p.mask) {
-    const int m = p.mask_row ? p.mask_row[r] : r;
-    if (m >= p.masks) bad();
-    else if (m >= 0) words = p.mask + m * p.mask_stride;
-  }
-  // (uniform over the CTA from here on)
-  if (length > 0) {
+  if (mask >= p.masks && mask >= 0) bad();
+  // the words of this thread's logits (one of each four neighbours, or of each one)
+  constexpr int kWords = kPer / 4;
+  const int32_t* words = mask >= 0 && mask < p.masks ? p.mask + mask * p.mask_stride : nullptr;
+  unsigned bits[kWords];
 #pragma unroll
-    for (int i = 0; i < kPer / 4; ++i) reinterpret_cast<uint4*>(count_s)[threadIdx.x + i * kThreads] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    each(past, length, [&](int t, int i) {
-      const unsigned j = (unsigned)t - (unsigned)lo;
-      if (j >= (unsigned)size) return;
-      if (i < prompt) atomicOr(&count_s[j], kSeen);
-      else atomicAdd(&count_s[j], 1u);
-    });
-    __syncthreads();
-  }
-  auto adjust = [&](float y, unsigned count, bool allowed) {
-    if (count) {
-      y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
-      const unsigned made = count & ~kSeen;
-      if (made) y = __fsub_rn(y, __fadd_rn(__fmul_rn(frequency, (float)made), presence));
-    }
-    return allowed ? y : -INFINITY;
-  };
+  for (int k = 0; k < kWords; ++k) bits[k] = words && vec && at(4 * k) < size ? (unsigned)words[(lo + at(4 * k)) >> 5] : ~0u;
+  // the lists' first tokens, for all of their passes
+  constexpr int kTokens = 8, kEntries = 2;
+  int token[kTokens], entry[kEntries];
+#pragma unroll
+  for (int k = 0; k < kTokens; ++k) token[k] = (int)threadIdx.x + k * kThreads < length ? past[threadIdx.x + k * kThreads] : -1;
+#pragma unroll
+  for (int k = 0; k < kEntries; ++k)
+    entry[k] = (int)threadIdx.x + k * kThreads < biases ? p.bias_token[bias0 + threadIdx.x + k * kThreads] : -1;
+  // the slice, masked
   if (vec) {
 #pragma unroll
     for (int k = 0; k < kPer; k += 4) {
       const int j = at(k);
       if (j >= size) break;
-      uint4 c = make_uint4(0, 0, 0, 0);
-      if (length > 0) c = *reinterpret_cast<const uint4*>(count_s + j);
-      const unsigned w = words ? (unsigned)words[(lo + j) >> 5] >> ((lo + j) & 31) : 0xfu;
-      if ((c.x | c.y | c.z | c.w) != 0 || (w & 0xfu) != 0xfu) {
-        v[k] = adjust(v[k], c.x, w & 1u);
-        v[k + 1] = adjust(v[k + 1], c.y, w & 2u);
-        v[k + 2] = adjust(v[k + 2], c.z, w & 4u);
-        v[k + 3] = adjust(v[k + 3], c.w, w & 8u);
+      const unsigned w = bits[k / 4] >> ((lo + j) & 31);
+      if ((w & 0xfu) != 0xfu) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+          if (!(w >> i & 1u)) v[k + i] = -INFINITY;
       }
       if (j + 3 < size) {
         *reinterpret_cast<float4*>(out + j) = make_float4(v[k], v[k + 1], v[k + 2], v[k + 3]);
@@ -162,28 +134,89 @@ __global__ void __launch_bounds__(kThreads, PER == 32 ? 4 : 8) adjust_kernel(con
     for (int k = 0; k < kPer; ++k) {
       const int j = at(k);
       if (j >= size) break;
-      const unsigned c = length > 0 ? count_s[j] : 0u;
-      const unsigned w = words ? (unsigned)words[(lo + j) >> 5] >> ((lo + j) & 31) : 1u;
-      out[j] = c || !(w & 1u) ? adjust(v[k], c, w & 1u) : v[k];
+      out[j] = words && !((unsigned)words[(lo + j) >> 5] >> ((lo + j) & 31) & 1u) ? -INFINITY : v[k];
     }
   }
-  if (biases == 0) return;
-  // f(index of the token in the slice, entry) for the row's entries in this slice
-  auto entries = [&](auto f) {
-    each(p.bias_token + bias0, biases, [&](int t, int i) {
+  // (length and biases are the same for the whole CTA)
+  if (length == 0 && biases == 0) return;
+  // f(place in the slice, index in the list) for the slice's tokens of a list, whose
+  // first ones are held
+  auto each = [&](const int32_t* list, int count, const auto& held, auto f) {
+    constexpr int N = sizeof(held) / sizeof(int) == 1 ? 0 : sizeof(held) / sizeof(int);  // (one: none)
+    auto one = [&](int t, int i) {
       const unsigned j = (unsigned)t - (unsigned)lo;
-      if (j < (unsigned)size) f(j, (unsigned)i);
-    });
+      if (j < (unsigned)size) f(j, i);
+    };
+#pragma unroll
+    for (int k = 0; k < N; ++k)
+      if ((int)threadIdx.x + k * kThreads < count) one(held[k], threadIdx.x + k * kThreads);
+#pragma unroll 4
+    for (int i = threadIdx.x + N * kThreads; i < count; i += kThreads) one(list[i], i);
   };
-  __syncthreads();
-  entries([&](unsigned j, unsigned) { count_s[j] = 0; });
-  __syncthreads();
-  entries([&](unsigned j, unsigned i) { atomicMax(&count_s[j], i + 1); });
-  __syncthreads();
-  entries([&](unsigned j, unsigned i) {
-    const bool allowed = !words || ((unsigned)words[(lo + j) >> 5] >> ((lo + j) & 31) & 1u);
-    if (count_s[j] == i + 1 && allowed) out[j] = __fadd_rn(out[j], p.bias_value[bias0 + i]);
-  });
+  auto allowed = [&](unsigned j) { return !words || ((unsigned)words[(lo + j) >> 5] >> ((lo + j) & 31) & 1u); };
+  if (length > 0) {
+    auto count = [&](unsigned j, bool in_prompt) {
+      if (in_prompt) atomicOr(&count_s[j], kSeen);
+      else atomicAdd(&count_s[j], 1u);
+    };
+    auto change = [&](unsigned j) {
+      const unsigned n = atomicExch(&count_s[j], 0u), made = n & ~kSeen;
+      if (n == 0 || !allowed(j)) return;
+      float y = out[j];
+      y = y > 0.f ? __fdiv_rn(y, rep) : __fmul_rn(y, rep);
+      if (made) y = __fsub_rn(y, __fadd_rn(__fmul_rn(frequency, (float)made), presence));
+      out[j] = y;
+    };
+    const int lane = threadIdx.x & 31;
+    auto note = [&](int t, int i) {
+      const unsigned j = (unsigned)t - (unsigned)lo;
+      const bool in = i < length && j < (unsigned)size;
+      const unsigned hits = __ballot_sync(0xffffffffu, in);
+      if (hits == 0) return;
+      int first = 0;
+      if (lane == 0) first = atomicAdd(&notes_s, __popc(hits));
+      first = __shfl_sync(0xffffffffu, first, 0) + __popc(hits & ((1u << lane) - 1));
+      if (in) {
+        count_s[j] = 0;
+        if (first < kNotes) note_s[first] = (uint16_t)(j | (i < prompt ? 0x8000u : 0u));
+      }
+    };
+#pragma unroll
+    for (int k = 0; k < kTokens; ++k) note(token[k], threadIdx.x + k * kThreads);
+#pragma unroll 1
+    for (int i0 = kTokens * kThreads; i0 < length; i0 += kTokens * kThreads) {
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) {
+        const int i = i0 + k * kThreads + (int)threadIdx.x;
+        token[k] = i < length ? past[i] : -1;
+      }
+#pragma unroll
+      for (int k = 0; k < kTokens; ++k) note(token[k], i0 + k * kThreads + (int)threadIdx.x);
+    }
+    __syncthreads();  // (the copies are out, too)
+    const int notes = notes_s;
+    if (notes <= kNotes) {
+      for (int n = threadIdx.x; n < notes; n += kThreads) count(note_s[n] & 0x7fffu, note_s[n] & 0x8000u);
+      __syncthreads();
+      for (int n = threadIdx.x; n < notes; n += kThreads) change(note_s[n] & 0x7fffu);
+    } else {  // through the history again
+      constexpr int none[1] = {-1};
+      each(past, length, none, [&](unsigned j, int i) { count(j, i < prompt); });
+      __syncthreads();
+      each(past, length, none, [&](unsigned j, int) { change(j); });
+    }
+  }
+  if (biases > 0) {
+    const int32_t* list = p.bias_token + bias0;
+    __syncthreads();
+    each(list, biases, entry, [&](unsigned j, int) { count_s[j] = 0; });
+    __syncthreads();
+    each(list, biases, entry, [&](unsigned j, int i) { atomicMax(&count_s[j], (unsigned)i + 1); });
+    __syncthreads();
+    each(list, biases, entry, [&](unsigned j, int i) {
+      if (count_s[j] == (unsigned)i + 1 && allowed(j)) out[j] = __fadd_rn(out[j], p.bias_value[bias0 + i]);
+    });
+  }
 }
 
 template <int PER>
