@@ -5,10 +5,10 @@
 // and then changes the logits of the slice's tokens in that (noted down in shared
 // memory as they come), each once, by whoever of their occurrences takes the count
 // (whole numbers: the order of the atomics does not matter); the last bias entry of
-// each token likewise.  Bound by
-// memory, 8 bytes a logit; the history is read by every slice of its row, mostly from
-// L2, so slices are as long as registers hold, unless a call has too few to fill the SMs
-// with.
+// each token likewise.  Bound by memory, 8 bytes a logit: 256 rows of 120,832 in 39 us
+// without histories (6.4 TB/s, the rate of a copy), 65 us with histories of 2,000
+// tokens, 40 biases and masks: every slice of a row goes through its history (from L2),
+// 14 us, and changes its tokens' logits, 8 us.
 #include <cuda_runtime.h>
 
 #include <algorithm>
