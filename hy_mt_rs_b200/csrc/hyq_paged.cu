@@ -31,7 +31,15 @@ struct AppendArgs {
   float* q_out;
   int64_t out_stride;
   bool vec;  // 8-bit: the codes of a row are 8-byte aligned
+  bool staged;  // the rows of q, k and v are 16-byte aligned
 };
+// Calls of more rows than append_rows_kernel holds at once (three CTAs an SM) stage
+// their rows in shared memory, of up to 64 KB.  Measured, 32 query and 8 kv heads of 128,
+// staged / not, int8 and f16 caches, us: 1 row 6.2 / 4.8 and 5.1 / 4.1, 256 rows 7.4 / 6.1
+// and 6.2 / 5.1, 512 rows 8.9 / 9.7 and 7.5 / 8.1, 8,208 rows 73 / 92 and 65 / 77; 8,208
+// rows of 14 and 2 heads of 64 24 / 41, of 64 and 8 of 128 136 / 146.
+constexpr int kStageMax = 64 * 1024;
+constexpr int kStagedRows = 3 * 148 + 1;
 
 template <Kv KV>
 __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
@@ -42,22 +50,40 @@ __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
 // One CTA per row of the activations, 16 lanes per head: lane l holds values
 // l, l + 16, ... of its head, so that the sum of squares runs in dot_x86's
 // order (one accumulator a lane, then the lane sum) and the two values of a
-// rotated pair meet in one thread: no value leaves its registers between the
-// load and the store.  Each group takes BATCH heads at a time, their loads in
-// flight together, and with those of the tables.  Bound by memory: 8,208 tokens
-// of 32 query and 8 kv heads of 128 into an f32 cache (403 MB) 84 us, 4.8 TB/s, in
-// accesses of 4 bytes a lane, 64 contiguous bytes of a head, with 35 % of the warps
-// (108 us with registers for six CTAs an SM instead of three); 64 tokens 3.6 us.
+// rotated pair meet in one thread.  Few rows are bound by latency (64 tokens 3.6 us):
+// each group takes BATCH heads at a time, their loads in flight together, and with
+// those of the tables.  Many rows (STAGED) come whole, by three bulk copies, while the
+// CTA finds their page and tables: the loads above are 4 bytes a lane, and three CTAs an
+// SM keep too few of them in flight, where eight CTAs of four warps have a row of 25 KB
+// each under way.  Bound by memory and by that search (row, page, tables, one after the
+// other): 8,208 tokens of 32 query and 8 kv heads of 128 into an f32 cache (403 MB)
+// 69 us, 5.8 TB/s, f16 65 us, int8 73 us (351 MB).
 // Into an 8-bit cache a head's largest magnitude comes from its 16 lanes, and the
 // codes go through shared memory, so that a lane writes neighbouring ones.
-template <int DIM, Kv KV>
-__global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant__ AppendArgs a) {
-  constexpr int EL = DIM / 16, BATCH = 3;
-  __shared__ __align__(8) uint8_t codes_s[is_8bit(KV) ? 256 : 8][is_8bit(KV) ? EL : 8];  // DIM of each group of 16 lanes
-  grid_dependency_wait();
-  allow_dependents_launch();
+template <int DIM, Kv KV, bool STAGED>
+__global__ void __launch_bounds__(STAGED ? 128 : 256, STAGED ? 8 : 3) append_rows_kernel(const __grid_constant__ AppendArgs a) {
+  constexpr int EL = DIM / 16, BATCH = STAGED ? 1 : 3, THREADS = STAGED ? 128 : 256, GROUPS = THREADS / 16;
+  __shared__ __align__(8) uint8_t codes_s[is_8bit(KV) ? THREADS : 8][is_8bit(KV) ? EL : 8];  // DIM of each group of 16 lanes
+  extern __shared__ __align__(16) float stage[];  // STAGED: the row's heads, queries, keys, values
+  __shared__ __align__(8) uint64_t bar_s;
   const int t = blockIdx.x, l = threadIdx.x & 15, part = threadIdx.x >> 4;
   const int units = a.heads + 2 * a.c.kv_heads;
+  if (STAGED && threadIdx.x == 0) {
+    mbar_init(smem_addr(&bar_s), 1);
+    mbar_fence_init();
+  }
+  grid_dependency_wait();
+  allow_dependents_launch();
+  if constexpr (STAGED) {
+    if (threadIdx.x == 0) {
+      const uint32_t bar = smem_addr(&bar_s), to = smem_addr(stage), qb = a.heads * DIM * 4, kb = a.c.kv_heads * DIM * 4;
+      mbar_arrive_expect_tx(bar, qb + 2 * kb);
+      bulk_g2s(to, a.q + t * a.q_stride, qb, bar);
+      bulk_g2s(to + qb, a.k + t * a.k_stride, kb, bar);
+      bulk_g2s(to + qb + kb, a.v + t * a.v_stride, kb, bar);
+    }
+    __syncthreads();
+  }
   auto source = [&](int u) {
     return u < a.heads                    ? a.q + t * a.q_stride + u * DIM
            : u < a.heads + a.c.kv_heads ? a.k + t * a.k_stride + (u - a.heads) * DIM
@@ -67,13 +93,13 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
   auto load = [&](int u0) {
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
-      const int u = u0 + 16 * b;
-      const float* src = source(u < units ? u : 0);
+      const int u = u0 + GROUPS * b;
+      const float* src = STAGED ? stage + (u < units ? u : 0) * DIM : source(u < units ? u : 0);
 #pragma unroll
       for (int i = 0; i < EL; ++i) x[b][i] = u < units ? src[l + 16 * i] : 0.f;
     }
   };
-  load(part);  // these do not wait for the tables
+  if (!STAGED) load(part);  // these do not wait for the tables
   float wq[EL], wk[EL];
 #pragma unroll
   for (int i = 0; i < EL; ++i) {
@@ -81,13 +107,16 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
     wk[i] = a.k_norm ? a.k_norm[l + 16 * i] : 1.f;
   }
   const int s = seq_of_row(a.c, t);
-  if (s < 0) return;
-  const Seq sq = load_seq(a.c, s);
-  if (t - sq.row0 >= sq.n) return;
+  const Seq sq = s < 0 ? Seq{} : load_seq(a.c, s);
   const int pos = sq.pos + (t - sq.row0);
-  const int page = checked_page(a.c, sq.pages[pos / a.c.page_size]);
-  if (page < 0 || pos >= a.positions) {
-    if (threadIdx.x == 0) atomicOr(a.c.status, DEV_BAD_ARGS);
+  int page = -1;
+  if (s >= 0 && t - sq.row0 < sq.n) {
+    page = checked_page(a.c, sq.pages[pos / a.c.page_size]);
+    if (pos >= a.positions) page = -1;
+    if (page < 0 && threadIdx.x == 0) atomicOr(a.c.status, DEV_BAD_ARGS);
+  }
+  if (page < 0) {
+    if (STAGED && threadIdx.x == 0 && !mbar_wait(smem_addr(&bar_s), 0, nullptr)) atomicOr(a.c.status, DEV_TIMEOUT_DRAIN);
     return;
   }
   float cs[EL / 2], sn[EL / 2];
@@ -98,11 +127,15 @@ __global__ void __launch_bounds__(256) append_rows_kernel(const __grid_constant_
   }
   const int64_t row = (int64_t)page * a.c.page_stride + (int64_t)(pos % a.c.page_size) * a.c.row_stride;
   const int64_t scales = is_8bit(KV) ? scale_at(a.c, page, 0, pos % a.c.page_size) : 0;
-  for (int u0 = part; u0 - part < units; u0 += 16 * BATCH) {
-    if (u0 != part) load(u0);
+  if (STAGED && !mbar_wait(smem_addr(&bar_s), 0, nullptr)) {
+    atomicOr(a.c.status, DEV_TIMEOUT_FULL);
+    return;
+  }
+  for (int u0 = part; u0 - part < units; u0 += GROUPS * BATCH) {
+    if (STAGED || u0 != part) load(u0);
 #pragma unroll
     for (int b = 0; b < BATCH; ++b) {
-      const int u = u0 + 16 * b;
+      const int u = u0 + GROUPS * b;
       if (u - part >= units) break;  // the same for the whole CTA
       const bool rotated = u < a.heads + a.c.kv_heads, is_q = u < a.heads;
       const float* w = is_q ? a.q_norm : a.k_norm;
@@ -482,7 +515,14 @@ cudaError_t launch_gather(const GatherArgs& a, bool f16, cudaStream_t st) {
 
 template <Kv KV>
 cudaError_t launch_append(const AppendArgs& a, cudaStream_t st) {
-  auto kern = a.c.dim == 128 ? append_rows_kernel<128, KV> : a.c.dim == 64 ? append_rows_kernel<64, KV> : append_kernel<KV>;
+  const int64_t bytes = (int64_t)(a.heads + 2 * a.c.kv_heads) * a.c.dim * 4;
+  if (a.staged && (a.c.dim == 128 || a.c.dim == 64) && bytes <= kStageMax && a.c.tokens >= kStagedRows) {
+    static std::atomic<uint64_t> set[2];
+    auto kern = a.c.dim == 128 ? append_rows_kernel<128, KV, true> : append_rows_kernel<64, KV, true>;
+    const cudaError_t e = allow_smem(kern, kStageMax, set[a.c.dim == 128]);
+    return e != cudaSuccess ? e : launch_ex(kern, dim3((unsigned)a.c.tokens), dim3(128), (size_t)bytes, st, a);
+  }
+  auto kern = a.c.dim == 128 ? append_rows_kernel<128, KV, false> : a.c.dim == 64 ? append_rows_kernel<64, KV, false> : append_kernel<KV>;
   return launch_ex(kern, dim3((unsigned)a.c.tokens), dim3(256), 0, st, a);
 }
 
@@ -603,6 +643,7 @@ int rope_append(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_page
   a.out_stride = out_stride;
   using namespace hyq::paged;
   a.vec = a.c.dim % 8 == 0 && ((a.c.page_stride | a.c.head_stride | a.c.row_stride) & 7) == 0 && aligned(a.c.k, 8) && aligned(a.c.v, 8);
+  a.staged = aligned(q, 16) && aligned(k, 16) && aligned(v, 16) && ((q_stride | k_stride | v_stride) & 3) == 0;
   const cudaStream_t st = (cudaStream_t)stream;
   switch (kv->dtype) {
     case kF32: return done(launch_append<kF32>(a, st), name);

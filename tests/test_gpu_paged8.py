@@ -156,6 +156,52 @@ def test_append_matches_the_f32_cache(cuda, heads, kvh, dim, page, norms, first,
     assert quant.device_status() == 0
 
 
+@pytest.mark.parametrize("kind", [*KINDS, "f16", "f32"])
+@pytest.mark.parametrize("heads,kvh,dim,first", [(16, 4, 128, False), (14, 2, 64, True), (3, 3, 64, False), (96, 16, 128, True), (104, 13, 128, False)])
+def test_append_of_many_rows(cuda, heads, kvh, dim, first, kind):
+    """Rows that come by bulk copies, rows that cannot (4 bytes off) and, the last
+    ones, rows too long for it: the same, a call's few rows as its many; rows behind the
+    last sequence, and behind the tables, are left; in place too."""
+    import torch
+    from hy_mt_rs_b200 import quant
+    new, ctx = [300, 1, 0, 150], [17, 40, 3, 0]
+    s = _append_inputs(cuda, new, ctx, heads, kvh, dim, 32, seed=heads)
+    t = sum(new)
+    pad = lambda x: torch.cat([x, torch.full_like(x[:5], math.nan)])  # noqa: E731
+    s["q"], s["new_k"], s["new_v"] = (pad(s[n]) for n in ("q", "new_k", "new_v"))
+
+    def run(off, lo=0, hi=len(new), out=None):
+        c = dict(s)
+        for n in ("q", "new_k", "new_v"):
+            x = torch.empty(s[n].numel() + off, device=cuda)[off:].view(s[n].shape)
+            c[n] = x.copy_(s[n])
+        if kind in KINDS:
+            k, v, scales = _pages8(cuda, s["k"], kind)
+        else:
+            k, v = (torch.full(s["k"].shape, 7.0, dtype=torch.float16 if kind == "f16" else torch.float32, device=cuda) for _ in range(2))
+            scales = {}
+        q = torch.full_like(c["q"], 7.0) if out is None else c["q"]
+        if lo or hi < len(new):  # these sequences' rows alone
+            a, b = s["starts"][lo], s["starts"][hi] if hi < len(new) else t
+            c.update({n: c[n][a:b] for n in ("q", "new_k", "new_v")}, table=s["table"][s["slots"][lo:hi]].contiguous(),
+                     row_start=s["row_start"][lo:hi + 1] - a, pos=s["pos"][lo:hi])
+            q = q[a:b]
+        _append(c, k, v, True, first, out=q, **scales)
+        return [q, *(x.view(torch.uint8) for x in (k, v)), *scales.values()]
+
+    many, off, inplace = run(0), run(1), run(0, out=True)
+    assert (many[0][t:] == 7.0).all() and inplace[0][t:].isnan().all()
+    assert torch.equal(inplace[0][:t], many[0][:t])
+    for a, b in zip(many, off):
+        assert torch.equal(a, b)
+    few = run(0, 3, 4)
+    assert torch.equal(few[0], many[0][s["starts"][3]:t])
+    held = s["table"][s["slots"][3], :-(-150 // 32)].long()
+    for a, b in zip(many[1:], few[1:]):
+        assert torch.equal(a[held], b[held])
+    assert quant.device_status() == 0
+
+
 @pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim", [128, 64, 80])
 def test_append_rows_that_are_not_finite(cuda, dim, kind):
