@@ -35,9 +35,9 @@ struct AppendArgs {
 };
 // Calls of more rows than append_rows_kernel holds at once (three CTAs an SM) stage
 // their rows in shared memory, of up to 64 KB.  Measured, 32 query and 8 kv heads of 128,
-// staged / not, int8 and f16 caches, us: 1 row 6.2 / 4.8 and 5.1 / 4.1, 256 rows 7.4 / 6.1
-// and 6.2 / 5.1, 512 rows 8.9 / 9.7 and 7.5 / 8.1, 8,208 rows 73 / 92 and 65 / 77; 8,208
-// rows of 14 and 2 heads of 64 24 / 41, of 64 and 8 of 128 136 / 146.
+// staged / not, f16 cache, us: 1 row 5.1 / 4.1, 256 rows 6.2 / 5.1, 512 rows 7.5 / 8.1,
+// 8,208 rows 65 / 77 (int8, with some more to do: 512 rows 10.3 / 11.0, 8,208 rows 77 / 98);
+// 8,208 rows of 14 and 2 heads of 64 24 / 41, of 64 and 8 of 128 (int8) 138 / 152.
 constexpr int kStageMax = 64 * 1024;
 constexpr int kStagedRows = 3 * 148 + 1;
 
@@ -57,7 +57,7 @@ __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
 // SM keep too few of them in flight, where eight CTAs of four warps have a row of 25 KB
 // each under way.  Bound by memory and by that search (row, page, tables, one after the
 // other): 8,208 tokens of 32 query and 8 kv heads of 128 into an f32 cache (403 MB)
-// 69 us, 5.8 TB/s, f16 65 us, int8 73 us (351 MB).
+// 69 us, 5.8 TB/s, f16 65 us, e4m3 74 us (353 MB).
 // Into an 8-bit cache a head's largest magnitude comes from its 16 lanes, and the
 // codes go through shared memory, so that a lane writes neighbouring ones.
 template <int DIM, Kv KV, bool STAGED>
@@ -128,9 +128,13 @@ __global__ void __launch_bounds__(STAGED ? 128 : 256, STAGED ? 8 : 3) append_row
   const int64_t row = (int64_t)page * a.c.page_stride + (int64_t)(pos % a.c.page_size) * a.c.row_stride;
   const int64_t scales = is_8bit(KV) ? scale_at(a.c, page, 0, pos % a.c.page_size) : 0;
   if (STAGED && !mbar_wait(smem_addr(&bar_s), 0, nullptr)) {
-    atomicOr(a.c.status, DEV_TIMEOUT_FULL);
+    if (threadIdx.x == 0) {  // (not before the copies are in, if that can be)
+      atomicOr(a.c.status, DEV_TIMEOUT_FULL);
+      if (!mbar_wait(smem_addr(&bar_s), 0, nullptr)) atomicOr(a.c.status, DEV_TIMEOUT_DRAIN);
+    }
     return;
   }
+  uint32_t again = 0;  // turns of this warp with codes that f32 leaves open (31: and later ones)
   for (int u0 = part; u0 - part < units; u0 += GROUPS * BATCH) {
     if (STAGED || u0 != part) load(u0);
 #pragma unroll
@@ -161,20 +165,30 @@ __global__ void __launch_bounds__(STAGED ? 128 : 256, STAGED ? 8 : 3) append_row
       }
       if (!a.norm_first) norm();
       uint32_t top = 0;
-      if constexpr (is_8bit(KV)) {
+      const bool coded = is_8bit(KV) && u - (part & 1) + 1 >= a.heads;  // one of the warp's two heads
+      if (coded) {
 #pragma unroll
         for (int i = 0; i < EL; ++i) top = max(top, __float_as_uint(x[b][i]) & 0x7fffffffu);
 #pragma unroll
         for (int o = 8; o > 0; o >>= 1) top = max(top, __shfl_xor_sync(0xffffffffu, top, o));
       }
-      if (is_8bit(KV)) __syncwarp();  // the codes of the heads before are out
-      const RowCode code = is_8bit(KV) ? row_code<KV>(top) : RowCode{};
-      if constexpr (is_8bit(KV)) {
+      if (coded) __syncwarp();  // the codes of the heads before are out
+      RowCode code{};
+      if constexpr (is_8bit(KV)) if (coded) {
+        code = row_code<KV>(top);
         uint8_t* mine = codes_s[threadIdx.x & ~15];
+        bool close = false;
         if (!is_q && u < units) {
+          float edge = KV == kI8 ? 0.f : INFINITY;
+          uint8_t codes[EL];
 #pragma unroll
-          for (int i = 0; i < EL; ++i) mine[l + 16 * i] = encode<KV>(x[b][i], code.inverse);
+          for (int i = 0; i < EL; ++i) codes[i] = encode<KV>(__fmul_rn(x[b][i], code.inverse), edge);
+#pragma unroll
+          for (int i = 0; i < EL; ++i) mine[l + 16 * i] = code.inverse == 0.f ? 0 : codes[i];
+          close = code.inverse != 0.f && near_border<KV>(edge, rotated);
         }
+        const int turn = min((u - part) / GROUPS, 31);
+        if (__any_sync(0xffffffffu, close)) again |= 1u << turn;
         __syncwarp();
       }
       if (u >= units) continue;
@@ -204,6 +218,40 @@ __global__ void __launch_bounds__(STAGED ? 128 : 256, STAGED ? 8 : 3) append_row
       }
     }
   }
+  // Those codes in 64 bits, without the row's norm, which they do not depend on.  (After
+  // the others, when the registers are free: amid them 87 us where this took 80.)
+  if constexpr (is_8bit(KV)) {
+    if (!again) return;
+    __syncwarp();  // the codes and scales from above are written
+    for (int turn = 0; turn * GROUPS < units; ++turn) {
+      if (!(again >> min(turn, 31) & 1)) continue;
+      const int u = part + GROUPS * turn, kh = (u - a.heads) % a.c.kv_heads;
+      const bool coded = u >= a.heads && u < units, key = u < a.heads + a.c.kv_heads;
+      const float* src = (STAGED ? stage + (coded ? u : 0) * DIM : source(coded ? u : 0)) + l;
+      double y[EL], largest = 0;
+#pragma unroll
+      for (int i = 0; i < EL; ++i) y[i] = src[16 * i];
+      if (key) {
+#pragma unroll
+        for (int i = 0; i < EL / 2; ++i) {
+          const double w0 = wk[i], w1 = wk[i + EL / 2], c = cs[i], n = sn[i];
+          const double x0 = a.norm_first ? y[i] * w0 : y[i], x1 = a.norm_first ? y[i + EL / 2] * w1 : y[i + EL / 2];
+          y[i] = x0 * c - x1 * n;
+          y[i + EL / 2] = x0 * n + x1 * c;
+          if (!a.norm_first) y[i] *= w0, y[i + EL / 2] *= w1;
+        }
+      }
+#pragma unroll
+      for (int i = 0; i < EL; ++i) largest = fmax(largest, fabs(y[i]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) largest = fmax(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+      if (!coded || !((key ? a.c.k_scale : a.c.v_scale)[scales + kh * a.c.scale_head_stride] > 0.f)) continue;  // 0, NaN: codes are 0
+      uint8_t* to = static_cast<uint8_t*>(key ? a.c.k : a.c.v) + row + kh * a.c.head_stride + l;
+      const double inverse = kLargest<KV> / largest;
+#pragma unroll
+      for (int i = 0; i < EL; ++i) to[16 * i] = encode<KV>(y[i] * inverse);
+    }
+  }
 }
 
 // Any other even head size: a warp per head at a time, the head in
@@ -228,12 +276,19 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
   const float* cs = a.cos_tab + (int64_t)pos * half;
   const float* sn = a.sin_tab + (int64_t)pos * half;
   const int64_t row = (int64_t)page * a.c.page_stride + (int64_t)(pos % a.c.page_size) * a.c.row_stride;
-  // a head's values into an 8-bit cache
-  auto quantise = [&](const float* x, void* base, float* scale_base, int kh) {
+  // a head's values into an 8-bit cache: x in f32, value(i) in 64 bits up to a factor
+  auto quantise = [&](const float* x, auto value, void* base, float* scale_base, int kh) {
     uint32_t top = 0;
-    for (int i = lane; i < dim; i += 32) top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+    double largest = 0;
+    for (int i = lane; i < dim; i += 32) {
+      top = max(top, __float_as_uint(x[i]) & 0x7fffffffu);
+      largest = fmax(largest, fabs(value(i)));
+    }
     const RowCode code = row_code<KV>(__reduce_max_sync(0xffffffffu, top));
-    for (int i = lane; i < dim; i += 32) static_cast<uint8_t*>(base)[row + kh * a.c.head_stride + i] = encode<KV>(x[i], code.inverse);
+    for (int o = 16; o > 0; o >>= 1) largest = fmax(largest, __shfl_xor_sync(0xffffffffu, largest, o));
+    const double inverse = kLargest<KV> / largest;
+    for (int i = lane; i < dim; i += 32)
+      static_cast<uint8_t*>(base)[row + kh * a.c.head_stride + i] = code.inverse == 0.f ? 0 : encode<KV>(value(i) * inverse);
     if (lane == 0) scale_base[scale_at(a.c, page, kh, pos % a.c.page_size)] = code.scale;
   };
   for (int u = warp; u < a.heads + 2 * a.c.kv_heads; u += 8) {
@@ -241,7 +296,7 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
       const int kh = u - a.heads - a.c.kv_heads;
       const float* x = a.v + t * a.v_stride + kh * dim;
       if constexpr (is_8bit(KV)) {
-        quantise(x, a.c.v, a.c.v_scale, kh);
+        quantise(x, [&](int i) { return (double)x[i]; }, a.c.v, a.c.v_scale, kh);
       } else {
         for (int i = lane; i < dim; i += 32) store_kv<KV>(a.c.v, row + kh * a.c.head_stride + i, x[i]);
       }
@@ -271,7 +326,16 @@ __global__ void __launch_bounds__(256) append_kernel(const __grid_constant__ App
       __syncwarp();
     }
     if (is_8bit(KV) && !is_q) {
-      if constexpr (is_8bit(KV)) quantise(h, a.c.k, a.c.k_scale, kh);
+      if constexpr (is_8bit(KV)) {
+        auto value = [&](int i) {
+          const int j = i < half ? i : i - half;
+          const double w0 = w && a.norm_first ? w[j] : 1.f, w1 = w && a.norm_first ? w[j + half] : 1.f;
+          const double x0 = x[j] * w0, x1 = x[j + half] * w1;
+          const double y = i < half ? x0 * cs[j] - x1 * sn[j] : x0 * sn[j] + x1 * cs[j];
+          return w && !a.norm_first ? y * w[i] : y;
+        };
+        quantise(h, value, a.c.k, a.c.k_scale, kh);
+      }
       continue;
     }
     for (int i = lane; i < dim; i += 32) {

@@ -130,19 +130,48 @@ struct RowCode {
   float scale, inverse;
 };
 template <Kv KV>
+constexpr double kLargest = KV == kI8 ? 127.0 : 448.0;  // code
+template <Kv KV>
 __device__ __forceinline__ RowCode row_code(uint32_t top) {
-  constexpr float largest = KV == kI8 ? 127.f : 448.f;
+  constexpr float largest = (float)kLargest<KV>;
   if (top >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.f};
   if (top < (127u - 90u) << 23) return {0.f, 0.f};
   const float x = __uint_as_float(top);
   return {__fdiv_rn(x, largest), __fdiv_rn(largest, x)};
 }
-// Code of x in a row with this inverse: the nearest to their product, ties to even.
+// Code of y, a value of magnitude kLargest (1 + 2^-22) at most in a row's unit: the
+// nearest, ties to even; and how near the border between two codes is: how far y is
+// from its code's value (int8), from the border (e4m3, whose numbers below 2^-6 are as
+// far apart as those above).
 template <Kv KV>
-__device__ __forceinline__ uint8_t encode(float x, float inverse) {
-  const float y = inverse == 0.f ? 0.f : __fmul_rn(x, inverse);
-  if constexpr (KV == kI8) return (uint8_t)(int8_t)max(-127, min(127, __float2int_rn(y)));
-  return (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+__device__ __forceinline__ uint8_t encode(float y, float& edge) {
+  if constexpr (KV == kI8) {
+    const float t = __fadd_rn(y, 12582912.f);  // 1.5 * 2^23: the whole number in the low bits
+    edge = fmaxf(edge, fabsf(y - __fsub_rn(t, 12582912.f)));
+    return (uint8_t)__float_as_uint(t);
+  } else {
+    const float z = fmaf(fabsf(y) < 0.015625f ? 1.f : 0.f, 0.015625f, fabsf(y));
+    edge = fminf(edge, fabsf(z - __uint_as_float((__float_as_uint(z) & 0xfff00000u) | 0x80000u)));
+    return (uint8_t)__nv_cvt_float_to_fp8(y, __NV_SATFINITE, __NV_E4M3);
+  }
+}
+// Whether a border is as near as f32 arithmetic may have moved y over it.  From a row as
+// it came, in units of 2^-24 of its largest magnitude: norm (two roundings), rotation
+// (two more; 4 in all of a pair's length, which is at most sqrt(2) times that magnitude:
+// 5.7), the magnitude itself as much, its quotient and the product 2; 13.4 * 2^-24 * 127
+// (448) < 2^-13 (2^-11), without norm and rotation 2 * 2^-24 * 127 < 2^-16 (2^-14).
+template <Kv KV>
+__device__ __forceinline__ bool near_border(float edge, bool rotated) {
+  if constexpr (KV == kI8) return edge > 0.5f - (rotated ? 1.f / 8192 : 1.f / 65536);
+  else return edge < (rotated ? 1.f / 2048 : 1.f / 16384);
+}
+// The code in 64 bits, y off by less than 2^-44: int8's is rounded to 2^-40 first and
+// e4m3's to f32, so that what lies on a border goes to the even side.  (No quotient
+// x * 127 / top of f32 numbers is nearer to a border than 2^-26 and not on it.)
+template <Kv KV>
+__device__ __forceinline__ uint8_t encode(double y) {
+  if constexpr (KV == kI8) return (uint8_t)(int8_t)max(-127, min(127, __double2int_rn(__dsub_rn(__dadd_rn(y, 6144.0), 6144.0))));
+  else return (uint8_t)__nv_cvt_float_to_fp8((float)y, __NV_SATFINITE, __NV_E4M3);
 }
 
 // A tile of `rows` of a sequence's (token, query head) rows of one kv head.

@@ -514,9 +514,10 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
  * k_scale or v_scale; a value is code * scale.  (For the other types the scales
  * are not read.)
  * Appending sets scale = the row's largest magnitude / 127 (int8) or / 448
- * (e4m3), and each code to the one nearest to value * (127 or 448 / that
- * magnitude), ties to even, each step in f32; a row of magnitudes below 2^-90 has
- * scale and codes 0.  A row with an infinity or NaN has codes 0 and a NaN scale:
+ * (e4m3), in f32, and each code to the one nearest to value * (127 or 448 / that
+ * magnitude), ties to even, of the rotated and normalised keys and the values as they
+ * are before any rounding to f32 (in 64 bits, where f32 leaves it open; e4m3 by way of
+ * the nearest f32); a row of magnitudes below 2^-90 has scale and codes 0.  A row with an infinity or NaN has codes 0 and a NaN scale:
  * it reads back as NaN throughout.  Attention makes NaN of rows
  * that see such a position, and of no others.  The codes 0x7f and 0xff of e4m3,
  * which appending does not write, count as +-480. */
@@ -531,7 +532,8 @@ typedef struct hyq_paged_kv8 {
 
 /* hyq_paged_rope_append and hyq_paged_attention over such a cache.  The queries
  * that come out are hyq_paged_rope_append's, bit for bit; attention has f32
- * accuracy over the values that the codes stand for. */
+ * accuracy over the values that the codes stand for.  (Rows of v whose scale is below
+ * 2^-100 may count as zeros; sums of values from about 2^106 on may overflow.) */
 int hyq_paged_rope_append_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
                               int heads, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                               const float* cos_tab, const float* sin_tab, int64_t positions, const float* q_norm,

@@ -28,16 +28,18 @@ def _values(codes, scale):
     return x * scale.double()[..., None]
 
 
-def _quantise(x, kind):
-    """Codes and scales of rows of f32 values, by the documented rule, on the CPU."""
+def _quantise(x, kind, exact=None):
+    """Codes and scales of rows of f32 values, by the documented rule, on the CPU.
+    exact: what they are before their roundings to f32, up to a factor of the row."""
     import torch
     dtype, largest = _types()[kind]
     x = x.cpu()
     top = x.abs().amax(-1)
     top = torch.where(top < 2.0 ** -90, 0.0, top)
     scale = top / largest
-    y = x * torch.where(top > 0, largest / top, 0.0)[..., None]
-    codes = y.round().clamp(-127, 127).to(dtype) if kind == "i8" else y.to(dtype)
+    y = x.double() if exact is None else exact.cpu()
+    y = y * largest / y.abs().amax(-1, keepdim=True).clamp(min=1e-300)
+    codes = y.round().clamp(-127, 127).to(dtype) if kind == "i8" else y.float().to(dtype)
     bad = ~torch.isfinite(x).all(-1)
     scale[bad] = math.nan
     codes.view(torch.uint8)[bad | (top == 0)] = 0    # (not -0)
@@ -115,6 +117,16 @@ def _append(s, k_pages, v_pages, norms=True, first=False, **scales):
                              s["sin"], *w, 1e-5, first, **scales)
 
 
+def _exact_keys(s, t, p, norms, first):
+    """Row t's keys at position p in 64 bits, up to each head's norm."""
+    import torch
+    x, w = s["new_k"][t].double(), s["k_norm"].double() if norms else 1.0
+    a, b = (x * w if first else x).chunk(2, -1)
+    c, n = s["cos"][p].double(), s["sin"][p].double()
+    y = torch.cat([a * c - b * n, a * n + b * c], -1)
+    return (y if first else y * w).cpu()
+
+
 def _pages8(dev, like, kind, layout="hnd"):
     """Empty 8-bit pages of a shape: codes 3 and scales -1, to see what is written."""
     import torch
@@ -133,8 +145,8 @@ def _pages8(dev, like, kind, layout="hnd"):
 @pytest.mark.parametrize("norms,first", [(False, False), (True, False), (True, True)])
 @pytest.mark.parametrize("heads,kvh,dim,page", [(16, 4, 128, 64), (8, 8, 64, 16), (6, 2, 80, 7), (3, 1, 6, 5), (4, 2, 256, 32)])
 def test_append_matches_the_f32_cache(cuda, heads, kvh, dim, page, norms, first, layout, kind):
-    """Queries bit for bit; codes and scales those of the f32 cache's rows; nothing
-    else written."""
+    """Queries bit for bit; scales those of the f32 cache's rows, codes those of the rows
+    in 64 bits; nothing else written."""
     import torch
     from hy_mt_rs_b200 import quant
     s = _append_inputs(cuda, [1, 0, 37, 2], [0, 9, 63, 130], heads, kvh, dim, page, seed=dim)
@@ -146,14 +158,61 @@ def test_append_matches_the_f32_cache(cuda, heads, kvh, dim, page, norms, first,
     k8, v8, scales = _pages8(cuda, k32, kind, layout)
     q8 = _append(s, k8, v8, norms, first, **scales)
     assert torch.equal(q8, q32)
-    for x, codes, scale in ((k32, k8, scales["k_scale"]), (v32, v8, scales["v_scale"])):
-        want, want_scale = _quantise(x, kind)
+    exact = k32.double().cpu()
+    for i, n in enumerate(s["new"]):
+        for j in range(n):
+            p, t = s["ctx"][i] + j, s["starts"][i] + j
+            exact[int(s["table"][s["slots"][i], p // page]), :, p % page] = _exact_keys(s, t, p, norms, first)
+    for x, y, codes, scale in ((k32, exact, k8, scales["k_scale"]), (v32, None, v8, scales["v_scale"])):
+        want, want_scale = _quantise(x, kind, y)
         written = (x != 777.0).any(-1).cpu() | (x == 0).all(-1).cpu()
         assert torch.equal(scale.cpu()[written], want_scale[written])
         assert torch.equal(codes.view(torch.uint8).cpu()[written], want.view(torch.uint8)[written])
         assert (codes.view(torch.uint8).cpu()[~written] == 3).all() and (scale.cpu()[~written] == -1).all()
     assert int((scales["k_scale"] != -1).sum()) == sum(s["new"]) * kvh
     assert quant.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim,tokens", [(128, 40), (128, 4000), (64, 4000), (80, 40)])
+def test_append_next_to_borders_between_codes(cuda, dim, tokens, kind):
+    """Values a few f32 steps from a border between two codes fall on their own side;
+    keys too, which f32 arithmetic moves by more than that."""
+    import torch
+    s = _append_inputs(cuda, [tokens], [0], 2, 2, dim, 64, seed=dim + tokens, positions=tokens)
+    g = torch.Generator(device=cuda).manual_seed(4)
+    top = 1 + torch.rand(tokens, 2, 1, generator=g, device=cuda, dtype=torch.float64)
+    if kind == "i8":
+        border = torch.randint(-127, 127, (tokens, 2, dim), generator=g, device=cuda) + 0.5
+    else:
+        codes = torch.randint(0, 126, (tokens, 2, dim), generator=g, device=cuda).to(torch.uint8)
+        up = [c.view(torch.float8_e4m3fn).double() for c in (codes, codes + 1)]
+        border = (up[0] + up[1]) / 2 * (2 * torch.randint(0, 2, codes.shape, generator=g, device=cuda) - 1)
+    x = (border * top / _types()[kind][1]).float()
+    x = x.view(torch.int32).add(torch.randint(-2, 3, x.shape, generator=g, device=cuda, dtype=torch.int32)).view(torch.float32)
+    x[..., 5] = top[..., 0].float()
+    s["new_v"] = x
+    # keys that the rotation takes next to borders
+    c, n = (s[t][:, None].double() for t in ("cos", "sin"))
+    a, b = (border * top / _types()[kind][1]).chunk(2, -1)
+    s["new_k"] = torch.cat([a * c + b * n, b * c - a * n], -1).float()
+    k8, v8, scales = _pages8(cuda, s["k"], kind)
+    k32, v32 = (torch.full_like(s[t], 777.0) for t in ("k", "v"))
+    _append(s, k32, v32, False)
+    _append(s, k8, v8, False, **scales)
+    pages = s["table"][0, :-(-tokens // 64)].long()
+    rows = lambda t: t[pages].transpose(1, 2).reshape(-1, 2, *t.shape[3:])[:tokens].cpu()  # noqa: E731
+    c, n, k = (t.cpu() for t in (c, n, s["new_k"].double()))
+    a, b = k.chunk(2, -1)
+    exact = torch.cat([a * c - b * n, a * n + b * c], -1)
+    off = 0
+    for x, y, codes, scale in ((rows(k32), exact, k8, "k_scale"), (rows(v32), None, v8, "v_scale")):
+        want, want_scale = _quantise(x, kind, y)
+        assert torch.equal(rows(scales[scale]), want_scale)
+        assert torch.equal(rows(codes.view(torch.uint8)), want.view(torch.uint8))
+        y = x * (_types()[kind][1] / x.abs().amax(-1))[..., None]   # f32 all the way takes the wrong side of some
+        off += int(((y.round() if kind == "i8" else y.to(want.dtype).float()) != want.float()).sum())
+    assert off > 0
 
 
 @pytest.mark.parametrize("kind", [*KINDS, "f16", "f32"])
