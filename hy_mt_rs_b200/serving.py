@@ -189,6 +189,8 @@ class PagedBatch:
             raise ValueError(f"{used} answers need as many slots, there are {self.slots}")
         if max(len(p) for p in prompts) + n_new > self.m.cfg.positions:
             raise ValueError("prompt + generated tokens exceed the rotary tables")
+        if mask is not None and mask.shape[0] not in (1, len(prompts)):
+            raise ValueError(f"{mask.shape[0]} masks for {len(prompts)} prompts")
         random = torch.Generator(device=dev).manual_seed(seed)
         prompt_ids = self._ints(*prompts)
         fed = [0] * len(prompts)

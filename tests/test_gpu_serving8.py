@@ -155,3 +155,14 @@ def test_generate_with_adjusted_logits(cuda):
                     assert abs(y[got[i][0][step]] - y[best]) <= 2e-3 * np.linalg.norm(y[np.isfinite(y)])
                     break
                 made.append(best)
+
+
+def test_generate_wants_a_mask_for_all_or_for_each_prompt(cuda):
+    import torch
+    from hy_mt_rs_b200.serving import PagedBatch
+    model = _model(cuda, "dense", True)
+    batch = PagedBatch(model, 3, page_size=32)
+    words = torch.full((2, (model.cfg.vocab + 31) // 32), -1, dtype=torch.int32, device=cuda)
+    with pytest.raises(ValueError, match="2 masks for 3 prompts"):
+        batch.generate([[1], [2], [3]], 2, mask=words)
+    assert batch.generate([[1], [2]], 2, mask=words) == batch.generate([[1], [2]], 2)
