@@ -16,6 +16,12 @@
 // and 4 kv heads of 128, f16, 269 MB) 54 us, 5.0 TB/s; 4 of 60,000 to 100,000
 // (32 and 8 heads, 1.3 GB) 205 to 215 us, 6.1 to 6.4 TB/s; one of 512 positions (f32) 10.4 to 11.1 us,
 // all latency: the plan of the line, the copies, the partial results' join.
+// Over 8-bit caches (half the bytes) the same kernel is bound by its instructions'
+// latencies: the 64 requests 54 us (139 MB, 2.6 TB/s), the four long ones 166 us (e4m3,
+// 677 MB, 4.1 TB/s) at 58 % of the issue slots, 10.7 warps an SM and half of the
+// instructions on the integer pipe (1,240 for 32 positions, of them 450 to take e4m3
+// codes to f16).  Sixteen positions at a time and four CTAs an SM instead of 32 and
+// three: 186 us (registers spill at 128 a thread).
 // Chunks, bound by the products and by each CTA's own walk over the positions:
 // 200 tokens at 0 21 us, 8 sequences of 40 at 100 20 us (f16); longer ones go to
 // the kernels on tcgen05.

@@ -31,6 +31,11 @@
 // Tensor memory: S / P and X of both row tiles, 128 columns each: all 512.
 // X is not accumulated there over the tiles: the tensor cores cut their sums,
 // which over 1,000 steps would cost 1e-5.
+//
+// PREFIX: the segments are groups' tokens over their shared prefix, few rows over many
+// positions: one row tile a segment, whose position tiles the two softmax groups take
+// in turn (their halves meet through tensor memory at the end), and five slots in the
+// ring, in the place of the other row tile's queries.
 #include <cuda.h>
 #include <cudaTypedefs.h>
 
