@@ -80,8 +80,9 @@ def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None,
     queries q [tokens, heads, head_dim] over the pages, which hold the new
     tokens' keys and values already; [tokens, heads, head_dim] (into `out`
     when given).  max_new and max_len bound any sequence's new tokens and its
-    length after them (max_len: the table's reach by default).  workspace:
-    attention_workspace(...), made here when not given."""
+    length after them (max_len: the table's reach by default).  k_scale and
+    v_scale: those of 8-bit pages.  workspace: attention_workspace(...), made
+    here when not given."""
     if workspace is None:
         if not isinstance(q, torch.Tensor) or q.dim() != 3:
             raise HyqError(-2, "q: expected [tokens, heads, head_dim] with contiguous heads")
