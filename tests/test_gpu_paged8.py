@@ -262,6 +262,37 @@ def test_append_of_many_rows(cuda, heads, kvh, dim, first, kind):
 
 
 @pytest.mark.parametrize("kind", KINDS)
+def test_append_of_many_rows_captured_and_replayed(cuda, kind):
+    """Beside another stream's call of its own, and with rows that are not finite."""
+    import torch
+    s, o = (_append_inputs(cuda, [500, 40], [3, 30], 16, 4, 128, 32, seed=i, positions=600) for i in (1, 2))
+    out = [torch.zeros_like(s["q"]) for _ in range(3)]
+    pages = [_pages8(cuda, s["k"], kind) for _ in range(3)]
+    calls = [lambda i=i, c=c: _append(c, *pages[i][:2], out=out[i], **pages[i][2]) for i, c in enumerate((s, o, s))]
+    stream, other = torch.cuda.Stream(), torch.cuda.Stream()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph, stream=stream):
+        calls[0]()
+    for turn in range(2):
+        s["q"].normal_()
+        s["new_v"].normal_()
+        if turn:
+            s["new_k"][7, 1, 3], s["new_v"][450, 0, 0] = math.inf, math.nan
+        torch.cuda.synchronize()
+        graph.replay()
+        with torch.cuda.stream(other):
+            calls[1]()
+        torch.cuda.synchronize()
+        calls[2]()
+        both = [[out[i], *(t.view(torch.uint8) for t in pages[i][:2]), *pages[i][2].values()] for i in (0, 2)]
+        for a, b in zip(*both):
+            assert torch.equal(a.nan_to_num(-7.0), b.nan_to_num(-7.0)) if a.is_floating_point() else torch.equal(a, b)
+        for name in ("k_scale", "v_scale"):
+            assert int(pages[0][2][name].isnan().sum()) == turn
+
+
+@pytest.mark.parametrize("kind", KINDS)
 @pytest.mark.parametrize("dim", [128, 64, 80])
 def test_append_rows_that_are_not_finite(cuda, dim, kind):
     """Codes 0 and a NaN scale; other rows as they would be."""
