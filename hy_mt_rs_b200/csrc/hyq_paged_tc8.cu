@@ -466,9 +466,18 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
                      : "l"(o), "l"(row));
       }
     };
+    // A warp whose wait ran out does nothing more, raises the abort flag, which ends the
+    // others' waits, and goes on to the next tile's barrier, where all four leave: none
+    // may be left waiting there for it.
+    auto waited = [&](uint32_t bar, uint32_t parity) {
+      if (ok && !warp_wait(bar, parity, abort_flag)) {
+        ok = false;
+        *abort_flag = 1;
+      }
+    };
     auto take = [&]() {  // the ring's next slot
       const int slot = issued % kSlots;
-      ok = issued < kSlots || warp_wait(empty(slot), ((issued / kSlots) - 1) & 1, abort_flag);
+      if (issued >= kSlots) waited(empty(slot), ((issued / kSlots) - 1) & 1);
       ++issued;
       return slot;
     };
@@ -509,12 +518,14 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
       const bool bad = __any_sync(0xffffffffu, held && !isfinite(vs));
       if (lane == 0) top_s[(i & 1) * 4 + lw] = make_uint2(most, bad ? 0u : least);
       const int k_slot = take();
-      if (!ok) break;
       // (V of tile i - 2 was there, whose products followed that tile's softmax)
+      if (ok) {
 #pragma unroll
-      for (int r = 0; r < IT; ++r) put(k_slot, r, kr[r].x, kr[r].y, kr[r].z, kr[r].w);
-      fence_proxy_async_smem();
-      asm volatile("bar.sync 1, 128;" ::: "memory");
+        for (int r = 0; r < IT; ++r) put(k_slot, r, kr[r].x, kr[r].y, kr[r].z, kr[r].w);
+        fence_proxy_async_smem();
+      }
+      ok = bar_red_and(1, 128, ok);
+      if (!ok) break;
       uint32_t top = 0, low = 0x7f800000u;
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
@@ -533,8 +544,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         // (here the ring alone does not say that the softmax of tile i - 2, whose scales
         // these replace, is done: its V's products do)
         ask();
-        if (ok && i >= 2) ok = warp_wait(empty((2 * i - 3) % kSlots), ((2 * i - 3) / kSlots) & 1, abort_flag);
-        if (!ok) break;
+        if (i >= 2) waited(empty((2 * i - 3) % kSlots), ((2 * i - 3) / kSlots) & 1);
+        if (!ok) continue;
       }
       // the unit: above the largest scale (a tile of zeros keeps the one before)
       if (top) lift = min(max((int)(top >> 23) - 126, -100), 100);
@@ -552,7 +563,7 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
       }
       if constexpr (!PREFIX) {
         ask();
-        if (!ok) break;
+        if (!ok) continue;
       }
       if (i + 1 < tiles) {
         if (++j == x.nt) {
