@@ -23,6 +23,11 @@ namespace logits {
 
 constexpr int kThreads = 256;
 constexpr unsigned kSeen = 0x80000000u;       // of a count: the token stands in the prompt
+// Entries of a row's history and of the bias lists: the loops over them look up to this
+// many past the last, in 32 bits.
+constexpr int kPastEnd = 65536;
+constexpr int64_t kMostEntries = INT32_MAX - kPastEnd;
+static_assert(kPastEnd >= 16 * kThreads, "eight entries of each thread at a time, four turns unrolled");
 
 struct Args {
   const float* x;
@@ -243,10 +248,10 @@ extern "C" int hyq_logits_adjust(const float* logits, int64_t n, int64_t stride,
   if (!logits || !out || (p.history && !p.length) || (!p.history && (p.repetition || p.presence || p.frequency)) ||
       (p.bias_start && (!p.bias_token || !p.bias_value)))
     return hyq::api_fail(HYQ_E_INVALID, "%s: null pointer", name);
-  if (p.history && (p.slots <= 0 || p.slots > INT32_MAX || p.history_width < 0 || p.history_width > INT32_MAX ||
+  if (p.history && (p.slots <= 0 || p.slots > INT32_MAX || p.history_width < 0 || p.history_width > kMostEntries ||
                     p.history_stride < p.history_width || (!p.slot && rows > p.slots)))
     return hyq::api_fail(HYQ_E_SHAPE, "%s: shape of the history", name);
-  if (p.bias_start && (p.bias_count < 0 || p.bias_count > INT32_MAX)) return hyq::api_fail(HYQ_E_SHAPE, "%s: number of biases", name);
+  if (p.bias_start && (p.bias_count < 0 || p.bias_count > kMostEntries)) return hyq::api_fail(HYQ_E_SHAPE, "%s: number of biases", name);
   if (p.mask && (p.masks <= 0 || p.masks > INT32_MAX || p.mask_stride < (n + 31) / 32 || (!p.mask_row && rows > p.masks)))
     return hyq::api_fail(HYQ_E_SHAPE, "%s: shape of the mask", name);
   if (logits == out && stride != out_stride) return hyq::api_fail(HYQ_E_SHAPE, "%s: in place with two strides", name);

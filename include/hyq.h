@@ -665,7 +665,7 @@ int hyq_sample(const float* logits, int64_t n, int64_t stride, int64_t rows, con
  * needs a history).  Tokens that are none of the n are skipped.  NaN stays NaN.
  * A slot or mask row past the last, a length outside 0 .. history_width and
  * bias entries outside 0 .. bias_count - 1 leave that part out for the row and
- * raise HYQ_DEV_BAD_ARGS. */
+ * raise HYQ_DEV_BAD_ARGS.  history_width and bias_count end 65536 below 2^31. */
 typedef struct hyq_adjust {
   const int32_t* history;
   int64_t slots, history_width, history_stride;

@@ -20,3 +20,12 @@ def test_rows_of_a_sample_fit_a_grid():
     from hy_mt_rs_b200._native import lib
     for rows in (2 ** 31 - 1, 2 ** 28):
         assert lib.hyq_sample(PTR, 100, 100, rows, None, None, None, None, PTR, PTR, None, None) == SHAPE
+
+
+def test_entries_of_histories_and_biases_end_below_2_to_the_31():
+    """The adjust kernel's loops over a row's history and biases count in 32 bits, some
+    turns past the last entry."""
+    from test_paged8_refusals import _adjust
+    for n in (2 ** 31 - 1, 2 ** 31 - 2048, 2 ** 31 - 65536):
+        assert _adjust(width=n, history_stride=n) == SHAPE
+        assert _adjust(bias_count=n) == SHAPE
