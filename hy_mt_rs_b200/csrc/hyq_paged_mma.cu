@@ -520,7 +520,10 @@ template <Kv KV>
 cudaError_t few(const AttendArgs& a, int64_t rows, bool beside, cudaStream_t st) {
   if constexpr (is_8bit(KV)) {
     const int group = a.heads / a.c.kv_heads;
-    const int shares = group > 8 ? 1 : std::max(1, ((int)rows / group + 8 / group - 1) / (8 / group));  // 3 at most
+    // Shares of a sequence with more than eight rows, 3 at most: as many as 16 rows need,
+    // whatever max_new says (one with more tokens than that would lose its last ones).
+    // None where max_new fits eight rows: such a sequence is reported then.
+    const int shares = rows <= 8 || group > 8 ? 1 : (kRows / group + 8 / group - 1) / (8 / group);
     if (group <= 8)
       return a.c.dim == 128 ? few<128, KV, 1>(a, shares, beside, st) : few<64, KV, 1>(a, shares, beside, st);
   }

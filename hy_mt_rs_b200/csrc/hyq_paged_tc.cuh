@@ -86,7 +86,8 @@ __device__ __forceinline__ int seen_tiles(const Seq& s, int group, int tile, int
 // for each segment (its queries in, its results out, a start of the pipeline).
 // PREFIX: the segments are those of the groups' prefixes, and each sequence's and
 // each token's prefix is written down; a group whose prefix some sequence of it does
-// not hold (DEV_BAD_ARGS), or that is a single sequence, has none.
+// not hold, or that has one with more new tokens than max_new (DEV_BAD_ARGS both), or
+// that is a single sequence, has none.
 template <int ROWS, bool PREFIX>
 __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ AttendArgs a, const __grid_constant__ Plan plan) {
   grid_dependency_wait();
@@ -145,14 +146,14 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
           const int slot = a.c.slot ? a.c.slot[i] : i;
           if (in && off_s[lo] > 0 &&
               (a.c.row_start[i + 1] - a.c.row_start[i] != s.n || slot < 0 || slot >= a.c.slots || s.pos < off_s[lo] ||
-               (int64_t)s.pos + s.n > (int64_t)a.c.width * a.c.page_size || s.n * group > kFewRows)) {
+               (int64_t)s.pos + s.n > (int64_t)a.c.width * a.c.page_size || s.n > g.max_new)) {
             atomicOr(a.c.status, DEV_BAD_ARGS);
             atomicExch(&off_s[lo], 0);
           }
         } else {
           const int p = in ? off_s[lo] : 0;
           g.first[i] = p;
-          if (s.n * group > kFewRows) atomicOr(a.c.status, DEV_BAD_ARGS);  // max_new was too small: nobody takes it
+          if (s.n > g.max_new) atomicOr(a.c.status, DEV_BAD_ARGS);  // the kernel of own positions may not take it, and does not tell
         }
       }
       __syncthreads();

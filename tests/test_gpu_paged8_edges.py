@@ -1,0 +1,77 @@
+"""Attention over 8-bit caches and of shared prefixes at their edges: a max_new that
+is too small, workspaces of used memory, overlapped launches."""
+import math
+
+import pytest
+
+from test_gpu_paged import _int, _reference
+from test_gpu_paged8 import KINDS, _attend, _make8
+from test_gpu_shared import _attend as _attend_shared
+from test_gpu_shared import _make as _make_shared
+
+pytestmark = pytest.mark.gpu
+
+
+def _bound(s):
+    """test_gpu_paged8._close's reference and bound."""
+    import torch
+    ref, tol = _reference(s)
+    heads = s["q"].shape[1]
+    group = heads // s["k"].shape[1]
+    for i, (n, c) in enumerate(zip(s["new"], s["ctx"])):
+        a = s["starts"][i]
+        held = s["table"][s["slots"][i], :-(-(n + c) // s["page"])].long()
+        for h in range(heads if n and s["kv"] else 0):
+            k, v = (s[x][held, h // group].double().reshape(-1, s["q"].shape[2])[:n + c] for x in ("k", "v"))
+            x = s["q"][a:a + n, h].double() @ k.T / math.sqrt(s["q"].shape[2])
+            hide = torch.arange(n + c, device=x.device)[None] > torch.arange(c, n + c, device=x.device)[:, None]
+            p = torch.softmax(x.masked_fill(hide, -math.inf), -1)
+            tol[a:a + n, h] += 2.0 ** -18 * (p @ v.abs().amax(-1))[:, None]
+    return ref, tol
+
+
+def _right_or_left(got, s, ref, tol, fill, status):
+    """Every sequence's rows within their bound; or left alone, and reported."""
+    import torch
+    for i, n in enumerate(s["new"]):
+        rows = slice(s["starts"][i], s["starts"][i] + n)
+        if torch.equal(got[rows], torch.full_like(got[rows], fill)) and n:
+            assert status == 8, i
+        else:
+            err = (got[rows].double() - ref[rows]).abs()
+            assert (err <= tol[rows]).all(), (i, float((err / tol[rows]).max()))
+
+
+# ------------------------------------------------------------------- max_new
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("heads,kvh,max_new,new", [(6, 2, 3, [5, 1]), (6, 2, 4, [5, 2]), (10, 2, 2, [3, 1, 2]), (8, 2, 1, [3, 1]),
+                                                   (8, 2, 2, [4, 1]), (3, 3, 9, [16, 2]), (14, 2, 1, [2, 1]), (8, 2, 2, [40, 1])])
+def test_more_tokens_than_max_new(cuda, heads, kvh, max_new, new, kind):
+    """A sequence with more new tokens than max_new is taken whole, or left alone and
+    reported; the others are right."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant
+    s = _make8(cuda, new, [50, 300, 20][:len(new)], heads, kvh, 128, 16, kind, seed=heads)
+    out = torch.full_like(s["q"], 7.0)
+    paged.attention(s["q"], s["k_pages"], s["v_pages"], s["table"], s["row_start"], s["pos"], max_new, out=out, **s["kv"])
+    _right_or_left(out, s, *_bound(s), 7.0, quant.device_status())
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", *KINDS])
+@pytest.mark.parametrize("heads,kvh,max_new,new", [(8, 2, 1, [1, 3, 1]), (8, 2, 2, [1, 4, 2]), (6, 2, 3, [5, 1, 2]), (8, 2, 1, [1, 1, 7])])
+def test_more_tokens_than_max_new_behind_a_prefix(cuda, heads, kvh, max_new, new, kind):
+    """Likewise of a group, next to a group without such a sequence; never outputs made
+    of what the workspace held; reported in any case."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant
+    s = _make_shared(cuda, [(150, [(9 + i, n) for i, n in enumerate(new)]), (200, [(0, 1), (31, 1)])], heads, kvh, 128, 32, kind, seed=4)
+    t = s["q"].shape[0]
+    ws = paged.attention_shared_workspace(heads, 128, t, cuda)
+    ws[4096:] = torch.full((ws.numel() // 4,), 1.0, device=cuda).view(torch.uint8)[:ws.numel() - 4096]
+    out = torch.full_like(s["q"], 7.0)
+    paged.attention_shared(s["q"], s["k_pages"], s["v_pages"], s["table"], s["row_start"], s["pos"], s["group_start"], s["shared"],
+                           max_new, out=out, workspace=ws, **s["kv"])
+    status = quant.device_status()
+    assert status == 8
+    _right_or_left(out, s, *_bound(s), 7.0, status)
+    assert (out[sum(new):] != 7.0).all()
