@@ -83,7 +83,10 @@ __device__ __forceinline__ float high(uint64_t a) { return __uint_as_float((uint
 // scores_to_weights() over codes: the columns' scores are times ks[c], and the
 // weights times vs[c], up to 1, V's scales in the tile's unit 2^lift.  A weight is
 // 2^(s + lift - m) before that, and l the sum of 2^(s - m): the reference follows what
-// the stored products can be at most, over all tiles, whatever their units.
+// the stored products can be at most, over all tiles, whatever their units.  So it may
+// rise by the units alone, and what there is so far counts all the same: outputs and
+// sum go down by 2^(before - m) however far that is.  (In f32 they reach zero 2^126
+// further down: see the header on scales that far apart.)
 __device__ __forceinline__ void code_scores_to_weights(uint32_t st, bool first, bool masked, int unseen_from, float factor, float& m,
                                                        float& l, float& down, const float* ks, const float* vs, float lift) {
   // the scores of columns c .. c + 31, and the largest
@@ -131,15 +134,12 @@ __device__ __forceinline__ void code_scores_to_weights(uint32_t st, bool first, 
     uint64_t u[16];
     const float top = fmaf(scores(u, c), factor, lift), over = top - m - kBias;
     if (__any_sync(0xffffffffu, over > kSlack)) {
-      // raise the reference, by whole powers of two where what there is so far
-      // still counts; what this tile has so far follows
+      // raise the reference, by whole powers of two unless it is far (or the first
+      // above -inf); what this tile has so far follows
       float f = 1.f;
-      if (over > 64.f) {
-        f = 0.f;
-        m = reference(top);
-      } else if (over > kSlack) {
+      if (over > kSlack) {
         const float before = m;
-        m = fmaxf(m + ceilf(over), reference(top));
+        m = over > 64.f ? reference(top) : fmaxf(m + ceilf(over), reference(top));
         f = ex2(before - m);
       }
       back = (m == -INFINITY ? 0.f : -m) + lift;

@@ -1,5 +1,5 @@
 """Attention over 8-bit caches and of shared prefixes at their edges: a max_new that
-is too small, workspaces of used memory, overlapped launches."""
+is too small, tiles of far units, workspaces of used memory, overlapped launches."""
 import math
 
 import pytest
@@ -75,3 +75,53 @@ def test_more_tokens_than_max_new_behind_a_prefix(cuda, heads, kvh, max_new, new
     assert status == 8
     _right_or_left(out, s, *_bound(s), 7.0, status)
     assert (out[sum(new):] != 7.0).all()
+
+
+# -------------------------------------------------------------- units of tiles
+def _scaled(s, factor):
+    """The values with V's scales times factor(positions) of every sequence."""
+    import torch
+    from test_gpu_paged8 import _values
+    scale = s["kv"]["v_scale"]
+    times = torch.ones_like(scale)
+    for i, (n, c) in enumerate(zip(s["new"], s["ctx"])):
+        p = torch.arange(n + c, device=scale.device)
+        times[s["table"][s["slots"][i]][(p // s["page"]).long()].long(), :, p % s["page"]] = factor(p).float()[:, None]
+    scale *= times
+    s["v"] = _values(s["v_pages"], scale)
+    return s
+
+
+UNITS = [(2.0 ** -70, 1.0), (1.0, 2.0 ** -70), (2.0 ** -30, 2.0 ** 70), (2.0 ** 50, 2.0 ** -50), (2.0 ** -20, 2.0 ** -12)]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("first,then", UNITS)
+@pytest.mark.parametrize("new,ctx", [([200, 1], [700, 300]), ([1, 3], [900, 400])])
+def test_tiles_of_far_units(cuda, new, ctx, first, then, dim, kind):
+    """Whole tiles of 128 positions whose scales of V are alike, far from those of the
+    next tiles: their positions keep their weights, whatever their values' size."""
+    import torch
+    s = _make8(cuda, new, ctx, 16, 4, dim, 32, kind, seed=12, spread=0.1)
+    _scaled(s, lambda p: torch.where(p // 128 % 3 == 0, first, then))
+    _close_far(_attend(s), s)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("first,then", UNITS)
+def test_tiles_of_far_units_in_a_prefix(cuda, first, then, kind):
+    import torch
+    s = _make_shared(cuda, [(640, [(9, 1), (0, 2), (50, 1)]), (200, [(1, 1), (70, 2)])], 8, 2, 128, 32, kind, seed=6)
+    _scaled(s, lambda p: torch.where(p // 128 % 3 == 0, first, then))
+    _close_far(_attend_shared(s), s)
+
+
+def _close_far(got, s):
+    """Within the element-wise bound alone: outputs are sums of very different sizes."""
+    import torch
+    from hy_mt_rs_b200 import quant
+    ref, tol = _bound(s)
+    assert torch.isfinite(got).all() and quant.device_status() == 0
+    err = (got.double() - ref).abs()
+    assert (err <= tol).all(), float((err / tol).max())
