@@ -547,8 +547,11 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
         if (i >= 2) waited(empty((2 * i - 3) % kSlots), ((2 * i - 3) / kSlots) & 1);
         if (!ok) continue;
       }
-      // the unit: above the largest scale (a tile of zeros keeps the one before)
+      // the unit: above the largest scale (a tile of zeros keeps the one before, and the
+      // first of a piece takes 2^-60, as the few-token kernel's rows of zeros do: small
+      // values behind it keep their bits, whatever the piece before this one held)
       if (top) lift = min(max((int)(top >> 23) - 126, -100), 100);
+      else if (j == 0) lift = -60;
       const float unit = code_unit<KV>(), down = __uint_as_float((uint32_t)(127 - lift) << 23);
       k_scale_s[(i & 1) * kTile + pos_in] = ks * unit;
       v_scale_s[(i & 1) * kTile + pos_in] = isfinite(vs) ? vs * down : 0.f;

@@ -533,10 +533,10 @@ typedef struct hyq_paged_kv8 {
 /* hyq_paged_rope_append and hyq_paged_attention over such a cache.  The queries
  * that come out are hyq_paged_rope_append's, bit for bit; attention has f32
  * accuracy over the values that the codes stand for, where the scales of v that a
- * token sees lie within 2^110 of each other, and from 2^-75 to 2^50 if rows of zeros
- * are among them: beyond that small values, or their rows' weights, may be lost.  (Rows
- * of v whose scale is below 2^-100 may count as zeros in any case; sums of values from
- * about 2^106 on may overflow.) */
+ * token sees lie within 2^100 of each other, and from 2^-40 to 2^40 if rows of zeros are
+ * among them: beyond that small values, or the weights of their rows or of those of
+ * zeros, may be lost.  (Rows of v whose scale is below 2^-100 may count as zeros; sums
+ * of values from about 2^106 on may overflow.) */
 int hyq_paged_rope_append_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batch, const float* q, int64_t q_stride,
                               int heads, const float* k, int64_t k_stride, const float* v, int64_t v_stride,
                               const float* cos_tab, const float* sin_tab, int64_t positions, const float* q_norm,

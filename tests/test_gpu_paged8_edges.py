@@ -92,6 +92,11 @@ def _scaled(s, factor):
     return s
 
 
+def _where(condition, a, b):
+    import torch
+    return torch.where(condition, a, b)
+
+
 UNITS = [(2.0 ** -70, 1.0), (1.0, 2.0 ** -70), (2.0 ** -30, 2.0 ** 70), (2.0 ** 50, 2.0 ** -50), (2.0 ** -20, 2.0 ** -12)]
 
 
@@ -104,7 +109,7 @@ def test_tiles_of_far_units(cuda, new, ctx, first, then, dim, kind):
     next tiles: their positions keep their weights, whatever their values' size."""
     import torch
     s = _make8(cuda, new, ctx, 16, 4, dim, 32, kind, seed=12, spread=0.1)
-    _scaled(s, lambda p: torch.where(p // 128 % 3 == 0, first, then))
+    _scaled(s, lambda p: _where(p // 128 % 3 == 0, first, then))
     _close_far(_attend(s), s)
 
 
@@ -113,7 +118,7 @@ def test_tiles_of_far_units(cuda, new, ctx, first, then, dim, kind):
 def test_tiles_of_far_units_in_a_prefix(cuda, first, then, kind):
     import torch
     s = _make_shared(cuda, [(640, [(9, 1), (0, 2), (50, 1)]), (200, [(1, 1), (70, 2)])], 8, 2, 128, 32, kind, seed=6)
-    _scaled(s, lambda p: torch.where(p // 128 % 3 == 0, first, then))
+    _scaled(s, lambda p: _where(p // 128 % 3 == 0, first, then))
     _close_far(_attend_shared(s), s)
 
 
@@ -125,3 +130,44 @@ def _close_far(got, s):
     assert torch.isfinite(got).all() and quant.device_status() == 0
     err = (got.double() - ref).abs()
     assert (err <= tol).all(), float((err / tol).max())
+
+
+SIZES = [1.0, 2.0 ** -15, 2.0 ** -30, 2.0 ** 40]
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("new,ctx", [([200, 260], [700, 600]), ([1, 3], [900, 400])])
+def test_tiles_of_zeros_before_small_values(cuda, new, ctx, size, kind):
+    """Sequences that begin with positions whose values are zeros, the second one behind
+    one of large values: the values that follow keep their bits."""
+    from test_gpu_paged8 import _values
+    s = _make8(cuda, new, ctx, 16, 4, 128, 32, kind, seed=13, spread=0.1)
+    large = s["table"][s["slots"][0]].long()
+    large = large[large >= 0]
+    keep = s["kv"]["v_scale"][large].clone()
+    _scaled(s, lambda p: _where(p < 256, 0.0, size))
+    _close_far(_attend(s), s)
+    s["kv"]["v_scale"][large] = keep * 2.0 ** 60
+    s["v"] = _values(s["v_pages"], s["kv"]["v_scale"])
+    _close_far(_attend(s), s)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("new,ctx", [([200, 260], [700, 600]), ([1, 3], [900, 4000]), ([20], [150])])
+def test_rows_of_zeros_among_others(cuda, new, ctx, size, kind):
+    """Single positions without a value, and whole tiles of them, next to values: their
+    weights count."""
+    s = _make8(cuda, new, ctx, 8, 2, 128, 32, kind, seed=14, spread=0.1)
+    _scaled(s, lambda p: _where((p % 3 == 1) | (p // 128 % 2 == 0) & (p > 60), 0.0, size))
+    _close_far(_attend(s), s)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("size", SIZES)
+@pytest.mark.parametrize("first", [256, 0])
+def test_prefixes_with_rows_of_zeros(cuda, first, size, kind):
+    s = _make_shared(cuda, [(640, [(9, 1), (0, 2), (50, 1)]), (300, [(1, 1), (70, 2)])], 8, 2, 128, 32, kind, seed=7)
+    _scaled(s, lambda p: _where((p < first) | (p % 3 == 1) & (first == 0), 0.0, size))
+    _close_far(_attend_shared(s), s)
