@@ -64,6 +64,7 @@ template <int DIM, Kv KV, bool STAGED>
 __global__ void __launch_bounds__(STAGED ? 128 : 256, STAGED ? 8 : 3) append_rows_kernel(const __grid_constant__ AppendArgs a) {
   constexpr int EL = DIM / 16, BATCH = STAGED ? 1 : 3, THREADS = STAGED ? 128 : 256, GROUPS = THREADS / 16;
   __shared__ __align__(8) uint8_t codes_s[is_8bit(KV) ? THREADS : 8][is_8bit(KV) ? EL : 8];  // DIM of each group of 16 lanes
+  __shared__ float limit_s[is_8bit(KV) ? THREADS / 32 : 1];  // each warp's border_limit() of keys
   extern __shared__ __align__(16) float stage[];  // STAGED: the row's heads, queries, keys, values
   __shared__ __align__(8) uint64_t bar_s;
   const int t = blockIdx.x, l = threadIdx.x & 15, part = threadIdx.x >> 4;
@@ -105,6 +106,17 @@ __global__ void __launch_bounds__(STAGED ? 128 : 256, STAGED ? 8 : 3) append_row
   for (int i = 0; i < EL; ++i) {
     wq[i] = a.q_norm ? a.q_norm[l + 16 * i] : 1.f;
     wk[i] = a.k_norm ? a.k_norm[l + 16 * i] : 1.f;
+  }
+  if constexpr (is_8bit(KV)) {
+    float uneven = 1.f;  // the key weights' largest ratio in a rotated pair, where they come after
+    if (a.k_norm && !a.norm_first) {
+#pragma unroll
+      for (int i = 0; i < EL / 2; ++i) uneven = fmaxf(uneven, ratio_of(wk[i], wk[i + EL / 2]));
+#pragma unroll
+      for (int o = 8; o > 0; o >>= 1) uneven = fmaxf(uneven, __shfl_xor_sync(0xffffffffu, uneven, o));
+    }
+    if ((threadIdx.x & 31) == 0) limit_s[threadIdx.x >> 5] = border_limit<KV>(uneven);
+    __syncwarp();
   }
   const int s = seq_of_row(a.c, t);
   const Seq sq = s < 0 ? Seq{} : load_seq(a.c, s);
@@ -185,7 +197,7 @@ __global__ void __launch_bounds__(STAGED ? 128 : 256, STAGED ? 8 : 3) append_row
           for (int i = 0; i < EL; ++i) codes[i] = encode<KV>(__fmul_rn(x[b][i], code.inverse), edge);
 #pragma unroll
           for (int i = 0; i < EL; ++i) mine[l + 16 * i] = code.inverse == 0.f ? 0 : codes[i];
-          close = code.inverse != 0.f && near_border<KV>(edge, rotated);
+          close = code.inverse != 0.f && near_border<KV>(edge, rotated ? limit_s[threadIdx.x >> 5] : border_limit<KV>(kUnrotated));
         }
         const int turn = min((u - part) / GROUPS, 31);
         if (__any_sync(0xffffffffu, close)) again |= 1u << turn;

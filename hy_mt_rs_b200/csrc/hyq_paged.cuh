@@ -156,18 +156,32 @@ __device__ __forceinline__ uint8_t encode(float y, float& edge) {
   }
 }
 // Whether a border is as near as f32 arithmetic may have moved y over it.  From a row as
-// it came, in units of 2^-24 of its largest magnitude: norm (two roundings), rotation
-// (two more; 4 in all of a pair's length, which is at most sqrt(2) times that magnitude:
-// 5.7), the magnitude itself as much, its quotient and the product 2; 13.4 * 2^-24 * 127
-// (448) < 2^-13 (2^-11), without norm and rotation 2 * 2^-24 * 127 < 2^-16 (2^-14).
+// it came, in units of 2^-24 of its largest magnitude: rotation (two roundings of a
+// pair's length, which is at most sqrt(2) times that magnitude: 2.9), norm (two of the
+// value itself), the magnitude as much again, its quotient and the product 2: 11.7 *
+// 2^-24 * 127 (448) < 2^-13 (2^-11); without norm and rotation 2 * 2^-24 * 127 < 2^-16
+// (2^-14).  Where weights follow the rotation, a value's share of its pair's error goes
+// by its own weight, and the largest magnitude may be the other one's: with `uneven`,
+// the largest ratio of a pair's weights, 2.9 becomes 2.9 * uneven, and 11.7
+// 6 + 5.7 * uneven, which is less than (1 + uneven) / 2 of those limits.
 template <Kv KV>
-__device__ __forceinline__ bool near_border(float edge, bool rotated) {
-  if constexpr (KV == kI8) return edge > 0.5f - (rotated ? 1.f / 8192 : 1.f / 65536);
-  else return edge < (rotated ? 1.f / 2048 : 1.f / 16384);
+__device__ __forceinline__ constexpr float border_limit(float uneven) {
+  return (0.5f + 0.5f * uneven) / (KV == kI8 ? 8192 : 2048);
 }
-// The code in 64 bits, y off by less than 2^-44: int8's is rounded to 2^-40 first and
-// e4m3's to f32, so that what lies on a border goes to the even side.  (No quotient
-// x * 127 / top of f32 numbers is nearer to a border than 2^-26 and not on it.)
+constexpr float kUnrotated = -0.75f;  // (1 + this) / 2 is 1 / 8
+template <Kv KV>
+__device__ __forceinline__ bool near_border(float edge, float limit) {
+  return KV == kI8 ? edge > 0.5f - limit : edge < limit;
+}
+// The ratio of two weights, 1 at least (1 of zeros, whose products are exact).
+__device__ __forceinline__ float ratio_of(float a, float b) {
+  const float hi = fmaxf(fabsf(a), fabsf(b)), lo = fminf(fabsf(a), fabsf(b));
+  return hi == 0.f ? 1.f : 1.000001f * __fdividef(hi, lo);
+}
+// The code in 64 bits, y off by less than 2^-43 * uneven (e4m3: 2^-41): int8's is rounded
+// to 2^-40 first and e4m3's to f32, so that what lies on a border goes to the even side.
+// (No quotient x * 127 / top of f32 numbers is nearer to a border than 2^-32 and not on
+// it; a rotated key may be.)
 template <Kv KV>
 __device__ __forceinline__ uint8_t encode(double y) {
   if constexpr (KV == kI8) return (uint8_t)(int8_t)max(-127, min(127, __double2int_rn(__dsub_rn(__dadd_rn(y, 6144.0), 6144.0))));

@@ -516,8 +516,9 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
  * Appending sets scale = the row's largest magnitude / 127 (int8) or / 448
  * (e4m3), in f32, and each code to the one nearest to value * (127 or 448 / that
  * magnitude), ties to even, of the rotated and normalised keys and the values as they
- * are before any rounding to f32 (in 64 bits, where f32 leaves it open; e4m3 by way of
- * the nearest f32); a row of magnitudes below 2^-90 has scale and codes 0.  A row with an infinity or NaN has codes 0 and a NaN scale:
+ * are before any rounding to f32 (where f32 leaves it open, in 64-bit arithmetic rounded
+ * to 2^-40 of a step; e4m3 by way of the nearest f32); a row of magnitudes below 2^-90
+ * has scale and codes 0.  A row with an infinity or NaN has codes 0 and a NaN scale:
  * it reads back as NaN throughout.  Attention makes NaN of rows
  * that see such a position, and of no others.  The codes 0x7f and 0xff of e4m3,
  * which appending does not write, count as +-480. */

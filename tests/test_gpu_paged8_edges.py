@@ -1,5 +1,6 @@
 """Attention over 8-bit caches and of shared prefixes at their edges: a max_new that
-is too small, tiles of far units, workspaces of used memory, overlapped launches."""
+is too small, tiles of far units, keys under uneven weights, workspaces of used memory,
+overlapped launches."""
 import math
 
 import pytest
@@ -171,3 +172,77 @@ def test_prefixes_with_rows_of_zeros(cuda, first, size, kind):
     s = _make_shared(cuda, [(640, [(9, 1), (0, 2), (50, 1)]), (300, [(1, 1), (70, 2)])], 8, 2, 128, 32, kind, seed=7)
     _scaled(s, lambda p: _where((p < first) | (p % 3 == 1) & (first == 0), 0.0, size))
     _close_far(_attend_shared(s), s)
+
+
+# ------------------------------------------------------------------- append
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("ratio", [1, 20, 200, 1000])
+@pytest.mark.parametrize("first", [False, True])
+@pytest.mark.parametrize("dim,tokens", [(128, 40), (128, 8000), (64, 8000), (80, 40)])
+def test_keys_next_to_borders_under_uneven_weights(cuda, dim, tokens, first, ratio, kind):
+    """Heads with one value next to a border between two codes (the others lie on codes),
+    whose weight is `ratio` times its partner's in the rotation: f32 moves it by a share
+    of the pair.  All codes are those of 64 bits, where 2^-38 * ratio of a value does not
+    decide (the kernel's 64-bit roundings: 2^-43 * ratio of 127, then 2^-40)."""
+    import torch
+    from test_gpu_paged8 import _append, _append_inputs, _exact_keys, _pages8, _quantise, _types
+    s = _append_inputs(cuda, [tokens], [0], 2, 2, dim, 64, seed=dim + tokens, positions=tokens)
+    g = torch.Generator(device=cuda).manual_seed(5)
+    rand = lambda *n: torch.rand(*n, generator=g, device=cuda, dtype=torch.float64)  # noqa: E731
+    whole = lambda lo, hi, *n: torch.randint(lo, hi, n, generator=g, device=cuda)  # noqa: E731
+    half, largest = dim // 2, _types()[kind][1]
+    heavy = torch.arange(half, device=cuda) % 2 == 0
+    heavy = torch.cat([heavy, ~heavy])
+    s["k_norm"] = (torch.where(heavy, float(ratio), 1.0) * (1 + 0.1 * rand(dim))).float()
+    w, top = s["k_norm"].double(), 1 + rand(tokens, 2, 1)
+
+    def code(n):
+        return n.double() if kind == "i8" else n.to(torch.uint8).view(torch.float8_e4m3fn).double()
+
+    n = whole(0, 127, tokens, 2, dim)
+    z = code(n) * (2 * whole(0, 2, tokens, 2, dim) - 1)
+    at = whole(0, half // 2, tokens, 2, 1) * 2 + whole(0, 2, tokens, 2, 1) * (half + 1)      # a heavy one
+    n = whole(0, 126, tokens, 2, 1)
+    z.scatter_(2, at, (code(n) + code(n + 1)) / 2)
+    z.scatter_(2, (at + half) % dim, code(whole(112 if kind == "f8" else 64, 126, tokens, 2, 1)))
+    on_top = (at + 2) % half
+    z = z.scatter(2, on_top, torch.full_like(top, largest)) / largest * top
+    c, sn = (s[t][:tokens, None].double() for t in ("cos", "sin"))
+    a, b = (z if first else z / w).chunk(2, -1)
+    x = torch.cat([a * c + b * sn, b * c - a * sn], -1)
+    s["new_k"] = (x / w if first else x).float()
+    k8, v8, scales = _pages8(cuda, s["k"], kind)
+    k32, v32 = (torch.full_like(s[t], 777.0) for t in ("k", "v"))
+    _append(s, k32, v32, True, first)
+    _append(s, k8, v8, True, first, **scales)
+    pages = s["table"][0, :-(-tokens // 64)].long()
+    rows = lambda t: t[pages].transpose(1, 2).reshape(-1, 2, *t.shape[3:])[:tokens].cpu()  # noqa: E731
+    exact = torch.stack([_exact_keys(s, t, t, True, first) for t in range(tokens)])
+    got = rows(k8.view(torch.uint8))
+    wants = [_quantise(rows(k32), kind, exact)]
+    assert torch.equal(rows(scales["k_scale"]), wants[0][1])
+    # what the kernel's 64-bit roundings may move over a border
+    y = exact * largest / exact.abs().amax(-1, keepdim=True)
+    either = [(v.round().clamp(-127, 127).to(torch.int8) if kind == "i8" else v.float().to(torch.float8_e4m3fn)).view(torch.uint8)
+              for v in (y * (1 - 2.0 ** -38 * ratio), y * (1 + 2.0 ** -38 * ratio))]
+    wrong = (got != wants[0][0].view(torch.uint8)) & ((got == either[0]) == (got == either[1]))
+    assert not wrong.any(), int(wrong.sum())
+
+
+def test_weights_of_zero(cuda):
+    """A pair with one weight of zero, and one with two: its values are 0 or anything, and
+    the codes those of 64 bits."""
+    import torch
+    from test_gpu_paged8 import _append, _append_inputs, _exact_keys, _pages8, _quantise
+    for tokens in (40, 1000):
+        s = _append_inputs(cuda, [tokens], [0], 2, 2, 128, 64, seed=tokens, positions=tokens)
+        s["k_norm"][[3, 7, 71]] = 0.0
+        k8, v8, scales = _pages8(cuda, s["k"], "i8")
+        k32, v32 = (torch.full_like(s[t], 777.0) for t in ("k", "v"))
+        _append(s, k32, v32, True, False)
+        _append(s, k8, v8, True, False, **scales)
+        pages = s["table"][0, :-(-tokens // 64)].long()
+        rows = lambda t: t[pages].transpose(1, 2).reshape(-1, 2, *t.shape[3:])[:tokens].cpu()  # noqa: E731
+        exact = torch.stack([_exact_keys(s, t, t, True, False) for t in range(tokens)])
+        want, want_scale = _quantise(rows(k32), "i8", exact)
+        assert torch.equal(rows(scales["k_scale"]), want_scale) and torch.equal(rows(k8), want)
