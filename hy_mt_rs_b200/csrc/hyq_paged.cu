@@ -740,6 +740,7 @@ int attend_args(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_page
   if (!q || !out || !workspace) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
   const int64_t qw = (int64_t)heads * kv->head_dim;
   if (q_stride < qw || out_stride < qw) return api_fail(HYQ_E_SHAPE, "%s: shape of the activations", name);
+  if (q == out && q_stride != out_stride) return api_fail(HYQ_E_SHAPE, "%s: in place with two strides", name);
   if (!aligned(q, 4) || !aligned(out, 4) || !aligned(workspace, 16))
     return api_fail(HYQ_E_ALIGN, "%s: alignment of q, out or the workspace", name);
   a.q = q;

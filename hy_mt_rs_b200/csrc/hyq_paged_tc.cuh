@@ -255,7 +255,9 @@ inline cudaError_t launch_beside(const AttendArgs& a, Kv kv, cudaStream_t st) {
   own.out = a.groups.out;
   own.out_stride = a.groups.out_stride;
   own.ml = a.groups.ml;
-  return launch_few(own, kv, a.groups.max_new, true, st);
+  // (in place: its outputs are written where the prefixes' kernel reads queries, so it
+  // comes after that)
+  return launch_few(own, kv, a.groups.max_new, own.out != own.q, st);
 }
 
 // What a CTA does of a segment.

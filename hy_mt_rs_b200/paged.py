@@ -79,7 +79,7 @@ def attention(q, k_pages, v_pages, table, row_start, pos, max_new, max_len=None,
     """hyq_paged_attention: causal grouped-query attention of the rotated
     queries q [tokens, heads, head_dim] over the pages, which hold the new
     tokens' keys and values already; [tokens, heads, head_dim] (into `out`
-    when given).  max_new and max_len bound any sequence's new tokens and its
+    when given; q itself is allowed).  max_new and max_len bound any sequence's new tokens and its
     length after them (max_len: the table's reach by default).  k_scale and
     v_scale: those of 8-bit pages.  workspace: attention_workspace(...), made
     here when not given."""

@@ -488,7 +488,8 @@ int hyq_paged_rope_append(const hyq_paged_kv* kv, const hyq_paged_batch* batch, 
 /* Causal grouped-query attention of the new tokens over the pages
  * (attention_into, model.rs:949-1021): the token at position p of sequence s
  * sees the sequence's positions 0 ..= p, whose keys and values must be in the
- * pages already.  out [tokens, heads, head_dim], rows out_stride floats apart.
+ * pages already.  out [tokens, heads, head_dim], rows out_stride floats apart; q
+ * itself is allowed, with its stride.
  * f32 accuracy over either cache type.  Keys and values past a token's position
  * (page tails, later tokens of its chunk) never reach its output, whatever they
  * hold.  Every weight counts as above zero: an infinity in a value that a token

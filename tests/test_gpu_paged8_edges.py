@@ -246,3 +246,47 @@ def test_weights_of_zero(cuda):
         exact = torch.stack([_exact_keys(s, t, t, True, False) for t in range(tokens)])
         want, want_scale = _quantise(rows(k32), "i8", exact)
         assert torch.equal(rows(scales["k_scale"]), want_scale) and torch.equal(rows(k8), want)
+
+
+# ----------------------------------------------------------------- in place
+@pytest.mark.parametrize("kind", ["f32", "f16", *KINDS])
+@pytest.mark.parametrize("dim", [128, 80])
+@pytest.mark.parametrize("new,ctx", [([1, 3, 2], [900, 40, 5000]), ([200, 1, 70], [700, 300, 9]), ([40, 1], [20, 5])])
+def test_in_place(cuda, new, ctx, dim, kind):
+    """Outputs in the queries' place: the same bits."""
+    import torch
+    from test_gpu_paged import _make
+    if kind in KINDS:
+        s = _make8(cuda, new, ctx, 8, 2, dim, 32, kind, seed=21)
+    else:
+        s = _make(cuda, new, ctx, 8, 2, dim, 32, kind == "f16", seed=21)
+        s.update(kv={}, k_pages=s["k"], v_pages=s["v"])
+    want, wide = _attend(s), torch.full((sum(new), 11, dim), 3.0, device=cuda)
+    wide[:, :8] = s["q"]
+    s["q"] = wide[:, :8]
+    _attend(s, out=s["q"])
+    assert torch.equal(s["q"], want) and (wide[:, 8:] == 3).all()
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", *KINDS])
+@pytest.mark.parametrize("per", [2, 70])
+def test_in_place_behind_a_prefix(cuda, per, kind):
+    """A sequence's own positions are done long before its group's prefix: queries are
+    read by that first."""
+    import torch
+    s = _make_shared(cuda, [(6000, [((i * 37) % 20, 1) for i in range(per)]), (200, [(0, 1), (31, 2)])], 16, 4, 128, 64, kind, seed=22)
+    want, q = _attend_shared(s), s["q"].clone()
+    for _ in range(5):
+        s["q"] = q.clone()
+        _attend_shared(s, out=s["q"])
+        assert torch.equal(s["q"], want)
+
+
+def test_in_place_wants_the_queries_stride(cuda):
+    import torch
+    from hy_mt_rs_b200._native import HyqError
+    s = _make8(cuda, [1, 3], [90, 40], 8, 2, 128, 32, "i8", seed=21)
+    buf = torch.zeros(4 * 11 * 128, device=cuda)
+    s["q"] = buf.view(4, 11, 128)[:, :8]
+    with pytest.raises(HyqError, match="in place with two strides"):
+        _attend(s, out=buf[:4 * 8 * 128].view(4, 8, 128))
