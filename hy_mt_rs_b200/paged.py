@@ -143,6 +143,7 @@ class PagedCache:
     (nothing changed; a reserve's positions are -1, which rope_append and
     attention skip).  `changes` counts the calls that changed lengths."""
 
+    @torch.inference_mode(False)    # tensors that count their changes, wherever the cache is made
     def __init__(self, layers, kv_heads, head_dim, pages, page_size, slots, table_width, device, dtype=torch.float16):
         z = lambda *n: torch.zeros(*n, dtype=torch.int32, device=device)  # noqa: E731
         if dtype in _CODES:

@@ -182,6 +182,16 @@ class PagedBatch:
         the prompt and the answer so far; bias: {token: value}; mask [1 or prompts,
         (vocab + 31) // 32] (int32): the tokens that all requests, or each
         prompt's, may take (sampling.adjust states the rules)."""
+        try:
+            return self._generate(prompts, n_new, answers, (temperature, top_k, top_p, min_p), seed,
+                                  dict(repetition=repetition, presence=presence, frequency=frequency), bias, mask)
+        except BaseException:
+            # a step or fork may have lacked pages: what is known of lengths, and of what
+            # forks share, is read again
+            self._held_at = None
+            raise
+
+    def _generate(self, prompts, n_new, answers, filters, seed, penalties, bias, mask):
         dev, used = self.m.device, len(prompts) * answers
         if not prompts or min(len(p) for p in prompts) < 1 or answers < 1 or n_new < 1:
             raise ValueError("at least one prompt token, answer and new token")
@@ -200,7 +210,6 @@ class PagedBatch:
         short = torch.zeros(1, dtype=torch.int32, device=dev)
         self.cache.free(self._ints(range(self.slots))[0])
         self._known([0] * self.slots)
-        penalties = dict(repetition=repetition, presence=presence, frequency=frequency)
         history = None
         if any(p is not None for p in penalties.values()):
             history = torch.full((self.slots, self.m.cfg.positions), -1, dtype=torch.int32, device=dev)
@@ -252,8 +261,7 @@ class PagedBatch:
                 if mask is not None:
                     more.update(mask=mask, mask_row=slot // answers if mask.shape[0] > 1 else torch.zeros_like(slot))
                 sampling.adjust(picked, **more, out=picked)
-            token, _ = sampling.sample(picked, torch.rand(len(sources), generator=random, device=dev), temperature, top_k, top_p,
-                                       min_p)
+            token, _ = sampling.sample(picked, torch.rand(len(sources), generator=random, device=dev), *filters)
             if history is not None:
                 history[slot.long(), (told[slot.long()] + column).long()] = token
             latest[slot.long()] = token
