@@ -492,14 +492,14 @@ struct CodeRows {
 #pragma unroll
         for (int j = 0; j < 4; ++j) s[b][nb][j] = (s[b][nb][j] + lo[nb][j]) * factor[2 * nb + (j & 1)];
     }
-    float inverse[4], keep[4];  // of position g + 8 e: 1 / scale of V, and 0 where that is below 2^-100
+    float inverse[4], keep[4];  // of position g + 8 e: 1 / |scale of V|, and its sign, or 0 where it is below 2^-100
     bool up = false;
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const float ks = lds_f32(ks_s + 4 * (g + 8 * e)), vs = lds_f32(vs_s + 4 * (g + 8 * e));
-      const bool finite = vs < INFINITY;
-      keep[e] = vs < 7.8886091e-31f ? 0.f : 1.f;             // 2^-100
-      const float v = keep[e] == 0.f ? 8.6736174e-19f : vs;  // 2^-60: the weight of a row of zeros
+      const bool finite = fabsf(vs) < INFINITY;
+      keep[e] = fabsf(vs) < 7.8886091e-31f ? 0.f : copysignf(1.f, vs);  // 2^-100
+      const float v = keep[e] == 0.f ? 8.6736174e-19f : fabsf(vs);      // 2^-60: the weight of a row of zeros
       inverse[e] = finite ? __frcp_rn(v) : 1.f;
       const float lift = finite ? __log2f(v) : __uint_as_float(0x7fc00000u);
 #pragma unroll

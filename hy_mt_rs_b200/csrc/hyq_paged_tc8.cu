@@ -511,8 +511,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
     ahead = entry(1);
 #pragma unroll 1
     for (int i = 0; i < tiles; ++i) {
-      const uint32_t bits = __float_as_uint(vs);
-      const bool usable = bits - 1u < 0x7f7fffffu;  // positive and finite
+      const uint32_t bits = __float_as_uint(vs) & 0x7fffffffu;
+      const bool usable = bits - 1u < 0x7f7fffffu;  // finite and not zero
       const uint32_t most = __reduce_max_sync(0xffffffffu, usable ? bits : 0u),
                      least = __reduce_min_sync(0xffffffffu, usable ? bits : 0x7f800000u);
       const bool bad = __any_sync(0xffffffffu, held && !isfinite(vs));
@@ -673,8 +673,8 @@ __global__ void __launch_bounds__(kThreads, 1) chunk_tc8_kernel(const __grid_con
               for (int i = 0; i < 4; ++i) s = fmaf(q[4 * d + i], code_value<KV>((uint8_t)(w >> (8 * i))), s);
             }
             s *= scale * (ks[pos - p0] / code_unit<KV>());
-            const bool usable = v_unit > 0.f && isfinite(v_unit);
-            const float own = usable ? fminf(fmaxf((float)((int)(__float_as_uint(v_unit) >> 23) - 126), -100.f), 100.f) : lift;
+            const bool usable = v_unit != 0.f && isfinite(v_unit);
+            const float own = usable ? fminf(fmaxf((float)((int)(__float_as_uint(v_unit) >> 23 & 0xffu) - 126), -100.f), 100.f) : lift;
             const float u = s + own, back = __uint_as_float((uint32_t)(127 - (int)own) << 23);
             if (m == -INFINITY) {
               m = reference(u);

@@ -290,3 +290,34 @@ def test_in_place_wants_the_queries_stride(cuda):
     s["q"] = buf.view(4, 11, 128)[:, :8]
     with pytest.raises(HyqError, match="in place with two strides"):
         _attend(s, out=buf[:4 * 8 * 128].view(4, 8, 128))
+
+
+# --------------------------------------------------------------------- scales
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("dim", [64, 128, 80])
+@pytest.mark.parametrize("far", [False, True])
+@pytest.mark.parametrize("new,ctx", [([1, 3], [900, 400]), ([200, 1], [500, 70]), ([20], [60])])
+def test_scales_of_either_sign(cuda, new, ctx, far, dim, kind):
+    """A value is code * scale: scales that appending does not write, below zero, count like
+    any; also in tiles that are left out of the products (`far`)."""
+    import torch
+    from test_gpu_paged8 import _values
+    s = _make8(cuda, new, ctx, 8, 2, dim, 16, kind, seed=31)
+    g = torch.Generator(device=cuda).manual_seed(6)
+    for name in ("k", "v"):
+        scale = s["kv"][name + "_scale"]
+        scale *= 1 - 2 * torch.randint(0, 2, scale.shape, generator=g, device=cuda).float()
+        if far and name == "v":
+            scale *= torch.exp2(torch.randint(-20, 21, scale.shape, generator=g, device=cuda).float())
+        s[name] = _values(s[name + "_pages"], scale)
+    _close_far(_attend(s), s)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("far", [False, True])
+def test_scales_of_a_prefix_of_either_sign(cuda, far, kind):
+    """And 2^20 apart within a prefix's tiles, behind and in front of whole ones."""
+    import torch
+    s = _make_shared(cuda, [(900, [(9, 1), (0, 2), (150, 1)]), (300, [(1, 1), (270, 2)])], 8, 2, 128, 32, kind, seed=8)
+    _scaled(s, lambda p: (1 - 2 * (p * 7 // 3 % 2)) * _where((p // 256 % 2 == 1) & far, torch.exp2(10.0 - (p * 37 % 21)), 1.0))
+    _close_far(_attend_shared(s), s)
