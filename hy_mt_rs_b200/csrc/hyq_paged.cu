@@ -383,6 +383,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
   grid_dependency_wait();
   allow_dependents_launch();
   const int t = blockIdx.x, kvh = blockIdx.y, dim = a.c.dim, G = a.heads / a.c.kv_heads;
+  if (a.groups.n && kvh == 0) check_groups(a.c, a.groups);
   const int s = seq_of_row(a.c, t);
   if (s < 0) return;
   const Seq sq = load_seq(a.c, s);
@@ -857,10 +858,9 @@ int hyq_paged_attention_shared(const hyq_paged_kv8* kv, const hyq_paged_batch* b
   a.groups.shared = shared;
   a.groups.n = (int)groups;
   a.groups.max_new = batch->max_new;
-  if (!shared_supported(a, type) || !worth_sharing(a, type, groups, max_shared)) {
-    a.groups = {};
+  // (its kernels of few rows look the groups over)
+  if (!shared_supported(a, type) || !worth_sharing(a, type, groups, max_shared))
     return attend(a, type, batch->max_new, batch->max_len, name, st);
-  }
   return done(launch_shared(a, type, st), name);
 }
 

@@ -236,6 +236,34 @@ struct Groups {
   int64_t max_new;        // of any sequence
 };
 
+// The last group that starts at or before sequence i (start ascending).
+__device__ __forceinline__ int group_of(const Groups& g, int i) {
+  int lo = 0, hi = g.n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (g.start[mid] <= i) lo = mid;
+    else hi = mid - 1;
+  }
+  return lo;
+}
+// Whether group i's entries are none that a batch can have.
+__device__ __forceinline__ bool bad_group(const Cache& c, const Groups& g, int i) {
+  const int first = g.start[i], last = g.start[i + 1];
+  return first < 0 || first > last || last > c.seqs || g.shared[i] < 0;
+}
+// The groups of a call whose sequences are taken each on their own all the same, looked
+// over by all threads of the grid's first dimension: a bad one is reported.
+__device__ __forceinline__ void check_groups(const Cache& c, const Groups& g) {
+  const int threads = gridDim.x * blockDim.x;
+  bool bad = false;
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < g.n; i += threads) bad = bad || bad_group(c, g, i);
+  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < c.seqs; i += threads) {
+    const int k = group_of(g, i), first = g.start[k], last = g.start[k + 1];
+    bad = bad || (first <= i && i < last && last - first > 1 && c.pos[i] < g.shared[k]);
+  }
+  if (bad) atomicOr(c.status, DEV_BAD_ARGS);
+}
+
 // hyq_paged_attention's activations and output.
 struct AttendArgs {
   Cache c;

@@ -132,6 +132,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
   const int64_t work = (int64_t)carry * kvh_n;
   const int ctas = (int)min((int64_t)gridDim.x, work), cta = blockIdx.x;
   if (cta >= ctas) {
+    if (!PART && a.groups.n) check_groups(a.c, a.groups);
     if (beside && cta == 0) grid_dependency_wait();
     return;
   }
@@ -198,6 +199,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
     }
   };
   open(false);
+  if (!PART && a.groups.n) check_groups(a.c, a.groups);  // (while the first copies come)
   for (int piece = 1; at < end; ++piece) {
     {
       const Seq& s = cur.s;

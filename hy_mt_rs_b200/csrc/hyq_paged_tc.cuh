@@ -121,9 +121,8 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
     for (int i = threadIdx.x; i < a.c.tokens; i += 1024) g.token[i] = make_int2(-1, 0);
     bool bad = false;
     for (int i = threadIdx.x; i < units; i += 1024) {
-      const int first = g.start[i], last = g.start[i + 1], p = g.shared[i];
-      bad = bad || first < 0 || first > last || last > a.c.seqs || p < 0;
-      off_s[i] = last - first > 1 ? p : 0;
+      bad = bad || bad_group(a.c, g, i);
+      off_s[i] = g.start[i + 1] - g.start[i] > 1 ? g.shared[i] : 0;
     }
     if (__syncthreads_or(bad)) {  // no groups then
       if (threadIdx.x == 0) atomicOr(a.c.status, DEV_BAD_ARGS);
@@ -134,12 +133,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
 #pragma unroll 1
     for (int turn = 0; turn < 2; ++turn) {
       for (int i = threadIdx.x; i < a.c.seqs; i += 1024) {
-        int lo = 0, hi = units - 1;  // the last group that starts at or before i
-        while (lo < hi) {
-          const int mid = (lo + hi + 1) >> 1;
-          if (g.start[mid] <= i) lo = mid;
-          else hi = mid - 1;
-        }
+        const int lo = group_of(g, i);
         const bool in = g.start[lo] <= i && i < g.start[lo + 1];
         const Seq s = load_seq(a.c, i);
         if (turn == 0) {
@@ -187,13 +181,7 @@ __global__ void __launch_bounds__(1024) plan_kernel(const __grid_constant__ Atte
   if constexpr (PREFIX) {
     for (int i = threadIdx.x; i < a.c.seqs; i += 1024) {
       if (g.first[i] == 0) continue;
-      int lo = 0, hi = units - 1;
-      while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (g.start[mid] <= i) lo = mid;
-        else hi = mid - 1;
-      }
-      const int row0 = a.c.row_start[g.start[lo]];
+      const int lo = group_of(g, i), row0 = a.c.row_start[g.start[lo]];
       for (int t = a.c.row_start[i]; t < a.c.row_start[i + 1]; ++t) g.token[t] = make_int2(off_s[lo], t - row0);
     }
   }

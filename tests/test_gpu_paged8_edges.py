@@ -321,3 +321,40 @@ def test_scales_of_a_prefix_of_either_sign(cuda, far, kind):
     s = _make_shared(cuda, [(900, [(9, 1), (0, 2), (150, 1)]), (300, [(1, 1), (270, 2)])], 8, 2, 128, 32, kind, seed=8)
     _scaled(s, lambda p: (1 - 2 * (p * 7 // 3 % 2)) * _where((p // 256 % 2 == 1) & far, torch.exp2(10.0 - (p * 37 % 21)), 1.0))
     _close_far(_attend_shared(s), s)
+
+
+# --------------------------------------------------------------------- groups
+@pytest.mark.parametrize("kind,dim", [("f32", 128), ("f16", 64), ("i8", 128), ("f8", 128), ("f16", 80), ("i8", 256)])
+def test_bad_groups_of_small_prefixes_are_reported(cuda, kind, dim):
+    """Also where the prefixes are not worth their own kernels, or not for them: the same
+    outputs, and the device status; none for good groups."""
+    import torch
+    from hy_mt_rs_b200 import quant
+    groups = [(140, [(9, 1), (0, 1), (50, 1)]), (200, [(1, 1), (70, 2)])]
+    s = _make_shared(cuda, groups, 8, 2, dim, 32, kind, seed=4)
+    good = [([140, 200], [0, 3, 5]), ([140], [0, 2]), ([200], [3, 5]), ([], [0]), ([140, 9999, 200], [0, 3, 3, 5]), ([99999, 1], [0, 1, 1]),
+            ([0, 0], [0, 1, 5])]
+    bad = [([141, 200], [0, 3, 5]), ([-1, 200], [0, 3, 5]), ([140, 200], [0, 3, 6]), ([140, 200], [0, 6, 5]), ([140, 200], [-1, 3, 5]),
+           ([140, 2 ** 31 - 1], [0, 3, 5]), ([140, 202], [0, 3, 5])]
+    want = None
+    for shared, start in good + bad:
+        s.update(shared=_int(shared, cuda), group_start=_int(start, cuda))
+        got = _attend_shared(s, max_len=400, max_shared=300)
+        want = got if want is None else want
+        assert torch.equal(got, want)
+        assert quant.device_status() == (0 if (shared, start) in good else 8), (shared, start)
+
+
+def test_many_groups_of_small_prefixes(cuda):
+    """More groups than a block has threads, one of them bad, wherever it is."""
+    import torch
+    from hy_mt_rs_b200 import quant
+    n = 700
+    s = _make_shared(cuda, [(3, [(i % 3, 1), (0, 1)]) for i in range(n)], 4, 2, 64, 16, "f16", seed=2)
+    want = _attend_shared(s, max_len=10, max_shared=10)
+    assert quant.device_status() == 0
+    for i in (0, 299, n - 1):
+        s["shared"][i] = 4      # its second sequence holds three
+        assert torch.equal(_attend_shared(s, max_len=10, max_shared=10), want)
+        assert quant.device_status() == 8
+        s["shared"][i] = 3
