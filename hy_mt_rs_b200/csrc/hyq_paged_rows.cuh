@@ -181,14 +181,13 @@ struct Rows {
   float o[DIM / 8][4];
   float m[2], l[2];                     // reference and sum of the weights
 
-  // Fragments of the `live` rows that stage_queries() left at q_s.  (step 0: every
-  // token sees up to s.pos.)
-  __device__ __forceinline__ void load(uint32_t q_s, const float* factor_s, const Seq& s, int group, int r0, int live, int step = 1) {
+  // Fragments of the `live` rows that stage_queries() left at q_s.
+  __device__ __forceinline__ void load(uint32_t q_s, const float* factor_s, const Seq& s, int group, int r0, int live) {
     const int lane = threadIdx.x & 31, mat = lane >> 3, row = 8 * (mat & 1) + (lane & 7);
 #pragma unroll
     for (int i = 0; i < 2; ++i) {
       const int r = (lane >> 2) + 8 * i;
-      sees[i] = s.pos + step * min((r0 + r) / group, s.n - 1);
+      sees[i] = s.pos + min((r0 + r) / group, s.n - 1);
       factor[i] = F32 ? 1.0f : factor_s[r];
     }
     if constexpr (!F32) {
@@ -424,12 +423,12 @@ struct CodeRows {
   float o[VT][NB][4];
   float m[kPer], l[kPer];
 
-  __device__ __forceinline__ void load(uint32_t q_s, const float* factor_s, const Seq& s, int group, int r0, int live, int step = 1) {
+  __device__ __forceinline__ void load(uint32_t q_s, const float* factor_s, const Seq& s, int group, int r0, int live) {
     const int lane = threadIdx.x & 31;
 #pragma unroll
     for (int i = 0; i < kPer; ++i) {
       factor[i] = factor_s[row(i)] * code_unit<KV>();
-      sees[i] = s.pos + step * min((r0 + row(i)) / group, s.n - 1);
+      sees[i] = s.pos + min((r0 + row(i)) / group, s.n - 1);
       // (rows without a query never raise the references, whatever was in their place)
       m[i] = row(i) < live ? -INFINITY : INFINITY;
       l[i] = 0.f;
