@@ -520,9 +520,10 @@ int hyq_paged_attention(const hyq_paged_kv* kv, const hyq_paged_batch* batch, co
  * are before any rounding to f32 (where f32 leaves it open, in 64-bit arithmetic rounded
  * to 2^-40 of a step; e4m3 by way of the nearest f32); a row of magnitudes below 2^-90
  * has scale and codes 0.  A row with an infinity or NaN has codes 0 and a NaN scale:
- * it reads back as NaN throughout.  Attention makes NaN of rows
- * that see such a position, and of no others.  The codes 0x7f and 0xff of e4m3,
- * which appending does not write, count as +-480. */
+ * it reads back as NaN throughout.  Attention makes NaN of rows that see such a
+ * position, and of no others.  What appending does not write: scales below zero count
+ * like any, infinite ones make infinities or NaN of what sees them, and the codes 0x7f
+ * and 0xff of e4m3 count as +-480. */
 #define HYQ_KV_I8 2
 #define HYQ_KV_F8 3
 

@@ -358,3 +358,120 @@ def test_many_groups_of_small_prefixes(cuda):
         assert torch.equal(_attend_shared(s, max_len=10, max_shared=10), want)
         assert quant.device_status() == 8
         s["shared"][i] = 3
+
+
+# ------------------------------------------------- prefixes that are not finite
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("where", [0, 130, 640, 899])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_prefix_scales_that_are_not_finite(cuda, where, bad, kind):
+    """A row of V of the prefix with such a scale makes its group NaN in that kv head (an
+    infinite one infinities or NaN), one of K too, one behind the prefix its own sequence; the
+    other head and the other group stay within their bound."""
+    import torch
+    s = _make_shared(cuda, [(900, [(9, 1), (0, 2), (150, 1)]), (300, [(1, 1), (270, 2)])], 8, 2, 128, 32, kind, seed=9)
+    ref, tol = _bound(s)
+    gone = (lambda x: bool(torch.isnan(x).all())) if math.isnan(bad) else (lambda x: not torch.isfinite(x).any())  # noqa: E731
+    near = lambda got, rows, heads: bool(((got.double() - ref).abs() <= tol)[rows, heads].all())  # noqa: E731
+    page, row = int(s["table"][0, where // 32]), where % 32
+    pages = {page} if where < 896 else {int(s["table"][i, 28]) for i in range(3)}    # (the partial page: each one's own)
+    for page in pages:
+        s["kv"]["v_scale"][page, 1, row] = bad
+    got = _attend_shared(s)
+    assert gone(got[:4, 4:])
+    assert near(got, slice(0, 4), slice(0, 4)) and near(got, slice(4, None), slice(0, 8))
+    s["kv"]["k_scale"][int(s["table"][3, 2]), 0, 5] = math.nan     # position 69 of the other group's
+    got = _attend_shared(s)
+    assert torch.isnan(got[4:, :4]).all() and gone(got[:4, 4:])
+    assert near(got, slice(0, 4), slice(0, 4)) and near(got, slice(4, None), slice(4, 8))
+    for page in pages:
+        s["kv"]["v_scale"][page, 1, row] = 0.01
+    s["kv"]["v_scale"][int(s["table"][2, 1000 // 32]), 0, 1000 % 32] = bad     # sequence 2's own
+    got = _attend_shared(s)
+    assert gone(got[3, :4]) and near(got, slice(0, 3), slice(0, 4))
+
+
+# -------------------------------------------------- workspaces, overlapped launches
+def _calls(cuda, kind):
+    """Calls of this file's operators that reach their kernels, and their workspaces."""
+    import torch
+    from hy_mt_rs_b200 import paged
+    from test_gpu_paged import _make
+    out = []
+    for new, ctx in (([200, 1], [700, 300]), ([1, 3, 2], [900, 40, 5000]), ([40, 1], [20, 5])):
+        if kind in KINDS:
+            s = _make8(cuda, new, ctx, 8, 2, 128, 32, kind, seed=41)
+        else:
+            s = _make(cuda, new, ctx, 8, 2, 128, 32, kind == "f16", seed=41)
+            s.update(kv={}, k_pages=s["k"], v_pages=s["v"])
+        out.append((s, _attend, paged.attention_workspace(8, 128, cuda)))
+    s = _make_shared(cuda, [(900, [(9, 1), (0, 2), (150, 1)]), (300, [(1, 1), (270, 2)])], 8, 2, 128, 32, kind, seed=42)
+    out.append((s, _attend_shared, paged.attention_shared_workspace(8, 128, s["q"].shape[0], cuda)))
+    return out
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", *KINDS])
+def test_workspaces_of_used_memory(cuda, kind):
+    """Only a workspace's first bytes are zero: the same bits, call after call."""
+    import torch
+    for s, attend, ws in _calls(cuda, kind):
+        want = attend(s)
+        for x in (math.nan, 1e38, -1e-3):
+            ws[4096:] = torch.full((ws.numel() // 4 + 1,), x, device=cuda).view(torch.uint8)[:ws.numel() - 4096]
+            for _ in range(2):
+                assert torch.equal(attend(s, workspace=ws), want)
+            assert int(ws[:4096].amax()) == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", *KINDS])
+@pytest.mark.parametrize("captured", [False, True])
+def test_overlapped_launches(cuda, captured, kind):
+    """Chains of appends, reads, attention and adjusted logits in which each takes what the
+    one before wrote, with programmatic launches and without: the same bits."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant, sampling
+    from test_gpu_paged8 import _append_inputs
+    g = torch.Generator(device=cuda).manual_seed(3)
+    history = torch.randint(0, 9000, (8, 5000), generator=g, device=cuda, dtype=torch.int32)
+    length = torch.full((8,), 5000, dtype=torch.int32, device=cuda)
+    chains = []
+    for s, attend, ws in _calls(cuda, kind):
+        a = _append_inputs(cuda, s["new"], s["ctx"], 8, 2, 128, 32, seed=7, positions=6000)
+        a["many"] = [torch.randn(600, h, 128, generator=g, device=cuda) for h in (8, 2, 2)]
+
+        def chain(s=s, attend=attend, ws=ws, a=a):
+            # (rows behind the last sequence take the staged append to them as well)
+            q, k, v = a["many"]
+            t = s["q"].shape[0]
+            q[:t], k[:t], v[:t] = s["q"], a["new_k"], a["new_v"]
+            pages = (s["k_pages"], s["v_pages"], s["table"], s["row_start"], s["pos"])
+            rotated = paged.rope_append(q, k, v, *pages, a["cos"], a["sin"], a["q_norm"], a["k_norm"], slot=s["slot"], **s["kv"])
+            x = attend(dict(s, q=rotated[:t]), workspace=ws)
+            back = paged.gather(*pages, t, slot=s["slot"], **s["kv"])
+            y = attend(dict(s, q=x), workspace=ws)
+            logits = torch.nn.functional.pad(y.reshape(t, -1)[:1].repeat(8, 9), (0, 0))
+            z = sampling.adjust(logits, history, length, repetition=1.2, frequency=0.1)
+            return [x, *back, y, z, *(p.view(torch.uint8) for p in pages[:2])]
+
+        chains.append(chain)
+    want = [[t.clone() for t in c()] for c in chains]       # (the appends write the same rows again)
+    stream = torch.cuda.Stream()
+    torch.cuda.synchronize()
+    try:
+        quant.set_launch_overlap(True)
+        for c, w in zip(chains, want):
+            if captured:
+                graph = torch.cuda.CUDAGraph()
+                with torch.cuda.graph(graph, stream=stream):
+                    got = c()
+                for _ in range(3):
+                    graph.replay()
+            else:
+                for _ in range(3):
+                    got = c()
+            torch.cuda.synchronize()
+            for x, y in zip(got, w):
+                assert torch.equal(x, y)
+    finally:
+        quant.set_launch_overlap(False)
+    assert quant.device_status() == 0
