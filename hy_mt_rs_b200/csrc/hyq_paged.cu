@@ -57,7 +57,9 @@ __device__ __forceinline__ void store_kv(void* base, int64_t i, float x) {
 // SM keep too few of them in flight, where eight CTAs of four warps have a row of 25 KB
 // each under way.  Bound by memory and by that search (row, page, tables, one after the
 // other): 8,208 tokens of 32 query and 8 kv heads of 128 into an f32 cache (403 MB)
-// 69 us, 5.8 TB/s, f16 65 us, e4m3 74 us (353 MB).
+// 69 us, 5.8 TB/s, f16 65 us, e4m3 75 us (353 MB; with the norm after the rotation 77,
+// and 88 where weights of a pair are 10 to 50 times each other's: more heads are next to
+// borders then and done again).
 // Into an 8-bit cache a head's largest magnitude comes from its 16 lanes, and the
 // codes go through shared memory, so that a lane writes neighbouring ones.
 template <int DIM, Kv KV, bool STAGED>

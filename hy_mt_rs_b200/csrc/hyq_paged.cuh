@@ -299,11 +299,13 @@ cudaError_t launch_few(const AttendArgs& a, Kv kv, int64_t max_new, bool beside,
 cudaError_t launch_chunks(const AttendArgs& a, Kv kv, cudaStream_t st);  // the others
 // Whether that is faster than the kernels on tcgen05: one launch instead of
 // three, but every CTA goes through its rows' positions alone, at 0.04 us (f16
-// caches) or 0.16 us (f32) for each.  Measured with 16 query and 4 kv heads, us
-// here / there: f16, 40 tokens at 100, 8 sequences 20 / 35; 200 tokens at 0 21 /
-// 28; 5 tokens at 300, 64 sequences 31 / 51; 64 tokens at 500 36 / 34; 40 tokens
-// at 300, 32 sequences 60 / 48; f32, 16 tokens at 0 13 / 21; 64 tokens at 0 21 /
-// 21; 8 tokens at 100, 8 sequences 29 / 22.
+// caches), 0.05 us (8-bit) or 0.16 us (f32) for each.  Measured with 16 query and 4 kv
+// heads, us here / there: f16, 40 tokens at 100, 8 sequences 20 / 35; 200 tokens at 0
+// 21 / 28; 5 tokens at 300, 64 sequences 31 / 51; 64 tokens at 500 36 / 34; 40 tokens
+// at 300, 32 sequences 60 / 48; int8 (e4m3 within 1), the same five 23 / 35, 24 / 30,
+// 38 / 60, 45 / 35 and, at 100, 53 / 47; 64 tokens at 200 30 / 33, at 350 37 / 35, 40
+// at 300, 8 sequences 33 / 37; f32, 16 tokens at 0 13 / 21; 64 tokens at 0 21 / 21;
+// 8 tokens at 100, 8 sequences 29 / 22.
 bool chunks_short(const AttendArgs& a, Kv kv, int64_t max_len);
 // hyq_paged_tc.cu: the others on tcgen05 (f16 caches; the workspace past
 // mma_workspace_bytes), and launch_few beside them.

@@ -18,10 +18,10 @@
 // all latency: the plan of the line, the copies, the partial results' join.
 // Over 8-bit caches (half the bytes) the same kernel is bound by its instructions'
 // latencies: the 64 requests 54 us (139 MB, 2.6 TB/s), the four long ones 166 us (e4m3,
-// 677 MB, 4.1 TB/s) at 58 % of the issue slots, 10.7 warps an SM and half of the
-// instructions on the integer pipe (1,240 for 32 positions, of them 450 to take e4m3
-// codes to f16).  Sixteen positions at a time and four CTAs an SM instead of 32 and
-// three: 186 us (registers spill at 128 a thread).
+// 677 MB, 4.1 TB/s) at 53 % of the issue slots and 10.7 warps an SM, the integer pipe
+// 58 % busy (1,240 instructions for 32 positions; it takes e4m3 codes to f16).  Sixteen
+// positions at a time and four CTAs an SM instead of 32 and three: 186 us (registers
+// spill at 128 a thread).
 // Chunks, bound by the products and by each CTA's own walk over the positions:
 // 200 tokens at 0 21 us, 8 sequences of 40 at 100 20 us (f16); longer ones go to
 // the kernels on tcgen05.

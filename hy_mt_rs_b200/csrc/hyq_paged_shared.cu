@@ -20,13 +20,15 @@ size_t shared_workspace_bytes(int heads, int dim, int64_t tokens) {
 
 // Whether a call's prefixes are worth their own kernels: reading them for every
 // sequence costs 5 to 6 TB/s of L2, which reaches the three launches' own time at about
-// 150 MB.  Measured with 16 query and 4 kv heads, one group, shared / each on its own,
-// us: f16, 16 sequences of 2,000 (61 MB) 43 / 23, 32 (127 MB) 44 / 33, 64 (258 MB) 45 /
-// 51, 16 of 8,000 (246 MB) 37 / 47; int8, 32 of 2,000 (65 MB) 45 / 34, 64 (133 MB) 47 /
-// 51, 64 of 8,000 57 / 138; f32, 16 of 2,000 (123 MB) 46 / 41, 32 (254 MB) 48 / 69.
+// 130 (f32) to 230 MB (f16).  Measured with 16 query and 4 kv heads, one group, shared /
+// each on its own, us in a graph: f16, 16 sequences of 2,000 (61 MB) 43 / 23, 32 (127 MB)
+// 45 / 31, 48 (193 MB) 46 / 40, 64 (258 MB) 46 / 50, 16 of 8,000 (246 MB) 47 / 46; int8 and
+// e4m3, 32 of 2,000 (65 MB) 50 / 32, 64 (133 MB) 56 / 51, 16 of 8,000 (127 MB) 50 / 45, 32
+// (262 MB) 51 / 77; f32, 16 of 2,000 (123 MB) 44 / 40, 8 of 8,000 (229 MB) 43 / 63, 32 of
+// 2,000 (254 MB) 46 / 67.
 bool worth_sharing(const AttendArgs& a, Kv kv, int64_t groups, int64_t max_shared) {
   const int64_t row = 2 * ((int64_t)a.c.dim * value_bytes(kv) + (is_8bit(kv) ? 4 : 0)) * a.c.kv_heads;
-  return groups > 0 && (a.c.seqs - groups) * max_shared * row >= 150000000;
+  return groups > 0 && (double)((a.c.seqs - groups) * max_shared) * row >= 150e6;
 }
 
 bool shared_supported(const AttendArgs& a, Kv kv) { return mma_supported(a, kv) && chunks_tc_supported(a, kv); }

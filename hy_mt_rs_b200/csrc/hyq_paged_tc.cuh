@@ -45,7 +45,15 @@ struct Plan {
   Start* start;    // [kMaxCtas + 1]
   Segment* seg;    // [kMaxSegs]
   int most;        // segments that the rows of the call can make
-  int least;       // prefixes: tiles of a CTA's range, at least (more: there is other work for the SMs left)
+  // Prefixes: tiles of a CTA's range, at least (shorter ranges leave more pieces to merge,
+  // longer ones a longer chain; what the cut does to the pieces shows as much).  Measured
+  // at least = 2 / 4 / 6 / 8 / 12 with 16 query and 4 kv heads, us of a call: int8 (8), 64
+  // sequences behind 8,000 positions 62 / 59 / 55 / 53 / 74, 32 behind 8,000 56 / 42 / 54 /
+  // 51 / 71, four groups of 8 behind 12,003 (32 and 8 heads) 133 / 132 / 132 / 132 / 132;
+  // f16 (6), the same 57 / 57 / 56 / 47 / 62, 44 / 37 / 49 / 42 / 59 and 95 / 94 / 94 / 94 /
+  // 94, 32 behind 4,000 (32 and 8 heads) 54 / 47 / 47 / 51 / 58; f32 (4), the first two up
+  // to 8, 77 / 75 / 80 / 70, 55 / 51 / 61 / 64, the last 66 / 63 / 60 / 68.
+  int least;
 };
 constexpr size_t kPlanBytes = 16 + (kMaxCtas + 1) * sizeof(Start) + (size_t)kMaxSegs * sizeof(Segment);
 template <int ROWS>

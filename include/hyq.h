@@ -556,8 +556,9 @@ int hyq_paged_attention_kv8(const hyq_paged_kv8* kv, const hyq_paged_batch* batc
  * positions 0 .. shared[g] - 1 hold the same keys and values: they are read
  * through the table row of the group's first sequence.  shared[g] is at most the
  * pos of each of its sequences (else the group has no prefix: its sequences are
- * taken each on their own, and HYQ_DEV_BAD_ARGS is raised; a group_start that
- * does not ascend from 0 to seqs does that to all groups).  Every cache type; for
+ * taken each on their own, and HYQ_DEV_BAD_ARGS is raised; a group with a sequence
+ * of more than max_new tokens likewise; a group_start that does not ascend within
+ * 0 .. seqs does that to all groups).  Every cache type; for
  * few new tokens: max_new times the query heads per kv head is at most 16.
  * max_shared bounds any shared[g] (a prefix past it counts all the same).
  * Head sizes other than 64 and 128, and pages that the chunks' kernels do not take
