@@ -60,8 +60,12 @@ struct Smem {
   static constexpr int q = 0;                            // [row tile][hi, lo]
   static constexpr int ring = (PREFIX ? 2 : 4) * tile;
   static constexpr int bars = ring + slots * tile;
-  // full[slots], empty[slots], s_full[2], p_full[2], x_full[2], q_full[2], clean[2], half[2]
-  static constexpr int n_bars = 2 * slots + 12;
+  // A tile's turn among these comes when the products have waited for the one that had
+  // it before: V of masked tile i + cleans is in a slot of the ring that is only free
+  // when a product behind that wait is done (five slots: of K of the next piece).
+  static constexpr int cleans = PREFIX ? 3 : 2;
+  // full[slots], empty[slots], s_full[2], p_full[2], x_full[2], q_full[2], half[2], clean[cleans]
+  static constexpr int n_bars = 2 * slots + 10 + cleans;
   static constexpr int factors = bars + 8 * n_bars;      // (prefixes) powers of two of the rows' queries
   static constexpr int misc = factors + (PREFIX ? kTile * 4 : 0);         // tensor memory address, abort, unused, dirty
   static constexpr int total = misc + 32 + 1024;         // the base is moved to 1024 bytes
@@ -94,8 +98,8 @@ __global__ void __launch_bounds__(kThreads, 1)
   auto p_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 2 + w); };
   auto x_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 4 + w); };
   auto q_full = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 6 + w); };
-  auto half = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 10 + w); };  // given, taken (split pieces)
-  auto clean = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 8 + (i & 1)); };  // of masked tile i
+  auto half = [&](int w) { return base + L::bars + 8 * (2 * kSlots + 8 + w); };  // given, taken (split pieces)
+  auto clean = [&](int i) { return base + L::bars + 8 * (2 * kSlots + 10 + i % L::cleans); };  // of masked tile i: phase i / cleans
   volatile int* misc = reinterpret_cast<volatile int*>(base_g + L::misc);
   volatile int* abort_flag = misc + 1;
   const int warp = uniform(threadIdx.x >> 5), lane = threadIdx.x & 31;
@@ -120,9 +124,9 @@ __global__ void __launch_bounds__(kThreads, 1)
         mbar_init(p_full(w), 4);
         mbar_init(x_full(w), 1);
         mbar_init(q_full(w), 4);
-        mbar_init(clean(w), 2);
         mbar_init(half(w), 4);
       }
+      for (int i = 0; i < L::cleans; ++i) mbar_init(clean(i), 2);
       mbar_fence_init();
     }
   }
@@ -265,7 +269,7 @@ __global__ void __launch_bounds__(kThreads, 1)
             const int n = first + 2 * j + 1, w = j & 1;
             ok = wait(full(n % kSlots), (n / kSlots) & 1);
             if (ok && j >= jm) {
-              ok = wait(clean(masked), (masked >> 1) & 1);
+              ok = wait(clean(masked), (masked / L::cleans) & 1);
               ++masked;
             }
             ok = ok && wait(p_full(w), steps[w] & 1);
@@ -303,7 +307,7 @@ __global__ void __launch_bounds__(kThreads, 1)
           ok = wait(full(slot), phase);
           advance();
           if (ok && j >= jm) {
-            ok = wait(clean(masked), (masked >> 1) & 1);
+            ok = wait(clean(masked), (masked / L::cleans) & 1);
             ++masked;
           }
           const int k_slot = slot;

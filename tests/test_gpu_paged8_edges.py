@@ -475,3 +475,16 @@ def test_overlapped_launches(cuda, captured, kind):
     finally:
         quant.set_launch_overlap(False)
     assert quant.device_status() == 0
+
+
+@pytest.mark.parametrize("kind", ["f32", "f16", *KINDS])
+@pytest.mark.parametrize("groups", [60, 200])
+def test_many_short_prefixes(cuda, groups, kind):
+    """CTAs that go through one prefix after another, each of a tile or two of which the last
+    is masked: the pipelines run ahead from one into the next."""
+    s = _make_shared(cuda, [(40 + 53 * i % 230, [(i % 9, 1), (0, 1 + i % 2)]) for i in range(groups)], 16, 4, 128, 32, kind, seed=groups)
+    want = _attend_shared(s)
+    _close_far(want, s)
+    import torch
+    for _ in range(20):
+        assert torch.equal(_attend_shared(s), want)
