@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kThreads) attend_kernel(const __grid_constant_
   grid_dependency_wait();
   allow_dependents_launch();
   const int t = blockIdx.x, kvh = blockIdx.y, dim = a.c.dim, G = a.heads / a.c.kv_heads;
-  if (a.groups.n && kvh == 0) check_groups(a.c, a.groups);
+  if (a.groups.n && kvh == 0) check_groups<int64_t>(a.c, a.groups);
   const int s = seq_of_row(a.c, t);
   if (s < 0) return;
   const Seq sq = load_seq(a.c, s);
@@ -743,7 +743,7 @@ int attend_args(const hyq_paged_kv* kv, const hyq_paged_kv8* kv8, const hyq_page
   if (!q || !out || !workspace) return api_fail(HYQ_E_INVALID, "%s: null pointer", name);
   const int64_t qw = (int64_t)heads * kv->head_dim;
   if (q_stride < qw || out_stride < qw) return api_fail(HYQ_E_SHAPE, "%s: shape of the activations", name);
-  if (q == out && q_stride != out_stride) return api_fail(HYQ_E_SHAPE, "%s: in place with two strides", name);
+  if (q == out && q_stride != out_stride && batch->tokens > 1) return api_fail(HYQ_E_SHAPE, "%s: in place with two strides", name);
   if (!aligned(q, 4) || !aligned(out, 4) || !aligned(workspace, 16))
     return api_fail(HYQ_E_ALIGN, "%s: alignment of q, out or the workspace", name);
   a.q = q;

@@ -252,14 +252,17 @@ __device__ __forceinline__ bool bad_group(const Cache& c, const Groups& g, int i
   return first < 0 || first > last || last > c.seqs || g.shared[i] < 0;
 }
 // The groups of a call whose sequences are taken each on their own all the same, looked
-// over by all threads of the grid's first dimension: a bad one is reported.
+// over by all threads of the grid's first dimension: a bad one is reported.  INDEX: holds
+// the number of threads.
+template <typename INDEX>
 __device__ __forceinline__ void check_groups(const Cache& c, const Groups& g) {
-  const int threads = gridDim.x * blockDim.x;
+  const INDEX threads = (INDEX)gridDim.x * blockDim.x, mine = (INDEX)blockIdx.x * blockDim.x + threadIdx.x;
   bool bad = false;
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < g.n; i += threads) bad = bad || bad_group(c, g, i);
-  for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < c.seqs; i += threads) {
-    const int k = group_of(g, i), first = g.start[k], last = g.start[k + 1];
-    bad = bad || (first <= i && i < last && last - first > 1 && c.pos[i] < g.shared[k]);
+  for (INDEX i = mine; i < g.n; i += threads) bad = bad || bad_group(c, g, (int)i);
+  for (INDEX i = mine; i < c.seqs; i += threads) {
+    const int k = group_of(g, (int)i), first = g.start[k], last = g.start[k + 1], p = g.shared[k];
+    const bool in = first <= i && i < last && last - first > 1 && p > 0;
+    bad = bad || (in && (c.pos[i] < p || (int64_t)c.row_start[i + 1] - c.row_start[i] > g.max_new));
   }
   if (bad) atomicOr(c.status, DEV_BAD_ARGS);
 }

@@ -96,6 +96,7 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
     s.n = min(s.n - before, kRows / group);
     return s;
   };
+  if (!PART && a.groups.n) check_groups<int>(a.c, a.groups);
   // prefix sum of the sequences' tiles; sequences with more rows are the
   // chunk kernel's
   int carry = 0;
@@ -132,7 +133,6 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
   const int64_t work = (int64_t)carry * kvh_n;
   const int ctas = (int)min((int64_t)gridDim.x, work), cta = blockIdx.x;
   if (cta >= ctas) {
-    if (!PART && a.groups.n) check_groups(a.c, a.groups);
     if (beside && cta == 0) grid_dependency_wait();
     return;
   }
@@ -199,7 +199,6 @@ __global__ void __launch_bounds__(kThreads, Geo<DIM, KV, NB>::ctas)
     }
   };
   open(false);
-  if (!PART && a.groups.n) check_groups(a.c, a.groups);  // (while the first copies come)
   for (int piece = 1; at < end; ++piece) {
     {
       const Seq& s = cur.s;

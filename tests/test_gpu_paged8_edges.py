@@ -290,6 +290,11 @@ def test_in_place_wants_the_queries_stride(cuda):
     s["q"] = buf.view(4, 11, 128)[:, :8]
     with pytest.raises(HyqError, match="in place with two strides"):
         _attend(s, out=buf[:4 * 8 * 128].view(4, 8, 128))
+    s = _make8(cuda, [1], [90], 8, 2, 128, 32, "i8", seed=21)     # one row has none
+    want, buf = _attend(s), torch.zeros(11 * 128, device=cuda)
+    buf[:1024] = s["q"].flatten()
+    s["q"] = buf.as_strided((1, 8, 128), (11 * 128, 128, 1))
+    assert torch.equal(_attend(s, out=buf[:1024].view(1, 8, 128)), want)
 
 
 # --------------------------------------------------------------------- scales
@@ -488,3 +493,34 @@ def test_many_short_prefixes(cuda, groups, kind):
     import torch
     for _ in range(20):
         assert torch.equal(_attend_shared(s), want)
+
+
+def test_groups_of_a_batch_of_very_many_rows(cuda):
+    """Rows behind the last sequence count as the call's, 2^25 of them here: threads of the
+    grid that looks the groups over are numbered in 64 bits."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant
+    s = _make_shared(cuda, [(30, [(2, 1), (0, 2), (9, 1)])], 1, 1, 8, 16, "f16", seed=3)
+    few = _attend_shared(s, max_len=50, max_shared=30)
+    wide, out = (torch.zeros(2 ** 25 + 4, 1, 8, device=cuda) for _ in range(2))
+    wide[:4] = s["q"]
+    ws = paged.attention_shared_workspace(1, 8, wide.shape[0], cuda)
+    for shared, status in ((30, 0), (31, 8)):
+        s["shared"][0] = shared
+        _attend_shared(dict(s, q=wide), max_len=50, max_shared=30, out=out, workspace=ws)
+        assert torch.equal(out[:4], few) and not out[4:].any()
+        assert quant.device_status() == status
+
+
+@pytest.mark.parametrize("kind,dim", [("f16", 128), ("i8", 128), ("f32", 80)])
+def test_more_tokens_than_max_new_behind_a_small_prefix(cuda, kind, dim):
+    """Reported as behind a large one; the sequences are right, or left alone."""
+    import torch
+    from hy_mt_rs_b200 import paged, quant
+    s = _make_shared(cuda, [(150, [(9, 1), (3, 2), (0, 1)]), (200, [(0, 1), (31, 1)])], 8, 2, dim, 32, kind, seed=4)
+    out = torch.full_like(s["q"], 7.0)
+    paged.attention_shared(s["q"], s["k_pages"], s["v_pages"], s["table"], s["row_start"], s["pos"], s["group_start"], s["shared"],
+                           1, max_len=400, max_shared=200, out=out, **s["kv"])
+    status = quant.device_status()
+    assert status == 8
+    _right_or_left(out, s, *_bound(s), 7.0, status)
