@@ -345,6 +345,10 @@ PyObject* adjust(PyObject*, PyObject* const* a, Py_ssize_t n) {
     p.repetition = static_cast<const float*>(optional(a[5], x, "repetition", at::kFloat, rows));
     p.presence = static_cast<const float*>(optional(a[6], x, "presence", at::kFloat, rows));
     p.frequency = static_cast<const float*>(optional(a[7], x, "frequency", at::kFloat, rows));
+    if (a[1] != Py_None && p.history_width == 0 && p.slots > 0) {  // no token in any: a tensor without elements has no address
+      p.history = nullptr;
+      p.repetition = p.presence = p.frequency = nullptr;
+    }
     if (a[8] != Py_None) {
       const at::Tensor& t = plain(a[9], "bias tokens", at::kInt);
       same_device(x, t, "bias tokens");

@@ -65,3 +65,21 @@ def test_strides_in_place_and_replayed(cuda, n):
         torch.cuda.synchronize()
         np.testing.assert_array_equal(out.cpu().numpy(), _expected(y, c))
         assert torch.equal(beside, out)
+
+
+def test_histories_of_width_zero(cuda):
+    """Rows that can hold no token: penalties change nothing, biases and masks do."""
+    import torch
+    from hy_mt_rs_b200 import quant, sampling
+    from hy_mt_rs_b200._native import HyqError
+    c, x = _case(4, 700, 5, 2), _logits(4, 700, 2)
+    a = _args(c, cuda)
+    a.update(history=torch.empty(6, 0, dtype=torch.int32, device=cuda), length=torch.zeros(6, dtype=torch.int32, device=cuda))
+    a.pop("prompt")
+    got = sampling.adjust(torch.from_numpy(x).to(cuda), **a)
+    np.testing.assert_array_equal(got.cpu().numpy(), _expected(x, {k: c[k] for k in ("bias", "mask", "mask_row")}))
+    got = sampling.adjust(torch.from_numpy(x).to(cuda), a["history"], a["length"], repetition=1.5, frequency=0.5)
+    np.testing.assert_array_equal(got.cpu().numpy(), x)
+    with pytest.raises(HyqError):
+        sampling.adjust(torch.from_numpy(x).to(cuda), a["history"], a["length"][:5], repetition=1.5)
+    assert quant.device_status() == 0
